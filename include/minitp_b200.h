@@ -228,6 +228,77 @@ int mtpb_embedding(void* comm, const int64_t* ids, const void* table, void* out,
 int mtpb_argmax(void* comm, const void* logits, int M, int V_local, int64_t ld, int64_t vstart,
                 int64_t* ids_out, int64_t* scratch, int dtype, void* stream);
 
+/* ---------------------------------------------------------- beam search
+ * No counterpart in the reference, which decodes greedily.
+ *
+ * One selection step for G prompts of W beams (1 <= W <= 64): from logits
+ * [G*W, V] (row stride ld) and running scores fp32 [G][W], the k best
+ * (1 <= k <= 64) of all (beam b, token v) of a prompt by
+ *   total(b, v) = score[b] + log_softmax(logits[b])[v],
+ * best first, equal totals by the lower b * V + v. Sums over the vocabulary
+ * are fp32 per chunk; totals are formed and compared in fp64. Outputs [G][k]:
+ * scores fp32 (the rounded totals), parents (b) and tokens (v) int64, and
+ * finished flags (may be NULL).
+ *   - A NaN logit counts as -inf: that token is never picked. +inf logits
+ *     share the probability of their row.
+ *   - `finished` (uint8 [G][W], may be NULL): a finished beam has one
+ *     candidate, token `eos` at the beam's own score; its logits are not read.
+ *     out_finished = finished[parent] or token == eos. eos < 0: no end token.
+ *   - A beam whose score is -inf or NaN, or without a logit above -inf, has
+ *     no candidate. Places without a candidate get score -inf, parent 0 and
+ *     token eos (0 without one).
+ * `block`: workspace of mtpb_beam_block_bytes(G*W, V, k) bytes, 16-byte
+ * aligned, private to the call until it has run. */
+long long mtpb_beam_block_bytes(int rows, int V_plan, int k);
+int mtpb_beam_select(const void* logits, int64_t ld, int G, int W, int V, const float* scores,
+                     const uint8_t* finished, int64_t eos, int k, float* out_scores,
+                     int64_t* out_parents, int64_t* out_tokens, uint8_t* out_finished, void* block,
+                     int dtype, void* stream);
+
+/* The two halves of mtpb_beam_select for a vocabulary in shards.
+ * mtpb_beam_candidates reduces one shard (columns [vstart, vstart + V_local)
+ * of the vocabulary) of every row to a block of
+ * mtpb_beam_block_bytes(rows, V_plan, k) bytes; V_plan, the same on every
+ * shard, is at least the largest V_local. mtpb_beam_pick selects from `parts`
+ * such blocks, one after another in memory in any shard order (made with the same V_plan and k_block = k of the
+ * candidates >= the k picked here). */
+int mtpb_beam_candidates(const void* logits, int64_t ld, int rows, int V_local, int64_t vstart,
+                         int V_plan, int k, const uint8_t* finished, void* block, int dtype,
+                         void* stream);
+int mtpb_beam_pick(const void* blocks, int parts, int G, int W, int V_plan, int k_block,
+                   const float* scores, const uint8_t* finished, int64_t eos, int k,
+                   float* out_scores, int64_t* out_parents, int64_t* out_tokens,
+                   uint8_t* out_finished, void* stream);
+
+/* Cache rows follow the chosen beams, in place: in every layer's K and V
+ * cache [G*W, hkv, cap, hd], positions [0, n) of row g*W + w become those of
+ * row src = g*W + parents[g][w], with n = lens[src] (device int32 [G*W];
+ * clamped to [0, cap]) or `len` when lens is NULL. Positions from n on are
+ * left as they were, and so is a row whose parent is itself or outside
+ * [0, W). 1 <= W <= 64; hd * sizeof(dtype) a multiple of 16; k_caches and
+ * v_caches: host arrays of n_layers device pointers. */
+int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers,
+                    const int64_t* parents, const int* lens, int len, int G, int W, int hkv,
+                    int cap, int hd, int dtype, void* stream);
+
+/* Grouped-query attention of rows that share a prefix. Rows n = g*W + w;
+ * q and out [G*W*T, hq*hd]; prefix caches [G, hkv, cap_p, hd]; own caches
+ * [G*W, hkv, cap, hd]. Token t (of T) of row n attends to positions
+ * [0, prefix_lens[g]) of its group's prefix and [0, cache_lens[n] - (T-1-t))
+ * of its own cache (cache_lens counts the T tokens' own positions too); a
+ * token that sees none gets 0. Lengths: device int32 arrays, clamped to their
+ * cache's capacity, or the host value for every group / row when the array is
+ * NULL. scale = 1/sqrt(hd); hd 16, 32, 64 or 128. Softmax statistics and sums
+ * are fp32. `ws`: at least mtpb_shared_attention_workspace(...) bytes,
+ * 16-byte aligned, private to the call until it has run. */
+long long mtpb_shared_attention_workspace(int G, int W, int T, int hq, int hkv, int hd, int cap_p,
+                                          int cap, int dtype);
+int mtpb_shared_attention(const void* q, const void* k_prefix, const void* v_prefix,
+                          const int* prefix_lens, int prefix_len, const void* k_cache,
+                          const void* v_cache, const int* cache_lens, int cache_len, void* out,
+                          int G, int W, int T, int hq, int hkv, int hd, int cap_p, int cap,
+                          int dtype, void* ws, uint64_t ws_bytes, void* stream);
+
 /* ---------------------------------------------------------------- model
  * A TP Qwen2 decoder whose weights stay in caller-owned device tensors.
  * ref: minitp/layer.py:68-124 (TPQwen2ForCausalLM), minitp/attention.py,

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_float, c_int, c_int64, c_longlong, c_uint32, c_uint64, c_void_p
 
 import torch
 
@@ -101,6 +101,19 @@ SIGNATURES: dict[str, tuple] = {
                                c_int, c_void_p]),
     "mtpb_argmax": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int,
                             c_void_p]),
+    "mtpb_beam_block_bytes": (c_longlong, [c_int, c_int, c_int]),
+    "mtpb_beam_select": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "mtpb_beam_candidates": (c_int, [c_void_p, c_int64, c_int, c_int, c_int64, c_int, c_int, c_void_p, c_void_p,
+                                     c_int, c_void_p]),
+    "mtpb_beam_pick": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_int,
+                               c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mtpb_kv_reorder": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                c_int, c_int, c_void_p]),
+    "mtpb_shared_attention_workspace": (c_longlong, [c_int] * 9),
+    "mtpb_shared_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                      c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                      c_void_p, c_uint64, c_void_p]),
     "mtpb_model_create": (c_int, [POINTER(ModelDesc), c_void_p, POINTER(c_void_p)]),
     "mtpb_model_set_layer": (c_int, [c_void_p, c_int, POINTER(LayerDesc)]),
     "mtpb_model_reserve": (c_int, [c_void_p, c_int, c_int]),

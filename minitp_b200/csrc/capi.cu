@@ -19,6 +19,7 @@
 #include "ar_rows.cuh"
 #include "decode_mk_launch.cuh"
 #include "gemm_tc.cuh"
+#include "host_util.cuh"
 
 #include <cudaTypedefs.h>
 
@@ -1222,6 +1223,24 @@ int model_forward(ModelHost& mh, const FwdArgs& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+namespace mtpb {
+
+int host_fail(int code, const char* msg) noexcept {
+  try {
+    g_err = msg;
+  } catch (...) {  // no memory for the text: the code alone tells
+  }
+  return code;
+}
+int host_fail_cuda(cudaError_t e, const char* what) noexcept {
+  char text[256];
+  std::snprintf(text, sizeof(text), "%s: %s", what, cudaGetErrorString(e));
+  return host_fail(MTPB_ERR_CUDA, text);
+}
+bool host_pdl() noexcept { return g_pdl; }
+
+}  // namespace mtpb
 
 // =====================================================================
 // extern "C"

@@ -1,0 +1,377 @@
+// C ABI of beam search and of attention over a shared prefix (declared in
+// include/minitp_b200.h): host checks, launch plans and workspaces.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "beam.cuh"
+#include "host_util.cuh"
+#include "shared_attn.cuh"
+
+using namespace mtpb;
+
+namespace {
+
+int bad(const char* msg) { return host_fail(MTPB_ERR_INVALID, msg); }
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+size_t es_of(int dtype) { return dtype == MTPB_BF16 ? 2 : 4; }
+bool dtype_ok(int dtype) { return dtype == MTPB_BF16 || dtype == MTPB_F32; }
+
+// ------------------------------------------------------------------ selection
+// Chunks of a row: a function of the sizes alone, so that every rank cuts its
+// shard alike.
+struct BeamPlan {
+  int nchunk, chunk;
+};
+
+BeamPlan beam_plan(long long rows, int V) {
+  BeamPlan b;
+  const long long want = std::max<long long>(1, (4 * 148 + rows - 1) / rows);
+  b.nchunk = int(std::min<long long>(want, (V + 4095) / 4096));
+  b.chunk = (V + b.nchunk - 1) / b.nchunk;
+  b.chunk = (b.chunk + 7) / 8 * 8;
+  b.nchunk = (V + b.chunk - 1) / b.chunk;
+  return b;
+}
+
+size_t beam_cand_bytes(long long rows, const BeamPlan& b, int k) { return size_t(rows) * b.nchunk * k * 8; }
+size_t beam_block(long long rows, const BeamPlan& b, int k) {
+  return (beam_cand_bytes(rows, b, k) + size_t(rows) * b.nchunk * sizeof(BeamStat) + 15) / 16 * 16;
+}
+
+int beam_check(long long rows, long long V, int k) {
+  if (rows < 1 || rows > (1 << 20)) return bad("beam selection: need 1 .. 2^20 rows");
+  if (V < 1 || V > 0x7FFFFFFFll) return bad("beam selection: empty vocabulary, or one of 2^31 or more");
+  if (k < 1 || k > kBeamMaxK) return bad("beam selection: k must be in [1, 64]");
+  return MTPB_OK;
+}
+
+int beam_rows(const void* logits, long long ld, int rows, int V, long long vstart, int V_plan, int k,
+              const uint8_t* finished, void* block, int dtype, cudaStream_t st) {
+  const BeamPlan b = beam_plan(rows, V_plan);
+  BeamRowsParams p;
+  p.logits = logits;
+  p.ld = ld;
+  p.V = V;
+  p.k = k;
+  p.vstart = vstart;
+  p.nchunk = b.nchunk;
+  p.chunk = b.chunk;
+  p.finished = finished;
+  p.cand = static_cast<uint64_t*>(block);
+  p.stat = reinterpret_cast<BeamStat*>(static_cast<char*>(block) + beam_cand_bytes(rows, b, k));
+  const dim3 grid(b.nchunk, rows);
+  return dtype == MTPB_BF16 ? host_launch(beam_rows_kernel<bf16>, grid, dim3(kBeamThreads), 0, st, p)
+                            : host_launch(beam_rows_kernel<float>, grid, dim3(kBeamThreads), 0, st, p);
+}
+
+int beam_pick(const void* blocks, int parts, int G, int W, int V_plan, int kc, const float* scores,
+              const uint8_t* finished, long long eos, int k, float* out_scores, int64_t* out_parents,
+              int64_t* out_tokens, uint8_t* out_finished, cudaStream_t st) {
+  const int rows = G * W;
+  const BeamPlan b = beam_plan(rows, V_plan);
+  const size_t block = beam_block(rows, b, kc);
+  BeamPickParams p;
+  p.cand = static_cast<const uint64_t*>(blocks);
+  p.stat = reinterpret_cast<const BeamStat*>(static_cast<const char*>(blocks) + beam_cand_bytes(rows, b, kc));
+  p.cand_part = block / 8;
+  p.stat_part = block / sizeof(BeamStat);
+  p.parts = parts;
+  p.rows = rows;
+  p.nchunk = b.nchunk;
+  p.scores = scores;
+  p.finished = finished;
+  p.W = W;
+  p.k = k;
+  p.kc = kc;
+  p.eos = eos;
+  p.out_scores = out_scores;
+  p.out_parents = reinterpret_cast<long long*>(out_parents);
+  p.out_tokens = reinterpret_cast<long long*>(out_tokens);
+  p.out_finished = out_finished;
+  return host_launch(beam_pick_kernel, dim3(G), dim3(kBeamThreads), 0, st, p);
+}
+
+int pick_check(int G, int W, const float* scores, const uint8_t* finished, long long eos, const float* out_scores,
+               const int64_t* out_parents, const int64_t* out_tokens) {
+  if (G < 1 || W < 1 || W > kBeamMaxW || (long long)G * W > (1 << 20))
+    return bad("beam selection: need 1 .. 64 beams and at most 2^20 rows");
+  if (!scores || !out_scores || !out_parents || !out_tokens) return bad("beam selection: null tensor");
+  if (finished && eos < 0) return bad("beam selection: finished beams need an end token");
+  if (eos > 0xFFFFFFFFll) return bad("beam selection: end token out of range");
+  return MTPB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+long long mtpb_beam_block_bytes(int rows, int V_plan, int k) {
+  const int r = beam_check(rows, V_plan, k);
+  if (r != MTPB_OK) return r;
+  return (long long)beam_block(rows, beam_plan(rows, V_plan), k);
+}
+
+int mtpb_beam_candidates(const void* logits, int64_t ld, int rows, int V_local, int64_t vstart, int V_plan, int k,
+                         const uint8_t* finished, void* block, int dtype, void* stream) {
+  const int r = beam_check(rows, V_plan, k);
+  if (r != MTPB_OK) return r;
+  if ((!logits && V_local > 0) || !block) return bad("beam_candidates: null tensor");
+  if (!dtype_ok(dtype)) return bad("unsupported dtype");
+  if (rows > 65535) return bad("beam_candidates: more than 65535 rows");
+  if (V_local < 0 || V_local > V_plan || ld < V_local) return bad("beam_candidates: need 0 <= V_local <= V_plan, ld");
+  if (vstart < 0 || vstart + V_local > 0xFFFFFFFFll) return bad("beam_candidates: vocabulary ids out of range");
+  if (!al16(block)) return bad("beam_candidates: block must be 16-byte aligned");
+  return beam_rows(logits, ld, rows, V_local, vstart, V_plan, k, finished, block, dtype,
+                   static_cast<cudaStream_t>(stream));
+}
+
+int mtpb_beam_pick(const void* blocks, int parts, int G, int W, int V_plan, int k_block, const float* scores,
+                   const uint8_t* finished, int64_t eos, int k, float* out_scores, int64_t* out_parents,
+                   int64_t* out_tokens, uint8_t* out_finished, void* stream) {
+  int r = pick_check(G, W, scores, finished, eos, out_scores, out_parents, out_tokens);
+  if (r != MTPB_OK) return r;
+  r = beam_check((long long)G * W, V_plan, k_block);
+  if (r != MTPB_OK) return r;
+  if (!blocks || !al16(blocks)) return bad("beam_pick: blocks must be 16-byte aligned");
+  if (parts < 1 || parts > 64) return bad("beam_pick: need 1 .. 64 shards");
+  if (k < 1 || k > k_block) return bad("beam_pick: k must be in [1, the blocks' k]");
+  return beam_pick(blocks, parts, G, W, V_plan, k_block, scores, finished, eos, k, out_scores, out_parents,
+                   out_tokens, out_finished, static_cast<cudaStream_t>(stream));
+}
+
+int mtpb_beam_select(const void* logits, int64_t ld, int G, int W, int V, const float* scores,
+                     const uint8_t* finished, int64_t eos, int k, float* out_scores, int64_t* out_parents,
+                     int64_t* out_tokens, uint8_t* out_finished, void* block, int dtype, void* stream) {
+  int r = pick_check(G, W, scores, finished, eos, out_scores, out_parents, out_tokens);
+  if (r != MTPB_OK) return r;
+  r = mtpb_beam_candidates(logits, ld, G * W, V, 0, V, k, finished, block, dtype, stream);
+  if (r != MTPB_OK) return r;
+  return beam_pick(block, 1, G, W, V, k, scores, finished, eos, k, out_scores, out_parents, out_tokens, out_finished,
+                   static_cast<cudaStream_t>(stream));
+}
+
+int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers, const int64_t* parents,
+                    const int* lens, int len, int G, int W, int hkv, int cap, int hd, int dtype, void* stream) {
+  if (!k_caches || !v_caches || !parents) return bad("kv_reorder: null tensor");
+  if (!dtype_ok(dtype)) return bad("unsupported dtype");
+  if (n_layers < 1 || G < 1 || W < 1 || W > kBeamMaxW || hkv < 1 || cap < 1 || hd < 1)
+    return bad("kv_reorder: sizes must be positive, with at most 64 rows a group");
+  if ((long long)G * hkv > 65535) return bad("kv_reorder: groups x heads exceed 65535");
+  if (!lens && (len < 0 || len > cap)) return bad("kv_reorder: length outside the cache");
+  const size_t bytes = size_t(hd) * es_of(dtype);
+  if (bytes % 16) return bad("kv_reorder: head_dim x element size must be a multiple of 16 bytes");
+  for (int l = 0; l < n_layers; ++l)
+    if (!k_caches[l] || !v_caches[l] || !al16(k_caches[l]) || !al16(v_caches[l]))
+      return bad("kv_reorder: caches must be 16-byte aligned");
+  const bool wide = W > 32;  // 8-byte columns keep 64 rows in registers
+  const long long rv = bytes / (wide ? 8 : 16);
+  const long long top = lens ? cap : len;
+  if (W == 1 || top == 0) return MTPB_OK;
+  const long long blocks = (top * rv + kReorderThreads - 1) / kReorderThreads;
+  if (blocks > 0x7FFFFFFFll) return bad("kv_reorder: cache too long");
+  for (int l0 = 0; l0 < n_layers; l0 += kReorderLayers) {
+    const int n = std::min(kReorderLayers, n_layers - l0);
+    ReorderParams p;
+    std::memset(&p, 0, sizeof(p));
+    for (int l = 0; l < n; ++l) {
+      p.k[l] = k_caches[l0 + l];
+      p.v[l] = v_caches[l0 + l];
+    }
+    p.parents = reinterpret_cast<const long long*>(parents);
+    p.lens = lens;
+    p.len = len;
+    p.G = G;
+    p.W = W;
+    p.hkv = hkv;
+    p.cap = cap;
+    p.rv = int(rv);
+    const dim3 grid((unsigned)blocks, G * hkv, 2 * n), block(kReorderThreads);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int r = wide      ? host_launch(reorder_kernel<uint2, 64>, grid, block, 0, st, p)
+                  : W <= 4  ? host_launch(reorder_kernel<uint4, 4>, grid, block, 0, st, p)
+                  : W <= 8  ? host_launch(reorder_kernel<uint4, 8>, grid, block, 0, st, p)
+                  : W <= 16 ? host_launch(reorder_kernel<uint4, 16>, grid, block, 0, st, p)
+                            : host_launch(reorder_kernel<uint4, 32>, grid, block, 0, st, p);
+    if (r != MTPB_OK) return r;
+  }
+  return MTPB_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ attention over a shared prefix
+namespace {
+
+struct SaPlan {
+  int rpt;  // rows a tile / 16
+  int sp, so, ptiles, otiles;
+  long long pitems, items;
+  size_t rows, ml_bytes, o_bytes;
+};
+
+// Row tiles of 64 when a group (or a row of many tokens) fills them, else of
+// 16; key ranges until the items give every SM four, but no range below two
+// key tiles.
+int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
+  if (a.G < 1 || a.W < 1 || a.T < 1 || a.hq < 1 || a.hkv < 1 || a.cap_p < 1 || a.cap < 1)
+    return bad("shared_attention: sizes must be positive");
+  if (a.hq % a.hkv) return bad("shared_attention: hq must be a multiple of hkv");
+  if (a.hd != 16 && a.hd != 32 && a.hd != 64 && a.hd != 128)
+    return bad("shared_attention: head_dim must be 16, 32, 64 or 128");
+  if (!dtype_ok(a.dtype)) return bad("unsupported dtype");
+  const double rows = double(a.G) * a.W * a.T * a.hq;
+  if (rows > double(1 << 28)) return bad("shared_attention: more than 2^28 (token, head) rows");
+  SaPlan pl;
+  const int per = a.hq / a.hkv;
+  const long long prow = (long long)a.W * a.T * per, orow = (long long)a.T * per;
+  pl.rpt = orow >= 64 ? 4 : 1;
+  const int tile = 16 * pl.rpt;
+  pl.ptiles = int((prow + tile - 1) / tile);
+  pl.otiles = int((orow + tile - 1) / tile);
+  const long long pbase = (long long)a.G * a.hkv * pl.ptiles, obase = (long long)a.G * a.W * a.hkv * pl.otiles;
+  const int top_p = a.prefix_lens ? a.cap_p : a.prefix_len, top_o = a.cache_lens ? a.cap : a.cache_len;
+  const long long want = 4ll * 148;
+  auto splits = [&](long long base, int top) {
+    const long long most = std::max(1, (top + 2 * kSaKT - 1) / (2 * kSaKT));
+    return int(std::max<long long>(1, std::min<long long>(std::min<long long>(most, 64), (want + base - 1) / base)));
+  };
+  pl.sp = splits(pbase, top_p);
+  pl.so = splits(obase, top_o);
+  pl.pitems = pbase * pl.sp;
+  pl.items = pl.pitems + obase * pl.so;
+  if (pl.items > 0x7FFFFFFFll) return bad("shared_attention: too many rows");
+  pl.rows = size_t(rows);
+  pl.ml_bytes = (pl.rows * (pl.sp + pl.so) * 8 + 255) / 256 * 256;
+  pl.o_bytes = pl.rows * (pl.sp + pl.so) * a.hd * 4;
+  *out = pl;
+  return MTPB_OK;
+}
+
+template <typename T, int HD>
+int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
+  const int r = pl.rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)pl.items), dim3(kSaThreads),
+                                          sa_simt_smem<HD, 4>(), st, p)
+                            : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)pl.items), dim3(kSaThreads),
+                                          sa_simt_smem<HD, 1>(), st, p);
+  if (r != MTPB_OK) return r;
+  const size_t n = pl.rows * (HD / 4);
+  return host_launch(sa_join_kernel<T, HD>, dim3(unsigned((n + kSaJoinThreads - 1) / kSaJoinThreads)),
+                     dim3(kSaJoinThreads), 0, st, p);
+}
+
+template <typename T>
+int sa_launch_hd(const SaPlan& pl, const SaParams& p, int hd, cudaStream_t st) {
+  switch (hd) {
+    case 16: return sa_launch<T, 16>(pl, p, st);
+    case 32: return sa_launch<T, 32>(pl, p, st);
+    case 64: return sa_launch<T, 64>(pl, p, st);
+    default: return sa_launch<T, 128>(pl, p, st);
+  }
+}
+
+}  // namespace
+
+namespace mtpb {
+
+long long shared_attn_workspace(const SharedAttnArgs& a) {
+  SaPlan pl;
+  const int r = sa_plan(a, &pl);
+  return r == MTPB_OK ? (long long)(pl.ml_bytes + pl.o_bytes) : r;
+}
+
+int shared_attn_run(const SharedAttnArgs& a, void* ws, size_t ws_bytes, cudaStream_t st) {
+  SaPlan pl;
+  const int r = sa_plan(a, &pl);
+  if (r != MTPB_OK) return r;
+  if (!a.q || !a.k_prefix || !a.v_prefix || !a.k_cache || !a.v_cache || !a.out || !ws)
+    return bad("shared_attention: null tensor");
+  if (!al16(a.q) || !al16(a.k_prefix) || !al16(a.v_prefix) || !al16(a.k_cache) || !al16(a.v_cache) || !al16(a.out) ||
+      !al16(ws))
+    return bad("shared_attention: tensors must be 16-byte aligned");
+  if (!a.prefix_lens && (a.prefix_len < 0 || a.prefix_len > a.cap_p))
+    return bad("shared_attention: prefix length outside the prefix cache");
+  if (!a.cache_lens && (a.cache_len < 0 || a.cache_len > a.cap))
+    return bad("shared_attention: length outside the cache");
+  if (ws_bytes < pl.ml_bytes + pl.o_bytes) return bad("shared_attention: workspace too small");
+  SaParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = a.q;
+  p.kp = a.k_prefix;
+  p.vp = a.v_prefix;
+  p.plen = a.prefix_lens;
+  p.plen_all = a.prefix_len;
+  p.kc = a.k_cache;
+  p.vc = a.v_cache;
+  p.clen = a.cache_lens;
+  p.clen_all = a.cache_len;
+  p.out = a.out;
+  p.G = a.G;
+  p.W = a.W;
+  p.T = a.T;
+  p.hq = a.hq;
+  p.hkv = a.hkv;
+  p.cap_p = a.cap_p;
+  p.cap = a.cap;
+  p.scale = 1.0f / std::sqrt(float(a.hd));
+  p.sp = pl.sp;
+  p.so = pl.so;
+  p.ptiles = pl.ptiles;
+  p.otiles = pl.otiles;
+  p.pitems = int(pl.pitems);
+  p.items = int(pl.items);
+  p.part_ml = static_cast<float*>(ws);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.ml_bytes);
+  return a.dtype == MTPB_BF16 ? sa_launch_hd<bf16>(pl, p, a.hd, st) : sa_launch_hd<float>(pl, p, a.hd, st);
+}
+
+}  // namespace mtpb
+
+extern "C" {
+
+long long mtpb_shared_attention_workspace(int G, int W, int T, int hq, int hkv, int hd, int cap_p, int cap,
+                                          int dtype) {
+  SharedAttnArgs a;
+  std::memset(&a, 0, sizeof(a));
+  static const int any = 0;
+  a.G = G;
+  a.W = W;
+  a.T = T;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.hd = hd;
+  a.cap_p = cap_p;
+  a.cap = cap;
+  a.dtype = dtype;
+  a.prefix_lens = a.cache_lens = &any;  // lengths on the device: plans go by the capacities
+  return shared_attn_workspace(a);
+}
+
+int mtpb_shared_attention(const void* q, const void* k_prefix, const void* v_prefix, const int* prefix_lens,
+                          int prefix_len, const void* k_cache, const void* v_cache, const int* cache_lens,
+                          int cache_len, void* out, int G, int W, int T, int hq, int hkv, int hd, int cap_p, int cap,
+                          int dtype, void* ws, uint64_t ws_bytes, void* stream) {
+  SharedAttnArgs a;
+  a.q = q;
+  a.k_prefix = k_prefix;
+  a.v_prefix = v_prefix;
+  a.prefix_lens = prefix_lens;
+  a.prefix_len = prefix_len;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.cache_lens = cache_lens;
+  a.cache_len = cache_len;
+  a.out = out;
+  a.G = G;
+  a.W = W;
+  a.T = T;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.hd = hd;
+  a.cap_p = cap_p;
+  a.cap = cap;
+  a.dtype = dtype;
+  return shared_attn_run(a, ws, size_t(ws_bytes), static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

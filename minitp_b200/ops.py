@@ -7,6 +7,8 @@ stream. None of them has a CPU path: CPU tensors raise.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from minitp_b200 import _lib
@@ -171,4 +173,210 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, hq:
     _lib.call("mtpb_attention", _c(q).data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), b, t, hq,
               hkv, hd, k_cache.shape[2], cache_len, _lib.dtype_code(q.dtype), _comm_handle(comm),
               _lib.stream_ptr(q.device))
+    return out
+
+
+# ---------------------------------------------------------------------- #
+# beam search, and attention over a shared prefix (no counterpart in the reference)
+# ---------------------------------------------------------------------- #
+def _same_device(name: str, *tensors: torch.Tensor | None) -> torch.device:
+    """The tensors' one CUDA device; raises when there is none or another."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _lib.require_cuda(t)
+        if t.device != dev:
+            raise _lib.MinitpB200Error(f"{name}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """Call a C entry with ``dev`` current (its kernels go to that device's stream)."""
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args)
+        return
+    with torch.cuda.device(dev):
+        _lib.call(name, *args)
+
+
+def _beam_inputs(name: str, logits, scores, k, finished, eos_token_id, least: int = 1):
+    """Checks shared by the beam selection calls -> (device, logits as rows, row stride)."""
+    if logits.dim() != 3 or scores.dim() != 2 or scores.shape != logits.shape[:2]:
+        raise _lib.MinitpB200Error(f"{name}: need logits [G, W, V] and scores [G, W], got {tuple(logits.shape)} and "
+                                   f"{tuple(scores.shape)}")
+    dev = _same_device(name, logits, scores, finished)
+    if scores.dtype != torch.float32 or not scores.is_contiguous():
+        raise _lib.MinitpB200Error(f"{name}: scores must be contiguous fp32")
+    g, w, v = logits.shape
+    if not (1 <= w <= 64 and 1 <= k <= 64 and g >= 1 and v >= least):
+        raise _lib.MinitpB200Error(f"{name}: need 1..64 beams, k in [1, 64] and a non-empty vocabulary")
+    if finished is not None:
+        if finished.dtype != torch.bool or finished.shape != scores.shape or not finished.is_contiguous():
+            raise _lib.MinitpB200Error(f"{name}: finished must be contiguous bool [G, W]")
+        if eos_token_id is None:
+            raise _lib.MinitpB200Error(f"{name}: finished beams need eos_token_id")
+    if eos_token_id is not None and not 0 <= eos_token_id < 2**32 - 1:
+        raise _lib.MinitpB200Error(f"{name}: eos_token_id {eos_token_id} out of range")
+    # rows of one stride are read in place; anything else is packed first
+    if logits.stride(2) != 1 or (g > 1 and w > 1 and logits.stride(0) != w * logits.stride(1)):
+        logits = logits.contiguous()
+    ld = logits.stride(1) if w > 1 else logits.stride(0) if g > 1 else v
+    if ld < v:  # an expanded dimension
+        logits, ld = logits.contiguous(), v
+    return dev, logits, ld
+
+
+def _beam_outputs(dev, g: int, k: int, flags: bool):
+    ids = torch.empty(2, g, k, dtype=torch.int64, device=dev)
+    return (torch.empty(g, k, dtype=torch.float32, device=dev), ids[0], ids[1],
+            torch.empty(g, k, dtype=torch.bool, device=dev) if flags else None)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: torch.Tensor | None = None,
+                eos_token_id: int | None = None):
+    """One beam-search step: the ``k`` best continuations of each prompt.
+
+    ``logits [G, W, V]`` (fp32 or bf16) of W beams, running ``scores [G, W]``
+    (fp32 sums of log-probabilities; -inf: an unused beam). A candidate (b, v)
+    scores ``scores[b] + log_softmax(logits[b])[v]``; equal scores go to the
+    lower ``b * V + v``. A beam flagged in ``finished`` (bool [G, W]) has one
+    candidate, ``eos_token_id`` at its own score.
+
+    Returns ``(scores, parents, tokens, finished)``, each ``[G, k]``, best
+    first (``finished`` is None without ``eos_token_id``). Places without a
+    candidate hold score -inf, parent 0 and the end token (or 0).
+    """
+    dev, logits, ld = _beam_inputs("beam_select", logits, scores, k, finished, eos_token_id)
+    g, w, v = logits.shape
+    out, parents, tokens, done = _beam_outputs(dev, g, k, eos_token_id is not None)
+    block = torch.empty(beam_block_bytes(g * w, v, k), dtype=torch.uint8, device=dev)
+    _call_on(dev, "mtpb_beam_select", logits.data_ptr(), ld, g, w, v, scores.data_ptr(), _lib.ptr(finished),
+             -1 if eos_token_id is None else eos_token_id, k, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+             _lib.ptr(done), block.data_ptr(), _lib.dtype_code(logits.dtype), _lib.stream_ptr(dev))
+    return out, parents, tokens, done
+
+
+def beam_block_bytes(rows: int, v_plan: int, k: int) -> int:
+    """Bytes of one shard's candidate block (``beam_candidates``)."""
+    n = _lib.load().mtpb_beam_block_bytes(rows, v_plan, k)
+    if n < 0:
+        _lib.check(n)
+    return n
+
+
+def beam_candidates(local_logits: torch.Tensor, k: int, vstart: int, v_plan: int,
+                    finished: torch.Tensor | None = None) -> torch.Tensor:
+    """One vocabulary shard ``[G, W, V_local]`` (columns from ``vstart``; it may be empty) reduced to a
+    block of candidates (uint8 [n]). ``v_plan``: the largest shard's columns, the same on every rank."""
+    g, w, v = local_logits.shape
+    zeros = local_logits.new_empty((g, w), dtype=torch.float32)  # stands for the scores in the checks
+    dev, x, ld = _beam_inputs("beam_candidates", local_logits, zeros, k, finished, 0, least=0)
+    block = torch.empty(beam_block_bytes(g * w, v_plan, k), dtype=torch.uint8, device=dev)
+    _call_on(dev, "mtpb_beam_candidates", x.data_ptr(), ld, g * w, v, vstart, v_plan, k, _lib.ptr(finished),
+             block.data_ptr(), _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
+    return block
+
+
+def beam_pick(blocks: torch.Tensor, scores: torch.Tensor, k: int, v_plan: int, finished: torch.Tensor | None = None,
+              eos_token_id: int | None = None):
+    """``beam_select``'s result from the candidate blocks ``[shards, n]`` of every vocabulary shard."""
+    dev = _same_device("beam_pick", blocks, scores, finished)
+    g, w = scores.shape
+    if blocks.dim() != 2 or blocks.dtype != torch.uint8 or not blocks.is_contiguous() or \
+            blocks.shape[1] != beam_block_bytes(g * w, v_plan, k):
+        raise _lib.MinitpB200Error("beam_pick: blocks must be contiguous uint8 [shards, beam_block_bytes(rows, v_plan, k)]")
+    if scores.dtype != torch.float32 or not scores.is_contiguous():
+        raise _lib.MinitpB200Error("beam_pick: scores must be contiguous fp32")
+    if finished is not None and (finished.dtype != torch.bool or finished.shape != scores.shape
+                                 or not finished.is_contiguous() or eos_token_id is None):
+        raise _lib.MinitpB200Error("beam_pick: finished must be contiguous bool [G, W], with eos_token_id")
+    out, parents, tokens, done = _beam_outputs(dev, g, k, eos_token_id is not None)
+    _call_on(dev, "mtpb_beam_pick", blocks.data_ptr(), blocks.shape[0], g, w, v_plan, k, scores.data_ptr(),
+             _lib.ptr(finished), -1 if eos_token_id is None else eos_token_id, k, out.data_ptr(), parents.data_ptr(),
+             tokens.data_ptr(), _lib.ptr(done), _lib.stream_ptr(dev))
+    return out, parents, tokens, done
+
+
+def _length_arg(name: str, lengths, count: int, dev):
+    """(device pointer or None, host value) of a per-row length argument."""
+    if isinstance(lengths, int):
+        return None, lengths
+    if lengths.dtype != torch.int32 or lengths.shape != (count,) or not lengths.is_contiguous() or \
+            lengths.device != dev:
+        raise _lib.MinitpB200Error(f"{name}: lengths must be an int or contiguous int32 [{count}] on {dev}")
+    return lengths.data_ptr(), 0
+
+
+def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
+    """In place, in every layer: row ``g * W + w`` becomes row ``g * W + parents[g, w]``.
+
+    ``k_caches`` / ``v_caches``: lists of ``[G * W, hkv, cap, hd]`` caches;
+    ``parents`` int64 ``[G, W]``. The first ``lengths`` positions of the source
+    row are copied (an int, or int32 ``[G * W]`` by source row); later ones stay
+    as they were. A parent outside [0, W) leaves its row alone.
+    """
+    name = "reorder_cache_"
+    if parents.dim() != 2 or parents.dtype != torch.int64 or not parents.is_contiguous():
+        raise _lib.MinitpB200Error(f"{name}: parents must be contiguous int64 [G, W]")
+    caches = [*k_caches, *v_caches]
+    n = len(caches) // 2
+    if n == 0 or len(k_caches) != n or len(v_caches) != n:
+        raise _lib.MinitpB200Error(f"{name}: need as many K as V caches")
+    first = caches[0]
+    dev = _same_device(name, parents, first)
+    shape, dtype = first.shape, first.dtype
+    g, w = parents.shape
+    if first.dim() != 4 or shape[0] != g * w:
+        raise _lib.MinitpB200Error(f"{name}: caches must be [{g * w}, hkv, cap, hd], got {tuple(shape)}")
+    for t in caches:
+        if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+            raise _lib.MinitpB200Error(f"{name}: caches must be contiguous, of one shape, dtype and device")
+    lens, length = _length_arg(name, lengths, g * w, dev)
+    ptrs = (ctypes.c_void_p * (2 * n))(*[t.data_ptr() for t in caches])
+    _call_on(dev, "mtpb_kv_reorder", ptrs, ctypes.addressof(ptrs) + 8 * n, n, parents.data_ptr(), lens, length, g, w,
+             shape[1], shape[2], shape[3], _lib.dtype_code(dtype), _lib.stream_ptr(dev))
+
+
+def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, prefix_lens,
+                            k_cache: torch.Tensor, v_cache: torch.Tensor, cache_lens, hq: int,
+                            hkv: int) -> torch.Tensor:
+    """Grouped-query attention of rows that share a prefix -> ``[N, T, hq * hd]``.
+
+    ``q [N, T, hq * hd]``; prefix caches ``[G, hkv, cap_p, hd]``, one for every
+    ``N / G`` consecutive rows; own caches ``[N, hkv, cap, hd]``. Token t of row
+    n sees positions ``[0, prefix_lens[g])`` of the prefix and
+    ``[0, cache_lens[n] - (T - 1 - t))`` of its own cache (which holds the T
+    tokens already); one that sees nothing gets 0. Lengths are ints or int32
+    tensors ``[G]`` / ``[N]``, clamped to their cache.
+    """
+    name = "shared_prefix_attention"
+    dev = _same_device(name, q, k_prefix, v_prefix, k_cache, v_cache)
+    if q.dim() != 3 or k_prefix.dim() != 4 or k_cache.dim() != 4:
+        raise _lib.MinitpB200Error(f"{name}: need q [N, T, hq*hd] and caches [rows, hkv, cap, hd]")
+    n, t, _ = q.shape
+    g, _, cap_p, hd = k_prefix.shape
+    cap = k_cache.shape[2]
+    if g < 1 or n < 1 or t < 1 or n % g or hq < 1 or hkv < 1 or hq % hkv:
+        raise _lib.MinitpB200Error(f"{name}: {n} rows of {t} tokens in {g} groups, {hq} heads over {hkv}")
+    if q.shape[2] != hq * hd or k_prefix.shape != (g, hkv, cap_p, hd) or v_prefix.shape != k_prefix.shape or \
+            k_cache.shape != (n, hkv, cap, hd) or v_cache.shape != k_cache.shape:
+        raise _lib.MinitpB200Error(f"{name}: shapes {tuple(q.shape)}, {tuple(k_prefix.shape)}, {tuple(k_cache.shape)} "
+                                   "do not fit together")
+    for c in (k_prefix, v_prefix, k_cache, v_cache):
+        if c.dtype != q.dtype or not c.is_contiguous():
+            raise _lib.MinitpB200Error(f"{name}: caches must be contiguous and of q's dtype")
+    q = _c(q)
+    plen, plen_all = _length_arg(name, prefix_lens, g, dev)
+    clen, clen_all = _length_arg(name, cache_lens, n, dev)
+    code = _lib.dtype_code(q.dtype)
+    need = _lib.load().mtpb_shared_attention_workspace(g, n // g, t, hq, hkv, hd, cap_p, cap, code)
+    if need < 0:
+        _lib.check(need)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    out = torch.empty_like(q)
+    _call_on(dev, "mtpb_shared_attention", q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), plen, plen_all,
+             k_cache.data_ptr(), v_cache.data_ptr(), clen, clen_all, out.data_ptr(), g, n // g, t, hq, hkv, hd, cap_p,
+             cap, code, ws.data_ptr(), need, _lib.stream_ptr(dev))
     return out

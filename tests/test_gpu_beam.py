@@ -1,0 +1,350 @@
+"""Beam selection, cache reordering and shared-prefix attention against plain 64-bit implementations."""
+
+import math
+
+import pytest
+import torch
+
+from tests import beam_ref
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ------------------------------------------------------------------ selection
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("g,w,v,k", [(1, 1, 1, 1), (1, 4, 1000, 4), (2, 3, 7, 5), (3, 8, 5000, 8), (1, 4, 151936, 4),
+                                     (2, 1, 151937, 64), (1, 64, 333, 64), (5, 5, 4097, 10), (1, 2, 8192, 33),
+                                     (40, 2, 20001, 4), (2, 2, 31, 64)])
+def test_select(lib, dtype, g, w, v, k):
+    from minitp_b200 import ops
+
+    r = _gen(g * 1000 + w * 100 + v + k)
+    x = (torch.randn(g, w, v, generator=r) * 3).to(DT[dtype])
+    s = torch.randn(g, w, generator=r) * 2 - 20
+    got = ops.beam_select(x.cuda(), s.cuda(), k)
+    beam_ref.check_select(got, x, s, k)
+    fin = torch.rand(g, w, generator=r) < 0.4
+    got = ops.beam_select(x.cuda(), s.cuda(), k, fin.cuda(), v // 2)
+    beam_ref.check_select(got, x, s, k, fin, v // 2)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_select_ties_go_to_the_lowest_index(lib, dtype):
+    from minitp_b200 import ops
+
+    for v, k in [(20, 6), (9000, 16), (30000, 64)]:
+        x = torch.zeros(1, 3, v, dtype=DT[dtype])
+        x[0, 2, 5] = -0.0  # the same value as +0.0
+        s = torch.zeros(1, 3)
+        out, par, tok, _ = ops.beam_select(x.cuda(), s.cuda(), k)
+        flat = (par * v + tok).cpu()[0].tolist()
+        assert flat == list(range(k))
+        assert float((out.cpu().double() + math.log(v)).abs().max()) <= beam_ref.select_tolerance(v, out.cpu().double())
+        # few distinct values: long runs of equal logits across chunk borders
+        y = torch.randint(0, 3, (1, 3, v), generator=_gen(v)).to(DT[dtype])
+        s = torch.tensor([[-1.0, -1.5, -9.0]])
+        beam_ref.check_select(ops.beam_select(y.cuda(), s.cuda(), k), y, s, k)
+
+
+def test_select_masks_infinities_and_nan(lib):
+    from minitp_b200 import ops
+
+    inf, nan = math.inf, math.nan
+    lowest = torch.finfo(torch.float32).min
+    x = torch.full((4, 3, 40), -inf)
+    x[0, 0, :3] = torch.tensor([1.0, nan, 2.0])  # a banned token by NaN
+    x[0, 1, 7] = 0.5  # one token left; beam 2 has none
+    x[1, 0, 4:6] = inf  # two +inf tokens share the probability
+    x[1, 0, 8] = 3.0
+    x[1, 1] = lowest  # masked by the type's lowest value: a uniform row
+    x[1, 2] = nan
+    x[2] = torch.randn(3, 40, generator=_gen(1))
+    s = torch.tensor([[-1.0, -2.0, 0.0], [-1.0, -2.0, -3.0], [-inf, nan, -4.0], [0.0, 0.0, 0.0]])
+    for k in (1, 3, 8, 50):
+        beam_ref.check_select(ops.beam_select(x.cuda(), s.cuda(), k), x, s, k)
+    out, par, tok, _ = ops.beam_select(x.cuda(), s.cuda(), 4)
+    assert out[3].tolist() == [-inf] * 4 and par[3].tolist() == [0] * 4 and tok[3].tolist() == [0] * 4
+    assert out[1, 0].item() == pytest.approx(-1 - math.log(2), abs=1e-6) and tok[1, :2].tolist() == [4, 5]
+    fin = torch.tensor([[False, True, True]] * 4)
+    for k in (1, 3, 8):
+        beam_ref.check_select(ops.beam_select(x.cuda(), s.cuda(), k, fin.cuda(), 39), x, s, k, fin, 39)
+    y = x.to(torch.bfloat16)  # the lowest fp32 value becomes -inf there
+    beam_ref.check_select(ops.beam_select(y.cuda(), s.cuda(), 8), y, s, 8)
+
+
+def test_select_first_step_from_one_beam(lib):
+    """The first step: one live beam per prompt gives k different tokens."""
+    from minitp_b200 import ops
+
+    x = torch.randn(2, 1, 999, generator=_gen(3))
+    s = torch.zeros(2, 1)
+    out, par, tok, _ = ops.beam_select(x.cuda(), s.cuda(), 8)
+    want = torch.log_softmax(x.double(), -1)[:, 0].topk(8)
+    assert torch.equal(tok.cpu(), want.indices) and int(par.sum()) == 0
+    # the same from 8 beams of which one is in use
+    x8 = x.expand(2, 8, 999).contiguous()
+    s8 = torch.full((2, 8), -math.inf)
+    s8[:, 0] = 0
+    again = ops.beam_select(x8.cuda(), s8.cuda(), 8)
+    assert torch.equal(again[2], tok) and torch.equal(again[0], out)
+
+
+def test_select_strides(lib):
+    from minitp_b200 import ops
+
+    r = _gen(5)
+    big = torch.randn(6, 4, 1013, generator=r).cuda()
+    s = torch.randn(6, 4, generator=r).cuda()
+    views = [big[:, :, 3:1000], big[:, :, 1:2], big[:, ::2, :800], big[::2], big.transpose(0, 1)[:, :4],
+             big[:1, :1].expand(6, 4, 1013), big[:, 1:2], big[2:3, :, 5:]]
+    for x in views:
+        sc = s[: x.shape[0], : x.shape[1]].contiguous()
+        beam_ref.check_select(ops.beam_select(x, sc, 4), x, sc, 4)
+    xb = torch.randn(3, 2, 2051, generator=r).to(torch.bfloat16).cuda()[:, :, 1:]  # rows off every vector border
+    beam_ref.check_select(ops.beam_select(xb, s[:3, :2].contiguous(), 7), xb, s[:3, :2], 7)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("parts,v", [(2, 151937), (3, 10), (8, 4099), (4, 3)])
+def test_select_from_vocabulary_shards(lib, dtype, parts, v):
+    """Candidates of uneven shards, picked together, are the selection over the whole vocabulary."""
+    from minitp_b200 import ops
+    from minitp_b200.parallel.linear import shard_range
+
+    r = _gen(v)
+    g, w, k, eos = 2, 4, 8, 1
+    x = (torch.randn(g, w, v, generator=r) * 2).to(DT[dtype]).cuda()
+    s = torch.randn(g, w, generator=r).cuda()
+    fin = (torch.rand(g, w, generator=r) < 0.3).cuda()
+    plan = -(-v // parts)
+    blocks = []
+    for p in range(parts):
+        a, b = shard_range(v, p, parts)
+        blocks.append(ops.beam_candidates(x[:, :, a:b], k, a, plan, fin))
+    got = ops.beam_pick(torch.stack(blocks), s, k, plan, fin, eos)
+    beam_ref.check_select(got, x, s, k, fin, eos)
+
+
+def test_select_streams_and_graph(lib):
+    """Two calls at once on two streams, and a captured call replayed on new inputs."""
+    from minitp_b200 import ops
+
+    r = _gen(9)
+    xs = [torch.randn(4, 4, 30000, generator=r).cuda() for _ in range(2)]
+    s = torch.randn(4, 4, generator=r).cuda()
+    want = [ops.beam_select(x, s, 4) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for st, x in zip(streams, xs):
+            with torch.cuda.stream(st):
+                got.append(ops.beam_select(x, s, 4))
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(o[:3], want[i % 2][:3]))
+    x = xs[0].clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = ops.beam_select(x, s, 4)
+    for i in (1, 0, 1):
+        x.copy_(xs[i])
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(o[:3], want[i][:3]))
+
+
+# ------------------------------------------------------------------ reordering
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("layers,g,w,hkv,hd,cap", [(1, 1, 1, 1, 16, 4), (2, 1, 4, 2, 16, 9), (3, 2, 8, 1, 64, 33),
+                                                   (2, 3, 5, 4, 128, 17), (1, 1, 16, 2, 64, 40), (70, 1, 3, 1, 16, 5),
+                                                   (2, 1, 27, 2, 32, 12), (1, 2, 64, 1, 128, 7)])
+def test_reorder(lib, dtype, layers, g, w, hkv, hd, cap):
+    from minitp_b200 import ops
+
+    r = _gen(layers * 100 + w)
+    mk = lambda: [torch.randn(g * w, hkv, cap, hd, generator=r).to(DT[dtype]) for _ in range(layers)]  # noqa: E731
+    for parents in (torch.randint(0, w, (g, w), generator=r), torch.arange(w).flip(0).repeat(g, 1),
+                    torch.arange(w).roll(1).repeat(g, 1), torch.zeros(g, w, dtype=torch.int64),
+                    torch.arange(w).repeat(g, 1)):
+        for lengths in (torch.randint(0, cap + 1, (g * w,), generator=r, dtype=torch.int32), cap, 0, 1):
+            k, v = mk(), mk()
+            kg, vg = [t.cuda() for t in k], [t.cuda() for t in v]
+            ops.reorder_cache_(kg, vg, parents.cuda(), lengths if isinstance(lengths, int) else lengths.cuda())
+            ln = [lengths] * (g * w) if isinstance(lengths, int) else lengths
+            for a, b in zip(kg + vg, k + v):
+                assert torch.equal(a.cpu(), beam_ref.reorder(b, parents, ln))
+
+
+def test_reorder_leaves_rows_of_parents_out_of_range(lib):
+    from minitp_b200 import ops
+
+    k, v = (torch.randn(4, 1, 6, 16).cuda() for _ in range(2))
+    k0, v0 = k.clone(), v.clone()
+    parents = torch.tensor([[1, -1, 4, 2 ** 40]]).cuda()
+    lens = torch.tensor([3, 100, -5, 6], dtype=torch.int32).cuda()  # clamped to the cache
+    ops.reorder_cache_([k], [v], parents, lens)
+    k0[0], v0[0] = k0[1], v0[1]
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+def test_reorder_in_a_graph(lib):
+    from minitp_b200 import ops
+
+    r = _gen(2)
+    src = [torch.randn(8, 2, 20, 64, generator=r).cuda() for _ in range(4)]
+    k, v = [t.clone() for t in src[:2]], [t.clone() for t in src[2:]]
+    parents = torch.arange(4).repeat(2, 1).cuda()
+    lens = torch.full((8,), 20, dtype=torch.int32).cuda()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.reorder_cache_(k, v, parents, lens)
+    for seed in (3, 4):
+        parents.copy_(torch.randint(0, 4, (2, 4), generator=_gen(seed)))
+        lens.fill_(seed * 4)
+        for a, b in zip(k + v, src):
+            a.copy_(b)
+        g.replay()
+        for a, b in zip(k + v, src):
+            assert torch.equal(a.cpu(), beam_ref.reorder(b.cpu(), parents.cpu(), lens.cpu()))
+
+
+# ------------------------------------------------------------------ attention
+def _attention_case(seed, dtype, g, w, t, hq, hkv, hd, cap_p, plens, cap, clens, poison=math.nan):
+    r = _gen(seed)
+    dt = DT[dtype]
+    q = (torch.randn(g * w, t, hq * hd, generator=r) * 1.5).to(dt)
+    kp, vp = (torch.randn(g, hkv, cap_p, hd, generator=r).to(dt) for _ in range(2))
+    kc, vc = (torch.randn(g * w, hkv, cap, hd, generator=r).to(dt) for _ in range(2))
+    for i, n in enumerate(plens):  # what lies behind the last position is never used
+        kp[i, :, max(0, n):] = poison
+        vp[i, :, max(0, n):] = poison
+    for i, n in enumerate(clens):
+        kc[i, :, max(0, n):] = poison
+        vc[i, :, max(0, n):] = poison
+    return q, kp, vp, torch.tensor(plens, dtype=torch.int32), kc, vc, torch.tensor(clens, dtype=torch.int32)
+
+
+def _check_attention(case, hq, hkv):
+    from minitp_b200 import ops
+
+    got = ops.shared_prefix_attention(*(x.cuda() for x in case), hq, hkv).cpu()
+    want, tol = beam_ref.attend(*case, hq, hkv)
+    assert got.dtype == case[0].dtype
+    off = (got.double() - want).abs()
+    assert torch.isfinite(got.float()).all()
+    assert bool((off <= tol).all()), float((off - tol).max())
+    return got
+
+
+HEADS = [(4, 2, 16), (8, 4, 32), (14, 2, 64), (7, 1, 128), (28, 4, 128), (4, 1, 128), (3, 3, 64)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,hd", HEADS)
+@pytest.mark.parametrize("g,w,plens,clens", [
+    (1, 1, [1], [1]),
+    (1, 4, [128], [16] * 4),
+    (2, 3, [65, 200], [0, 1, 2, 63, 64, 65]),
+    (3, 2, [0, 1, 513], [0, 5, 0, 130, 129, 0]),
+])
+def test_attention_single_tokens(lib, dtype, hq, hkv, hd, g, w, plens, clens):
+    case = _attention_case(hq * hd + g + w, dtype, g, w, 1, hq, hkv, hd, max(plens) + 3, plens, max(clens) + 2, clens)
+    got = _check_attention(case, hq, hkv)
+    for r in range(g * w):
+        if plens[r // w] == 0 and clens[r] == 0:
+            assert int((got[r] != 0).sum()) == 0  # nothing seen: zeros
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,hd", [(4, 2, 16), (14, 2, 64), (7, 1, 128)])
+@pytest.mark.parametrize("g,w,t,plens,clens", [
+    (1, 2, 5, [70], [5, 9]),
+    (2, 2, 19, [0, 33], [19, 25, 40, 3]),  # fewer own positions than tokens: the first tokens see only the prefix
+    (1, 1, 140, [129], [140]),
+    (2, 1, 33, [300, 0], [0, 60]),
+])
+def test_attention_many_tokens(lib, dtype, hq, hkv, hd, g, w, t, plens, clens):
+    case = _attention_case(hq + hd + t, dtype, g, w, t, hq, hkv, hd, max(plens) + 1, plens, max(clens) + 5, clens)
+    _check_attention(case, hq, hkv)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_attention_wide_groups_and_long_prefixes(lib, dtype):
+    # 40 rows x 7 heads fill more than two row tiles; the prefix ends inside a key tile
+    case = _attention_case(1, dtype, 1, 40, 1, 7, 1, 128, 1500, [1333], 40, [i for i in range(40)])
+    _check_attention(case, 7, 1)
+    case = _attention_case(2, dtype, 2, 3, 1, 14, 2, 64, 5000, [4999, 2500], 700, [700, 1, 0, 333, 512, 640])
+    _check_attention(case, 14, 2)
+
+
+def test_attention_large_scores_and_masked_infinities(lib):
+    """Scores of hundreds (one key takes all), and infinities behind the last position."""
+    for dtype in ("fp32", "bf16"):
+        case = _attention_case(3, dtype, 1, 3, 1, 4, 2, 64, 200, [190], 30, [10, 0, 30], poison=math.inf)
+        q = (case[0].float() * 40).to(DT[dtype])
+        _check_attention((q, *case[1:]), 4, 2)
+
+
+def test_attention_lengths_are_clamped_and_may_be_ints(lib):
+    from minitp_b200 import ops
+
+    q, kp, vp, pl, kc, vc, cl = (x.cuda() for x in _attention_case(4, "bf16", 2, 2, 1, 14, 2, 64, 50, [50, 50], 20,
+                                                                   [20] * 4))
+    want = ops.shared_prefix_attention(q, kp, vp, pl, kc, vc, cl, 14, 2)
+    big = torch.tensor([51, 2 ** 30], dtype=torch.int32).cuda()
+    assert torch.equal(ops.shared_prefix_attention(q, kp, vp, big, kc, vc, cl + 7, 14, 2), want)
+    assert torch.equal(ops.shared_prefix_attention(q, kp, vp, 50, kc, vc, 20, 14, 2), want)
+    none = ops.shared_prefix_attention(q, kp, vp, pl * 0 - 3, kc, vc, 0, 14, 2)
+    assert int((none != 0).sum()) == 0
+
+
+def test_attention_equals_attention_over_one_cache(lib):
+    """Prefix and own cache laid end to end give the framework's plain attention."""
+    from minitp_b200 import ops
+
+    for dtype in ("fp32", "bf16"):
+        p, c = 300, 40
+        case = _attention_case(6, dtype, 1, 4, 1, 14, 2, 64, p, [p], c, [c] * 4)
+        q, kp, vp, pl, kc, vc, cl = (x.cuda() for x in case)
+        got = ops.shared_prefix_attention(q, kp, vp, pl, kc, vc, cl, 14, 2)
+        k = torch.cat([kp.expand(4, -1, -1, -1), kc], 2).contiguous()
+        v = torch.cat([vp.expand(4, -1, -1, -1), vc], 2).contiguous()
+        one = ops.attention(q, k, v, 14, 2, p + c - 1)
+        want, tol = beam_ref.attend(*case, 14, 2)
+        assert bool(((got.cpu().double() - want).abs() <= tol).all())
+        assert bool(((one.cpu().double() - want).abs() <= tol).all())
+
+
+def test_attention_streams_and_graph(lib):
+    from minitp_b200 import ops
+
+    cases = [[x.cuda() for x in _attention_case(s, "bf16", 1, 8, 1, 28, 4, 128, 700, [600], 64, [40] * 8)]
+             for s in (1, 2)]
+    want = [ops.shared_prefix_attention(*c, 28, 4) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for st, c in zip(streams, cases):
+            with torch.cuda.stream(st):
+                got.append(ops.shared_prefix_attention(*c, 28, 4))
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 2])
+    own = [x.clone() for x in cases[0]]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = ops.shared_prefix_attention(*own, 28, 4)
+    for i in (1, 0, 1):
+        for a, b in zip(own, cases[i]):
+            a.copy_(b)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want[i])
