@@ -348,6 +348,24 @@ int mtpb_model_forward(void* model, const int64_t* ids, int B, int T, const int6
                        int cache_len, void* const* k_caches, void* const* v_caches, int cap,
                        void* logits, int last_only, void* stream);
 
+/* Forward of N x T tokens whose rows share prefixes: as mtpb_model_forward
+ * over the rows' own caches [N, hkv, cap, hd], but every row also attends to
+ * its group's prefix (k_prefix / v_prefix: host arrays of n_layers device
+ * pointers, each [G, hkv, cap_p, hd]; group g holds rows g*N/G ..; valid
+ * positions prefix_lens[g], device int32 [G], or prefix_len when NULL).
+ * rope_pos (device int64 [T], required) counts the prefix too. slot_ptr
+ * (device int32, may be NULL, T == 1 only): the own-cache slot of the new
+ * token, read on the device instead of cache_len, so that a captured step can
+ * be replayed. The workspace of the attention belongs to the model and is
+ * allocated on the first call of a size, which must not be under capture.
+ * No counterpart in the reference. */
+int mtpb_model_forward_shared(void* model, const int64_t* ids, int N, int T,
+                              const int64_t* rope_pos, const int* slot_ptr, int cache_len,
+                              void* const* k_caches, void* const* v_caches, int cap,
+                              const void* const* k_prefix, const void* const* v_prefix,
+                              const int* prefix_lens, int prefix_len, int G, int cap_p,
+                              void* logits, int last_only, void* stream);
+
 /* One greedy decode step for B rows, all state on the device: reads the
  * tokens from `tok` (device int64 [B]) and the position from
  * mtpb_comm_pos_ptr(), runs the model, selects the next tokens (distributed

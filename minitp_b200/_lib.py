@@ -120,6 +120,9 @@ SIGNATURES: dict[str, tuple] = {
     "mtpb_model_destroy": (c_int, [c_void_p]),
     "mtpb_model_forward": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,
                                    c_void_p, c_int, c_void_p]),
+    "mtpb_model_forward_shared": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                                          c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
+                                          c_int, c_void_p]),
     "mtpb_model_decode_step": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                        c_void_p, c_void_p]),
     "mtpb_model_decode_kernels": (c_int, [c_void_p, c_int, c_int, POINTER(c_int)]),

@@ -714,6 +714,9 @@ struct ModelHost {
   std::vector<MkLayer> mk_host;  // what mk_layers currently holds
   char* mk_scratch = nullptr;
   size_t mk_bytes = 0;
+  // workspace of the shared-prefix attention
+  void* sa_ws = nullptr;
+  size_t sa_bytes = 0;
 };
 
 int g_decode_impl = 0;  // 0: megakernel when the shape allows it, 1: kernel chain
@@ -757,6 +760,14 @@ int model_reserve(ModelHost& mh, int rows, cudaStream_t st) {
   return MTPB_OK;
 }
 
+// Prefix caches shared by groups of consecutive rows (mtpb_model_forward_shared).
+struct SharedPrefix {
+  int G, cap, len;
+  const int* lens;  // device [G], or NULL: len for all
+  const void* const* k;
+  const void* const* v;
+};
+
 struct FwdArgs {
   const long long* ids;  // embedding input [M]
   int B, T;
@@ -772,7 +783,51 @@ struct FwdArgs {
   long long* tok_out;
   long long* out_ids;
   int ld_out;
+  const SharedPrefix* shared;  // rows attend to a shared prefix as well (NULL: to their own cache only)
 };
+
+// The attention of layer l over tokens [pos, pos + tc) of every row (pos:
+// pos_base, or the device slot of a captured step).
+SharedAttnArgs shared_args(const ModelHost& mh, const FwdArgs& a, int l, int tc, int pos_base) {
+  const mtpb_model_desc& d = mh.d;
+  const SharedPrefix& sp = *a.shared;
+  SharedAttnArgs s;
+  s.q = mh.q;
+  s.k_prefix = sp.k[l];
+  s.v_prefix = sp.v[l];
+  s.prefix_lens = sp.lens;
+  s.prefix_len = sp.len;
+  s.k_cache = a.kc[l];
+  s.v_cache = a.vc[l];
+  s.cache_lens = a.pos_ptr;
+  s.cache_stride = 0;
+  s.cache_len = a.pos_ptr ? tc : pos_base + tc;
+  s.out = mh.attn;
+  s.G = sp.G;
+  s.W = a.B / sp.G;
+  s.T = tc;
+  s.hq = d.hq_local;
+  s.hkv = d.hkv_local;
+  s.hd = d.head_dim;
+  s.cap_p = sp.cap;
+  s.cap = a.cap;
+  s.dtype = d.dtype;
+  return s;
+}
+
+// Workspace of the shared-prefix attention for tc tokens a row.
+int shared_reserve(ModelHost& mh, const FwdArgs& a, int tc, cudaStream_t st) {
+  const long long need = shared_attn_workspace(shared_args(mh, a, 0, tc, a.cache_len));
+  if (need < 0) return int(need);
+  if (size_t(need) <= mh.sa_bytes) return MTPB_OK;
+  if (capturing(st)) return fail(MTPB_ERR_INVALID, "shared-prefix forward: run one call eagerly before graph capture");
+  MTPB_CUDA(cudaFree(mh.sa_ws));  // waits for the kernels that use it
+  mh.sa_ws = nullptr;
+  mh.sa_bytes = 0;
+  MTPB_CUDA(cudaMalloc(&mh.sa_ws, size_t(need)));
+  mh.sa_bytes = size_t(need);
+  return MTPB_OK;
+}
 
 // One forward over tokens [t0, t0 + tc) of every batch row (a chunk of the
 // caller's T tokens). Every collective payload is B * tc * H elements, which
@@ -790,7 +845,8 @@ int model_chunk_t(ModelHost& mh, const FwdArgs& a, int t0, int tc, bool last_chu
   const bool chunked = tc != a.T;
   // decode steps of many rows take the tensor cores, which read x from global
   // memory: no fused consume prologue for them
-  const bool tc_decode = a.decode && d.dtype == MTPB_BF16 && M >= g_tc_min_rows_decode;
+  const bool step = a.decode || (a.shared && a.T == 1);  // one token a row
+  const bool tc_decode = step && d.dtype == MTPB_BF16 && M >= g_tc_min_rows_decode;
   const bool fused_x = size_t(M) * H * sizeof(T) <= kXsStageMax && tc == 1 && !tc_decode;
   // sites consumed by the separate pass may take the two-shot form
   const int ts = fused_x ? 0 : ts_cols_for(size_t(M) * H * sizeof(T), H, comm.world, d.dtype);
@@ -867,7 +923,7 @@ int model_chunk_t(ModelHost& mh, const FwdArgs& a, int t0, int tc, bool last_chu
     // fused QKV + RoPE + KV append, consuming site 2l (embedding or previous down)
     {
       GemvParams g = gemv_base(ly.qkv_w, ly.qkv_b, M, qrows, H, qrows / 2);
-      g.decode = a.decode ? 1 : 0;
+      g.decode = step ? 1 : 0;
       MTPB_TRY(prepare_input(g, uint32_t(2 * l), ly.ln1, true));
       g.y = mh.q;
       g.ldy = hq * hd;
@@ -887,12 +943,17 @@ int model_chunk_t(ModelHost& mh, const FwdArgs& a, int t0, int tc, bool last_chu
       MTPB_TRY(gemv_dispatch<kEpiRope>(d.dtype, g, st));
     }
     // attention over the cache
-    MTPB_TRY(attn_run(d.dtype, mh.q, a.kc[l], a.vc[l], mh.attn, a.B, tc, hq, hkv, hd, a.cap, a.pos_ptr,
-                      pos_base, mh.ascr, comm.status(), st));
+    if (a.shared) {
+      const SharedAttnArgs sa = shared_args(mh, a, l, tc, pos_base);
+      MTPB_TRY(shared_attn_run(sa, mh.sa_ws, mh.sa_bytes, st));
+    } else {
+      MTPB_TRY(attn_run(d.dtype, mh.q, a.kc[l], a.vc[l], mh.attn, a.B, tc, hq, hkv, hd, a.cap, a.pos_ptr,
+                        pos_base, mh.ascr, comm.status(), st));
+    }
     // o_proj partial -> push site 2l+1
     {
       GemvParams g = gemv_base(ly.o_w, nullptr, M, H, hq * hd, H);
-      g.decode = a.decode ? 1 : 0;
+      g.decode = step ? 1 : 0;
       g.x = mh.attn;
       g.ldx = hq * hd;
       g.comm = comm;
@@ -905,7 +966,7 @@ int model_chunk_t(ModelHost& mh, const FwdArgs& a, int t0, int tc, bool last_chu
     // gate/up + SwiGLU, consuming site 2l+1
     {
       GemvParams g = gemv_base(ly.gu_w, nullptr, M, 2 * d.inter_local, H, d.inter_local);
-      g.decode = a.decode ? 1 : 0;
+      g.decode = step ? 1 : 0;
       MTPB_TRY(prepare_input(g, uint32_t(2 * l + 1), ly.ln2, true));
       g.y = mh.act;
       g.ldy = d.inter_local;
@@ -914,7 +975,7 @@ int model_chunk_t(ModelHost& mh, const FwdArgs& a, int t0, int tc, bool last_chu
     // down partial -> push site 2l+2
     {
       GemvParams g = gemv_base(ly.down_w, nullptr, M, H, d.inter_local, H);
-      g.decode = a.decode ? 1 : 0;
+      g.decode = step ? 1 : 0;
       g.x = mh.act;
       g.ldx = d.inter_local;
       g.comm = comm;
@@ -932,7 +993,7 @@ int model_chunk_t(ModelHost& mh, const FwdArgs& a, int t0, int tc, bool last_chu
   {
     const int rows = a.last_only ? a.B : M;
     GemvParams g = gemv_base(d.lm_head, nullptr, rows, vloc, H, vloc);
-    g.decode = a.decode ? 1 : 0;
+    g.decode = step ? 1 : 0;
     const bool direct = fused_x && rows == M;
     MTPB_TRY(prepare_input(g, uint32_t(2 * L), d.final_norm, direct));
     if (!direct && a.last_only) {
@@ -985,6 +1046,7 @@ int model_forward_t(ModelHost& mh, const FwdArgs& a, cudaStream_t st) {
   if (a.decode && (a.T != 1 || a.B > 64)) return fail(MTPB_ERR_INVALID, "decode step: T == 1 and B <= 64");
   const int tc = int(std::min<size_t>(size_t(a.T), comm.slot_bytes / row_bytes));
   MTPB_TRY(model_reserve(mh, a.B * tc, st));
+  if (a.shared) MTPB_TRY(shared_reserve(mh, a, tc, st));
   for (int t0 = 0; t0 < a.T; t0 += tc) {
     const int n = std::min(tc, a.T - t0);
     MTPB_TRY(model_chunk_t<T>(mh, a, t0, n, t0 + n == a.T, st));
@@ -1634,6 +1696,7 @@ int mtpb_model_destroy(void* model) {
   cudaFree(mh->ascr.counters);
   cudaFree(mh->mk_scratch);
   cudaFree(mh->mk_layers);
+  cudaFree(mh->sa_ws);
   delete mh;
   return MTPB_OK;
 }
@@ -1733,6 +1796,42 @@ int mtpb_model_forward(void* model, const int64_t* ids, int B, int T, const int6
   a.cap = cap;
   a.logits = logits;
   a.last_only = last_only;
+  return model_forward(*mh, a, static_cast<cudaStream_t>(stream));
+}
+
+int mtpb_model_forward_shared(void* model, const int64_t* ids, int N, int T, const int64_t* rope_pos,
+                              const int* slot_ptr, int cache_len, void* const* k_caches, void* const* v_caches, int cap,
+                              const void* const* k_prefix, const void* const* v_prefix, const int* prefix_lens,
+                              int prefix_len, int G, int cap_p, void* logits, int last_only, void* stream) {
+  if (!model || !ids || !rope_pos || !k_caches || !v_caches || !k_prefix || !v_prefix || !logits)
+    return fail(MTPB_ERR_INVALID, "model_forward_shared: null argument");
+  if (N <= 0 || T <= 0 || G <= 0 || N % G) return fail(MTPB_ERR_INVALID, "model_forward_shared: need rows in G equal groups");
+  if (cap <= 0 || cap_p <= 0 || cache_len < 0) return fail(MTPB_ERR_INVALID, "model_forward_shared: empty cache");
+  if (slot_ptr && T != 1) return fail(MTPB_ERR_INVALID, "model_forward_shared: a device slot needs T == 1");
+  if (!prefix_lens && (prefix_len < 0 || prefix_len > cap_p))
+    return fail(MTPB_ERR_INVALID, "model_forward_shared: prefix length outside the prefix cache");
+  auto* mh = static_cast<ModelHost*>(model);
+  SharedPrefix sp;
+  sp.G = G;
+  sp.cap = cap_p;
+  sp.len = prefix_len;
+  sp.lens = prefix_lens;
+  sp.k = k_prefix;
+  sp.v = v_prefix;
+  FwdArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.ids = reinterpret_cast<const long long*>(ids);
+  a.B = N;
+  a.T = T;
+  a.rope_pos = reinterpret_cast<const long long*>(rope_pos);
+  a.cache_len = cache_len;
+  a.pos_ptr = const_cast<int*>(slot_ptr);  // only read: no argmax, no advance
+  a.kc = k_caches;
+  a.vc = v_caches;
+  a.cap = cap;
+  a.logits = logits;
+  a.last_only = last_only;
+  a.shared = &sp;
   return model_forward(*mh, a, static_cast<cudaStream_t>(stream));
 }
 

@@ -304,7 +304,8 @@ int shared_attn_run(const SharedAttnArgs& a, void* ws, size_t ws_bytes, cudaStre
   p.kc = a.k_cache;
   p.vc = a.v_cache;
   p.clen = a.cache_lens;
-  p.clen_all = a.cache_len;
+  p.clen_stride = a.cache_stride;
+  p.clen_add = a.cache_len;
   p.out = a.out;
   p.G = a.G;
   p.W = a.W;
@@ -331,8 +332,7 @@ extern "C" {
 
 long long mtpb_shared_attention_workspace(int G, int W, int T, int hq, int hkv, int hd, int cap_p, int cap,
                                           int dtype) {
-  SharedAttnArgs a;
-  std::memset(&a, 0, sizeof(a));
+  SharedAttnArgs a = {};
   static const int any = 0;
   a.G = G;
   a.W = W;
@@ -360,7 +360,7 @@ int mtpb_shared_attention(const void* q, const void* k_prefix, const void* v_pre
   a.k_cache = k_cache;
   a.v_cache = v_cache;
   a.cache_lens = cache_lens;
-  a.cache_len = cache_len;
+  a.cache_len = cache_lens ? 0 : cache_len;
   a.out = out;
   a.G = G;
   a.W = W;

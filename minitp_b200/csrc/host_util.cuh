@@ -57,8 +57,9 @@ struct SharedAttnArgs {
   const int* prefix_lens;               // device [G], or NULL: prefix_len for all
   int prefix_len;
   const void *k_cache, *v_cache;        // [N][hkv][cap][hd]
-  const int* cache_lens;                // device [N], or NULL: cache_len for all
-  int cache_len;
+  const int* cache_lens;                // device [N], or NULL
+  int cache_stride = 1;                 // 0: every row reads cache_lens[0]
+  int cache_len;                        // added to the device value (alone without one)
   void* out;                            // [N*T][hq*hd]
   int G, W, T, hq, hkv, hd, cap_p, cap; // N = G * W
   int dtype;

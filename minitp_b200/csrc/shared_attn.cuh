@@ -23,7 +23,7 @@ struct SaParams {
   int plen_all;
   const void *kc, *vc;
   const int* clen;
-  int clen_all;
+  int clen_stride, clen_add;
   void* out;
   int G, W, T, hq, hkv, cap_p, cap;
   float scale;
@@ -39,8 +39,9 @@ __device__ __forceinline__ int sa_prefix_len(const SaParams& p, int g) {
   return max(0, min(n, p.cap_p));
 }
 __device__ __forceinline__ int sa_cache_len(const SaParams& p, int n) {
-  const int c = p.clen ? p.clen[n] : p.clen_all;
-  return max(0, min(c, p.cap));
+  // 64 bits: the sum of a length from the device and the host's offset
+  const long long c = (p.clen ? (long long)p.clen[size_t(n) * p.clen_stride] : 0) + p.clen_add;
+  return int(c < 0 ? 0 : c > p.cap ? p.cap : c);
 }
 
 // What an item covers.

@@ -12,6 +12,8 @@ import ctypes
 
 import torch
 
+from minitp_b200 import ops
+
 
 class KVCache:
     def __init__(
@@ -53,6 +55,14 @@ class KVCache:
 
     def advance(self, tokens: int) -> None:
         self.seq_len += tokens
+
+    def reorder_(self, parents: torch.Tensor, lengths=None) -> None:
+        """Row ``g * W + w`` becomes row ``g * W + parents[g, w]`` in every layer, in place (beam search).
+
+        ``parents``: int64 ``[G, W]`` with G * W rows in all. Copies the first ``lengths`` positions (an int,
+        or int32 ``[G * W]`` by source row; default: the fill cursor).
+        """
+        ops.reorder_cache_(self.k, self.v, parents, self.seq_len if lengths is None else lengths)
 
     def poison(self, value: float = float("nan")) -> None:
         for buf in (*self.k, *self.v):

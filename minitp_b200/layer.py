@@ -167,12 +167,18 @@ class TPQwen2ForCausalLM(nn.Module):
         kv_cache: KVCache | None = None,
         gather_logits: bool = False,
         last_only: bool = False,
+        prefix_cache: KVCache | None = None,
     ) -> torch.Tensor:
         """Logits ``[B, T, V_local]`` (``[B, 1, V_local]`` with ``last_only``).
 
         Reference: minitp/layer.py:91-124. ``last_only`` computes the LM head
         for the last token only (what greedy selection consumes); the other
         rows are not materialised.
+
+        ``prefix_cache`` (not in the reference): a filled cache of G rows that
+        the B rows share, B / G consecutive rows each. Row b then continues
+        prefix ``b // (B / G)``: it attends to that prefix and to its own
+        ``kv_cache``, and positions default to the places after both.
         """
         _lib.require_cuda(input_ids)
         b, t = input_ids.shape
@@ -184,6 +190,9 @@ class TPQwen2ForCausalLM(nn.Module):
                          self.model.embed_tokens.weight.dtype, input_ids.device)
         kv.check_room(t)
         rope_pos = None
+        if positions is None and prefix_cache is not None:
+            start = prefix_cache.seq_len + kv.seq_len
+            positions = torch.arange(start, start + t, device=input_ids.device)
         if positions is not None:
             rope_pos = positions.reshape(-1)
             if rope_pos.dtype != torch.int64:
@@ -198,12 +207,41 @@ class TPQwen2ForCausalLM(nn.Module):
         rows = b if last_only else b * t
         vloc = self.lm_head.vocab_end - self.lm_head.vocab_start
         logits = torch.empty(rows, vloc, dtype=self.model.embed_tokens.weight.dtype, device=input_ids.device)
-        kp, vp = kv.pointer_arrays()
-        _lib.call("mtpb_model_forward", h, ids.data_ptr(), b, t, _lib.ptr(rope_pos), kv.seq_len, kp, vp,
-                  kv.max_seq_len, logits.data_ptr(), 1 if last_only else 0, _lib.stream_ptr(input_ids.device))
+        if prefix_cache is not None:
+            self._forward_shared(ids, rope_pos, kv, kv.seq_len, prefix_cache, logits, last_only)
+        else:
+            kp, vp = kv.pointer_arrays()
+            _lib.call("mtpb_model_forward", h, ids.data_ptr(), b, t, _lib.ptr(rope_pos), kv.seq_len, kp, vp,
+                      kv.max_seq_len, logits.data_ptr(), 1 if last_only else 0, _lib.stream_ptr(input_ids.device))
         if kv_cache is not None:
             kv_cache.advance(t)
         out = logits.view(b, 1 if last_only else t, vloc)
         if gather_logits and self.ctx.tp_size > 1:
             return self.lm_head.gather(out)
         return out
+
+    def _forward_shared(self, ids: torch.Tensor, rope_pos: torch.Tensor, kv: KVCache, slot, prefix: KVCache,
+                       logits: torch.Tensor, last_only: bool = True) -> None:
+        """One forward of ``ids [N, T]`` behind ``prefix`` into ``logits`` (``mtpb_model_forward_shared``).
+
+        ``rope_pos`` int64 ``[T]``; ``slot``: the own-cache position of the first token, an int or (T = 1, for
+        a captured step) a device int32 ``[1]``. The caches' cursors are neither read nor moved, except the
+        prefix's, which is its length.
+        """
+        n, t = ids.shape
+        groups = prefix.k[0].shape[0]
+        if n % groups:
+            raise ValueError(f"{n} rows do not divide into {groups} shared prefixes")
+        if kv.k[0].shape[0] != n or len(prefix.k) != len(kv.k):
+            raise ValueError(f"the own cache holds {kv.k[0].shape[0]} rows of {len(kv.k)} layers, the prefix "
+                             f"{len(prefix.k)} layers; need {n} rows")
+        if prefix.k[0].shape[1:2] + prefix.k[0].shape[3:] != kv.k[0].shape[1:2] + kv.k[0].shape[3:] or \
+                prefix.k[0].dtype != kv.k[0].dtype or prefix.k[0].device != kv.k[0].device:
+            raise ValueError("prefix and own cache differ in heads, head_dim, dtype or device")
+        on_device = isinstance(slot, torch.Tensor)
+        kp, vp = kv.pointer_arrays()
+        pk, pv = prefix.pointer_arrays()
+        _lib.call("mtpb_model_forward_shared", self.native(), ids.data_ptr(), n, t, rope_pos.data_ptr(),
+                  slot.data_ptr() if on_device else None, 0 if on_device else slot, kp, vp, kv.max_seq_len, pk, pv,
+                  None, prefix.seq_len, groups, prefix.max_seq_len, logits.data_ptr(), 1 if last_only else 0,
+                  _lib.stream_ptr(ids.device))

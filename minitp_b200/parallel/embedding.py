@@ -12,7 +12,7 @@ import torch
 import torch.nn as nn
 
 from minitp_b200 import ops
-from minitp_b200.distributed import all_gather
+from minitp_b200.distributed import all_gather, all_gather_dim0
 from minitp_b200.distributed.context import ParallelContext
 from minitp_b200.parallel.linear import shard_range
 
@@ -108,3 +108,19 @@ class VocabParallelLMHead(nn.Module):
                 f"(vocab_size={self.vocab_size}); use the bitpack encoding"
             )
         return ops.argmax(local_logits, self.vocab_start, _comm(self.ctx))
+
+    @torch.no_grad()
+    def beam_select(self, local_logits: torch.Tensor, scores: torch.Tensor, k: int,
+                    finished: torch.Tensor | None = None, eos_token_id: int | None = None):
+        """The ``k`` best continuations per prompt over the sharded vocab (``ops.beam_select``), same on all ranks.
+
+        ``local_logits [G, W, V_local]``, ``scores`` fp32 ``[G, W]``. With tp > 1 every rank reduces its shard
+        to candidates, the ranks exchange those (not the logits) and each picks from all of them.
+        """
+        if self.ctx.tp_size == 1:
+            return ops.beam_select(local_logits, scores, k, finished, eos_token_id)
+        plan = self._max_local_vocab()
+        mine = ops.beam_candidates(local_logits, k, self.vocab_start, plan, finished)
+        blocks = torch.empty(self.ctx.tp_size, mine.numel(), dtype=mine.dtype, device=mine.device)
+        all_gather_dim0(blocks, mine, self.ctx.process_group)
+        return ops.beam_pick(blocks, scores, k, plan, finished, eos_token_id)

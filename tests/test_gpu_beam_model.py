@@ -1,0 +1,195 @@
+"""Beam search and decoding behind a shared prefix through the model, against plain CPU runs of the oracle model."""
+
+import math
+
+import pytest
+import torch
+
+from minitp_b200 import config as mcfg
+from oracle.model import OracleConfig, OracleModel, checkpoint_tensors
+
+pytestmark = pytest.mark.gpu
+
+_CACHE: dict = {}
+
+
+def _models(dtype=torch.float32):
+    if dtype not in _CACHE:
+        from minitp_b200.distributed.context import context_for
+        from minitp_b200.weight_loader import load_synthetic_tp
+
+        cfg = mcfg.baseline_tiny()
+        gpu = load_synthetic_tp(cfg, context_for(1, "cuda"), dtype=dtype, device=torch.device("cuda"))
+        _CACHE[dtype] = gpu, OracleModel(OracleConfig.of(cfg), checkpoint_tensors(cfg), tp=1), cfg
+    return _CACHE[dtype]
+
+
+def _log_probs(oracle, ids):
+    """fp64 log-softmax of the oracle's logits after each row of ids (the whole sequence is run anew)."""
+    oracle.reset(*ids.shape)
+    return torch.log_softmax(oracle.forward(ids, torch.arange(ids.shape[1]))[:, -1].double(), -1)
+
+
+def _plain_beam(oracle, ids, new, w, eos):
+    """Beam search by the definition, every hypothesis run from its first token."""
+    out = []
+    for row in ids:
+        hyps = [(0.0, row.tolist(), False)]
+        for _ in range(new):
+            cand = []
+            live = [h for h in hyps if not h[2]]
+            lp = _log_probs(oracle, torch.tensor([h[1] for h in live])) if live else None
+            at = 0
+            for b, (sc, seq, fin) in enumerate(hyps):
+                if fin:
+                    cand.append((sc, b, eos, seq))
+                    continue
+                top = lp[at].topk(w)
+                at += 1
+                cand += [(sc + float(v), b, int(t), seq) for v, t in zip(top.values, top.indices)]
+            cand.sort(key=lambda c: (-c[0], c[1], c[2]))
+            hyps = [(sc, seq + [t], t == eos) for sc, b, t, seq in cand[:w]]
+        out.append(hyps)
+    return out
+
+
+def _prompt(cfg, b, n, seed):
+    return torch.randint(0, cfg.vocab_size, (b, n), generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("b,p,new,w", [(1, 8, 12, 4), (3, 5, 6, 2), (2, 1, 5, 8), (1, 20, 1, 3), (1, 7, 9, 1)])
+def test_generate_beam_fp32(lib, b, p, new, w):
+    from minitp_b200.beam import generate_beam
+
+    gpu, oracle, cfg = _models()
+    ids = _prompt(cfg, b, p, b * 10 + p)
+    got, scores = generate_beam(gpu, ids.cuda(), new, w, num_return=w)
+    again, _ = generate_beam(gpu, ids.cuda(), new, w, num_return=w)  # the kept session's graph
+    assert torch.equal(got, again)
+    want = _plain_beam(oracle, ids, new, w, eos=-1)
+    for i in range(b):
+        assert got[i].tolist() == [h[1] for h in want[i]]
+        # fp32 logits within 1e-4 of the oracle's largest: every step's log-probability within twice that
+        assert scores[i].tolist() == pytest.approx([h[0] for h in want[i]], abs=2e-4 * new)
+    assert gpu.ctx.comm().status() == 0
+
+
+def test_generate_beam_end_token(lib):
+    from minitp_b200.beam import generate_beam
+
+    gpu, oracle, cfg = _models()
+    ids = _prompt(cfg, 2, 6, 5)
+    free, _ = generate_beam(gpu, ids.cuda(), 8, 4, num_return=4)
+    eos = int(free[0, 1, 6 + 3])  # a token that a good hypothesis emits on its way
+    got, scores = generate_beam(gpu, ids.cuda(), 8, 4, eos_token_id=eos, num_return=4, early_stop=False)
+    want = _plain_beam(oracle, ids, 8, 4, eos)
+    for i in range(2):
+        assert got[i].tolist() == [h[1] for h in want[i]]
+        assert scores[i].tolist() == pytest.approx([h[0] for h in want[i]], abs=2e-3)
+    norm, ns = generate_beam(gpu, ids.cuda(), 8, 4, eos_token_id=eos, num_return=4, length_penalty=1.0)
+    assert bool((ns[:, :-1] >= ns[:, 1:]).all())
+    for i in range(2):
+        length = [len(h[1]) - 6 if eos not in h[1][6:] else h[1][6:].index(eos) + 1 for h in want[i]]
+        assert ns[i].tolist() == pytest.approx(sorted((h[0] / n for h, n in zip(want[i], length)), reverse=True), abs=2e-3)
+
+
+def test_generate_beam_of_one_is_greedy(lib):
+    from minitp_b200.beam import generate_beam
+    from minitp_b200.generation import generate_greedy
+
+    gpu, _, cfg = _models()
+    ids = _prompt(cfg, 3, 9, 1).cuda()
+    got, scores = generate_beam(gpu, ids, 20, 1)
+    assert torch.equal(got[:, 0], generate_greedy(gpu, ids, 20, early_stop=False))
+    assert scores.shape == (3, 1) and bool((scores < 0).all())
+
+
+def test_generate_beam_stops_when_all_beams_ended(lib):
+    from minitp_b200.beam import generate_beam
+
+    gpu, _, cfg = _models()
+    ids = _prompt(cfg, 1, 6, 7).cuda()
+    free, _ = generate_beam(gpu, ids, 10, 1)
+    eos = int(free[0, 0, 8])
+    got, _ = generate_beam(gpu, ids, 10, 1, eos_token_id=eos)
+    end = free[0, 0, 6:].tolist().index(eos)
+    assert got.shape[2] == 6 + end + 1 and torch.equal(got[0, 0], free[0, 0, : 6 + end + 1])
+
+
+def test_more_beams_than_tokens(lib):
+    """A vocabulary smaller than the number of beams leaves places without a candidate in the first step."""
+    from minitp_b200 import ops
+
+    x = torch.randn(1, 1, 5, generator=torch.Generator().manual_seed(0))
+    out, par, tok, _ = ops.beam_select(x.cuda(), torch.zeros(1, 1).cuda(), 8)
+    assert torch.isinf(out[0, 5:]).all() and sorted(tok[0, :5].tolist()) == [0, 1, 2, 3, 4]
+    # and the next step goes on from the five in use
+    y = torch.randn(1, 8, 5, generator=torch.Generator().manual_seed(1))
+    nxt = ops.beam_select(y.cuda(), out, 8)
+    assert torch.isfinite(nxt[0]).all() and int(nxt[1].max()) < 5
+
+
+@pytest.mark.parametrize("g,n,p,t,new", [(1, 3, 10, 4, 8), (2, 4, 33, 1, 5), (1, 9, 70, 20, 6)])
+def test_generate_shared_prefix_equals_whole_prompts(lib, g, n, p, t, new):
+    """fp32: the tokens of the same prompts run whole by the oracle."""
+    from minitp_b200.beam import generate_shared_prefix
+
+    gpu, oracle, cfg = _models()
+    pre, ids = _prompt(cfg, g, p, 3), _prompt(cfg, n, t, 4)
+    whole = torch.cat([pre.repeat_interleave(n // g, 0), ids], 1)
+    want = oracle.generate(whole, new)[:, p:]
+    for _ in range(2):
+        got = generate_shared_prefix(gpu, pre.cuda(), ids.cuda(), new)
+        assert torch.equal(got.cpu(), want)
+    eos = int(want[0, t + 2])
+    stop = generate_shared_prefix(gpu, pre.cuda(), ids.cuda(), new, eos_token_id=eos)
+    for i in range(n):
+        row, ref = stop[i, t:].tolist(), want[i, t:].tolist()
+        end = ref.index(eos) + 1 if eos in ref else len(ref)
+        assert row[:end] == ref[: len(row)][:end] and all(x == eos for x in row[end:])
+    assert gpu.ctx.comm().status() == 0
+
+
+def test_forward_behind_a_prefix_poisoned_caches(lib):
+    """Chunked forwards behind a prefix, with NaN in every slot that holds no token."""
+    from minitp_b200.generation import make_kv_cache
+
+    gpu, oracle, cfg = _models()
+    pre, ids = _prompt(cfg, 2, 37, 1), _prompt(cfg, 4, 11, 2)
+    prefix, own = make_kv_cache(gpu, 2, 50), make_kv_cache(gpu, 4, 16)
+    prefix.poison()
+    own.poison()
+    gpu(pre.cuda(), kv_cache=prefix)
+    a = gpu(ids[:, :6].cuda(), kv_cache=own, prefix_cache=prefix)
+    b = gpu(ids[:, 6:7].cuda(), kv_cache=own, prefix_cache=prefix)
+    c = gpu(ids[:, 7:].cuda(), kv_cache=own, prefix_cache=prefix)
+    got = torch.cat([a, b, c], 1).cpu()
+    whole = torch.cat([pre.repeat_interleave(2, 0), ids], 1)
+    full = gpu(whole.cuda()).cpu()[:, 37:]
+    err = float((got - full).abs().max() / full.abs().max())
+    assert err <= 1e-4 and math.isfinite(err)  # the framework's fp32 logit tolerance
+    assert own.seq_len == 11
+
+
+def test_forward_refuses_caches_that_do_not_fit(lib):
+    from minitp_b200.beam import generate_beam, generate_shared_prefix
+    from minitp_b200.generation import make_kv_cache
+
+    gpu, _, cfg = _models()
+    ids = _prompt(cfg, 3, 2, 1).cuda()
+    prefix = make_kv_cache(gpu, 2, 8)
+    gpu(ids[:2], kv_cache=prefix)
+    with pytest.raises(ValueError, match="divide"):
+        gpu(ids, kv_cache=make_kv_cache(gpu, 3, 8), prefix_cache=prefix)
+    with pytest.raises(ValueError, match="rows"):
+        gpu(ids[:2], kv_cache=make_kv_cache(gpu, 4, 8), prefix_cache=prefix)
+    with pytest.raises(ValueError, match="overflow"):
+        gpu(ids[:2], kv_cache=make_kv_cache(gpu, 2, 1), prefix_cache=prefix)
+    for bad in (dict(num_beams=0), dict(num_beams=65), dict(num_beams=2, num_return=3),
+                dict(num_beams=2, eos_token_id=cfg.vocab_size)):
+        with pytest.raises(ValueError):
+            generate_beam(gpu, ids, 4, **bad)
+    with pytest.raises(ValueError, match="max_new_tokens"):
+        generate_beam(gpu, ids, 0, 2)
+    with pytest.raises(ValueError, match="divide"):
+        generate_shared_prefix(gpu, ids[:2], ids, 4)
