@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <cstdlib>
 
 #include "beam.cuh"
 #include "host_util.cuh"
@@ -204,7 +205,10 @@ int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers, 
 namespace {
 
 struct SaPlan {
-  int rpt;  // rows a tile / 16
+  bool token;       // one token a row on sa_token_kernel
+  bool inline_pre;  // it reads the prefix too: no other launch
+  int warps;
+  int rpt;  // CUDA-core items: rows a tile / 16
   int sp, so, ptiles, otiles;
   long long pitems, items;
   size_t rows, ml_bytes, o_bytes;
@@ -222,39 +226,75 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   if (!dtype_ok(a.dtype)) return bad("unsupported dtype");
   const double rows = double(a.G) * a.W * a.T * a.hq;
   if (rows > double(1 << 28)) return bad("shared_attention: more than 2^28 (token, head) rows");
-  SaPlan pl;
+  SaPlan pl = {};
   const int per = a.hq / a.hkv;
-  const long long prow = (long long)a.W * a.T * per, orow = (long long)a.T * per;
-  pl.rpt = orow >= 64 ? 4 : 1;
-  const int tile = 16 * pl.rpt;
-  pl.ptiles = int((prow + tile - 1) / tile);
-  pl.otiles = int((orow + tile - 1) / tile);
-  const long long pbase = (long long)a.G * a.hkv * pl.ptiles, obase = (long long)a.G * a.W * a.hkv * pl.otiles;
   const int top_p = a.prefix_lens ? a.cap_p : a.prefix_len, top_o = a.cache_lens ? a.cap : a.cache_len;
-  const long long want = 4ll * 148;
+  const long long N = (long long)a.G * a.W;
+  pl.token = a.dtype == MTPB_BF16 && a.T == 1 && (a.hd == 64 || a.hd == 128) && N <= 65535;
+  const int sms = host_sms();
+  const long long want = 4ll * sms;
   auto splits = [&](long long base, int top) {
     const long long most = std::max(1, (top + 2 * kSaKT - 1) / (2 * kSaKT));
     return int(std::max<long long>(1, std::min<long long>(std::min<long long>(most, 64), (want + base - 1) / base)));
   };
-  pl.sp = splits(pbase, top_p);
-  pl.so = splits(obase, top_o);
+  const long long prow = (long long)a.W * a.T * per, orow = (long long)a.T * per;
+  pl.rpt = orow >= 64 ? 4 : 1;
+  const int tile = 16 * pl.rpt;
+  pl.ptiles = int((prow + tile - 1) / tile);
+  const long long pbase = (long long)a.G * a.hkv * pl.ptiles;
+  if (pl.token) {
+    pl.otiles = (per + 15) / 16;
+    const long long ctas = N * a.hkv * pl.otiles;
+    static const long long lim = getenv("SA_INLINE") ? atoll(getenv("SA_INLINE")) : 2048;
+    pl.inline_pre = top_p <= lim;
+    pl.warps = 4;
+    if (getenv("SA_WARPS")) pl.warps = atoi(getenv("SA_WARPS"));
+    pl.so = 1;
+    if (!pl.inline_pre)
+      while (ctas * pl.so * 2 <= 2 * sms && top_o / (pl.so * 2) >= 256 && pl.so < 64) pl.so *= 2;
+  } else {
+    pl.otiles = int((orow + tile - 1) / tile);
+    pl.so = splits(N * a.hkv * pl.otiles, top_o);
+  }
+  pl.sp = pl.inline_pre ? 0 : splits(pbase, top_p);
   pl.pitems = pbase * pl.sp;
-  pl.items = pl.pitems + obase * pl.so;
+  pl.items = pl.pitems + (pl.token ? 0 : N * a.hkv * pl.otiles * pl.so);
   if (pl.items > 0x7FFFFFFFll) return bad("shared_attention: too many rows");
   pl.rows = size_t(rows);
-  pl.ml_bytes = (pl.rows * (pl.sp + pl.so) * 8 + 255) / 256 * 256;
-  pl.o_bytes = pl.rows * (pl.sp + pl.so) * a.hd * 4;
+  const int slots = pl.sp + (pl.token && pl.so == 1 ? 0 : pl.so);
+  pl.ml_bytes = (pl.rows * slots * 8 + 255) / 256 * 256;
+  pl.o_bytes = pl.rows * slots * a.hd * 4;
   *out = pl;
   return MTPB_OK;
 }
 
+template <int HD, int NW>
+int sa_launch_token(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
+  const dim3 grid(unsigned(p.hkv * pl.otiles), unsigned(p.G * p.W), unsigned(pl.so));
+  const bool wide = p.hq / p.hkv > 8;
+  return wide ? host_launch(sa_token_kernel<HD, NW, true>, grid, dim3(32 * NW), sa_token_smem<HD, NW, true>(), st, p,
+                            int(pl.inline_pre))
+              : host_launch(sa_token_kernel<HD, NW, false>, grid, dim3(32 * NW), sa_token_smem<HD, NW, false>(), st, p,
+                            int(pl.inline_pre));
+}
+
 template <typename T, int HD>
 int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
-  const int r = pl.rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)pl.items), dim3(kSaThreads),
-                                          sa_simt_smem<HD, 4>(), st, p)
-                            : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)pl.items), dim3(kSaThreads),
-                                          sa_simt_smem<HD, 1>(), st, p);
-  if (r != MTPB_OK) return r;
+  if (pl.items > 0) {
+    const int r = pl.rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)pl.items), dim3(kSaThreads),
+                                            sa_simt_smem<HD, 4>(), st, p)
+                              : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)pl.items), dim3(kSaThreads),
+                                            sa_simt_smem<HD, 1>(), st, p);
+    if (r != MTPB_OK) return r;
+  }
+  if constexpr (sizeof(T) == 2 && HD >= 64) {
+    if (pl.token) {
+      const int r = pl.warps == 4   ? sa_launch_token<HD, 4>(pl, p, st)
+                    : pl.warps == 8 ? sa_launch_token<HD, 8>(pl, p, st)
+                                    : sa_launch_token<HD, 16>(pl, p, st);
+      if (r != MTPB_OK || pl.so == 1) return r;
+    }
+  }
   const size_t n = pl.rows * (HD / 4);
   return host_launch(sa_join_kernel<T, HD>, dim3(unsigned((n + kSaJoinThreads - 1) / kSaJoinThreads)),
                      dim3(kSaJoinThreads), 0, st, p);
@@ -284,7 +324,8 @@ int shared_attn_run(const SharedAttnArgs& a, void* ws, size_t ws_bytes, cudaStre
   SaPlan pl;
   const int r = sa_plan(a, &pl);
   if (r != MTPB_OK) return r;
-  if (!a.q || !a.k_prefix || !a.v_prefix || !a.k_cache || !a.v_cache || !a.out || !ws)
+  if (!a.q || !a.k_prefix || !a.v_prefix || !a.k_cache || !a.v_cache || !a.out ||
+      (!ws && pl.ml_bytes + pl.o_bytes > 0))
     return bad("shared_attention: null tensor");
   if (!al16(a.q) || !al16(a.k_prefix) || !al16(a.v_prefix) || !al16(a.k_cache) || !al16(a.v_cache) || !al16(a.out) ||
       !al16(ws))

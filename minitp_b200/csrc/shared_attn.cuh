@@ -151,8 +151,8 @@ __global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
   float* ks = qs + size_t(R) * QS;
   float* vs = ks + size_t(kSaKT) * QS;
   float* ps = vs + size_t(kSaKT) * QS;
-  pdl_launch();
   pdl_wait();
+  pdl_launch();  // after the wait: sa_token_kernel counts on it
   const int tid = threadIdx.x, rg = tid >> 4, sub = tid & 15;
   const SaItem s = sa_item<HD, int(sizeof(T))>(p, blockIdx.x, R, kSaKT);
   const size_t nrow = size_t(p.G) * p.W * p.T * p.hq;
@@ -270,6 +270,246 @@ __global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
     if (s.j0 < s.j1)
 #pragma unroll
       for (int d = 0; d < DPT; ++d) p.part_o[at * HD + sub * DPT + d] = o[i][d];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// One token a row, bf16, head dim 64 or 128: a CTA takes up to 16 query heads
+// of one (row, KV head) and streams the row's own cache (and, inline, the
+// prefix) from global memory straight into mma.sync fragments: 16 rows (heads)
+// x 16 keys a warp and step, the warps on every NW-th block of 16 keys. A
+// K or V byte is used once, so the kernel is bound by the loads, and the
+// 16-row tensor instructions cost less than unpacking to fp32 would.
+//
+// Fragments without shared memory: the dot product's order of dims and the
+// output's order of dims are free, so both are chosen to make every load 16
+// bytes. Thread (g = lane / 4, c = lane % 4) loads dims 32 j + 8 c .. + 7 of
+// key g (K) or head g (Q): four register pairs that serve as the "k" and
+// "k + 8" halves of two steps. For V it loads keys 2c, 2c+1, 2c+8, 2c+9 at
+// dims 64 b + 8 g .. + 7; two keys' values of a dim, put together by a byte
+// permute, are the operand of column g of output tile i = dim % 8.
+//
+// Probabilities are rounded to bf16 for the second product (the sums of the
+// denominator are not): half a step of bf16 of each term, as the result's own
+// rounding.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// NW warps; WIDE: more than 8 heads a tile (rows 8..15 in use).
+template <int HD, int NW, bool WIDE>
+__host__ __device__ constexpr size_t sa_token_smem() {
+  return size_t(NW) * (WIDE ? 16 : 8) * (HD + 2) * sizeof(float);
+}
+
+template <int HD, int NW, bool WIDE>
+__global__ void __launch_bounds__(32 * NW) sa_token_kernel(const SaParams p, const int inline_prefix) {  // inline_prefix: so == 1, no prefix items
+  constexpr int R = WIDE ? 16 : 8;
+  constexpr int JB = HD / 32, VB = HD / 64;
+  extern __shared__ __align__(16) float smf[];
+  float* so = smf;                  // [NW][R][HD]
+  float* sml = so + NW * R * HD;    // [NW][R][2]
+  // the kernel of the prefix items, if one runs before this, has waited for
+  // the kernels before it: only its partial sums are not yet there
+  pdl_launch();
+  if (inline_prefix) pdl_wait();
+  const int per = p.hq / p.hkv;
+  const int tile = blockIdx.x % p.otiles, kvh = blockIdx.x / p.otiles;
+  const int n = blockIdx.y, split = blockIdx.z;
+  const int rows = min(16, per - tile * 16);
+  const int head0 = kvh * per + tile * 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int gi = n / p.W;
+  const size_t po = (size_t(gi) * p.hkv + kvh) * p.cap_p * HD, co = (size_t(n) * p.hkv + kvh) * p.cap * HD;
+  const int plen = inline_prefix ? sa_prefix_len(p, gi) : 0;
+  const int clen = sa_cache_len(p, n);
+  const int chunk = ((clen + p.so - 1) / p.so + 15) / 16 * 16;
+  const int own0 = min(clen, split * chunk), own1 = min(clen, own0 + chunk);
+  uint4 q0[JB], q1[JB];
+  {
+    const bf16* qp = static_cast<const bf16*>(p.q) + (size_t(n) * p.hq + head0) * HD + c * 8;
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+      q0[j] = g < rows ? ld_vec(qp + size_t(g) * HD + 32 * j) : make_uint4(0, 0, 0, 0);
+      q1[j] = WIDE && g + 8 < rows ? ld_vec(qp + size_t(g + 8) * HD + 32 * j) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  const float sl2 = p.scale * kLog2e;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // max (scaled, base 2) and this thread's part of the sum
+  float o[VB * 8][4];
+#pragma unroll
+  for (int i = 0; i < VB * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  const int nb0 = (plen + 15) / 16, nb = nb0 + (own1 - own0 + 15) / 16;
+  for (int b = warp; b < nb; b += NW) {
+    const bool own = b >= nb0;
+    const int key0 = own ? own0 + (b - nb0) * 16 : b * 16, end = own ? own1 : plen;
+    uint4 kf[2][JB], vf[4][VB];
+    const size_t at = (own ? co : po) + size_t(key0) * HD;
+    const bf16* kp = static_cast<const bf16*>(own ? p.kc : p.kp) + at + c * 8;
+    const bf16* vp = static_cast<const bf16*>(own ? p.vc : p.vp) + at + g * 8;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < JB; ++j)
+        kf[t][j] = key0 + 8 * t + g < end ? ld_stream(kp + size_t(8 * t + g) * HD + 32 * j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 2 * c + (r & 1) + (r >> 1) * 8;
+#pragma unroll
+      for (int v = 0; v < VB; ++v)
+        vf[r][v] = key0 + k < end ? ld_stream(vp + size_t(k) * HD + 64 * v) : make_uint4(0, 0, 0, 0);
+    }
+    float s[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < JB; ++j) {
+        mma_bf16(s[t], q0[j].x, q1[j].x, q0[j].y, q1[j].y, kf[t][j].x, kf[t][j].y);
+        mma_bf16(s[t], q0[j].z, q1[j].z, q0[j].w, q1[j].w, kf[t][j].z, kf[t][j].w);
+      }
+    }
+    float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool in = key0 + 8 * t + 2 * c + e < end;
+        s[t][e] = in ? s[t][e] * sl2 : -INFINITY;
+        x0 = fmaxf(x0, s[t][e]);
+        if (WIDE) {
+          s[t][2 + e] = in ? s[t][2 + e] * sl2 : -INFINITY;
+          x1 = fmaxf(x1, s[t][2 + e]);
+        }
+      }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+      if (WIDE) x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+    }
+    // the block's first key is inside the range: the new maxima are not -inf
+    // (but for a key whose score is: then the row keeps exp(-inf - 0) = 0)
+    if (__any_sync(0xffffffffu, x0 > m0 || (WIDE && x1 > m1))) {
+      const float n0 = fmaxf(m0, x0), a0 = exp2_approx(m0 - (n0 == -INFINITY ? 0.f : n0));
+      const float n1 = fmaxf(m1, x1), a1 = WIDE ? exp2_approx(m1 - (n1 == -INFINITY ? 0.f : n1)) : 1.f;
+      m0 = n0;
+      l0 *= a0;
+      m1 = n1;
+      l1 *= a1;
+#pragma unroll
+      for (int i = 0; i < VB * 8; ++i) {
+        o[i][0] *= a0;
+        o[i][1] *= a0;
+        if (WIDE) {
+          o[i][2] *= a1;
+          o[i][3] *= a1;
+        }
+      }
+    }
+    const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+    uint32_t pa[2][2];  // [key half][row half]
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float e0 = exp2_approx(s[t][0] - r0), e1 = exp2_approx(s[t][1] - r0);
+      l0 += e0 + e1;
+      pa[t][0] = pack_bf16(e0, e1);
+      pa[t][1] = 0;
+      if (WIDE) {
+        const float e2 = exp2_approx(s[t][2] - r1), e3 = exp2_approx(s[t][3] - r1);
+        l1 += e2 + e3;
+        pa[t][1] = pack_bf16(e2, e3);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VB; ++v) {
+      const uint32_t* k0 = reinterpret_cast<const uint32_t*>(&vf[0][v]);
+      const uint32_t* k1 = reinterpret_cast<const uint32_t*>(&vf[1][v]);
+      const uint32_t* k8 = reinterpret_cast<const uint32_t*>(&vf[2][v]);
+      const uint32_t* k9 = reinterpret_cast<const uint32_t*>(&vf[3][v]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;  // upper or lower halves of two words
+        mma_bf16(o[v * 8 + i], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(k0[i / 2], k1[i / 2], sel),
+                 __byte_perm(k8[i / 2], k9[i / 2], sel));
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+    if (WIDE) l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+  }
+  if (c == 0) {
+    *reinterpret_cast<float2*>(sml + (warp * R + g) * 2) = make_float2(m0 * kLn2, l0);
+    if (WIDE) *reinterpret_cast<float2*>(sml + (warp * R + g + 8) * 2) = make_float2(m1 * kLn2, l1);
+  }
+#pragma unroll
+  for (int v = 0; v < VB; ++v)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int d = 64 * v + 8 * (2 * c + e) + i;
+        so[(warp * R + g) * HD + d] = o[v * 8 + i][e];
+        if (WIDE) so[(warp * R + g + 8) * HD + d] = o[v * 8 + i][2 + e];
+      }
+  __syncthreads();
+  if (!inline_prefix) pdl_wait();  // the prefix items' partial sums
+  const bool last = p.so == 1;  // else a slot for the join
+  const size_t nrow = size_t(p.G) * p.W * p.hq;
+  for (int i = threadIdx.x; i < rows * (HD / 4); i += 32 * NW) {
+    const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+    const size_t row = size_t(n) * p.hq + head0 + r;
+    float mx = -INFINITY;
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sml[(w * R + r) * 2]);
+    if (last && !inline_prefix)
+      for (int s = 0; s < p.sp; ++s) mx = fmaxf(mx, __ldcg(p.part_ml + (s * nrow + row) * 2));
+    float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+    auto add = [&](float m, float l, const float4& f) {
+      const float w = expf(m - mx);
+      den = fmaf(w, l, den);
+      num[0] = fmaf(w, f.x, num[0]);
+      num[1] = fmaf(w, f.y, num[1]);
+      num[2] = fmaf(w, f.z, num[2]);
+      num[3] = fmaf(w, f.w, num[3]);
+    };
+    for (int w = 0; w < NW; ++w) {
+      const float m = sml[(w * R + r) * 2];
+      if (m != -INFINITY) add(m, sml[(w * R + r) * 2 + 1], *reinterpret_cast<const float4*>(so + (w * R + r) * HD + d));
+    }
+    if (last && !inline_prefix)
+      for (int s = 0; s < p.sp; ++s) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (s * nrow + row) * 2));
+        if (ml.x != -INFINITY) add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * nrow + row) * HD + d)));
+      }
+    if (last) {
+      const float inv = den > 0.f ? 1.f / den : 0.f;
+      *reinterpret_cast<uint2*>(static_cast<bf16*>(p.out) + row * HD + d) =
+          make_uint2(pack_bf16(num[0] * inv, num[1] * inv), pack_bf16(num[2] * inv, num[3] * inv));
+    } else {
+      const size_t at = size_t(p.sp + split) * nrow + row;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mx, den);
+      *reinterpret_cast<float4*>(p.part_o + at * HD + d) = make_float4(num[0], num[1], num[2], num[3]);
+    }
   }
 }
 

@@ -54,11 +54,11 @@ def test_reorder_refusals(lib):
 
 
 def test_attention_refusals(lib):
-    ok = dict(q=P, kp=P, vp=P, pl=None, plen=5, kc=P, vc=P, cl=None, clen=5, out=P, G=2, W=4, T=1, hq=14, hkv=2, hd=64,
-              cap_p=8, cap=8, dtype=_lib.MTPB_BF16, ws=P, n=1 << 30, st=None)
+    ok = dict(q=P, kp=P, vp=P, pl=None, plen=1 << 20, kc=P, vc=P, cl=None, clen=5, out=P, G=2, W=4, T=1, hq=14, hkv=2, hd=64,
+              cap_p=1 << 20, cap=8, dtype=_lib.MTPB_BF16, ws=P, n=1 << 30, st=None)
     for change, match in [(dict(q=None), "null"), (dict(ws=None), "null"), (dict(n=16), "workspace"),
                           (dict(hd=80), "head_dim"), (dict(hkv=4), "multiple"), (dict(T=0), "positive"),
-                          (dict(cap=0), "positive"), (dict(plen=9), "prefix length"), (dict(plen=-1), "prefix length"),
+                          (dict(cap=0), "positive"), (dict(plen=(1 << 20) + 1), "prefix length"), (dict(plen=-1), "prefix length"),
                           (dict(clen=9), "length outside"), (dict(kp=P + 2), "aligned"), (dict(dtype=9), "dtype"),
                           (dict(G=1 << 20, W=1 << 10), "rows")]:
         _refused(lib, "mtpb_shared_attention", list((ok | change).values()), match)
