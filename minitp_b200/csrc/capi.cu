@@ -812,6 +812,7 @@ SharedAttnArgs shared_args(const ModelHost& mh, const FwdArgs& a, int l, int tc,
   s.cap_p = sp.cap;
   s.cap = a.cap;
   s.dtype = d.dtype;
+  s.status = mh.comm->dev.status();
   return s;
 }
 
@@ -1301,6 +1302,7 @@ int host_fail_cuda(cudaError_t e, const char* what) noexcept {
   return host_fail(MTPB_ERR_CUDA, text);
 }
 bool host_pdl() noexcept { return g_pdl; }
+void* host_tensor_map_encoder() noexcept { return reinterpret_cast<void*>(tensor_map_encoder()); }
 
 }  // namespace mtpb
 

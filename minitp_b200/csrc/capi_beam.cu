@@ -3,11 +3,12 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <cstdlib>
 
 #include "beam.cuh"
 #include "host_util.cuh"
 #include "shared_attn.cuh"
+
+#include <cudaTypedefs.h>
 
 using namespace mtpb;
 
@@ -207,6 +208,7 @@ namespace {
 struct SaPlan {
   bool token;       // one token a row on sa_token_kernel
   bool inline_pre;  // it reads the prefix too: no other launch
+  bool tc;          // the other items on sa_tc_kernel, else on the CUDA cores
   int warps;
   int rpt;  // CUDA-core items: rows a tile / 16
   int sp, so, ptiles, otiles;
@@ -214,9 +216,24 @@ struct SaPlan {
   size_t rows, ml_bytes, o_bytes;
 };
 
-// Row tiles of 64 when a group (or a row of many tokens) fills them, else of
-// 16; key ranges until the items give every SM four, but no range below two
-// key tiles.
+// Key ranges for `base` tensor-core items of up to `top` keys: the number that
+// makes waves x (key tiles a range + a start-up of about four) smallest, with
+// the partial sums' traffic (written and read again) beside it.
+int sa_tc_splits(long long base, int top, size_t rows, int hd, int sms) {
+  const int tiles = std::max(1, (top + kSaTcKeys - 1) / kSaTcKeys);
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= std::min(tiles, 64); ++s) {
+    const double waves = double((base * s + sms - 1) / sms);
+    const double us = waves * (0.7 * ((tiles + s - 1) / s) + 2.8) + double(rows) * s * hd * 8 / 4e6;
+    if (s == 1 || us < least) {
+      best = s;
+      least = us;
+    }
+  }
+  return best;
+}
+
 int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   if (a.G < 1 || a.W < 1 || a.T < 1 || a.hq < 1 || a.hkv < 1 || a.cap_p < 1 || a.cap < 1)
     return bad("shared_attention: sizes must be positive");
@@ -227,45 +244,74 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   const double rows = double(a.G) * a.W * a.T * a.hq;
   if (rows > double(1 << 28)) return bad("shared_attention: more than 2^28 (token, head) rows");
   SaPlan pl = {};
+  pl.rows = size_t(rows);
   const int per = a.hq / a.hkv;
   const int top_p = a.prefix_lens ? a.cap_p : a.prefix_len, top_o = a.cache_lens ? a.cap : a.cache_len;
   const long long N = (long long)a.G * a.W;
-  pl.token = a.dtype == MTPB_BF16 && a.T == 1 && (a.hd == 64 || a.hd == 128) && N <= 65535;
   const int sms = host_sms();
-  const long long want = 4ll * sms;
+  pl.tc = a.dtype == MTPB_BF16 && (a.hd == 64 || a.hd == 128);
+  pl.token = pl.tc && a.T == 1 && N <= 65535;
+  const long long prow = (long long)a.W * a.T * per, orow = (long long)a.T * per;
+  // CUDA-core items: row tiles of 64 when a row's tokens fill them, else of 16
+  pl.rpt = orow >= 64 ? 4 : 1;
+  const int tile = pl.tc ? kSaTcRows : 16 * pl.rpt;
+  pl.ptiles = int((prow + tile - 1) / tile);
+  pl.otiles = pl.token ? (per + 15) / 16 : int((orow + tile - 1) / tile);
+  const long long pbase = (long long)a.G * a.hkv * pl.ptiles, obase = N * a.hkv * pl.otiles;
+  // key ranges until the items give every SM four, but none below two key tiles
   auto splits = [&](long long base, int top) {
-    const long long most = std::max(1, (top + 2 * kSaKT - 1) / (2 * kSaKT));
+    const long long most = std::max(1, (top + 2 * kSaKT - 1) / (2 * kSaKT)), want = 4ll * sms;
     return int(std::max<long long>(1, std::min<long long>(std::min<long long>(most, 64), (want + base - 1) / base)));
   };
-  const long long prow = (long long)a.W * a.T * per, orow = (long long)a.T * per;
-  pl.rpt = orow >= 64 ? 4 : 1;
-  const int tile = 16 * pl.rpt;
-  pl.ptiles = int((prow + tile - 1) / tile);
-  const long long pbase = (long long)a.G * a.hkv * pl.ptiles;
   if (pl.token) {
-    pl.otiles = (per + 15) / 16;
-    const long long ctas = N * a.hkv * pl.otiles;
-    static const long long lim = getenv("SA_INLINE") ? atoll(getenv("SA_INLINE")) : 2048;
-    pl.inline_pre = top_p <= lim;
+    // the prefix read by every row's CTA: one launch, but N / G reads of each
+    // position, through L2, and one CTA's pace along it
+    const long long pre = (long long)top_p * a.hd * 4;
+    pl.inline_pre = pre <= (256 << 10) && obase * pre <= (32ll << 20);
     pl.warps = 4;
-    if (getenv("SA_WARPS")) pl.warps = atoi(getenv("SA_WARPS"));
     pl.so = 1;
     if (!pl.inline_pre)
-      while (ctas * pl.so * 2 <= 2 * sms && top_o / (pl.so * 2) >= 256 && pl.so < 64) pl.so *= 2;
+      while (obase * pl.so * 2 <= 2 * sms && top_o / (pl.so * 2) >= 256 && pl.so < 64) pl.so *= 2;
   } else {
-    pl.otiles = int((orow + tile - 1) / tile);
-    pl.so = splits(N * a.hkv * pl.otiles, top_o);
+    pl.so = pl.tc ? sa_tc_splits(obase, top_o, pl.rows, a.hd, sms) : splits(obase, top_o);
   }
-  pl.sp = pl.inline_pre ? 0 : splits(pbase, top_p);
+  pl.sp = pl.inline_pre ? 0 : pl.tc ? sa_tc_splits(pbase, top_p, pl.rows, a.hd, sms) : splits(pbase, top_p);
   pl.pitems = pbase * pl.sp;
-  pl.items = pl.pitems + (pl.token ? 0 : N * a.hkv * pl.otiles * pl.so);
+  pl.items = pl.pitems + (pl.token ? 0 : obase * pl.so);
   if (pl.items > 0x7FFFFFFFll) return bad("shared_attention: too many rows");
-  pl.rows = size_t(rows);
   const int slots = pl.sp + (pl.token && pl.so == 1 ? 0 : pl.so);
   pl.ml_bytes = (pl.rows * slots * 8 + 255) / 256 * 256;
   pl.o_bytes = pl.rows * slots * a.hd * 4;
   *out = pl;
   return MTPB_OK;
+}
+
+// Map of caches [planes][cap][hd] bf16, boxes of 128 positions x 64 dims with
+// the 128-byte swizzle; positions from cap on read as zeros.
+int sa_map(CUtensorMap* map, const void* ptr, long long planes, int cap, int hd) {
+  const auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(host_tensor_map_encoder());
+  if (!enc) return host_fail(MTPB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  if (planes > 0x7FFFFFFFll) return bad("shared_attention: too many rows");
+  const cuuint64_t dims[3] = {cuuint64_t(hd), cuuint64_t(cap), cuuint64_t(planes)};
+  const cuuint64_t strides[2] = {cuuint64_t(hd) * 2, cuuint64_t(cap) * hd * 2};
+  const cuuint32_t box[3] = {64, kSaTcKeys, 1}, one[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MTPB_OK : host_fail(MTPB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+}
+
+template <int HD>
+int sa_launch_tc(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
+  CUtensorMap m[4];
+  const long long N = (long long)p.G * p.W;
+  int r = sa_map(m, p.kp, (long long)p.G * p.hkv, p.cap_p, HD);
+  if (r == MTPB_OK) r = sa_map(m + 1, p.vp, (long long)p.G * p.hkv, p.cap_p, HD);
+  if (r == MTPB_OK) r = sa_map(m + 2, p.kc, N * p.hkv, p.cap, HD);
+  if (r == MTPB_OK) r = sa_map(m + 3, p.vc, N * p.hkv, p.cap, HD);
+  if (r != MTPB_OK) return r;
+  return host_launch(sa_tc_kernel<HD>, dim3((unsigned)pl.items), dim3(kSaTcThreads), SaTcCfg<HD>::kSmem, st, p, m[0],
+                     m[1], m[2], m[3]);
 }
 
 template <int HD, int NW>
@@ -280,7 +326,15 @@ int sa_launch_token(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
 
 template <typename T, int HD>
 int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
-  if (pl.items > 0) {
+  bool done = pl.items == 0;
+  if constexpr (sizeof(T) == 2 && HD >= 64) {
+    if (!done && pl.tc) {
+      const int r = sa_launch_tc<HD>(pl, p, st);
+      if (r != MTPB_OK) return r;
+      done = true;
+    }
+  }
+  if (!done) {
     const int r = pl.rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)pl.items), dim3(kSaThreads),
                                             sa_simt_smem<HD, 4>(), st, p)
                               : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)pl.items), dim3(kSaThreads),
@@ -364,6 +418,7 @@ int shared_attn_run(const SharedAttnArgs& a, void* ws, size_t ws_bytes, cudaStre
   p.items = int(pl.items);
   p.part_ml = static_cast<float*>(ws);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.ml_bytes);
+  p.status = a.status;
   return a.dtype == MTPB_BF16 ? sa_launch_hd<bf16>(pl, p, a.hd, st) : sa_launch_hd<float>(pl, p, a.hd, st);
 }
 

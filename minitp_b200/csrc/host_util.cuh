@@ -16,6 +16,9 @@ int host_fail_cuda(cudaError_t e, const char* what) noexcept;
 // Whether later launches use programmatic dependent launch (mtpb_set_pdl).
 bool host_pdl() noexcept;
 
+// cuTensorMapEncodeTiled (a PFN_cuTensorMapEncodeTiled_v12000), or NULL.
+void* host_tensor_map_encoder() noexcept;
+
 // Multiprocessors of the current device (a constant of the device, asked once).
 inline int host_sms() {
   static int per_dev[64] = {};
@@ -63,6 +66,7 @@ struct SharedAttnArgs {
   void* out;                            // [N*T][hq*hd]
   int G, W, T, hq, hkv, hd, cap_p, cap; // N = G * W
   int dtype;
+  uint32_t* status = nullptr;           // word for error bits, or NULL: the library's own
 };
 // Workspace bytes of a call (no device access; < 0: an MTPB_ERR_* code).
 long long shared_attn_workspace(const SharedAttnArgs& a);

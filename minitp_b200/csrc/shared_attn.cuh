@@ -12,7 +12,7 @@
 // denominator (a slot per key range), and a second kernel joins the slots.
 #pragma once
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace mtpb {
 
@@ -32,7 +32,11 @@ struct SaParams {
   int pitems, items;   // prefix items, all items
   float* part_o;     // [slot][row = (n * T + t) * hq + h][hd]
   float* part_ml;    // [slot][row][2]: max (base e, scaled), sum
+  uint32_t* status;  // of a communicator, or NULL: g_sa_status
 };
+
+// Error bits of calls without a communicator's status word.
+__device__ uint32_t g_sa_status;
 
 __device__ __forceinline__ int sa_prefix_len(const SaParams& p, int g) {
   const int n = p.plen ? p.plen[g] : p.plen_all;
@@ -50,6 +54,7 @@ struct SaItem {
   int row0, rows;     // (token, head) rows of the tile: first, count (of the item's own numbering)
   int j0, j1;         // keys [j0, j1)
   int n0, kvh, slot;  // first batch row
+  int plane;          // (group or row) x KV head: which [cap][hd] block of the cache
   bool own;
 };
 
@@ -76,7 +81,8 @@ __device__ __forceinline__ SaItem sa_item(const SaParams& p, int it, int tile, i
     s.n0 = g * p.W;
     total = p.W * p.T * per;
     s.row0 = t * tile;
-    const size_t off = (size_t(g) * p.hkv + s.kvh) * p.cap_p * HD * ES;
+    s.plane = g * p.hkv + s.kvh;
+    const size_t off = size_t(s.plane) * p.cap_p * HD * ES;
     s.k = static_cast<const char*>(p.kp) + off;
     s.v = static_cast<const char*>(p.vp) + off;
     s.slot = split;
@@ -92,7 +98,8 @@ __device__ __forceinline__ SaItem sa_item(const SaParams& p, int it, int tile, i
     len = sa_cache_len(p, s.n0);
     total = p.T * per;
     s.row0 = t * tile;
-    const size_t off = (size_t(s.n0) * p.hkv + s.kvh) * p.cap * HD * ES;
+    s.plane = s.n0 * p.hkv + s.kvh;
+    const size_t off = size_t(s.plane) * p.cap * HD * ES;
     s.k = static_cast<const char*>(p.kc) + off;
     s.v = static_cast<const char*>(p.vc) + off;
     s.slot = p.sp + split;
@@ -510,6 +517,322 @@ __global__ void __launch_bounds__(32 * NW) sa_token_kernel(const SaParams p, con
       if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mx, den);
       *reinterpret_cast<float4*>(p.part_o + at * HD + d) = make_float4(num[0], num[1], num[2], num[3]);
     }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Items on the tensor cores (bf16, head dim 64 or 128): tiles of 128 (token,
+// head) rows by 128 keys, one item a CTA.
+//   warp 0      TMA: K and V tiles (128 keys x 64 dims boxes, 128-byte
+//               swizzle) into their rings;
+//   warp 1      MMA issue: S = Q K^T into one of two tensor-memory tiles,
+//               O += P V into one of two accumulators;
+//   warps 2-5   softmax of the even key tiles, a row a thread; warps 6-9 of
+//               the odd ones. The two streams have their own max, sum and O
+//               and are joined at the end, so one stream's softmax runs under
+//               the other's and under the MMAs.
+// P goes through shared memory as bf16 (K-major A operand); V is read as it
+// lies (N-major B operand). The max that the exponentials are taken against is
+// replaced, and O rescaled in tensor memory, only when a row's max has grown by
+// more than 2^8: until then P is at most 2^8, which costs no precision, as a
+// later division by the sum takes the factor out.
+// Keys from the end of the range on are masked by selection; their V rows are
+// zeroed in shared memory, since 0 x NaN would not be 0.
+// ---------------------------------------------------------------------------
+constexpr int kSaTcRows = 128, kSaTcKeys = 128;
+constexpr int kSaTcThreads = 320;
+constexpr uint32_t kSaTcSub = 128 * 64 * 2;  // a 128 x 64 bf16 subtile
+
+template <int HD>
+struct SaTcCfg {
+  static constexpr int kSubs = HD / 64;
+  static constexpr int kStages = HD == 128 ? 2 : 4;
+  static constexpr uint32_t kTile = kSubs * kSaTcSub;  // a K, V or Q tile
+  static constexpr uint32_t kP = 2 * kSaTcSub;
+  static constexpr uint32_t kOffK = kTile, kOffV = kOffK + kStages * kTile, kOffP = kOffV + kStages * kTile;
+  static constexpr size_t kSmem = size_t(kOffP) + 2 * kP + 1024;
+  static constexpr uint32_t kTmemCols = 512, kTmemO = 256;  // S tiles at 0 and 128
+  static constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+  // B of P V: N (dims) contiguous
+  static constexpr uint32_t kIdescO =
+      (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kSaTcThreads, 1)
+    sa_tc_kernel(const SaParams p, const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
+                 const __grid_constant__ CUtensorMap map_kc, const __grid_constant__ CUtensorMap map_vc) {
+  using C = SaTcCfg<HD>;
+  constexpr int S = C::kStages;
+  constexpr uint64_t kBudget = 2000000000ull;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t kfull[S], kempty[S], vfull[S], vempty[S], qfull, s_full[2], s_free[2], p_full[2], pv_done[2], drain;
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_sh;
+  volatile int* abort = &abort_sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
+  pdl_wait();
+  pdl_launch();  // after the wait: sa_token_kernel counts on it
+  const SaItem it = sa_item<HD, 2>(p, blockIdx.x, kSaTcRows, kSaTcKeys);
+  const size_t nrow = size_t(p.G) * p.W * p.T * p.hq;
+  if (it.j0 >= it.j1) {
+    for (int r = threadIdx.x; r < it.rows; r += kSaTcThreads) {
+      const SaRow x = sa_row(p, it, r);
+      const size_t at = it.slot * nrow + (size_t(x.n) * p.T + x.t) * p.hq + x.head;
+      *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+  const int nt = (it.j1 - it.j0 + kSaTcKeys - 1) / kSaTcKeys;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(kfull + s, 1);
+      mbar_init(kempty + s, 1);
+      mbar_init(vfull + s, 1);
+      mbar_init(vempty + s, 1);
+    }
+    mbar_init(&qfull, 8);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(s_full + x, 1);
+      mbar_init(s_free + x, 4);
+      mbar_init(p_full + x, 4);
+      mbar_init(pv_done + x, 1);
+    }
+    mbar_init(&drain, 1);
+    *abort = 0;
+    mbar_init_fence();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                 "r"(C::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  int issued = 0;  // warp 0: tiles whose copies were issued
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const CUtensorMap* mk = it.own ? &map_kc : &map_kp;
+      const CUtensorMap* mv = it.own ? &map_vc : &map_vp;
+      for (int t = 0; t < nt && !*abort; ++t) {
+        const int s = t % S, j = it.j0 + t * kSaTcKeys;
+        const uint32_t par = uint32_t((t / S) & 1) ^ 1u;
+        if (t >= S && !(mbar_wait(kempty + s, par, kBudget, abort) && mbar_wait(vempty + s, par, kBudget, abort))) {
+          *abort = 1;
+          break;
+        }
+        mbar_arrive_expect_tx(kfull + s, C::kTile);
+#pragma unroll
+        for (int b = 0; b < C::kSubs; ++b)
+          tma_load_3d(base + C::kOffK + s * C::kTile + b * kSaTcSub, mk, b * 64, j, it.plane, kfull + s);
+        mbar_arrive_expect_tx(vfull + s, C::kTile);
+#pragma unroll
+        for (int b = 0; b < C::kSubs; ++b)
+          tma_load_3d(base + C::kOffV + s * C::kTile + b * kSaTcSub, mv, b * 64, j, it.plane, vfull + s);
+        issued = t + 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = mbar_wait(&qfull, 0u, kBudget, abort);
+      auto pv = [&](int u) {
+        const int y = u & 1, s = u % S;
+        if (!mbar_wait(vfull + s, uint32_t((u / S) & 1), kBudget, abort) ||
+            !mbar_wait(p_full + y, uint32_t((u >> 1) & 1), kBudget, abort))
+          return false;
+        tc_fence_after();
+        const uint32_t pa = base + C::kOffP + y * C::kP, vb = base + C::kOffV + s * C::kTile;
+#pragma unroll
+        for (int k = 0; k < kSaTcKeys / 16; ++k)
+          tc_mma(tmem + C::kTmemO + y * HD, tc_smem_desc(pa + (k >> 2) * kSaTcSub + (k & 3) * 32),
+                 tc_smem_desc_mn(vb + k * 2048, kSaTcSub), C::kIdescO, (u > 1 || k > 0) ? 1u : 0u);
+        tc_commit(vempty + s);
+        tc_commit(pv_done + y);
+        return true;
+      };
+      for (int t = 0; ok && t < nt; ++t) {
+        const int x = t & 1, s = t % S;
+        ok = mbar_wait(kfull + s, uint32_t((t / S) & 1), kBudget, abort) &&
+             (t < 2 || mbar_wait(s_free + x, uint32_t(((t >> 1) - 1) & 1), kBudget, abort));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t kb = base + C::kOffK + s * C::kTile;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          tc_mma(tmem + x * 128, tc_smem_desc(base + (k >> 2) * kSaTcSub + (k & 3) * 32),
+                 tc_smem_desc(kb + (k >> 2) * kSaTcSub + (k & 3) * 32), C::kIdescS, k > 0 ? 1u : 0u);
+        tc_commit(kempty + s);
+        tc_commit(s_full + x);
+        if (t > 0) ok = pv(t - 1);
+      }
+      if (ok) ok = pv(nt - 1);
+      if (!ok) *abort = 1;
+    }
+  } else {
+    // ---- softmax warps
+    const int stid = int(threadIdx.x) - 64, x = stid >> 7;
+    const int quarter = warp & 3, r = quarter * 32 + lane;
+    for (int i = stid; i < kSaTcRows * (HD / 8); i += 256) {
+      const int row = i / (HD / 8), c = i - row * (HD / 8);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row < it.rows) {
+        const SaRow w = sa_row(p, it, row);
+        v = ld_vec(static_cast<const bf16*>(p.q) + ((size_t(w.n) * p.T + w.t) * p.hq + w.head) * HD + c * 8);
+      }
+      *reinterpret_cast<uint4*>(smem + (c >> 3) * kSaTcSub + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&qfull);
+    const uint32_t trow = tmem + (uint32_t(quarter * 32) << 16);
+    const uint32_t ts = trow + x * 128, to = trow + C::kTmemO + x * HD;
+    unsigned char* pbuf = smem + C::kOffP + x * C::kP + r * 128;
+    int lim = it.j1;  // keys [0, lim) are seen
+    if (r < it.rows) lim = min(lim, sa_limit(p, it, sa_row(p, it, r)));
+    const float sl2 = p.scale * kLog2e;
+    float m = -INFINITY, l = 0.f;  // reference max (scaled, base 2), sum
+    bool ok = true;
+    for (int u = x; u < nt; u += 2) {
+      const int k = u >> 1, j = it.j0 + u * kSaTcKeys;
+      ok = mbar_wait(s_full + x, uint32_t(k & 1), kBudget, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      float sc[kSaTcKeys];
+#pragma unroll
+      for (int c = 0; c < kSaTcKeys; c += 32) tc_ld32(ts + c, reinterpret_cast<uint32_t*>(sc + c));
+      tc_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free + x);
+      if (__any_sync(0xffffffffu, j + kSaTcKeys > lim)) {
+#pragma unroll
+        for (int c = 0; c < kSaTcKeys; ++c) sc[c] = j + c < lim ? sc[c] : -INFINITY;
+      }
+      float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+      for (int c = 4; c < kSaTcKeys; ++c) mx[c & 3] = fmaxf(mx[c & 3], sc[c]);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+      const bool grow = top > m + 8.f;
+      if (k > 0) {  // the stream's previous P V has read P and written O
+        ok = mbar_wait(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+        const float a = grow ? exp2_approx(m - top) : 1.f;
+        if (grow) m = top;
+        l *= a;
+        if (k > 0) {
+#pragma unroll
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            tc_ld32(to + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+            tc_st16(to + c, o);
+            tc_st16(to + c + 16, o + 16);
+          }
+          tc_wait_st();
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < kSaTcKeys; c += 8) {
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = exp2_approx(fmaf(sc[c + i], sl2, -ref));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i & 3] += e[i];
+        *reinterpret_cast<uint4*>(pbuf + (c >> 6) * kSaTcSub + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
+            make_uint4(pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7]));
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (j + kSaTcKeys > it.j1) {  // the last tile: V rows behind the range
+        const int s = u % S;
+        ok = mbar_wait(vfull + s, uint32_t((u / S) & 1), kBudget, abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (j + r >= it.j1) {
+#pragma unroll
+          for (int b = 0; b < C::kSubs; ++b)
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint4*>(smem + C::kOffV + s * C::kTile + b * kSaTcSub + r * 128 + c * 16) =
+                  make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + x);
+    }
+    const int mine = (nt + 1 - x) >> 1;  // tiles of this stream
+    if (ok && mine > 0) ok = mbar_wait(pv_done + x, uint32_t((mine - 1) & 1), kBudget, abort);
+    if (!ok) *abort = 1;
+    // statistics of the streams, each in its own P buffer (read for the last time)
+    float2* ml_sh = reinterpret_cast<float2*>(smem + C::kOffP);
+    ml_sh[x * (C::kP / 8) + r] = make_float2(mine > 0 ? m : -INFINITY, l);
+    tc_fence_before();
+    named_sync(1, 256);  // both streams' O and statistics
+    tc_fence_after();
+    const float2 a = ml_sh[r], b = ml_sh[C::kP / 8 + r];
+    const float top = fmaxf(a.x, b.x), ref = top == -INFINITY ? 0.f : top;
+    const float wa = exp2_approx(a.x - ref), wb = exp2_approx(b.x - ref);
+    const bool write = r < it.rows;
+    size_t at = 0;
+    if (write) {
+      const SaRow w = sa_row(p, it, r);
+      at = it.slot * nrow + (size_t(w.n) * p.T + w.t) * p.hq + w.head;
+      if (x == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(top * kLn2, a.y * wa + b.y * wb);
+    }
+    // stream x joins dims [x * HD / 2, (x + 1) * HD / 2)
+#pragma unroll
+    for (int c = x * (HD / 2); c < (x + 1) * (HD / 2); c += 16) {
+      uint32_t o0[16], o1[16];
+      tc_ld16(trow + C::kTmemO + c, o0);
+      if (nt > 1) tc_ld16(trow + C::kTmemO + HD + c, o1);
+      tc_wait_ld();
+      if (write) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          float f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f[i] = __uint_as_float(o0[e + i]) * wa;
+            if (nt > 1) f[i] = fmaf(__uint_as_float(o1[e + i]), wb, f[i]);
+          }
+          *reinterpret_cast<float4*>(p.part_o + at * HD + c + e) = make_float4(f[0], f[1], f[2], f[3]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  // ---- teardown: copies and MMAs in flight land before the memory goes away
+  if (warp == 0 && lane == 0) {
+    int never = 0;
+    for (int t = max(0, issued - S); t < issued; ++t) {
+      mbar_wait(kfull + t % S, uint32_t((t / S) & 1), kBudget, &never);
+      mbar_wait(vfull + t % S, uint32_t((t / S) & 1), kBudget, &never);
+    }
+  }
+  if (warp == 1 && lane == 0) {
+    int never = 0;
+    tc_commit(&drain);
+    mbar_wait(&drain, 0u, kBudget, &never);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort) atomicOr(p.status ? p.status : &g_sa_status, kStatusTimeout);
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
   }
 }
 
