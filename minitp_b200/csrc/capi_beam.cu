@@ -209,9 +209,11 @@ struct SaPlan {
   bool token;       // one token a row on sa_token_kernel
   bool inline_pre;  // it reads the prefix too: no other launch
   bool tc;          // the other items on sa_tc_kernel, else on the CUDA cores
+  int mt;           // its row tiles a CTA
   int warps;
   int rpt;  // CUDA-core items: rows a tile / 16
   int sp, so, ptiles, otiles;
+  int pblocks, oblocks;
   long long pitems, items;
   size_t rows, ml_bytes, o_bytes;
 };
@@ -254,7 +256,9 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   const long long prow = (long long)a.W * a.T * per, orow = (long long)a.T * per;
   // CUDA-core items: row tiles of 64 when a row's tokens fill them, else of 16
   pl.rpt = orow >= 64 ? 4 : 1;
-  const int tile = pl.tc ? kSaTcRows : 16 * pl.rpt;
+  // two row tiles a CTA from the second on (for most items)
+  pl.mt = prow > 128 ? 2 : 1;
+  const int tile = pl.tc ? 128 * pl.mt : 16 * pl.rpt;
   pl.ptiles = int((prow + tile - 1) / tile);
   pl.otiles = pl.token ? (per + 15) / 16 : int((orow + tile - 1) / tile);
   const long long pbase = (long long)a.G * a.hkv * pl.ptiles, obase = N * a.hkv * pl.otiles;
@@ -279,9 +283,13 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   pl.pitems = pbase * pl.sp;
   pl.items = pl.pitems + (pl.token ? 0 : obase * pl.so);
   if (pl.items > 0x7FFFFFFFll) return bad("shared_attention: too many rows");
-  const int slots = pl.sp + (pl.token && pl.so == 1 ? 0 : pl.so);
-  pl.ml_bytes = (pl.rows * slots * 8 + 255) / 256 * 256;
-  pl.o_bytes = pl.rows * slots * a.hd * 4;
+  pl.pblocks = int((prow + 31) / 32);
+  pl.oblocks = int((orow + 31) / 32);
+  const size_t blocks = size_t(pl.sp) * a.G * a.hkv * pl.pblocks +
+                        size_t(pl.token && pl.so == 1 ? 0 : pl.so) * N * a.hkv * pl.oblocks;
+  pl.ml_bytes = blocks * 32 * 8;
+  pl.o_bytes = blocks * 32 * a.hd * 4;
+  if (N * a.hkv * pl.oblocks > 0x7FFFFFFFll) return bad("shared_attention: too many rows");
   *out = pl;
   return MTPB_OK;
 }
@@ -310,8 +318,9 @@ int sa_launch_tc(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
   if (r == MTPB_OK) r = sa_map(m + 2, p.kc, N * p.hkv, p.cap, HD);
   if (r == MTPB_OK) r = sa_map(m + 3, p.vc, N * p.hkv, p.cap, HD);
   if (r != MTPB_OK) return r;
-  return host_launch(sa_tc_kernel<HD>, dim3((unsigned)pl.items), dim3(kSaTcThreads), SaTcCfg<HD>::kSmem, st, p, m[0],
-                     m[1], m[2], m[3]);
+  const dim3 grid((unsigned)pl.items), block(kSaTcThreads);
+  return pl.mt == 2 ? host_launch(sa_tc_kernel<HD, 2>, grid, block, SaTcCfg<HD, 2>::kSmem, st, p, m[0], m[1], m[2], m[3])
+                    : host_launch(sa_tc_kernel<HD, 1>, grid, block, SaTcCfg<HD, 1>::kSmem, st, p, m[0], m[1], m[2], m[3]);
 }
 
 template <int HD, int NW>
@@ -349,9 +358,8 @@ int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
       if (r != MTPB_OK || pl.so == 1) return r;
     }
   }
-  const size_t n = pl.rows * (HD / 4);
-  return host_launch(sa_join_kernel<T, HD>, dim3(unsigned((n + kSaJoinThreads - 1) / kSaJoinThreads)),
-                     dim3(kSaJoinThreads), 0, st, p);
+  return host_launch(sa_join_kernel<T, HD>, dim3(unsigned(p.G * p.W * p.hkv * pl.oblocks)), dim3(kSaJoinThreads), 0, st,
+                     p);
 }
 
 template <typename T>
@@ -416,7 +424,9 @@ int shared_attn_run(const SharedAttnArgs& a, void* ws, size_t ws_bytes, cudaStre
   p.otiles = pl.otiles;
   p.pitems = int(pl.pitems);
   p.items = int(pl.items);
-  p.part_ml = static_cast<float*>(ws);
+  p.pblocks = pl.pblocks;
+  p.oblocks = pl.oblocks;
+  p.part_ml = static_cast<float2*>(ws);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.ml_bytes);
   p.status = a.status;
   return a.dtype == MTPB_BF16 ? sa_launch_hd<bf16>(pl, p, a.hd, st) : sa_launch_hd<float>(pl, p, a.hd, st);

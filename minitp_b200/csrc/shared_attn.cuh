@@ -30,8 +30,10 @@ struct SaParams {
   int sp, so;        // key ranges of the prefix and of an own cache
   int ptiles, otiles;  // row tiles of a (group, KV head) and of a (row, KV head)
   int pitems, items;   // prefix items, all items
-  float* part_o;     // [slot][row = (n * T + t) * hq + h][hd]
-  float* part_ml;    // [slot][row][2]: max (base e, scaled), sum
+  // partial sums, in blocks of 32 rows (SaPart)
+  int pblocks, oblocks;  // blocks of a prefix plane, of an own plane
+  float* part_o;         // [block][hd / 4][32 rows][4]
+  float2* part_ml;       // [block][32 rows]: max (base e, scaled), sum
   uint32_t* status;  // of a communicator, or NULL: g_sa_status
 };
 
@@ -53,10 +55,24 @@ struct SaItem {
   const void *k, *v;  // first position of this KV head
   int row0, rows;     // (token, head) rows of the tile: first, count (of the item's own numbering)
   int j0, j1;         // keys [j0, j1)
-  int n0, kvh, slot;  // first batch row
+  int n0, kvh, split;  // first batch row
   int plane;          // (group or row) x KV head: which [cap][hd] block of the cache
   bool own;
 };
+
+// Where a row's partial sums lie. A plane is a (group, KV head) or (row, KV
+// head); its rows (token, head) are cut into blocks of 32 that lie dims-major,
+// so that the 32 lanes of a warp, each with a row, move 512 bytes at once.
+struct SaPart {
+  size_t ml, o;  // elements of part_ml, part_o (dims 0..3; + 128 every 4 dims)
+};
+template <int HD>
+__device__ __forceinline__ SaPart sa_part(const SaParams& p, bool own, int split, int plane, int r) {
+  const size_t pp = size_t(p.G) * p.hkv, op = pp * p.W;
+  const size_t b = (own ? p.sp * pp * p.pblocks + (split * op + plane) * p.oblocks
+                        : (split * pp + plane) * p.pblocks) + (r >> 5);
+  return SaPart{b * 32 + (r & 31), b * 32 * HD + (r & 31) * 4};
+}
 
 // Row r of an item: token r / per of the item's rows, query head r % per of its KV head.
 struct SaRow {
@@ -85,7 +101,7 @@ __device__ __forceinline__ SaItem sa_item(const SaParams& p, int it, int tile, i
     const size_t off = size_t(s.plane) * p.cap_p * HD * ES;
     s.k = static_cast<const char*>(p.kp) + off;
     s.v = static_cast<const char*>(p.vp) + off;
-    s.slot = split;
+    s.split = split;
   } else {
     splits = p.so;
     it -= p.pitems;
@@ -102,7 +118,7 @@ __device__ __forceinline__ SaItem sa_item(const SaParams& p, int it, int tile, i
     const size_t off = size_t(s.plane) * p.cap * HD * ES;
     s.k = static_cast<const char*>(p.kc) + off;
     s.v = static_cast<const char*>(p.vc) + off;
-    s.slot = p.sp + split;
+    s.split = split;
   }
   s.rows = min(tile, total - s.row0);
   if (s.own) {  // no key past the last token of the tile
@@ -162,7 +178,6 @@ __global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
   pdl_launch();  // after the wait: sa_token_kernel counts on it
   const int tid = threadIdx.x, rg = tid >> 4, sub = tid & 15;
   const SaItem s = sa_item<HD, int(sizeof(T))>(p, blockIdx.x, R, kSaKT);
-  const size_t nrow = size_t(p.G) * p.W * p.T * p.hq;
   for (int i = tid; i < R * (HD / VE); i += kSaThreads) {
     const int r = i / (HD / VE), c = i - r * (HD / VE);
     float f[VE];
@@ -271,12 +286,14 @@ __global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
   for (int i = 0; i < RPT; ++i) {
     const int r = rg * RPT + i;
     if (r >= s.rows) continue;
-    const SaRow x = sa_row(p, s, r);
-    const size_t at = s.slot * nrow + (size_t(x.n) * p.T + x.t) * p.hq + x.head;
-    if (sub == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m[i], l[i]);
+    const SaPart at = sa_part<HD>(p, s.own, s.split, s.plane, s.row0 + r);
+    if (sub == 0) p.part_ml[at.ml] = make_float2(m[i], l[i]);
     if (s.j0 < s.j1)
 #pragma unroll
-      for (int d = 0; d < DPT; ++d) p.part_o[at * HD + sub * DPT + d] = o[i][d];
+      for (int d = 0; d < DPT; ++d) {
+        const int dim = sub * DPT + d;
+        p.part_o[at.o + (dim >> 2) * 128 + (dim & 3)] = o[i][d];
+      }
   }
 }
 
@@ -481,117 +498,124 @@ __global__ void __launch_bounds__(32 * NW) sa_token_kernel(const SaParams p, con
       }
   __syncthreads();
   if (!inline_prefix) pdl_wait();  // the prefix items' partial sums
-  const bool last = p.so == 1;  // else a slot for the join
-  const size_t nrow = size_t(p.G) * p.W * p.hq;
+  const bool last = p.so == 1;  // else partial sums for the join
+  const int pslots = last && !inline_prefix ? p.sp : 0;
   for (int i = threadIdx.x; i < rows * (HD / 4); i += 32 * NW) {
-    const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
-    const size_t row = size_t(n) * p.hq + head0 + r;
+    const int q = i / rows, r = i - q * rows;
+    const int pr = (n - gi * p.W) * per + tile * 16 + r;  // row of the prefix plane
     float mx = -INFINITY;
+#pragma unroll
     for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sml[(w * R + r) * 2]);
-    if (last && !inline_prefix)
-      for (int s = 0; s < p.sp; ++s) mx = fmaxf(mx, __ldcg(p.part_ml + (s * nrow + row) * 2));
+#pragma unroll 4
+    for (int s = 0; s < pslots; ++s)
+      mx = fmaxf(mx, __ldcg(p.part_ml + sa_part<HD>(p, false, s, gi * p.hkv + kvh, pr).ml).x);
+    const float ref = mx == -INFINITY ? 0.f : mx;
     float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
     auto add = [&](float m, float l, const float4& f) {
-      const float w = expf(m - mx);
+      const float w = m == -INFINITY ? 0.f : expf(m - ref);
       den = fmaf(w, l, den);
-      num[0] = fmaf(w, f.x, num[0]);
-      num[1] = fmaf(w, f.y, num[1]);
-      num[2] = fmaf(w, f.z, num[2]);
-      num[3] = fmaf(w, f.w, num[3]);
-    };
-    for (int w = 0; w < NW; ++w) {
-      const float m = sml[(w * R + r) * 2];
-      if (m != -INFINITY) add(m, sml[(w * R + r) * 2 + 1], *reinterpret_cast<const float4*>(so + (w * R + r) * HD + d));
-    }
-    if (last && !inline_prefix)
-      for (int s = 0; s < p.sp; ++s) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (s * nrow + row) * 2));
-        if (ml.x != -INFINITY) add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * nrow + row) * HD + d)));
+      if (w != 0.f) {  // an empty range leaves its sums unwritten
+        num[0] = fmaf(w, f.x, num[0]);
+        num[1] = fmaf(w, f.y, num[1]);
+        num[2] = fmaf(w, f.z, num[2]);
+        num[3] = fmaf(w, f.w, num[3]);
       }
+    };
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+      add(sml[(w * R + r) * 2], sml[(w * R + r) * 2 + 1], *reinterpret_cast<const float4*>(so + (w * R + r) * HD + 4 * q));
+#pragma unroll 4
+    for (int s = 0; s < pslots; ++s) {
+      const SaPart at = sa_part<HD>(p, false, s, gi * p.hkv + kvh, pr);
+      const float2 ml = __ldcg(p.part_ml + at.ml);
+      add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part_o + at.o + q * 128)));
+    }
     if (last) {
       const float inv = den > 0.f ? 1.f / den : 0.f;
-      *reinterpret_cast<uint2*>(static_cast<bf16*>(p.out) + row * HD + d) =
+      *reinterpret_cast<uint2*>(static_cast<bf16*>(p.out) + (size_t(n) * p.hq + head0 + r) * HD + 4 * q) =
           make_uint2(pack_bf16(num[0] * inv, num[1] * inv), pack_bf16(num[2] * inv, num[3] * inv));
     } else {
-      const size_t at = size_t(p.sp + split) * nrow + row;
-      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mx, den);
-      *reinterpret_cast<float4*>(p.part_o + at * HD + d) = make_float4(num[0], num[1], num[2], num[3]);
+      const SaPart at = sa_part<HD>(p, true, split, n * p.hkv + kvh, tile * 16 + r);
+      if (q == 0) p.part_ml[at.ml] = make_float2(mx, den);
+      *reinterpret_cast<float4*>(p.part_o + at.o + q * 128) = make_float4(num[0], num[1], num[2], num[3]);
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Items on the tensor cores (bf16, head dim 64 or 128): tiles of 128 (token,
-// head) rows by 128 keys, one item a CTA.
-//   warp 0      TMA: K and V tiles (128 keys x 64 dims boxes, 128-byte
-//               swizzle) into their rings;
-//   warp 1      MMA issue: S = Q K^T into one of two tensor-memory tiles,
-//               O += P V into one of two accumulators;
-//   warps 2-5   softmax of the even key tiles, a row a thread; warps 6-9 of
-//               the odd ones. The two streams have their own max, sum and O
-//               and are joined at the end, so one stream's softmax runs under
-//               the other's and under the MMAs.
-// P goes through shared memory as bf16 (K-major A operand); V is read as it
-// lies (N-major B operand). The max that the exponentials are taken against is
-// replaced, and O rescaled in tensor memory, only when a row's max has grown by
-// more than 2^8: until then P is at most 2^8, which costs no precision, as a
-// later division by the sum takes the factor out.
+// Items on the tensor cores (bf16, head dim 64 or 128), one item a CTA, key
+// tiles of 128. Two streams share the K and V tiles' ring, each with an MMA
+// warp, a softmax warpgroup (a row a thread) and its own tensor memory:
+//   MT 2: stream x has rows 128 x .. of the item's 256 and all key tiles, so
+//         a K/V byte brought in from L2 serves 256 rows;
+//   MT 1: both have the item's 128 rows, stream x the key tiles t = x mod 2,
+//         and the streams are joined at the end.
+// One stream's softmax runs under the other's and under the MMAs:
+//   warp 0 loads (TMA, 128 keys x 64 dims boxes, 128-byte swizzle), warps 1
+//   and 2 issue S = Q K^T and O += P V of their stream, warps 4-7 and 8-11
+//   turn S into P.
+// P is bf16 in tensor memory, the A operand of P V; for head dim 128, where S
+// and O fill the 512 columns, it takes the place of its S, and the stream's
+// next S waits for the P V that reads it. V is read as it lies (N-major B).
+// The max that the exponentials are taken against is replaced, and O rescaled
+// in tensor memory, only when a row's max has grown by more than 2^8: until
+// then P is at most 2^8, which costs no precision, as the division by the sum
+// takes the factor out.
 // Keys from the end of the range on are masked by selection; their V rows are
 // zeroed in shared memory, since 0 x NaN would not be 0.
 // ---------------------------------------------------------------------------
-constexpr int kSaTcRows = 128, kSaTcKeys = 128;
-constexpr int kSaTcThreads = 320;
+constexpr int kSaTcKeys = 128;
+constexpr int kSaTcThreads = 384;
 constexpr uint32_t kSaTcSub = 128 * 64 * 2;  // a 128 x 64 bf16 subtile
 
-template <int HD>
+template <int HD, int MT>
 struct SaTcCfg {
   static constexpr int kSubs = HD / 64;
-  static constexpr int kStages = HD == 128 ? 2 : 4;
   static constexpr uint32_t kTile = kSubs * kSaTcSub;  // a K, V or Q tile
-  static constexpr uint32_t kP = 2 * kSaTcSub;
-  static constexpr uint32_t kOffK = kTile, kOffV = kOffK + kStages * kTile, kOffP = kOffV + kStages * kTile;
-  static constexpr size_t kSmem = size_t(kOffP) + 2 * kP + 1024;
-  static constexpr uint32_t kTmemCols = 512, kTmemO = 256;  // S tiles at 0 and 128
+  // ring of K and V tiles: what 224 KB leave beside Q (at most six of each)
+  static constexpr int kRing = HD == 128 ? 7 - MT : 12;
+  static constexpr uint32_t kOffRing = MT * kTile;
+  static constexpr size_t kSmem = size_t(kOffRing) + kRing * kTile + 1024;
+  static constexpr bool kAlias = HD == 128;  // P in the place of S
+  static constexpr uint32_t kS = 128;        // columns from stream to stream of S; of O: HD
+  static constexpr uint32_t kO = 256, kP = kAlias ? 0 : 384, kPStep = kAlias ? 128 : 64;
   static constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);
   // B of P V: N (dims) contiguous
   static constexpr uint32_t kIdescO =
       (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 };
 
-template <int HD>
+template <int HD, int MT>
 __global__ void __launch_bounds__(kSaTcThreads, 1)
     sa_tc_kernel(const SaParams p, const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
                  const __grid_constant__ CUtensorMap map_kc, const __grid_constant__ CUtensorMap map_vc) {
-  using C = SaTcCfg<HD>;
-  constexpr int S = C::kStages;
+  using C = SaTcCfg<HD, MT>;
+  constexpr int NB = C::kRing;
   constexpr uint64_t kBudget = 2000000000ull;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t kfull[S], kempty[S], vfull[S], vempty[S], qfull, s_full[2], s_free[2], p_full[2], pv_done[2], drain;
+  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2], pv_done[2], drain[2];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_sh;
+  __shared__ float2 ml_sh[128];  // MT 1: stream 1's statistics
   volatile int* abort = &abort_sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
   pdl_wait();
   pdl_launch();  // after the wait: sa_token_kernel counts on it
-  const SaItem it = sa_item<HD, 2>(p, blockIdx.x, kSaTcRows, kSaTcKeys);
-  const size_t nrow = size_t(p.G) * p.W * p.T * p.hq;
+  const SaItem it = sa_item<HD, 2>(p, blockIdx.x, 128 * MT, kSaTcKeys);
   if (it.j0 >= it.j1) {
-    for (int r = threadIdx.x; r < it.rows; r += kSaTcThreads) {
-      const SaRow x = sa_row(p, it, r);
-      const size_t at = it.slot * nrow + (size_t(x.n) * p.T + x.t) * p.hq + x.head;
-      *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(-INFINITY, 0.f);
-    }
+    for (int r = threadIdx.x; r < it.rows; r += kSaTcThreads)
+      p.part_ml[sa_part<HD>(p, it.own, it.split, it.plane, it.row0 + r).ml] = make_float2(-INFINITY, 0.f);
     return;
   }
   const int nt = (it.j1 - it.j0 + kSaTcKeys - 1) / kSaTcKeys;
+  // tiles of a stream: first, step
+  constexpr int kStep = MT == 2 ? 1 : 2;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S; ++s) {
-      mbar_init(kfull + s, 1);
-      mbar_init(kempty + s, 1);
-      mbar_init(vfull + s, 1);
-      mbar_init(vempty + s, 1);
+    for (int s = 0; s < NB; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, MT);  // each stream that reads the tile
     }
     mbar_init(&qfull, 8);
     for (int x = 0; x < 2; ++x) {
@@ -599,14 +623,14 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
       mbar_init(s_free + x, 4);
       mbar_init(p_full + x, 4);
       mbar_init(pv_done + x, 1);
+      mbar_init(drain + x, 1);
     }
-    mbar_init(&drain, 1);
     *abort = 0;
     mbar_init_fence();
   }
-  if (warp == 1) {
+  if (warp == 3) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
-                 "r"(C::kTmemCols)
+                 "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -614,102 +638,123 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
-  int issued = 0;  // warp 0: tiles whose copies were issued
+  int issued = 0;  // warp 0: ring entries whose copies were issued
 
   if (warp == 0) {
     if (lane == 0) {
       const CUtensorMap* mk = it.own ? &map_kc : &map_kp;
       const CUtensorMap* mv = it.own ? &map_vc : &map_vp;
-      for (int t = 0; t < nt && !*abort; ++t) {
-        const int s = t % S, j = it.j0 + t * kSaTcKeys;
-        const uint32_t par = uint32_t((t / S) & 1) ^ 1u;
-        if (t >= S && !(mbar_wait(kempty + s, par, kBudget, abort) && mbar_wait(vempty + s, par, kBudget, abort))) {
+      for (int i = 0; i < 2 * nt && !*abort; ++i) {  // K and V of each tile in turn
+        const int s = i % NB, j = it.j0 + (i >> 1) * kSaTcKeys;
+        if (i >= NB && !mbar_wait_soon(empty + s, uint32_t((i / NB) & 1) ^ 1u, kBudget, abort)) {
           *abort = 1;
           break;
         }
-        mbar_arrive_expect_tx(kfull + s, C::kTile);
+        mbar_arrive_expect_tx(full + s, C::kTile);
 #pragma unroll
         for (int b = 0; b < C::kSubs; ++b)
-          tma_load_3d(base + C::kOffK + s * C::kTile + b * kSaTcSub, mk, b * 64, j, it.plane, kfull + s);
-        mbar_arrive_expect_tx(vfull + s, C::kTile);
-#pragma unroll
-        for (int b = 0; b < C::kSubs; ++b)
-          tma_load_3d(base + C::kOffV + s * C::kTile + b * kSaTcSub, mv, b * 64, j, it.plane, vfull + s);
-        issued = t + 1;
+          tma_load_3d(base + C::kOffRing + s * C::kTile + b * kSaTcSub, i & 1 ? mv : mk, b * 64, j, it.plane, full + s);
+        issued = i + 1;
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 2) {
+    // ---- MMA issue of stream x
+    const int x = warp - 1;
     if (lane == 0) {
-      bool ok = mbar_wait(&qfull, 0u, kBudget, abort);
-      auto pv = [&](int u) {
-        const int y = u & 1, s = u % S;
-        if (!mbar_wait(vfull + s, uint32_t((u / S) & 1), kBudget, abort) ||
-            !mbar_wait(p_full + y, uint32_t((u >> 1) & 1), kBudget, abort))
-          return false;
+      const int first = MT == 2 ? 0 : x;
+      const uint32_t qb = base + (MT == 2 ? x : 0) * C::kTile;
+      const uint32_t ts = tmem + x * C::kS, to = tmem + C::kO + x * HD, tp = tmem + C::kP + x * C::kPStep;
+      bool ok = first >= nt || mbar_wait_soon(&qfull, 0u, kBudget, abort);
+      auto qk = [&](int t, int k) {
+        const int i = 2 * t, s = i % NB;
+        if (!mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort)) return false;
+        // S is free: read by the softmax, and (aliased) its P read by P V
+        if (k > 0 && !mbar_wait_soon(C::kAlias ? pv_done + x : s_free + x, uint32_t((k - 1) & 1), kBudget, abort)) return false;
         tc_fence_after();
-        const uint32_t pa = base + C::kOffP + y * C::kP, vb = base + C::kOffV + s * C::kTile;
+        const uint32_t kb = base + C::kOffRing + s * C::kTile;
 #pragma unroll
-        for (int k = 0; k < kSaTcKeys / 16; ++k)
-          tc_mma(tmem + C::kTmemO + y * HD, tc_smem_desc(pa + (k >> 2) * kSaTcSub + (k & 3) * 32),
-                 tc_smem_desc_mn(vb + k * 2048, kSaTcSub), C::kIdescO, (u > 1 || k > 0) ? 1u : 0u);
-        tc_commit(vempty + s);
-        tc_commit(pv_done + y);
+        for (int q = 0; q < HD / 16; ++q)
+          tc_mma(ts, tc_smem_desc(qb + (q >> 2) * kSaTcSub + (q & 3) * 32),
+                 tc_smem_desc(kb + (q >> 2) * kSaTcSub + (q & 3) * 32), C::kIdescS, q > 0 ? 1u : 0u);
+        tc_commit(s_full + x);
+        tc_commit(empty + s);
         return true;
       };
-      for (int t = 0; ok && t < nt; ++t) {
-        const int x = t & 1, s = t % S;
-        ok = mbar_wait(kfull + s, uint32_t((t / S) & 1), kBudget, abort) &&
-             (t < 2 || mbar_wait(s_free + x, uint32_t(((t >> 1) - 1) & 1), kBudget, abort));
-        if (!ok) break;
+      auto pv = [&](int t, int k) {
+        const int i = 2 * t + 1, s = i % NB;
+        if (!mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort) ||
+            !mbar_wait_soon(p_full + x, uint32_t(k & 1), kBudget, abort))
+          return false;
         tc_fence_after();
-        const uint32_t kb = base + C::kOffK + s * C::kTile;
+        const uint32_t vb = base + C::kOffRing + s * C::kTile;
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
-          tc_mma(tmem + x * 128, tc_smem_desc(base + (k >> 2) * kSaTcSub + (k & 3) * 32),
-                 tc_smem_desc(kb + (k >> 2) * kSaTcSub + (k & 3) * 32), C::kIdescS, k > 0 ? 1u : 0u);
-        tc_commit(kempty + s);
-        tc_commit(s_full + x);
-        if (t > 0) ok = pv(t - 1);
+        for (int q = 0; q < kSaTcKeys / 16; ++q)
+          tc_mma_ta(to, tp + q * 8, tc_smem_desc_mn(vb + q * 2048, kSaTcSub), C::kIdescO, (k > 0 || q > 0) ? 1u : 0u);
+        tc_commit(pv_done + x);
+        tc_commit(empty + s);
+        return true;
+      };
+      if (C::kAlias) {
+        for (int t = first, k = 0; ok && t < nt; t += kStep, ++k) ok = qk(t, k) && pv(t, k);
+      } else {  // the next S under this one's softmax
+        if (ok && first < nt) ok = qk(first, 0);
+        for (int t = first, k = 0; ok && t < nt; t += kStep, ++k) {
+          if (t + kStep < nt) ok = qk(t + kStep, k + 1);
+          ok = ok && pv(t, k);
+        }
       }
-      if (ok) ok = pv(nt - 1);
       if (!ok) *abort = 1;
     }
-  } else {
-    // ---- softmax warps
-    const int stid = int(threadIdx.x) - 64, x = stid >> 7;
+  } else if (warp >= 4) {
+    // ---- softmax of stream x
+    const int stid = int(threadIdx.x) - 128, x = stid >> 7;
     const int quarter = warp & 3, r = quarter * 32 + lane;
-    for (int i = stid; i < kSaTcRows * (HD / 8); i += 256) {
-      const int row = i / (HD / 8), c = i - row * (HD / 8);
-      uint4 v = make_uint4(0, 0, 0, 0);
+    {  // Q: a row (MT 1: half a row) a thread, all loads in flight at once
+      constexpr int N = HD / 8 / (3 - MT);
+      const int row = MT == 2 ? stid : stid & 127, c0 = MT == 2 ? 0 : x * N;
+      uint4 v[N];
       if (row < it.rows) {
         const SaRow w = sa_row(p, it, row);
-        v = ld_vec(static_cast<const bf16*>(p.q) + ((size_t(w.n) * p.T + w.t) * p.hq + w.head) * HD + c * 8);
+        const bf16* q = static_cast<const bf16*>(p.q) + ((size_t(w.n) * p.T + w.t) * p.hq + w.head) * HD + c0 * 8;
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = ld_vec(q + c * 8);
+      } else {
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = make_uint4(0, 0, 0, 0);
       }
-      *reinterpret_cast<uint4*>(smem + (c >> 3) * kSaTcSub + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+      unsigned char* dst = smem + (row >> 7) * C::kTile + (row & 127) * 128;
+#pragma unroll
+      for (int c = 0; c < N; ++c)
+        *reinterpret_cast<uint4*>(dst + ((c0 + c) >> 3) * kSaTcSub + ((((c0 + c) & 7) ^ (row & 7)) << 4)) = v[c];
     }
     fence_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&qfull);
     const uint32_t trow = tmem + (uint32_t(quarter * 32) << 16);
-    const uint32_t ts = trow + x * 128, to = trow + C::kTmemO + x * HD;
-    unsigned char* pbuf = smem + C::kOffP + x * C::kP + r * 128;
-    int lim = it.j1;  // keys [0, lim) are seen
-    if (r < it.rows) lim = min(lim, sa_limit(p, it, sa_row(p, it, r)));
+    const uint32_t ts = trow + x * C::kS, to = trow + C::kO + x * HD, tp = trow + C::kP + x * C::kPStep;
+    const int row = MT == 2 ? x * 128 + r : r;
+    const bool write = row < it.rows;
+    SaRow w = {};
+    if (write) w = sa_row(p, it, row);
+    const int lim = write ? min(it.j1, sa_limit(p, it, w)) : it.j1;  // keys [0, lim) are seen
     const float sl2 = p.scale * kLog2e;
     float m = -INFINITY, l = 0.f;  // reference max (scaled, base 2), sum
     bool ok = true;
-    for (int u = x; u < nt; u += 2) {
-      const int k = u >> 1, j = it.j0 + u * kSaTcKeys;
-      ok = mbar_wait(s_full + x, uint32_t(k & 1), kBudget, abort);
+    int k = 0;
+    for (int t = MT == 2 ? 0 : x; t < nt; t += kStep, ++k) {
+      const int j = it.j0 + t * kSaTcKeys;
+      ok = mbar_wait_soon(s_full + x, uint32_t(k & 1), kBudget, abort);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       float sc[kSaTcKeys];
 #pragma unroll
       for (int c = 0; c < kSaTcKeys; c += 32) tc_ld32(ts + c, reinterpret_cast<uint32_t*>(sc + c));
       tc_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_free + x);
+      if (!C::kAlias) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free + x);
+      }
       if (__any_sync(0xffffffffu, j + kSaTcKeys > lim)) {
 #pragma unroll
         for (int c = 0; c < kSaTcKeys; ++c) sc[c] = j + c < lim ? sc[c] : -INFINITY;
@@ -719,8 +764,8 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
       for (int c = 4; c < kSaTcKeys; ++c) mx[c & 3] = fmaxf(mx[c & 3], sc[c]);
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
       const bool grow = top > m + 8.f;
-      if (k > 0) {  // the stream's previous P V has read P and written O
-        ok = mbar_wait(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
+      if (!C::kAlias && k > 0) {  // the stream's previous P V has read P (aliased: it came before this S)
+        ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
       }
@@ -730,85 +775,86 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
         l *= a;
         if (k > 0) {
 #pragma unroll
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tc_ld32(to + c, o);
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t o[16];
+            tc_ld16(to + c, o);
             tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
             tc_st16(to + c, o);
-            tc_st16(to + c + 16, o + 16);
           }
-          tc_wait_st();
         }
       }
       const float ref = m == -INFINITY ? 0.f : m;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < kSaTcKeys; c += 8) {
-        float e[8];
+      for (int c = 0; c < kSaTcKeys; c += 32) {
+        uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = exp2_approx(fmaf(sc[c + i], sl2, -ref));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i & 3] += e[i];
-        *reinterpret_cast<uint4*>(pbuf + (c >> 6) * kSaTcSub + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
-            make_uint4(pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7]));
+        for (int i = 0; i < 32; i += 2) {
+          const float e0 = exp2_approx(fmaf(sc[c + i], sl2, -ref)), e1 = exp2_approx(fmaf(sc[c + i + 1], sl2, -ref));
+          sum[i & 2] += e0;
+          sum[(i & 2) + 1] += e1;
+          pk[i / 2] = pack_bf16(e0, e1);
+        }
+        tc_st16(tp + c / 2, pk);
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      if (j + kSaTcKeys > it.j1) {  // the last tile: V rows behind the range
-        const int s = u % S;
-        ok = mbar_wait(vfull + s, uint32_t((u / S) & 1), kBudget, abort);
+      if (j + kSaTcKeys > it.j1) {  // the last tile: V rows behind the range (MT 2: both streams write the same zeros)
+        const int i = 2 * t + 1, s = i % NB;
+        ok = mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (j + r >= it.j1) {
 #pragma unroll
           for (int b = 0; b < C::kSubs; ++b)
 #pragma unroll
             for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<uint4*>(smem + C::kOffV + s * C::kTile + b * kSaTcSub + r * 128 + c * 16) =
+              *reinterpret_cast<uint4*>(smem + C::kOffRing + s * C::kTile + b * kSaTcSub + r * 128 + c * 16) =
                   make_uint4(0, 0, 0, 0);
         }
+        fence_async_smem();
       }
-      fence_async_smem();
+      tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + x);
     }
-    const int mine = (nt + 1 - x) >> 1;  // tiles of this stream
-    if (ok && mine > 0) ok = mbar_wait(pv_done + x, uint32_t((mine - 1) & 1), kBudget, abort);
+    if (ok && k > 0) ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
     if (!ok) *abort = 1;
-    // statistics of the streams, each in its own P buffer (read for the last time)
-    float2* ml_sh = reinterpret_cast<float2*>(smem + C::kOffP);
-    ml_sh[x * (C::kP / 8) + r] = make_float2(mine > 0 ? m : -INFINITY, l);
-    tc_fence_before();
-    named_sync(1, 256);  // both streams' O and statistics
     tc_fence_after();
-    const float2 a = ml_sh[r], b = ml_sh[C::kP / 8 + r];
-    const float top = fmaxf(a.x, b.x), ref = top == -INFINITY ? 0.f : top;
-    const float wa = exp2_approx(a.x - ref), wb = exp2_approx(b.x - ref);
-    const bool write = r < it.rows;
-    size_t at = 0;
-    if (write) {
-      const SaRow w = sa_row(p, it, r);
-      at = it.slot * nrow + (size_t(w.n) * p.T + w.t) * p.hq + w.head;
-      if (x == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(top * kLn2, a.y * wa + b.y * wb);
+    float wb = 0.f, wa = 1.f;
+    if (MT == 1) {
+      if (x == 1) ml_sh[r] = make_float2(k > 0 ? m : -INFINITY, l);
+      tc_fence_before();
+      named_sync(1, 256);
+      tc_fence_after();
+      const float2 b = ml_sh[r];
+      const float top = fmaxf(m, b.x), ref = top == -INFINITY ? 0.f : top;
+      wa = exp2_approx(m - ref);
+      wb = exp2_approx(b.x - ref);
+      l = l * wa + b.y * wb;
+      m = top;
     }
-    // stream x joins dims [x * HD / 2, (x + 1) * HD / 2)
+    if (MT == 2 || x == 0) {
+      const SaPart at = sa_part<HD>(p, it.own, it.split, it.plane, it.row0 + row);
+      if (write) p.part_ml[at.ml] = make_float2(m * kLn2, l);
 #pragma unroll
-    for (int c = x * (HD / 2); c < (x + 1) * (HD / 2); c += 16) {
-      uint32_t o0[16], o1[16];
-      tc_ld16(trow + C::kTmemO + c, o0);
-      if (nt > 1) tc_ld16(trow + C::kTmemO + HD + c, o1);
-      tc_wait_ld();
-      if (write) {
+      for (int c = 0; c < HD; c += 16) {
+        uint32_t o0[16], o1[16];
+        tc_ld16(to + c, o0);
+        if (MT == 1 && nt > 1) tc_ld16(to + HD + c, o1);
+        tc_wait_ld();
+        if (write) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          float f[4];
+          for (int e = 0; e < 16; e += 4) {
+            float f[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[i] = __uint_as_float(o0[e + i]) * wa;
-            if (nt > 1) f[i] = fmaf(__uint_as_float(o1[e + i]), wb, f[i]);
+            for (int i = 0; i < 4; ++i) {
+              f[i] = __uint_as_float(o0[e + i]) * wa;
+              if (MT == 1 && nt > 1) f[i] = fmaf(__uint_as_float(o1[e + i]), wb, f[i]);
+            }
+            *reinterpret_cast<float4*>(p.part_o + at.o + (c + e) * 32) = make_float4(f[0], f[1], f[2], f[3]);
           }
-          *reinterpret_cast<float4*>(p.part_o + at * HD + c + e) = make_float4(f[0], f[1], f[2], f[3]);
         }
       }
     }
@@ -817,58 +863,81 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   // ---- teardown: copies and MMAs in flight land before the memory goes away
   if (warp == 0 && lane == 0) {
     int never = 0;
-    for (int t = max(0, issued - S); t < issued; ++t) {
-      mbar_wait(kfull + t % S, uint32_t((t / S) & 1), kBudget, &never);
-      mbar_wait(vfull + t % S, uint32_t((t / S) & 1), kBudget, &never);
-    }
+    for (int i = max(0, issued - NB); i < issued; ++i) mbar_wait(full + i % NB, uint32_t((i / NB) & 1), kBudget, &never);
   }
-  if (warp == 1 && lane == 0) {
+  if ((warp == 1 || warp == 2) && lane == 0) {
     int never = 0;
-    tc_commit(&drain);
-    mbar_wait(&drain, 0u, kBudget, &never);
+    tc_commit(drain + warp - 1);
+    mbar_wait(drain + warp - 1, 0u, kBudget, &never);
   }
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort) atomicOr(p.status ? p.status : &g_sa_status, kStatusTimeout);
-  if (warp == 1) {
+  if (warp == 3) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
 // ---------------------------------------------------------------------------
-// Join of the slots: one thread per (row, 4 dims).
+// Join of the key ranges: a CTA takes 32 rows of an own plane, a row a lane
+// and 4 dims a warp and step; the result goes through shared memory so that
+// whole rows are written.
 // ---------------------------------------------------------------------------
 constexpr int kSaJoinThreads = 256;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams p) {
+  constexpr int VE = VecTraits<T>::kElems;
+  __shared__ float res[32][HD + 1];
   pdl_launch();
   pdl_wait();
-  const size_t nrow = size_t(p.G) * p.W * p.T * p.hq;
-  const size_t i = size_t(blockIdx.x) * kSaJoinThreads + threadIdx.x;
-  const size_t row = i / (HD / 4);
-  const int d = int(i - row * (HD / 4)) * 4;
-  if (row >= nrow) return;
-  const int slots = p.sp + p.so;
-  float mx = -INFINITY;
-  for (int s = 0; s < slots; ++s) mx = fmaxf(mx, p.part_ml[(s * nrow + row) * 2]);
-  float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-  for (int s = 0; s < slots; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * nrow + row) * 2);
-    if (ml.x == -INFINITY) continue;
-    const float w = expf(ml.x - mx);
-    den = fmaf(w, ml.y, den);
-    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (s * nrow + row) * HD + d);
-    num[0] = fmaf(w, o.x, num[0]);
-    num[1] = fmaf(w, o.y, num[1]);
-    num[2] = fmaf(w, o.z, num[2]);
-    num[3] = fmaf(w, o.w, num[3]);
-  }
-  const float inv = den > 0.f ? 1.f / den : 0.f;
-  T* dst = static_cast<T*>(p.out) + row * HD + d;
+  const int per = p.hq / p.hkv;
+  const int blk = blockIdx.x % p.oblocks, plane = blockIdx.x / p.oblocks;
+  const int n = plane / p.hkv, kvh = plane - n * p.hkv, gi = n / p.W;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = blk * 32 + lane, rows = p.T * per;
+  if (r < rows) {
+    const int pr = (n - gi * p.W) * rows + r, pplane = gi * p.hkv + kvh;
+    float mx = -INFINITY;
+#pragma unroll 4
+    for (int s = 0; s < p.sp; ++s) mx = fmaxf(mx, p.part_ml[sa_part<HD>(p, false, s, pplane, pr).ml].x);
+#pragma unroll 4
+    for (int s = 0; s < p.so; ++s) mx = fmaxf(mx, p.part_ml[sa_part<HD>(p, true, s, plane, r).ml].x);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    for (int q = warp; q < HD / 4; q += kSaJoinThreads / 32) {
+      float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+      auto add = [&](const SaPart& at) {
+        const float2 ml = p.part_ml[at.ml];
+        const float4 f = *reinterpret_cast<const float4*>(p.part_o + at.o + q * 128);
+        const float w = ml.x == -INFINITY ? 0.f : expf(ml.x - ref);
+        den = fmaf(w, ml.y, den);
+        if (w != 0.f) {  // an empty range leaves its sums unwritten
+          num[0] = fmaf(w, f.x, num[0]);
+          num[1] = fmaf(w, f.y, num[1]);
+          num[2] = fmaf(w, f.z, num[2]);
+          num[3] = fmaf(w, f.w, num[3]);
+        }
+      };
+#pragma unroll 4
+      for (int s = 0; s < p.sp; ++s) add(sa_part<HD>(p, false, s, pplane, pr));
+#pragma unroll 4
+      for (int s = 0; s < p.so; ++s) add(sa_part<HD>(p, true, s, plane, r));
+      const float inv = den > 0.f ? 1.f / den : 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) dst[e] = from_f<T>(num[e] * inv);
+      for (int e = 0; e < 4; ++e) res[lane][4 * q + e] = num[e] * inv;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * (HD / VE); i += kSaJoinThreads) {
+    const int rr = i / (HD / VE), c = (i - rr * (HD / VE)) * VE, row = blk * 32 + rr;
+    if (row >= rows) break;
+    float f[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = res[rr][c + e];
+    const int t = row / per, head = kvh * per + row - t * per;
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + ((size_t(n) * p.T + t) * p.hq + head) * HD + c) = pack_vec(f);
+  }
 }
 
 }  // namespace mtpb

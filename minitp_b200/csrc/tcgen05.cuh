@@ -50,6 +50,16 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* r) {
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// A (M 128, bf16) from tensor memory: row i in lane i, two consecutive values of K a column
+__device__ __forceinline__ void tc_mma_ta(uint32_t tmem, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem),
+      "r"(ta), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // 32 consecutive columns of this thread's tensor-memory lane (no wait)
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* r) {
   tc_ld16(taddr, r);

@@ -58,6 +58,17 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64
   return true;
 }
 
+// The same wait for barriers that usually complete soon: the timer, whose
+// reading takes longer than such a wait, is left alone for the first polls
+// (each of which may itself sleep in hardware).
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, uint64_t budget_ns,
+                                               const volatile int* abort) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, budget_ns, abort);
+}
+
 // 1-D bulk copy global -> this CTA's shared memory, completing on `bar`.
 // dst and src 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
