@@ -336,6 +336,31 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Two fp32 values an instruction (sm_100), and the largest of three.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -593,12 +618,13 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   constexpr int NB = C::kRing;
   constexpr uint64_t kBudget = 2000000000ull;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2], pv_done[2], drain[2];
+  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2], pv_done[2], drain[2],
+      turn[2][4];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_sh;
   __shared__ float2 ml_sh[128];  // MT 1: stream 1's statistics
   volatile int* abort = &abort_sh;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
   pdl_wait();
@@ -624,6 +650,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
       mbar_init(p_full + x, 4);
       mbar_init(pv_done + x, 1);
       mbar_init(drain + x, 1);
+      for (int q = 0; q < 4; ++q) mbar_init(&turn[x][q], 1);
     }
     *abort = 0;
     mbar_init_fence();
@@ -641,70 +668,76 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   int issued = 0;  // warp 0: ring entries whose copies were issued
 
   if (warp == 0) {
-    if (lane == 0) {
-      const CUtensorMap* mk = it.own ? &map_kc : &map_kp;
-      const CUtensorMap* mv = it.own ? &map_vc : &map_vp;
-      for (int i = 0; i < 2 * nt && !*abort; ++i) {  // K and V of each tile in turn
-        const int s = i % NB, j = it.j0 + (i >> 1) * kSaTcKeys;
-        if (i >= NB && !mbar_wait_soon(empty + s, uint32_t((i / NB) & 1) ^ 1u, kBudget, abort)) {
-          *abort = 1;
-          break;
-        }
+    const CUtensorMap* mk = it.own ? &map_kc : &map_kp;
+    const CUtensorMap* mv = it.own ? &map_vc : &map_vp;
+    for (int i = 0; i < 2 * nt; ++i) {  // K and V of each tile in turn
+      const int s = i % NB, j = it.j0 + (i >> 1) * kSaTcKeys;
+      const bool ok = i < NB || mbar_wait_soon(empty + s, uint32_t((i / NB) & 1) ^ 1u, kBudget, abort);
+      if (!__all_sync(0xffffffffu, ok)) {
+        *abort = 1;
+        break;
+      }
+      if (elect_one()) {
         mbar_arrive_expect_tx(full + s, C::kTile);
 #pragma unroll
         for (int b = 0; b < C::kSubs; ++b)
           tma_load_3d(base + C::kOffRing + s * C::kTile + b * kSaTcSub, i & 1 ? mv : mk, b * 64, j, it.plane, full + s);
-        issued = i + 1;
       }
+      issued = i + 1;
     }
   } else if (warp == 1 || warp == 2) {
     // ---- MMA issue of stream x
-    const int x = warp - 1;
-    if (lane == 0) {
-      const int first = MT == 2 ? 0 : x;
-      const uint32_t qb = base + (MT == 2 ? x : 0) * C::kTile;
-      const uint32_t ts = tmem + x * C::kS, to = tmem + C::kO + x * HD, tp = tmem + C::kP + x * C::kPStep;
-      bool ok = first >= nt || mbar_wait_soon(&qfull, 0u, kBudget, abort);
-      auto qk = [&](int t, int k) {
-        const int i = 2 * t, s = i % NB;
-        if (!mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort)) return false;
-        // S is free: read by the softmax, and (aliased) its P read by P V
-        if (k > 0 && !mbar_wait_soon(C::kAlias ? pv_done + x : s_free + x, uint32_t((k - 1) & 1), kBudget, abort)) return false;
-        tc_fence_after();
-        const uint32_t kb = base + C::kOffRing + s * C::kTile;
+    const int x = warp - 1, first = MT == 2 ? 0 : x;
+    const uint64_t dq = tc_smem_desc(base + (MT == 2 ? x : 0) * C::kTile);
+    const uint32_t ts = tmem + x * C::kS, to = tmem + C::kO + x * HD, tp = tmem + C::kP + x * C::kPStep;
+    auto wait = [&](uint64_t* bar, int phase) {
+      return __all_sync(0xffffffffu, mbar_wait_soon(bar, uint32_t(phase & 1), kBudget, abort));
+    };
+    auto qk = [&](int t, int k) {
+      const int i = 2 * t, s = i % NB;
+      // S is free: read by the softmax, and (aliased) its P read by P V
+      if (!wait(full + s, i / NB) || (k > 0 && !wait(C::kAlias ? pv_done + x : s_free + x, k - 1))) return false;
+      tc_fence_after();
+      const uint64_t dk = tc_smem_desc(base + C::kOffRing + s * C::kTile);
+      if (elect_one()) {
 #pragma unroll
-        for (int q = 0; q < HD / 16; ++q)
-          tc_mma(ts, tc_smem_desc(qb + (q >> 2) * kSaTcSub + (q & 3) * 32),
-                 tc_smem_desc(kb + (q >> 2) * kSaTcSub + (q & 3) * 32), C::kIdescS, q > 0 ? 1u : 0u);
+        for (int q = 0; q < HD / 16; ++q) {
+          const uint32_t off = ((q >> 2) * kSaTcSub + (q & 3) * 32) >> 4;
+          tc_mma(ts, dq + off, dk + off, C::kIdescS, q > 0 ? 1u : 0u);
+        }
         tc_commit(s_full + x);
         tc_commit(empty + s);
-        return true;
-      };
-      auto pv = [&](int t, int k) {
-        const int i = 2 * t + 1, s = i % NB;
-        if (!mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort) ||
-            !mbar_wait_soon(p_full + x, uint32_t(k & 1), kBudget, abort))
-          return false;
-        tc_fence_after();
-        const uint32_t vb = base + C::kOffRing + s * C::kTile;
+      }
+      __syncwarp();
+      return true;
+    };
+    auto pv = [&](int t, int k) {
+      const int i = 2 * t + 1, s = i % NB;
+      if (!wait(full + s, i / NB) || !wait(p_full + x, k)) return false;
+      tc_fence_after();
+      const uint64_t dv = tc_smem_desc_mn(base + C::kOffRing + s * C::kTile, kSaTcSub);
+      const uint32_t acc = k > 0 ? 1u : 0u;
+      if (elect_one()) {
 #pragma unroll
         for (int q = 0; q < kSaTcKeys / 16; ++q)
-          tc_mma_ta(to, tp + q * 8, tc_smem_desc_mn(vb + q * 2048, kSaTcSub), C::kIdescO, (k > 0 || q > 0) ? 1u : 0u);
+          tc_mma_ta(to, tp + q * 8, dv + ((q * 2048) >> 4), C::kIdescO, q > 0 ? 1u : acc);
         tc_commit(pv_done + x);
         tc_commit(empty + s);
-        return true;
-      };
-      if (C::kAlias) {
-        for (int t = first, k = 0; ok && t < nt; t += kStep, ++k) ok = qk(t, k) && pv(t, k);
-      } else {  // the next S under this one's softmax
-        if (ok && first < nt) ok = qk(first, 0);
-        for (int t = first, k = 0; ok && t < nt; t += kStep, ++k) {
-          if (t + kStep < nt) ok = qk(t + kStep, k + 1);
-          ok = ok && pv(t, k);
-        }
       }
-      if (!ok) *abort = 1;
+      __syncwarp();
+      return true;
+    };
+    bool ok = first >= nt || wait(&qfull, 0);
+    if (C::kAlias) {
+      for (int t = first, k = 0; ok && t < nt; t += kStep, ++k) ok = qk(t, k) && pv(t, k);
+    } else {  // the next S under this one's softmax
+      if (ok && first < nt) ok = qk(first, 0);
+      for (int t = first, k = 0; ok && t < nt; t += kStep, ++k) {
+        if (t + kStep < nt) ok = qk(t + kStep, k + 1);
+        ok = ok && pv(t, k);
+      }
     }
+    if (!ok) *abort = 1;
   } else if (warp >= 4) {
     // ---- softmax of stream x
     const int stid = int(threadIdx.x) - 128, x = stid >> 7;
@@ -761,8 +794,12 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
       }
       float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
-      for (int c = 4; c < kSaTcKeys; ++c) mx[c & 3] = fmaxf(mx[c & 3], sc[c]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+      for (int c = 4; c < kSaTcKeys - 4; c += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], sc[c + i], sc[c + 4 + i]);
+      mx[0] = max3(mx[0], sc[124], sc[125]);
+      mx[1] = max3(mx[1], sc[126], sc[127]);
+      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl2;
       const bool grow = top > m + 8.f;
       if (!C::kAlias && k > 0) {  // the stream's previous P V has read P (aliased: it came before this S)
         ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
@@ -786,20 +823,30 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
         }
       }
       const float ref = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      // the exponentials of the two warps of a scheduler take turns: one
+      // stream's run under the other's MMAs, and not both at half pace
+      if (x == 1 || k > 0) {
+        ok = mbar_wait_soon(&turn[x][quarter], uint32_t(x == 1 ? k & 1 : (k - 1) & 1), kBudget, abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < kSaTcKeys; c += 32) {
         uint32_t pk[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          const float e0 = exp2_approx(fmaf(sc[c + i], sl2, -ref)), e1 = exp2_approx(fmaf(sc[c + i + 1], sl2, -ref));
-          sum[i & 2] += e0;
-          sum[(i & 2) + 1] += e1;
-          pk[i / 2] = pack_bf16(e0, e1);
+          float2 e = fma2(make_float2(sc[c + i], sc[c + i + 1]), make_float2(sl2, sl2), make_float2(-ref, -ref));
+          e.x = exp2_approx(e.x);
+          e.y = exp2_approx(e.y);
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+          pk[i / 2] = pack_bf16(e.x, e.y);
         }
         tc_st16(tp + c / 2, pk);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&turn[1 - x][quarter]);
+      sum[0] = add2(sum[0], sum[1]);
+      l += sum[0].x + sum[0].y;
       if (j + kSaTcKeys > it.j1) {  // the last tile: V rows behind the range (MT 2: both streams write the same zeros)
         const int i = 2 * t + 1, s = i % NB;
         ok = mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort);
@@ -861,13 +908,16 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   }
   __syncwarp();
   // ---- teardown: copies and MMAs in flight land before the memory goes away
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     int never = 0;
     for (int i = max(0, issued - NB); i < issued; ++i) mbar_wait(full + i % NB, uint32_t((i / NB) & 1), kBudget, &never);
   }
-  if ((warp == 1 || warp == 2) && lane == 0) {
+  if (warp == 1 || warp == 2) {
+    // behind every MMA of the warp (a commit follows those of its own thread:
+    // the elected lane is the same each time)
     int never = 0;
-    tc_commit(drain + warp - 1);
+    if (elect_one()) tc_commit(drain + warp - 1);
+    __syncwarp();
     mbar_wait(drain + warp - 1, 0u, kBudget, &never);
   }
   tc_fence_before();

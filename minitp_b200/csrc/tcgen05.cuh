@@ -50,6 +50,16 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* r) {
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// True in one lane of a converged warp. The compiler knows that a branch on it
+// holds one thread: behind it an MMA (its operands are uniform registers) issues
+// every 64 cycles, the rate of the tensor cores at N 128; behind `lane == 0` it
+// took 182 cycles, whatever the shape (64 to 256 MMAs timed in a row).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // A (M 128, bf16) from tensor memory: row i in lane i, two consecutive values of K a column
 __device__ __forceinline__ void tc_mma_ta(uint32_t tmem, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
