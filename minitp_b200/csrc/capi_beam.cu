@@ -210,7 +210,6 @@ struct SaPlan {
   bool inline_pre;  // it reads the prefix too: no other launch
   bool tc;          // the other items on sa_tc_kernel, else on the CUDA cores
   int mt;           // its row tiles a CTA
-  int warps;
   int rpt;  // CUDA-core items: rows a tile / 16
   int sp, so, ptiles, otiles;
   int pblocks, oblocks;
@@ -225,7 +224,7 @@ int sa_tc_splits(long long base, int top, size_t rows, int hd, int sms) {
   const int tiles = std::max(1, (top + kSaTcKeys - 1) / kSaTcKeys);
   int best = 1;
   double least = 0;
-  for (int s = 1; s <= std::min(tiles, 64); ++s) {
+  for (int s = 1; s <= std::min(tiles, kSaMaxSplits); ++s) {
     const double waves = double((base * s + sms - 1) / sms);
     const double us = waves * (0.7 * ((tiles + s - 1) / s) + 2.8) + double(rows) * s * hd * 8 / 4e6;
     if (s == 1 || us < least) {
@@ -265,14 +264,13 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   // key ranges until the items give every SM four, but none below two key tiles
   auto splits = [&](long long base, int top) {
     const long long most = std::max(1, (top + 2 * kSaKT - 1) / (2 * kSaKT)), want = 4ll * sms;
-    return int(std::max<long long>(1, std::min<long long>(std::min<long long>(most, 64), (want + base - 1) / base)));
+    return int(std::max<long long>(1, std::min<long long>(std::min<long long>(most, kSaMaxSplits), (want + base - 1) / base)));
   };
   if (pl.token) {
     // the prefix read by every row's CTA: one launch, but N / G reads of each
     // position, through L2, and one CTA's pace along it
     const long long pre = (long long)top_p * a.hd * 4;
     pl.inline_pre = pre <= (256 << 10) && obase * pre <= (32ll << 20);
-    pl.warps = 4;
     pl.so = 1;
     if (!pl.inline_pre)
       while (obase * pl.so * 2 <= 2 * sms && top_o / (pl.so * 2) >= 256 && pl.so < 64) pl.so *= 2;
@@ -323,14 +321,12 @@ int sa_launch_tc(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
                     : host_launch(sa_tc_kernel<HD, 1>, grid, block, SaTcCfg<HD, 1>::kSmem, st, p, m[0], m[1], m[2], m[3]);
 }
 
-template <int HD, int NW>
+template <int HD>
 int sa_launch_token(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
-  const dim3 grid(unsigned(p.hkv * pl.otiles), unsigned(p.G * p.W), unsigned(pl.so));
-  const bool wide = p.hq / p.hkv > 8;
-  return wide ? host_launch(sa_token_kernel<HD, NW, true>, grid, dim3(32 * NW), sa_token_smem<HD, NW, true>(), st, p,
-                            int(pl.inline_pre))
-              : host_launch(sa_token_kernel<HD, NW, false>, grid, dim3(32 * NW), sa_token_smem<HD, NW, false>(), st, p,
-                            int(pl.inline_pre));
+  const dim3 grid(unsigned(p.hkv * pl.otiles), unsigned(p.G * p.W), unsigned(pl.so)), block(32 * kSaTokenWarps);
+  const int inl = pl.inline_pre;
+  return p.hq / p.hkv > 8 ? host_launch(sa_token_kernel<HD, true>, grid, block, sa_token_smem<HD, true>(), st, p, inl)
+                          : host_launch(sa_token_kernel<HD, false>, grid, block, sa_token_smem<HD, false>(), st, p, inl);
 }
 
 template <typename T, int HD>
@@ -352,9 +348,7 @@ int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
   }
   if constexpr (sizeof(T) == 2 && HD >= 64) {
     if (pl.token) {
-      const int r = pl.warps == 4   ? sa_launch_token<HD, 4>(pl, p, st)
-                    : pl.warps == 8 ? sa_launch_token<HD, 8>(pl, p, st)
-                                    : sa_launch_token<HD, 16>(pl, p, st);
+      const int r = sa_launch_token<HD>(pl, p, st);
       if (r != MTPB_OK || pl.so == 1) return r;
     }
   }

@@ -12,6 +12,8 @@
 // denominator (a slot per key range), and a second kernel joins the slots.
 #pragma once
 
+#include <type_traits>
+
 #include "tcgen05.cuh"
 
 namespace mtpb {
@@ -39,6 +41,7 @@ struct SaParams {
 
 // Error bits of calls without a communicator's status word.
 __device__ uint32_t g_sa_status;
+
 
 __device__ __forceinline__ int sa_prefix_len(const SaParams& p, int g) {
   const int n = p.plen ? p.plen[g] : p.plen_all;
@@ -300,10 +303,13 @@ __global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
 // ---------------------------------------------------------------------------
 // One token a row, bf16, head dim 64 or 128: a CTA takes up to 16 query heads
 // of one (row, KV head) and streams the row's own cache (and, inline, the
-// prefix) from global memory straight into mma.sync fragments: 16 rows (heads)
-// x 16 keys a warp and step, the warps on every NW-th block of 16 keys. A
-// K or V byte is used once, so the kernel is bound by the loads, and the
-// 16-row tensor instructions cost less than unpacking to fp32 would.
+// prefix) from global memory straight into mma.sync fragments, 16 keys a warp
+// and step, the warps on every NW-th block of 16 keys. A K or V byte is used
+// once, so the kernel is bound by the loads (a block's are in flight under the
+// arithmetic of the one before), and the tensor instructions cost less than
+// unpacking to fp32 would. S = Q K^T has 16 rows (heads, half of them unused
+// below 9), O^T = V^T P^T has 8 or 16 columns (heads): the registers of P, a
+// result of the first, are as they stand the B operand of the second.
 //
 // Fragments without shared memory: the dot product's order of dims and the
 // output's order of dims are free, so both are chosen to make every load 16
@@ -311,7 +317,7 @@ __global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
 // key g (K) or head g (Q): four register pairs that serve as the "k" and
 // "k + 8" halves of two steps. For V it loads keys 2c, 2c+1, 2c+8, 2c+9 at
 // dims 64 b + 8 g .. + 7; two keys' values of a dim, put together by a byte
-// permute, are the operand of column g of output tile i = dim % 8.
+// permute, are an operand of row g of an output tile.
 //
 // Probabilities are rounded to bf16 for the second product (the sums of the
 // denominator are not): half a step of bf16 of each term, as the result's own
@@ -361,20 +367,43 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// 2^x of two values on the fp32 pipe: x = n + f with n the nearest integer
+// (read off the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by the cubic
+// of least relative error there (7.5e-5 by the Remez exchange, a fiftieth of
+// bf16's half step), n added to the exponent. For x <= 126; below -125 the
+// result is 2^-125.
+__device__ __forceinline__ float2 exp2_cubic(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
+  x.x = fmaxf(x.x, -125.f);
+  x.y = fmaxf(x.y, -125.f);
+  const float2 r = add2(x, magic);
+  const float2 f = fma2(add2(r, back), make_float2(-1.f, -1.f), x);
+  float2 q = fma2(f, make_float2(0.0551716685295105f, 0.0551716685295105f),
+                  make_float2(0.2426111251115799f, 0.2426111251115799f));
+  q = fma2(q, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
+  q = fma2(q, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
+  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(r.x) << 23)),
+                     __int_as_float(__float_as_int(q.y) + (__float_as_int(r.y) << 23)));
+}
+
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
-// NW warps; WIDE: more than 8 heads a tile (rows 8..15 in use).
-template <int HD, int NW, bool WIDE>
+constexpr int kSaTokenWarps = 4;  // 8 took 57.5 us where 4 took 55.8 (64 rows of the 7B heads behind 16384 positions)
+constexpr int kSaMaxSplits = 64;  // key ranges of a prefix
+
+// WIDE: more than 8 heads a tile (rows 8..15 in use).
+template <int HD, bool WIDE>
 __host__ __device__ constexpr size_t sa_token_smem() {
-  return size_t(NW) * (WIDE ? 16 : 8) * (HD + 2) * sizeof(float);
+  return size_t(kSaTokenWarps) * (WIDE ? 16 : 8) * (HD + 2) * sizeof(float);
 }
 
-template <int HD, int NW, bool WIDE>
-__global__ void __launch_bounds__(32 * NW) sa_token_kernel(const SaParams p, const int inline_prefix) {  // inline_prefix: so == 1, no prefix items
-  constexpr int R = WIDE ? 16 : 8;
-  constexpr int JB = HD / 32, VB = HD / 64;
+template <int HD, bool WIDE>
+__global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const SaParams p, const int inline_prefix) {  // inline_prefix: so == 1, no prefix items
+  constexpr int NT = WIDE ? 2 : 1, R = 8 * NT;
+  constexpr int JB = HD / 32, VB = HD / 64, NW = kSaTokenWarps;
   extern __shared__ __align__(16) float smf[];
+  __shared__ float2 pml[kSaMaxSplits * R];  // max and sum of the prefix's key ranges
   float* so = smf;                  // [NW][R][HD]
   float* sml = so + NW * R * HD;    // [NW][R][2]
   // the kernel of the prefix items, if one runs before this, has waited for
@@ -403,15 +432,23 @@ __global__ void __launch_bounds__(32 * NW) sa_token_kernel(const SaParams p, con
     }
   }
   const float sl2 = p.scale * kLog2e;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // max (scaled, base 2) and this thread's part of the sum
-  float o[VB * 8][4];
+  float m[NT], l[NT];  // of heads g and g + 8: max (scaled, base 2), this thread's part of the sum
+  float o[NT][VB * 4][4];  // dims x heads: [head half][64 v + 8 g + 2 w + row half][head 2c, 2c + 1]
 #pragma unroll
-  for (int i = 0; i < VB * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int h = 0; h < NT; ++h) {
+    m[h] = -INFINITY;
+    l[h] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VB * 4; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
+  }
   const int nb0 = (plen + 15) / 16, nb = nb0 + (own1 - own0 + 15) / 16;
-  for (int b = warp; b < nb; b += NW) {
+  struct Block {
+    uint4 k[2][JB], v[4][VB];
+  };
+  auto load = [&](Block& f, int b) {
+    if (b >= nb) return;
     const bool own = b >= nb0;
     const int key0 = own ? own0 + (b - nb0) * 16 : b * 16, end = own ? own1 : plen;
-    uint4 kf[2][JB], vf[4][VB];
     const size_t at = (own ? co : po) + size_t(key0) * HD;
     const bf16* kp = static_cast<const bf16*>(own ? p.kc : p.kp) + at + c * 8;
     const bf16* vp = static_cast<const bf16*>(own ? p.vc : p.vp) + at + g * 8;
@@ -419,121 +456,122 @@ __global__ void __launch_bounds__(32 * NW) sa_token_kernel(const SaParams p, con
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int j = 0; j < JB; ++j)
-        kf[t][j] = key0 + 8 * t + g < end ? ld_stream(kp + size_t(8 * t + g) * HD + 32 * j) : make_uint4(0, 0, 0, 0);
+        f.k[t][j] = key0 + 8 * t + g < end ? ld_stream(kp + size_t(8 * t + g) * HD + 32 * j) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int k = 2 * c + (r & 1) + (r >> 1) * 8;
 #pragma unroll
       for (int v = 0; v < VB; ++v)
-        vf[r][v] = key0 + k < end ? ld_stream(vp + size_t(k) * HD + 64 * v) : make_uint4(0, 0, 0, 0);
+        f.v[r][v] = key0 + k < end ? ld_stream(vp + size_t(k) * HD + 64 * v) : make_uint4(0, 0, 0, 0);
     }
+  };
+  auto step = [&](const Block& f, int b) {
+    const bool own = b >= nb0;
+    const int key0 = own ? own0 + (b - nb0) * 16 : b * 16, end = own ? own1 : plen;
     float s[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < JB; ++j) {
-        mma_bf16(s[t], q0[j].x, q1[j].x, q0[j].y, q1[j].y, kf[t][j].x, kf[t][j].y);
-        mma_bf16(s[t], q0[j].z, q1[j].z, q0[j].w, q1[j].w, kf[t][j].z, kf[t][j].w);
+        mma_bf16(s[t], q0[j].x, q1[j].x, q0[j].y, q1[j].y, f.k[t][j].x, f.k[t][j].y);
+        mma_bf16(s[t], q0[j].z, q1[j].z, q0[j].w, q1[j].w, f.k[t][j].z, f.k[t][j].w);
       }
     }
-    float x0 = -INFINITY, x1 = -INFINITY;
+    float x[NT];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int h = 0; h < NT; ++h) {
+      x[h] = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bool in = key0 + 8 * t + 2 * c + e < end;
-        s[t][e] = in ? s[t][e] * sl2 : -INFINITY;
-        x0 = fmaxf(x0, s[t][e]);
-        if (WIDE) {
-          s[t][2 + e] = in ? s[t][2 + e] * sl2 : -INFINITY;
-          x1 = fmaxf(x1, s[t][2 + e]);
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[t][2 * h + e] = key0 + 8 * t + 2 * c + e < end ? s[t][2 * h + e] * sl2 : -INFINITY;
+          x[h] = fmaxf(x[h], s[t][2 * h + e]);
         }
-      }
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-      if (WIDE) x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+      x[h] = fmaxf(x[h], __shfl_xor_sync(0xffffffffu, x[h], 1));
+      x[h] = fmaxf(x[h], __shfl_xor_sync(0xffffffffu, x[h], 2));
     }
-    // the block's first key is inside the range: the new maxima are not -inf
-    // (but for a key whose score is: then the row keeps exp(-inf - 0) = 0)
-    if (__any_sync(0xffffffffu, x0 > m0 || (WIDE && x1 > m1))) {
-      const float n0 = fmaxf(m0, x0), a0 = exp2_approx(m0 - (n0 == -INFINITY ? 0.f : n0));
-      const float n1 = fmaxf(m1, x1), a1 = WIDE ? exp2_approx(m1 - (n1 == -INFINITY ? 0.f : n1)) : 1.f;
-      m0 = n0;
-      l0 *= a0;
-      m1 = n1;
-      l1 *= a1;
+    // (a row of scores that are all -inf keeps its max: exp(-inf - 0) = 0)
+    if (__any_sync(0xffffffffu, x[0] > m[0] || x[NT - 1] > m[NT - 1])) {
 #pragma unroll
-      for (int i = 0; i < VB * 8; ++i) {
-        o[i][0] *= a0;
-        o[i][1] *= a0;
-        if (WIDE) {
-          o[i][2] *= a1;
-          o[i][3] *= a1;
+      for (int h = 0; h < NT; ++h) {
+        const float top = fmaxf(m[h], x[h]), a = exp2_approx(m[h] - (top == -INFINITY ? 0.f : top));
+        m[h] = top;
+        l[h] *= a;
+        const float a0 = __shfl_sync(0xffffffffu, a, 8 * c), a1 = __shfl_sync(0xffffffffu, a, 8 * c + 4);
+#pragma unroll
+        for (int i = 0; i < VB * 4; ++i) {
+          o[h][i][0] *= a0;
+          o[h][i][1] *= a1;
+          o[h][i][2] *= a0;
+          o[h][i][3] *= a1;
         }
       }
     }
-    const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-    uint32_t pa[2][2];  // [key half][row half]
+    uint32_t pb[NT][2];  // [head half][key half]
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float e0 = exp2_approx(s[t][0] - r0), e1 = exp2_approx(s[t][1] - r0);
-      l0 += e0 + e1;
-      pa[t][0] = pack_bf16(e0, e1);
-      pa[t][1] = 0;
-      if (WIDE) {
-        const float e2 = exp2_approx(s[t][2] - r1), e3 = exp2_approx(s[t][3] - r1);
-        l1 += e2 + e3;
-        pa[t][1] = pack_bf16(e2, e3);
+    for (int h = 0; h < NT; ++h) {
+      const float ref = m[h] == -INFINITY ? 0.f : m[h];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float e0 = exp2_approx(s[t][2 * h] - ref), e1 = exp2_approx(s[t][2 * h + 1] - ref);
+        l[h] += e0 + e1;
+        pb[h][t] = pack_bf16(e0, e1);
       }
     }
 #pragma unroll
     for (int v = 0; v < VB; ++v) {
-      const uint32_t* k0 = reinterpret_cast<const uint32_t*>(&vf[0][v]);
-      const uint32_t* k1 = reinterpret_cast<const uint32_t*>(&vf[1][v]);
-      const uint32_t* k8 = reinterpret_cast<const uint32_t*>(&vf[2][v]);
-      const uint32_t* k9 = reinterpret_cast<const uint32_t*>(&vf[3][v]);
+      const uint32_t* k0 = reinterpret_cast<const uint32_t*>(&f.v[0][v]);
+      const uint32_t* k1 = reinterpret_cast<const uint32_t*>(&f.v[1][v]);
+      const uint32_t* k8 = reinterpret_cast<const uint32_t*>(&f.v[2][v]);
+      const uint32_t* k9 = reinterpret_cast<const uint32_t*>(&f.v[3][v]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;  // upper or lower halves of two words
-        mma_bf16(o[v * 8 + i], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(k0[i / 2], k1[i / 2], sel),
-                 __byte_perm(k8[i / 2], k9[i / 2], sel));
+      for (int w = 0; w < 4; ++w) {  // lower and upper halves of the two keys' words: dims 2w and 2w + 1
+        const uint32_t a0 = __byte_perm(k0[w], k1[w], 0x5410u), a1 = __byte_perm(k0[w], k1[w], 0x7632u);
+        const uint32_t a2 = __byte_perm(k8[w], k9[w], 0x5410u), a3 = __byte_perm(k8[w], k9[w], 0x7632u);
+#pragma unroll
+        for (int h = 0; h < NT; ++h) mma_bf16(o[h][v * 4 + w], a0, a1, a2, a3, pb[h][0], pb[h][1]);
       }
     }
+  };
+  // the next block's loads are in flight under this one's arithmetic
+  Block f0, f1;
+  load(f0, warp);
+  for (int b = warp; b < nb; b += 2 * NW) {
+    load(f1, b + NW);
+    step(f0, b);
+    if (b + NW >= nb) break;
+    load(f0, b + 2 * NW);
+    step(f1, b + NW);
   }
 #pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-    if (WIDE) l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+  for (int h = 0; h < NT; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    if (c == 0) *reinterpret_cast<float2*>(sml + (warp * R + g + 8 * h) * 2) = make_float2(m[h] * kLn2, l[h]);
+#pragma unroll
+    for (int v = 0; v < VB; ++v)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float2*>(so + (warp * R + 8 * h + 2 * c + e) * HD + 64 * v + 8 * g + 2 * w) =
+              make_float2(o[h][v * 4 + w][e], o[h][v * 4 + w][2 + e]);
   }
-  if (c == 0) {
-    *reinterpret_cast<float2*>(sml + (warp * R + g) * 2) = make_float2(m0 * kLn2, l0);
-    if (WIDE) *reinterpret_cast<float2*>(sml + (warp * R + g + 8) * 2) = make_float2(m1 * kLn2, l1);
-  }
-#pragma unroll
-  for (int v = 0; v < VB; ++v)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int d = 64 * v + 8 * (2 * c + e) + i;
-        so[(warp * R + g) * HD + d] = o[v * 8 + i][e];
-        if (WIDE) so[(warp * R + g + 8) * HD + d] = o[v * 8 + i][2 + e];
-      }
-  __syncthreads();
   if (!inline_prefix) pdl_wait();  // the prefix items' partial sums
   const bool last = p.so == 1;  // else partial sums for the join
   const int pslots = last && !inline_prefix ? p.sp : 0;
+  const int pplane = gi * p.hkv + kvh, pr0 = (n - gi * p.W) * per + tile * 16;  // this tile's first row of the prefix plane
+  for (int i = threadIdx.x; i < pslots * R; i += 32 * NW)
+    if (i % R < rows) pml[i] = __ldcg(p.part_ml + sa_part<HD>(p, false, i / R, pplane, pr0 + i % R).ml);
+  __syncthreads();
   for (int i = threadIdx.x; i < rows * (HD / 4); i += 32 * NW) {
     const int q = i / rows, r = i - q * rows;
-    const int pr = (n - gi * p.W) * per + tile * 16 + r;  // row of the prefix plane
     float mx = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sml[(w * R + r) * 2]);
-#pragma unroll 4
-    for (int s = 0; s < pslots; ++s)
-      mx = fmaxf(mx, __ldcg(p.part_ml + sa_part<HD>(p, false, s, gi * p.hkv + kvh, pr).ml).x);
+    for (int s = 0; s < pslots; ++s) mx = fmaxf(mx, pml[s * R + r].x);
     const float ref = mx == -INFINITY ? 0.f : mx;
     float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
     auto add = [&](float m, float l, const float4& f) {
@@ -549,11 +587,16 @@ __global__ void __launch_bounds__(32 * NW) sa_token_kernel(const SaParams p, con
 #pragma unroll
     for (int w = 0; w < NW; ++w)
       add(sml[(w * R + r) * 2], sml[(w * R + r) * 2 + 1], *reinterpret_cast<const float4*>(so + (w * R + r) * HD + 4 * q));
-#pragma unroll 4
-    for (int s = 0; s < pslots; ++s) {
-      const SaPart at = sa_part<HD>(p, false, s, gi * p.hkv + kvh, pr);
-      const float2 ml = __ldcg(p.part_ml + at.ml);
-      add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part_o + at.o + q * 128)));
+    constexpr int U = 8;  // ranges whose sums are loaded together
+    for (int s0 = 0; s0 < pslots; s0 += U) {
+      float4 f[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s0 + u < pslots)
+          f[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + sa_part<HD>(p, false, s0 + u, pplane, pr0 + r).o + q * 128));
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s0 + u < pslots) add(pml[(s0 + u) * R + r].x, pml[(s0 + u) * R + r].y, f[u]);
     }
     if (last) {
       const float inv = den > 0.f ? 1.f / den : 0.f;
@@ -590,6 +633,8 @@ __global__ void __launch_bounds__(32 * NW) sa_token_kernel(const SaParams p, con
 // zeroed in shared memory, since 0 x NaN would not be 0.
 // ---------------------------------------------------------------------------
 constexpr int kSaTcKeys = 128;
+constexpr int kSaCubic = 4;  // of 16 pairs of exponentials, on the fp32 pipe (0: 54.2, 4: 52.9, 6: 55.0, 8: 60.1 us on
+                             // 64 rows of the 7B heads behind 16384 positions; 72, 69, 76, 76 us on 16 rows of 128 tokens)
 constexpr int kSaTcThreads = 384;
 constexpr uint32_t kSaTcSub = 128 * 64 * 2;  // a 128 x 64 bf16 subtile
 
@@ -618,8 +663,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   constexpr int NB = C::kRing;
   constexpr uint64_t kBudget = 2000000000ull;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2], pv_done[2], drain[2],
-      turn[2][4];
+  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2][2], pv_done[2], drain[2];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_sh;
   __shared__ float2 ml_sh[128];  // MT 1: stream 1's statistics
@@ -628,6 +672,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
   pdl_wait();
+
   pdl_launch();  // after the wait: sa_token_kernel counts on it
   const SaItem it = sa_item<HD, 2>(p, blockIdx.x, 128 * MT, kSaTcKeys);
   if (it.j0 >= it.j1) {
@@ -647,10 +692,9 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
     for (int x = 0; x < 2; ++x) {
       mbar_init(s_full + x, 1);
       mbar_init(s_free + x, 4);
-      mbar_init(p_full + x, 4);
+      for (int h = 0; h < 2; ++h) mbar_init(&p_full[x][h], 4);
       mbar_init(pv_done + x, 1);
       mbar_init(drain + x, 1);
-      for (int q = 0; q < 4; ++q) mbar_init(&turn[x][q], 1);
     }
     *abort = 0;
     mbar_init_fence();
@@ -713,18 +757,24 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
     };
     auto pv = [&](int t, int k) {
       const int i = 2 * t + 1, s = i % NB;
-      if (!wait(full + s, i / NB) || !wait(p_full + x, k)) return false;
-      tc_fence_after();
+      if (!wait(full + s, i / NB)) return false;
       const uint64_t dv = tc_smem_desc_mn(base + C::kOffRing + s * C::kTile, kSaTcSub);
-      const uint32_t acc = k > 0 ? 1u : 0u;
-      if (elect_one()) {
 #pragma unroll
-        for (int q = 0; q < kSaTcKeys / 16; ++q)
-          tc_mma_ta(to, tp + q * 8, dv + ((q * 2048) >> 4), C::kIdescO, q > 0 ? 1u : acc);
-        tc_commit(pv_done + x);
-        tc_commit(empty + s);
+      for (int h = 0; h < 2; ++h) {  // the first half of the keys under the second half's exponentials
+        if (!wait(&p_full[x][h], k)) return false;
+        tc_fence_after();
+        const uint32_t acc = h > 0 || k > 0 ? 1u : 0u;
+        if (elect_one()) {
+#pragma unroll
+          for (int q = 4 * h; q < 4 * h + 4; ++q)
+            tc_mma_ta(to, tp + q * 8, dv + ((q * 2048) >> 4), C::kIdescO, q > 4 * h ? 1u : acc);
+          if (h == 1) {
+            tc_commit(pv_done + x);
+            tc_commit(empty + s);
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
       return true;
     };
     bool ok = first >= nt || wait(&qfull, 0);
@@ -788,7 +838,8 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free + x);
       }
-      if (__any_sync(0xffffffffu, j + kSaTcKeys > lim)) {
+      const bool masked = __any_sync(0xffffffffu, j + kSaTcKeys > lim);
+      if (masked) {
 #pragma unroll
         for (int c = 0; c < kSaTcKeys; ++c) sc[c] = j + c < lim ? sc[c] : -INFINITY;
       }
@@ -823,30 +874,6 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
         }
       }
       const float ref = m == -INFINITY ? 0.f : m;
-      // the exponentials of the two warps of a scheduler take turns: one
-      // stream's run under the other's MMAs, and not both at half pace
-      if (x == 1 || k > 0) {
-        ok = mbar_wait_soon(&turn[x][quarter], uint32_t(x == 1 ? k & 1 : (k - 1) & 1), kBudget, abort);
-        if (!__all_sync(0xffffffffu, ok)) break;
-      }
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int c = 0; c < kSaTcKeys; c += 32) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float2 e = fma2(make_float2(sc[c + i], sc[c + i + 1]), make_float2(sl2, sl2), make_float2(-ref, -ref));
-          e.x = exp2_approx(e.x);
-          e.y = exp2_approx(e.y);
-          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
-          pk[i / 2] = pack_bf16(e.x, e.y);
-        }
-        tc_st16(tp + c / 2, pk);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&turn[1 - x][quarter]);
-      sum[0] = add2(sum[0], sum[1]);
-      l += sum[0].x + sum[0].y;
       if (j + kSaTcKeys > it.j1) {  // the last tile: V rows behind the range (MT 2: both streams write the same zeros)
         const int i = 2 * t + 1, s = i % NB;
         ok = mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort);
@@ -861,10 +888,41 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
         }
         fence_async_smem();
       }
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + x);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      // kCubic of 16 pairs on the fp32 pipe, which the special-function unit
+      // (8 cycles a warp and value) leaves idle; masked tiles need exact zeros
+      auto exps = [&](auto cubic) {
+        constexpr int kCubic = decltype(cubic)::value;
+#pragma unroll
+        for (int c = 0; c < kSaTcKeys; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float2 e = fma2(make_float2(sc[c + i], sc[c + i + 1]), make_float2(sl2, sl2), make_float2(-ref, -ref));
+            if ((i >> 1) * kCubic % 16 < kCubic) {
+              e = exp2_cubic(e);
+            } else {
+              e.x = exp2_approx(e.x);
+              e.y = exp2_approx(e.y);
+            }
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+            pk[i / 2] = pack_bf16(e.x, e.y);
+          }
+          tc_st16(tp + c / 2, pk);
+          if (c & 32) {  // half of the keys
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[x][c >> 6]);
+          }
+        }
+      };
+      if (masked)
+        exps(std::integral_constant<int, 0>{});
+      else
+        exps(std::integral_constant<int, kSaCubic>{});
+      sum[0] = add2(sum[0], sum[1]);
+      l += sum[0].x + sum[0].y;
     }
     if (ok && k > 0) ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
     if (!ok) *abort = 1;
@@ -922,6 +980,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+
   if (threadIdx.x == 0 && *abort) atomicOr(p.status ? p.status : &g_sa_status, kStatusTimeout);
   if (warp == 3) {
     tc_fence_after();
