@@ -245,7 +245,7 @@ int mtpb_argmax(void* comm, const void* logits, int M, int V_local, int64_t ld, 
  *     candidate, token `eos` at the beam's own score; its logits are not read.
  *     out_finished = finished[parent] or token == eos. eos < 0: no end token.
  *   - A beam whose score is -inf or NaN, or without a logit above -inf, has
- *     no candidate. Places without a candidate get score -inf, parent 0 and
+ *     no candidate, and neither is a total below the range of fp32 one. Places without a candidate get score -inf, parent 0 and
  *     token eos (0 without one).
  * `block`: workspace of mtpb_beam_block_bytes(G*W, V, k) bytes, 16-byte
  * aligned, private to the call until it has run. */

@@ -10,21 +10,28 @@
 // whose score is -inf or NaN, or whose logits are all -inf, has none.
 //
 // Inside one row the order of totals is the order of the logits, so the
-// vocabulary is cut into chunks: one CTA per (row, chunk) finds the chunk's
-// max, sum and k best logits (packed keys: value, then lower id), and one CTA
-// per prompt merges the chunks of all its beams.
+// vocabulary is cut into chunks: one CTA per (row, chunk) reduces its columns
+// in one pass to the sum and the k best logits (packed keys: value, then lower
+// id), and one CTA per prompt merges the chunks of all its beams.
 #pragma once
 
-#include "common.cuh"
+#include "tma.cuh"
 
 namespace mtpb {
 
 constexpr int kBeamMaxK = 64;
 constexpr int kBeamMaxW = 64;
 
+// Sum of a chunk's exponentials, s = sum 2^(x log2(e) - beam_ref(m)). m need
+// not be the maximum: it keeps s in range. -inf: nothing summed. Where m is
+// 10^30 or more (an infinity, a mask of the type's lowest value), neighbours of
+// m are further off than any exponential reaches: s counts the values equal to m.
 struct BeamStat {
-  float m, s;  // max of the chunk's logits and sum of exp(x - m)
+  float m, s;
 };
+constexpr float kBeamLog2e = 1.44269504088896340736f;
+__device__ __forceinline__ float beam_ref(float m) { return __fmul_rn(m, kBeamLog2e); }
+__device__ __forceinline__ bool beam_far(float m) { return !(fabsf(m) < 1e30f); }
 
 // Order-preserving key of a finite or +inf logit and its id; 0: no candidate.
 __device__ __forceinline__ uint32_t beam_val_key(float v) {
@@ -34,23 +41,25 @@ __device__ __forceinline__ uint32_t beam_val_key(float v) {
 __device__ __forceinline__ float beam_key_val(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
-__device__ __forceinline__ uint64_t beam_key(float v, uint32_t id) {
-  if (v == -INFINITY) return 0;
-  return (uint64_t(beam_val_key(v == 0.f ? 0.f : v)) << 32) | (0xFFFFFFFFu - id);
-}
+// Key of a logit that may be -inf or NaN (0), or -0 (as +0).
+__device__ __forceinline__ uint32_t beam_logit_key(float v) { return v > -INFINITY ? beam_val_key(v + 0.f) : 0u; }
+__device__ __forceinline__ uint64_t beam_key(uint32_t key, uint32_t id) { return (uint64_t(key) << 32) | (0xFFFFFFFFu - id); }
 
-// max of key over the block; valid in every thread. `red`: one word per warp.
-__device__ __forceinline__ uint64_t block_max_u64(uint64_t v, uint64_t* red) {
+__device__ __forceinline__ float beam_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// What a sum against m counts in one against the larger top.
+__device__ __forceinline__ float beam_weight(float m, float top) {
+  return m == top ? 1.f : fmaxf(beam_exp2(beam_ref(m) - beam_ref(top)), 0.f);  // (inf - inf: 0)
+}
+__device__ __forceinline__ uint64_t warp_max_u64(uint64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const uint64_t u = __shfl_xor_sync(0xffffffffu, v, o);
     v = u > v ? u : v;
   }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int nw = blockDim.x >> 5;
-  for (int i = 0; i < nw; ++i) v = red[i] > v ? red[i] : v;
   return v;
 }
 
@@ -66,40 +75,266 @@ struct BeamRowsParams {
 };
 
 constexpr int kBeamThreads = 256;
+constexpr int kBeamWarps = kBeamThreads / 32;
+constexpr int kBeamVecs = 4;   // 16-byte vectors a lane and tile
+constexpr int kBeamCap = 192;  // candidates a warp holds between two cuts to the k best
+
+// One warp's candidates: every value of the warp's columns that may be among
+// the chunk's k best. A value enters when its key is above `thr`, below which
+// at least k values are known; when the buffer fills, it is cut to its k best.
+struct BeamList {
+  uint64_t* buf;  // [kBeamCap], shared memory
+  int n;
+  uint32_t thr;
+  int k;
+};
+
+// The k best of the warp's buffer, in their place; thr becomes the k-th key:
+// later columns have higher ids and must beat it. Each entry counts those above it.
+__device__ __forceinline__ void beam_cut(BeamList& l) {
+  const int lane = threadIdx.x & 31;
+  constexpr int E = kBeamCap / 32;
+  uint64_t mine[E];
+  int rank[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    mine[e] = lane + 32 * e < l.n ? l.buf[lane + 32 * e] : 0;
+    rank[e] = 0;
+  }
+  for (int i = 0; i < l.n; ++i) {
+    const uint64_t o = l.buf[i];
+#pragma unroll
+    for (int e = 0; e < E; ++e) rank[e] += o > mine[e] ? 1 : 0;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (mine[e] && rank[e] < l.k) l.buf[rank[e]] = mine[e];
+  __syncwarp();
+  if (l.n >= l.k) {
+    l.n = l.k;
+    l.thr = max(l.thr, uint32_t(l.buf[l.k - 1] >> 32));
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsParams p) {
-  __shared__ uint64_t red[kBeamThreads / 32];
-  __shared__ float redf[kBeamThreads / 32];
+  constexpr int VE = VecTraits<T>::kElems, E = kBeamVecs * VE;
+  __shared__ uint64_t buf[kBeamWarps][kBeamCap];
+  __shared__ uint64_t all[kBeamWarps * kBeamMaxK];
+  __shared__ float2 stat[kBeamWarps];
+  __shared__ uint32_t floor_key;  // at least k of the chunk's values have this key or a higher one
+  __shared__ int total;
   pdl_launch();
   pdl_wait();
   const int row = blockIdx.y, ch = blockIdx.x;
   if (p.finished && p.finished[row]) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    floor_key = 0;
+    total = 0;
+  }
+  __syncthreads();
   const int c0 = ch * p.chunk, c1 = min(p.V, c0 + p.chunk);
   const T* x = static_cast<const T*>(p.logits) + int64_t(row) * p.ld;
-  uint64_t* out = p.cand + (size_t(row) * p.nchunk + ch) * p.k;
-  uint64_t last = ~0ull;
-  float m = -INFINITY;
-  for (int j = 0; j < p.k; ++j) {
-    uint64_t best = 0;
-    for (int c = c0 + threadIdx.x; c < c1; c += kBeamThreads) {
-      const uint64_t key = beam_key(fmaxf(to_f(x[c]), -INFINITY), uint32_t(p.vstart + c));
-      if (key < last && key > best) best = key;
+  // whole 16-byte vectors from the one that holds column c0; col0 + i * VE is the first column of vector i
+  const int skew = int((reinterpret_cast<uintptr_t>(x + c0) & 15u) / sizeof(T));
+  const int col0 = c0 - skew;
+  const int nvec = c1 > c0 ? (c1 - col0 + VE - 1) / VE : 0;
+  auto load = [&](uint4 (&v)[kBeamVecs], int tile) {
+#pragma unroll
+    for (int u = 0; u < kBeamVecs; ++u) {
+      const int i = (tile * kBeamVecs + u) * 32 + lane, col = col0 + i * VE;
+      if (i < nvec && col >= c0 && col + VE <= c1) {
+        v[u] = ld_stream(x + col);
+      } else {  // the chunk's ends: the columns inside it, -inf for the others
+        float f[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          f[e] = i < nvec && col + e >= c0 && col + e < c1 ? to_f(x[col + e]) : -INFINITY;
+        v[u] = pack_vec(f);
+      }
     }
-    best = block_max_u64(best, red);
-    if (threadIdx.x == 0) out[j] = best;
-    if (j == 0) m = best ? beam_key_val(uint32_t(best >> 32)) : -INFINITY;
-    last = best;
-    if (best == 0) {
-      for (int i = j + 1 + threadIdx.x; i < p.k; i += kBeamThreads) out[i] = 0;
-      break;
+  };
+  BeamList l{buf[warp], 0, 0u, p.k};
+  float m = -INFINITY, c = 0.f, s = 0.f;  // reference and sum of this lane
+  const int ntile = (nvec + 32 * kBeamVecs - 1) / (32 * kBeamVecs);
+  uint4 v[kBeamVecs], next[kBeamVecs];
+  if (warp < ntile) load(v, warp);
+  for (int t = warp; t < ntile; t += kBeamWarps) {
+    if (t + kBeamWarps < ntile) load(next, t + kBeamWarps);
+    float q[kBeamVecs];  // max of each vector (a NaN is passed over)
+#pragma unroll
+    for (int u = 0; u < kBeamVecs; ++u) {
+      float f[VE];
+      unpack(v[u], f);
+      q[u] = f[0];
+#pragma unroll
+      for (int e = 1; e < VE; ++e) q[u] = fmaxf(q[u], f[e]);
     }
+    const float top = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+    // ---- sum: the reference follows the maximum only when it has to
+    if (top - m > 40.f) {
+      s = beam_far(m) || beam_far(top) ? 0.f : s * beam_exp2(beam_ref(m) - beam_ref(top));
+      m = top;
+      c = beam_ref(m);
+    }
+    float part = 0.f;
+    if (!beam_far(m)) {
+#pragma unroll
+      for (int u = 0; u < kBeamVecs; ++u) {
+        float f[VE];
+        unpack(v[u], f);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) part += beam_exp2(fmaf(f[e], kBeamLog2e, -c));
+      }
+    }
+    if (beam_far(m) || !(part < INFINITY)) {  // counted values, or a NaN among them
+      part = 0.f;
+#pragma unroll
+      for (int u = 0; u < kBeamVecs; ++u) {
+        float f[VE];
+        unpack(v[u], f);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          if (beam_far(m))
+            part += f[e] == m && m > -INFINITY ? 1.f : 0.f;
+          else if (f[e] == f[e])
+            part += beam_exp2(fmaf(f[e], kBeamLog2e, -c));
+        }
+      }
+    }
+    s += part;
+    // ---- candidates
+    if (t == warp) {
+      // the k-th of the warp's 32 * kBeamVecs vector maxima: k values lie at or above it
+      uint32_t kq[kBeamVecs], cut = 0;
+#pragma unroll
+      for (int u = 0; u < kBeamVecs; ++u) kq[u] = beam_logit_key(q[u]);
+      for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+        const uint32_t cand = cut | bit;
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < kBeamVecs; ++u) n += __popc(__ballot_sync(0xffffffffu, kq[u] >= cand));
+        if (n >= p.k) cut = cand;
+        if (n == p.k) break;
+      }
+      if (cut) {
+        l.thr = cut - 1;
+        if (lane == 0) atomicMax(&floor_key, cut);
+      }
+    }
+    const uint32_t fk = *reinterpret_cast<volatile uint32_t*>(&floor_key);
+    uint32_t thr = max(l.thr, fk ? fk - 1 : 0u);
+    if (__any_sync(0xffffffffu, beam_logit_key(top) > thr)) {
+      for (int attempt = 0;; ++attempt) {
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < kBeamVecs; ++u) {
+          float f[VE];
+          unpack(v[u], f);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) n += beam_logit_key(f[e]) > thr ? 1 : 0;
+        }
+        int at = n;  // inclusive prefix over the lanes
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, at, o);
+          if (lane >= o) at += up;
+        }
+        const int more = __shfl_sync(0xffffffffu, at, 31);
+        if (l.n + more <= kBeamCap) {
+          at += l.n - n;
+#pragma unroll
+          for (int u = 0; u < kBeamVecs; ++u) {
+            float f[VE];
+            unpack(v[u], f);
+            const uint32_t id = uint32_t(p.vstart + col0 + ((t * kBeamVecs + u) * 32 + lane) * VE);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              const uint32_t key = beam_logit_key(f[e]);
+              if (key > thr) l.buf[at++] = beam_key(key, id + e);
+            }
+          }
+          l.n += more;
+          __syncwarp();
+          break;
+        }
+        if (attempt == 0 && l.n > 0) {
+          beam_cut(l);
+          thr = max(thr, l.thr);
+          continue;
+        }
+        // long runs of equal values: the k best of the buffer and this tile, one after another
+        uint64_t last = ~0ull, keep0 = 0, keep1 = 0;  // lane i keeps the i-th and the (i + 32)-th
+        int got = 0;
+        for (; got < p.k; ++got) {
+          uint64_t best = 0;
+          for (int i = lane; i < l.n; i += 32) {
+            const uint64_t o = l.buf[i];
+            if (o < last && o > best) best = o;
+          }
+#pragma unroll
+          for (int u = 0; u < kBeamVecs; ++u) {
+            float f[VE];
+            unpack(v[u], f);
+            const uint32_t id = uint32_t(p.vstart + col0 + ((t * kBeamVecs + u) * 32 + lane) * VE);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              const uint32_t key = beam_logit_key(f[e]);
+              const uint64_t o = beam_key(key, id + e);
+              if (key && o < last && o > best) best = o;
+            }
+          }
+          best = warp_max_u64(best);
+          if (!best) break;
+          last = best;
+          if (lane == (got & 31)) (got < 32 ? keep0 : keep1) = best;
+        }
+        __syncwarp();
+        if (lane < got) l.buf[lane] = keep0;
+        if (lane + 32 < got) l.buf[lane + 32] = keep1;
+        __syncwarp();
+        l.n = got;
+        if (got == p.k) l.thr = max(l.thr, uint32_t(last >> 32));
+        break;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kBeamVecs; ++u) v[u] = next[u];
   }
-  float s = 0.f;
-  for (int c = c0 + threadIdx.x; c < c1; c += kBeamThreads)
-    s += expf(fminf(fmaxf(to_f(x[c]), -INFINITY) - m, 0.f));
-  s = block_sum(s, redf);
-  if (threadIdx.x == 0) p.stat[size_t(row) * p.nchunk + ch] = BeamStat{m, s};
+  // ---- the chunk's sum
+  float cm = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
+  s = warp_sum(s * beam_weight(m, cm));
+  if (lane == 0) stat[warp] = make_float2(cm, s);
+  // ---- the chunk's k best: the warps' candidates above the common floor, ranked
+  if (l.n > p.k) beam_cut(l);
+  __syncthreads();
+  const uint32_t fk = floor_key;
+  for (int i = lane; i < l.n; i += 32) {
+    const uint64_t o = l.buf[i];
+    if (uint32_t(o >> 32) >= fk) all[atomicAdd(&total, 1)] = o;
+  }
+  __syncthreads();
+  const int n = total;
+  uint64_t* out = p.cand + (size_t(row) * p.nchunk + ch) * p.k;
+  for (int i = threadIdx.x; i < n; i += kBeamThreads) {
+    const uint64_t o = all[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += all[j] > o ? 1 : 0;
+    if (rank < p.k) out[rank] = o;
+  }
+  for (int i = n + threadIdx.x; i < p.k; i += kBeamThreads) out[i] = 0;
+  if (threadIdx.x == 0) {
+    float m = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kBeamWarps; ++w) m = fmaxf(m, stat[w].x);
+#pragma unroll
+    for (int w = 0; w < kBeamWarps; ++w) sum += stat[w].y * beam_weight(stat[w].x, m);
+    p.stat[size_t(row) * p.nchunk + ch] = BeamStat{m, sum};
+  }
 }
 
 struct BeamPickParams {
@@ -127,94 +362,137 @@ __device__ __forceinline__ bool beam_better(const BeamCand& x, const BeamCand& y
   return x.id < y.id;
 }
 
+constexpr int kPickCap = 512;  // candidates ranked against each other
+
 __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickParams p) {
-  // per beam: score - (max + log sum), as total = (x - max) + base; base NaN: no candidate
+  // of each beam: total = (x - top) + base
   __shared__ double base[kBeamMaxW];
   __shared__ float top[kBeamMaxW];
-  __shared__ double red_t[kBeamThreads / 32];
-  __shared__ uint32_t red_b[kBeamThreads / 32], red_i[kBeamThreads / 32];
+  __shared__ uint8_t fin[kBeamMaxW];
+  __shared__ BeamCand list[kPickCap];
+  __shared__ int total;
   pdl_launch();
   pdl_wait();
-  const int g = blockIdx.x, tid = threadIdx.x;
-  if (tid < p.W) {
-    const int row = g * p.W + tid;
+  const int g = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) total = 0;
+  for (int b = warp; b < p.W; b += kBeamWarps) {  // a warp a beam
+    const int row = g * p.W + b;
     const double sc = p.scores[row];
-    if (p.finished && p.finished[row]) {
-      top[tid] = 0.f;
-      base[tid] = sc;
-    } else {
-      float m = -INFINITY;
-      for (int q = 0; q < p.parts; ++q)
-        for (int c = 0; c < p.nchunk; ++c) m = fmaxf(m, p.stat[q * p.stat_part + size_t(row) * p.nchunk + c].m);
+    const bool f = p.finished && p.finished[row];
+    double bs = sc;
+    float m = -INFINITY;
+    if (!f) {
+      const int n = p.parts * p.nchunk;
+      auto at = [&](int i) {
+        const int q = i / p.nchunk;
+        return p.stat[q * p.stat_part + size_t(row) * p.nchunk + (i - q * p.nchunk)];
+      };
+      for (int i = lane; i < n; i += 32) m = fmaxf(m, at(i).m);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       double s = 0.0;
-      for (int q = 0; q < p.parts; ++q)
-        for (int c = 0; c < p.nchunk; ++c) {
-          const BeamStat t = p.stat[q * p.stat_part + size_t(row) * p.nchunk + c];
-          if (t.m != -INFINITY) s += double(t.s) * exp(t.m == m ? 0.0 : double(t.m) - double(m));
-        }
-      top[tid] = m;
-      base[tid] = sc - log(s);
+      for (int i = lane; i < n; i += 32) {
+        const BeamStat t = at(i);
+        if (t.m == m)
+          s += double(t.s);
+        else if (!beam_far(m))
+          s += double(t.s) * exp2(double(beam_ref(t.m)) - double(beam_ref(m)));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      // log sum exp - m, the rounding of the reference taken out
+      constexpr double kLn2d = 0.69314718055994530942;
+      bs = sc - kLn2d * log2(s) - (beam_far(m) ? 0.0 : kLn2d * double(beam_ref(m)) - double(m));
+    }
+    if (lane == 0) {
+      base[b] = bs;
+      top[b] = m;
+      fin[b] = f;
     }
   }
   __syncthreads();
-  const int n = p.parts * p.W * p.nchunk * p.kc;
+  const int per = p.nchunk * p.kc, n = p.parts * p.W * per;
+  // candidate i; total -inf: none
+  auto cand = [&](int i) {
+    BeamCand c{-INFINITY, 0u, 0u};
+    const int q = i / (p.W * per), r = i - q * p.W * per, b = r / per, o = r - b * per;
+    c.b = b;
+    if (fin[b]) {
+      if (q || o) return c;
+      c.id = uint32_t(p.eos);
+      c.total = base[b];
+    } else {
+      const uint64_t key = p.cand[q * p.cand_part + size_t(g * p.W + b) * per + o];
+      if (!key) return c;
+      c.id = 0xFFFFFFFFu - uint32_t(key);
+      const float x = beam_key_val(uint32_t(key >> 32));
+      c.total = (x == top[b] ? 0.0 : double(x) - double(top[b])) + base[b];
+    }
+    if (!(c.total > -INFINITY)) c.total = -INFINITY;  // (or NaN)
+    return c;
+  };
+  // a floor that k candidates reach: the k-th of the threads' best totals, rounded to fp32 (which keeps the order)
+  float best = -INFINITY;
+  for (int i = tid; i < n; i += kBeamThreads) best = fmaxf(best, float(cand(i).total));
+  uint32_t cut = 0;
+  const uint32_t key = beam_logit_key(best);
+  for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+    const int m = __syncthreads_count(key >= (cut | bit));
+    if (m >= p.k) cut |= bit;
+    if (m == p.k) break;
+  }
+  for (int i = tid; i < n; i += kBeamThreads) {
+    const BeamCand c = cand(i);
+    const uint32_t ck = beam_logit_key(float(c.total));
+    if (ck && ck >= cut) {
+      const int at = atomicAdd(&total, 1);
+      if (at < kPickCap) list[at] = c;
+    }
+  }
+  __syncthreads();
+  auto put = [&](int j, bool none, const BeamCand& c) {
+    const size_t o = size_t(g) * p.k + j;
+    const long long tok = none ? (p.eos >= 0 ? p.eos : 0) : (long long)c.id;
+    const int par = none ? 0 : int(c.b);
+    p.out_scores[o] = none ? -INFINITY : float(c.total);
+    p.out_parents[o] = par;
+    p.out_tokens[o] = tok;
+    if (p.out_finished) p.out_finished[o] = (p.eos >= 0 && tok == p.eos) || fin[par];
+  };
+  const int got = total;
+  if (got <= kPickCap) {
+    for (int i = tid; i < got; i += kBeamThreads) {
+      const BeamCand c = list[i];
+      int rank = 0;
+      for (int j = 0; j < got; ++j) rank += beam_better(list[j], c) ? 1 : 0;
+      if (rank < p.k) put(rank, false, c);
+    }
+    for (int j = got + tid; j < p.k; j += kBeamThreads) put(j, true, BeamCand{});
+    return;
+  }
+  // more equal totals than the list holds: the k best one after another
   BeamCand last{INFINITY, 0, 0};
-  bool first = true;
   for (int j = 0; j < p.k; ++j) {
-    BeamCand best{-INFINITY, ~0u, ~0u};
+    BeamCand win{-INFINITY, ~0u, ~0u};
     for (int i = tid; i < n; i += kBeamThreads) {
-      const int per = p.nchunk * p.kc;
-      const int q = i / (p.W * per), r = i - q * p.W * per, b = r / per, o = r - b * per;
-      const int row = g * p.W + b;
-      BeamCand c;
-      c.b = b;
-      if (p.finished && p.finished[row]) {
-        if (q || o) continue;
-        c.id = uint32_t(p.eos);
-        c.total = base[b];
-      } else {
-        const uint64_t key = p.cand[q * p.cand_part + size_t(row) * per + o];
-        if (!key) continue;
-        c.id = 0xFFFFFFFFu - uint32_t(key);
-        const float x = beam_key_val(uint32_t(key >> 32));
-        c.total = (x == top[b] ? 0.0 : double(x) - double(top[b])) + base[b];
-      }
-      if (!(c.total > -INFINITY)) continue;
-      if (!first && !beam_better(last, c)) continue;
-      if (beam_better(c, best)) best = c;
+      const BeamCand c = cand(i);
+      if (c.total > -INFINITY && (j == 0 || beam_better(last, c)) && beam_better(c, win)) win = c;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       BeamCand c;
-      c.total = __shfl_xor_sync(0xffffffffu, best.total, o);
-      c.b = __shfl_xor_sync(0xffffffffu, best.b, o);
-      c.id = __shfl_xor_sync(0xffffffffu, best.id, o);
-      if (beam_better(c, best)) best = c;
+      c.total = __shfl_xor_sync(0xffffffffu, win.total, o);
+      c.b = __shfl_xor_sync(0xffffffffu, win.b, o);
+      c.id = __shfl_xor_sync(0xffffffffu, win.id, o);
+      if (beam_better(c, win)) win = c;
     }
     __syncthreads();
-    if ((tid & 31) == 0) {
-      red_t[tid >> 5] = best.total;
-      red_b[tid >> 5] = best.b;
-      red_i[tid >> 5] = best.id;
-    }
+    if (lane == 0) list[warp] = win;
     __syncthreads();
-    for (int i = 0; i < kBeamThreads / 32; ++i) {
-      const BeamCand c{red_t[i], red_b[i], red_i[i]};
-      if (beam_better(c, best)) best = c;
-    }
-    last = best;
-    first = false;
-    if (tid == 0) {
-      const bool none = best.b == ~0u;
-      const size_t o = size_t(g) * p.k + j;
-      const long long tok = none ? (p.eos >= 0 ? p.eos : 0) : (long long)best.id;
-      const int par = none ? 0 : int(best.b);
-      p.out_scores[o] = none ? -INFINITY : float(best.total);
-      p.out_parents[o] = par;
-      p.out_tokens[o] = tok;
-      if (p.out_finished)
-        p.out_finished[o] = (p.eos >= 0 && tok == p.eos) || (p.finished && p.finished[size_t(g) * p.W + par]);
-    }
+    for (int i = 0; i < kBeamWarps; ++i)
+      if (beam_better(list[i], win)) win = list[i];
+    last = win;
+    if (tid == 0) put(j, win.b == ~0u, win);
   }
 }
 

@@ -28,6 +28,7 @@ struct BeamPlan {
 
 BeamPlan beam_plan(long long rows, int V) {
   BeamPlan b;
+  // four CTAs for each of B200's 148 SMs, but no chunk below 4096 columns
   const long long want = std::max<long long>(1, (4 * 148 + rows - 1) / rows);
   b.nchunk = int(std::min<long long>(want, (V + 4095) / 4096));
   b.chunk = (V + b.nchunk - 1) / b.nchunk;
