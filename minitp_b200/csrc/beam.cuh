@@ -77,44 +77,84 @@ struct BeamRowsParams {
 constexpr int kBeamThreads = 256;
 constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamVecs = 4;   // 16-byte vectors a lane and tile
-constexpr int kBeamCap = 192;  // candidates a warp holds between two cuts to the k best
+constexpr int kBeamCap = 160;  // candidates a warp holds between two cuts to the k best: 64, and room for 32 at a time
 
-// One warp's candidates: every value of the warp's columns that may be among
-// the chunk's k best. A value enters when its key is above `thr`, below which
-// at least k values are known; when the buffer fills, it is cut to its k best.
+// One warp's candidates: every value of the warp's columns so far that may be
+// among the chunk's k best, i.e. whose key is at least `least`.
 struct BeamList {
   uint64_t* buf;  // [kBeamCap], shared memory
   int n;
-  uint32_t thr;
-  int k;
+  uint32_t least;
+  uint32_t kth;  // after a cut: key of the k-th; else 0
 };
 
-// The k best of the warp's buffer, in their place; thr becomes the k-th key:
-// later columns have higher ids and must beat it. Each entry counts those above it.
-__device__ __forceinline__ void beam_cut(BeamList& l) {
+// Largest t, in steps of 2^low, with count(t) >= k, for keys that lie in
+// [least, most]: bit by bit below the bits that those two share, until the
+// count is k.
+template <typename Count>
+__device__ __forceinline__ uint32_t beam_search(int k, uint32_t least, uint32_t most, int low, const Count& count) {
+  const uint32_t diff = least ^ most;
+  if (!diff) return most;
+  const int high = 31 - __clz(diff);
+  uint32_t t = high == 31 ? 0u : most & ~((2u << high) - 1u);
+  for (int b = high; b >= low; --b) {
+    const int n = count(t | (1u << b));
+    if (n >= k) t |= 1u << b;
+    if (n == k) break;
+  }
+  return t;
+}
+
+// Cuts the warp's buffer of more than k to its k best (in no order).
+__device__ __forceinline__ void beam_cut(BeamList& l, int k, uint32_t* floor_key) {
   const int lane = threadIdx.x & 31;
   constexpr int E = kBeamCap / 32;
-  uint64_t mine[E];
-  int rank[E];
+  uint32_t hi[E], lo[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    mine[e] = lane + 32 * e < l.n ? l.buf[lane + 32 * e] : 0;
-    rank[e] = 0;
+    const uint64_t o = lane + 32 * e < l.n ? l.buf[lane + 32 * e] : 0;
+    hi[e] = uint32_t(o >> 32);
+    lo[e] = uint32_t(o);
   }
-  for (int i = 0; i < l.n; ++i) {
-    const uint64_t o = l.buf[i];
+  auto count = [&](auto&& in) {
+    int n = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) rank[e] += o > mine[e] ? 1 : 0;
-  }
-  __syncwarp();
+    for (int e = 0; e < E; ++e) n += __popc(__ballot_sync(0xffffffffu, in(e)));
+    return n;
+  };
+  uint32_t most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
   for (int e = 0; e < E; ++e)
-    if (mine[e] && rank[e] < l.k) l.buf[rank[e]] = mine[e];
+    if (hi[e]) {
+      most = max(most, hi[e]);
+      least = min(least, hi[e]);
+    }
+  most = __reduce_max_sync(0xffffffffu, most);
+  least = __reduce_min_sync(0xffffffffu, least);
+  const uint32_t t = beam_search(k, least, most, 0, [&](uint32_t v) { return count([&](int e) { return hi[e] >= v; }); });
+  const int above = count([&](int e) { return hi[e] > t; });
+  uint32_t u = 0;  // of those equal to t, the lowest ids (the largest low words)
+  if (above + count([&](int e) { return hi[e] == t; }) > k && above < k)
+    u = beam_search(k - above, 0u, 0xFFFFFFFFu, 0,
+                    [&](uint32_t v) { return count([&](int e) { return hi[e] == t && lo[e] >= v; }); });
+  least = 0xFFFFFFFFu;
+  int n = 0;
   __syncwarp();
-  if (l.n >= l.k) {
-    l.n = l.k;
-    l.thr = max(l.thr, uint32_t(l.buf[l.k - 1] >> 32));
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool in = hi[e] > t || (hi[e] == t && lo[e] >= u);
+    const uint32_t b = __ballot_sync(0xffffffffu, in);
+    if (in) {
+      l.buf[n + __popc(b & ((1u << lane) - 1u))] = (uint64_t(hi[e]) << 32) | lo[e];
+      least = min(least, hi[e]);
+    }
+    n += __popc(b);
   }
+  __syncwarp();
+  l.n = n;
+  l.kth = __reduce_min_sync(0xffffffffu, least);
+  l.least = max(l.least, l.kth);
+  if (lane == 0) atomicMax(floor_key, l.kth);
 }
 
 template <typename T>
@@ -156,7 +196,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
       }
     }
   };
-  BeamList l{buf[warp], 0, 0u, p.k};
+  BeamList l{buf[warp], 0, 0x00800000u, 0u};  // least: the key of the lowest finite value
   float m = -INFINITY, c = 0.f, s = 0.f;  // reference and sum of this lane
   const int ntile = (nvec + 32 * kBeamVecs - 1) / (32 * kBeamVecs);
   uint4 v[kBeamVecs], next[kBeamVecs];
@@ -208,97 +248,53 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
     // ---- candidates
     if (t == warp) {
       // the k-th of the warp's 32 * kBeamVecs vector maxima: k values lie at or above it
-      uint32_t kq[kBeamVecs], cut = 0;
+      uint32_t kq[kBeamVecs];
 #pragma unroll
       for (int u = 0; u < kBeamVecs; ++u) kq[u] = beam_logit_key(q[u]);
-      for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-        const uint32_t cand = cut | bit;
+      const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(kq[0], kq[1]), max(kq[2], kq[3])));
+      const uint32_t least = __reduce_min_sync(0xffffffffu, min(min(kq[0], kq[1]), min(kq[2], kq[3])));
+      // (bf16 values differ in the upper half of their keys only)
+      const uint32_t cut = beam_search(p.k, least, most, sizeof(T) == 2 ? 16 : 0, [&](uint32_t x) {
         int n = 0;
 #pragma unroll
-        for (int u = 0; u < kBeamVecs; ++u) n += __popc(__ballot_sync(0xffffffffu, kq[u] >= cand));
-        if (n >= p.k) cut = cand;
-        if (n == p.k) break;
-      }
-      if (cut) {
-        l.thr = cut - 1;
-        if (lane == 0) atomicMax(&floor_key, cut);
-      }
+        for (int u = 0; u < kBeamVecs; ++u) n += __popc(__ballot_sync(0xffffffffu, kq[u] >= x));
+        return n;
+      });
+      if (lane == 0) atomicMax(&floor_key, cut);
+      l.least = max(l.least, cut);
     }
-    const uint32_t fk = *reinterpret_cast<volatile uint32_t*>(&floor_key);
-    uint32_t thr = max(l.thr, fk ? fk - 1 : 0u);
-    if (__any_sync(0xffffffffu, beam_logit_key(top) > thr)) {
-      for (int attempt = 0;; ++attempt) {
-        int n = 0;
+    l.least = max(l.least, *reinterpret_cast<volatile uint32_t*>(&floor_key));
+    float ge = beam_key_val(l.least);
+    if (__any_sync(0xffffffffu, top >= ge)) {
+      uint32_t mine = 0;  // this lane's values that enter
 #pragma unroll
-        for (int u = 0; u < kBeamVecs; ++u) {
-          float f[VE];
-          unpack(v[u], f);
+      for (int u = 0; u < kBeamVecs; ++u) {
+        if (!__any_sync(0xffffffffu, q[u] >= ge)) continue;
+        float f[VE];
+        unpack(v[u], f);
 #pragma unroll
-          for (int e = 0; e < VE; ++e) n += beam_logit_key(f[e]) > thr ? 1 : 0;
-        }
-        int at = n;  // inclusive prefix over the lanes
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, at, o);
-          if (lane >= o) at += up;
-        }
-        const int more = __shfl_sync(0xffffffffu, at, 31);
-        if (l.n + more <= kBeamCap) {
-          at += l.n - n;
-#pragma unroll
-          for (int u = 0; u < kBeamVecs; ++u) {
-            float f[VE];
-            unpack(v[u], f);
-            const uint32_t id = uint32_t(p.vstart + col0 + ((t * kBeamVecs + u) * 32 + lane) * VE);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              const uint32_t key = beam_logit_key(f[e]);
-              if (key > thr) l.buf[at++] = beam_key(key, id + e);
-            }
-          }
-          l.n += more;
-          __syncwarp();
-          break;
-        }
-        if (attempt == 0 && l.n > 0) {
-          beam_cut(l);
-          thr = max(thr, l.thr);
-          continue;
-        }
-        // long runs of equal values: the k best of the buffer and this tile, one after another
-        uint64_t last = ~0ull, keep0 = 0, keep1 = 0;  // lane i keeps the i-th and the (i + 32)-th
-        int got = 0;
-        for (; got < p.k; ++got) {
-          uint64_t best = 0;
-          for (int i = lane; i < l.n; i += 32) {
-            const uint64_t o = l.buf[i];
-            if (o < last && o > best) best = o;
-          }
-#pragma unroll
-          for (int u = 0; u < kBeamVecs; ++u) {
-            float f[VE];
-            unpack(v[u], f);
-            const uint32_t id = uint32_t(p.vstart + col0 + ((t * kBeamVecs + u) * 32 + lane) * VE);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              const uint32_t key = beam_logit_key(f[e]);
-              const uint64_t o = beam_key(key, id + e);
-              if (key && o < last && o > best) best = o;
-            }
-          }
-          best = warp_max_u64(best);
-          if (!best) break;
-          last = best;
-          if (lane == (got & 31)) (got < 32 ? keep0 : keep1) = best;
-        }
-        __syncwarp();
-        if (lane < got) l.buf[lane] = keep0;
-        if (lane + 32 < got) l.buf[lane + 32] = keep1;
-        __syncwarp();
-        l.n = got;
-        if (got == p.k) l.thr = max(l.thr, uint32_t(last >> 32));
-        break;
+        for (int e = 0; e < VE; ++e) mine |= f[e] >= ge ? 1u << (u * VE + e) : 0u;
       }
+      // one value of each lane at a time
+      while (true) {
+        const uint32_t b = __ballot_sync(0xffffffffu, mine != 0);
+        if (!b) break;
+        if (mine) {
+          const int i = __ffs(mine) - 1, u = i / VE, e = i - u * VE;
+          mine &= mine - 1;
+          const uint4 w = u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : v[3];
+          const int word = e * int(sizeof(T)) / 4;
+          const uint32_t bits = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
+          const float val = sizeof(T) == 4 ? __uint_as_float(bits) : __uint_as_float(e & 1 ? bits & 0xFFFF0000u : bits << 16);
+          const uint32_t id = uint32_t(p.vstart + col0 + ((t * kBeamVecs + u) * 32 + lane) * VE + e);
+          l.buf[l.n + __popc(b & ((1u << lane) - 1u))] = beam_key(beam_logit_key(val), id);
+        }
+        l.n += __popc(b);
+        __syncwarp();
+        if (l.n > kBeamCap - 32) beam_cut(l, p.k, &floor_key);
+      }
+      // later columns have higher ids: they have to beat the k-th, not to equal it
+      if (l.kth) l.least = max(l.least, l.kth + 1);
     }
 #pragma unroll
     for (int u = 0; u < kBeamVecs; ++u) v[u] = next[u];
@@ -309,8 +305,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
   for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
   s = warp_sum(s * beam_weight(m, cm));
   if (lane == 0) stat[warp] = make_float2(cm, s);
-  // ---- the chunk's k best: the warps' candidates above the common floor, ranked
-  if (l.n > p.k) beam_cut(l);
+  // ---- the chunk's k best: the warps' candidates (at most 64 each) from the common floor on, ranked
+  if (l.n > kBeamMaxK) beam_cut(l, p.k, &floor_key);
   __syncthreads();
   const uint32_t fk = floor_key;
   for (int i = lane; i < l.n; i += 32) {
@@ -363,6 +359,7 @@ __device__ __forceinline__ bool beam_better(const BeamCand& x, const BeamCand& y
 }
 
 constexpr int kPickCap = 512;  // candidates ranked against each other
+constexpr int kPickHeld = 4;   // keys a thread keeps in registers
 
 __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickParams p) {
   // of each beam: total = (x - top) + base
@@ -371,10 +368,32 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
   __shared__ uint8_t fin[kBeamMaxW];
   __shared__ BeamCand list[kPickCap];
   __shared__ int total;
+  __shared__ uint32_t most_sh, least_sh;
   pdl_launch();
   pdl_wait();
   const int g = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) total = 0;
+  const int per = p.nchunk * p.kc, n = p.parts * p.W * per;
+  // candidate i is of beam b; its key (0 for a finished beam's, which were not written)
+  auto where = [&](int i, int& q, int& b, int& o) {
+    q = i / (p.W * per);
+    const int r = i - q * p.W * per;
+    b = r / per;
+    o = r - b * per;
+  };
+  auto key_at = [&](int i) -> uint64_t {
+    int q, b, o;
+    where(i, q, b, o);
+    const int row = g * p.W + b;
+    return p.finished && p.finished[row] ? 0 : p.cand[q * p.cand_part + size_t(row) * per + o];
+  };
+  uint64_t held[kPickHeld];  // the keys of the first candidates of each thread, loaded under the sums
+#pragma unroll
+  for (int h = 0; h < kPickHeld; ++h) held[h] = tid + h * kBeamThreads < n ? key_at(tid + h * kBeamThreads) : 0;
+  if (tid == 0) {
+    total = 0;
+    most_sh = 0;
+    least_sh = 0xFFFFFFFFu;
+  }
   for (int b = warp; b < p.W; b += kBeamWarps) {  // a warp a beam
     const int row = g * p.W + b;
     const double sc = p.scores[row];
@@ -411,18 +430,17 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
     }
   }
   __syncthreads();
-  const int per = p.nchunk * p.kc, n = p.parts * p.W * per;
-  // candidate i; total -inf: none
-  auto cand = [&](int i) {
+  // candidate i with its key; total -inf: none
+  auto cand = [&](int i, uint64_t key) {
     BeamCand c{-INFINITY, 0u, 0u};
-    const int q = i / (p.W * per), r = i - q * p.W * per, b = r / per, o = r - b * per;
+    int q, b, o;
+    where(i, q, b, o);
     c.b = b;
     if (fin[b]) {
       if (q || o) return c;
       c.id = uint32_t(p.eos);
       c.total = base[b];
     } else {
-      const uint64_t key = p.cand[q * p.cand_part + size_t(g * p.W + b) * per + o];
       if (!key) return c;
       c.id = 0xFFFFFFFFu - uint32_t(key);
       const float x = beam_key_val(uint32_t(key >> 32));
@@ -431,24 +449,33 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
     if (!(c.total > -INFINITY)) c.total = -INFINITY;  // (or NaN)
     return c;
   };
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int h = 0; h < kPickHeld; ++h)
+      if (tid + h * kBeamThreads < n) f(cand(tid + h * kBeamThreads, held[h]));
+    for (int i = tid + kPickHeld * kBeamThreads; i < n; i += kBeamThreads) f(cand(i, key_at(i)));
+  };
   // a floor that k candidates reach: the k-th of the threads' best totals, rounded to fp32 (which keeps the order)
   float best = -INFINITY;
-  for (int i = tid; i < n; i += kBeamThreads) best = fmaxf(best, float(cand(i).total));
-  uint32_t cut = 0;
+  each([&](const BeamCand& c) { best = fmaxf(best, float(c.total)); });
   const uint32_t key = beam_logit_key(best);
-  for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-    const int m = __syncthreads_count(key >= (cut | bit));
-    if (m >= p.k) cut |= bit;
-    if (m == p.k) break;
+  {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, key), lo = __reduce_min_sync(0xffffffffu, key);
+    if (lane == 0) {
+      atomicMax(&most_sh, hi);
+      atomicMin(&least_sh, lo);
+    }
   }
-  for (int i = tid; i < n; i += kBeamThreads) {
-    const BeamCand c = cand(i);
+  __syncthreads();
+  const uint32_t cut =
+      beam_search(p.k, least_sh, most_sh, 0, [&](uint32_t v) { return __syncthreads_count(key >= v); });
+  each([&](const BeamCand& c) {
     const uint32_t ck = beam_logit_key(float(c.total));
     if (ck && ck >= cut) {
       const int at = atomicAdd(&total, 1);
       if (at < kPickCap) list[at] = c;
     }
-  }
+  });
   __syncthreads();
   auto put = [&](int j, bool none, const BeamCand& c) {
     const size_t o = size_t(g) * p.k + j;
@@ -474,10 +501,9 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
   BeamCand last{INFINITY, 0, 0};
   for (int j = 0; j < p.k; ++j) {
     BeamCand win{-INFINITY, ~0u, ~0u};
-    for (int i = tid; i < n; i += kBeamThreads) {
-      const BeamCand c = cand(i);
+    each([&](const BeamCand& c) {
       if (c.total > -INFINITY && (j == 0 || beam_better(last, c)) && beam_better(c, win)) win = c;
-    }
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       BeamCand c;
