@@ -8,6 +8,7 @@ stream. None of them has a CPU path: CPU tensors raise.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -182,23 +183,25 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, hq:
 def _same_device(name: str, *tensors: torch.Tensor | None) -> torch.device:
     """The tensors' one CUDA device; raises when there is none or another."""
     dev = tensors[0].device
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
+    if dev.type != "cuda":
+        _lib.require_cuda(tensors[0])
+    for t in tensors[1:]:
+        if t is not None and t.device != dev:
             _lib.require_cuda(t)
-        if t.device != dev:
             raise _lib.MinitpB200Error(f"{name}: tensors on {dev} and {t.device}")
     return dev
 
 
 def _call_on(dev: torch.device, name: str, *args) -> None:
-    """Call a C entry with ``dev`` current (its kernels go to that device's stream)."""
-    if torch.cuda.current_device() == dev.index:
-        _lib.call(name, *args)
-        return
-    with torch.cuda.device(dev):
-        _lib.call(name, *args)
+    """Call a C entry with ``dev`` current and its current stream as the last argument."""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = getattr(_lib.load(), name)(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(_lib.load(), name)(*args, stream)
+    if rc:
+        _lib.check(rc)
 
 
 def _beam_inputs(name: str, logits, scores, k, finished, eos_token_id, least: int = 1):
@@ -229,9 +232,9 @@ def _beam_inputs(name: str, logits, scores, k, finished, eos_token_id, least: in
 
 
 def _beam_outputs(dev, g: int, k: int, flags: bool):
-    ids = torch.empty(2, g, k, dtype=torch.int64, device=dev)
-    return (torch.empty(g, k, dtype=torch.float32, device=dev), ids[0], ids[1],
-            torch.empty(g, k, dtype=torch.bool, device=dev) if flags else None)
+    parents, tokens = torch.empty((2, g, k), dtype=torch.int64, device=dev).unbind(0)
+    return (torch.empty((g, k), dtype=torch.float32, device=dev), parents, tokens,
+            torch.empty((g, k), dtype=torch.bool, device=dev) if flags else None)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: torch.Tensor | None = None,
@@ -254,7 +257,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: to
     block = torch.empty(beam_block_bytes(g * w, v, k), dtype=torch.uint8, device=dev)
     _call_on(dev, "mtpb_beam_select", logits.data_ptr(), ld, g, w, v, scores.data_ptr(), _lib.ptr(finished),
              -1 if eos_token_id is None else eos_token_id, k, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
-             _lib.ptr(done), block.data_ptr(), _lib.dtype_code(logits.dtype), _lib.stream_ptr(dev))
+             _lib.ptr(done), block.data_ptr(), _lib.dtype_code(logits.dtype))
     return out, parents, tokens, done
 
 
@@ -275,7 +278,7 @@ def beam_candidates(local_logits: torch.Tensor, k: int, vstart: int, v_plan: int
     dev, x, ld = _beam_inputs("beam_candidates", local_logits, zeros, k, finished, 0, least=0)
     block = torch.empty(beam_block_bytes(g * w, v_plan, k), dtype=torch.uint8, device=dev)
     _call_on(dev, "mtpb_beam_candidates", x.data_ptr(), ld, g * w, v, vstart, v_plan, k, _lib.ptr(finished),
-             block.data_ptr(), _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
+             block.data_ptr(), _lib.dtype_code(x.dtype))
     return block
 
 
@@ -295,7 +298,7 @@ def beam_pick(blocks: torch.Tensor, scores: torch.Tensor, k: int, v_plan: int, f
     out, parents, tokens, done = _beam_outputs(dev, g, k, eos_token_id is not None)
     _call_on(dev, "mtpb_beam_pick", blocks.data_ptr(), blocks.shape[0], g, w, v_plan, k, scores.data_ptr(),
              _lib.ptr(finished), -1 if eos_token_id is None else eos_token_id, k, out.data_ptr(), parents.data_ptr(),
-             tokens.data_ptr(), _lib.ptr(done), _lib.stream_ptr(dev))
+             tokens.data_ptr(), _lib.ptr(done))
     return out, parents, tokens, done
 
 
@@ -307,6 +310,9 @@ def _length_arg(name: str, lengths, count: int, dev):
             lengths.device != dev:
         raise _lib.MinitpB200Error(f"{name}: lengths must be an int or contiguous int32 [{count}] on {dev}")
     return lengths.data_ptr(), 0
+
+
+_SHAPE_TYPE_PLACE = operator.attrgetter("shape", "dtype", "device")
 
 
 def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
@@ -321,8 +327,8 @@ def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
     if parents.dim() != 2 or parents.dtype != torch.int64 or not parents.is_contiguous():
         raise _lib.MinitpB200Error(f"{name}: parents must be contiguous int64 [G, W]")
     caches = [*k_caches, *v_caches]
-    n = len(caches) // 2
-    if n == 0 or len(k_caches) != n or len(v_caches) != n:
+    n = len(k_caches)
+    if n == 0 or len(v_caches) != n:
         raise _lib.MinitpB200Error(f"{name}: need as many K as V caches")
     first = caches[0]
     dev = _same_device(name, parents, first)
@@ -330,13 +336,12 @@ def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
     g, w = parents.shape
     if first.dim() != 4 or shape[0] != g * w:
         raise _lib.MinitpB200Error(f"{name}: caches must be [{g * w}, hkv, cap, hd], got {tuple(shape)}")
-    for t in caches:
-        if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
-            raise _lib.MinitpB200Error(f"{name}: caches must be contiguous, of one shape, dtype and device")
+    if set(map(_SHAPE_TYPE_PLACE, caches)) != {(shape, dtype, dev)} or not all(map(torch.Tensor.is_contiguous, caches)):
+        raise _lib.MinitpB200Error(f"{name}: caches must be contiguous, of one shape, dtype and device")
     lens, length = _length_arg(name, lengths, g * w, dev)
-    ptrs = (ctypes.c_void_p * (2 * n))(*[t.data_ptr() for t in caches])
+    ptrs = (ctypes.c_void_p * (2 * n))(*map(torch.Tensor.data_ptr, caches))
     _call_on(dev, "mtpb_kv_reorder", ptrs, ctypes.addressof(ptrs) + 8 * n, n, parents.data_ptr(), lens, length, g, w,
-             shape[1], shape[2], shape[3], _lib.dtype_code(dtype), _lib.stream_ptr(dev))
+             shape[1], shape[2], shape[3], _lib.dtype_code(dtype))
 
 
 def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, prefix_lens,
@@ -374,9 +379,9 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     need = _lib.load().mtpb_shared_attention_workspace(g, n // g, t, hq, hkv, hd, cap_p, cap, code)
     if need < 0:
         _lib.check(need)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     out = torch.empty_like(q)
     _call_on(dev, "mtpb_shared_attention", q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), plen, plen_all,
              k_cache.data_ptr(), v_cache.data_ptr(), clen, clen_all, out.data_ptr(), g, n // g, t, hq, hkv, hd, cap_p,
-             cap, code, ws.data_ptr(), need, _lib.stream_ptr(dev))
+             cap, code, _lib.ptr(ws), need)
     return out
