@@ -45,14 +45,9 @@ __device__ __forceinline__ float beam_key_val(uint32_t k) {
 __device__ __forceinline__ uint32_t beam_logit_key(float v) { return v > -INFINITY ? beam_val_key(v + 0.f) : 0u; }
 __device__ __forceinline__ uint64_t beam_key(uint32_t key, uint32_t id) { return (uint64_t(key) << 32) | (0xFFFFFFFFu - id); }
 
-__device__ __forceinline__ float beam_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // What a sum against m counts in one against the larger top.
 __device__ __forceinline__ float beam_weight(float m, float top) {
-  return m == top ? 1.f : fmaxf(beam_exp2(beam_ref(m) - beam_ref(top)), 0.f);  // (inf - inf: 0)
+  return m == top ? 1.f : fmaxf(exp2_approx(beam_ref(m) - beam_ref(top)), 0.f);  // (inf - inf: 0)
 }
 __device__ __forceinline__ uint64_t warp_max_u64(uint64_t v) {
 #pragma unroll
@@ -157,14 +152,38 @@ __device__ __forceinline__ void beam_cut(BeamList& l, int k, uint32_t* floor_key
   if (lane == 0) atomicMax(floor_key, l.kth);
 }
 
+// The k-th key among the warps' candidates of their first tiles, as the
+// chunk's floor (one warp; at most the first 32 of each).
+__device__ __forceinline__ void beam_floor(const uint64_t (*buf)[kBeamCap], const int* count, int k, uint32_t* floor_key) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[kBeamWarps], most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+  for (int w = 0; w < kBeamWarps; ++w) {
+    key[w] = lane < count[w] ? uint32_t(buf[w][lane] >> 32) : 0;
+    most = max(most, key[w]);
+    least = min(least, key[w] ? key[w] : 0xFFFFFFFFu);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  least = __reduce_min_sync(0xffffffffu, least);
+  auto above = [&](uint32_t x) {
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < kBeamWarps; ++w) n += __popc(__ballot_sync(0xffffffffu, key[w] >= x));
+    return n;
+  };
+  if (least > most || above(least) < k) return;
+  const uint32_t cut = beam_search(k, least, most, 0, above);
+  if (lane == 0) atomicMax(floor_key, cut);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsParams p) {
-  constexpr int VE = VecTraits<T>::kElems, E = kBeamVecs * VE;
+  constexpr int VE = VecTraits<T>::kElems;
   __shared__ uint64_t buf[kBeamWarps][kBeamCap];
   __shared__ uint64_t all[kBeamWarps * kBeamMaxK];
   __shared__ float2 stat[kBeamWarps];
   __shared__ uint32_t floor_key;  // at least k of the chunk's values have this key or a higher one
-  __shared__ int total;
+  __shared__ int total, count[kBeamWarps];
   pdl_launch();
   pdl_wait();
   const int row = blockIdx.y, ch = blockIdx.x;
@@ -199,6 +218,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
   BeamList l{buf[warp], 0, 0x00800000u, 0u};  // least: the key of the lowest finite value
   float m = -INFINITY, c = 0.f, s = 0.f;  // reference and sum of this lane
   const int ntile = (nvec + 32 * kBeamVecs - 1) / (32 * kBeamVecs);
+  const bool rounds = ntile > kBeamWarps;
   uint4 v[kBeamVecs], next[kBeamVecs];
   if (warp < ntile) load(v, warp);
   for (int t = warp; t < ntile; t += kBeamWarps) {
@@ -208,26 +228,33 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
     for (int u = 0; u < kBeamVecs; ++u) {
       float f[VE];
       unpack(v[u], f);
-      q[u] = f[0];
+      q[u] = fmaxf(f[0], f[1]);
 #pragma unroll
-      for (int e = 1; e < VE; ++e) q[u] = fmaxf(q[u], f[e]);
+      for (int e = 2; e < VE; e += 2) q[u] = max3(q[u], f[e], f[e + 1]);
     }
-    const float top = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+    const float top = fmaxf(max3(q[0], q[1], q[2]), q[3]);
     // ---- sum: the reference follows the maximum only when it has to
     if (top - m > 40.f) {
-      s = beam_far(m) || beam_far(top) ? 0.f : s * beam_exp2(beam_ref(m) - beam_ref(top));
+      s = beam_far(m) || beam_far(top) ? 0.f : s * exp2_approx(beam_ref(m) - beam_ref(top));
       m = top;
       c = beam_ref(m);
     }
     float part = 0.f;
     if (!beam_far(m)) {
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int u = 0; u < kBeamVecs; ++u) {
         float f[VE];
         unpack(v[u], f);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) part += beam_exp2(fmaf(f[e], kBeamLog2e, -c));
+        for (int e = 0; e < VE; e += 2) {
+          float2 d = fma2(make_float2(f[e], f[e + 1]), make_float2(kBeamLog2e, kBeamLog2e), make_float2(-c, -c));
+          d.x = exp2_approx(d.x);
+          d.y = exp2_approx(d.y);
+          sum = add2(sum, d);
+        }
       }
+      part = sum.x + sum.y;
     }
     if (beam_far(m) || !(part < INFINITY)) {  // counted values, or a NaN among them
       part = 0.f;
@@ -240,7 +267,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
           if (beam_far(m))
             part += f[e] == m && m > -INFINITY ? 1.f : 0.f;
           else if (f[e] == f[e])
-            part += beam_exp2(fmaf(f[e], kBeamLog2e, -c));
+            part += exp2_approx(fmaf(f[e], kBeamLog2e, -c));
         }
       }
     }
@@ -298,6 +325,11 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
     }
 #pragma unroll
     for (int u = 0; u < kBeamVecs; ++u) v[u] = next[u];
+    if (t == warp && rounds) {  // every warp is here: it has a first tile, and others follow
+      if (lane == 0) count[warp] = l.n;
+      __syncthreads();
+      if (warp == 0) beam_floor(buf, count, p.k, &floor_key);
+    }
   }
   // ---- the chunk's sum
   float cm = m;

@@ -28,9 +28,9 @@ struct BeamPlan {
 
 BeamPlan beam_plan(long long rows, int V) {
   BeamPlan b;
-  // four CTAs for each of B200's 148 SMs, but no chunk below 4096 columns
-  const long long want = std::max<long long>(1, (4 * 148 + rows - 1) / rows);
-  b.nchunk = int(std::min<long long>(want, (V + 4095) / 4096));
+  // at most two CTAs for each of B200's 148 SMs, no chunk below 8192 columns
+  const long long want = std::max<long long>(1, 2 * 148 / rows);
+  b.nchunk = int(std::min<long long>(want, (V + 8191) / 8192));
   b.chunk = (V + b.nchunk - 1) / b.nchunk;
   b.chunk = (b.chunk + 7) / 8 * 8;
   b.nchunk = (V + b.chunk - 1) / b.chunk;
