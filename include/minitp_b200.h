@@ -299,6 +299,12 @@ int mtpb_shared_attention(const void* q, const void* k_prefix, const void* v_pre
                           int G, int W, int T, int hq, int hkv, int hd, int cap_p, int cap,
                           int dtype, void* ws, uint64_t ws_bytes, void* stream);
 
+/* Error bits (1: a bounded wait inside a kernel ran out, its results are
+ * void) of the beam selections and shared-prefix attentions of the current
+ * device since the last call; clears them. Synchronises the device. (A
+ * model's forward reports to its communicator's status word instead.) */
+int mtpb_beam_status(uint32_t* status_out /* host */);
+
 /* ---------------------------------------------------------------- model
  * A TP Qwen2 decoder whose weights stay in caller-owned device tensors.
  * ref: minitp/layer.py:68-124 (TPQwen2ForCausalLM), minitp/attention.py,

@@ -114,6 +114,7 @@ SIGNATURES: dict[str, tuple] = {
     "mtpb_shared_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                       c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                       c_void_p, c_uint64, c_void_p]),
+    "mtpb_beam_status": (c_int, [POINTER(c_uint32)]),
     "mtpb_model_create": (c_int, [POINTER(ModelDesc), c_void_p, POINTER(c_void_p)]),
     "mtpb_model_set_layer": (c_int, [c_void_p, c_int, POINTER(LayerDesc)]),
     "mtpb_model_reserve": (c_int, [c_void_p, c_int, c_int]),

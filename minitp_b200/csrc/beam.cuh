@@ -100,7 +100,11 @@ __device__ __forceinline__ uint32_t beam_search(int k, uint32_t least, uint32_t 
   return t;
 }
 
-// Cuts the warp's buffer of more than k to its k best (in no order).
+// Cuts the warp's buffer of more than k to its k best (in no order). The keys
+// of bf16 values differ in their upper halves only (LOW 16): the k-th is then
+// found to that step, which is exact (a positive one's lower half is 0, a
+// negative one's all ones).
+template <int LOW>
 __device__ __forceinline__ void beam_cut(BeamList& l, int k, uint32_t* floor_key) {
   const int lane = threadIdx.x & 31;
   constexpr int E = kBeamCap / 32;
@@ -112,10 +116,10 @@ __device__ __forceinline__ void beam_cut(BeamList& l, int k, uint32_t* floor_key
     lo[e] = uint32_t(o);
   }
   auto count = [&](auto&& in) {
-    int n = 0;
+    uint32_t n = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) n += __popc(__ballot_sync(0xffffffffu, in(e)));
-    return n;
+    for (int e = 0; e < E; ++e) n += in(e) ? 1u : 0u;
+    return int(__reduce_add_sync(0xffffffffu, n));
   };
   uint32_t most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
@@ -126,7 +130,8 @@ __device__ __forceinline__ void beam_cut(BeamList& l, int k, uint32_t* floor_key
     }
   most = __reduce_max_sync(0xffffffffu, most);
   least = __reduce_min_sync(0xffffffffu, least);
-  const uint32_t t = beam_search(k, least, most, 0, [&](uint32_t v) { return count([&](int e) { return hi[e] >= v; }); });
+  uint32_t t = beam_search(k, least, most, LOW, [&](uint32_t v) { return count([&](int e) { return hi[e] >= v; }); });
+  if (LOW == 16 && !(t & 0x80000000u)) t |= 0xFFFFu;
   const int above = count([&](int e) { return hi[e] > t; });
   uint32_t u = 0;  // of those equal to t, the lowest ids (the largest low words)
   if (above + count([&](int e) { return hi[e] == t; }) > k && above < k)
@@ -152,77 +157,108 @@ __device__ __forceinline__ void beam_cut(BeamList& l, int k, uint32_t* floor_key
   if (lane == 0) atomicMax(floor_key, l.kth);
 }
 
-// The k-th key among the warps' candidates of their first tiles, as the
-// chunk's floor (one warp; at most the first 32 of each).
-__device__ __forceinline__ void beam_floor(const uint64_t (*buf)[kBeamCap], const int* count, int k, uint32_t* floor_key) {
+// Takes the candidates below `least` out of the warp's buffer.
+__device__ __forceinline__ void beam_drop(BeamList& l, uint32_t least) {
   const int lane = threadIdx.x & 31;
-  uint32_t key[kBeamWarps], most = 0, least = 0xFFFFFFFFu;
+  int n = 0;
+  for (int i0 = 0; i0 < l.n; i0 += 32) {
+    const uint64_t o = i0 + lane < l.n ? l.buf[i0 + lane] : 0;
+    const bool in = uint32_t(o >> 32) >= least && o;
+    const uint32_t b = __ballot_sync(0xffffffffu, in);  // (reads of this step before its writes, which go no further)
+    if (in) l.buf[n + __popc(b & ((1u << lane) - 1u))] = o;
+    n += __popc(b);
+    __syncwarp();
+  }
+  l.n = n;
+}
+
+// The k-th key among the warps' candidates (at most 32 of each, a lane's keys
+// here), as the chunk's floor.
+template <int LOW>
+__device__ __forceinline__ void beam_floor(const uint32_t (&key)[kBeamWarps], int k, uint32_t* floor_key) {
+  uint32_t most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
   for (int w = 0; w < kBeamWarps; ++w) {
-    key[w] = lane < count[w] ? uint32_t(buf[w][lane] >> 32) : 0;
     most = max(most, key[w]);
     least = min(least, key[w] ? key[w] : 0xFFFFFFFFu);
   }
   most = __reduce_max_sync(0xffffffffu, most);
   least = __reduce_min_sync(0xffffffffu, least);
   auto above = [&](uint32_t x) {
-    int n = 0;
+    uint32_t n = 0;
 #pragma unroll
-    for (int w = 0; w < kBeamWarps; ++w) n += __popc(__ballot_sync(0xffffffffu, key[w] >= x));
-    return n;
+    for (int w = 0; w < kBeamWarps; ++w) n += key[w] >= x ? 1u : 0u;
+    return int(__reduce_add_sync(0xffffffffu, n));
   };
   if (least > most || above(least) < k) return;
-  const uint32_t cut = beam_search(k, least, most, 0, above);
-  if (lane == 0) atomicMax(floor_key, cut);
+  const uint32_t cut = beam_search(k, least, most, LOW, above);
+  if ((threadIdx.x & 31) == 0) atomicMax(floor_key, cut);
 }
 
+// The chunk's 16-byte vectors come through a ring in shared memory, 16 KB
+// rounds filled by bulk copies (warp 8), so that what is in flight does not
+// depend on the registers of the warps that compute. Warp w < 8 takes vectors
+// 128 w .. of each round; columns before the first and behind the last whole
+// vector are warp 0's first and warp 7's last.
+constexpr int kBeamRound = kBeamWarps * 32 * kBeamVecs;  // vectors
+constexpr int kBeamStages = 4;
+constexpr size_t kBeamRing = size_t(kBeamStages) * kBeamRound * 16;
+
+// Set when a bounded wait of a selection ran out (its results are then void).
+__device__ uint32_t g_beam_status;
+
+// (CTAs an SM: three of fp32 took 66 us where two took 88, on 32 x 16 rows of
+// 151937; two of bf16 20.8 where three, which spill, took 23.2, on 8 x 8 of 152064.)
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsParams p) {
-  constexpr int VE = VecTraits<T>::kElems;
+__global__ void __launch_bounds__(kBeamThreads + 32, sizeof(T) == 2 ? 2 : 3) beam_rows_kernel(const BeamRowsParams p) {
+  constexpr int VE = VecTraits<T>::kElems, kLow = sizeof(T) == 2 ? 16 : 0;
+  constexpr uint64_t kBudget = 2000000000ull;
+  extern __shared__ __align__(128) uint4 ring[];
   __shared__ uint64_t buf[kBeamWarps][kBeamCap];
-  __shared__ uint64_t all[kBeamWarps * kBeamMaxK];
+  uint64_t* all = reinterpret_cast<uint64_t*>(ring);  // at the end: [kBeamWarps * kBeamMaxK]
+  __shared__ uint64_t full[kBeamStages], empty[kBeamStages];
   __shared__ float2 stat[kBeamWarps];
   __shared__ uint32_t floor_key;  // at least k of the chunk's values have this key or a higher one
-  __shared__ int total, count[kBeamWarps];
+  __shared__ int total, count[kBeamWarps], abort_sh;
+  volatile int* abort = &abort_sh;
   pdl_launch();
   pdl_wait();
   const int row = blockIdx.y, ch = blockIdx.x;
   if (p.finished && p.finished[row]) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = ch * p.chunk, c1 = max(c0, min(p.V, c0 + p.chunk));
+  const T* x = static_cast<const T*>(p.logits) + int64_t(row) * p.ld;
+  const int off = int((reinterpret_cast<uintptr_t>(x + c0) & 15u) / sizeof(T));
+  const int head = min(c1 - c0, off ? VE - off : 0);  // columns before the first vector
+  const int nvec = (c1 - c0 - head) / VE, tail = c1 - c0 - head - nvec * VE;
+  const int v0 = c0 + head;  // first column of vector 0
+  const int rounds = (nvec + kBeamRound - 1) / kBeamRound;
+  auto copy = [&](int r) {  // one thread
+    const int s = r % kBeamStages, n = min(kBeamRound, nvec - r * kBeamRound);
+    mbar_arrive_expect_tx(full + s, uint32_t(n) * 16);
+    bulk_g2s(ring + s * kBeamRound, x + v0 + int64_t(r) * kBeamRound * VE, uint32_t(n) * 16, full + s);
+  };
+  if (threadIdx.x == kBeamThreads) {
+    for (int s = 0; s < kBeamStages; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, kBeamWarps);
+    }
+    mbar_init_fence();
+    for (int r = 0; r < min(rounds, kBeamStages); ++r) copy(r);
+  }
   if (threadIdx.x == 0) {
     floor_key = 0;
     total = 0;
+    *abort = 0;
   }
   __syncthreads();
-  const int c0 = ch * p.chunk, c1 = min(p.V, c0 + p.chunk);
-  const T* x = static_cast<const T*>(p.logits) + int64_t(row) * p.ld;
-  // whole 16-byte vectors from the one that holds column c0; col0 + i * VE is the first column of vector i
-  const int skew = int((reinterpret_cast<uintptr_t>(x + c0) & 15u) / sizeof(T));
-  const int col0 = c0 - skew;
-  const int nvec = c1 > c0 ? (c1 - col0 + VE - 1) / VE : 0;
-  auto load = [&](uint4 (&v)[kBeamVecs], int tile) {
-#pragma unroll
-    for (int u = 0; u < kBeamVecs; ++u) {
-      const int i = (tile * kBeamVecs + u) * 32 + lane, col = col0 + i * VE;
-      if (i < nvec && col >= c0 && col + VE <= c1) {
-        v[u] = ld_stream(x + col);
-      } else {  // the chunk's ends: the columns inside it, -inf for the others
-        float f[VE];
-#pragma unroll
-        for (int e = 0; e < VE; ++e)
-          f[e] = i < nvec && col + e >= c0 && col + e < c1 ? to_f(x[col + e]) : -INFINITY;
-        v[u] = pack_vec(f);
-      }
-    }
-  };
-  BeamList l{buf[warp], 0, 0x00800000u, 0u};  // least: the key of the lowest finite value
+  BeamList l{buf[warp & 7], 0, 0x00800000u, 0u};  // least: the key of the lowest finite value
   float m = -INFINITY, c = 0.f, s = 0.f;  // reference and sum of this lane
-  const int ntile = (nvec + 32 * kBeamVecs - 1) / (32 * kBeamVecs);
-  const bool rounds = ntile > kBeamWarps;
-  uint4 v[kBeamVecs], next[kBeamVecs];
-  if (warp < ntile) load(v, warp);
-  for (int t = warp; t < ntile; t += kBeamWarps) {
-    if (t + kBeamWarps < ntile) load(next, t + kBeamWarps);
+  // after the rounds 1, 2, 4, 8 .. (all of them full) the k-th of all warps' candidates becomes the floor:
+  // a later value enters with odds k / (values seen), not k / (values of one warp's first tile)
+  auto refloor = [&](int r) { return r + 1 < rounds && (r & (r + 1)) == 0; };
+  // a tile: vector u of this lane holds columns col + u * 32 * VE ..
+  auto tile = [&](const uint4 (&v)[kBeamVecs], int col, bool first) {
     float q[kBeamVecs];  // max of each vector (a NaN is passed over)
 #pragma unroll
     for (int u = 0; u < kBeamVecs; ++u) {
@@ -273,19 +309,18 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
     }
     s += part;
     // ---- candidates
-    if (t == warp) {
+    if (first) {
       // the k-th of the warp's 32 * kBeamVecs vector maxima: k values lie at or above it
       uint32_t kq[kBeamVecs];
 #pragma unroll
       for (int u = 0; u < kBeamVecs; ++u) kq[u] = beam_logit_key(q[u]);
       const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(kq[0], kq[1]), max(kq[2], kq[3])));
       const uint32_t least = __reduce_min_sync(0xffffffffu, min(min(kq[0], kq[1]), min(kq[2], kq[3])));
-      // (bf16 values differ in the upper half of their keys only)
-      const uint32_t cut = beam_search(p.k, least, most, sizeof(T) == 2 ? 16 : 0, [&](uint32_t x) {
-        int n = 0;
+      const uint32_t cut = beam_search(p.k, least, most, kLow, [&](uint32_t x) {
+        uint32_t n = 0;
 #pragma unroll
-        for (int u = 0; u < kBeamVecs; ++u) n += __popc(__ballot_sync(0xffffffffu, kq[u] >= x));
-        return n;
+        for (int u = 0; u < kBeamVecs; ++u) n += kq[u] >= x ? 1u : 0u;
+        return int(__reduce_add_sync(0xffffffffu, n));
       });
       if (lane == 0) atomicMax(&floor_key, cut);
       l.least = max(l.least, cut);
@@ -313,55 +348,119 @@ __global__ void __launch_bounds__(kBeamThreads) beam_rows_kernel(const BeamRowsP
           const int word = e * int(sizeof(T)) / 4;
           const uint32_t bits = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
           const float val = sizeof(T) == 4 ? __uint_as_float(bits) : __uint_as_float(e & 1 ? bits & 0xFFFF0000u : bits << 16);
-          const uint32_t id = uint32_t(p.vstart + col0 + ((t * kBeamVecs + u) * 32 + lane) * VE + e);
+          const uint32_t id = uint32_t(p.vstart + col + u * 32 * VE + e);
           l.buf[l.n + __popc(b & ((1u << lane) - 1u))] = beam_key(beam_logit_key(val), id);
         }
         l.n += __popc(b);
         __syncwarp();
-        if (l.n > kBeamCap - 32) beam_cut(l, p.k, &floor_key);
+        if (l.n > kBeamCap - 32) beam_cut<kLow>(l, p.k, &floor_key);
       }
       // later columns have higher ids: they have to beat the k-th, not to equal it
       if (l.kth) l.least = max(l.least, l.kth + 1);
     }
+  };
+  auto edge = [&](int n, int col) {  // columns col .. col + n - 1, n < VE
+    uint4 v[kBeamVecs];
 #pragma unroll
-    for (int u = 0; u < kBeamVecs; ++u) v[u] = next[u];
-    if (t == warp && rounds) {  // every warp is here: it has a first tile, and others follow
-      if (lane == 0) count[warp] = l.n;
-      __syncthreads();
-      if (warp == 0) beam_floor(buf, count, p.k, &floor_key);
+    for (int u = 0; u < kBeamVecs; ++u) {
+      float f[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[e] = u == 0 && e == 0 && lane < n ? to_f(x[col + lane]) : -INFINITY;
+      v[u] = pack_vec(f);
     }
-  }
-  // ---- the chunk's sum
-  float cm = m;
+    tile(v, col + lane, false);
+  };
+  if (warp == kBeamWarps) {
+    if (lane == 0) {
+      int r = kBeamStages;
+      for (; r < rounds; ++r) {
+        if (!mbar_wait_soon(empty + r % kBeamStages, uint32_t((r / kBeamStages) & 1) ^ 1u, kBudget, abort)) {
+          *abort = 1;
+          break;
+        }
+        copy(r);
+      }
+      if (*abort) {  // copies in flight land before the memory goes away
+        int never = 0;
+        for (int i = max(0, min(r, rounds) - kBeamStages); i < min(r, rounds); ++i)
+          mbar_wait(full + i % kBeamStages, uint32_t((i / kBeamStages) & 1), kBudget, &never);
+      }
+    }
+    __syncwarp();
+  } else {
+    if (warp == 0 && head) edge(head, c0);
+    for (int r = 0; r < rounds; ++r) {
+      const int sg = r % kBeamStages, at = r * kBeamRound + warp * 32 * kBeamVecs + lane;
+      const bool ok = mbar_wait_soon(full + sg, uint32_t((r / kBeamStages) & 1), kBudget, abort);
+      if (!__all_sync(0xffffffffu, ok)) {
+        *abort = 1;
+        for (int i = r; i < rounds; ++i)
+          if (refloor(i)) {  // the others come there
+            named_sync(1, kBeamThreads);
+            named_sync(1, kBeamThreads);
+          }
+        break;
+      }
+      uint4 v[kBeamVecs];
+      constexpr uint32_t kNone = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;  // -inf
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
-  s = warp_sum(s * beam_weight(m, cm));
-  if (lane == 0) stat[warp] = make_float2(cm, s);
-  // ---- the chunk's k best: the warps' candidates (at most 64 each) from the common floor on, ranked
-  if (l.n > kBeamMaxK) beam_cut(l, p.k, &floor_key);
+      for (int u = 0; u < kBeamVecs; ++u)
+        v[u] = at + 32 * u < nvec ? ring[sg * kBeamRound + warp * 32 * kBeamVecs + lane + 32 * u]
+                                  : make_uint4(kNone, kNone, kNone, kNone);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + sg);
+      if (at - lane >= nvec) break;  // nothing more for this warp (the last round)
+      tile(v, v0 + at * VE, r == 0);
+      if (refloor(r)) {
+        beam_drop(l, *reinterpret_cast<volatile uint32_t*>(&floor_key));
+        if (lane == 0) count[warp] = l.n;
+        named_sync(1, kBeamThreads);
+        uint32_t key[kBeamWarps];
+        if (warp == 0) {
+#pragma unroll
+          for (int w = 0; w < kBeamWarps; ++w) key[w] = lane < count[w] ? uint32_t(buf[w][lane] >> 32) : 0;
+        }
+        named_sync(1, kBeamThreads);  // the buffers may change again
+        if (warp == 0) beam_floor<kLow>(key, p.k, &floor_key);
+      }
+    }
+    if (warp == kBeamWarps - 1 && tail) edge(tail, c1 - tail);
+  }
   __syncthreads();
-  const uint32_t fk = floor_key;
-  for (int i = lane; i < l.n; i += 32) {
-    const uint64_t o = l.buf[i];
-    if (uint32_t(o >> 32) >= fk) all[atomicAdd(&total, 1)] = o;
-  }
-  __syncthreads();
-  const int n = total;
-  uint64_t* out = p.cand + (size_t(row) * p.nchunk + ch) * p.k;
-  for (int i = threadIdx.x; i < n; i += kBeamThreads) {
-    const uint64_t o = all[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += all[j] > o ? 1 : 0;
-    if (rank < p.k) out[rank] = o;
-  }
-  for (int i = n + threadIdx.x; i < p.k; i += kBeamThreads) out[i] = 0;
-  if (threadIdx.x == 0) {
-    float m = -INFINITY, sum = 0.f;
+  if (*abort && threadIdx.x == 0) atomicOr(&g_beam_status, kStatusTimeout);
+  if (warp < kBeamWarps) {
+    // ---- the chunk's sum
+    float cm = m;
 #pragma unroll
-    for (int w = 0; w < kBeamWarps; ++w) m = fmaxf(m, stat[w].x);
+    for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
+    s = warp_sum(s * beam_weight(m, cm));
+    if (lane == 0) stat[warp] = make_float2(cm, s);
+    // ---- the chunk's k best: the warps' candidates (at most 64 each) from the common floor on, ranked
+    if (l.n > kBeamMaxK) beam_cut<kLow>(l, p.k, &floor_key);
+    named_sync(1, kBeamThreads);
+    const uint32_t fk = floor_key;
+    for (int i = lane; i < l.n; i += 32) {
+      const uint64_t o = l.buf[i];
+      if (uint32_t(o >> 32) >= fk) all[atomicAdd(&total, 1)] = o;
+    }
+    named_sync(1, kBeamThreads);
+    const int n = total;
+    uint64_t* out = p.cand + (size_t(row) * p.nchunk + ch) * p.k;
+    for (int i = threadIdx.x; i < n; i += kBeamThreads) {
+      const uint64_t o = all[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += all[j] > o ? 1 : 0;
+      if (rank < p.k) out[rank] = o;
+    }
+    for (int i = n + threadIdx.x; i < p.k; i += kBeamThreads) out[i] = 0;
+    if (threadIdx.x == 0) {
+      float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kBeamWarps; ++w) sum += stat[w].y * beam_weight(stat[w].x, m);
-    p.stat[size_t(row) * p.nchunk + ch] = BeamStat{m, sum};
+      for (int w = 0; w < kBeamWarps; ++w) top = fmaxf(top, stat[w].x);
+#pragma unroll
+      for (int w = 0; w < kBeamWarps; ++w) sum += stat[w].y * beam_weight(stat[w].x, top);
+      p.stat[size_t(row) * p.nchunk + ch] = BeamStat{top, sum};
+    }
   }
 }
 

@@ -64,8 +64,9 @@ int beam_rows(const void* logits, long long ld, int rows, int V, long long vstar
   p.cand = static_cast<uint64_t*>(block);
   p.stat = reinterpret_cast<BeamStat*>(static_cast<char*>(block) + beam_cand_bytes(rows, b, k));
   const dim3 grid(b.nchunk, rows);
-  return dtype == MTPB_BF16 ? host_launch(beam_rows_kernel<bf16>, grid, dim3(kBeamThreads), 0, st, p)
-                            : host_launch(beam_rows_kernel<float>, grid, dim3(kBeamThreads), 0, st, p);
+  const dim3 threads(kBeamThreads + 32);
+  return dtype == MTPB_BF16 ? host_launch(beam_rows_kernel<bf16>, grid, threads, kBeamRing, st, p)
+                            : host_launch(beam_rows_kernel<float>, grid, threads, kBeamRing, st, p);
 }
 
 int beam_pick(const void* blocks, int parts, int G, int W, int V_plan, int kc, const float* scores,
@@ -476,3 +477,17 @@ int mtpb_shared_attention(const void* q, const void* k_prefix, const void* v_pre
 }
 
 }  // extern "C"
+
+extern "C" int mtpb_beam_status(uint32_t* status_out) {
+  if (!status_out) return bad("beam_status: null argument");
+  uint32_t a = 0, b = 0;
+  const uint32_t zero = 0;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&a, g_sa_status, sizeof(a));
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&b, g_beam_status, sizeof(b));
+  if (e == cudaSuccess && a) e = cudaMemcpyToSymbol(g_sa_status, &zero, sizeof(zero));
+  if (e == cudaSuccess && b) e = cudaMemcpyToSymbol(g_beam_status, &zero, sizeof(zero));
+  if (e != cudaSuccess) return host_fail_cuda(e, "beam_status");
+  *status_out = a | b;
+  return MTPB_OK;
+}

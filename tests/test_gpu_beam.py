@@ -348,3 +348,14 @@ def test_attention_streams_and_graph(lib):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(o, want[i])
+
+
+def test_status_is_clean(lib):
+    """No bounded wait of the calls above ran out."""
+    import ctypes
+
+    from minitp_b200 import _lib
+
+    st = ctypes.c_uint32(7)
+    _lib.call("mtpb_beam_status", ctypes.byref(st))
+    assert st.value == 0
