@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   constexpr int NB = C::kRing;
   constexpr uint64_t kBudget = 2000000000ull;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2][2], pv_done[2], drain[2];
+  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2][2], pv_done[2], drain[2], turn[2][4];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_sh;
   __shared__ float2 ml_sh[128];  // MT 1: stream 1's statistics
@@ -664,6 +664,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
       for (int h = 0; h < 2; ++h) mbar_init(&p_full[x][h], 4);
       mbar_init(pv_done + x, 1);
       mbar_init(drain + x, 1);
+      for (int q = 0; q < 4; ++q) mbar_init(&turn[x][q], 1);
     }
     *abort = 0;
     mbar_init_fence();
@@ -761,23 +762,26 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
     // ---- softmax of stream x
     const int stid = int(threadIdx.x) - 128, x = stid >> 7;
     const int quarter = warp & 3, r = quarter * 32 + lane;
-    {  // Q: a row (MT 1: half a row) a thread, all loads in flight at once
-      constexpr int N = HD / 8 / (3 - MT);
-      const int row = MT == 2 ? stid : stid & 127, c0 = MT == 2 ? 0 : x * N;
-      uint4 v[N];
-      if (row < it.rows) {
-        const SaRow w = sa_row(p, it, row);
-        const bf16* q = static_cast<const bf16*>(p.q) + ((size_t(w.n) * p.T + w.t) * p.hq + w.head) * HD + c0 * 8;
-#pragma unroll
-        for (int c = 0; c < N; ++c) v[c] = ld_vec(q + c * 8);
-      } else {
-#pragma unroll
-        for (int c = 0; c < N; ++c) v[c] = make_uint4(0, 0, 0, 0);
+    {  // Q: a warp's rows, whole rows side by side in the lanes, all loads in flight at once
+      constexpr int RW = 16 * MT, CH = HD / 8, RI = 32 / CH, N = RW / RI;  // rows a warp, chunks a row, rows a load
+      const int row0 = (warp - 4) * RW, at = row0 + (lane & (RW - 1));
+      unsigned long long off = ~0ull;  // of row `at` in q
+      if (at < it.rows) {
+        const SaRow w = sa_row(p, it, at);
+        off = ((size_t(w.n) * p.T + w.t) * p.hq + w.head) * HD;
       }
-      unsigned char* dst = smem + (row >> 7) * C::kTile + (row & 127) * 128;
+      uint4 v[N];
 #pragma unroll
-      for (int c = 0; c < N; ++c)
-        *reinterpret_cast<uint4*>(dst + ((c0 + c) >> 3) * kSaTcSub + ((((c0 + c) & 7) ^ (row & 7)) << 4)) = v[c];
+      for (int i = 0; i < N; ++i) {
+        const unsigned long long o = __shfl_sync(0xffffffffu, off, i * RI + lane / CH);
+        v[i] = o != ~0ull ? ld_vec(static_cast<const bf16*>(p.q) + o + (lane % CH) * 8) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = row0 + i * RI + lane / CH, c = lane % CH;
+        *reinterpret_cast<uint4*>(smem + (row >> 7) * C::kTile + (c >> 3) * kSaTcSub + (row & 127) * 128 +
+                                  (((c & 7) ^ (row & 7)) << 4)) = v[i];
+      }
     }
     fence_async_smem();
     __syncwarp();
@@ -857,6 +861,12 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
         }
         fence_async_smem();
       }
+      // the exponentials of the two warps of a scheduler take turns: one stream's
+      // run under the other's MMAs, and not both at half pace (51.3 -> 49.1 us)
+      if (x == 1 || k > 0) {
+        ok = mbar_wait_soon(&turn[x][quarter], uint32_t(x == 1 ? k & 1 : (k - 1) & 1), kBudget, abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       // kCubic of 16 pairs on the fp32 pipe, which the special-function unit
       // (8 cycles a warp and value) leaves idle; masked tiles need exact zeros
@@ -878,6 +888,10 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
             pk[i / 2] = pack_bf16(e.x, e.y);
           }
           tc_st16(tp + c / 2, pk);
+          if (c == kSaTcKeys - 32) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&turn[1 - x][quarter]);
+          }
           if (c & 32) {  // half of the keys
             tc_wait_st();
             tc_fence_before();
