@@ -10,7 +10,37 @@
 
 #include <cudaTypedefs.h>
 
+#include <mutex>
+
 using namespace mtpb;
+
+namespace mtpb {
+
+cudaError_t host_allow_smem(const void* kern, size_t smem) noexcept {
+  struct Entry {
+    const void* kern;
+    int dev;
+    size_t smem;
+  };
+  static Entry known[64];
+  static int n = 0;
+  static std::mutex mu;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  int i = 0;
+  while (i < n && (known[i].kern != kern || known[i].dev != dev)) ++i;
+  if (i < n && known[i].smem >= smem) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e == cudaSuccess && i < 64) {  // (a full table asks again each time)
+    known[i] = Entry{kern, dev, smem};
+    n = std::max(n, i + 1);
+  }
+  return e;
+}
+
+}  // namespace mtpb
 
 namespace {
 

@@ -19,6 +19,10 @@ bool host_pdl() noexcept;
 // cuTensorMapEncodeTiled (a PFN_cuTensorMapEncodeTiled_v12000), or NULL.
 void* host_tensor_map_encoder() noexcept;
 
+// Lets `kern` use `smem` bytes of shared memory on the current device (asked
+// of the driver once for each kernel, device and larger size).
+cudaError_t host_allow_smem(const void* kern, size_t smem) noexcept;
+
 // Multiprocessors of the current device (a constant of the device, asked once).
 inline int host_sms() {
   static int per_dev[64] = {};
@@ -36,7 +40,7 @@ inline int host_sms() {
 template <typename Kern, typename... Args>
 int host_launch(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const Args&... args) {
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    const cudaError_t e = host_allow_smem(reinterpret_cast<const void*>(kern), smem);
     if (e != cudaSuccess) return host_fail_cuda(e, "cudaFuncSetAttribute");
   }
   cudaLaunchConfig_t cfg = {};

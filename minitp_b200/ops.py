@@ -232,8 +232,8 @@ def _beam_inputs(name: str, logits, scores, k, finished, eos_token_id, least: in
 
 
 def _beam_outputs(dev, g: int, k: int, flags: bool):
-    parents, tokens = torch.empty((2, g, k), dtype=torch.int64, device=dev).unbind(0)
-    return (torch.empty((g, k), dtype=torch.float32, device=dev), parents, tokens,
+    parents = torch.empty((g, k), dtype=torch.int64, device=dev)
+    return (torch.empty((g, k), dtype=torch.float32, device=dev), parents, torch.empty_like(parents),
             torch.empty((g, k), dtype=torch.bool, device=dev) if flags else None)
 
 
