@@ -25,6 +25,11 @@
 
 using namespace mtpb;
 
+// Bumped by every mtpb_set_* call and whenever a buffer that belongs to a model
+// moves: a CUDA graph captured over the library bakes in the settings and the
+// addresses of its capture, so holders of a graph compare epochs.
+std::atomic<uint64_t> g_settings_epoch{0};
+
 namespace {
 
 thread_local std::string g_err;
@@ -519,6 +524,7 @@ int attn_run(int dtype, const void* q, const void* kc, const void* vc, void* out
       cudaStreamIsCapturing(st, &cs);
       if (cs != cudaStreamCaptureStatusNone)
         return fail(MTPB_ERR_INVALID, "attention scratch must be reserved before graph capture");
+      g_settings_epoch.fetch_add(1);
       cudaFree(scr.part_o);
       cudaFree(scr.part_ml);
       cudaFree(scr.counters);
@@ -741,8 +747,10 @@ int model_reserve(ModelHost& mh, int rows, cudaStream_t st) {
   const size_t lb = size_t(64) * size_t(d.vocab_end - d.vocab_start) * es;
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   const size_t total = up(qb) * 2 + up(ab) + up(hb) * 3 + up(lb) + 64 * 8;
+  g_settings_epoch.fetch_add(1);  // graphs captured over the old buffers must not run again
   cudaFree(mh.scratch);
   mh.scratch = nullptr;
+  mh.reserved_rows = 0;
   MTPB_CUDA(cudaMalloc(&mh.scratch, total));
   char* p = mh.scratch;
   mh.q = p; p += up(qb);
@@ -822,6 +830,7 @@ int shared_reserve(ModelHost& mh, const FwdArgs& a, int tc, cudaStream_t st) {
   if (need < 0) return int(need);
   if (size_t(need) <= mh.sa_bytes) return MTPB_OK;
   if (capturing(st)) return fail(MTPB_ERR_INVALID, "shared-prefix forward: run one call eagerly before graph capture");
+  g_settings_epoch.fetch_add(1);
   MTPB_CUDA(cudaFree(mh.sa_ws));  // waits for the kernels that use it
   mh.sa_ws = nullptr;
   mh.sa_bytes = 0;
@@ -1309,10 +1318,6 @@ void* host_tensor_map_encoder() noexcept { return reinterpret_cast<void*>(tensor
 // =====================================================================
 // extern "C"
 // =====================================================================
-// Bumped by every mtpb_set_* call: a CUDA graph captured over the library
-// bakes in the settings of its capture, so holders of a graph compare epochs.
-std::atomic<uint64_t> g_settings_epoch{0};
-
 extern "C" {
 
 const char* mtpb_last_error(void) { return g_err.c_str(); }
@@ -1674,6 +1679,7 @@ int mtpb_model_reserve(void* model, int max_rows, int max_cap) {
     const size_t need_o = size_t(M) * mh->d.hq_local * ns * mh->d.head_dim;
     const size_t need_ml = size_t(M) * mh->d.hq_local * ns * 2, need_c = size_t(M) * mh->d.hkv_local;
     if (need_o > s.o_elems || need_ml > s.ml_elems || need_c > s.ctr_elems) {
+      g_settings_epoch.fetch_add(1);
       cudaFree(s.part_o);
       cudaFree(s.part_ml);
       cudaFree(s.counters);

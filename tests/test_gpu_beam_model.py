@@ -193,3 +193,27 @@ def test_forward_refuses_caches_that_do_not_fit(lib):
         generate_beam(gpu, ids, 0, 2)
     with pytest.raises(ValueError, match="divide"):
         generate_shared_prefix(gpu, ids[:2], ids, 4)
+
+
+def test_graphs_kept_over_a_larger_prompt(lib):
+    """A later, larger prompt moves the model's buffers: the graphs captured before it are not replayed over the old ones."""
+    from minitp_b200.beam import generate_beam, generate_shared_prefix
+    from minitp_b200.generation import generate_greedy
+
+    gpu, _, cfg = _models()
+    gpu.release_native()  # the smallest buffers again
+    pre, ids = _prompt(cfg, 1, 40, 1).cuda(), _prompt(cfg, 12, 3, 2).cuda()
+
+    def small():
+        return (generate_shared_prefix(gpu, pre, ids, 6), generate_beam(gpu, ids[:2], 6, 6)[0],
+                generate_greedy(gpu, ids, 6, early_stop=False))  # 12 rows: a graph of the kernel chain
+
+    want = small()
+    for length in (100, 300):
+        generate_greedy(gpu, _prompt(cfg, 14, length, 3).cuda(), 3, early_stop=False)
+        generate_shared_prefix(gpu, _prompt(cfg, 1, 10 * length, 4).cuda(), ids, 3)
+        torch.cuda.synchronize()
+        again = small()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(again, want))
+    assert gpu.ctx.comm().status() == 0
