@@ -196,7 +196,7 @@ __device__ __forceinline__ void beam_floor(const uint32_t (&key)[kBeamWarps], in
 }
 
 // The chunk's 16-byte vectors come through a ring in shared memory, 16 KB
-// rounds filled by bulk copies (warp 8), so that what is in flight does not
+// rounds filled by bulk copies (warp 8, which also finds the floors), so that what is in flight does not
 // depend on the registers of the warps that compute. Warp w < 8 takes vectors
 // 128 w .. of each round; columns before the first and behind the last whole
 // vector are warp 0's first and warp 7's last.
@@ -315,7 +315,9 @@ __global__ void __launch_bounds__(kBeamThreads + 32, sizeof(T) == 2 ? 2 : 3) bea
 #pragma unroll
       for (int u = 0; u < kBeamVecs; ++u) kq[u] = beam_logit_key(q[u]);
       const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(kq[0], kq[1]), max(kq[2], kq[3])));
-      const uint32_t least = __reduce_min_sync(0xffffffffu, min(min(kq[0], kq[1]), min(kq[2], kq[3])));
+      // 32 lanes reach the least of their maxima; for more than 32 the least of all bounds the k-th
+      const uint32_t least = __reduce_min_sync(0xffffffffu, p.k <= 32 ? max(max(kq[0], kq[1]), max(kq[2], kq[3]))
+                                                                      : min(min(kq[0], kq[1]), min(kq[2], kq[3])));
       const uint32_t cut = beam_search(p.k, least, most, kLow, [&](uint32_t x) {
         uint32_t n = 0;
 #pragma unroll
@@ -371,20 +373,32 @@ __global__ void __launch_bounds__(kBeamThreads + 32, sizeof(T) == 2 ? 2 : 3) bea
     tile(v, col + lane, false);
   };
   if (warp == kBeamWarps) {
-    if (lane == 0) {
-      int r = kBeamStages;
-      for (; r < rounds; ++r) {
-        if (!mbar_wait_soon(empty + r % kBeamStages, uint32_t((r / kBeamStages) & 1) ^ 1u, kBudget, abort)) {
+    int copied = min(rounds, kBeamStages);
+    for (int r = 0; r + 1 < rounds; ++r) {
+      if (r + kBeamStages < rounds && !__any_sync(0xffffffffu, *abort)) {
+        const bool ok =
+            mbar_wait_soon(empty + r % kBeamStages, uint32_t((r / kBeamStages) & 1), kBudget, abort);
+        if (__all_sync(0xffffffffu, ok)) {
+          if (lane == 0) copy(r + kBeamStages);
+          copied = r + kBeamStages + 1;
+        } else {
           *abort = 1;
-          break;
         }
-        copy(r);
+        __syncwarp();
       }
-      if (*abort) {  // copies in flight land before the memory goes away
-        int never = 0;
-        for (int i = max(0, min(r, rounds) - kBeamStages); i < min(r, rounds); ++i)
-          mbar_wait(full + i % kBeamStages, uint32_t((i / kBeamStages) & 1), kBudget, &never);
+      if (refloor(r)) {  // (with or without an abort: the other warps come there)
+        named_sync(1, kBeamThreads + 32);
+        uint32_t key[kBeamWarps];
+#pragma unroll
+        for (int w = 0; w < kBeamWarps; ++w) key[w] = lane < count[w] ? uint32_t(buf[w][lane] >> 32) : 0;
+        named_sync(1, kBeamThreads + 32);  // the buffers may change again
+        beam_floor<kLow>(key, p.k, &floor_key);
       }
+    }
+    if (*abort) {  // copies in flight land before the memory goes away
+      int never = 0;
+      for (int i = max(0, copied - kBeamStages); i < copied; ++i)
+        mbar_wait(full + i % kBeamStages, uint32_t((i / kBeamStages) & 1), kBudget, &never);
     }
     __syncwarp();
   } else {
@@ -396,8 +410,9 @@ __global__ void __launch_bounds__(kBeamThreads + 32, sizeof(T) == 2 ? 2 : 3) bea
         *abort = 1;
         for (int i = r; i < rounds; ++i)
           if (refloor(i)) {  // the others come there
-            named_sync(1, kBeamThreads);
-            named_sync(1, kBeamThreads);
+            if (lane == 0) count[warp] = 0;
+            named_sync(1, kBeamThreads + 32);
+            named_sync(1, kBeamThreads + 32);
           }
         break;
       }
@@ -414,14 +429,8 @@ __global__ void __launch_bounds__(kBeamThreads + 32, sizeof(T) == 2 ? 2 : 3) bea
       if (refloor(r)) {
         beam_drop(l, *reinterpret_cast<volatile uint32_t*>(&floor_key));
         if (lane == 0) count[warp] = l.n;
-        named_sync(1, kBeamThreads);
-        uint32_t key[kBeamWarps];
-        if (warp == 0) {
-#pragma unroll
-          for (int w = 0; w < kBeamWarps; ++w) key[w] = lane < count[w] ? uint32_t(buf[w][lane] >> 32) : 0;
-        }
-        named_sync(1, kBeamThreads);  // the buffers may change again
-        if (warp == 0) beam_floor<kLow>(key, p.k, &floor_key);
+        named_sync(1, kBeamThreads + 32);
+        named_sync(1, kBeamThreads + 32);  // warp 8 has the keys; it finds the floor under the next round
       }
     }
     if (warp == kBeamWarps - 1 && tail) edge(tail, c1 - tail);
@@ -437,13 +446,13 @@ __global__ void __launch_bounds__(kBeamThreads + 32, sizeof(T) == 2 ? 2 : 3) bea
     if (lane == 0) stat[warp] = make_float2(cm, s);
     // ---- the chunk's k best: the warps' candidates (at most 64 each) from the common floor on, ranked
     if (l.n > kBeamMaxK) beam_cut<kLow>(l, p.k, &floor_key);
-    named_sync(1, kBeamThreads);
+    named_sync(2, kBeamThreads);
     const uint32_t fk = floor_key;
     for (int i = lane; i < l.n; i += 32) {
       const uint64_t o = l.buf[i];
       if (uint32_t(o >> 32) >= fk) all[atomicAdd(&total, 1)] = o;
     }
-    named_sync(1, kBeamThreads);
+    named_sync(2, kBeamThreads);
     const int n = total;
     uint64_t* out = p.cand + (size_t(row) * p.nchunk + ch) * p.k;
     for (int i = threadIdx.x; i < n; i += kBeamThreads) {
