@@ -500,6 +500,7 @@ __device__ __forceinline__ bool beam_better(const BeamCand& x, const BeamCand& y
 
 constexpr int kPickCap = 512;  // candidates ranked against each other
 constexpr int kPickHeld = 4;   // keys a thread keeps in registers
+constexpr int kPickAll = 96;   // candidates ranked without a floor
 
 __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickParams p) {
   // of each beam: total = (x - top) + base
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
   pdl_wait();
   const int g = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per = p.nchunk * p.kc, n = p.parts * p.W * per;
-  // candidate i is of beam b; its key (0 for a finished beam's, which were not written)
+  // candidate i is of beam b; its key (a finished beam's were not written, and are not used)
   auto where = [&](int i, int& q, int& b, int& o) {
     q = i / (p.W * per);
     const int r = i - q * p.W * per;
@@ -523,8 +524,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
   auto key_at = [&](int i) -> uint64_t {
     int q, b, o;
     where(i, q, b, o);
-    const int row = g * p.W + b;
-    return p.finished && p.finished[row] ? 0 : p.cand[q * p.cand_part + size_t(row) * per + o];
+    return __ldcg(p.cand + q * p.cand_part + size_t(g * p.W + b) * per + o);
   };
   uint64_t held[kPickHeld];  // the keys of the first candidates of each thread, loaded under the sums
 #pragma unroll
@@ -546,17 +546,20 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
         const int q = i / p.nchunk;
         return p.stat[q * p.stat_part + size_t(row) * p.nchunk + (i - q * p.nchunk)];
       };
-      for (int i = lane; i < n; i += 32) m = fmaxf(m, at(i).m);
+      const BeamStat mine = lane < n ? at(lane) : BeamStat{-INFINITY, 0.f};
+      m = mine.m;
+      for (int i = lane + 32; i < n; i += 32) m = fmaxf(m, at(i).m);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       double s = 0.0;
-      for (int i = lane; i < n; i += 32) {
-        const BeamStat t = at(i);
+      auto add = [&](const BeamStat& t) {
         if (t.m == m)
           s += double(t.s);
         else if (!beam_far(m))
           s += double(t.s) * exp2(double(beam_ref(t.m)) - double(beam_ref(m)));
-      }
+      };
+      add(mine);
+      for (int i = lane + 32; i < n; i += 32) add(at(i));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       // log sum exp - m, the rounding of the reference taken out
@@ -595,20 +598,21 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
       if (tid + h * kBeamThreads < n) f(cand(tid + h * kBeamThreads, held[h]));
     for (int i = tid + kPickHeld * kBeamThreads; i < n; i += kBeamThreads) f(cand(i, key_at(i)));
   };
-  // a floor that k candidates reach: the k-th of the threads' best totals, rounded to fp32 (which keeps the order)
-  float best = -INFINITY;
-  each([&](const BeamCand& c) { best = fmaxf(best, float(c.total)); });
-  const uint32_t key = beam_logit_key(best);
-  {
+  // a floor that k candidates reach: the k-th of the threads' best totals,
+  // rounded to fp32 (which keeps the order); few candidates are all ranked
+  uint32_t cut = 0;
+  if (n > kPickAll) {
+    float best = -INFINITY;
+    each([&](const BeamCand& c) { best = fmaxf(best, float(c.total)); });
+    const uint32_t key = beam_logit_key(best);
     const uint32_t hi = __reduce_max_sync(0xffffffffu, key), lo = __reduce_min_sync(0xffffffffu, key);
     if (lane == 0) {
       atomicMax(&most_sh, hi);
       atomicMin(&least_sh, lo);
     }
+    __syncthreads();
+    cut = beam_search(p.k, least_sh, most_sh, 0, [&](uint32_t v) { return __syncthreads_count(key >= v); });
   }
-  __syncthreads();
-  const uint32_t cut =
-      beam_search(p.k, least_sh, most_sh, 0, [&](uint32_t v) { return __syncthreads_count(key >= v); });
   each([&](const BeamCand& c) {
     const uint32_t ck = beam_logit_key(float(c.total));
     if (ck && ck >= cut) {
