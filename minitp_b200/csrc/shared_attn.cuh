@@ -641,7 +641,6 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
   pdl_wait();
-
   pdl_launch();  // after the wait: sa_token_kernel counts on it
   const SaItem it = sa_item<HD, 2>(p, blockIdx.x, 128 * MT, kSaTcKeys);
   if (it.j0 >= it.j1) {
