@@ -299,13 +299,16 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
     return int(std::max<long long>(1, std::min<long long>(std::min<long long>(most, kSaMaxSplits), (want + base - 1) / base)));
   };
   if (pl.token) {
-    // the prefix read by every row's CTA: one launch, but N / G reads of each
-    // position, through L2, and one CTA's pace along it
-    const long long pre = (long long)top_p * a.hd * 4;
-    pl.inline_pre = pre <= (256 << 10) && obase * pre <= (32ll << 20);
+    // long own caches of few rows in ranges of at least 512 keys (about 5 us of
+    // one CTA's pace), which a third launch joins
     pl.so = 1;
-    if (!pl.inline_pre)
-      while (obase * pl.so * 2 <= 2 * sms && top_o / (pl.so * 2) >= 256 && pl.so < 64) pl.so *= 2;
+    while (obase * pl.so * 2 <= 2 * sms && top_o / (pl.so * 2) >= 512 && pl.so < kSaMaxSplits) pl.so *= 2;
+    // the prefix read by every row's CTA: one launch, but N / G reads of each
+    // position, through L2, and one CTA's pace along it. 4 beams behind 128
+    // positions: 3.4 us against 7 with the tensor-core items; 8 x 8 beams
+    // behind 1024: 30 us against 21.
+    const long long pre = (long long)top_p * a.hd * 4;
+    pl.inline_pre = pl.so == 1 && pre <= (256 << 10) && obase * pre <= (32ll << 20);
   } else {
     pl.so = pl.tc ? sa_tc_splits(obase, top_o, pl.rows, a.hd, sms) : splits(obase, top_o);
   }

@@ -602,8 +602,10 @@ __global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const S
 // zeroed in shared memory, since 0 x NaN would not be 0.
 // ---------------------------------------------------------------------------
 constexpr int kSaTcKeys = 128;
-constexpr int kSaCubic = 4;  // of 16 pairs of exponentials, on the fp32 pipe (0: 54.2, 4: 52.9, 6: 55.0, 8: 60.1 us on
-                             // 64 rows of the 7B heads behind 16384 positions; 72, 69, 76, 76 us on 16 rows of 128 tokens)
+// Of 16 pairs of exponentials, on the fp32 pipe (0, 2, 4, 6: 46.6, 46.8, 46.5,
+// 47.1 us on 64 rows of the 7B heads behind 16384 positions; 67.4, 68.8, 65.9,
+// 71.2 us on 16 rows of 128 tokens behind 4001).
+constexpr int kSaCubic = 4;
 constexpr int kSaTcThreads = 384;
 constexpr uint32_t kSaTcSub = 128 * 64 * 2;  // a 128 x 64 bf16 subtile
 
@@ -886,18 +888,20 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
             sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
             pk[i / 2] = pack_bf16(e.x, e.y);
           }
-          tc_st16(tp + c / 2, pk);
-          if (c == kSaTcKeys - 32) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&turn[1 - x][quarter]);
-          }
-          if (c & 32) {  // half of the keys
+          if (c == 64) {  // the first half of the keys: its stores have landed meanwhile
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[x][c >> 6]);
+            if (lane == 0) mbar_arrive(&p_full[x][0]);
           }
+          tc_st16(tp + c / 2, pk);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&turn[1 - x][quarter]);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x][1]);
       };
       if (masked)
         exps(std::integral_constant<int, 0>{});

@@ -243,7 +243,7 @@ def _check_attention(case, hq, hkv):
     return got
 
 
-HEADS = [(4, 2, 16), (8, 4, 32), (14, 2, 64), (7, 1, 128), (28, 4, 128), (4, 1, 128), (3, 3, 64)]
+HEADS = [(4, 2, 16), (8, 4, 32), (14, 2, 64), (7, 1, 128), (28, 4, 128), (4, 1, 128), (3, 3, 64), (20, 1, 64)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
@@ -282,6 +282,16 @@ def test_attention_wide_groups_and_long_prefixes(lib, dtype):
     _check_attention(case, 7, 1)
     case = _attention_case(2, dtype, 2, 3, 1, 14, 2, 64, 5000, [4999, 2500], 700, [700, 1, 0, 333, 512, 640])
     _check_attention(case, 14, 2)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,hd", [(14, 2, 64), (4, 1, 128), (40, 2, 128)])
+def test_attention_long_own_caches_of_few_rows(lib, dtype, hq, hkv, hd):
+    """Own caches cut into key ranges, behind no prefix, a short one and one of many ranges."""
+    case = _attention_case(hq, dtype, 3, 1, 1, hq, hkv, hd, 3000, [0, 64, 2999], 2200, [2200, 700, 0])
+    _check_attention(case, hq, hkv)
+    case = _attention_case(hq + 1, dtype, 1, 2, 1, hq, hkv, hd, 1, [1], 4100, [4099, 1])
+    _check_attention(case, hq, hkv)
 
 
 def test_attention_large_scores_and_masked_infinities(lib):

@@ -217,3 +217,28 @@ def test_graphs_kept_over_a_larger_prompt(lib):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(again, want))
     assert gpu.ctx.comm().status() == 0
+
+
+def test_bf16_logits_behind_a_prefix(lib):
+    """bf16, the 0.5B shape with two layers: rows behind a shared prefix against the whole prompts, many tokens and
+    one at a time, within the framework's bf16 logit tolerance (0.5 absolute)."""
+    from minitp_b200.distributed.context import context_for
+    from minitp_b200.generation import make_kv_cache
+    from minitp_b200.weight_loader import load_synthetic_tp
+
+    cfg = mcfg.qwen25_05b(num_layers=2)
+    gpu = load_synthetic_tp(cfg, context_for(1, "cuda"), dtype=torch.bfloat16, device=torch.device("cuda"))
+    for groups, rows, p, t, cap in ((1, 12, 1500, 40, 64), (2, 4, 200, 1, 8)):
+        pre, ids = _prompt(cfg, groups, p, 1).cuda(), _prompt(cfg, rows, t + 3, 2).cuda()
+        prefix, own = make_kv_cache(gpu, groups, p + 5), make_kv_cache(gpu, rows, cap)
+        prefix.poison()
+        own.poison()
+        gpu(pre, kv_cache=prefix, last_only=True)
+        got = [gpu(ids[:, :t], kv_cache=own, prefix_cache=prefix)]
+        got += [gpu(ids[:, t + i:t + i + 1], kv_cache=own, prefix_cache=prefix) for i in range(3)]
+        got = torch.cat(got, 1).float()
+        whole = gpu(torch.cat([pre.repeat_interleave(rows // groups, 0), ids], 1))[:, p:].float()
+        assert bool(torch.isfinite(got).all())
+        assert float((got - whole).abs().max()) <= 0.5
+        assert float((got - whole).abs().max() / whole.abs().max()) <= 0.1
+    assert gpu.ctx.comm().status() == 0
