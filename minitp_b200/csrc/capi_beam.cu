@@ -242,7 +242,7 @@ struct SaPlan {
   bool inline_pre;  // it reads the prefix too: no other launch
   bool tc;          // the other items on sa_tc_kernel, else on the CUDA cores
   int mt;           // its row tiles a CTA
-  int rpt;  // CUDA-core items: rows a tile / 16
+  int prpt, orpt;  // CUDA-core items: rows a tile / 16, of prefix and of own items
   int sp, so, ptiles, otiles;
   int pblocks, oblocks;
   long long pitems, items;
@@ -285,13 +285,14 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   pl.tc = a.dtype == MTPB_BF16 && (a.hd == 64 || a.hd == 128);
   pl.token = pl.tc && a.T == 1 && N <= 65535;
   const long long prow = (long long)a.W * a.T * per, orow = (long long)a.T * per;
-  // CUDA-core items: row tiles of 64 when a row's tokens fill them, else of 16
-  pl.rpt = orow >= 64 ? 4 : 1;
+  // CUDA-core items: row tiles of 64 when there are as many rows, else of 16
+  pl.prpt = prow >= 64 ? 4 : 1;
+  pl.orpt = orow >= 64 ? 4 : 1;
   // two row tiles a CTA from the second on (for most items)
   pl.mt = prow > 128 ? 2 : 1;
-  const int tile = pl.tc ? 128 * pl.mt : 16 * pl.rpt;
-  pl.ptiles = int((prow + tile - 1) / tile);
-  pl.otiles = pl.token ? (per + 15) / 16 : int((orow + tile - 1) / tile);
+  const int ptile = pl.tc ? 128 * pl.mt : 16 * pl.prpt, otile = pl.token ? 16 : pl.tc ? 128 * pl.mt : 16 * pl.orpt;
+  pl.ptiles = int((prow + ptile - 1) / ptile);
+  pl.otiles = int((orow + otile - 1) / otile);
   const long long pbase = (long long)a.G * a.hkv * pl.ptiles, obase = N * a.hkv * pl.otiles;
   // key ranges until the items give every SM four, but none below two key tiles
   auto splits = [&](long long base, int top) {
@@ -375,10 +376,18 @@ int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
     }
   }
   if (!done) {
-    const int r = pl.rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)pl.items), dim3(kSaThreads),
-                                            sa_simt_smem<HD, 4>(), st, p)
-                              : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)pl.items), dim3(kSaThreads),
-                                            sa_simt_smem<HD, 1>(), st, p);
+    auto items = [&](int rpt, long long first, long long n) {
+      if (n == 0) return MTPB_OK;
+      SaParams q = p;
+      q.item0 = int(first);
+      return rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 4>(),
+                                    st, q)
+                      : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 1>(),
+                                    st, q);
+    };
+    const bool both = pl.prpt == pl.orpt;
+    int r = items(pl.prpt, 0, both ? pl.items : pl.pitems);
+    if (r == MTPB_OK && !both) r = items(pl.orpt, pl.pitems, pl.items - pl.pitems);
     if (r != MTPB_OK) return r;
   }
   if constexpr (sizeof(T) == 2 && HD >= 64) {

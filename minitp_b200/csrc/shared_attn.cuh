@@ -32,6 +32,7 @@ struct SaParams {
   int sp, so;        // key ranges of the prefix and of an own cache
   int ptiles, otiles;  // row tiles of a (group, KV head) and of a (row, KV head)
   int pitems, items;   // prefix items, all items
+  int item0;           // CUDA-core items: first of this launch
   // partial sums, in blocks of 32 rows (SaPart)
   int pblocks, oblocks;  // blocks of a prefix plane, of an own plane
   float* part_o;         // [block][hd / 4][32 rows][4]
@@ -154,7 +155,8 @@ __device__ __forceinline__ int sa_limit(const SaParams& p, const SaItem& s, cons
 // Items on the CUDA cores (fp32, and bf16 head dims below 64): tiles of
 // 16 * RPT rows by 64 keys in shared memory, all fp32; thread (rg, sub) of
 // 16 x 16 holds rows rg * RPT.. against keys sub + 16 k, then the same rows'
-// dims sub * HD / 16... A row's max and sum are half-warp shuffles.
+// dims sub * HD / 16... A row's max and sum are half-warp shuffles. Prefix and
+// own items are two launches where their row counts call for other tiles.
 // ---------------------------------------------------------------------------
 constexpr int kSaThreads = 256;
 constexpr int kSaKT = 64;
@@ -162,25 +164,25 @@ constexpr int kSaPad = 4;
 
 template <int HD, int RPT>
 __host__ __device__ constexpr size_t sa_simt_smem() {
-  return (size_t(16 * RPT) * (HD + kSaPad) + 2 * size_t(kSaKT) * (HD + kSaPad) + size_t(16 * RPT) * (kSaKT + kSaPad)) *
+  return (size_t(16 * RPT) * (HD + kSaPad) + size_t(kSaKT) * (HD + kSaPad) + size_t(16 * RPT) * (kSaKT + kSaPad)) *
          sizeof(float);
 }
 
 template <typename T, int HD, int RPT>
-__global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
+__global__ void __launch_bounds__(kSaThreads, 2) sa_simt_kernel(const SaParams p) {
   constexpr int VE = VecTraits<T>::kElems;
   constexpr int R = 16 * RPT;
   constexpr int DPT = HD / 16;
   constexpr int QS = HD + kSaPad, PS = kSaKT + kSaPad;
   extern __shared__ __align__(16) float smf[];
   float* qs = smf;
-  float* ks = qs + size_t(R) * QS;
-  float* vs = ks + size_t(kSaKT) * QS;
-  float* ps = vs + size_t(kSaKT) * QS;
+  float* ks = qs + size_t(R) * QS;  // a tile of K, then of V
+  float* vs = ks;
+  float* ps = ks + size_t(kSaKT) * QS;
   pdl_wait();
   pdl_launch();  // after the wait: sa_token_kernel counts on it
   const int tid = threadIdx.x, rg = tid >> 4, sub = tid & 15;
-  const SaItem s = sa_item<HD, int(sizeof(T))>(p, blockIdx.x, R, kSaKT);
+  const SaItem s = sa_item<HD, int(sizeof(T))>(p, p.item0 + blockIdx.x, R, kSaKT);
   for (int i = tid; i < R * (HD / VE); i += kSaThreads) {
     const int r = i / (HD / VE), c = i - r * (HD / VE);
     float f[VE];
@@ -208,25 +210,35 @@ __global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
 #pragma unroll
     for (int d = 0; d < DPT; ++d) o[i][d] = 0.f;
   }
-  for (int j0 = s.j0; j0 < s.j1; j0 += kSaKT) {
-    __syncthreads();
-    for (int i = tid; i < kSaKT * (HD / VE); i += kSaThreads) {
-      const int j = i / (HD / VE), c = i - j * (HD / VE);
-      float kf[VE], vf[VE];
-      if (j0 + j < s.j1) {
-        unpack(ld_vec(static_cast<const T*>(s.k) + size_t(j0 + j) * HD + c * VE), kf);
-        unpack(ld_vec(static_cast<const T*>(s.v) + size_t(j0 + j) * HD + c * VE), vf);
-      } else {
+  // a tile on its way from memory: loaded under the arithmetic on the one before
+  constexpr int NV = kSaKT * (HD / VE) / kSaThreads > 0 ? kSaKT * (HD / VE) / kSaThreads : 1;
+  uint4 next[NV];
+  auto fetch = [&](const void* from, int j0) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) kf[e] = vf[e] = 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        ks[size_t(j) * QS + c * VE + e] = kf[e];
-        vs[size_t(j) * QS + c * VE + e] = vf[e];
-      }
+    for (int u = 0; u < NV; ++u) {
+      const int i = tid + u * kSaThreads, j = i / (HD / VE), c = i - j * (HD / VE);
+      next[u] = j < kSaKT && j0 + j < s.j1 ? ld_vec(static_cast<const T*>(from) + size_t(j0 + j) * HD + c * VE)
+                                           : make_uint4(0, 0, 0, 0);
     }
+  };
+  auto put = [&]() {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int i = tid + u * kSaThreads, j = i / (HD / VE), c = i - j * (HD / VE);
+      if (j >= kSaKT) break;
+      float f[VE];
+      unpack(next[u], f);
+#pragma unroll
+      for (int e = 0; e < VE; e += 4)
+        *reinterpret_cast<float4*>(ks + size_t(j) * QS + c * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+    }
+  };
+  if (s.j0 < s.j1) fetch(s.k, s.j0);
+  for (int j0 = s.j0; j0 < s.j1; j0 += kSaKT) {
+    __syncthreads();  // the last tile of V is used up (and q is there)
+    put();
     __syncthreads();
+    fetch(s.v, j0);
     float sc[RPT][4];
 #pragma unroll
     for (int i = 0; i < RPT; ++i)
@@ -271,17 +283,33 @@ __global__ void __launch_bounds__(kSaThreads) sa_simt_kernel(const SaParams p) {
 #pragma unroll
       for (int d = 0; d < DPT; ++d) o[i][d] *= alpha;
     }
-    __syncwarp();
+    __syncthreads();  // K is used up
+    put();
+    __syncthreads();
+    if (j0 + kSaKT < s.j1) fetch(s.k, j0 + kSaKT);
+    // (four keys at a time: behind the range both factors are 0)
     const int kn = min(kSaKT, s.j1 - j0);
-    for (int j = 0; j < kn; ++j) {
-      float vv[DPT];
+    for (int j = 0; j < kn; j += 4) {
+      float4 pr[RPT];
 #pragma unroll
-      for (int d = 0; d < DPT; ++d) vv[d] = vs[size_t(j) * QS + sub * DPT + d];
+      for (int i = 0; i < RPT; ++i) pr[i] = *reinterpret_cast<const float4*>(ps + size_t(rg * RPT + i) * PS + j);
 #pragma unroll
-      for (int i = 0; i < RPT; ++i) {
-        const float pr = ps[size_t(rg * RPT + i) * PS + j];
+      for (int jj = 0; jj < 4; ++jj) {
+        float vv[DPT];
+        const float* vr = vs + size_t(j + jj) * QS + sub * DPT;
+        if constexpr (DPT % 4 == 0) {
 #pragma unroll
-        for (int d = 0; d < DPT; ++d) o[i][d] = fmaf(pr, vv[d], o[i][d]);
+          for (int d = 0; d < DPT; d += 4) *reinterpret_cast<float4*>(vv + d) = *reinterpret_cast<const float4*>(vr + d);
+        } else {
+#pragma unroll
+          for (int d = 0; d < DPT; ++d) vv[d] = vr[d];
+        }
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+          const float w = jj == 0 ? pr[i].x : jj == 1 ? pr[i].y : jj == 2 ? pr[i].z : pr[i].w;
+#pragma unroll
+          for (int d = 0; d < DPT; ++d) o[i][d] = fmaf(w, vv[d], o[i][d]);
+        }
       }
     }
   }
