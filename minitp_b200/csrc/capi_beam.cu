@@ -252,11 +252,11 @@ struct SaPlan {
 // Key ranges for `base` tensor-core items of up to `top` keys: the number that
 // makes waves x (key tiles a range + a start-up of about four) smallest, with
 // the partial sums' traffic (written and read again) beside it.
-int sa_tc_splits(long long base, int top, size_t rows, int hd, int sms) {
+int sa_tc_splits(long long base, int top, int limit, size_t rows, int hd, int sms) {
   const int tiles = std::max(1, (top + kSaTcKeys - 1) / kSaTcKeys);
   int best = 1;
   double least = 0;
-  for (int s = 1; s <= std::min(tiles, kSaMaxSplits); ++s) {
+  for (int s = 1; s <= std::min(tiles, limit); ++s) {
     const double waves = double((base * s + sms - 1) / sms);
     const double us = waves * (0.7 * ((tiles + s - 1) / s) + 2.8) + double(rows) * s * hd * 8 / 4e6;
     if (s == 1 || us < least) {
@@ -285,9 +285,11 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   pl.tc = a.dtype == MTPB_BF16 && (a.hd == 64 || a.hd == 128);
   pl.token = pl.tc && a.T == 1 && N <= 65535;
   const long long prow = (long long)a.W * a.T * per, orow = (long long)a.T * per;
-  // CUDA-core items: row tiles of 64 when there are as many rows, else of 16
-  pl.prpt = prow >= 64 ? 4 : 1;
-  pl.orpt = orow >= 64 ? 4 : 1;
+  // CUDA-core items: row tiles of 128, 64 or 16 by the rows there are (a larger
+  // tile reads less shared memory a product, which bounds these items)
+  auto rpt = [](long long rows_) { return rows_ > 96 ? 8 : rows_ > 32 ? 4 : 1; };
+  pl.prpt = rpt(prow);
+  pl.orpt = rpt(orow);
   // two row tiles a CTA from the second on (for most items)
   pl.mt = prow > 128 ? 2 : 1;
   const int ptile = pl.tc ? 128 * pl.mt : 16 * pl.prpt, otile = pl.token ? 16 : pl.tc ? 128 * pl.mt : 16 * pl.orpt;
@@ -295,15 +297,15 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   pl.otiles = int((orow + otile - 1) / otile);
   const long long pbase = (long long)a.G * a.hkv * pl.ptiles, obase = N * a.hkv * pl.otiles;
   // key ranges until the items give every SM four, but none below two key tiles
-  auto splits = [&](long long base, int top) {
+  auto splits = [&](long long base, int top, int limit) {
     const long long most = std::max(1, (top + 2 * kSaKT - 1) / (2 * kSaKT)), want = 4ll * sms;
-    return int(std::max<long long>(1, std::min<long long>(std::min<long long>(most, kSaMaxSplits), (want + base - 1) / base)));
+    return int(std::max<long long>(1, std::min<long long>(std::min<long long>(most, limit), (want + base - 1) / base)));
   };
   if (pl.token) {
     // long own caches of few rows in ranges of at least 512 keys (about 5 us of
     // one CTA's pace), which a third launch joins
     pl.so = 1;
-    while (obase * pl.so * 2 <= 2 * sms && top_o / (pl.so * 2) >= 512 && pl.so < kSaMaxSplits) pl.so *= 2;
+    while (obase * pl.so * 2 <= 2 * sms && top_o / (pl.so * 2) >= 512 && pl.so < kSaMaxOwn) pl.so *= 2;
     // the prefix read by every row's CTA: one launch, but N / G reads of each
     // position, through L2, and one CTA's pace along it. 4 beams behind 128
     // positions: 3.4 us against 7 with the tensor-core items; 8 x 8 beams
@@ -311,9 +313,11 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
     const long long pre = (long long)top_p * a.hd * 4;
     pl.inline_pre = pl.so == 1 && pre <= (256 << 10) && obase * pre <= (32ll << 20);
   } else {
-    pl.so = pl.tc ? sa_tc_splits(obase, top_o, pl.rows, a.hd, sms) : splits(obase, top_o);
+    pl.so = pl.tc ? sa_tc_splits(obase, top_o, kSaMaxOwn, pl.rows, a.hd, sms) : splits(obase, top_o, kSaMaxOwn);
   }
-  pl.sp = pl.inline_pre ? 0 : pl.tc ? sa_tc_splits(pbase, top_p, pl.rows, a.hd, sms) : splits(pbase, top_p);
+  pl.sp = pl.inline_pre ? 0
+          : pl.tc       ? sa_tc_splits(pbase, top_p, kSaMaxSplits, pl.rows, a.hd, sms)
+                        : splits(pbase, top_p, kSaMaxSplits);
   pl.pitems = pbase * pl.sp;
   pl.items = pl.pitems + (pl.token ? 0 : obase * pl.so);
   if (pl.items > 0x7FFFFFFFll) return bad("shared_attention: too many rows");
@@ -380,9 +384,11 @@ int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
       if (n == 0) return MTPB_OK;
       SaParams q = p;
       q.item0 = int(first);
-      return rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 4>(),
-                                    st, q)
-                      : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 1>(),
+      return rpt == 8   ? host_launch(sa_simt_kernel<T, HD, 8>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 8>(),
+                                      st, q)
+             : rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 4>(),
+                                      st, q)
+                        : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 1>(),
                                     st, q);
     };
     const bool both = pl.prpt == pl.orpt;
@@ -396,8 +402,8 @@ int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
       if (r != MTPB_OK || pl.so == 1) return r;
     }
   }
-  return host_launch(sa_join_kernel<T, HD>, dim3(unsigned(p.G * p.W * p.hkv * pl.oblocks)), dim3(kSaJoinThreads), 0, st,
-                     p);
+  return host_launch(sa_join_kernel<T, HD>, dim3(unsigned(p.G * p.W * p.hkv * pl.oblocks)), dim3(kSaJoinThreads),
+                     size_t(p.sp + p.so) * 32 * sizeof(float2), st, p);
 }
 
 template <typename T>

@@ -169,7 +169,7 @@ __host__ __device__ constexpr size_t sa_simt_smem() {
 }
 
 template <typename T, int HD, int RPT>
-__global__ void __launch_bounds__(kSaThreads, 2) sa_simt_kernel(const SaParams p) {
+__global__ void __launch_bounds__(kSaThreads, RPT == 8 ? 1 : 2) sa_simt_kernel(const SaParams p) {
   constexpr int VE = VecTraits<T>::kElems;
   constexpr int R = 16 * RPT;
   constexpr int DPT = HD / 16;
@@ -387,7 +387,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 constexpr int kSaTokenWarps = 4;  // 8 took 57.5 us where 4 took 55.8 (64 rows of the 7B heads behind 16384 positions)
-constexpr int kSaMaxSplits = 64;  // key ranges of a prefix
+constexpr int kSaMaxSplits = 64, kSaMaxOwn = 32;  // key ranges of a prefix, of an own cache
 
 // WIDE: more than 8 heads a tile (rows 8..15 in use).
 template <int HD, bool WIDE>
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const S
 #pragma unroll
     for (int w = 0; w < NW; ++w)
       add(sml[(w * R + r) * 2], sml[(w * R + r) * 2 + 1], *reinterpret_cast<const float4*>(so + (w * R + r) * HD + 4 * q));
-    constexpr int U = 8;  // ranges whose sums are loaded together
+    constexpr int U = 4;  // ranges whose sums are loaded together
     for (int s0 = 0; s0 < pslots; s0 += U) {
       float4 f[U];
 #pragma unroll
@@ -1003,61 +1003,76 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// Join of the key ranges: a CTA takes 32 rows of an own plane, a row a lane
-// and 4 dims a warp and step; the result goes through shared memory so that
-// whole rows are written.
+// Join of the key ranges: a CTA takes 32 rows of an own plane. The ranges'
+// weights come first (a thread a row and range); then a thread sums 4 dims of
+// a row over the ranges, four loads in flight; the result goes through shared
+// memory so that whole rows are written.
 // ---------------------------------------------------------------------------
 constexpr int kSaJoinThreads = 256;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams p) {
-  constexpr int VE = VecTraits<T>::kElems;
+  constexpr int VE = VecTraits<T>::kElems, U = 4;
+  extern __shared__ float2 sa_ml[];  // a range and row: max, sum; then weight
+  float2* ml = sa_ml;
   __shared__ float res[32][HD + 1];
+  __shared__ float inv[32];
   pdl_launch();
   pdl_wait();
-  const int per = p.hq / p.hkv;
+  const int per = p.hq / p.hkv, tid = threadIdx.x;
   const int blk = blockIdx.x % p.oblocks, plane = blockIdx.x / p.oblocks;
   const int n = plane / p.hkv, kvh = plane - n * p.hkv, gi = n / p.W;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = blk * 32 + lane, rows = p.T * per;
-  if (r < rows) {
-    const int pr = (n - gi * p.W) * rows + r, pplane = gi * p.hkv + kvh;
-    float mx = -INFINITY;
-#pragma unroll 4
-    for (int s = 0; s < p.sp; ++s) mx = fmaxf(mx, p.part_ml[sa_part<HD>(p, false, s, pplane, pr).ml].x);
-#pragma unroll 4
-    for (int s = 0; s < p.so; ++s) mx = fmaxf(mx, p.part_ml[sa_part<HD>(p, true, s, plane, r).ml].x);
+  const int total = p.T * per, rows = min(32, total - blk * 32), slots = p.sp + p.so;
+  const int pr0 = (n - gi * p.W) * total + blk * 32, pplane = gi * p.hkv + kvh;
+  auto part = [&](int s, int r) {
+    return s < p.sp ? sa_part<HD>(p, false, s, pplane, pr0 + r) : sa_part<HD>(p, true, s - p.sp, plane, blk * 32 + r);
+  };
+  for (int i = tid; i < slots * 32; i += kSaJoinThreads)
+    if ((i & 31) < rows) ml[i] = __ldcg(p.part_ml + part(i >> 5, i & 31).ml);
+  __syncthreads();
+  if (tid < rows) {
+    float mx = -INFINITY, den = 0.f;
+    for (int s = 0; s < slots; ++s) mx = fmaxf(mx, ml[s * 32 + tid].x);
     const float ref = mx == -INFINITY ? 0.f : mx;
-    for (int q = warp; q < HD / 4; q += kSaJoinThreads / 32) {
-      float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-      auto add = [&](const SaPart& at) {
-        const float2 ml = p.part_ml[at.ml];
-        const float4 f = *reinterpret_cast<const float4*>(p.part_o + at.o + q * 128);
-        const float w = ml.x == -INFINITY ? 0.f : expf(ml.x - ref);
-        den = fmaf(w, ml.y, den);
-        if (w != 0.f) {  // an empty range leaves its sums unwritten
-          num[0] = fmaf(w, f.x, num[0]);
-          num[1] = fmaf(w, f.y, num[1]);
-          num[2] = fmaf(w, f.z, num[2]);
-          num[3] = fmaf(w, f.w, num[3]);
-        }
-      };
-#pragma unroll 4
-      for (int s = 0; s < p.sp; ++s) add(sa_part<HD>(p, false, s, pplane, pr));
-#pragma unroll 4
-      for (int s = 0; s < p.so; ++s) add(sa_part<HD>(p, true, s, plane, r));
-      const float inv = den > 0.f ? 1.f / den : 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) res[lane][4 * q + e] = num[e] * inv;
+    for (int s = 0; s < slots; ++s) {
+      const float2 v = ml[s * 32 + tid];
+      const float w = v.x == -INFINITY ? 0.f : expf(v.x - ref);
+      den = fmaf(w, v.y, den);
+      ml[s * 32 + tid].x = w;
     }
+    inv[tid] = den > 0.f ? 1.f / den : 0.f;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 32 * (HD / VE); i += kSaJoinThreads) {
-    const int rr = i / (HD / VE), c = (i - rr * (HD / VE)) * VE, row = blk * 32 + rr;
-    if (row >= rows) break;
+  for (int i = tid; i < rows * (HD / 4); i += kSaJoinThreads) {
+    const int q = i / rows, r = i - q * rows;
+    float num[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < slots; s0 += U) {
+      float4 f[U];
+      float w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        w[u] = s0 + u < slots ? ml[(s0 + u) * 32 + r].x : 0.f;
+        if (w[u] != 0.f)  // an empty range leaves its sums unwritten
+          f[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + part(s0 + u, r).o + q * 128));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (w[u] != 0.f) {
+          num[0] = fmaf(w[u], f[u].x, num[0]);
+          num[1] = fmaf(w[u], f[u].y, num[1]);
+          num[2] = fmaf(w[u], f[u].z, num[2]);
+          num[3] = fmaf(w[u], f[u].w, num[3]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) res[r][4 * q + e] = num[e] * inv[r];
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * (HD / VE); i += kSaJoinThreads) {
+    const int r = i / (HD / VE), c = (i - r * (HD / VE)) * VE, row = blk * 32 + r;
     float f[VE];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) f[e] = res[rr][c + e];
+    for (int e = 0; e < VE; ++e) f[e] = res[r][c + e];
     const int t = row / per, head = kvh * per + row - t * per;
     *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + ((size_t(n) * p.T + t) * p.hq + head) * HD + c) = pack_vec(f);
   }
