@@ -824,10 +824,15 @@ SharedAttnArgs shared_args(const ModelHost& mh, const FwdArgs& a, int l, int tc,
   return s;
 }
 
-// Workspace of the shared-prefix attention for tc tokens a row.
+// Workspace of the shared-prefix attention for chunks of tc tokens a row (and a last one of the rest).
 int shared_reserve(ModelHost& mh, const FwdArgs& a, int tc, cudaStream_t st) {
-  const long long need = shared_attn_workspace(shared_args(mh, a, 0, tc, a.cache_len));
+  long long need = shared_attn_workspace(shared_args(mh, a, 0, tc, a.cache_len));
   if (need < 0) return int(need);
+  if (a.T % tc) {  // fewer tokens may be cut into more key ranges
+    const long long rest = shared_attn_workspace(shared_args(mh, a, 0, a.T % tc, a.cache_len));
+    if (rest < 0) return int(rest);
+    need = std::max(need, rest);
+  }
   if (size_t(need) <= mh.sa_bytes) return MTPB_OK;
   if (capturing(st)) return fail(MTPB_ERR_INVALID, "shared-prefix forward: run one call eagerly before graph capture");
   g_settings_epoch.fetch_add(1);

@@ -332,6 +332,13 @@ int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   return MTPB_OK;
 }
 
+// The call with lengths that are known on the device only: planned by the capacities.
+SharedAttnArgs by_capacity(SharedAttnArgs a) {
+  static const int any = 0;
+  a.prefix_lens = a.cache_lens = &any;
+  return a;
+}
+
 // Map of caches [planes][cap][hd] bf16, boxes of 128 positions x 64 dims with
 // the 128-byte swizzle; positions from cap on read as zeros.
 int sa_map(CUtensorMap* map, const void* ptr, long long planes, int cap, int hd) {
@@ -422,13 +429,16 @@ namespace mtpb {
 
 long long shared_attn_workspace(const SharedAttnArgs& a) {
   SaPlan pl;
-  const int r = sa_plan(a, &pl);
+  const int r = sa_plan(by_capacity(a), &pl);
   return r == MTPB_OK ? (long long)(pl.ml_bytes + pl.o_bytes) : r;
 }
 
 int shared_attn_run(const SharedAttnArgs& a, void* ws, size_t ws_bytes, cudaStream_t st) {
   SaPlan pl;
-  const int r = sa_plan(a, &pl);
+  int r = sa_plan(a, &pl);
+  // fewer keys than the capacity can call for more ranges, and more partial
+  // sums, than the workspace was made for: then the capacities' plan
+  if (r == MTPB_OK && pl.ml_bytes + pl.o_bytes > ws_bytes) r = sa_plan(by_capacity(a), &pl);
   if (r != MTPB_OK) return r;
   if (!a.q || !a.k_prefix || !a.v_prefix || !a.k_cache || !a.v_cache || !a.out ||
       (!ws && pl.ml_bytes + pl.o_bytes > 0))
@@ -483,7 +493,6 @@ extern "C" {
 long long mtpb_shared_attention_workspace(int G, int W, int T, int hq, int hkv, int hd, int cap_p, int cap,
                                           int dtype) {
   SharedAttnArgs a = {};
-  static const int any = 0;
   a.G = G;
   a.W = W;
   a.T = T;
@@ -493,7 +502,6 @@ long long mtpb_shared_attention_workspace(int G, int W, int T, int hq, int hkv, 
   a.cap_p = cap_p;
   a.cap = cap;
   a.dtype = dtype;
-  a.prefix_lens = a.cache_lens = &any;  // lengths on the device: plans go by the capacities
   return shared_attn_workspace(a);
 }
 

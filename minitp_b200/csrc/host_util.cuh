@@ -72,7 +72,8 @@ struct SharedAttnArgs {
   int dtype;
   uint32_t* status = nullptr;           // word for error bits, or NULL: the library's own
 };
-// Workspace bytes of a call (no device access; < 0: an MTPB_ERR_* code).
+// Workspace bytes of calls of these sizes, whatever their lengths (no device
+// access; < 0: an MTPB_ERR_* code).
 long long shared_attn_workspace(const SharedAttnArgs& a);
 int shared_attn_run(const SharedAttnArgs& a, void* ws, size_t ws_bytes, cudaStream_t st);
 

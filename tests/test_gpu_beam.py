@@ -315,6 +315,18 @@ def test_attention_lengths_are_clamped_and_may_be_ints(lib):
     assert int((none != 0).sum()) == 0
 
 
+@pytest.mark.parametrize("t,hkv,hd,cap_p,plen,cap,clen", [
+    (1, 2, 128, 9000, 7937, 1000, 151), (1, 1, 64, 9000, 5489, 1000, 271), (2, 2, 128, 9000, 6473, 300, 72)])
+def test_attention_shorter_than_the_capacity(lib, t, hkv, hd, cap_p, plen, cap, clen):
+    """Host lengths whose own plan would take more key ranges than the capacities' plan."""
+    from minitp_b200 import ops
+
+    q, kp, vp, pl, kc, vc, cl = _attention_case(9, "bf16", 1, 1, t, hkv, hkv, hd, cap_p, [plen], cap, [clen])
+    want, tol = beam_ref.attend(q, kp, vp, pl, kc, vc, cl, hkv, hkv)
+    got = ops.shared_prefix_attention(q.cuda(), kp.cuda(), vp.cuda(), plen, kc.cuda(), vc.cuda(), clen, hkv, hkv).cpu()
+    assert bool(((got.double() - want).abs() <= tol).all())
+
+
 def test_attention_equals_attention_over_one_cache(lib):
     """Prefix and own cache laid end to end give the framework's plain attention."""
     from minitp_b200 import ops
