@@ -378,36 +378,28 @@ int sa_launch_token(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
 
 template <typename T, int HD>
 int sa_launch(const SaPlan& pl, const SaParams& p, cudaStream_t st) {
-  bool done = pl.items == 0;
   if constexpr (sizeof(T) == 2 && HD >= 64) {
-    if (!done && pl.tc) {
+    if (pl.items > 0) {
       const int r = sa_launch_tc<HD>(pl, p, st);
       if (r != MTPB_OK) return r;
-      done = true;
     }
-  }
-  if (!done) {
+    if (pl.token) {
+      const int r = sa_launch_token<HD>(pl, p, st);
+      if (r != MTPB_OK || pl.so == 1) return r;
+    }
+  } else {
     auto items = [&](int rpt, long long first, long long n) {
-      if (n == 0) return MTPB_OK;
       SaParams q = p;
       q.item0 = int(first);
-      return rpt == 8   ? host_launch(sa_simt_kernel<T, HD, 8>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 8>(),
-                                      st, q)
-             : rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 4>(),
-                                      st, q)
-                        : host_launch(sa_simt_kernel<T, HD, 1>, dim3((unsigned)n), dim3(kSaThreads), sa_simt_smem<HD, 1>(),
-                                    st, q);
+      const dim3 grid((unsigned)n), block(kSaThreads);
+      return rpt == 8   ? host_launch(sa_simt_kernel<T, HD, 8>, grid, block, sa_simt_smem<HD, 8>(), st, q)
+             : rpt == 4 ? host_launch(sa_simt_kernel<T, HD, 4>, grid, block, sa_simt_smem<HD, 4>(), st, q)
+                        : host_launch(sa_simt_kernel<T, HD, 1>, grid, block, sa_simt_smem<HD, 1>(), st, q);
     };
     const bool both = pl.prpt == pl.orpt;
     int r = items(pl.prpt, 0, both ? pl.items : pl.pitems);
     if (r == MTPB_OK && !both) r = items(pl.orpt, pl.pitems, pl.items - pl.pitems);
     if (r != MTPB_OK) return r;
-  }
-  if constexpr (sizeof(T) == 2 && HD >= 64) {
-    if (pl.token) {
-      const int r = sa_launch_token<HD>(pl, p, st);
-      if (r != MTPB_OK || pl.so == 1) return r;
-    }
   }
   return host_launch(sa_join_kernel<T, HD>, dim3(unsigned(p.G * p.W * p.hkv * pl.oblocks)), dim3(kSaJoinThreads),
                      size_t(p.sp + p.so) * 32 * sizeof(float2), st, p);

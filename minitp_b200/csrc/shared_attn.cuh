@@ -10,6 +10,12 @@
 // read once per row tile and not once per row; own items hold those of one
 // row. Every item writes its rows' unnormalised sums with their max and
 // denominator (a slot per key range), and a second kernel joins the slots.
+//
+// NaN and infinities go where the formula takes them and nowhere else: a score
+// that is NaN or +inf makes its row NaN (a sum that is NaN is handed on with a
+// NaN max, which no join passes over); positions that a token does not see
+// reach it neither through K (its scores are selected away) nor through V (0
+// times NaN would be NaN: such terms are left out or zeroed).
 #pragma once
 
 #include <type_traits>
@@ -150,6 +156,8 @@ __device__ __forceinline__ SaRow sa_row(const SaParams& p, const SaItem& s, int 
 __device__ __forceinline__ int sa_limit(const SaParams& p, const SaItem& s, const SaRow& x) {
   return s.own ? sa_cache_len(p, x.n) - (p.T - 1 - x.t) : s.j1;
 }
+// The max handed on with sum l.
+__device__ __forceinline__ float sa_max_of(float m, float l) { return l == l ? m : l; }
 
 // ---------------------------------------------------------------------------
 // Items on the CUDA cores (fp32, and bf16 head dims below 64): tiles of
@@ -196,11 +204,12 @@ __global__ void __launch_bounds__(kSaThreads, RPT == 8 ? 1 : 2) sa_simt_kernel(c
 #pragma unroll
     for (int e = 0; e < VE; ++e) qs[size_t(r) * QS + c * VE + e] = f[e] * p.scale;
   }
-  int lim[RPT];
+  int lim[RPT], low = s.j1;
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
     const int r = rg * RPT + i;
-    lim[i] = r < s.rows ? sa_limit(p, s, sa_row(p, s, r)) : 0;
+    lim[i] = r < s.rows ? sa_limit(p, s, sa_row(p, s, r)) : s.j1;
+    low = min(low, lim[i]);
   }
   float m[RPT], l[RPT], o[RPT][DPT];
 #pragma unroll
@@ -289,6 +298,18 @@ __global__ void __launch_bounds__(kSaThreads, RPT == 8 ? 1 : 2) sa_simt_kernel(c
     if (j0 + kSaKT < s.j1) fetch(s.k, j0 + kSaKT);
     // (four keys at a time: behind the range both factors are 0)
     const int kn = min(kSaKT, s.j1 - j0);
+    if (j0 + kn > low) {  // keys that not every row sees
+#pragma unroll 1
+      for (int j = 0; j < kn; ++j)
+#pragma unroll
+        for (int i = 0; i < RPT; ++i)
+          if (j0 + j < lim[i]) {
+            const float w = ps[size_t(rg * RPT + i) * PS + j];
+#pragma unroll
+            for (int d = 0; d < DPT; ++d) o[i][d] = fmaf(w, vs[size_t(j) * QS + sub * DPT + d], o[i][d]);
+          }
+      continue;
+    }
     for (int j = 0; j < kn; j += 4) {
       float4 pr[RPT];
 #pragma unroll
@@ -318,7 +339,7 @@ __global__ void __launch_bounds__(kSaThreads, RPT == 8 ? 1 : 2) sa_simt_kernel(c
     const int r = rg * RPT + i;
     if (r >= s.rows) continue;
     const SaPart at = sa_part<HD>(p, s.own, s.split, s.plane, s.row0 + r);
-    if (sub == 0) p.part_ml[at.ml] = make_float2(m[i], l[i]);
+    if (sub == 0) p.part_ml[at.ml] = make_float2(sa_max_of(m[i], l[i]), l[i]);
     if (s.j0 < s.j1)
 #pragma unroll
       for (int d = 0; d < DPT; ++d) {
@@ -363,6 +384,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
 }
 // 2^x of two values on the fp32 pipe: x = n + f with n the nearest integer
 // (read off the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by the cubic
@@ -546,7 +572,7 @@ __global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const S
   for (int h = 0; h < NT; ++h) {
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (c == 0) *reinterpret_cast<float2*>(sml + (warp * R + g + 8 * h) * 2) = make_float2(m[h] * kLn2, l[h]);
+    if (c == 0) *reinterpret_cast<float2*>(sml + (warp * R + g + 8 * h) * 2) = make_float2(sa_max_of(m[h] * kLn2, l[h]), l[h]);
 #pragma unroll
     for (int v = 0; v < VB; ++v)
 #pragma unroll
@@ -601,7 +627,7 @@ __global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const S
           make_uint2(pack_bf16(num[0] * inv, num[1] * inv), pack_bf16(num[2] * inv, num[3] * inv));
     } else {
       const SaPart at = sa_part<HD>(p, true, split, n * p.hkv + kvh, tile * 16 + r);
-      if (q == 0) p.part_ml[at.ml] = make_float2(mx, den);
+      if (q == 0) p.part_ml[at.ml] = make_float2(sa_max_of(mx, den), den);
       *reinterpret_cast<float4*>(p.part_o + at.o + q * 128) = make_float4(num[0], num[1], num[2], num[3]);
     }
   }
@@ -627,7 +653,11 @@ __global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const S
 // then P is at most 2^8, which costs no precision, as the division by the sum
 // takes the factor out.
 // Keys from the end of the range on are masked by selection; their V rows are
-// zeroed in shared memory, since 0 x NaN would not be 0.
+// zeroed in shared memory, since 0 x NaN would not be 0. In tiles of own items
+// that not every token sees, the NaN and infinities among V are zeroed too; a
+// negative sum tells the join, which adds them to the rows that do see them.
+// (Added here they cost the softmax registers: 66 -> 76 us on 16 rows of 128
+// tokens behind 4001.)
 // ---------------------------------------------------------------------------
 constexpr int kSaTcKeys = 128;
 // Of 16 pairs of exponentials, on the fp32 pipe (0, 2, 4, 6: 46.6, 46.8, 46.5,
@@ -654,6 +684,34 @@ struct SaTcCfg {
       (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 };
 
+// Row r of a V tile: behind the range it becomes zeros; one that not every
+// token sees loses its NaN and infinities, and *odd tells of them. (A call, to
+// take no registers from the softmax.)
+template <int HD>
+__device__ __noinline__ void sa_clean_row(unsigned char* tile, int r, bool behind, bool unseen, int* odd) {
+  auto at = [&](int i) { return reinterpret_cast<uint4*>(tile + (i >> 3) * kSaTcSub + r * 128 + (((i ^ r) & 7) << 4)); };
+  if (behind) {
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) *at(i) = make_uint4(0, 0, 0, 0);
+  } else if (unseen) {
+    uint32_t nan = 0;  // two bf16, NaN when a value was not finite
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) {
+      const uint4 v = *at(i);
+      nan = fma_bf16x2(v.x, 0u, fma_bf16x2(v.y, 0u, fma_bf16x2(v.z, 0u, fma_bf16x2(v.w, 0u, nan))));
+    }
+    if (nan & 0x7FFF7FFFu) {
+      *static_cast<volatile int*>(odd) = 1;
+      __threadfence_block();
+#pragma unroll 1
+      for (int i = 0; i < HD; ++i) {
+        uint16_t* h = reinterpret_cast<uint16_t*>(at(i >> 3)) + (i & 7);
+        if ((*h & 0x7F80u) == 0x7F80u) *h = 0;
+      }
+    }
+  }
+}
+
 template <int HD, int MT>
 __global__ void __launch_bounds__(kSaTcThreads, 1)
     sa_tc_kernel(const SaParams p, const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
@@ -664,7 +722,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2][2], pv_done[2], drain[2], turn[2][4];
   __shared__ uint32_t tmem_base;
-  __shared__ int abort_sh;
+  __shared__ int abort_sh, odd_sh;  // odd_sh: values of V were zeroed
   __shared__ float2 ml_sh[128];  // MT 1: stream 1's statistics
   volatile int* abort = &abort_sh;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -696,6 +754,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
       for (int q = 0; q < 4; ++q) mbar_init(&turn[x][q], 1);
     }
     *abort = 0;
+    odd_sh = 0;
     mbar_init_fence();
   }
   if (warp == 3) {
@@ -823,6 +882,7 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
     if (write) w = sa_row(p, it, row);
     const int lim = write ? min(it.j1, sa_limit(p, it, w)) : it.j1;  // keys [0, lim) are seen
     const float sl2 = p.scale * kLog2e;
+    const int low = p.T > 1 ? min(it.j1, sa_limit(p, it, sa_row(p, it, 0))) : it.j1;  // keys [0, low) are seen by all
     float m = -INFINITY, l = 0.f;  // reference max (scaled, base 2), sum
     bool ok = true;
     int k = 0;
@@ -849,11 +909,11 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
 #pragma unroll
       for (int c = 4; c < kSaTcKeys - 4; c += 8)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], sc[c + i], sc[c + 4 + i]);
-      mx[0] = max3(mx[0], sc[124], sc[125]);
-      mx[1] = max3(mx[1], sc[126], sc[127]);
-      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl2;
-      const bool grow = top > m + 8.f;
+        for (int i = 0; i < 4; ++i) mx[i] = max3_nan(mx[i], sc[c + i], sc[c + 4 + i]);
+      mx[0] = max3_nan(mx[0], sc[124], sc[125]);
+      mx[1] = max3_nan(mx[1], sc[126], sc[127]);
+      const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sl2;
+      const bool grow = !(top <= m + 8.f);  // (NaN stays: exp2_cubic would lose it)
       if (!C::kAlias && k > 0) {  // the stream's previous P V has read P (aliased: it came before this S)
         ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -876,18 +936,11 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
         }
       }
       const float ref = m == -INFINITY ? 0.f : m;
-      if (j + kSaTcKeys > it.j1) {  // the last tile: V rows behind the range (MT 2: both streams write the same zeros)
+      if (j + kSaTcKeys > low) {  // V rows behind the range, or not seen by all (MT 2: both streams write the same zeros)
         const int i = 2 * t + 1, s = i % NB;
         ok = mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort);
         if (!__all_sync(0xffffffffu, ok)) break;
-        if (j + r >= it.j1) {
-#pragma unroll
-          for (int b = 0; b < C::kSubs; ++b)
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<uint4*>(smem + C::kOffRing + s * C::kTile + b * kSaTcSub + r * 128 + c * 16) =
-                  make_uint4(0, 0, 0, 0);
-        }
+        sa_clean_row<HD>(smem + C::kOffRing + s * C::kTile, r, j + r >= it.j1, j + r >= low, &odd_sh);
         fence_async_smem();
       }
       // the exponentials of the two warps of a scheduler take turns: one stream's
@@ -952,10 +1005,11 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
       wa = exp2_approx(m - ref);
       wb = exp2_approx(b.x - ref);
       l = l * wa + b.y * wb;
-      m = top;
+      m = sa_max_of(top, l);
     }
     if (MT == 2 || x == 0) {
       const SaPart at = sa_part<HD>(p, it.own, it.split, it.plane, it.row0 + row);
+      if (odd_sh) l = -l;
       if (write) p.part_ml[at.ml] = make_float2(m * kLn2, l);
 #pragma unroll
       for (int c = 0; c < HD; c += 16) {
@@ -1017,6 +1071,7 @@ __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams 
   float2* ml = sa_ml;
   __shared__ float res[32][HD + 1];
   __shared__ float inv[32];
+  __shared__ int odd[32];  // keys [odd, ..) of the own cache may hold values of V that were left out; -1: none
   pdl_launch();
   pdl_wait();
   const int per = p.hq / p.hkv, tid = threadIdx.x;
@@ -1032,14 +1087,17 @@ __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams 
   __syncthreads();
   if (tid < rows) {
     float mx = -INFINITY, den = 0.f;
+    bool left_out = false;
     for (int s = 0; s < slots; ++s) mx = fmaxf(mx, ml[s * 32 + tid].x);
     const float ref = mx == -INFINITY ? 0.f : mx;
     for (int s = 0; s < slots; ++s) {
       const float2 v = ml[s * 32 + tid];
       const float w = v.x == -INFINITY ? 0.f : expf(v.x - ref);
-      den = fmaf(w, v.y, den);
+      den = fmaf(w, fabsf(v.y), den);
+      left_out |= v.y < 0.f;
       ml[s * 32 + tid].x = w;
     }
+    odd[tid] = left_out ? max(0, sa_cache_len(p, n) - (p.T - 1)) : -1;
     inv[tid] = den > 0.f ? 1.f / den : 0.f;
   }
   __syncthreads();
@@ -1062,6 +1120,15 @@ __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams 
           num[1] = fmaf(w[u], f[u].y, num[1]);
           num[2] = fmaf(w[u], f[u].z, num[2]);
           num[3] = fmaf(w[u], f[u].w, num[3]);
+        }
+    }
+    if (odd[r] >= 0) {
+      const T* v = static_cast<const T*>(p.vc) + size_t(plane) * p.cap * HD + 4 * q;
+      const int end = sa_cache_len(p, n) - (p.T - 1 - (blk * 32 + r) / per);
+      for (int key = odd[r]; key < end; ++key)
+        for (int e = 0; e < 4; ++e) {
+          const float x = to_f(v[size_t(key) * HD + e]);
+          if (!(fabsf(x) < INFINITY)) num[e] += x;
         }
     }
 #pragma unroll

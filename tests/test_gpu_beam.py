@@ -302,6 +302,71 @@ def test_attention_large_scores_and_masked_infinities(lib):
         _check_attention((q, *case[1:]), 4, 2)
 
 
+ODD_SIZES = [  # dtype, hq, hkv, hd, g, w, t: each kernel and tile
+    ("fp32", 4, 2, 16, 1, 3, 1), ("fp32", 4, 1, 64, 1, 2, 5), ("fp32", 4, 1, 128, 1, 2, 70), ("bf16", 4, 2, 32, 1, 2, 20),
+    ("bf16", 14, 2, 64, 1, 3, 1), ("bf16", 20, 1, 128, 1, 3, 1), ("bf16", 4, 2, 64, 1, 40, 1), ("bf16", 4, 2, 64, 1, 3, 5),
+    ("bf16", 2, 1, 128, 1, 2, 60), ("bf16", 8, 1, 64, 1, 2, 40), ("bf16", 8, 1, 128, 1, 2, 150)]
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,hd,g,w,t", ODD_SIZES)
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_attention_odd_values_stay_where_they_are_seen(lib, dtype, hq, hkv, hd, g, w, t, odd):
+    """A value of an own V that is not finite reaches its dim of the tokens that see it, and nothing else."""
+    from minitp_b200 import ops
+
+    q, kp, vp, pl, kc, vc, cl = _attention_case(11, dtype, g, w, t, hq, hkv, hd, 300, [260] * g, t + 9, [t + 7] * (g * w))
+    places = sorted({3, 7, 7 + t // 3, 6 + t})
+    for n, j in enumerate(places):
+        vc[1, hkv - 1, j, (5 + 9 * n) % hd] = odd
+    got = ops.shared_prefix_attention(*(x.cuda() for x in (q, kp, vp, pl, kc, vc, cl)), hq, hkv).cpu()
+    got = got.view(g * w, t, hq, hd).double()
+    clean = vc.clone()
+    clean[:, :, :t + 7][~torch.isfinite(vc[:, :, :t + 7])] = 0
+    want, tol = (x.view(g * w, t, hq, hd) for x in beam_ref.attend(q, kp, vp, pl, kc, clean, cl, hq, hkv))
+    reached = torch.zeros(got.shape, dtype=torch.bool)
+    per = hq // hkv
+    for n, j in enumerate(places):  # token i sees own positions [0, 8 + i)
+        reached[1, max(0, j - 7):, (hkv - 1) * per:, (5 + 9 * n) % hd] = True
+    assert torch.equal(~torch.isfinite(got), reached)
+    assert bool(((got - want).abs() <= tol)[~reached].all())
+    if odd == math.inf:
+        assert bool((got[reached] == odd).all())
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,hd,g,w,t", ODD_SIZES)
+def test_attention_nan_scores(lib, dtype, hq, hkv, hd, g, w, t):
+    """A NaN in a query, or in a key that is seen, makes the rows NaN that score with it, and no other."""
+    from minitp_b200 import ops
+
+    q, kp, vp, pl, kc, vc, cl = _attention_case(12, dtype, g, w, t, hq, hkv, hd, 300, [260] * g, t + 9, [t + 7] * (g * w))
+    per = hq // hkv
+    clean = [x.clone() for x in (q, kp, vp, pl, kc, vc, cl)]
+    want, tol = (x.view(g * w, t, hq, hd) for x in beam_ref.attend(*clean, hq, hkv))
+
+    def check(case, reached):
+        got = ops.shared_prefix_attention(*(x.cuda() for x in case), hq, hkv).cpu().view(g * w, t, hq, hd).double()
+        assert torch.equal(got.isnan(), reached)
+        assert bool(((got - want).abs() <= tol)[~reached].all())
+
+    one = q.clone()
+    one.view(g * w, t, hq, hd)[1, t // 2, 1, 3] = math.nan
+    reached = torch.zeros(g * w, t, hq, hd, dtype=torch.bool)
+    reached[1, t // 2, 1] = True
+    check((one, kp, vp, pl, kc, vc, cl), reached)
+    for j in (0, 2, 8, 5 + t):  # of the own cache of row 0
+        one = kc.clone()
+        one[0, 0, j, 1] = math.nan
+        reached = torch.zeros(g * w, t, hq, hd, dtype=torch.bool)
+        reached[0, max(0, j - 7):, :per] = True
+        check((q, kp, vp, pl, one, vc, cl), reached)
+    for j in (0, 128, 133, 259):  # of the prefix, which every row of the group sees
+        one = kp.clone()
+        one[0, 0, j, 1] = math.nan
+        reached = torch.zeros(g * w, t, hq, hd, dtype=torch.bool)
+        reached[:, :, :per] = True
+        check((q, one, vp, pl, kc, vc, cl), reached)
+
+
 def test_attention_lengths_are_clamped_and_may_be_ints(lib):
     from minitp_b200 import ops
 
