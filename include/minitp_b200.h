@@ -245,8 +245,8 @@ int mtpb_argmax(void* comm, const void* logits, int M, int V_local, int64_t ld, 
  *     candidate, token `eos` at the beam's own score; its logits are not read.
  *     out_finished = finished[parent] or token == eos. eos < 0: no end token.
  *   - A beam whose score is -inf or NaN, or without a logit above -inf, has
- *     no candidate, and neither is a total below the range of fp32 one. Places without a candidate get score -inf, parent 0 and
- *     token eos (0 without one).
+ *     no candidate; a total below fp32's range is none. Places without a
+ *     candidate get score -inf, parent 0 and token eos (0 without one).
  * `block`: workspace of mtpb_beam_block_bytes(G*W, V, k) bytes, 16-byte
  * aligned, private to the call until it has run. */
 long long mtpb_beam_block_bytes(int rows, int V_plan, int k);
@@ -260,8 +260,8 @@ int mtpb_beam_select(const void* logits, int64_t ld, int G, int W, int V, const 
  * of the vocabulary) of every row to a block of
  * mtpb_beam_block_bytes(rows, V_plan, k) bytes; V_plan, the same on every
  * shard, is at least the largest V_local. mtpb_beam_pick selects from `parts`
- * such blocks, one after another in memory in any shard order (made with the same V_plan and k_block = k of the
- * candidates >= the k picked here). */
+ * such blocks, one after another in memory in any shard order, all made with
+ * the same V_plan and with k_block >= the k picked here. */
 int mtpb_beam_candidates(const void* logits, int64_t ld, int rows, int V_local, int64_t vstart,
                          int V_plan, int k, const uint8_t* finished, void* block, int dtype,
                          void* stream);
@@ -276,7 +276,8 @@ int mtpb_beam_pick(const void* blocks, int parts, int G, int W, int V_plan, int 
  * clamped to [0, cap]) or `len` when lens is NULL. Positions from n on are
  * left as they were, and so is a row whose parent is itself or outside
  * [0, W). 1 <= W <= 64; hd * sizeof(dtype) a multiple of 16; k_caches and
- * v_caches: host arrays of n_layers device pointers. */
+ * v_caches: host arrays of n_layers device pointers, to caches that do not
+ * overlap. */
 int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers,
                     const int64_t* parents, const int* lens, int len, int G, int W, int hkv,
                     int cap, int hd, int dtype, void* stream);
@@ -287,9 +288,11 @@ int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers,
  * [0, prefix_lens[g]) of its group's prefix and [0, cache_lens[n] - (T-1-t))
  * of its own cache (cache_lens counts the T tokens' own positions too); a
  * token that sees none gets 0. Lengths: device int32 arrays, clamped to their
- * cache's capacity, or the host value for every group / row when the array is
- * NULL. scale = 1/sqrt(hd); hd 16, 32, 64 or 128. Softmax statistics and sums
- * are fp32. `ws`: at least mtpb_shared_attention_workspace(...) bytes,
+ * cache's capacity, or the host value (0 .. capacity) for every group / row
+ * when the array is NULL. scale = 1/sqrt(hd); hd 16, 32, 64 or 128. Softmax
+ * statistics and sums are fp32; bf16 probabilities are rounded to bf16 for
+ * their product with V. What a token does not see does not reach it, NaN and
+ * infinities included. `ws`: at least mtpb_shared_attention_workspace(...) bytes,
  * 16-byte aligned, private to the call until it has run. */
 long long mtpb_shared_attention_workspace(int G, int W, int T, int hq, int hkv, int hd, int cap_p,
                                           int cap, int dtype);

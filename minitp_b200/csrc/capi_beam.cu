@@ -2,6 +2,7 @@
 // include/minitp_b200.h): host checks, launch plans and workspaces.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 
 #include "beam.cuh"
@@ -154,7 +155,7 @@ int mtpb_beam_candidates(const void* logits, int64_t ld, int rows, int V_local, 
   if (!dtype_ok(dtype)) return bad("unsupported dtype");
   if (rows > 65535) return bad("beam_candidates: more than 65535 rows");
   if (V_local < 0 || V_local > V_plan || ld < V_local) return bad("beam_candidates: need 0 <= V_local <= V_plan, ld");
-  if (vstart < 0 || vstart + V_local > 0xFFFFFFFFll) return bad("beam_candidates: vocabulary ids out of range");
+  if (vstart < 0 || vstart > 0xFFFFFFFFll - V_local) return bad("beam_candidates: vocabulary ids out of range");
   if (!al16(block)) return bad("beam_candidates: block must be 16-byte aligned");
   return beam_rows(logits, ld, rows, V_local, vstart, V_plan, k, finished, block, dtype,
                    static_cast<cudaStream_t>(stream));
@@ -185,6 +186,21 @@ int mtpb_beam_select(const void* logits, int64_t ld, int G, int W, int V, const 
                    static_cast<cudaStream_t>(stream));
 }
 
+// Whether two of the caches (n of `bytes` each) share memory; < 0: no memory to tell.
+static int caches_overlap(void* const* k, void* const* v, int n, size_t bytes) {
+  auto* at = static_cast<uintptr_t*>(std::malloc(2 * size_t(n) * sizeof(uintptr_t)));
+  if (!at) return -1;
+  for (int l = 0; l < n; ++l) {
+    at[2 * l] = reinterpret_cast<uintptr_t>(k[l]);
+    at[2 * l + 1] = reinterpret_cast<uintptr_t>(v[l]);
+  }
+  std::sort(at, at + 2 * size_t(n));
+  int found = 0;
+  for (size_t i = 1; i < 2 * size_t(n); ++i) found |= at[i] - at[i - 1] < bytes;
+  std::free(at);
+  return found;
+}
+
 int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers, const int64_t* parents,
                     const int* lens, int len, int G, int W, int hkv, int cap, int hd, int dtype, void* stream) {
   if (!k_caches || !v_caches || !parents) return bad("kv_reorder: null tensor");
@@ -204,6 +220,9 @@ int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers, 
   if (W == 1 || top == 0) return MTPB_OK;
   const long long blocks = (top * rv + kReorderThreads - 1) / kReorderThreads;
   if (blocks > 0x7FFFFFFFll) return bad("kv_reorder: cache too long");
+  // (one launch works on all of them at once)
+  const int shared = caches_overlap(k_caches, v_caches, n_layers, size_t(G) * W * hkv * cap * bytes);
+  if (shared) return bad(shared < 0 ? "kv_reorder: out of memory" : "kv_reorder: caches overlap");
   for (int l0 = 0; l0 < n_layers; l0 += kReorderLayers) {
     const int n = std::min(kReorderLayers, n_layers - l0);
     ReorderParams p;
@@ -270,6 +289,7 @@ int sa_tc_splits(long long base, int top, int limit, size_t rows, int hd, int sm
 int sa_plan(const SharedAttnArgs& a, SaPlan* out) {
   if (a.G < 1 || a.W < 1 || a.T < 1 || a.hq < 1 || a.hkv < 1 || a.cap_p < 1 || a.cap < 1)
     return bad("shared_attention: sizes must be positive");
+  if (a.cap_p > 1 << 30 || a.cap > 1 << 30) return bad("shared_attention: caches of more than 2^30 positions");
   if (a.hq % a.hkv) return bad("shared_attention: hq must be a multiple of hkv");
   if (a.hd != 16 && a.hd != 32 && a.hd != 64 && a.hd != 128)
     return bad("shared_attention: head_dim must be 16, 32, 64 or 128");

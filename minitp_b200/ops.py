@@ -213,8 +213,8 @@ def _beam_inputs(name: str, logits, scores, k, finished, eos_token_id, least: in
     if scores.dtype != torch.float32 or not scores.is_contiguous():
         raise _lib.MinitpB200Error(f"{name}: scores must be contiguous fp32")
     g, w, v = logits.shape
-    if not (1 <= w <= 64 and 1 <= k <= 64 and g >= 1 and v >= least):
-        raise _lib.MinitpB200Error(f"{name}: need 1..64 beams, k in [1, 64] and a non-empty vocabulary")
+    if not (1 <= w <= 64 and 1 <= k <= 64 and g >= 1 and least <= v < 2**31):
+        raise _lib.MinitpB200Error(f"{name}: need 1..64 beams, k in [1, 64] and a vocabulary of 1 .. 2^31 - 1")
     if finished is not None:
         if finished.dtype != torch.bool or finished.shape != scores.shape or not finished.is_contiguous():
             raise _lib.MinitpB200Error(f"{name}: finished must be contiguous bool [G, W]")
@@ -273,6 +273,9 @@ def beam_candidates(local_logits: torch.Tensor, k: int, vstart: int, v_plan: int
                     finished: torch.Tensor | None = None) -> torch.Tensor:
     """One vocabulary shard ``[G, W, V_local]`` (columns from ``vstart``; it may be empty) reduced to a
     block of candidates (uint8 [n]). ``v_plan``: the largest shard's columns, the same on every rank."""
+    if local_logits.dim() != 3 or not (0 <= vstart < 2**32 and 1 <= v_plan < 2**31):
+        raise _lib.MinitpB200Error(f"beam_candidates: need logits [G, W, V_local], a start below 2^32 and a plan of at "
+                                   f"least one column, got {tuple(local_logits.shape)}, {vstart} and {v_plan}")
     g, w, v = local_logits.shape
     zeros = local_logits.new_empty((g, w), dtype=torch.float32)  # stands for the scores in the checks
     dev, x, ld = _beam_inputs("beam_candidates", local_logits, zeros, k, finished, 0, least=0)
@@ -286,6 +289,10 @@ def beam_pick(blocks: torch.Tensor, scores: torch.Tensor, k: int, v_plan: int, f
               eos_token_id: int | None = None):
     """``beam_select``'s result from the candidate blocks ``[shards, n]`` of every vocabulary shard."""
     dev = _same_device("beam_pick", blocks, scores, finished)
+    if scores.dim() != 2 or not (1 <= k <= 64 and 1 <= v_plan < 2**31):
+        raise _lib.MinitpB200Error(f"beam_pick: need scores [G, W] and k in [1, 64], got {tuple(scores.shape)} and {k}")
+    if eos_token_id is not None and not 0 <= eos_token_id < 2**32 - 1:
+        raise _lib.MinitpB200Error(f"beam_pick: eos_token_id {eos_token_id} out of range")
     g, w = scores.shape
     if blocks.dim() != 2 or blocks.dtype != torch.uint8 or not blocks.is_contiguous() or \
             blocks.shape[1] != beam_block_bytes(g * w, v_plan, k):
@@ -302,11 +309,13 @@ def beam_pick(blocks: torch.Tensor, scores: torch.Tensor, k: int, v_plan: int, f
     return out, parents, tokens, done
 
 
-def _length_arg(name: str, lengths, count: int, dev):
+def _length_arg(name: str, lengths, count: int, cap: int, dev):
     """(device pointer or None, host value) of a per-row length argument."""
     if isinstance(lengths, int):
+        if not 0 <= lengths <= cap:
+            raise _lib.MinitpB200Error(f"{name}: length {lengths} outside the cache of {cap} positions")
         return None, lengths
-    if lengths.dtype != torch.int32 or lengths.shape != (count,) or not lengths.is_contiguous() or \
+    if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or lengths.shape != (count,) or not lengths.is_contiguous() or \
             lengths.device != dev:
         raise _lib.MinitpB200Error(f"{name}: lengths must be an int or contiguous int32 [{count}] on {dev}")
     return lengths.data_ptr(), 0
@@ -321,7 +330,8 @@ def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
     ``k_caches`` / ``v_caches``: lists of ``[G * W, hkv, cap, hd]`` caches;
     ``parents`` int64 ``[G, W]``. The first ``lengths`` positions of the source
     row are copied (an int, or int32 ``[G * W]`` by source row); later ones stay
-    as they were. A parent outside [0, W) leaves its row alone.
+    as they were. A parent outside [0, W) leaves its row alone. No two caches may
+    share memory.
     """
     name = "reorder_cache_"
     if parents.dim() != 2 or parents.dtype != torch.int64 or not parents.is_contiguous():
@@ -338,7 +348,7 @@ def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
         raise _lib.MinitpB200Error(f"{name}: caches must be [{g * w}, hkv, cap, hd], got {tuple(shape)}")
     if set(map(_SHAPE_TYPE_PLACE, caches)) != {(shape, dtype, dev)} or not all(map(torch.Tensor.is_contiguous, caches)):
         raise _lib.MinitpB200Error(f"{name}: caches must be contiguous, of one shape, dtype and device")
-    lens, length = _length_arg(name, lengths, g * w, dev)
+    lens, length = _length_arg(name, lengths, g * w, shape[2], dev)
     ptrs = (ctypes.c_void_p * (2 * n))(*map(torch.Tensor.data_ptr, caches))
     _call_on(dev, "mtpb_kv_reorder", ptrs, ctypes.addressof(ptrs) + 8 * n, n, parents.data_ptr(), lens, length, g, w,
              shape[1], shape[2], shape[3], _lib.dtype_code(dtype))
@@ -353,8 +363,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     ``N / G`` consecutive rows; own caches ``[N, hkv, cap, hd]``. Token t of row
     n sees positions ``[0, prefix_lens[g])`` of the prefix and
     ``[0, cache_lens[n] - (T - 1 - t))`` of its own cache (which holds the T
-    tokens already); one that sees nothing gets 0. Lengths are ints or int32
-    tensors ``[G]`` / ``[N]``, clamped to their cache.
+    tokens already); one that sees nothing gets 0. Lengths are ints within their
+    cache, or int32 tensors ``[G]`` / ``[N]``, clamped to it.
     """
     name = "shared_prefix_attention"
     dev = _same_device(name, q, k_prefix, v_prefix, k_cache, v_cache)
@@ -373,8 +383,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         if c.dtype != q.dtype or not c.is_contiguous():
             raise _lib.MinitpB200Error(f"{name}: caches must be contiguous and of q's dtype")
     q = _c(q)
-    plen, plen_all = _length_arg(name, prefix_lens, g, dev)
-    clen, clen_all = _length_arg(name, cache_lens, n, dev)
+    plen, plen_all = _length_arg(name, prefix_lens, g, cap_p, dev)
+    clen, clen_all = _length_arg(name, cache_lens, n, cap, dev)
     code = _lib.dtype_code(q.dtype)
     need = _lib.load().mtpb_shared_attention_workspace(g, n // g, t, hq, hkv, hd, cap_p, cap, code)
     if need < 0:

@@ -53,6 +53,14 @@ def test_reorder_refusals(lib):
         _refused(lib, "mtpb_kv_reorder", list((ok | change).values()), match)
 
 
+def test_reorder_refuses_caches_that_overlap(lib):
+    size = 4 * 2 * 8 * 64 * 2  # bytes of a cache
+    for ks, vs in [((P, P + size), (P + 2 * size, P)), ((P, P + size - 16), (P + 4 * size, P + 8 * size)), ((P,), (P,))]:
+        n = len(ks)
+        arr = ctypes.c_void_p * n
+        _refused(lib, "mtpb_kv_reorder", (arr(*ks), arr(*vs), n, P, None, 5, 1, 4, 2, 8, 64, _lib.MTPB_BF16, None), "overlap")
+
+
 def test_attention_refusals(lib):
     ok = dict(q=P, kp=P, vp=P, pl=None, plen=1 << 20, kc=P, vc=P, cl=None, clen=5, out=P, G=2, W=4, T=1, hq=14, hkv=2, hd=64,
               cap_p=1 << 20, cap=8, dtype=_lib.MTPB_BF16, ws=P, n=1 << 30, st=None)

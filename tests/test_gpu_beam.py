@@ -446,3 +446,38 @@ def test_status_is_clean(lib):
     st = ctypes.c_uint32(7)
     _lib.call("mtpb_beam_status", ctypes.byref(st))
     assert st.value == 0
+
+
+def test_refusals_before_a_launch(lib):
+    """Arguments that the Python calls refuse for tensors on the device."""
+    from minitp_b200 import _lib, ops
+
+    def refused(match, call, *args):
+        with pytest.raises(_lib.MinitpB200Error, match=match):
+            call(*args)
+
+    a, b = (torch.zeros(2, 1, 4, 16, device="cuda") for _ in range(2))
+    parents = torch.zeros(1, 2, dtype=torch.long, device="cuda")
+    refused("overlap", ops.reorder_cache_, [a, a], [b, b], parents, 4)
+    refused("overlap", ops.reorder_cache_, [a], [a], parents, 4)
+    for n in (5, -1, 2 ** 32 + 4):
+        refused("outside", ops.reorder_cache_, [a], [b], parents, n)
+    refused("lengths must", ops.reorder_cache_, [a], [b], parents, 4.0)
+    refused("lengths must", ops.reorder_cache_, [a], [b], parents, torch.zeros(2, dtype=torch.long, device="cuda"))
+    q = torch.zeros(2, 1, 32, device="cuda")
+    c = torch.zeros(1, 1, 4, 16, device="cuda")
+    refused("outside", ops.shared_prefix_attention, q, c, c, 2 ** 32, a, b, 4, 2, 1)
+    refused("outside", ops.shared_prefix_attention, q, c, c, 4, a, b, 5, 2, 1)
+    refused("do not fit", ops.shared_prefix_attention, q, c, c, 4, a, b, 4, 1, 1)
+    refused("16-byte", ops.shared_prefix_attention, torch.zeros(65, device="cuda")[1:].view(2, 1, 32), c, c, 4, a, b, 4, 2, 1)
+    x, s = torch.zeros(1, 2, 10, device="cuda"), torch.zeros(1, 2, device="cuda")
+    refused("out of range", ops.beam_select, x, s, 2, None, 2 ** 32 - 1)
+    refused("eos_token_id", ops.beam_select, x, s, 2, torch.zeros(1, 2, dtype=torch.bool, device="cuda"))
+    refused("k in", ops.beam_select, x, s, 2 ** 32 + 2)
+    refused("beam_candidates", ops.beam_candidates, x, 2, 2 ** 32, 10)
+    refused("beam_candidates", ops.beam_candidates, x, 2, 0, 2 ** 32 + 10)
+    refused("beam_candidates", ops.beam_candidates, x[0], 2, 0, 10)
+    block = ops.beam_candidates(x, 2, 0, 10)
+    refused("beam_pick", ops.beam_pick, block[None], s[0], 2, 10)
+    refused("beam_pick", ops.beam_pick, block[None], s, 65, 10)
+    refused("blocks must", ops.beam_pick, block[None], s, 3, 10)
