@@ -99,6 +99,12 @@ def _session(model: TPQwen2ForCausalLM, kind: tuple, *shape) -> _SharedSession:
     return s
 
 
+def _check_positions(model: TPQwen2ForCausalLM, last: int) -> None:
+    """The position table covers ``last`` tokens (a step on the device could only flag one behind it)."""
+    if last > model.cfg.max_position_embeddings:
+        raise ValueError(f"{last} positions needed, the model has {model.cfg.max_position_embeddings}")
+
+
 @torch.inference_mode()
 def generate_beam(
     model: TPQwen2ForCausalLM,
@@ -131,6 +137,7 @@ def generate_beam(
         raise ValueError(f"eos_token_id {eos_token_id} outside the vocabulary")
     b, p = input_ids.shape
     w, eos, head = num_beams, eos_token_id, model.lm_head
+    _check_positions(model, p + max_new_tokens - 1)
     s = _session(model, ("beam", eos), b, w, p, max_new_tokens - 1, max_new_tokens, input_ids.device)
     s.prefix.seq_len = 0
     logits = model(input_ids, kv_cache=s.prefix, last_only=True)
@@ -196,6 +203,7 @@ def generate_shared_prefix(
         raise ValueError(f"{n} rows do not divide into {g} shared prefixes")
     if max_new_tokens < 1:
         raise ValueError("max_new_tokens must be at least 1")
+    _check_positions(model, p + t + max_new_tokens - 1)
     stops = early_stop and eos_token_id is not None
     eos = eos_token_id if stops else None
     s = _session(model, ("prefix", eos), g, n // g, p, t + max_new_tokens - 1, max_new_tokens, input_ids.device)

@@ -195,6 +195,21 @@ def test_forward_refuses_caches_that_do_not_fit(lib):
         generate_shared_prefix(gpu, ids[:2], ids, 4)
 
 
+def test_positions_behind_the_table_are_refused(lib):
+    from minitp_b200.beam import generate_beam, generate_shared_prefix
+
+    gpu, _, cfg = _models()
+    top = cfg.max_position_embeddings
+    ids = _prompt(cfg, 2, 3, 1).cuda()
+    with pytest.raises(ValueError, match="positions"):
+        generate_beam(gpu, ids, top - 1, 2)
+    with pytest.raises(ValueError, match="positions"):
+        generate_shared_prefix(gpu, ids[:1], ids, top - 4)
+    assert generate_beam(gpu, ids, top - 2, 2)[0].shape == (2, 1, top + 1)
+    assert generate_shared_prefix(gpu, ids[:1], ids, top - 5).shape == (2, top - 2)
+    gpu.ctx.comm().raise_on_error()
+
+
 def test_graphs_kept_over_a_larger_prompt(lib):
     """A later, larger prompt moves the model's buffers: the graphs captured before it are not replayed over the old ones."""
     from minitp_b200.beam import generate_beam, generate_shared_prefix
