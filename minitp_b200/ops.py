@@ -7,7 +7,7 @@ stream. None of them has a CPU path: CPU tensors raise.
 
 from __future__ import annotations
 
-import ctypes
+import array
 import operator
 
 import torch
@@ -321,7 +321,8 @@ def _length_arg(name: str, lengths, count: int, cap: int, dev):
     return lengths.data_ptr(), 0
 
 
-_SHAPE_TYPE_PLACE = operator.attrgetter("shape", "dtype", "device")
+# what a reordering asks of each of a model's caches (a loop over the 48 of the 0.5B shape costs three times this)
+_SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
 
 
 def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
@@ -346,11 +347,13 @@ def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
     g, w = parents.shape
     if first.dim() != 4 or shape[0] != g * w:
         raise _lib.MinitpB200Error(f"{name}: caches must be [{g * w}, hkv, cap, hd], got {tuple(shape)}")
-    if set(map(_SHAPE_TYPE_PLACE, caches)) != {(shape, dtype, dev)} or not all(map(torch.Tensor.is_contiguous, caches)):
+    if set(map(_SHAPE, caches)) != {shape} or set(map(_DTYPE, caches)) != {dtype} or \
+            set(map(torch.Tensor.get_device, caches)) != {dev.index} or not all(map(torch.Tensor.is_contiguous, caches)):
         raise _lib.MinitpB200Error(f"{name}: caches must be contiguous, of one shape, dtype and device")
     lens, length = _length_arg(name, lengths, g * w, shape[2], dev)
-    ptrs = (ctypes.c_void_p * (2 * n))(*map(torch.Tensor.data_ptr, caches))
-    _call_on(dev, "mtpb_kv_reorder", ptrs, ctypes.addressof(ptrs) + 8 * n, n, parents.data_ptr(), lens, length, g, w,
+    ptrs = array.array("Q", map(torch.Tensor.data_ptr, caches))
+    at, _ = ptrs.buffer_info()
+    _call_on(dev, "mtpb_kv_reorder", at, at + 8 * n, n, parents.data_ptr(), lens, length, g, w,
              shape[1], shape[2], shape[3], _lib.dtype_code(dtype))
 
 
