@@ -247,8 +247,9 @@ int mtpb_argmax(void* comm, const void* logits, int M, int V_local, int64_t ld, 
  *   - A beam whose score is -inf or NaN, or without a logit above -inf, has
  *     no candidate; a total below fp32's range is none. Places without a
  *     candidate get score -inf, parent 0 and token eos (0 without one).
- * `block`: workspace of mtpb_beam_block_bytes(G*W, V, k) bytes, 16-byte
- * aligned, private to the call until it has run. */
+ * V below 2^30. The outputs may not overlap the inputs. `block`: workspace of
+ * mtpb_beam_block_bytes(G*W, V, k) bytes, 16-byte aligned, private to the call
+ * until it has run. */
 long long mtpb_beam_block_bytes(int rows, int V_plan, int k);
 int mtpb_beam_select(const void* logits, int64_t ld, int G, int W, int V, const float* scores,
                      const uint8_t* finished, int64_t eos, int k, float* out_scores,
@@ -287,12 +288,13 @@ int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers,
  * [G*W, hkv, cap, hd]. Token t (of T) of row n attends to positions
  * [0, prefix_lens[g]) of its group's prefix and [0, cache_lens[n] - (T-1-t))
  * of its own cache (cache_lens counts the T tokens' own positions too); a
- * token that sees none gets 0. Lengths: device int32 arrays, clamped to their
+ * token that sees none, or whose scores are all -inf, gets 0. Lengths: device int32 arrays, clamped to their
  * cache's capacity, or the host value (0 .. capacity) for every group / row
  * when the array is NULL. scale = 1/sqrt(hd); hd 16, 32, 64 or 128. Softmax
  * statistics and sums are fp32; bf16 probabilities are rounded to bf16 for
  * their product with V. What a token does not see does not reach it, NaN and
- * infinities included. `ws`: at least mtpb_shared_attention_workspace(...) bytes,
+ * infinities included. out may not overlap an input; q, out and the caches are
+ * 16-byte aligned. `ws`: at least mtpb_shared_attention_workspace(...) bytes,
  * 16-byte aligned, private to the call until it has run. */
 long long mtpb_shared_attention_workspace(int G, int W, int T, int hq, int hkv, int hd, int cap_p,
                                           int cap, int dtype);

@@ -77,7 +77,7 @@ size_t beam_block(long long rows, const BeamPlan& b, int k) {
 
 int beam_check(long long rows, long long V, int k) {
   if (rows < 1 || rows > (1 << 20)) return bad("beam selection: need 1 .. 2^20 rows");
-  if (V < 1 || V > 0x7FFFFFFFll) return bad("beam selection: empty vocabulary, or one of 2^31 or more");
+  if (V < 1 || V >= 1ll << 30) return bad("beam selection: empty vocabulary, or one of 2^30 or more");
   if (k < 1 || k > kBeamMaxK) return bad("beam selection: k must be in [1, 64]");
   return MTPB_OK;
 }

@@ -230,6 +230,8 @@ class TPQwen2ForCausalLM(nn.Module):
         """
         n, t = ids.shape
         groups = prefix.k[0].shape[0]
+        if prefix is kv:
+            raise ValueError("the own cache has to be another one than the prefix")
         if n % groups:
             raise ValueError(f"{n} rows do not divide into {groups} shared prefixes")
         if kv.k[0].shape[0] != n or len(prefix.k) != len(kv.k):

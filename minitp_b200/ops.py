@@ -213,8 +213,8 @@ def _beam_inputs(name: str, logits, scores, k, finished, eos_token_id, least: in
     if scores.dtype != torch.float32 or not scores.is_contiguous():
         raise _lib.MinitpB200Error(f"{name}: scores must be contiguous fp32")
     g, w, v = logits.shape
-    if not (1 <= w <= 64 and 1 <= k <= 64 and g >= 1 and least <= v < 2**31):
-        raise _lib.MinitpB200Error(f"{name}: need 1..64 beams, k in [1, 64] and a vocabulary of 1 .. 2^31 - 1")
+    if not (1 <= w <= 64 and 1 <= k <= 64 and g >= 1 and least <= v < 2**30):
+        raise _lib.MinitpB200Error(f"{name}: need 1..64 beams, k in [1, 64] and a vocabulary of 1 .. 2^30 - 1")
     if finished is not None:
         if finished.dtype != torch.bool or finished.shape != scores.shape or not finished.is_contiguous():
             raise _lib.MinitpB200Error(f"{name}: finished must be contiguous bool [G, W]")
@@ -273,7 +273,7 @@ def beam_candidates(local_logits: torch.Tensor, k: int, vstart: int, v_plan: int
                     finished: torch.Tensor | None = None) -> torch.Tensor:
     """One vocabulary shard ``[G, W, V_local]`` (columns from ``vstart``; it may be empty) reduced to a
     block of candidates (uint8 [n]). ``v_plan``: the largest shard's columns, the same on every rank."""
-    if local_logits.dim() != 3 or not (0 <= vstart < 2**32 and 1 <= v_plan < 2**31):
+    if local_logits.dim() != 3 or not (0 <= vstart < 2**32 and 1 <= v_plan < 2**30):
         raise _lib.MinitpB200Error(f"beam_candidates: need logits [G, W, V_local], a start below 2^32 and a plan of at "
                                    f"least one column, got {tuple(local_logits.shape)}, {vstart} and {v_plan}")
     g, w, v = local_logits.shape
@@ -289,7 +289,7 @@ def beam_pick(blocks: torch.Tensor, scores: torch.Tensor, k: int, v_plan: int, f
               eos_token_id: int | None = None):
     """``beam_select``'s result from the candidate blocks ``[shards, n]`` of every vocabulary shard."""
     dev = _same_device("beam_pick", blocks, scores, finished)
-    if scores.dim() != 2 or not (1 <= k <= 64 and 1 <= v_plan < 2**31):
+    if scores.dim() != 2 or not (1 <= k <= 64 and 1 <= v_plan < 2**30):
         raise _lib.MinitpB200Error(f"beam_pick: need scores [G, W] and k in [1, 64], got {tuple(scores.shape)} and {k}")
     if eos_token_id is not None and not 0 <= eos_token_id < 2**32 - 1:
         raise _lib.MinitpB200Error(f"beam_pick: eos_token_id {eos_token_id} out of range")

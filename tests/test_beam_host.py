@@ -25,6 +25,7 @@ def test_select_refusals(lib):
                           (dict(eos=2 ** 32), "end token"), (dict(o=None), "null"), (dict(G=40000), "65535")]:
         _refused(lib, "mtpb_beam_select", list((ok | change).values()), match)
     assert lib.mtpb_beam_block_bytes(8, 151936, 65) < 0
+    assert lib.mtpb_beam_block_bytes(1, 2 ** 30 - 1, 4) > 0 > lib.mtpb_beam_block_bytes(1, 2 ** 30, 4)
     assert lib.mtpb_beam_block_bytes(0, 151936, 4) < 0
     assert lib.mtpb_beam_block_bytes(8, 151936, 4) > 0
 

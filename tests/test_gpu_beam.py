@@ -392,6 +392,22 @@ def test_attention_shorter_than_the_capacity(lib, t, hkv, hd, cap_p, plen, cap, 
     assert bool(((got.double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_attention_of_more_rows_than_a_grid_axis(lib, dtype):
+    from minitp_b200 import ops
+
+    n, hd = 65539, 64
+    r = _gen(13)
+    q, kp, vp = (torch.randn(*s, generator=r).to(DT[dtype]) for s in ((n, 1, 2 * hd), (1, 1, 70, hd), (1, 1, 70, hd)))
+    kc, vc = (torch.randn(n, 1, 6, hd, generator=r).to(DT[dtype]) for _ in range(2))
+    cl = torch.randint(0, 7, (n,), generator=r, dtype=torch.int32)
+    got = ops.shared_prefix_attention(*(x.cuda() for x in (q, kp, vp)), 65, kc.cuda(), vc.cuda(), cl.cuda(), 2, 1).cpu()
+    some = torch.tensor([0, 1, 127, 128, 32768, 65534, 65535, 65536, n - 1])
+    want, tol = beam_ref.attend(q[some], kp, vp, torch.tensor([65]), kc[some], vc[some], cl[some], 2, 1)
+    assert bool(((got[some].double() - want).abs() <= tol).all())
+    assert bool(torch.isfinite(got.float()).all())
+
+
 def test_attention_equals_attention_over_one_cache(lib):
     """Prefix and own cache laid end to end give the framework's plain attention."""
     from minitp_b200 import ops

@@ -195,6 +195,17 @@ def test_forward_refuses_caches_that_do_not_fit(lib):
         generate_shared_prefix(gpu, ids[:2], ids, 4)
 
 
+def test_a_cache_behind_itself_is_refused(lib):
+    from minitp_b200.generation import make_kv_cache
+
+    gpu, _, cfg = _models()
+    ids = _prompt(cfg, 2, 2, 1).cuda()
+    cache = make_kv_cache(gpu, 2, 8)
+    gpu(ids, kv_cache=cache)
+    with pytest.raises(ValueError, match="another"):
+        gpu(ids, kv_cache=cache, prefix_cache=cache)
+
+
 def test_positions_behind_the_table_are_refused(lib):
     from minitp_b200.beam import generate_beam, generate_shared_prefix
 
