@@ -232,9 +232,11 @@ def _beam_inputs(name: str, logits, scores, k, finished, eos_token_id, least: in
 
 
 def _beam_outputs(dev, g: int, k: int, flags: bool):
-    parents = torch.empty((g, k), dtype=torch.int64, device=dev)
-    return (torch.empty((g, k), dtype=torch.float32, device=dev), parents, torch.empty_like(parents),
-            torch.empty((g, k), dtype=torch.bool, device=dev) if flags else None)
+    # (empty_strided takes half of empty's time, which counts in a call of 20 us)
+    size, stride = (g, k), (k, 1)
+    parents = torch.empty_strided(size, stride, dtype=torch.int64, device=dev)
+    return (torch.empty_strided(size, stride, dtype=torch.float32, device=dev), parents, torch.empty_like(parents),
+            torch.empty_strided(size, stride, dtype=torch.bool, device=dev) if flags else None)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: torch.Tensor | None = None,
@@ -254,7 +256,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: to
     dev, logits, ld = _beam_inputs("beam_select", logits, scores, k, finished, eos_token_id)
     g, w, v = logits.shape
     out, parents, tokens, done = _beam_outputs(dev, g, k, eos_token_id is not None)
-    block = torch.empty(beam_block_bytes(g * w, v, k), dtype=torch.uint8, device=dev)
+    block = torch.empty_strided((beam_block_bytes(g * w, v, k),), (1,), dtype=torch.uint8, device=dev)
     _call_on(dev, "mtpb_beam_select", logits.data_ptr(), ld, g, w, v, scores.data_ptr(), _lib.ptr(finished),
              -1 if eos_token_id is None else eos_token_id, k, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
              _lib.ptr(done), block.data_ptr(), _lib.dtype_code(logits.dtype))
