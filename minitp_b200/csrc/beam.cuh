@@ -22,16 +22,25 @@ namespace mtpb {
 constexpr int kBeamMaxK = 64;
 constexpr int kBeamMaxW = 64;
 
-// Sum of a chunk's exponentials, s = sum 2^(x log2(e) - beam_ref(m)). m need
-// not be the maximum: it keeps s in range. -inf: nothing summed. Where m is
-// 10^30 or more (an infinity, a mask of the type's lowest value), neighbours of
-// m are further off than any exponential reaches: s counts the values equal to m.
+// Sum of a chunk's exponentials, s = sum exp(x - m). m need not be the maximum:
+// it keeps s in range. -inf: nothing summed.
 struct BeamStat {
   float m, s;
 };
+// While a lane sums, it takes 2^(x L - c) with one fused multiply-add a value:
+// L is log2(e) and c = m L, both rounded to fp32. The exponent is then off by
+// m L - c for every x alike: up to 64 for |m| below 2^30, so that sums stay in
+// range, and beam_own takes it out of the lane's sum. (Over a difference x - m,
+// L's own rounding counts 1.3e-8 of it.) From 2^30 on fp32 neighbours are at
+// least 64 apart (those below too): no other value's exponential counts beside
+// m's, so s counts the values equal to m, infinities among them.
 constexpr float kBeamLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float beam_ref(float m) { return __fmul_rn(m, kBeamLog2e); }
-__device__ __forceinline__ bool beam_far(float m) { return !(fabsf(m) < 1e30f); }
+__device__ __forceinline__ bool beam_far(float m) { return !(fabsf(m) < 1073741824.f); }
+// A lane's sum against m itself.
+__device__ __forceinline__ float beam_own(float m, float s) {
+  return beam_far(m) ? s : s * exp2_approx(-fmaf(m, kBeamLog2e, -beam_ref(m)));
+}
 
 // Order-preserving key of a finite or +inf logit and its id; 0: no candidate.
 __device__ __forceinline__ uint32_t beam_val_key(float v) {
@@ -47,7 +56,7 @@ __device__ __forceinline__ uint64_t beam_key(uint32_t key, uint32_t id) { return
 
 // What a sum against m counts in one against the larger top.
 __device__ __forceinline__ float beam_weight(float m, float top) {
-  return m == top ? 1.f : fmaxf(exp2_approx(beam_ref(m) - beam_ref(top)), 0.f);  // (inf - inf: 0)
+  return m == top ? 1.f : exp2_approx((m - top) * kBeamLog2e);  // (equal infinities: 1)
 }
 __device__ __forceinline__ uint64_t warp_max_u64(uint64_t v) {
 #pragma unroll
@@ -273,7 +282,7 @@ __global__ void __launch_bounds__(kBeamThreads + 32, sizeof(T) == 2 ? 2 : 3) bea
     }
     const float top = fmaxf(max3(q[0], q[1], q[2]), q[3]);
     // ---- sum: the reference follows the maximum only when it has to
-    if (top - m > 40.f) {
+    if (top - m > 40.f) {  // (every larger value, from 2^29 on)
       s = beam_far(m) || beam_far(top) ? 0.f : s * exp2_approx(beam_ref(m) - beam_ref(top));
       m = top;
       c = beam_ref(m);
@@ -445,7 +454,7 @@ __global__ void __launch_bounds__(kBeamThreads + 32, sizeof(T) == 2 ? 2 : 3) bea
     float cm = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
-    s = warp_sum(s * beam_weight(m, cm));
+    s = warp_sum(beam_own(m, s) * beam_weight(m, cm));
     if (lane == 0) stat[warp] = make_float2(cm, s);
     // ---- the chunk's k best: the warps' candidates (at most 64 each) from the common floor on, ranked
     if (l.n > kBeamMaxK) beam_cut<kLow>(l, p.k, &floor_key);
@@ -558,19 +567,15 @@ __global__ void __launch_bounds__(kBeamThreads) beam_pick_kernel(const BeamPickP
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       double s = 0.0;
+      constexpr double kLog2ed = 1.44269504088896340736, kLn2d = 0.69314718055994530942;
       auto add = [&](const BeamStat& t) {
-        if (t.m == m)
-          s += double(t.s);
-        else if (!beam_far(m))
-          s += double(t.s) * exp2(double(beam_ref(t.m)) - double(beam_ref(m)));
+        s += double(t.s) * (t.m == m ? 1.0 : exp2((double(t.m) - double(m)) * kLog2ed));
       };
       add(mine);
       for (int i = lane + 32; i < n; i += 32) add(at(i));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      // log sum exp - m, the rounding of the reference taken out
-      constexpr double kLn2d = 0.69314718055994530942;
-      bs = sc - kLn2d * log2(s) - (beam_far(m) ? 0.0 : kLn2d * double(beam_ref(m)) - double(m));
+      bs = sc - kLn2d * log2(s);
     }
     if (lane == 0) {
       base[b] = bs;

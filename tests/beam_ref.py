@@ -95,6 +95,26 @@ def check_select(got, logits, scores, k, finished=None, eos=None):
         assert torch.equal(done, (tok == eos) | old.gather(1, par))
 
 
+def check_totals(got, logits, scores, k):
+    """Every place holds the total of the candidate that it names, and is the place's best, each within
+    `select_tolerance` of its own size (one candidate of -1e9 loosens nothing for the others)."""
+    out, par, tok = (x.cpu() for x in got[:3])
+    best, wpar, wtok, _ = select(logits, scores, k)
+    t = totals(logits, scores)
+    v = logits.shape[-1]
+    for g in range(best.shape[0]):
+        assert len({(int(p), int(x)) for p, x, b in zip(par[g], tok[g], best[g]) if b > -math.inf}) == \
+            int((best[g] > -math.inf).sum())
+        for j in range(k):
+            at, want = (int(par[g, j]), int(tok[g, j])), float(best[g, j])
+            if want == -math.inf:
+                assert float(out[g, j]) == want and at == (int(wpar[g, j]), int(wtok[g, j]))
+                continue
+            tol = select_tolerance(v, best[g, j])
+            assert abs(float(out[g, j]) - want) <= tol, (g, j, float(out[g, j]), want)
+            assert abs(float(t[g, at[0], at[1]]) - want) <= 2 * tol
+
+
 def reorder(cache, parents, lengths):
     """The reordered copy of one [G*W, hkv, cap, hd] cache."""
     out = cache.clone()

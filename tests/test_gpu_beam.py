@@ -78,6 +78,51 @@ def test_select_masks_infinities_and_nan(lib):
     beam_ref.check_select(ops.beam_select(y.cuda(), s.cuda(), 8), y, s, 8)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e10, -3e10, -1e11, -1e12, -1e20, 1e4, 1e6, 1e9, 1e10, 1e12, 1e20])
+@pytest.mark.parametrize("v", [40, 30000])
+def test_select_logits_far_from_zero(lib, dtype, mask, v):
+    """Banned tokens of any large value beside a few live ones, and rows that hold nothing else."""
+    from minitp_b200 import ops
+
+    r = _gen(v + int(abs(mask)) % 1000)
+    x = torch.full((3, 3, v), mask)
+    live = torch.randint(0, v, (3, 3, 5), generator=r)
+    x.scatter_(2, live, torch.randn(3, 3, 5, generator=r) * 3)
+    x[1, 0] = mask  # one such row beside others
+    x[2, 1:] = mask
+    x[2, 0] = torch.randn(v, generator=r) * 3  # .. and beside a plain one
+    x = x.to(DT[dtype])
+    s = torch.randn(3, 3, generator=r) * 2 - 20
+    for k in (1, 3, 8, 24):
+        beam_ref.check_totals(ops.beam_select(x.cuda(), s.cuda(), k), x, s, k)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("v", [333, 20001])
+def test_select_logits_of_every_size(lib, dtype, v):
+    """Rows moved away from zero, rows of every spread, and logits around the border from which on equal
+    values are counted (2^30), where neighbours are 64 and 128 apart."""
+    from minitp_b200 import ops
+
+    r = _gen(v)
+    rows = [torch.randn(v, generator=r) * 3 + d for d in (-1e4, 1e4, -1e6, 1e6, 3e7, -3e8)]
+    rows += [torch.randn(v, generator=r) * 10.0 ** e for e in range(1, 16)]
+    border = 2.0 ** 30
+    steps = torch.tensor([-192.0, -128.0, -64.0, 0.0, 128.0, 256.0])
+    rows += [sign * (border + steps[torch.randint(0, n, (v,), generator=r)]) for n in (3, 4, 6) for sign in (1, -1)]
+    rows += [(border / 2 + steps[torch.randint(0, 6, (v,), generator=r)] / 2) * sign for sign in (1, -1)]
+    rows += [-(border + 64.0 * torch.randint(-8, 9, (v,), generator=r)), torch.full((v,), -border), torch.full((v,), border - 64)]
+    x = torch.stack(rows)[:, None].to(DT[dtype])
+    s = torch.randn(len(rows), 1, generator=r)
+    for k in (1, 9):
+        beam_ref.check_totals(ops.beam_select(x.cuda(), s.cuda(), k), x, s, k)
+    # pairs of such rows as the beams of one prompt
+    n = len(rows) // 2 * 2
+    x, s = x[:n].reshape(n // 2, 2, v), s[:n].reshape(n // 2, 2)
+    beam_ref.check_totals(ops.beam_select(x.cuda(), s.cuda(), 9), x, s, 9)
+
+
 def test_select_first_step_from_one_beam(lib):
     """The first step: one live beam per prompt gives k different tokens."""
     from minitp_b200 import ops
