@@ -1017,8 +1017,9 @@ __global__ void __launch_bounds__(kSaTcThreads, 1)
       wa = exp2_approx(m - ref);
       wb = exp2_approx(b.x - ref);
       l = l * wa + b.y * wb;
-      m = sa_max_of(top, l);
+      m = top;
     }
+    m = sa_max_of(m, l);  // (MT 2: tiles behind the NaN have set another max)
     if (MT == 2 || x == 0) {
       const SaPart at = sa_part<HD>(p, it.own, it.split, it.plane, it.row0 + row);
       if (odd_sh) l = -l;

@@ -412,6 +412,29 @@ def test_attention_nan_scores(lib, dtype, hq, hkv, hd, g, w, t):
         check((q, one, vp, pl, kc, vc, cl), reached)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("own", [False, True])
+def test_attention_nan_beside_a_range_of_far_higher_scores(lib, hd, own):
+    """A key range with a NaN score makes its rows NaN, however small its weight is in the join."""
+    from minitp_b200 import ops
+
+    n, t = (1, 40) if own else (40, 1)  # 160 rows of one KV head
+    hq, hkv, long = 4, 1, 26000
+    r = _gen(hd + own)
+    u = torch.randn(hd, generator=r)
+    u /= u.norm()
+    q = (u * 20 + 0.1 * torch.randn(n, t, hq, hd, generator=r)).view(n, t, hq * hd)
+    k, v = torch.randn(1, 1, long, hd, generator=r), torch.randn(1, 1, long, hd, generator=r)
+    k[0, 0, 20000:20010] += u * 15 * math.sqrt(hd)  # scores of about 300; the others' are below 100
+    small = torch.randn(1 if own else n, 1, t + 3, hd, generator=r)
+    q, k, v, small = (x.to(torch.bfloat16).cuda() for x in (q, k, v, small))
+    for j in (0, 1, 131, 4000, 19000):
+        bad = k.clone()
+        bad[0, 0, j, 3] = math.nan
+        caches = (small, small, 0, bad, v, long) if own else (bad, v, long, small, small, t + 3)
+        assert bool(ops.shared_prefix_attention(q, *caches, hq, hkv).isnan().all()), j
+
+
 def test_attention_lengths_are_clamped_and_may_be_ints(lib):
     from minitp_b200 import ops
 
