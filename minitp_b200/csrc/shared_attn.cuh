@@ -13,9 +13,10 @@
 //
 // NaN and infinities go where the formula takes them and nowhere else: a score
 // that is NaN or +inf makes its row NaN (a sum that is NaN is handed on with a
-// NaN max, which no join passes over); positions that a token does not see
-// reach it neither through K (its scores are selected away) nor through V (0
-// times NaN would be NaN: such terms are left out or zeroed).
+// NaN max, which no join passes over), and a NaN among V makes its dim NaN,
+// whatever the weight; positions that a token does not see reach it neither
+// through K (its scores are selected away) nor through V (0 times NaN would be
+// NaN: such terms are left out or zeroed).
 #pragma once
 
 #include <type_traits>
@@ -604,14 +605,13 @@ __global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const S
     const float ref = mx == -INFINITY ? 0.f : mx;
     float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
     auto add = [&](float m, float l, const float4& f) {
-      const float w = m == -INFINITY ? 0.f : expf(m - ref);
+      if (m == -INFINITY) return;  // an empty range leaves its sums unwritten
+      const float w = expf(m - ref);  // (0 takes a NaN or an infinity among the sums along)
       den = fmaf(w, l, den);
-      if (w != 0.f) {  // an empty range leaves its sums unwritten
-        num[0] = fmaf(w, f.x, num[0]);
-        num[1] = fmaf(w, f.y, num[1]);
-        num[2] = fmaf(w, f.z, num[2]);
-        num[3] = fmaf(w, f.w, num[3]);
-      }
+      num[0] = fmaf(w, f.x, num[0]);
+      num[1] = fmaf(w, f.y, num[1]);
+      num[2] = fmaf(w, f.z, num[2]);
+      num[3] = fmaf(w, f.w, num[3]);
     };
 #pragma unroll
     for (int w = 0; w < NW; ++w)
@@ -1081,7 +1081,7 @@ constexpr int kSaJoinThreads = 256;
 template <typename T, int HD>
 __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams p) {
   constexpr int VE = VecTraits<T>::kElems, U = 4;
-  extern __shared__ float2 sa_ml[];  // a range and row: max, sum; then weight
+  extern __shared__ float2 sa_ml[];  // a range and row: max, sum; then weight, -1 for an empty range
   float2* ml = sa_ml;
   __shared__ float res[32][HD + 1];
   __shared__ float inv[32];
@@ -1106,7 +1106,11 @@ __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams 
     const float ref = mx == -INFINITY ? 0.f : mx;
     for (int s = 0; s < slots; ++s) {
       const float2 v = ml[s * 32 + tid];
-      const float w = v.x == -INFINITY ? 0.f : expf(v.x - ref);
+      if (v.x == -INFINITY) {
+        ml[s * 32 + tid].x = -1.f;
+        continue;
+      }
+      const float w = expf(v.x - ref);
       den = fmaf(w, fabsf(v.y), den);
       left_out |= v.y < 0.f;
       ml[s * 32 + tid].x = w;
@@ -1123,13 +1127,13 @@ __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams 
       float w[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        w[u] = s0 + u < slots ? ml[(s0 + u) * 32 + r].x : 0.f;
-        if (w[u] != 0.f)  // an empty range leaves its sums unwritten
+        w[u] = s0 + u < slots ? ml[(s0 + u) * 32 + r].x : -1.f;
+        if (!(w[u] < 0.f))  // an empty range leaves its sums unwritten
           f[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + part(s0 + u, r).o + q * 128));
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (w[u] != 0.f) {
+        if (!(w[u] < 0.f)) {  // (a weight of 0 takes a NaN or an infinity among the sums along)
           num[0] = fmaf(w[u], f[u].x, num[0]);
           num[1] = fmaf(w[u], f[u].y, num[1]);
           num[2] = fmaf(w[u], f[u].z, num[2]);

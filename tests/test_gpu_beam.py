@@ -435,6 +435,36 @@ def test_attention_nan_beside_a_range_of_far_higher_scores(lib, hd, own):
         assert bool(ops.shared_prefix_attention(q, *caches, hq, hkv).isnan().all()), j
 
 
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype,hq,hkv,hd,g,w,t", ODD_SIZES)
+def test_attention_odd_values_of_keys_that_weigh_nothing(lib, dtype, hq, hkv, hd, g, w, t, odd):
+    """A NaN or an infinity among the V that a row sees reaches it from keys whose weight is below fp32's range too."""
+    from minitp_b200 import ops
+
+    r = _gen(hd + t)
+    n, long = g * w, 26000 if t > 1 else 3000
+    u = torch.randn(hd, generator=r)
+    u /= u.norm()
+    q = (u * 20 + 0.1 * torch.randn(n, t, hq, hd, generator=r)).view(n, t, hq * hd)
+    kp, vp = (torch.randn(g, hkv, long, hd, generator=r) for _ in range(2))
+    kc, vc = (torch.randn(n, hkv, 900 + t, hd, generator=r) for _ in range(2))
+    high = u * 30 * math.sqrt(hd)  # scores of about 600; the others' are below 200
+    kp[:, :, long - 9] += high
+    kc[:, :, 899] += high  # (every token sees it)
+    dev = [x.to(DT[dtype]).cuda() for x in (q, kp, vp, kc, vc)]
+    for own, j in ((False, 2), (False, 133), (False, long // 2), (True, 1), (True, 17), (True, 40), (True, 700)):
+        q_, kp_, vp_, kc_, vc_ = dev
+        bad = (vc_ if own else vp_).clone()
+        bad[0, hkv - 1, j, 5] = odd
+        args = (q_, kp_, vp_, long, kc_, bad, 900 + t - 1) if own else (q_, kp_, bad, long, kc_, vc_, 900 + t - 1)
+        got = ops.shared_prefix_attention(*args, hq, hkv).view(n, t, hq, hd)
+        reached = torch.zeros(n, t, hq, hd, dtype=torch.bool)
+        reached[: 1 if own else w, :, (hkv - 1) * (hq // hkv):, 5] = True
+        assert torch.equal(~torch.isfinite(got.float().cpu()), reached), (own, j)
+        if odd != odd:
+            assert bool(got.cpu()[reached].isnan().all())
+
+
 def test_attention_lengths_are_clamped_and_may_be_ints(lib):
     from minitp_b200 import ops
 
