@@ -247,7 +247,7 @@ int mtpb_argmax(void* comm, const void* logits, int M, int V_local, int64_t ld, 
  *   - A beam whose score is -inf or NaN, or without a logit above -inf, has
  *     no candidate; a total below fp32's range is none. Places without a
  *     candidate get score -inf, parent 0 and token eos (0 without one).
- * V below 2^30. The outputs may not overlap the inputs. `block`: workspace of
+ * V below 2^30, G * W (rows) at most 65535. The outputs may not overlap the inputs. `block`: workspace of
  * mtpb_beam_block_bytes(G*W, V, k) bytes, 16-byte aligned, private to the call
  * until it has run. */
 long long mtpb_beam_block_bytes(int rows, int V_plan, int k);
@@ -276,7 +276,7 @@ int mtpb_beam_pick(const void* blocks, int parts, int G, int W, int V_plan, int 
  * row src = g*W + parents[g][w], with n = lens[src] (device int32 [G*W];
  * clamped to [0, cap]) or `len` when lens is NULL. Positions from n on are
  * left as they were, and so is a row whose parent is itself or outside
- * [0, W). 1 <= W <= 64; hd * sizeof(dtype) a multiple of 16; k_caches and
+ * [0, W). 1 <= W <= 64; G * hkv at most 65535; hd * sizeof(dtype) a multiple of 16; k_caches and
  * v_caches: host arrays of n_layers device pointers, to caches that do not
  * overlap. */
 int mtpb_kv_reorder(void* const* k_caches, void* const* v_caches, int n_layers,

@@ -75,8 +75,10 @@ size_t beam_block(long long rows, const BeamPlan& b, int k) {
   return (beam_cand_bytes(rows, b, k) + size_t(rows) * b.nchunk * sizeof(BeamStat) + 15) / 16 * 16;
 }
 
+constexpr int kBeamMaxRows = 65535;  // a grid axis
+
 int beam_check(long long rows, long long V, int k) {
-  if (rows < 1 || rows > (1 << 20)) return bad("beam selection: need 1 .. 2^20 rows");
+  if (rows < 1 || rows > kBeamMaxRows) return bad("beam selection: need 1 .. 65535 rows");
   if (V < 1 || V >= 1ll << 30) return bad("beam selection: empty vocabulary, or one of 2^30 or more");
   if (k < 1 || k > kBeamMaxK) return bad("beam selection: k must be in [1, 64]");
   return MTPB_OK;
@@ -131,8 +133,8 @@ int beam_pick(const void* blocks, int parts, int G, int W, int V_plan, int kc, c
 
 int pick_check(int G, int W, const float* scores, const uint8_t* finished, long long eos, const float* out_scores,
                const int64_t* out_parents, const int64_t* out_tokens) {
-  if (G < 1 || W < 1 || W > kBeamMaxW || (long long)G * W > (1 << 20))
-    return bad("beam selection: need 1 .. 64 beams and at most 2^20 rows");
+  if (G < 1 || W < 1 || W > kBeamMaxW || (long long)G * W > kBeamMaxRows)
+    return bad("beam selection: need 1 .. 64 beams and at most 65535 rows");
   if (!scores || !out_scores || !out_parents || !out_tokens) return bad("beam selection: null tensor");
   if (finished && eos < 0) return bad("beam selection: finished beams need an end token");
   if (eos > 0xFFFFFFFFll) return bad("beam selection: end token out of range");
@@ -155,7 +157,6 @@ int mtpb_beam_candidates(const void* logits, int64_t ld, int rows, int V_local, 
   if (r != MTPB_OK) return r;
   if ((!logits && V_local > 0) || !block) return bad("beam_candidates: null tensor");
   if (!dtype_ok(dtype)) return bad("unsupported dtype");
-  if (rows > 65535) return bad("beam_candidates: more than 65535 rows");
   if (V_local < 0 || V_local > V_plan || ld < V_local) return bad("beam_candidates: need 0 <= V_local <= V_plan, ld");
   if (vstart < 0 || vstart > 0xFFFFFFFFll - V_local) return bad("beam_candidates: vocabulary ids out of range");
   if (!al16(block)) return bad("beam_candidates: block must be 16-byte aligned");

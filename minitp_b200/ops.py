@@ -251,7 +251,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: to
 
     Returns ``(scores, parents, tokens, finished)``, each ``[G, k]``, best
     first (``finished`` is None without ``eos_token_id``). Places without a
-    candidate hold score -inf, parent 0 and the end token (or 0).
+    candidate hold score -inf, parent 0 and the end token (or 0). At most 65535
+    beams in all (G * W), 64 of a prompt, and 64 candidates.
     """
     dev, logits, ld = _beam_inputs("beam_select", logits, scores, k, finished, eos_token_id)
     g, w, v = logits.shape
@@ -334,7 +335,7 @@ def reorder_cache_(k_caches, v_caches, parents: torch.Tensor, lengths) -> None:
     ``parents`` int64 ``[G, W]``. The first ``lengths`` positions of the source
     row are copied (an int, or int32 ``[G * W]`` by source row); later ones stay
     as they were. A parent outside [0, W) leaves its row alone. No two caches may
-    share memory.
+    share memory. W is at most 64, G * hkv at most 65535.
     """
     name = "reorder_cache_"
     if parents.dim() != 2 or parents.dtype != torch.int64 or not parents.is_contiguous():

@@ -42,6 +42,17 @@ def test_candidates_and_pick_refusals(lib):
         _refused(lib, "mtpb_beam_pick", list((ok | change).values()), match)
 
 
+def test_one_limit_of_rows(lib):
+    """A block can be sized for just the rows that the selection and its halves take."""
+    assert lib.mtpb_beam_block_bytes(65535, 1000, 4) > 0
+    for rows in (65536, 1 << 20, (1 << 20) + 1):
+        assert lib.mtpb_beam_block_bytes(rows, 1000, 4) == _lib.ERR_INVALID
+        assert "65535" in lib.mtpb_last_error().decode()
+    _refused(lib, "mtpb_beam_candidates", (P, 50, 65536, 50, 0, 60, 4, None, P, _lib.MTPB_BF16, None), "65535")
+    _refused(lib, "mtpb_beam_pick", (P, 2, 1024, 64, 60, 4, P, None, -1, 4, P, P, P, None, None), "65535")
+    _refused(lib, "mtpb_beam_select", (P, 100, 1024, 64, 100, P, None, -1, 4, P, P, P, None, P, _lib.MTPB_F32, None), "65535")
+
+
 def test_reorder_refusals(lib):
     arr = (ctypes.c_void_p * 2)(P, P)
     odd = (ctypes.c_void_p * 2)(P, P + 8)
