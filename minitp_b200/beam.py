@@ -19,15 +19,19 @@ from __future__ import annotations
 import torch
 
 from minitp_b200 import _lib
-from minitp_b200.generation import _MAX_SESSIONS, make_kv_cache, select_token
+from minitp_b200.generation import make_kv_cache, select_token
 from minitp_b200.layer import TPQwen2ForCausalLM
+
+
+_MAX_SHARED_SESSIONS = 4
 
 
 class _SharedSession:
     """Buffers of one shape behind a shared prefix, and the CUDA graph of its step.
 
-    Kept on the model between calls, with the decode sessions, and dropped with
-    the native model. ``slot`` and ``rope`` are the new token's place in the own
+    Kept on the model between calls, apart from the greedy decode sessions (these
+    keep their places whatever shapes are searched), and dropped with the native
+    model. ``slot`` and ``rope`` are the new token's place in the own
     cache and its position; ``lens`` the own cache's length after it, per row.
     """
 
@@ -86,15 +90,15 @@ class _SharedSession:
 
 
 def _session(model: TPQwen2ForCausalLM, kind: tuple, *shape) -> _SharedSession:
-    """The model's session of this kind and shape (with the decode sessions: at most four are kept)."""
+    """The model's session of this kind and shape (created on first use; at most four kept)."""
     native = model.native()  # first: (re)building the native model drops the model's sessions
-    cache = model.__dict__.setdefault("_decode_sessions", {})
+    cache = model.__dict__.setdefault("_shared_sessions", {})
     key = (*kind, *(str(x) for x in shape))
     s = cache.pop(key, None)
     if s is None or s.native != native:
         s = _SharedSession(model, native, *shape)
     cache[key] = s
-    while len(cache) > _MAX_SESSIONS:
+    while len(cache) > _MAX_SHARED_SESSIONS:
         cache.pop(next(iter(cache)))
     return s
 

@@ -245,6 +245,33 @@ def test_graphs_kept_over_a_larger_prompt(lib):
     assert gpu.ctx.comm().status() == 0
 
 
+def test_greedy_sessions_stay_over_other_searches(lib):
+    """Beam and shared-prefix shapes take no place of a greedy session: its buffers and graph are there for the next
+    call, and all of them go with the native model."""
+    from minitp_b200.beam import generate_beam, generate_shared_prefix
+    from minitp_b200.generation import decode_session, generate_greedy
+
+    gpu, _, cfg = _models()
+    ids = _prompt(cfg, 2, 5, 1).cuda()
+    want = generate_greedy(gpu, ids, 6, early_stop=False)
+    kept = decode_session(gpu, 2, 11, ids.device)
+    graph = kept.graph
+    for w in range(1, 5):
+        generate_beam(gpu, ids, 3, w)
+        generate_beam(gpu, ids, 3, w, eos_token_id=w)
+        generate_shared_prefix(gpu, ids[:1], ids[:, :w], 3)
+    again = decode_session(gpu, 2, 11, ids.device)
+    assert again is kept and again.graph is graph
+    assert torch.equal(generate_greedy(gpu, ids, 6, early_stop=False), want)
+    beams = generate_beam(gpu, ids, 3, 2)
+    for n in range(1, 6):  # nor the other way round
+        generate_greedy(gpu, ids, n, early_stop=False)
+    assert all(torch.equal(a, b) for a, b in zip(generate_beam(gpu, ids, 3, 2), beams))
+    gpu.release_native()
+    assert not any(k.endswith("_sessions") for k in vars(gpu))
+    assert torch.equal(generate_greedy(gpu, ids, 6, early_stop=False), want)
+
+
 def test_bf16_logits_behind_a_prefix(lib):
     """bf16, the 0.5B shape with two layers: rows behind a shared prefix against the whole prompts, many tokens and
     one at a time, within the framework's bf16 logit tolerance (0.5 absolute)."""
