@@ -207,6 +207,42 @@ def w_two_shot(rank, world, name):
     return res
 
 
+def beam_cfg():
+    """The tiny model with a vocabulary that no number of ranks divides."""
+    import dataclasses
+
+    from minitp_b200 import config as mcfg
+
+    return dataclasses.replace(mcfg.baseline_tiny(), vocab_size=997)
+
+
+BEAM_EOS = 589
+
+
+def beam_prompts():
+    r = torch.Generator().manual_seed(31)
+    return {k: torch.randint(0, 997, s, generator=r) for k, s in
+            (("ids", (2, 6)), ("prefix", (1, 17)), ("rows", (4, 3)))}
+
+
+def w_beam(rank, world):
+    """Beam search with and without an end token, and rows behind a shared prefix, on the ranks of a TP group."""
+    from minitp_b200.beam import generate_beam, generate_shared_prefix
+    from minitp_b200.weight_loader import load_synthetic_tp
+
+    ctx = ctx_for(rank, world)
+    model = load_synthetic_tp(beam_cfg(), ctx, dtype=torch.float32, device=ctx.device)
+    p = {k: v.cuda() for k, v in beam_prompts().items()}
+    res = {}
+    for name, eos in (("free", None), ("eos", BEAM_EOS)):
+        ids, scores = generate_beam(model, p["ids"], 6, 4, eos_token_id=eos, num_return=4, early_stop=False)
+        res[f"{name}_ids"], res[f"{name}_scores"] = ids.cpu().numpy(), scores.cpu().numpy()
+    res["shared"] = generate_shared_prefix(model, p["prefix"], p["rows"], 5).cpu().numpy()
+    torch.cuda.synchronize()
+    ctx.comm().raise_on_error()
+    return res
+
+
 def w_peer_timeout(rank, world):
     """Rank 1 skips one collective: rank 0's bounded wait must expire and report it.
 

@@ -85,6 +85,65 @@ def test_attention_refusals(lib):
     assert lib.mtpb_shared_attention_workspace(2, 4, 1, 14, 3, 64, 8, 8, 1) < 0
 
 
+def _cpu_candidates(local_logits, k, vstart, v_plan, finished=None):
+    """A stand-in for a shard's block: its best values with their ids and its sum of exponentials, as bytes."""
+    g, w, v = local_logits.shape
+    assert v <= v_plan
+    x = torch.full((g, w, v_plan), -torch.inf, dtype=torch.float64)
+    x[:, :, :v] = local_logits.double()
+    val, at = torch.cat([x, torch.full((g, w, k), -torch.inf, dtype=torch.float64)], -1).sort(dim=-1, descending=True, stable=True)
+    lse = torch.logsumexp(x, -1, keepdim=True)
+    return torch.cat([val[..., :k], (at[..., :k] + vstart).double(), lse], -1).reshape(-1).view(torch.uint8)
+
+
+def _cpu_pick(blocks, scores, k, v_plan, finished=None, eos_token_id=None):
+    g, w = scores.shape
+    rows = blocks.contiguous().view(torch.float64).view(blocks.shape[0], g, w, 2 * k + 1)
+    lse = torch.logsumexp(rows[..., -1], 0)
+    total = rows[..., :k] - lse[..., None] + scores.double()[..., None]
+    best = []
+    for i in range(g):
+        cand = [(-float(total[r, i, b, j]), b, int(rows[r, i, b, k + j])) for r in range(blocks.shape[0]) for b in range(w)
+                for j in range(k) if float(total[r, i, b, j]) > -torch.inf]
+        best.append(sorted(cand)[:k])
+    return [[(round(-s, 9), b, t) for s, b, t in row] for row in best]
+
+
+def _w_beam_select(rank, world, v):
+    import torch.distributed as dist
+
+    from minitp_b200.distributed.context import ParallelContext
+    from minitp_b200.parallel import embedding
+
+    embedding.ops.beam_candidates, embedding.ops.beam_pick = _cpu_candidates, _cpu_pick
+    head = embedding.VocabParallelLMHead(8, v, ParallelContext(rank, rank, world, rank, world, torch.device("cpu"), dist.group.WORLD))
+    x, s = _beam_case(v)
+    return head.beam_select(x[:, :, head.vocab_start:head.vocab_end], s, 4)
+
+
+def _beam_case(v):
+    r = torch.Generator().manual_seed(v)
+    return torch.randn(2, 3, v, generator=r), torch.randn(2, 3, generator=r)
+
+
+@pytest.mark.distributed
+@pytest.mark.parametrize("world,v", [(2, 101), (3, 10), (3, 2)])
+def test_selection_exchanges_the_shards_of_all_ranks(world, v):
+    """`VocabParallelLMHead.beam_select` over Gloo ranks (the kernels played by the stand-ins above): every rank gets
+    the whole vocabulary's candidates, of uneven and empty shards too."""
+    from tests.tp_harness import run_tp
+
+    res = run_tp(world, _w_beam_select, v)
+    x, s = _beam_case(v)
+    total = (s.double()[..., None] + torch.log_softmax(x.double(), -1)).view(2, -1)
+    val, at = total.sort(dim=-1, descending=True, stable=True)
+    n = min(4, 3 * v)
+    want = [[(round(float(a), 9), int(b) // v, int(b) % v) for a, b in zip(val[i, :n], at[i, :n])] for i in range(2)]
+    for r in range(world):
+        assert [[c[1:] for c in row] for row in res[r]] == [[c[1:] for c in row] for row in want]
+        assert [c[0] for row in res[r] for c in row] == pytest.approx([c[0] for row in want for c in row], abs=1e-8)
+
+
 def test_cpu_tensors_are_refused(lib):
     with pytest.raises(_lib.MinitpB200Error, match="CUDA"):
         ops.beam_select(torch.zeros(1, 2, 10), torch.zeros(1, 2), 2)

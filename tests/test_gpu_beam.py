@@ -176,6 +176,46 @@ def test_select_from_vocabulary_shards(lib, dtype, parts, v):
     beam_ref.check_select(got, x, s, k, fin, eos)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("tp,v", [(2, 1001), (3, 4099), (8, 11)])
+def test_select_by_the_ranks_of_a_vocabulary(lib, monkeypatch, dtype, tp, v):
+    """`VocabParallelLMHead.beam_select` of every rank, one after the other with the exchange played by the test: the
+    same places on all of them, those of the whole vocabulary."""
+    from minitp_b200 import ops
+    from minitp_b200.distributed.context import ParallelContext
+    from minitp_b200.parallel import embedding
+
+    r = _gen(v + tp)
+    g, w, k, eos = 3, 4, 4, v - 1
+    x = (torch.randn(g, w, v, generator=r) * 2).to(DT[dtype]).cuda()
+    s = torch.randn(g, w, generator=r).cuda()
+    fin = (torch.rand(g, w, generator=r) < 0.3).cuda()
+    heads = [embedding.VocabParallelLMHead(8, v, ParallelContext(i, i, tp, i, tp, torch.device("cuda"), None)) for i in range(tp)]
+    shards = [x[:, :, h.vocab_start:h.vocab_end].contiguous() for h in heads]
+    sent: dict = {}
+
+    class Sent(Exception):
+        pass
+
+    def send(out, mine, group):
+        assert out.shape == (tp, mine.numel()) and out.dtype == mine.dtype
+        sent[len(sent)] = mine
+        raise Sent
+
+    monkeypatch.setattr(embedding, "all_gather_dim0", send)
+    for h, part in zip(heads, shards):
+        with pytest.raises(Sent):
+            h.beam_select(part, s, k, fin, eos)
+    assert len({b.numel() for b in sent.values()}) == 1
+    monkeypatch.setattr(embedding, "all_gather_dim0", lambda out, mine, group: out.copy_(torch.stack(list(sent.values()))))
+    got = [h.beam_select(part, s, k, fin, eos) for h, part in zip(heads, shards)]
+    whole = ops.beam_select(x, s, k, fin, eos)
+    for o in got:
+        assert all(torch.equal(a, b) for a, b in zip(o, got[0]))
+        assert all(torch.equal(a, b) for a, b in zip(o[1:], whole[1:]))  # (scores: chunks are cut elsewhere)
+    beam_ref.check_select(got[0], x, s, k, fin, eos)
+
+
 def test_select_streams_and_graph(lib):
     """Two calls at once on two streams, and a captured call replayed on new inputs."""
     from minitp_b200 import ops

@@ -107,6 +107,26 @@ def test_tp2_fp32_tokens_two_shot_sites():
         assert np.array_equal(res[r]["tokens"], g["tokens"]), r
 
 
+def test_tp2_beam_search_and_shared_prefixes():
+    """Beam search and decoding behind a shared prefix at TP=2 (candidates exchanged, uneven vocabulary, no graph):
+    equal on both ranks, and the plain CPU runs' tokens and scores."""
+    from oracle.model import OracleConfig, OracleModel, checkpoint_tensors
+    from tests.test_gpu_beam_model import _plain_beam
+
+    res = mp_worker.run(2, mp_worker.w_beam)
+    for k in res[0]:
+        assert np.array_equal(res[0][k], res[1][k]), k
+    cfg, p = mp_worker.beam_cfg(), mp_worker.beam_prompts()
+    oracle = OracleModel(OracleConfig.of(cfg), checkpoint_tensors(cfg), tp=1)
+    for name, eos in (("free", -1), ("eos", mp_worker.BEAM_EOS)):
+        want = _plain_beam(oracle, p["ids"], 6, 4, eos)
+        for i in range(2):
+            assert res[0][f"{name}_ids"][i].tolist() == [h[1] for h in want[i]]
+            assert res[0][f"{name}_scores"][i].tolist() == pytest.approx([h[0] for h in want[i]], abs=2e-3)
+    whole = torch.cat([p["prefix"].repeat_interleave(4, 0), p["rows"]], 1)
+    assert np.array_equal(res[0]["shared"], oracle.generate(whole, 5)[:, 17:].numpy())
+
+
 def test_peer_timeout_is_reported():
     res = mp_worker.run(2, mp_worker.w_peer_timeout)
     assert bool(res[0]["ok_before"]) and bool(res[1]["ok_before"])
