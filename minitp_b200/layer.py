@@ -199,6 +199,9 @@ class TPQwen2ForCausalLM(nn.Module):
             if rope_pos.dtype != torch.int64:
                 rope_pos = rope_pos.to(torch.int64)
             rope_pos = rope_pos.contiguous()
+            if rope_pos.numel() < t or rope_pos.device != input_ids.device:
+                raise ValueError(f"positions must be [{t}] on {input_ids.device}, got {tuple(positions.shape)} on "
+                                 f"{positions.device}")
         elif t > 1 and kv.seq_len > 0:
             # the reference numbers multi-token inputs from 0 when no positions are given
             rope_pos = torch.arange(t, device=input_ids.device)

@@ -195,6 +195,24 @@ def test_forward_refuses_caches_that_do_not_fit(lib):
         generate_shared_prefix(gpu, ids[:2], ids, 4)
 
 
+def test_positions_that_do_not_cover_the_tokens_are_refused(lib):
+    from minitp_b200.generation import make_kv_cache
+
+    gpu, _, cfg = _models()
+    ids = _prompt(cfg, 2, 3, 1).cuda()
+    prefix, own = make_kv_cache(gpu, 2, 8), make_kv_cache(gpu, 2, 8)
+    gpu(ids, kv_cache=prefix)
+    for bad in (torch.arange(2).cuda(), torch.arange(0).cuda(), torch.arange(3)):
+        with pytest.raises(ValueError, match="positions"):
+            gpu(ids, positions=bad, kv_cache=own, prefix_cache=prefix)
+        with pytest.raises(ValueError, match="positions"):
+            gpu(ids, positions=bad, kv_cache=own)
+    assert own.seq_len == 0
+    a = gpu(ids, positions=torch.arange(3, 6).cuda(), kv_cache=own, prefix_cache=prefix)
+    own.seq_len = 0
+    assert torch.equal(a, gpu(ids, kv_cache=own, prefix_cache=prefix))
+
+
 def test_a_cache_behind_itself_is_refused(lib):
     from minitp_b200.generation import make_kv_cache
 
