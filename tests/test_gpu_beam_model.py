@@ -171,6 +171,29 @@ def test_forward_behind_a_prefix_poisoned_caches(lib):
     assert own.seq_len == 11
 
 
+def test_forward_behind_a_prefix_in_chunks(lib):
+    """More (row, token) pairs than one collective message holds go in chunks of tokens: the logits of each row are
+    those of a call of a few rows."""
+    from minitp_b200.generation import make_kv_cache
+
+    gpu, _, cfg = _models()
+    groups, n, t = 4, 512, 100  # 512 * 100 * 64 fp32 values, more than 8 MB
+    pre, ids = _prompt(cfg, groups, 70, 1).cuda(), _prompt(cfg, n, t, 2).cuda()
+    prefix, own = make_kv_cache(gpu, groups, 70), make_kv_cache(gpu, n, t + 1)
+    own.poison()
+    gpu(pre, kv_cache=prefix)
+    got = gpu(ids, kv_cache=own, prefix_cache=prefix)
+    nxt = gpu(ids[:, :1], kv_cache=own, prefix_cache=prefix)
+    for g, rows in ((0, slice(0, 3)), (1, slice(250, 256)), (3, slice(509, 512))):
+        one, mine = make_kv_cache(gpu, 1, 70), make_kv_cache(gpu, rows.stop - rows.start, t + 1)
+        gpu(pre[g:g + 1], kv_cache=one)
+        want = gpu(ids[rows], kv_cache=mine, prefix_cache=one)
+        assert float((got[rows] - want).abs().max() / want.abs().max()) <= 1e-4  # the framework's fp32 logit tolerance
+        want = gpu(ids[rows, :1], kv_cache=mine, prefix_cache=one)
+        assert float((nxt[rows] - want).abs().max() / want.abs().max()) <= 1e-4
+    assert gpu.ctx.comm().status() == 0
+
+
 def test_forward_refuses_caches_that_do_not_fit(lib):
     from minitp_b200.beam import generate_beam, generate_shared_prefix
     from minitp_b200.generation import make_kv_cache
