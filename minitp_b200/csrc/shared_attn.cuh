@@ -605,13 +605,14 @@ __global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const S
     const float ref = mx == -INFINITY ? 0.f : mx;
     float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
     auto add = [&](float m, float l, const float4& f) {
-      if (m == -INFINITY) return;  // an empty range leaves its sums unwritten
-      const float w = expf(m - ref);  // (0 takes a NaN or an infinity among the sums along)
+      const float w = m == -INFINITY ? 0.f : expf(m - ref);
       den = fmaf(w, l, den);
-      num[0] = fmaf(w, f.x, num[0]);
-      num[1] = fmaf(w, f.y, num[1]);
-      num[2] = fmaf(w, f.z, num[2]);
-      num[3] = fmaf(w, f.w, num[3]);
+      if (m != -INFINITY) {  // an empty range leaves its sums unwritten; one of weight 0 may hold a NaN
+        num[0] = fmaf(w, f.x, num[0]);
+        num[1] = fmaf(w, f.y, num[1]);
+        num[2] = fmaf(w, f.z, num[2]);
+        num[3] = fmaf(w, f.w, num[3]);
+      }
     };
 #pragma unroll
     for (int w = 0; w < NW; ++w)
