@@ -235,8 +235,8 @@ int mtpb_argmax(void* comm, const void* logits, int M, int V_local, int64_t ld, 
  * [G*W, V] (row stride ld) and running scores fp32 [G][W], the k best
  * (1 <= k <= 64) of all (beam b, token v) of a prompt by
  *   total(b, v) = score[b] + log_softmax(logits[b])[v],
- * best first, equal totals by the lower b * V + v. Sums over the vocabulary
- * are fp32 per chunk; totals are formed and compared in fp64. Outputs [G][k]:
+ * best first, equal totals by the lower b * V + v. Logits may be of any size
+ * (banned tokens at -1e9, say). Sums over the vocabulary are fp32 per chunk; totals are formed and compared in fp64. Outputs [G][k]:
  * scores fp32 (the rounded totals), parents (b) and tokens (v) int64, and
  * finished flags (may be NULL).
  *   - A NaN logit counts as -inf: that token is never picked. +inf logits

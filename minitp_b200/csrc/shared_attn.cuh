@@ -14,7 +14,8 @@
 // NaN and infinities go where the formula takes them and nowhere else: a score
 // that is NaN or +inf makes its row NaN (a sum that is NaN is handed on with a
 // NaN max, which no join passes over), and a NaN among V makes its dim NaN,
-// whatever the weight; positions that a token does not see reach it neither
+// whatever the weight (but for a key range whose scores are all -inf, which
+// counts as not seen); positions that a token does not see reach it neither
 // through K (its scores are selected away) nor through V (0 times NaN would be
 // NaN: such terms are left out or zeroed).
 #pragma once
@@ -666,11 +667,14 @@ __global__ void __launch_bounds__(32 * kSaTokenWarps, 2) sa_token_kernel(const S
 // (Added here they cost the softmax registers: 66 -> 76 us on 16 rows of 128
 // tokens behind 4001.)
 //
-// Bound by the chain S -> softmax -> P V of a stream, of which two run against
-// each other: about 3580 cycles a pair of key tiles for head dim 128 and 3010
-// for 64, of which the special-function unit has 1430. 64 rows of the 7B heads
-// behind 16384 positions: 28 us, 0.54 PFLOP/s; 16 rows of 128 tokens of the
-// 0.5B heads behind 4001 and 150: 57 us, 0.52 PFLOP/s, on 112 of 148 SMs.
+// A key tile is bound by the chain S -> softmax -> P V of a stream, of which two
+// run against each other: about 3580 cycles a pair of key tiles for head dim 128
+// and 3010 for 64, of which the special-function unit has 1430. An item's start
+// (barriers, tensor memory, Q, the first tiles) and end (the partial sums) come
+// on top, 8 us where a call's items have one tile instead of none. 64 rows of the
+// 7B heads behind 16384 positions: 28 us, 0.54 PFLOP/s, of which the 8 tiles of a
+// range are 15, on 128 of 148 SMs; 16 rows of 128 tokens of the 0.5B heads behind
+// 4001 and 150: 57 us, 0.52 PFLOP/s, of which the 32 tiles are 51, on 112 SMs.
 // ---------------------------------------------------------------------------
 constexpr int kSaTcKeys = 128;
 // Of 16 pairs of exponentials, on the fp32 pipe (0, 2, 4, 6: 46.6, 46.8, 46.5,
@@ -1107,13 +1111,13 @@ __global__ void __launch_bounds__(kSaJoinThreads) sa_join_kernel(const SaParams 
     const float ref = mx == -INFINITY ? 0.f : mx;
     for (int s = 0; s < slots; ++s) {
       const float2 v = ml[s * 32 + tid];
+      left_out |= v.y < 0.f;
       if (v.x == -INFINITY) {
         ml[s * 32 + tid].x = -1.f;
         continue;
       }
       const float w = expf(v.x - ref);
       den = fmaf(w, fabsf(v.y), den);
-      left_out |= v.y < 0.f;
       ml[s * 32 + tid].x = w;
     }
     odd[tid] = left_out ? max(0, sa_cache_len(p, n) - (p.T - 1)) : -1;
