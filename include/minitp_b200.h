@@ -310,6 +310,63 @@ int mtpb_shared_attention(const void* q, const void* k_prefix, const void* v_pre
  * model's forward reports to its communicator's status word instead.) */
 int mtpb_beam_status(uint32_t* status_out /* host */);
 
+/* ---------------------------------------------------------------- scoring of prompts
+ * (no counterpart in the reference) */
+
+/* Causal grouped-query attention over whole prompts packed one behind the
+ * other: prompt s holds the packed tokens [seq_starts[s], seq_starts[s+1])
+ * (device int32 [S+1], non-decreasing, within [0, total]; other values lead to
+ * no access outside the tensors, but their prompts are not defined). Token i
+ * attends to the tokens of its own prompt up to itself. k and v hold all
+ * `total` tokens, q and out the n tokens from `first` on; element (token, head,
+ * dim) of q lies at token * q_token + head * q_head + dim, k and v alike, out is
+ * [n, hq, hd]. Strides are in elements, at least hd and multiples of 16 bytes
+ * (that of an axis of one place too); q, k, v and out are 16-byte aligned. A
+ * token of no prompt, and one whose scores are all -inf, gets 0. scale =
+ * 1/sqrt(hd); hd 16, 32, 64 or 128; total * hq at most 2^30, S at most 2^20.
+ * Softmax statistics and sums are fp32; bf16 probabilities are rounded to bf16
+ * for their product with V. What a token does not see does not reach it, NaN
+ * and infinities included. out may not overlap an input. */
+int mtpb_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                          int64_t k_head, const void* v, int64_t v_token, int64_t v_head, void* out,
+                          const int* seq_starts, int S, int first, int n, int total, int hq, int hkv,
+                          int hd, int dtype, void* stream);
+
+/* Log-probabilities of given tokens, entropy and top alternatives of rows of
+ * logits [rows, V] (row stride ld elements): with log p = log_softmax(row),
+ * logprobs[r] = log p(targets[r]) (targets device int64 [rows]; NaN for an id
+ * outside [0, V); targets may be NULL, logprobs then too), entropy[r] =
+ * -sum p log p (natural units), and the k best log p with their ids in
+ * top_logprobs / top_ids [rows, k], best first, equal ones by the lower id
+ * (k 0: both may be NULL). A NaN logit counts as -inf; +inf logits share the
+ * probability. Places without a token above -inf hold -inf and id 0; a row
+ * without any has entropy 0 and log-probability -inf. k in [0, 64], V below
+ * 2^30, at most 2^24 rows. Sums are fp32 within a chunk of a row and fp64
+ * over chunks. `block`: workspace of mtpb_logprobs_block_bytes(rows, V, k)
+ * bytes, 16-byte aligned, private to the call until it has run. */
+long long mtpb_logprobs_block_bytes(int rows, int V_plan, int k);
+int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const int64_t* targets,
+                        int k, float* logprobs, float* entropy, float* top_logprobs,
+                        int64_t* top_ids, void* block, int dtype, void* stream);
+
+/* The two halves of mtpb_token_logprobs for a vocabulary in shards.
+ * mtpb_logprobs_block reduces one shard (columns [vstart, vstart + V_local) of
+ * the vocabulary) of every row to a block of mtpb_logprobs_block_bytes(rows,
+ * V_plan, k) bytes; V_plan, the same on every shard, is at least the largest
+ * V_local. mtpb_logprobs_join joins `parts` such blocks, one after another in
+ * memory in any shard order, all made with the same rows, V_plan and k_block,
+ * into the outputs of mtpb_token_logprobs; k at most k_block. A target that no
+ * shard holds gets NaN. */
+int mtpb_logprobs_block(const void* logits, int64_t ld, int rows, int V_local, int64_t vstart,
+                        int V_plan, const int64_t* targets, int k, void* block, int dtype,
+                        void* stream);
+int mtpb_logprobs_join(const void* blocks, int parts, int rows, int V_plan, int k_block,
+                       const int64_t* targets, int k, float* logprobs, float* entropy,
+                       float* top_logprobs, int64_t* top_ids, void* stream);
+
+/* As mtpb_beam_status, of the prompt attentions and log-probabilities. */
+int mtpb_scoring_status(uint32_t* status_out /* host */);
+
 /* ---------------------------------------------------------------- model
  * A TP Qwen2 decoder whose weights stay in caller-owned device tensors.
  * ref: minitp/layer.py:68-124 (TPQwen2ForCausalLM), minitp/attention.py,

@@ -24,9 +24,9 @@ LIB_PATH = os.path.join(OUT_DIR, "libminitp_b200.so")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 # translation units, compiled in parallel: the C ABI with the kernel chain, beam
-# search with the shared-prefix attention, and the decode megakernel's bf16 and
-# fp32 instantiations
-SOURCES = [os.path.join(CSRC, f) for f in ("capi.cu", "capi_beam.cu", "decode_mk_bf16.cu", "decode_mk_f32.cu")]
+# search with the shared-prefix attention, prompt scoring, and the decode
+# megakernel's bf16 and fp32 instantiations
+SOURCES = [os.path.join(CSRC, f) for f in ("capi.cu", "capi_beam.cu", "capi_scoring.cu", "decode_mk_bf16.cu", "decode_mk_f32.cu")]
 OBJ_DIR = os.path.join(REPO, "_build")
 
 

@@ -1,0 +1,251 @@
+// C ABI of packed prompt attention and token log-probabilities (declared in
+// include/minitp_b200.h): host checks, launch plans and workspaces.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "host_util.cuh"
+#include "logprobs.cuh"
+#include "prompt_attn.cuh"
+
+using namespace mtpb;
+
+namespace {
+
+int bad(const char* msg) { return host_fail(MTPB_ERR_INVALID, msg); }
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool dtype_ok(int dtype) { return dtype == MTPB_BF16 || dtype == MTPB_F32; }
+
+// ------------------------------------------------------------------ log-probabilities
+constexpr long long kLpMaxRows = 1ll << 24;
+
+// Chunks of a row: a function of the sizes alone, so that every rank cuts its
+// shard alike.
+struct LpPlan {
+  int nchunk, chunk;
+};
+
+LpPlan lp_plan(long long rows, int V) {
+  LpPlan b;
+  const long long want = std::max<long long>(1, std::min<long long>(32, 2 * 148 / rows));
+  b.nchunk = int(std::min<long long>(want, (V + 8191) / 8192));
+  b.chunk = (V + b.nchunk - 1) / b.nchunk;
+  b.chunk = (b.chunk + 7) / 8 * 8;
+  b.nchunk = (V + b.chunk - 1) / b.chunk;
+  return b;
+}
+
+size_t lp_stat_bytes(long long rows, const LpPlan& b) { return size_t(rows) * b.nchunk * sizeof(LpStat); }
+size_t lp_block(long long rows, const LpPlan& b, int k) {
+  return (lp_stat_bytes(rows, b) + size_t(rows) * b.nchunk * k * 8 + 15) / 16 * 16;
+}
+
+int lp_check(long long rows, long long V, int k) {
+  if (rows < 1 || rows > kLpMaxRows) return bad("token_logprobs: need 1 .. 2^24 rows");
+  if (V < 1 || V >= 1ll << 30) return bad("token_logprobs: empty vocabulary, or one of 2^30 or more");
+  if (k < 0 || k > kLpMaxK) return bad("token_logprobs: the alternatives must be in [0, 64]");
+  return MTPB_OK;
+}
+
+int lp_join(const void* blocks, int parts, int rows, int V_plan, int kc, const int64_t* targets, int k,
+            float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, cudaStream_t st) {
+  const LpPlan b = lp_plan(rows, V_plan);
+  const size_t block = lp_block(rows, b, kc);
+  LpJoinParams p;
+  p.stat = static_cast<const LpStat*>(blocks);
+  p.cand = reinterpret_cast<const uint64_t*>(static_cast<const char*>(blocks) + lp_stat_bytes(rows, b));
+  p.stat_part = block / sizeof(LpStat);
+  p.cand_part = block / 8;
+  p.parts = parts;
+  p.rows = rows;
+  p.nchunk = b.nchunk;
+  p.k = k;
+  p.kc = kc;
+  p.targets = reinterpret_cast<const long long*>(targets);
+  p.logprobs = logprobs;
+  p.entropy = entropy;
+  p.top_logprobs = top_logprobs;
+  p.top_ids = reinterpret_cast<long long*>(top_ids);
+  return host_launch(lp_join_kernel, dim3((rows + kLpJoinWarps - 1) / kLpJoinWarps), dim3(32 * kLpJoinWarps),
+                     size_t(k ? kLpJoinWarps : 0) * parts * b.nchunk, st, p);
+}
+
+int join_check(const int64_t* targets, int k, const float* logprobs, const float* entropy, const float* top_logprobs,
+               const int64_t* top_ids) {
+  if (!entropy || (targets && !logprobs) || (k > 0 && (!top_logprobs || !top_ids)))
+    return bad("token_logprobs: null tensor");
+  return MTPB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+long long mtpb_logprobs_block_bytes(int rows, int V_plan, int k) {
+  const int r = lp_check(rows, V_plan, k);
+  if (r != MTPB_OK) return r;
+  return (long long)lp_block(rows, lp_plan(rows, V_plan), k);
+}
+
+int mtpb_logprobs_block(const void* logits, int64_t ld, int rows, int V_local, int64_t vstart, int V_plan,
+                        const int64_t* targets, int k, void* block, int dtype, void* stream) {
+  const int r = lp_check(rows, V_plan, k);
+  if (r != MTPB_OK) return r;
+  if ((!logits && V_local > 0) || !block) return bad("token_logprobs: null tensor");
+  if (!dtype_ok(dtype)) return bad("unsupported dtype");
+  if (V_local < 0 || V_local > V_plan || ld < V_local)
+    return bad("token_logprobs: need 0 <= V_local <= V_plan, ld");
+  if (vstart < 0 || vstart > 0xFFFFFFFFll - V_local) return bad("token_logprobs: vocabulary ids out of range");
+  if (!al16(block)) return bad("token_logprobs: block must be 16-byte aligned");
+  const LpPlan b = lp_plan(rows, V_plan);
+  LpRowsParams p;
+  p.logits = logits;
+  p.ld = ld;
+  p.V = V_local;
+  p.k = k;
+  p.vstart = vstart;
+  p.nchunk = b.nchunk;
+  p.chunk = b.chunk;
+  p.targets = reinterpret_cast<const long long*>(targets);
+  p.stat = static_cast<LpStat*>(block);
+  p.cand = reinterpret_cast<uint64_t*>(static_cast<char*>(block) + lp_stat_bytes(rows, b));
+  const dim3 grid(unsigned(rows) * b.nchunk), threads(kLpThreads);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == MTPB_BF16 ? host_launch(lp_rows_kernel<bf16>, grid, threads, 0, st, p)
+                            : host_launch(lp_rows_kernel<float>, grid, threads, 0, st, p);
+}
+
+int mtpb_logprobs_join(const void* blocks, int parts, int rows, int V_plan, int k_block, const int64_t* targets, int k,
+                       float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, void* stream) {
+  int r = lp_check(rows, V_plan, k_block);
+  if (r == MTPB_OK) r = join_check(targets, k, logprobs, entropy, top_logprobs, top_ids);
+  if (r != MTPB_OK) return r;
+  if (!blocks || !al16(blocks)) return bad("token_logprobs: blocks must be 16-byte aligned");
+  if (parts < 1 || parts > 64) return bad("token_logprobs: need 1 .. 64 shards");
+  if (k < 0 || k > k_block) return bad("token_logprobs: more alternatives than the blocks hold");
+  return lp_join(blocks, parts, rows, V_plan, k_block, targets, k, logprobs, entropy, top_logprobs, top_ids,
+                 static_cast<cudaStream_t>(stream));
+}
+
+int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const int64_t* targets, int k, float* logprobs,
+                        float* entropy, float* top_logprobs, int64_t* top_ids, void* block, int dtype, void* stream) {
+  int r = lp_check(rows, V, k);
+  if (r == MTPB_OK) r = join_check(targets, k, logprobs, entropy, top_logprobs, top_ids);
+  if (r == MTPB_OK) r = mtpb_logprobs_block(logits, ld, rows, V, 0, V, targets, k, block, dtype, stream);
+  if (r != MTPB_OK) return r;
+  return lp_join(block, 1, rows, V, k, targets, k, logprobs, entropy, top_logprobs, top_ids,
+                 static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ attention over packed prompts
+namespace {
+
+template <typename T, int HD>
+int pa_launch(PaParams p, cudaStream_t st) {
+  constexpr int RPT = 4, ROWS = 16 * RPT;
+  const long long tiles = (long long)p.n * (p.hq / p.hkv) / ROWS + p.S + 1;
+  if (tiles * p.hkv > 0x7FFFFFFFll) return bad("prompt_attention: too many rows");
+  p.tiles = int(tiles);
+  return host_launch(pa_simt_kernel<T, HD, RPT>, dim3(unsigned(tiles * p.hkv)), dim3(kPaThreads),
+                     pa_simt_smem<HD, RPT>(), st, p);
+}
+
+template <typename T>
+int pa_launch_hd(const PaParams& p, int hd, cudaStream_t st) {
+  switch (hd) {
+    case 16: return pa_launch<T, 16>(p, st);
+    case 32: return pa_launch<T, 32>(p, st);
+    case 64: return pa_launch<T, 64>(p, st);
+    default: return pa_launch<T, 128>(p, st);
+  }
+}
+
+}  // namespace
+
+namespace mtpb {
+
+int prompt_attn_run(const PromptAttnArgs& a, cudaStream_t st) {
+  if (a.n < 0 || a.total < 0 || a.S < 0 || a.hq < 1 || a.hkv < 1) return bad("prompt_attention: negative size");
+  if (a.hq % a.hkv) return bad("prompt_attention: hq must be a multiple of hkv");
+  if (a.hd != 16 && a.hd != 32 && a.hd != 64 && a.hd != 128)
+    return bad("prompt_attention: head_dim must be 16, 32, 64 or 128");
+  if (!dtype_ok(a.dtype)) return bad("unsupported dtype");
+  if (a.first < 0 || (long long)a.first + a.n > a.total)
+    return bad("prompt_attention: the queries' tokens lie outside the packed tokens");
+  if ((long long)a.total * a.hq > 1 << 30) return bad("prompt_attention: more than 2^30 (token, head) rows");
+  if (a.S > 1 << 20) return bad("prompt_attention: more than 2^20 prompts");
+  if (a.n == 0) return MTPB_OK;
+  if (!a.q || !a.k || !a.v || !a.out || !a.seq_starts) return bad("prompt_attention: null tensor");
+  const int es = a.dtype == MTPB_BF16 ? 2 : 4, ve = 16 / es;
+  if (!al16(a.q) || !al16(a.k) || !al16(a.v) || !al16(a.out))
+    return bad("prompt_attention: tensors must be 16-byte aligned");
+  const long long strides[6] = {a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head};
+  for (long long s : strides)
+    if (s < a.hd || s % ve || s >= 1ll << 38)
+      return bad("prompt_attention: strides must be multiples of 16 bytes and no smaller than head_dim");
+  PaParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.q_ts = a.q_token;
+  p.q_hs = a.q_head;
+  p.k_ts = a.k_token;
+  p.k_hs = a.k_head;
+  p.v_ts = a.v_token;
+  p.v_hs = a.v_head;
+  p.out = a.out;
+  p.starts = a.seq_starts;
+  p.S = a.S;
+  p.first = a.first;
+  p.n = a.n;
+  p.total = a.total;
+  p.hq = a.hq;
+  p.hkv = a.hkv;
+  p.scale = 1.0f / std::sqrt(float(a.hd));
+  p.status = a.status;
+  return a.dtype == MTPB_BF16 ? pa_launch_hd<bf16>(p, a.hd, st) : pa_launch_hd<float>(p, a.hd, st);
+}
+
+}  // namespace mtpb
+
+extern "C" int mtpb_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                                     int64_t k_head, const void* v, int64_t v_token, int64_t v_head, void* out,
+                                     const int* seq_starts, int S, int first, int n, int total, int hq, int hkv, int hd,
+                                     int dtype, void* stream) {
+  PromptAttnArgs a;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_token = q_token;
+  a.q_head = q_head;
+  a.k_token = k_token;
+  a.k_head = k_head;
+  a.v_token = v_token;
+  a.v_head = v_head;
+  a.out = out;
+  a.seq_starts = seq_starts;
+  a.S = S;
+  a.first = first;
+  a.n = n;
+  a.total = total;
+  a.hq = hq;
+  a.hkv = hkv;
+  a.hd = hd;
+  a.dtype = dtype;
+  return prompt_attn_run(a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mtpb_scoring_status(uint32_t* status_out) {
+  if (!status_out) return bad("scoring_status: null argument");
+  uint32_t a = 0;
+  const uint32_t zero = 0;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&a, g_pa_status, sizeof(a));
+  if (e == cudaSuccess && a) e = cudaMemcpyToSymbol(g_pa_status, &zero, sizeof(zero));
+  if (e != cudaSuccess) return host_fail_cuda(e, "scoring_status");
+  *status_out = a;
+  return MTPB_OK;
+}

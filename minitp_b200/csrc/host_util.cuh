@@ -77,4 +77,15 @@ struct SharedAttnArgs {
 long long shared_attn_workspace(const SharedAttnArgs& a);
 int shared_attn_run(const SharedAttnArgs& a, void* ws, size_t ws_bytes, cudaStream_t st);
 
+// Causal attention over packed prompts (mtpb_prompt_attention).
+struct PromptAttnArgs {
+  const void *q, *k, *v;  // q [n], k and v [total] tokens; strides in elements
+  long long q_token, q_head, k_token, k_head, v_token, v_head;
+  void* out;              // [n][hq*hd]
+  const int* seq_starts;  // device [S + 1]
+  int S, first, n, total, hq, hkv, hd, dtype;
+  uint32_t* status = nullptr;  // word for error bits, or NULL: the library's own
+};
+int prompt_attn_run(const PromptAttnArgs& a, cudaStream_t st);
+
 }  // namespace mtpb

@@ -401,3 +401,156 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
              k_cache.data_ptr(), v_cache.data_ptr(), clen, clen_all, out.data_ptr(), g, n // g, t, hq, hkv, hd, cap_p,
              cap, code, _lib.ptr(ws), need)
     return out
+
+
+# ---------------------------------------------------------------------- #
+# scoring of prompts (no counterpart in the reference)
+# ---------------------------------------------------------------------- #
+def _packed_strides(name: str, t: torch.Tensor):
+    """``t [tokens, heads, hd]`` with its token and head strides, copied only where the kernels cannot read it in place."""
+    n, h, hd = t.shape
+    ts, hs = t.stride(0) if n > 1 else h * hd, t.stride(1) if h > 1 else hd
+    ve = 16 // t.element_size()
+    if t.stride(2) != 1 or ts < hd or hs < hd or ts % ve or hs % ve or t.data_ptr() % 16:
+        t = t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 == 0 else t.clone()
+        ts, hs = h * hd, hd
+    return t, ts, hs
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: torch.Tensor,
+                     first: int = 0) -> torch.Tensor:
+    """Causal grouped-query attention over packed prompts of different lengths -> ``[n, hq, hd]``.
+
+    Prompt s holds the packed tokens ``[seq_starts[s], seq_starts[s + 1])``
+    (int32 ``[S + 1]`` on the device, non-decreasing); each token attends to its
+    own prompt up to itself. ``k`` and ``v [tokens, hkv, hd]`` hold all tokens,
+    ``q [n, hq, hd]`` those from ``first`` on (all by default). Tokens and heads
+    may be strided (the parts of one projection's output are read in place). A
+    token of no prompt gets 0.
+    """
+    name = "prompt_attention"
+    dev = _same_device(name, q, k, v, seq_starts)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise _lib.MinitpB200Error(f"{name}: need q [n, hq, hd] and k, v [tokens, hkv, hd], got {tuple(q.shape)}, "
+                                   f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise _lib.MinitpB200Error(f"{name}: q, k and v must have one dtype")
+    if seq_starts.dtype != torch.int32 or seq_starts.dim() != 1 or seq_starts.numel() < 1 or \
+            not seq_starts.is_contiguous():
+        raise _lib.MinitpB200Error(f"{name}: seq_starts must be contiguous int32 [S + 1]")
+    n, hq, hd = q.shape
+    total, hkv, _ = k.shape
+    if hkv < 1 or hq < 1 or hq % hkv:
+        raise _lib.MinitpB200Error(f"{name}: {hq} heads over {hkv}")
+    if not 0 <= first <= total - n:
+        raise _lib.MinitpB200Error(f"{name}: tokens {first} .. {first + n} of {total} packed ones")
+    code = _lib.dtype_code(q.dtype)
+    out = torch.empty(n, hq, hd, dtype=q.dtype, device=dev)
+    (q, qt, qh), (k, kt, kh), (v, vt, vh) = (_packed_strides(name, t) for t in (q, k, v))
+    _call_on(dev, "mtpb_prompt_attention", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+             out.data_ptr(), seq_starts.data_ptr(), seq_starts.numel() - 1, first, n, total, hq, hkv, hd, code)
+    return out
+
+
+def _logprob_rows(name: str, logits: torch.Tensor, targets: torch.Tensor | None, top: int, least: int = 1):
+    """Checks shared by the log-probability calls -> (device, logits as rows, row stride, targets as rows)."""
+    if logits.dim() < 1:
+        raise _lib.MinitpB200Error(f"{name}: need logits [..., V]")
+    dev = _same_device(name, logits, targets)
+    v = logits.shape[-1]
+    if not (0 <= top <= 64 and least <= v < 2**30):
+        raise _lib.MinitpB200Error(f"{name}: need 0..64 alternatives and a vocabulary of 1 .. 2^30 - 1")
+    if targets is not None:
+        if targets.dtype != torch.int64 or targets.shape != logits.shape[:-1]:
+            raise _lib.MinitpB200Error(f"{name}: targets must be int64 {tuple(logits.shape[:-1])}")
+        targets = _c(targets)
+    rows = 1
+    for s in logits.shape[:-1]:
+        rows *= s
+    # rows of one stride are read in place; anything else is packed first
+    x = logits if logits.dim() == 2 else logits.reshape(rows, v)
+    if x.stride(1) != 1 and v > 1:
+        x = x.contiguous()
+    ld = x.stride(0) if rows > 1 else v
+    if ld < v:  # an expanded dimension
+        x, ld = x.contiguous(), v
+    return dev, x, ld, targets
+
+
+def _logprob_outputs(dev, shape, targets, top: int):
+    lp = None if targets is None else torch.empty(shape, dtype=torch.float32, device=dev)
+    ent = torch.empty(shape, dtype=torch.float32, device=dev)
+    if not top:
+        return lp, ent, None, None
+    tops = torch.empty(*shape, top, dtype=torch.float32, device=dev)
+    return lp, ent, tops, torch.empty(*shape, top, dtype=torch.int64, device=dev)
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0):
+    """Log-probabilities of given tokens, entropy and top alternatives of rows of logits.
+
+    ``logits [..., V]`` (fp32 or bf16), ``targets`` int64 ``[...]`` or None.
+    Returns ``(logprobs, entropy, top_logprobs, top_ids)``: fp32 ``[...]`` (None
+    without targets; NaN for an id outside the vocabulary), fp32 ``[...]`` in
+    natural units, and the ``top`` likeliest tokens, fp32 and int64
+    ``[..., top]``, best first, equal ones by the lower id (None with ``top``
+    0; at most 64). A NaN logit counts as -inf (a banned token); +inf logits
+    share the probability. Places without a token above -inf hold -inf and id
+    0; a row without any has entropy 0.
+    """
+    dev, x, ld, targets = _logprob_rows("token_logprobs", logits, targets, top)
+    rows, v = x.shape
+    out = _logprob_outputs(dev, logits.shape[:-1], targets, top)
+    if rows == 0:
+        return out
+    block = torch.empty_strided((logprobs_block_bytes(rows, v, top),), (1,), dtype=torch.uint8, device=dev)
+    _call_on(dev, "mtpb_token_logprobs", x.data_ptr(), ld, rows, v, _lib.ptr(targets), top, _lib.ptr(out[0]),
+             out[1].data_ptr(), _lib.ptr(out[2]), _lib.ptr(out[3]), block.data_ptr(), _lib.dtype_code(x.dtype))
+    return out
+
+
+def logprobs_block_bytes(rows: int, v_plan: int, top: int) -> int:
+    """Bytes of one shard's block (``logprobs_block``)."""
+    n = _lib.load().mtpb_logprobs_block_bytes(rows, v_plan, top)
+    if n < 0:
+        _lib.check(n)
+    return n
+
+
+def logprobs_block(local_logits: torch.Tensor, targets: torch.Tensor | None, top: int, vstart: int,
+                   v_plan: int) -> torch.Tensor:
+    """One vocabulary shard ``[..., V_local]`` (columns from ``vstart``; it may be empty) reduced to a block (uint8
+    [n]). ``v_plan``: the largest shard's columns, the same on every rank."""
+    if not (0 <= vstart < 2**32 and 1 <= v_plan < 2**30):
+        raise _lib.MinitpB200Error(f"logprobs_block: need a start below 2^32 and a plan of at least one column, got "
+                                   f"{vstart} and {v_plan}")
+    dev, x, ld, targets = _logprob_rows("logprobs_block", local_logits, targets, top, least=0)
+    rows, v = x.shape
+    if rows == 0:
+        return torch.empty(0, dtype=torch.uint8, device=dev)
+    block = torch.empty(logprobs_block_bytes(rows, v_plan, top), dtype=torch.uint8, device=dev)
+    _call_on(dev, "mtpb_logprobs_block", x.data_ptr(), ld, rows, v, vstart, v_plan, _lib.ptr(targets), top,
+             block.data_ptr(), _lib.dtype_code(x.dtype))
+    return block
+
+
+def logprobs_join(blocks: torch.Tensor, targets: torch.Tensor | None, shape, top: int, v_plan: int):
+    """``token_logprobs``'s result for rows of ``shape`` from the blocks ``[shards, n]`` of every vocabulary shard."""
+    dev = _same_device("logprobs_join", blocks, targets)
+    shape = torch.Size(shape)
+    rows = shape.numel()
+    if targets is not None and (targets.dtype != torch.int64 or targets.shape != shape):
+        raise _lib.MinitpB200Error(f"logprobs_join: targets must be int64 {tuple(shape)}")
+    if not (0 <= top <= 64 and 1 <= v_plan < 2**30):
+        raise _lib.MinitpB200Error(f"logprobs_join: need 0..64 alternatives, got {top}")
+    need = logprobs_block_bytes(rows, v_plan, top) if rows else 0
+    if blocks.dim() != 2 or blocks.dtype != torch.uint8 or not blocks.is_contiguous() or blocks.shape[1] != need:
+        raise _lib.MinitpB200Error(
+            "logprobs_join: blocks must be contiguous uint8 [shards, logprobs_block_bytes(rows, v_plan, top)]")
+    out = _logprob_outputs(dev, shape, targets, top)
+    if rows == 0:
+        return out
+    targets = None if targets is None else _c(targets)
+    _call_on(dev, "mtpb_logprobs_join", blocks.data_ptr(), blocks.shape[0], rows, v_plan, top, _lib.ptr(targets), top,
+             _lib.ptr(out[0]), out[1].data_ptr(), _lib.ptr(out[2]), _lib.ptr(out[3]))
+    return out
