@@ -8,6 +8,8 @@
 #include "logprobs.cuh"
 #include "prompt_attn.cuh"
 
+#include <cudaTypedefs.h>
+
 using namespace mtpb;
 
 namespace {
@@ -142,13 +144,50 @@ int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const i
 // ------------------------------------------------------------------ attention over packed prompts
 namespace {
 
+// Map of [total][hkv][hd] bf16 with the given strides, boxes of 128 tokens x 64
+// dims with the 128-byte swizzle; tokens from total on read as zeros.
+int pa_map(CUtensorMap* map, const void* ptr, const PaParams& p, long long ts, long long hs, int hd) {
+  const auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(host_tensor_map_encoder());
+  if (!enc) return host_fail(MTPB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[3] = {cuuint64_t(hd), cuuint64_t(p.total), cuuint64_t(p.hkv)};
+  const cuuint64_t strides[2] = {cuuint64_t(ts) * 2, cuuint64_t(hs) * 2};
+  const cuuint32_t box[3] = {64, kPaTcKeys, 1}, one[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MTPB_OK : host_fail(MTPB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+}
+
+// The grid's row tiles a KV head: no fewer than the prompts have, and one more
+// for tokens of no prompt.
+int pa_tiles(PaParams* p, int rows) {
+  const long long tiles = (long long)p->n * (p->hq / p->hkv) / rows + p->S + 1;
+  if (tiles * p->hkv > 0x7FFFFFFFll) return bad("prompt_attention: too many rows");
+  p->tiles = int(tiles);
+  return MTPB_OK;
+}
+
+template <int HD, int MT>
+int pa_launch_tc(PaParams p, cudaStream_t st) {
+  CUtensorMap mk, mv;
+  int r = pa_tiles(&p, 128 * MT);
+  if (r == MTPB_OK) r = pa_map(&mk, p.k, p, p.k_ts, p.k_hs, HD);
+  if (r == MTPB_OK) r = pa_map(&mv, p.v, p, p.v_ts, p.v_hs, HD);
+  if (r != MTPB_OK) return r;
+  return host_launch(pa_tc_kernel<HD, MT>, dim3(unsigned(p.tiles) * p.hkv), dim3(kPaTcThreads), PaTcCfg<HD, MT>::kSmem, st,
+                     p, mk, mv);
+}
+
 template <typename T, int HD>
 int pa_launch(PaParams p, cudaStream_t st) {
-  constexpr int RPT = 4, ROWS = 16 * RPT;
-  const long long tiles = (long long)p.n * (p.hq / p.hkv) / ROWS + p.S + 1;
-  if (tiles * p.hkv > 0x7FFFFFFFll) return bad("prompt_attention: too many rows");
-  p.tiles = int(tiles);
-  return host_launch(pa_simt_kernel<T, HD, RPT>, dim3(unsigned(tiles * p.hkv)), dim3(kPaThreads),
+  if constexpr (sizeof(T) == 2 && HD >= 64) {
+    const long long rows = (long long)p.n * p.hq;
+    return rows > 256ll * 148 ? pa_launch_tc<HD, 2>(p, st) : pa_launch_tc<HD, 1>(p, st);
+  }
+  constexpr int RPT = 4;
+  const int r = pa_tiles(&p, 16 * RPT);
+  if (r != MTPB_OK) return r;
+  return host_launch(pa_simt_kernel<T, HD, RPT>, dim3(unsigned(p.tiles) * p.hkv), dim3(kPaThreads),
                      pa_simt_smem<HD, RPT>(), st, p);
 }
 

@@ -18,7 +18,9 @@
 // it, and what a token does not see does not reach it.
 #pragma once
 
-#include "tcgen05.cuh"
+#include <type_traits>
+
+#include "softmax.cuh"
 
 namespace mtpb {
 
@@ -35,8 +37,6 @@ struct PaParams {
 
 // Set when a bounded wait of a prompt attention ran out (its results are then void).
 __device__ uint32_t g_pa_status;
-
-constexpr float kPaLog2e = 1.44269504088896340736f;
 
 // One tile's rows. Row r is token lo + (row0 + r) / G, query head
 // kvh * G + (row0 + r) % G, of a prompt from token `start` on.
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 #pragma unroll
     for (int d = 0; d < DP; ++d) o[a][d] = 0.f;
   }
-  const float sl2 = p.scale * kPaLog2e;
+  const float sl2 = p.scale * kLog2e;
   for (int j = 0; j < keys; j += kPaKeys) {
     __syncthreads();
     for (int i = tid; i < kPaKeys * (HD / VE); i += kPaThreads) {
@@ -338,6 +338,424 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 #pragma unroll
       for (int d = 0; d < DP; ++d) out[tx + 16 * d] = from_f<T>(l[a] == 0.f ? 0.f : o[a][d] / l[a]);
     }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Tiles on the tensor cores (bf16, head dim 64 or 128), one item a CTA, key
+// tiles of 128. Two streams share the ring of K and V tiles, each with an MMA
+// warp, a softmax warpgroup (a row a thread) and its own tensor memory:
+//   MT 2: stream x has rows 128 x .. of the item's 256 and their keys, so a
+//         K/V byte brought in from L2 serves 256 rows;
+//   MT 1: both have the item's 128 rows, stream x the key tiles t = x mod 2,
+//         and the streams are joined at the end.
+// One stream's softmax runs under the other's and under the MMAs:
+//   warp 0 loads (TMA, 128 keys x 64 dims boxes, 128-byte swizzle), warps 1
+//   and 2 issue S = Q K^T and O += P V of their stream, warps 4-7 and 8-11
+//   turn S into P, with the registers that warps 0-3 hand over (56 and 224 of
+//   168 a thread at launch).
+// P is bf16 in tensor memory, the A operand of P V; for head dim 128, where S
+// and O fill the 512 columns, it takes the place of its S, and the stream's
+// next S waits for the P V that reads it. V is read as it lies (N-major B).
+// The max that the exponentials are taken against is replaced, and O rescaled
+// in tensor memory, only when a row's max has grown by more than 2^8: until
+// then P is at most 2^8, which costs no precision, as the division by the sum
+// takes the factor out.
+// Keys that a row does not see are masked by selection. V rows behind the
+// tile's last key are zeroed in shared memory, since 0 x NaN would not be 0;
+// of those that not every row of the tile sees, the NaN and infinities are
+// zeroed and added at the end to the rows that do see them.
+// ---------------------------------------------------------------------------
+constexpr int kPaTcKeys = 128;
+constexpr int kPaTcThreads = 384;
+constexpr int kPaCubic = 4;  // of 16 pairs of exponentials, on the fp32 pipe
+
+template <int HD, int MT>
+struct PaTcCfg {
+  static constexpr int kSubs = HD / 64;
+  static constexpr uint32_t kTile = kSubs * kTcSub;  // a K, V or Q tile
+  // ring of K and V tiles: what 224 KB leave beside Q (at most six of each)
+  static constexpr int kRing = HD == 128 ? 7 - MT : 12;
+  static constexpr uint32_t kOffRing = MT * kTile;
+  static constexpr size_t kSmem = size_t(kOffRing) + kRing * kTile + 1024;
+  static constexpr bool kAlias = HD == 128;  // P in the place of S
+  static constexpr uint32_t kS = 128;        // columns from stream to stream of S; of O: HD
+  static constexpr uint32_t kO = 256, kP = kAlias ? 0 : 384, kPStep = kAlias ? 128 : 64;
+  static constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+  // B of P V: N (dims) contiguous
+  static constexpr uint32_t kIdescO =
+      (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+};
+
+template <int HD, int MT>
+__global__ void __launch_bounds__(kPaTcThreads, 1)
+    pa_tc_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+  using C = PaTcCfg<HD, MT>;
+  constexpr int NB = C::kRing, ROWS = 128 * MT;
+  constexpr uint64_t kBudget = 2000000000ull;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2][2], pv_done[2], drain[2], turn[2][4];
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_sh, odd_sh;  // odd_sh: values of V were zeroed
+  __shared__ float2 ml_sh[128];  // MT 1: stream 1's statistics
+  __shared__ PaItem it_sh;
+  volatile int* abort = &abort_sh;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
+  const int G = p.hq / p.hkv, kvh = blockIdx.x % p.hkv;
+  pdl_launch();
+  pdl_wait();
+  if (warp == 3) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (warp == 0) {
+    const PaItem mine = pa_item<ROWS>(p, blockIdx.x / p.hkv);
+    if (lane == 0) it_sh = mine;
+  } else if (threadIdx.x == 32) {
+    for (int s = 0; s < NB; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, MT);  // each stream that reads the tile
+    }
+    mbar_init(&qfull, 8);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(s_full + x, 1);
+      mbar_init(s_free + x, 4);
+      for (int h = 0; h < 2; ++h) mbar_init(&p_full[x][h], 4);
+      mbar_init(pv_done + x, 1);
+      mbar_init(drain + x, 1);
+      for (int q = 0; q < 4; ++q) mbar_init(&turn[x][q], 1);
+    }
+    *abort = 0;
+    odd_sh = 0;
+    mbar_init_fence();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  const PaItem it = it_sh;
+  // keys of the prompt that row r of the tile sees
+  auto seen = [&](int r) { return it.lo + (it.row0 + r) / G + 1 - it.start; };
+  const int keys = it.rows > 0 ? seen(it.rows - 1) : 0;
+  // tiles of stream x: first, step, and how many
+  constexpr int kStep = MT == 2 ? 1 : 2;
+  const int nt = (keys + kPaTcKeys - 1) / kPaTcKeys;
+  auto tiles_of = [&](int x) {
+    if (MT == 1) return (nt - x + 1) / 2;
+    return it.rows > 128 * x ? (seen(min(it.rows, 128 * x + 128) - 1) + kPaTcKeys - 1) / kPaTcKeys : 0;
+  };
+
+  // the end of every role: nobody uses tensor or shared memory any more
+  auto leave = [&]() {
+    tc_fence_before();
+    __syncwarp();
+    named_sync(2, kPaTcThreads);
+    if (warp == 3) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+      if (lane == 0 && *abort) atomicOr(p.status ? p.status : &g_pa_status, kStatusTimeout);
+    }
+  };
+
+  if (it.rows <= 0) {
+    pa_zero<bf16>(p, it, kvh, HD, kPaTcThreads);
+    leave();
+  } else if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      int issued = 0;  // ring entries whose copies were issued
+      for (int i = 0; i < 2 * nt; ++i) {  // K and V of each tile in turn
+        const int s = i % NB, j = it.start + (i >> 1) * kPaTcKeys;
+        const bool ok = i < NB || mbar_wait_soon(empty + s, uint32_t((i / NB) & 1) ^ 1u, kBudget, abort);
+        if (!__all_sync(0xffffffffu, ok)) {
+          *abort = 1;
+          break;
+        }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(full + s, C::kTile);
+#pragma unroll
+          for (int b = 0; b < C::kSubs; ++b)
+            tma_load_3d(base + C::kOffRing + s * C::kTile + b * kTcSub, i & 1 ? &map_v : &map_k, b * 64, j, kvh, full + s);
+        }
+        issued = i + 1;
+      }
+      // copies in flight land before the memory goes away
+      int never = 0;
+      for (int i = max(0, issued - NB); i < issued; ++i) mbar_wait(full + i % NB, uint32_t((i / NB) & 1), kBudget, &never);
+    } else if (warp < 3) {
+      // ---- MMA issue of stream x
+      const int x = warp - 1, first = MT == 2 ? 0 : x, mine = tiles_of(x);
+      const uint64_t dq = tc_smem_desc(base + (MT == 2 ? x : 0) * C::kTile);
+      const uint32_t ts = tmem + x * C::kS, to = tmem + C::kO + x * HD, tp = tmem + C::kP + x * C::kPStep;
+      auto wait = [&](uint64_t* bar, int phase) {
+        return __all_sync(0xffffffffu, mbar_wait_soon(bar, uint32_t(phase & 1), kBudget, abort));
+      };
+      auto qk = [&](int k) {
+        const int i = 2 * (first + k * kStep), s = i % NB;
+        // S is free: read by the softmax, and (aliased) its P read by P V
+        if (!wait(full + s, i / NB) || (k > 0 && !wait(C::kAlias ? pv_done + x : s_free + x, k - 1))) return false;
+        tc_fence_after();
+        const uint64_t dk = tc_smem_desc(base + C::kOffRing + s * C::kTile);
+        if (elect_one()) {
+#pragma unroll
+          for (int q = 0; q < HD / 16; ++q) {
+            const uint32_t off = ((q >> 2) * kTcSub + (q & 3) * 32) >> 4;
+            tc_mma(ts, dq + off, dk + off, C::kIdescS, q > 0 ? 1u : 0u);
+          }
+          tc_commit(s_full + x);
+          tc_commit(empty + s);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto pv = [&](int k) {
+        const int i = 2 * (first + k * kStep) + 1, s = i % NB;
+        if (!wait(full + s, i / NB)) return false;
+        const uint64_t dv = tc_smem_desc_mn(base + C::kOffRing + s * C::kTile, kTcSub);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // the first half of the keys under the second half's exponentials
+          if (!wait(&p_full[x][h], k)) return false;
+          tc_fence_after();
+          const uint32_t acc = h > 0 || k > 0 ? 1u : 0u;
+          if (elect_one()) {
+#pragma unroll
+            for (int q = 4 * h; q < 4 * h + 4; ++q)
+              tc_mma_ta(to, tp + q * 8, dv + ((q * 2048) >> 4), C::kIdescO, q > 4 * h ? 1u : acc);
+            if (h == 1) {
+              tc_commit(pv_done + x);
+              tc_commit(empty + s);
+            }
+          }
+          __syncwarp();
+        }
+        return true;
+      };
+      bool ok = mine == 0 || wait(&qfull, 0);
+      if (C::kAlias) {
+        for (int k = 0; ok && k < mine; ++k) ok = qk(k) && pv(k);
+      } else {  // the next S under this one's softmax
+        if (ok && mine > 0) ok = qk(0);
+        for (int k = 0; ok && k < mine; ++k) {
+          if (k + 1 < mine) ok = qk(k + 1);
+          ok = ok && pv(k);
+        }
+      }
+      if (MT == 2)  // the other stream's tiles, which this one does not read
+        for (int i = 2 * mine; ok && i < 2 * nt; ++i) {
+          ok = wait(full + i % NB, i / NB);
+          if (ok && lane == 0) mbar_arrive(empty + i % NB);
+        }
+      if (!ok) *abort = 1;
+      // behind every MMA of the warp (a commit follows those of its own thread:
+      // the elected lane is the same each time)
+      int never = 0;
+      if (elect_one()) tc_commit(drain + x);
+      __syncwarp();
+      mbar_wait(drain + x, 0u, kBudget, &never);
+    }
+    leave();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // ---- softmax of stream x
+    const int stid = int(threadIdx.x) - 128, x = stid >> 7;
+    const int quarter = warp & 3, r = quarter * 32 + lane;
+    {  // Q: a warp's rows, whole rows side by side in the lanes, all loads in flight at once
+      constexpr int RW = 16 * MT, CH = HD / 8, RI = 32 / CH, N = RW / RI;  // rows a warp, chunks a row, rows a load
+      const int row0 = (warp - 4) * RW, at = row0 + (lane & (RW - 1));
+      unsigned long long off = ~0ull;  // of row `at` in q
+      if (at < it.rows) {
+        const int row = it.row0 + at, t = row / G;
+        off = (it.lo + t - p.first) * p.q_ts + (kvh * G + row - t * G) * p.q_hs;
+      }
+      uint4 v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const unsigned long long o = __shfl_sync(0xffffffffu, off, i * RI + lane / CH);
+        v[i] = o != ~0ull ? ld_vec(static_cast<const bf16*>(p.q) + o + (lane % CH) * 8) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int row = row0 + i * RI + lane / CH, c = lane % CH;
+        *reinterpret_cast<uint4*>(smem + (row >> 7) * C::kTile + (c >> 3) * kTcSub + (row & 127) * 128 +
+                                  (((c & 7) ^ (row & 7)) << 4)) = v[i];
+      }
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&qfull);
+    const uint32_t trow = tmem + (uint32_t(quarter * 32) << 16);
+    const uint32_t ts = trow + x * C::kS, to = trow + C::kO + x * HD, tp = trow + C::kP + x * C::kPStep;
+    const int row = MT == 2 ? x * 128 + r : r;
+    const bool write = row < it.rows;
+    const int lim = write ? seen(row) : keys;  // keys [0, lim) are seen
+    const int low = seen(0);  // keys [0, low) are seen by all
+    const int mine = tiles_of(x), others = tiles_of(1 - x);
+    const float sl2 = p.scale * kLog2e;
+    float m = -INFINITY, l = 0.f;  // reference max (scaled, base 2), sum
+    bool ok = true;
+    int k = 0;
+    for (; k < mine; ++k) {
+      const int t = MT == 2 ? k : 2 * k + x, j = t * kPaTcKeys;
+      ok = mbar_wait_soon(s_full + x, uint32_t(k & 1), kBudget, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      float sc[kPaTcKeys];
+#pragma unroll
+      for (int c = 0; c < kPaTcKeys; c += 32) tc_ld32(ts + c, reinterpret_cast<uint32_t*>(sc + c));
+      tc_wait_ld();
+      if (!C::kAlias) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free + x);
+      }
+      const bool masked = __any_sync(0xffffffffu, j + kPaTcKeys > lim);
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < kPaTcKeys; ++c) sc[c] = j + c < lim ? sc[c] : -INFINITY;
+      }
+      float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+      for (int c = 4; c < kPaTcKeys - 4; c += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = max3_nan(mx[i], sc[c + i], sc[c + 4 + i]);
+      mx[0] = max3_nan(mx[0], sc[124], sc[125]);
+      mx[1] = max3_nan(mx[1], sc[126], sc[127]);
+      const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sl2;
+      const bool grow = !(top <= m + 8.f);  // (NaN stays: exp2_cubic would lose it)
+      if (!C::kAlias && k > 0) {  // the stream's previous P V has read P (aliased: it came before this S)
+        ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+        const float a = grow ? exp2_approx(m - top) : 1.f;
+        if (grow) m = top;
+        l *= a;
+        if (k > 0) {
+#pragma unroll
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t o[16];
+            tc_ld16(to + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+            tc_st16(to + c, o);
+          }
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      if (j + kPaTcKeys > low) {  // V rows behind the keys, or not seen by all (MT 2: both streams write the same zeros)
+        const int i = 2 * t + 1, s = i % NB;
+        ok = mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_clean_row<HD>(smem + C::kOffRing + s * C::kTile, r, j + r >= keys, j + r >= low, &odd_sh);
+        fence_async_smem();
+      }
+      // the exponentials of the two warps of a scheduler take turns: one stream's
+      // run under the other's MMAs, and not both at half pace
+      if (x == 1 ? k < others : k > 0 && k - 1 < others) {
+        ok = mbar_wait_soon(&turn[x][quarter], uint32_t(x == 1 ? k & 1 : (k - 1) & 1), kBudget, abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      // kCubic of 16 pairs on the fp32 pipe, which the special-function unit
+      // (8 cycles a warp and value) leaves idle; masked tiles need exact zeros
+      auto exps = [&](auto cubic) {
+        constexpr int kCubic = decltype(cubic)::value;
+#pragma unroll
+        for (int c = 0; c < kPaTcKeys; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float2 e = fma2(make_float2(sc[c + i], sc[c + i + 1]), make_float2(sl2, sl2), make_float2(-ref, -ref));
+            if ((i >> 1) * kCubic % 16 < kCubic) {
+              e = exp2_cubic(e);
+            } else {
+              e.x = exp2_approx(e.x);
+              e.y = exp2_approx(e.y);
+            }
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+            pk[i / 2] = pack_bf16(e.x, e.y);
+          }
+          if (c == 64) {  // the first half of the keys: its stores have landed meanwhile
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[x][0]);
+          }
+          tc_st16(tp + c / 2, pk);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&turn[1 - x][quarter]);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x][1]);
+      };
+      if (masked)
+        exps(std::integral_constant<int, 0>{});
+      else
+        exps(std::integral_constant<int, kPaCubic>{});
+      sum[0] = add2(sum[0], sum[1]);
+      l += sum[0].x + sum[0].y;
+    }
+    if (ok && k > 0) ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
+    if (!ok) *abort = 1;
+    tc_fence_after();
+    float wb = 0.f, wa = 1.f;
+    if (MT == 1) {
+      if (x == 1) ml_sh[r] = make_float2(k > 0 ? m : -INFINITY, l);
+      tc_fence_before();
+      named_sync(1, 256);
+      tc_fence_after();
+      const float2 b = ml_sh[r];
+      // (a NaN max or sum of either stream makes both weights, or the sum, NaN)
+      const float top = max3_nan(m, b.x, b.x), ref = top == -INFINITY ? 0.f : top;
+      wa = exp2_approx(m - ref);
+      wb = exp2_approx(b.x - ref);
+      l = l * wa + b.y * wb;
+    }
+    if ((MT == 2 || x == 0) && __any_sync(0xffffffffu, write)) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const bool odd = *static_cast<volatile int*>(&odd_sh) != 0, two = MT == 1 && nt > 1;
+      const int tok = it.lo + (it.row0 + row) / G, head = kvh * G + (it.row0 + row) % G;
+      bf16* out = static_cast<bf16*>(p.out) + (size_t(tok - p.first) * p.hq + head) * HD;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 16) {
+        uint32_t o0[16], o1[16];
+        tc_ld16(to + c, o0);
+        if (two) tc_ld16(to + HD + c, o1);
+        tc_wait_ld();
+        float f[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          f[e] = __uint_as_float(o0[e]) * wa;
+          if (two) f[e] = fmaf(__uint_as_float(o1[e]), wb, f[e]);
+        }
+        if (write) {
+          if (odd) {  // what was taken out of V
+            const bf16* v = static_cast<const bf16*>(p.v) + kvh * p.v_hs + it.start * p.v_ts + c;
+            for (int key = low; key < lim; ++key)
+              for (int e = 0; e < 16; ++e) {
+                const float y = to_f(v[key * p.v_ts + e]);
+                if (!(fabsf(y) < INFINITY))
+#pragma unroll
+                  for (int u = 0; u < 16; ++u) f[u] = u == e ? f[u] + y : f[u];
+              }
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            *reinterpret_cast<uint4*>(out + c + e) =
+                l == 0.f ? make_uint4(0, 0, 0, 0)
+                         : make_uint4(pack_bf16(f[e] * inv, f[e + 1] * inv), pack_bf16(f[e + 2] * inv, f[e + 3] * inv),
+                                      pack_bf16(f[e + 4] * inv, f[e + 5] * inv), pack_bf16(f[e + 6] * inv, f[e + 7] * inv));
+        }
+      }
+    }
+    leave();
   }
 }
 
