@@ -144,38 +144,52 @@ int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const i
 // ------------------------------------------------------------------ attention over packed prompts
 namespace {
 
-// Map of [total][hkv][hd] bf16 with the given strides, boxes of 128 tokens x 64
-// dims with the 128-byte swizzle; tokens from total on read as zeros.
-int pa_map(CUtensorMap* map, const void* ptr, const PaParams& p, long long ts, long long hs, int hd) {
+// Map of [tokens][heads][hd] bf16 with the given strides, boxes of 64 dims x
+// `bh` heads x `bt` tokens with the 128-byte swizzle. The coordinates are (dim,
+// head, token) for queries and (dim, token, head) for keys and values, whose
+// boxes hold one head. Tokens from the last on read as zeros.
+int pa_map(CUtensorMap* map, const void* ptr, int tokens, int heads, long long ts, long long hs, int hd, bool query, int bt,
+           int bh) {
   const auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(host_tensor_map_encoder());
   if (!enc) return host_fail(MTPB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-  const cuuint64_t dims[3] = {cuuint64_t(hd), cuuint64_t(p.total), cuuint64_t(p.hkv)};
-  const cuuint64_t strides[2] = {cuuint64_t(ts) * 2, cuuint64_t(hs) * 2};
-  const cuuint32_t box[3] = {64, kPaTcKeys, 1}, one[3] = {1, 1, 1};
+  const int h = query ? 1 : 2, t = 3 - h;  // the axes of heads and of tokens
+  cuuint64_t dims[3] = {cuuint64_t(hd)}, strides[2];
+  cuuint32_t box[3] = {64}, one[3] = {1, 1, 1};
+  dims[h] = cuuint64_t(heads);
+  dims[t] = cuuint64_t(tokens);
+  strides[h - 1] = cuuint64_t(hs) * 2;
+  strides[t - 1] = cuuint64_t(ts) * 2;
+  box[h] = cuuint32_t(bh);
+  box[t] = cuuint32_t(bt);
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, one,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? MTPB_OK : host_fail(MTPB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
 }
 
-// The grid's row tiles a KV head: no fewer than the prompts have, and one more
-// for tokens of no prompt.
-int pa_tiles(PaParams* p, int rows) {
-  const long long tiles = (long long)p->n * (p->hq / p->hkv) / rows + p->S + 1;
-  if (tiles * p->hkv > 0x7FFFFFFFll) return bad("prompt_attention: too many rows");
-  p->tiles = int(tiles);
-  return MTPB_OK;
+// Row groups and tokens of tiles of `rows` rows, and the items that there can
+// be at most: all heads of a KV head side by side, or as many of them as divide
+// them and fit.
+long long pa_items(PaParams* p, int rows) {
+  const int G = p->hq / p->hkv;
+  p->subs = 1;
+  while (G % p->subs || G / p->subs > rows) ++p->subs;
+  p->gs = G / p->subs;
+  p->planes = p->hkv * p->subs;
+  p->tt = rows / p->gs;
+  return ((long long)p->n / p->tt + p->S) * p->planes;
 }
 
 template <int HD, int MT>
 int pa_launch_tc(PaParams p, cudaStream_t st) {
-  CUtensorMap mk, mv;
-  int r = pa_tiles(&p, 128 * MT);
-  if (r == MTPB_OK) r = pa_map(&mk, p.k, p, p.k_ts, p.k_hs, HD);
-  if (r == MTPB_OK) r = pa_map(&mv, p.v, p, p.v_ts, p.v_hs, HD);
+  const long long items = pa_items(&p, 128 * MT);
+  CUtensorMap mq, mk, mv;
+  int r = pa_map(&mq, p.q, p.n, p.hq, p.q_ts, p.q_hs, HD, true, p.tt, p.gs);
+  if (r == MTPB_OK) r = pa_map(&mk, p.k, p.total, p.hkv, p.k_ts, p.k_hs, HD, false, kPaTcKeys, 1);
+  if (r == MTPB_OK) r = pa_map(&mv, p.v, p.total, p.hkv, p.v_ts, p.v_hs, HD, false, kPaTcKeys, 1);
   if (r != MTPB_OK) return r;
-  return host_launch(pa_tc_kernel<HD, MT>, dim3(unsigned(p.tiles) * p.hkv), dim3(kPaTcThreads), PaTcCfg<HD, MT>::kSmem, st,
-                     p, mk, mv);
+  const unsigned grid = unsigned(std::max<long long>(1, std::min<long long>(items, host_sms())));
+  return host_launch(pa_tc_kernel<HD, MT>, dim3(grid), dim3(kPaTcThreads), PaTcCfg<HD, MT>::kSmem, st, p, mq, mk, mv);
 }
 
 template <typename T, int HD>
@@ -183,12 +197,12 @@ int pa_launch(PaParams p, cudaStream_t st) {
   if constexpr (sizeof(T) == 2 && HD >= 64) {
     const long long rows = (long long)p.n * p.hq;
     return rows > 256ll * 148 ? pa_launch_tc<HD, 2>(p, st) : pa_launch_tc<HD, 1>(p, st);
+  } else {
+    constexpr int RPT = 4;
+    const long long items = pa_items(&p, 16 * RPT) + 1;
+    if (items > 0x7FFFFFFFll) return bad("prompt_attention: too many rows");
+    return host_launch(pa_simt_kernel<T, HD, RPT>, dim3(unsigned(items)), dim3(kPaThreads), pa_simt_smem<HD, RPT>(), st, p);
   }
-  constexpr int RPT = 4;
-  const int r = pa_tiles(&p, 16 * RPT);
-  if (r != MTPB_OK) return r;
-  return host_launch(pa_simt_kernel<T, HD, RPT>, dim3(unsigned(p.tiles) * p.hkv), dim3(kPaThreads),
-                     pa_simt_smem<HD, RPT>(), st, p);
 }
 
 template <typename T>
@@ -218,8 +232,8 @@ int prompt_attn_run(const PromptAttnArgs& a, cudaStream_t st) {
   if (a.n == 0) return MTPB_OK;
   if (!a.q || !a.k || !a.v || !a.out || !a.seq_starts) return bad("prompt_attention: null tensor");
   const int es = a.dtype == MTPB_BF16 ? 2 : 4, ve = 16 / es;
-  if (!al16(a.q) || !al16(a.k) || !al16(a.v) || !al16(a.out))
-    return bad("prompt_attention: tensors must be 16-byte aligned");
+  if (!al16(a.q) || !al16(a.k) || !al16(a.v) || (reinterpret_cast<uintptr_t>(a.out) & 31u))
+    return bad("prompt_attention: tensors must be 16-byte aligned, out 32-byte aligned");
   const long long strides[6] = {a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head};
   for (long long s : strides)
     if (s < a.hd || s % ve || s >= 1ll << 38)

@@ -30,7 +30,9 @@ struct PaParams {
   void* out;          // [n][hq][hd]
   const int* starts;  // device [S + 1]
   int S, first, n, total, hq, hkv;
-  int tiles;  // row tiles a KV head that the grid covers: at least as many as there are
+  int gs, subs;  // heads of a row group, groups of a KV head: gs * subs = G
+  int tt;        // tokens a tile: as many as its rows hold, gs rows each
+  int planes;    // hkv * subs
   float scale;
   uint32_t* status;  // error bits
 };
@@ -38,131 +40,145 @@ struct PaParams {
 // Set when a bounded wait of a prompt attention ran out (its results are then void).
 __device__ uint32_t g_pa_status;
 
-// One tile's rows. Row r is token lo + (row0 + r) / G, query head
-// kvh * G + (row0 + r) % G, of a prompt from token `start` on.
+// A tile: row r is token tok0 + r / gs, head r % gs of the row group.
 struct PaItem {
-  int start, lo;  // packed tokens
-  int row0, rows;  // rows 0: no tile; the CTA is then number `spare` of `spares`
-  int spare, spares;
-  int gap0, gap1;  // tokens [first, gap0) and [gap1, first + n) are of no prompt
+  int start;  // of the prompt (packed tokens)
+  int tok0, ntok;  // ntok 0: no tile
+  int plane;  // KV head and row group
 };
 
 // Prompts whose tiles are put in order (a lane has its share in registers).
 constexpr int kPaOrdered = 4 * 32;
 
-// Tile number i, by one warp. Tiles come in descending order of their place in
-// their prompt, which is how many keys they see, over all prompts, so that
-// the longest do not start last; with more than kPaOrdered prompts prompt after
-// prompt. The starts are made non-decreasing and cut to [0, total] first, so
-// that no values of theirs lead out of the tensors or make two tiles of a row.
-template <int ROWS>
-__device__ __forceinline__ PaItem pa_item(const PaParams& p, int i) {
-  const int lane = threadIdx.x & 31, G = p.hq / p.hkv, end = p.first + p.n;
-  PaItem it;
-  it.start = it.lo = it.row0 = it.rows = 0;
-  auto cut = [&](int t) { return min(max(t, 0), p.total); };
-  int at_least = cut(__ldg(p.starts));  // the largest start so far
-  it.gap0 = min(max(at_least, p.first), end);
+// The tiles of all prompts, by one warp, in the order of growing numbers. They
+// are numbered in descending order of their place in their prompt, which is how
+// many keys they see, over all prompts, so that the longest do not start last;
+// with more than kPaOrdered prompts prompt after prompt (the last tile first).
+// The starts are made non-decreasing and cut to [0, total] first, so that no
+// values of theirs lead out of the tensors or make two tiles of a token.
+struct PaTiles {
   struct Seq {
-    int start, lo, rows, nt, off;  // off: place of the first tile
+    int start, lo, n, nt, off;  // packed tokens from lo on, tiles, place of the first tile
   };
-  auto load = [&](int b) {  // prompt 32 b + lane
-    const int s = 32 * b + lane;
-    int hi = max(at_least, s < p.S ? cut(__ldg(p.starts + s + 1)) : 0);
+  int at_least;  // the largest start so far
+  int gap0, gap1;  // tokens [first, gap0) and [gap1, first + n) are of no prompt (gap1: once all were read)
+  int all;  // tiles: of all prompts, or (not ordered) of those before block b
+  int b, most;
+  Seq q[kPaOrdered / 32];
+
+  static __device__ __forceinline__ int cut(const PaParams& p, int t) { return min(max(t, 0), p.total); }
+
+  __device__ __forceinline__ Seq load(const PaParams& p, int blk) {  // prompt 32 blk + lane
+    const int lane = threadIdx.x & 31, s = 32 * blk + lane, end = p.first + p.n;
+    int hi = max(at_least, s < p.S ? cut(p, __ldg(p.starts + s + 1)) : 0);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, hi, o);
       if (lane >= o) hi = max(hi, u);
     }
     const int prev = __shfl_up_sync(0xffffffffu, hi, 1);
-    Seq q;
-    q.start = lane ? prev : at_least;
-    q.lo = max(q.start, p.first);
-    q.rows = max(0, min(hi, end) - q.lo) * G;
-    q.nt = (q.rows + ROWS - 1) / ROWS;
-    q.off = q.rows ? int((long long)(q.lo - q.start) * G / ROWS) : 0;
+    Seq r;
+    r.start = lane ? prev : at_least;
+    r.lo = max(r.start, p.first);
+    r.n = max(0, min(hi, end) - r.lo);
+    r.nt = (r.n + p.tt - 1) / p.tt;
+    r.off = r.n ? (r.lo - r.start) / p.tt : 0;
     at_least = __shfl_sync(0xffffffffu, hi, 31);
-    return q;
-  };
-  auto take = [&](int from, const Seq& q, int tile) {  // tile of lane `from`'s prompt
-    it.start = __shfl_sync(0xffffffffu, q.start, from);
-    it.lo = __shfl_sync(0xffffffffu, q.lo, from);
-    it.row0 = tile * ROWS;
-    it.rows = min(ROWS, __shfl_sync(0xffffffffu, q.rows, from) - it.row0);
-  };
-  int all = 0;
-  if (p.S <= kPaOrdered) {
-    Seq q[kPaOrdered / 32];
-    int most = 0;
+    return r;
+  }
+
+  __device__ __forceinline__ void open(const PaParams& p) {
+    at_least = cut(p, __ldg(p.starts));
+    gap0 = min(max(at_least, p.first), p.first + p.n);
+    all = b = most = 0;
+    if (p.S > kPaOrdered) {
+      q[0] = load(p, 0);
+      return;
+    }
 #pragma unroll
-    for (int b = 0; b < kPaOrdered / 32; ++b) {
-      q[b] = Seq{0, 0, 0, 0, 0};
-      if (32 * b < p.S) q[b] = load(b);
-      if (q[b].nt) most = max(most, q[b].off + q[b].nt);
-      all += q[b].nt;
+    for (int i = 0; i < kPaOrdered / 32; ++i) {
+      q[i] = Seq{0, 0, 0, 0, 0};
+      if (32 * i < p.S) q[i] = load(p, i);
+      if (q[i].nt) most = max(most, q[i].off + q[i].nt);
+      all += q[i].nt;
     }
     most = __reduce_max_sync(0xffffffffu, most);
     all = __reduce_add_sync(0xffffffffu, all);
-    if (i < all) {
-      auto above = [&](int c) {  // tiles at place c or behind it
-        int n = 0;
-#pragma unroll
-        for (int b = 0; b < kPaOrdered / 32; ++b) n += max(0, q[b].off + q[b].nt - max(c, q[b].off));
-        return __reduce_add_sync(0xffffffffu, n);
-      };
-      int lo = 0, hi = most;  // above(lo) > i >= above(hi)
-      while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2;
-        if (above(mid) > i)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      int left = i - above(lo + 1);  // of the tiles at place lo
-#pragma unroll
-      for (int b = 0; b < kPaOrdered / 32; ++b) {
-        const uint32_t m = __ballot_sync(0xffffffffu, q[b].off <= lo && lo < q[b].off + q[b].nt);
-        const int c = __popc(m);
-        if (left >= 0 && left < c) {
-          const int from = __fns(m, 0, left + 1);
-          take(from, q[b], lo - __shfl_sync(0xffffffffu, q[b].off, from));
-        }
-        left -= c;
-      }
-    }
-  } else {
-    for (int b = 0; 32 * b < p.S; ++b) {
-      const Seq q = load(b);
-      int upto = q.nt;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += u;
-      }
-      const int sum = __shfl_sync(0xffffffffu, upto, 31);
-      if (i >= all && i < all + sum) {
-        const int from = __popc(__ballot_sync(0xffffffffu, all + upto <= i));
-        take(from, q, all + __shfl_sync(0xffffffffu, upto, from) - 1 - i);  // a prompt's last tile first
-      }
-      all += sum;
-    }
+    gap1 = min(max(at_least, p.first), p.first + p.n);
   }
-  it.gap1 = min(max(at_least, p.first), end);
-  it.spare = i - all;
-  it.spares = p.tiles - all;
-  return it;
-}
 
-// What a CTA without a tile does: its share of the tokens of no prompt gets 0.
+  __device__ __forceinline__ PaItem take(const PaParams& p, int from, const Seq& r, int tile) {
+    PaItem it;
+    it.start = __shfl_sync(0xffffffffu, r.start, from);
+    it.tok0 = __shfl_sync(0xffffffffu, r.lo, from) + tile * p.tt;
+    it.ntok = min(p.tt, __shfl_sync(0xffffffffu, r.n, from) - tile * p.tt);
+    return it;
+  }
+
+  // Tile number i (no smaller than in the call before); ntok 0 when there is none.
+  __device__ __forceinline__ PaItem find(const PaParams& p, int i) {
+    const int lane = threadIdx.x & 31;
+    PaItem it{0, 0, 0, 0};
+    if (p.S > kPaOrdered) {
+      for (;; ++b) {
+        int upto = q[0].nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += u;
+        }
+        const int sum = __shfl_sync(0xffffffffu, upto, 31);
+        if (i < all + sum) {
+          const int from = __popc(__ballot_sync(0xffffffffu, all + upto <= i));
+          return take(p, from, q[0], all + __shfl_sync(0xffffffffu, upto, from) - 1 - i);
+        }
+        if (32 * (b + 1) >= p.S) break;
+        all += sum;
+        q[0] = load(p, b + 1);
+      }
+      gap1 = min(max(at_least, p.first), p.first + p.n);
+      return it;
+    }
+    if (i >= all) return it;
+    auto above = [&](int c) {  // tiles at place c or behind it
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < kPaOrdered / 32; ++k) n += max(0, q[k].off + q[k].nt - max(c, q[k].off));
+      return __reduce_add_sync(0xffffffffu, n);
+    };
+    int lo = 0, hi = most;  // above(lo) > i >= above(hi)
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if (above(mid) > i)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    int left = i - above(lo + 1);  // of the tiles at place lo
+#pragma unroll
+    for (int k = 0; k < kPaOrdered / 32; ++k) {
+      const uint32_t m = __ballot_sync(0xffffffffu, q[k].off <= lo && lo < q[k].off + q[k].nt);
+      const int c = __popc(m);
+      if (left >= 0 && left < c) {
+        const int from = __fns(m, 0, left + 1);
+        it = take(p, from, q[k], lo - __shfl_sync(0xffffffffu, q[k].off, from));
+      }
+      left -= c;
+    }
+    return it;
+  }
+};
+
+// A share of the tokens of no prompt gets 0: one warp, when all tiles have been found.
 template <typename T>
-__device__ __forceinline__ void pa_zero(const PaParams& p, const PaItem& it, int kvh, int hd, int threads) {
+__device__ __forceinline__ void pa_zero(const PaParams& p, const PaTiles& t, int hd, int share, int shares) {
   constexpr int VE = VecTraits<T>::kElems;
-  const int G = p.hq / p.hkv, vecs = G * hd / VE;  // of a token
-  const int n0 = it.gap0 - p.first, n1 = p.first + p.n - it.gap1;
-  for (int t = it.spare; t < n0 + n1; t += it.spares) {
-    const int at = t < n0 ? t : it.gap1 - p.first + (t - n0);
-    uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + ((size_t)at * p.hq + size_t(kvh) * G) * hd);
-    for (int i = threadIdx.x; i < vecs; i += threads) o[i] = make_uint4(0, 0, 0, 0);
+  const int vecs = p.hq * hd / VE;  // of a token
+  const int n0 = t.gap0 - p.first, n1 = p.first + p.n - t.gap1;
+  for (int i = share; i < n0 + n1; i += shares) {
+    const int at = i < n0 ? i : t.gap1 - p.first + (i - n0);
+    uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (size_t)at * p.hq * hd);
+    for (int e = threadIdx.x & 31; e < vecs; e += 32) o[e] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -194,38 +210,39 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
   __shared__ PaItem it_sh;
   pdl_launch();
   pdl_wait();
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, G = p.hq / p.hkv;
-  const int kvh = blockIdx.x % p.hkv;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   if (tid < 32) {
-    const PaItem it = pa_item<ROWS>(p, blockIdx.x / p.hkv);
+    PaTiles tiles;
+    tiles.open(p);
+    PaItem it = tiles.find(p, blockIdx.x / p.planes);
+    it.plane = blockIdx.x % p.planes;
     if (tid == 0) it_sh = it;
+    if (blockIdx.x == gridDim.x - 1) {  // (the grid has a CTA more than tiles)
+      it = tiles.find(p, 0x7FFFFFFF);
+      pa_zero<T>(p, tiles, HD, 0, 1);
+    }
   }
   __syncthreads();
   const PaItem it = it_sh;
-  if (it.rows <= 0) {
-    pa_zero<T>(p, it, kvh, HD, kPaThreads);
-    return;
-  }
+  if (it.ntok == 0) return;
+  const int rows = it.ntok * p.gs, kvh = it.plane / p.subs, head0 = it.plane * p.gs;
   const T* q = static_cast<const T*>(p.q);
   const T* k = static_cast<const T*>(p.k) + kvh * p.k_hs;
   const T* v = static_cast<const T*>(p.v) + kvh * p.v_hs;
-  auto token = [&](int r) { return it.lo + (it.row0 + r) / G; };
+  auto token = [&](int r) { return it.tok0 + r / p.gs; };
   for (int i = tid; i < ROWS * (HD / VE); i += kPaThreads) {
     const int r = i / (HD / VE), c = (i - r * (HD / VE)) * VE;
     float f[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) f[e] = 0.f;
-    if (r < it.rows) {
-      const int row = it.row0 + r;
-      unpack(ld_vec(q + (it.lo + row / G - p.first) * p.q_ts + (kvh * G + row % G) * p.q_hs + c), f);
-    }
+    if (r < rows) unpack(ld_vec(q + (token(r) - p.first) * p.q_ts + (head0 + r % p.gs) * p.q_hs + c), f);
 #pragma unroll
     for (int e = 0; e < VE; ++e) sq[r * LD + c + e] = f[e];
   }
   int lim[RPT];  // keys [0, lim) of the prompt are seen
 #pragma unroll
-  for (int a = 0; a < RPT; ++a) lim[a] = token(min(ty * RPT + a, it.rows - 1)) + 1 - it.start;
-  const int keys = token(it.rows - 1) + 1 - it.start, low = token(0) + 1 - it.start;
+  for (int a = 0; a < RPT; ++a) lim[a] = token(min(ty * RPT + a, rows - 1)) + 1 - it.start;
+  const int keys = token(rows - 1) + 1 - it.start, low = token(0) + 1 - it.start;
   float o[RPT][DP], m[RPT], l[RPT];
 #pragma unroll
   for (int a = 0; a < RPT; ++a) {
@@ -332,9 +349,9 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
   }
 #pragma unroll
   for (int a = 0; a < RPT; ++a) {
-    const int r = ty * RPT + a, row = it.row0 + r;
-    if (r < it.rows) {
-      T* out = static_cast<T*>(p.out) + (size_t(it.lo + row / G - p.first) * p.hq + kvh * G + row % G) * HD;
+    const int r = ty * RPT + a;
+    if (r < rows) {
+      T* out = static_cast<T*>(p.out) + (size_t(token(r) - p.first) * p.hq + head0 + r % p.gs) * HD;
 #pragma unroll
       for (int d = 0; d < DP; ++d) out[tx + 16 * d] = from_f<T>(l[a] == 0.f ? 0.f : o[a][d] / l[a]);
     }
@@ -342,18 +359,19 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Tiles on the tensor cores (bf16, head dim 64 or 128), one item a CTA, key
-// tiles of 128. Two streams share the ring of K and V tiles, each with an MMA
+// Tiles on the tensor cores (bf16, head dim 64 or 128), key tiles of 128. Two streams share the ring of K and V tiles, each with an MMA
 // warp, a softmax warpgroup (a row a thread) and its own tensor memory:
 //   MT 2: stream x has rows 128 x .. of the item's 256 and their keys, so a
 //         K/V byte brought in from L2 serves 256 rows;
 //   MT 1: both have the item's 128 rows, stream x the key tiles t = x mod 2,
 //         and the streams are joined at the end.
 // One stream's softmax runs under the other's and under the MMAs:
-//   warp 0 loads (TMA, 128 keys x 64 dims boxes, 128-byte swizzle), warps 1
-//   and 2 issue S = Q K^T and O += P V of their stream, warps 4-7 and 8-11
-//   turn S into P, with the registers that warps 0-3 hand over (56 and 224 of
-//   168 a thread at launch).
+//   warp 0 loads (TMA, 128-byte swizzle: boxes of 128 keys x 64 dims, and of a
+//   tile's tokens x heads x 64 dims), warps 1 and 2 issue S = Q K^T and O += P V
+//   of their stream, warps 4-7 and 8-11 turn S into P, with the registers that
+//   warps 0-3 hand over (56 and 224 of 168 a thread at launch).
+// A CTA an SM takes items in turn, which warp 3 finds two ahead: the next
+// item's Q, K and V are loaded, and its first S made, under the end of the last.
 // P is bf16 in tensor memory, the A operand of P V; for head dim 128, where S
 // and O fill the 512 columns, it takes the place of its S, and the stream's
 // next S waits for the P V that reads it. V is read as it lies (N-major B).
@@ -368,15 +386,17 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 // ---------------------------------------------------------------------------
 constexpr int kPaTcKeys = 128;
 constexpr int kPaTcThreads = 384;
-constexpr int kPaCubic = 4;  // of 16 pairs of exponentials, on the fp32 pipe
+constexpr int kPaCubic = 2;  // of 16 pairs of exponentials, on the fp32 pipe
 
 template <int HD, int MT>
 struct PaTcCfg {
+  static constexpr int kRows = 128 * MT;
   static constexpr int kSubs = HD / 64;
-  static constexpr uint32_t kTile = kSubs * kTcSub;  // a K, V or Q tile
-  // ring of K and V tiles: what 224 KB leave beside Q (at most six of each)
-  static constexpr int kRing = HD == 128 ? 7 - MT : 12;
-  static constexpr uint32_t kOffRing = MT * kTile;
+  static constexpr uint32_t kTile = kSubs * kTcSub;  // a K or V tile
+  static constexpr uint32_t kQSub = kRows * 128;     // 64 dims of the Q rows
+  // ring of K and V tiles: what 224 KB leave beside Q
+  static constexpr int kRing = HD == 128 ? 5 : 12;
+  static constexpr uint32_t kOffRing = kSubs * kQSub;
   static constexpr size_t kSmem = size_t(kOffRing) + kRing * kTile + 1024;
   static constexpr bool kAlias = HD == 128;  // P in the place of S
   static constexpr uint32_t kS = 128;        // columns from stream to stream of S; of O: HD
@@ -387,23 +407,43 @@ struct PaTcCfg {
       (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 };
 
+// A place in a ring of N barriers and its phase.
+template <int N>
+struct PaSlot {
+  int i = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+__device__ __forceinline__ void st_v8(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 template <int HD, int MT>
 __global__ void __launch_bounds__(kPaTcThreads, 1)
-    pa_tc_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    pa_tc_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v) {
   using C = PaTcCfg<HD, MT>;
-  constexpr int NB = C::kRing, ROWS = 128 * MT;
-  constexpr uint64_t kBudget = 2000000000ull;
+  constexpr int NB = C::kRing;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[NB], empty[NB], qfull, s_full[2], s_free[2], p_full[2][2], pv_done[2], drain[2], turn[2][4];
+  __shared__ uint64_t full[NB], empty[NB], q_full, q_empty, item_full[2], item_empty[2];
+  __shared__ uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2], o_free[2], drain[2];
   __shared__ uint32_t tmem_base;
-  __shared__ int abort_sh, odd_sh;  // odd_sh: values of V were zeroed
-  __shared__ float2 ml_sh[128];  // MT 1: stream 1's statistics
-  __shared__ PaItem it_sh;
+  __shared__ int abort_sh;
+  __shared__ int odd_sh[2];  // by the item's parity: its number + 1 when values of V were zeroed
+  __shared__ float2 ml_sh[2][MT == 1 ? 128 : 1];  // MT 1: stream 1's statistics, by the item's parity
+  __shared__ PaItem items[2];
   volatile int* abort = &abort_sh;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
-  const int G = p.hq / p.hkv, kvh = blockIdx.x % p.hkv;
   pdl_launch();
   pdl_wait();
   if (warp == 3) {
@@ -411,43 +451,46 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
                  "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  } else if (warp == 0) {
-    const PaItem mine = pa_item<ROWS>(p, blockIdx.x / p.hkv);
-    if (lane == 0) it_sh = mine;
-  } else if (threadIdx.x == 32) {
+  } else if (threadIdx.x == 0) {
     for (int s = 0; s < NB; ++s) {
       mbar_init(full + s, 1);
       mbar_init(empty + s, MT);  // each stream that reads the tile
     }
-    mbar_init(&qfull, 8);
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 2);
     for (int x = 0; x < 2; ++x) {
+      mbar_init(item_full + x, 1);
+      mbar_init(item_empty + x, 11);  // warps 0 to 2 and the softmax's
       mbar_init(s_full + x, 1);
       mbar_init(s_free + x, 4);
       for (int h = 0; h < 2; ++h) mbar_init(&p_full[x][h], 4);
       mbar_init(pv_done + x, 1);
+      mbar_init(o_free + x, 4);
       mbar_init(drain + x, 1);
-      for (int q = 0; q < 4; ++q) mbar_init(&turn[x][q], 1);
+      odd_sh[x] = 0;
     }
     *abort = 0;
-    odd_sh = 0;
     mbar_init_fence();
+  } else if (warp >= 4) {  // rows that no copy of Q writes (those behind tt * gs) stay zeros
+    const int used = p.tt * p.gs, left = (C::kRows - used) * 8;
+    for (int i = threadIdx.x - 128; i < left * C::kSubs; i += kPaTcThreads - 128)
+      *reinterpret_cast<uint4*>(smem + (i / left) * C::kQSub + used * 128 + (i % left) * 16) = make_uint4(0, 0, 0, 0);
+    fence_async_smem();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
-  const PaItem it = it_sh;
-  // keys of the prompt that row r of the tile sees
-  auto seen = [&](int r) { return it.lo + (it.row0 + r) / G + 1 - it.start; };
-  const int keys = it.rows > 0 ? seen(it.rows - 1) : 0;
-  // tiles of stream x: first, step, and how many
-  constexpr int kStep = MT == 2 ? 1 : 2;
-  const int nt = (keys + kPaTcKeys - 1) / kPaTcKeys;
-  auto tiles_of = [&](int x) {
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_lean(bar, parity & 1u, abort); };
+  // keys that the item's tile sees; key tiles of stream x (all of them in turn, or MT 1: every second)
+  auto keys_of = [&](const PaItem& it) { return it.tok0 + it.ntok - it.start; };
+  auto tiles_of = [&](const PaItem& it, int x) {
+    const int nt = (keys_of(it) + kPaTcKeys - 1) / kPaTcKeys;
     if (MT == 1) return (nt - x + 1) / 2;
-    return it.rows > 128 * x ? (seen(min(it.rows, 128 * x + 128) - 1) + kPaTcKeys - 1) / kPaTcKeys : 0;
+    if (x == 1) return it.ntok * p.gs > 128 ? nt : 0;
+    const int last = min(it.ntok * p.gs, 128) - 1;  // of the stream's rows
+    return (it.tok0 + last / p.gs + 1 - it.start + kPaTcKeys - 1) / kPaTcKeys;
   };
-
   // the end of every role: nobody uses tensor or shared memory any more
   auto leave = [&]() {
     tc_fence_before();
@@ -460,300 +503,390 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
     }
   };
 
-  if (it.rows <= 0) {
-    pa_zero<bf16>(p, it, kvh, HD, kPaTcThreads);
-    leave();
-  } else if (warp < 4) {
+  if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0) {
-      int issued = 0;  // ring entries whose copies were issued
-      for (int i = 0; i < 2 * nt; ++i) {  // K and V of each tile in turn
-        const int s = i % NB, j = it.start + (i >> 1) * kPaTcKeys;
-        const bool ok = i < NB || mbar_wait_soon(empty + s, uint32_t((i / NB) & 1) ^ 1u, kBudget, abort);
-        if (!__all_sync(0xffffffffu, ok)) {
+    if (warp == 3) {
+      // ---- items: tiles blockIdx, and then every gridDim-th, the direction
+      // reversed each time (the numbers go by falling cost)
+      PaTiles tiles;
+      tiles.open(p);
+      bool more = true;
+      for (int n = 0; more; ++n) {
+        const long long at = (long long)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        PaItem it = tiles.find(p, int(min(at / p.planes, 0x7FFFFFFFll)));
+        it.plane = int(at % p.planes);
+        more = it.ntok > 0;
+        if (n >= 2 && !__all_sync(0xffffffffu, wait(item_empty + (n & 1), (n >> 1) - 1))) {
           *abort = 1;
           break;
         }
-        if (elect_one()) {
-          mbar_arrive_expect_tx(full + s, C::kTile);
-#pragma unroll
-          for (int b = 0; b < C::kSubs; ++b)
-            tma_load_3d(base + C::kOffRing + s * C::kTile + b * kTcSub, i & 1 ? &map_v : &map_k, b * 64, j, kvh, full + s);
-        }
-        issued = i + 1;
-      }
-      // copies in flight land before the memory goes away
-      int never = 0;
-      for (int i = max(0, issued - NB); i < issued; ++i) mbar_wait(full + i % NB, uint32_t((i / NB) & 1), kBudget, &never);
-    } else if (warp < 3) {
-      // ---- MMA issue of stream x
-      const int x = warp - 1, first = MT == 2 ? 0 : x, mine = tiles_of(x);
-      const uint64_t dq = tc_smem_desc(base + (MT == 2 ? x : 0) * C::kTile);
-      const uint32_t ts = tmem + x * C::kS, to = tmem + C::kO + x * HD, tp = tmem + C::kP + x * C::kPStep;
-      auto wait = [&](uint64_t* bar, int phase) {
-        return __all_sync(0xffffffffu, mbar_wait_soon(bar, uint32_t(phase & 1), kBudget, abort));
-      };
-      auto qk = [&](int k) {
-        const int i = 2 * (first + k * kStep), s = i % NB;
-        // S is free: read by the softmax, and (aliased) its P read by P V
-        if (!wait(full + s, i / NB) || (k > 0 && !wait(C::kAlias ? pv_done + x : s_free + x, k - 1))) return false;
-        tc_fence_after();
-        const uint64_t dk = tc_smem_desc(base + C::kOffRing + s * C::kTile);
-        if (elect_one()) {
-#pragma unroll
-          for (int q = 0; q < HD / 16; ++q) {
-            const uint32_t off = ((q >> 2) * kTcSub + (q & 3) * 32) >> 4;
-            tc_mma(ts, dq + off, dk + off, C::kIdescS, q > 0 ? 1u : 0u);
-          }
-          tc_commit(s_full + x);
-          tc_commit(empty + s);
+        if (lane == 0) {
+          items[n & 1] = it;
+          mbar_arrive(item_full + (n & 1));
         }
         __syncwarp();
-        return true;
+      }
+      tiles.find(p, 0x7FFFFFFF);
+      pa_zero<bf16>(p, tiles, HD, blockIdx.x, gridDim.x);
+    } else if (elect_one()) {
+      // The item of number n, or none: one thread's.
+      auto item = [&](int n, PaItem* it) {
+        if (!wait(item_full + (n & 1), n >> 1)) {
+          *abort = 1;
+          return false;
+        }
+        *it = items[n & 1];
+        mbar_arrive(item_empty + (n & 1));
+        return it->ntok > 0;
       };
-      auto pv = [&](int k) {
-        const int i = 2 * (first + k * kStep) + 1, s = i % NB;
-        if (!wait(full + s, i / NB)) return false;
-        const uint64_t dv = tc_smem_desc_mn(base + C::kOffRing + s * C::kTile, kTcSub);
+      PaItem it;
+      bool ok = true;
+      if (warp == 0) {
+        PaSlot<NB> at;
+        int issued = 0, queries = 0;
+        for (int n = 0; ok && item(n, &it); ++n) {
+          const int nt = (keys_of(it) + kPaTcKeys - 1) / kPaTcKeys, kvh = it.plane / p.subs;
+          for (int i = 0; ok && i < 2 * nt; ++i) {  // K and V of each tile in turn
+            ok = issued < NB || wait(empty + at.i, at.phase ^ 1u);
+            if (!ok) break;
+            mbar_arrive_expect_tx(full + at.i, C::kTile);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // the first half of the keys under the second half's exponentials
-          if (!wait(&p_full[x][h], k)) return false;
-          tc_fence_after();
-          const uint32_t acc = h > 0 || k > 0 ? 1u : 0u;
-          if (elect_one()) {
+            for (int b = 0; b < C::kSubs; ++b)
+              tma_load_3d(base + C::kOffRing + at.i * C::kTile + b * kTcSub, i & 1 ? &map_v : &map_k, b * 64,
+                          it.start + (i >> 1) * kPaTcKeys, kvh, full + at.i);
+            at.next();
+            if (issued < NB) ++issued;
+            if (i == 0) {  // Q: when the item before has made its last S
+              ok = n == 0 || wait(&q_empty, n - 1);
+              if (!ok) break;
+              ++queries;
+              mbar_arrive_expect_tx(&q_full, uint32_t(p.tt * p.gs) * 128 * C::kSubs);
 #pragma unroll
-            for (int q = 4 * h; q < 4 * h + 4; ++q)
-              tc_mma_ta(to, tp + q * 8, dv + ((q * 2048) >> 4), C::kIdescO, q > 4 * h ? 1u : acc);
-            if (h == 1) {
-              tc_commit(pv_done + x);
-              tc_commit(empty + s);
+              for (int b = 0; b < C::kSubs; ++b)
+                tma_load_3d(base + b * C::kQSub, &map_q, b * 64, it.plane * p.gs, it.tok0 - p.first, &q_full);
             }
           }
-          __syncwarp();
+          if (!ok) *abort = 1;
         }
-        return true;
-      };
-      bool ok = mine == 0 || wait(&qfull, 0);
-      if (C::kAlias) {
-        for (int k = 0; ok && k < mine; ++k) ok = qk(k) && pv(k);
-      } else {  // the next S under this one's softmax
-        if (ok && mine > 0) ok = qk(0);
-        for (int k = 0; ok && k < mine; ++k) {
-          if (k + 1 < mine) ok = qk(k + 1);
-          ok = ok && pv(k);
+        // copies in flight land before the memory goes away: those of the last round of the ring, and Q
+        int never = 0;
+        if (issued < NB)
+          at = PaSlot<NB>();
+        else
+          at.phase ^= 1u;
+        for (int i = 0; i < issued; ++i) {
+          mbar_wait_lean(full + at.i, at.phase, &never);
+          at.next();
         }
+        if (queries > 0) mbar_wait_lean(&q_full, uint32_t(queries - 1) & 1u, &never);
+      } else {
+        // ---- MMA issue of stream x, by one thread
+        const int x = warp - 1;
+        const uint64_t dq = tc_smem_desc(base + (MT == 2 ? x : 0) * 128 * 128);
+        const uint32_t ts = tmem + x * C::kS, to = tmem + C::kO + x * HD, tp = tmem + C::kP + x * C::kPStep;
+        PaSlot<NB> ks, vs;  // of the next K and V tile of the item's
+        vs.next();
+        auto skip = [&](PaSlot<NB>& sl, int entries) {
+          for (int e = 0; e < entries; ++e) sl.next();
+        };
+        auto landed = [&](const PaSlot<NB>& sl) { return wait(full + sl.i, sl.phase); };
+        uint32_t kk = 0;  // tiles so far
+        auto qk = [&]() {
+          const uint64_t dk = tc_smem_desc(base + C::kOffRing + ks.i * C::kTile);
+          tc_fence_after();
+#pragma unroll
+          for (int q = 0; q < HD / 16; ++q)
+            tc_mma(ts, dq + (((q >> 2) * C::kQSub + (q & 3) * 32) >> 4), dk + (((q >> 2) * kTcSub + (q & 3) * 32) >> 4),
+                   C::kIdescS, q > 0 ? 1u : 0u);
+          tc_commit(s_full + x);
+          tc_commit(empty + ks.i);
+        };
+        auto pv = [&](bool first, int h) {  // the first half of the keys under the second half's exponentials
+          const uint64_t dv = tc_smem_desc_mn(base + C::kOffRing + vs.i * C::kTile, kTcSub);
+          tc_fence_after();
+#pragma unroll
+          for (int q = 4 * h; q < 4 * h + 4; ++q)
+            tc_mma_ta(to, tp + q * 8, dv + ((q * 2048) >> 4), C::kIdescO, q > 0 || !first ? 1u : 0u);
+          if (h == 1) {
+            tc_commit(pv_done + x);
+            tc_commit(empty + vs.i);
+          }
+        };
+        // entries of the ring from one tile of the stream to its next
+        constexpr int kStep = MT == 2 ? 2 : 4;
+        for (int n = 0; ok && item(n, &it); ++n) {
+          const int nt = (keys_of(it) + kPaTcKeys - 1) / kPaTcKeys, mine = tiles_of(it, x);
+          int left = 2 * nt;  // entries of the item that ks has not passed
+          auto pass = [&](int entries) {
+            skip(ks, entries);
+            skip(vs, entries);
+            left -= entries;
+          };
+          if (MT == 1 && x == 1) pass(2);
+          ok = wait(&q_full, n) && (mine == 0 || landed(ks));
+          // S is free: the softmax has read the item before's
+          if (!C::kAlias && mine > 0 && kk > 0) ok = ok && wait(s_free + x, kk - 1);
+          if (ok && mine > 0) qk();
+          if (ok && mine <= 1) {
+            if (mine == 1)
+              tc_commit(&q_empty);
+            else
+              mbar_arrive(&q_empty);
+          }
+          for (int k = 0; ok && k < mine; ++k, ++kk) {
+            const bool more = k + 1 < mine;
+            if (more) skip(ks, kStep);
+            if (!C::kAlias && more) {  // the next S under this one's softmax, which has read its own
+              ok = landed(ks) && wait(s_free + x, kk);
+              if (ok) {
+                qk();
+                if (k + 2 == mine) tc_commit(&q_empty);
+              }
+            }
+            ok = ok && landed(vs) && (k > 0 || n == 0 || wait(o_free + x, n - 1)) && wait(&p_full[x][0], kk);
+            if (ok) pv(k == 0, 0);
+            if (C::kAlias && more) ok = ok && landed(ks);
+            ok = ok && wait(&p_full[x][1], kk);
+            if (ok) pv(k == 0, 1);
+            if (C::kAlias && more && ok) {
+              // S takes the place of the P that the MMAs before it read: one thread's MMAs run in order
+              qk();
+              if (k + 2 == mine) tc_commit(&q_empty);
+            }
+            if (more) skip(vs, kStep);
+          }
+          // on to the next item's entries, past those that this stream does not read
+          if (mine > 0) left -= (mine - 1) * kStep;
+          if (MT == 2) {
+            if (mine > 0) {
+              skip(ks, 2);
+              skip(vs, 2);
+              left -= 2;
+            }
+            for (; ok && left > 0; left -= 2) {  // the other stream's tiles
+              ok = landed(ks) && landed(vs);
+              if (ok) {
+                mbar_arrive(empty + ks.i);
+                mbar_arrive(empty + vs.i);
+              }
+              skip(ks, 2);
+              skip(vs, 2);
+            }
+          } else {
+            skip(ks, left);
+            skip(vs, left);
+          }
+        }
+        if (!ok) *abort = 1;
+        int never = 0;
+        tc_commit(drain + x);  // behind every MMA of the thread
+        mbar_wait_lean(drain + x, 0u, &never);
       }
-      if (MT == 2)  // the other stream's tiles, which this one does not read
-        for (int i = 2 * mine; ok && i < 2 * nt; ++i) {
-          ok = wait(full + i % NB, i / NB);
-          if (ok && lane == 0) mbar_arrive(empty + i % NB);
-        }
-      if (!ok) *abort = 1;
-      // behind every MMA of the warp (a commit follows those of its own thread:
-      // the elected lane is the same each time)
-      int never = 0;
-      if (elect_one()) tc_commit(drain + x);
-      __syncwarp();
-      mbar_wait(drain + x, 0u, kBudget, &never);
     }
     leave();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ---- softmax of stream x
-    const int stid = int(threadIdx.x) - 128, x = stid >> 7;
+    const int x = (int(threadIdx.x) - 128) >> 7;
     const int quarter = warp & 3, r = quarter * 32 + lane;
-    {  // Q: a warp's rows, whole rows side by side in the lanes, all loads in flight at once
-      constexpr int RW = 16 * MT, CH = HD / 8, RI = 32 / CH, N = RW / RI;  // rows a warp, chunks a row, rows a load
-      const int row0 = (warp - 4) * RW, at = row0 + (lane & (RW - 1));
-      unsigned long long off = ~0ull;  // of row `at` in q
-      if (at < it.rows) {
-        const int row = it.row0 + at, t = row / G;
-        off = (it.lo + t - p.first) * p.q_ts + (kvh * G + row - t * G) * p.q_hs;
-      }
-      uint4 v[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const unsigned long long o = __shfl_sync(0xffffffffu, off, i * RI + lane / CH);
-        v[i] = o != ~0ull ? ld_vec(static_cast<const bf16*>(p.q) + o + (lane % CH) * 8) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int row = row0 + i * RI + lane / CH, c = lane % CH;
-        *reinterpret_cast<uint4*>(smem + (row >> 7) * C::kTile + (c >> 3) * kTcSub + (row & 127) * 128 +
-                                  (((c & 7) ^ (row & 7)) << 4)) = v[i];
-      }
-    }
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&qfull);
     const uint32_t trow = tmem + (uint32_t(quarter * 32) << 16);
     const uint32_t ts = trow + x * C::kS, to = trow + C::kO + x * HD, tp = trow + C::kP + x * C::kPStep;
     const int row = MT == 2 ? x * 128 + r : r;
-    const bool write = row < it.rows;
-    const int lim = write ? seen(row) : keys;  // keys [0, lim) are seen
-    const int low = seen(0);  // keys [0, low) are seen by all
-    const int mine = tiles_of(x), others = tiles_of(1 - x);
     const float sl2 = p.scale * kLog2e;
-    float m = -INFINITY, l = 0.f;  // reference max (scaled, base 2), sum
+    uint32_t entry = 0;  // of the ring, counted on: the item's first K tile
+    uint32_t kk = 0;  // tiles so far
     bool ok = true;
-    int k = 0;
-    for (; k < mine; ++k) {
-      const int t = MT == 2 ? k : 2 * k + x, j = t * kPaTcKeys;
-      ok = mbar_wait_soon(s_full + x, uint32_t(k & 1), kBudget, abort);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      float sc[kPaTcKeys];
-#pragma unroll
-      for (int c = 0; c < kPaTcKeys; c += 32) tc_ld32(ts + c, reinterpret_cast<uint32_t*>(sc + c));
-      tc_wait_ld();
-      if (!C::kAlias) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free + x);
+    for (int n = 0;; ++n) {
+      ok = ok && wait(item_full + (n & 1), n >> 1);
+      if (!__all_sync(0xffffffffu, ok)) ok = false;
+      if (!ok || items[n & 1].ntok == 0) {
+        if (!ok) *abort = 1;
+        // (MT 1: a warp whose wait ran out and one at the end, or with the item, meet at one barrier)
+        if (MT == 1) named_sync_and(1, 256, false);
+        break;
       }
-      const bool masked = __any_sync(0xffffffffu, j + kPaTcKeys > lim);
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < kPaTcKeys; ++c) sc[c] = j + c < lim ? sc[c] : -INFINITY;
+      int lim, low, keys, mine;  // keys [0, lim) are seen by the row, [0, low) by all, [0, keys) by one
+      {
+        const PaItem it = items[n & 1];
+        keys = keys_of(it);
+        mine = tiles_of(it, x);
+        lim = row < it.ntok * p.gs ? it.tok0 + row / p.gs + 1 - it.start : keys;
+        low = it.tok0 + 1 - it.start;
       }
-      float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
-#pragma unroll
-      for (int c = 4; c < kPaTcKeys - 4; c += 8)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = max3_nan(mx[i], sc[c + i], sc[c + 4 + i]);
-      mx[0] = max3_nan(mx[0], sc[124], sc[125]);
-      mx[1] = max3_nan(mx[1], sc[126], sc[127]);
-      const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sl2;
-      const bool grow = !(top <= m + 8.f);  // (NaN stays: exp2_cubic would lose it)
-      if (!C::kAlias && k > 0) {  // the stream's previous P V has read P (aliased: it came before this S)
-        ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
+      float m = -INFINITY, l = 0.f;  // reference max (scaled, base 2), sum
+      for (int k = 0; k < mine; ++k, ++kk) {
+        const int t = MT == 2 ? k : 2 * k + x, j = t * kPaTcKeys;
+        ok = wait(s_full + x, kk);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-        const float a = grow ? exp2_approx(m - top) : 1.f;
-        if (grow) m = top;
-        l *= a;
-        if (k > 0) {
+        float sc[kPaTcKeys];
 #pragma unroll
-          for (int c = 0; c < HD; c += 16) {
-            uint32_t o[16];
-            tc_ld16(to + c, o);
-            tc_wait_ld();
+        for (int c = 0; c < kPaTcKeys; c += 32) tc_ld32(ts + c, reinterpret_cast<uint32_t*>(sc + c));
+        tc_wait_ld();
+        if (!C::kAlias) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free + x);
+        }
+        const bool masked = __any_sync(0xffffffffu, j + kPaTcKeys > lim);
+        if (masked) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-            tc_st16(to + c, o);
+          for (int c = 0; c < kPaTcKeys; ++c) sc[c] = j + c < lim ? sc[c] : -INFINITY;
+        }
+        float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+        for (int c = 4; c < kPaTcKeys - 4; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = max3_nan(mx[i], sc[c + i], sc[c + 4 + i]);
+        mx[0] = max3_nan(mx[0], sc[124], sc[125]);
+        mx[1] = max3_nan(mx[1], sc[126], sc[127]);
+        const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sl2;
+        const bool grow = !(top <= m + 8.f);  // (NaN stays: exp2_cubic would lose it)
+        if (!C::kAlias && k > 0) {  // the stream's previous P V has read P (aliased: it came before this S)
+          ok = wait(pv_done + x, kk - 1);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          tc_fence_after();
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+          const float a = grow ? exp2_approx(m - top) : 1.f;
+          if (grow) m = top;
+          l *= a;
+          if (k > 0) {
+#pragma unroll
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t o[16];
+              tc_ld16(to + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+              tc_st16(to + c, o);
+            }
           }
         }
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-      if (j + kPaTcKeys > low) {  // V rows behind the keys, or not seen by all (MT 2: both streams write the same zeros)
-        const int i = 2 * t + 1, s = i % NB;
-        ok = mbar_wait_soon(full + s, uint32_t((i / NB) & 1), kBudget, abort);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        tc_clean_row<HD>(smem + C::kOffRing + s * C::kTile, r, j + r >= keys, j + r >= low, &odd_sh);
-        fence_async_smem();
-      }
-      // the exponentials of the two warps of a scheduler take turns: one stream's
-      // run under the other's MMAs, and not both at half pace
-      if (x == 1 ? k < others : k > 0 && k - 1 < others) {
-        ok = mbar_wait_soon(&turn[x][quarter], uint32_t(x == 1 ? k & 1 : (k - 1) & 1), kBudget, abort);
-        if (!__all_sync(0xffffffffu, ok)) break;
-      }
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      // kCubic of 16 pairs on the fp32 pipe, which the special-function unit
-      // (8 cycles a warp and value) leaves idle; masked tiles need exact zeros
-      auto exps = [&](auto cubic) {
-        constexpr int kCubic = decltype(cubic)::value;
+        const float ref = m == -INFINITY ? 0.f : m;
+        if (j + kPaTcKeys > low) {  // V rows behind the keys, or not seen by all (MT 2: both streams write the same zeros)
+          const uint32_t e = entry + 2 * t + 1, s = e % NB;
+          ok = wait(full + s, e / NB);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          tc_clean_row<HD>(smem + C::kOffRing + s * C::kTile, r, j + r >= keys, j + r >= low, odd_sh + (n & 1), n + 1);
+          fence_async_smem();
+        }
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // kCubic of 16 pairs on the fp32 pipe, which the special-function unit
+        // (8 cycles a warp and value) leaves idle; masked tiles need exact zeros
+        auto exps = [&](auto cubic) {
+          constexpr int kCubic = decltype(cubic)::value;
 #pragma unroll
-        for (int c = 0; c < kPaTcKeys; c += 32) {
-          uint32_t pk[16];
+          for (int c = 0; c < kPaTcKeys; c += 32) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float2 e = fma2(make_float2(sc[c + i], sc[c + i + 1]), make_float2(sl2, sl2), make_float2(-ref, -ref));
-            if ((i >> 1) * kCubic % 16 < kCubic) {
-              e = exp2_cubic(e);
-            } else {
-              e.x = exp2_approx(e.x);
-              e.y = exp2_approx(e.y);
+            for (int i = 0; i < 32; i += 2) {
+              float2 e = fma2(make_float2(sc[c + i], sc[c + i + 1]), make_float2(sl2, sl2), make_float2(-ref, -ref));
+              if ((i >> 1) * kCubic % 16 < kCubic) {
+                e = exp2_cubic(e);
+              } else {
+                e.x = exp2_approx(e.x);
+                e.y = exp2_approx(e.y);
+              }
+              sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+              pk[i / 2] = pack_bf16(e.x, e.y);
             }
-            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
-            pk[i / 2] = pack_bf16(e.x, e.y);
+            if (c == 64) {  // the first half of the keys: its stores have landed meanwhile
+              tc_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[x][0]);
+            }
+            tc_st16(tp + c / 2, pk);
           }
-          if (c == 64) {  // the first half of the keys: its stores have landed meanwhile
-            tc_wait_st();
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[x][1]);
+        };
+        if (masked)
+          exps(std::integral_constant<int, 0>{});
+        else
+          exps(std::integral_constant<int, kPaCubic>{});
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
+      }
+      if (ok && mine > 0) ok = wait(pv_done + x, kk - 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        *abort = 1;
+      }
+      tc_fence_after();
+      float wb = 0.f, wa = 1.f;
+      if (MT == 1) {
+        if (x == 1) ml_sh[n & 1][r] = make_float2(m, l);
+        tc_fence_before();
+        ok = named_sync_and(1, 256, ok);
+        tc_fence_after();
+        const float2 b = ml_sh[n & 1][r];
+        // (a NaN sum of either stream makes the whole sum NaN)
+        const float top = fmaxf(m, b.x), ref = top == -INFINITY ? 0.f : top;
+        wa = exp2_approx(m - ref);
+        wb = exp2_approx(b.x - ref);
+        l = l * wa + b.y * wb;
+      }
+      if (!ok) break;
+      if (MT == 2 || x == 0) {
+        const PaItem it = items[n & 1];
+        const bool write = row < it.ntok * p.gs, two = MT == 1 && keys > kPaTcKeys;
+        const int tok = it.tok0 + row / p.gs;
+        const bool odd = *static_cast<volatile int*>(odd_sh + (n & 1)) == n + 1;
+        const float inv = 1.f / l;
+        bf16* out = static_cast<bf16*>(p.out) + (size_t(tok - p.first) * p.hq + it.plane * p.gs + row % p.gs) * HD;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          float f[32];
+          if (mine > 0) {
+            uint32_t o1[32];
+            tc_ld32(to + c, reinterpret_cast<uint32_t*>(f));
+            if (two) tc_ld32(to + HD + c, o1);
+            tc_wait_ld();
+            if (MT == 1) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                f[e] *= wa;
+                if (two) f[e] = fmaf(__uint_as_float(o1[e]), wb, f[e]);
+              }
+            }
+          }
+          if (c == HD - 32) {  // O may be written again
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[x][0]);
+            if (lane == 0) {
+              mbar_arrive(o_free + x);
+              if (MT == 1) mbar_arrive(o_free + 1);
+            }
           }
-          tc_st16(tp + c / 2, pk);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&turn[1 - x][quarter]);
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x][1]);
-      };
-      if (masked)
-        exps(std::integral_constant<int, 0>{});
-      else
-        exps(std::integral_constant<int, kPaCubic>{});
-      sum[0] = add2(sum[0], sum[1]);
-      l += sum[0].x + sum[0].y;
-    }
-    if (ok && k > 0) ok = mbar_wait_soon(pv_done + x, uint32_t((k - 1) & 1), kBudget, abort);
-    if (!ok) *abort = 1;
-    tc_fence_after();
-    float wb = 0.f, wa = 1.f;
-    if (MT == 1) {
-      if (x == 1) ml_sh[r] = make_float2(k > 0 ? m : -INFINITY, l);
-      tc_fence_before();
-      named_sync(1, 256);
-      tc_fence_after();
-      const float2 b = ml_sh[r];
-      // (a NaN max or sum of either stream makes both weights, or the sum, NaN)
-      const float top = max3_nan(m, b.x, b.x), ref = top == -INFINITY ? 0.f : top;
-      wa = exp2_approx(m - ref);
-      wb = exp2_approx(b.x - ref);
-      l = l * wa + b.y * wb;
-    }
-    if ((MT == 2 || x == 0) && __any_sync(0xffffffffu, write)) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const bool odd = *static_cast<volatile int*>(&odd_sh) != 0, two = MT == 1 && nt > 1;
-      const int tok = it.lo + (it.row0 + row) / G, head = kvh * G + (it.row0 + row) % G;
-      bf16* out = static_cast<bf16*>(p.out) + (size_t(tok - p.first) * p.hq + head) * HD;
+          if (write) {
+            if (odd) {  // what was taken out of V
+              const bf16* v = static_cast<const bf16*>(p.v) + (it.plane / p.subs) * p.v_hs + it.start * p.v_ts + c;
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 16) {
-        uint32_t o0[16], o1[16];
-        tc_ld16(to + c, o0);
-        if (two) tc_ld16(to + HD + c, o1);
-        tc_wait_ld();
-        float f[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          f[e] = __uint_as_float(o0[e]) * wa;
-          if (two) f[e] = fmaf(__uint_as_float(o1[e]), wb, f[e]);
-        }
-        if (write) {
-          if (odd) {  // what was taken out of V
-            const bf16* v = static_cast<const bf16*>(p.v) + kvh * p.v_hs + it.start * p.v_ts + c;
-            for (int key = low; key < lim; ++key)
-              for (int e = 0; e < 16; ++e) {
-                const float y = to_f(v[key * p.v_ts + e]);
+              for (int i = low * 32; i < lim * 32; ++i) {
+                const float y = to_f(v[(i >> 5) * p.v_ts + (i & 31)]);
                 if (!(fabsf(y) < INFINITY))
 #pragma unroll
-                  for (int u = 0; u < 16; ++u) f[u] = u == e ? f[u] + y : f[u];
+                  for (int e = 0; e < 32; ++e) f[e] = e == (i & 31) ? f[e] + y : f[e];
               }
-          }
+            }
 #pragma unroll
-          for (int e = 0; e < 16; e += 8)
-            *reinterpret_cast<uint4*>(out + c + e) =
-                l == 0.f ? make_uint4(0, 0, 0, 0)
-                         : make_uint4(pack_bf16(f[e] * inv, f[e + 1] * inv), pack_bf16(f[e + 2] * inv, f[e + 3] * inv),
-                                      pack_bf16(f[e + 4] * inv, f[e + 5] * inv), pack_bf16(f[e + 6] * inv, f[e + 7] * inv));
+            for (int h = 0; h < 32; h += 16) {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                w[e] = l == 0.f ? 0u : pack_bf16(f[h + 2 * e] * inv, f[h + 2 * e + 1] * inv);
+              st_v8(out + c + h, w);
+            }
+          }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_empty + (n & 1));
+      entry += 2 * ((keys + kPaTcKeys - 1) / kPaTcKeys);
     }
     leave();
   }

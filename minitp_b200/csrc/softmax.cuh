@@ -41,10 +41,10 @@ constexpr float kLn2 = 0.69314718055994530942f;
 constexpr uint32_t kTcSub = 128 * 64 * 2;  // a 128 x 64 bf16 subtile
 
 // Row r of a V tile: behind the range it becomes zeros; one that not every
-// token sees loses its NaN and infinities, and *odd tells of them. (A call, to
+// token sees loses its NaN and infinities, and *odd = mark tells of them. (A call, to
 // take no registers from the softmax.)
 template <int HD>
-__device__ __noinline__ void tc_clean_row(unsigned char* tile, int r, bool behind, bool unseen, int* odd) {
+__device__ __noinline__ void tc_clean_row(unsigned char* tile, int r, bool behind, bool unseen, int* odd, int mark = 1) {
   auto at = [&](int i) { return reinterpret_cast<uint4*>(tile + (i >> 3) * kTcSub + r * 128 + (((i ^ r) & 7) << 4)); };
   if (behind) {
 #pragma unroll
@@ -57,7 +57,7 @@ __device__ __noinline__ void tc_clean_row(unsigned char* tile, int r, bool behin
       nan = fma_bf16x2(v.x, 0u, fma_bf16x2(v.y, 0u, fma_bf16x2(v.z, 0u, fma_bf16x2(v.w, 0u, nan))));
     }
     if (nan & 0x7FFF7FFFu) {
-      *static_cast<volatile int*>(odd) = 1;
+      *static_cast<volatile int*>(odd) = mark;
       __threadfence_block();
 #pragma unroll 1
       for (int i = 0; i < HD; ++i) {

@@ -69,6 +69,28 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, u
   return mbar_wait(bar, parity, budget_ns, abort);
 }
 
+// The same in few instructions, for code that is fetched anew each time it
+// runs (a straight-line body of many KB does not stay in the instruction
+// cache): bounded by two million polls, each of which sleeps in hardware for a
+// microsecond at most. After *abort became non-zero it does not wait.
+__device__ __forceinline__ bool mbar_wait_lean(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+  const uint32_t at = smem_u32(bar);
+#pragma unroll 1
+  for (int i = 0; i < 2000000; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(at), "r"(parity), "r"(1000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+  }
+  return false;
+}
+
 // 1-D bulk copy global -> this CTA's shared memory, completing on `bar`.
 // dst and src 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
