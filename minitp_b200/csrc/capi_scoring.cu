@@ -177,6 +177,8 @@ long long pa_items(PaParams* p, int rows) {
   p->gs = G / p->subs;
   p->planes = p->hkv * p->subs;
   p->tt = rows / p->gs;
+  p->tt_mul = ((1ull << 40) + p->tt - 1) / p->tt;
+  p->gs_mul = (65536u + p->gs - 1) / p->gs;
   return ((long long)p->n / p->tt + p->S) * p->planes;
 }
 

@@ -32,10 +32,15 @@ struct PaParams {
   int S, first, n, total, hq, hkv;
   int gs, subs;  // heads of a row group, groups of a KV head: gs * subs = G
   int tt;        // tokens a tile: as many as its rows hold, gs rows each
+  unsigned long long tt_mul;  // ceil(2^40 / tt): n / tt = n * tt_mul >> 40 for n < 2^30
+  uint32_t gs_mul;            // ceil(2^16 / gs), the same for rows of a tile
   int planes;    // hkv * subs
   float scale;
   uint32_t* status;  // error bits
 };
+
+__device__ __forceinline__ int pa_div_tt(const PaParams& p, int n) { return int((unsigned long long)n * p.tt_mul >> 40); }
+__device__ __forceinline__ int pa_div_gs(const PaParams& p, int row) { return int(uint32_t(row) * p.gs_mul >> 16); }
 
 // Set when a bounded wait of a prompt attention ran out (its results are then void).
 __device__ uint32_t g_pa_status;
@@ -48,7 +53,7 @@ struct PaItem {
 };
 
 // Prompts whose tiles are put in order (a lane has its share in registers).
-constexpr int kPaOrdered = 4 * 32;
+constexpr int kPaOrdered = 2 * 32;
 
 // The tiles of all prompts, by one warp, in the order of growing numbers. They
 // are numbered in descending order of their place in their prompt, which is how
@@ -68,9 +73,14 @@ struct PaTiles {
 
   static __device__ __forceinline__ int cut(const PaParams& p, int t) { return min(max(t, 0), p.total); }
 
-  __device__ __forceinline__ Seq load(const PaParams& p, int blk) {  // prompt 32 blk + lane
-    const int lane = threadIdx.x & 31, s = 32 * blk + lane, end = p.first + p.n;
-    int hi = max(at_least, s < p.S ? cut(p, __ldg(p.starts + s + 1)) : 0);
+  // the end of prompt 32 blk + lane (behind the last prompt: 0)
+  static __device__ __forceinline__ int end_of(const PaParams& p, int blk) {
+    const int s = 32 * blk + (threadIdx.x & 31);
+    return s < p.S ? cut(p, __ldg(p.starts + s + 1)) : 0;
+  }
+  __device__ __forceinline__ Seq load(const PaParams& p, int its_end) {
+    const int lane = threadIdx.x & 31, end = p.first + p.n;
+    int hi = max(at_least, its_end);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, hi, o);
@@ -81,24 +91,27 @@ struct PaTiles {
     r.start = lane ? prev : at_least;
     r.lo = max(r.start, p.first);
     r.n = max(0, min(hi, end) - r.lo);
-    r.nt = (r.n + p.tt - 1) / p.tt;
-    r.off = r.n ? (r.lo - r.start) / p.tt : 0;
+    r.nt = pa_div_tt(p, r.n + p.tt - 1);
+    r.off = r.n ? pa_div_tt(p, r.lo - r.start) : 0;
     at_least = __shfl_sync(0xffffffffu, hi, 31);
     return r;
   }
 
   __device__ __forceinline__ void open(const PaParams& p) {
+    int ends[kPaOrdered / 32];  // (all loads in flight at once)
+#pragma unroll
+    for (int i = 0; i < kPaOrdered / 32; ++i) ends[i] = end_of(p, i);
     at_least = cut(p, __ldg(p.starts));
     gap0 = min(max(at_least, p.first), p.first + p.n);
     all = b = most = 0;
     if (p.S > kPaOrdered) {
-      q[0] = load(p, 0);
+      q[0] = load(p, ends[0]);
       return;
     }
 #pragma unroll
     for (int i = 0; i < kPaOrdered / 32; ++i) {
       q[i] = Seq{0, 0, 0, 0, 0};
-      if (32 * i < p.S) q[i] = load(p, i);
+      if (32 * i < p.S) q[i] = load(p, ends[i]);
       if (q[i].nt) most = max(most, q[i].off + q[i].nt);
       all += q[i].nt;
     }
@@ -115,7 +128,8 @@ struct PaTiles {
     return it;
   }
 
-  // Tile number i (no smaller than in the call before); ntok 0 when there is none.
+  // Tile number i (no smaller than in the call before); ntok 0 when there is none. (Few instructions
+  // count: what is fetched here pushes the softmax's out of the instruction cache.)
   __device__ __forceinline__ PaItem find(const PaParams& p, int i) {
     const int lane = threadIdx.x & 31;
     PaItem it{0, 0, 0, 0};
@@ -134,7 +148,7 @@ struct PaTiles {
         }
         if (32 * (b + 1) >= p.S) break;
         all += sum;
-        q[0] = load(p, b + 1);
+        q[0] = load(p, end_of(p, b + 1));
       }
       gap1 = min(max(at_least, p.first), p.first + p.n);
       return it;
@@ -157,10 +171,11 @@ struct PaTiles {
     int left = i - above(lo + 1);  // of the tiles at place lo
 #pragma unroll
     for (int k = 0; k < kPaOrdered / 32; ++k) {
-      const uint32_t m = __ballot_sync(0xffffffffu, q[k].off <= lo && lo < q[k].off + q[k].nt);
+      const bool in = q[k].off <= lo && lo < q[k].off + q[k].nt;
+      const uint32_t m = __ballot_sync(0xffffffffu, in);
       const int c = __popc(m);
       if (left >= 0 && left < c) {
-        const int from = __fns(m, 0, left + 1);
+        const int from = __ffs(__ballot_sync(0xffffffffu, in && __popc(m & ((1u << lane) - 1u)) == left)) - 1;
         it = take(p, from, q[k], lo - __shfl_sync(0xffffffffu, q[k].off, from));
       }
       left -= c;
@@ -217,10 +232,7 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
     PaItem it = tiles.find(p, blockIdx.x / p.planes);
     it.plane = blockIdx.x % p.planes;
     if (tid == 0) it_sh = it;
-    if (blockIdx.x == gridDim.x - 1) {  // (the grid has a CTA more than tiles)
-      it = tiles.find(p, 0x7FFFFFFF);
-      pa_zero<T>(p, tiles, HD, 0, 1);
-    }
+    if (blockIdx.x == gridDim.x - 1) pa_zero<T>(p, tiles, HD, 0, 1);  // (the grid has a CTA more than tiles)
   }
   __syncthreads();
   const PaItem it = it_sh;
@@ -229,13 +241,13 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
   const T* q = static_cast<const T*>(p.q);
   const T* k = static_cast<const T*>(p.k) + kvh * p.k_hs;
   const T* v = static_cast<const T*>(p.v) + kvh * p.v_hs;
-  auto token = [&](int r) { return it.tok0 + r / p.gs; };
+  auto token = [&](int r) { return it.tok0 + pa_div_gs(p, r); };
   for (int i = tid; i < ROWS * (HD / VE); i += kPaThreads) {
     const int r = i / (HD / VE), c = (i - r * (HD / VE)) * VE;
     float f[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) f[e] = 0.f;
-    if (r < rows) unpack(ld_vec(q + (token(r) - p.first) * p.q_ts + (head0 + r % p.gs) * p.q_hs + c), f);
+    if (r < rows) unpack(ld_vec(q + (token(r) - p.first) * p.q_ts + (head0 + r - pa_div_gs(p, r) * p.gs) * p.q_hs + c), f);
 #pragma unroll
     for (int e = 0; e < VE; ++e) sq[r * LD + c + e] = f[e];
   }
@@ -351,7 +363,7 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
   for (int a = 0; a < RPT; ++a) {
     const int r = ty * RPT + a;
     if (r < rows) {
-      T* out = static_cast<T*>(p.out) + (size_t(token(r) - p.first) * p.hq + head0 + r % p.gs) * HD;
+      T* out = static_cast<T*>(p.out) + (size_t(token(r) - p.first) * p.hq + head0 + r - pa_div_gs(p, r) * p.gs) * HD;
 #pragma unroll
       for (int d = 0; d < DP; ++d) out[tx + 16 * d] = from_f<T>(l[a] == 0.f ? 0.f : o[a][d] / l[a]);
     }
@@ -369,7 +381,7 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 //   warp 0 loads (TMA, 128-byte swizzle: boxes of 128 keys x 64 dims, and of a
 //   tile's tokens x heads x 64 dims), warps 1 and 2 issue S = Q K^T and O += P V
 //   of their stream, warps 4-7 and 8-11 turn S into P, with the registers that
-//   warps 0-3 hand over (56 and 224 of 168 a thread at launch).
+//   warps 0-3 hand over.
 // A CTA an SM takes items in turn, which warp 3 finds two ahead: the next
 // item's Q, K and V are loaded, and its first S made, under the end of the last.
 // P is bf16 in tensor memory, the A operand of P V; for head dim 128, where S
@@ -386,7 +398,8 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 // ---------------------------------------------------------------------------
 constexpr int kPaTcKeys = 128;
 constexpr int kPaTcThreads = 384;
-constexpr int kPaCubic = 2;  // of 16 pairs of exponentials, on the fp32 pipe
+template <int HD>
+constexpr int kPaCubic = HD == 128 ? 2 : 4;  // of 16 pairs of exponentials, on the fp32 pipe
 
 template <int HD, int MT>
 struct PaTcCfg {
@@ -398,6 +411,9 @@ struct PaTcCfg {
   static constexpr int kRing = HD == 128 ? 5 : 12;
   static constexpr uint32_t kOffRing = kSubs * kQSub;
   static constexpr size_t kSmem = size_t(kOffRing) + kRing * kTile + 1024;
+  // registers a thread of warps 0-3 and of the softmax (168 at launch): 128 x a + 256 x b = 384 x 168
+  static constexpr int kRegs = HD == 128 ? 72 : 56, kRegsSoftmax = HD == 128 ? 216 : 224;
+  static_assert(128 * kRegs + 256 * kRegsSoftmax <= 384 * 168, "registers handed over");
   static constexpr bool kAlias = HD == 128;  // P in the place of S
   static constexpr uint32_t kS = 128;        // columns from stream to stream of S; of O: HD
   static constexpr uint32_t kO = 256, kP = kAlias ? 0 : 384, kPStep = kAlias ? 128 : 64;
@@ -433,12 +449,12 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
   using C = PaTcCfg<HD, MT>;
   constexpr int NB = C::kRing;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[NB], empty[NB], q_full, q_empty, item_full[2], item_empty[2];
+  __shared__ uint64_t full[NB], empty[NB], raw[NB], q_full, q_empty, item_full[2], item_empty[2];
   __shared__ uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2], o_free[2], drain[2];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_sh;
   __shared__ int odd_sh[2];  // by the item's parity: its number + 1 when values of V were zeroed
-  __shared__ float2 ml_sh[2][MT == 1 ? 128 : 1];  // MT 1: stream 1's statistics, by the item's parity
+  __shared__ float2 ml_sh[MT == 1 ? 2 : 1][2][MT == 1 ? 128 : 1];  // MT 1: by the item's parity and stream, statistics
   __shared__ PaItem items[2];
   volatile int* abort = &abort_sh;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -454,6 +470,7 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
   } else if (threadIdx.x == 0) {
     for (int s = 0; s < NB; ++s) {
       mbar_init(full + s, 1);
+      mbar_init(raw + s, 1);
       mbar_init(empty + s, MT);  // each stream that reads the tile
     }
     mbar_init(&q_full, 1);
@@ -465,7 +482,7 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
       mbar_init(s_free + x, 4);
       for (int h = 0; h < 2; ++h) mbar_init(&p_full[x][h], 4);
       mbar_init(pv_done + x, 1);
-      mbar_init(o_free + x, 4);
+      mbar_init(o_free + x, MT == 1 ? 8 : 4);
       mbar_init(drain + x, 1);
       odd_sh[x] = 0;
     }
@@ -489,7 +506,7 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
     if (MT == 1) return (nt - x + 1) / 2;
     if (x == 1) return it.ntok * p.gs > 128 ? nt : 0;
     const int last = min(it.ntok * p.gs, 128) - 1;  // of the stream's rows
-    return (it.tok0 + last / p.gs + 1 - it.start + kPaTcKeys - 1) / kPaTcKeys;
+    return (it.tok0 + pa_div_gs(p, last) + 1 - it.start + kPaTcKeys - 1) / kPaTcKeys;
   };
   // the end of every role: nobody uses tensor or shared memory any more
   auto leave = [&]() {
@@ -504,29 +521,48 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegs));
     if (warp == 3) {
       // ---- items: tiles blockIdx, and then every gridDim-th, the direction
-      // reversed each time (the numbers go by falling cost)
+      // reversed each time (the numbers go by falling cost). And the V tiles at
+      // an item's end: rows behind its keys become zeros, and of those that not
+      // every row of the item sees the NaN and infinities.
       PaTiles tiles;
       tiles.open(p);
-      bool more = true;
-      for (int n = 0; more; ++n) {
-        const long long at = (long long)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        PaItem it = tiles.find(p, int(min(at / p.planes, 0x7FFFFFFFll)));
-        it.plane = int(at % p.planes);
-        more = it.ntok > 0;
-        if (n >= 2 && !__all_sync(0xffffffffu, wait(item_empty + (n & 1), (n >> 1) - 1))) {
-          *abort = 1;
-          break;
+      PaSlot<NB> at;  // of the item's first K tile
+      uint32_t raws = 0;  // phases of `raw`, a bit each
+      bool ok = true;
+      PaItem it{0, 0, 0, 0};
+#pragma unroll 1
+      for (int n = -1; ok && (n < 0 || it.ntok > 0); ++n) {
+        const long long i = (long long)(n + 1) * gridDim.x + (n & 1 ? blockIdx.x : gridDim.x - 1 - blockIdx.x);
+        PaItem next = tiles.find(p, int(min(i / p.planes, 0x7FFFFFFFll)));
+        next.plane = int(i % p.planes);
+        const int keys = keys_of(it), low = it.tok0 + 1 - it.start, nt = n < 0 ? 0 : (keys + kPaTcKeys - 1) / kPaTcKeys;
+#pragma unroll 1
+        for (int t = 0; ok && t < nt; ++t) {
+          at.next();
+          if ((t + 1) * kPaTcKeys > low) {
+            ok = __all_sync(0xffffffffu, wait(raw + at.i, raws >> at.i));
+            raws ^= 1u << at.i;
+#pragma unroll 1
+            for (int r = max(low - t * kPaTcKeys, 0) + lane; ok && r < kPaTcKeys; r += 32)
+              tc_clean_row<HD>(smem + C::kOffRing + at.i * C::kTile, r, t * kPaTcKeys + r >= keys, true, odd_sh + (n & 1), n + 1);
+            fence_async_smem();
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(full + at.i);
+          }
+          at.next();
         }
-        if (lane == 0) {
-          items[n & 1] = it;
-          mbar_arrive(item_full + (n & 1));
+        if (n >= 1 && ok) ok = __all_sync(0xffffffffu, wait(item_empty + (~n & 1), ((n + 1) >> 1) - 1));
+        if (ok && lane == 0) {
+          items[~n & 1] = next;
+          mbar_arrive(item_full + (~n & 1));
         }
         __syncwarp();
+        it = next;
       }
-      tiles.find(p, 0x7FFFFFFF);
+      if (!ok) *abort = 1;
       pa_zero<bf16>(p, tiles, HD, blockIdx.x, gridDim.x);
     } else if (elect_one()) {
       // The item of number n, or none: one thread's.
@@ -544,16 +580,22 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
       if (warp == 0) {
         PaSlot<NB> at;
         int issued = 0, queries = 0;
+        uint32_t raws = 0, phases = 0;  // slots whose last copy completes on `raw`; the phases of those, a bit each
         for (int n = 0; ok && item(n, &it); ++n) {
           const int nt = (keys_of(it) + kPaTcKeys - 1) / kPaTcKeys, kvh = it.plane / p.subs;
           for (int i = 0; ok && i < 2 * nt; ++i) {  // K and V of each tile in turn
             ok = issued < NB || wait(empty + at.i, at.phase ^ 1u);
             if (!ok) break;
-            mbar_arrive_expect_tx(full + at.i, C::kTile);
+            // V tiles that not every row sees whole go by way of warp 3
+            const bool unseen = (i & 1) && ((i >> 1) + 1) * kPaTcKeys > it.tok0 + 1 - it.start;
+            uint64_t* bar = unseen ? raw + at.i : full + at.i;
+            raws = unseen ? raws | (1u << at.i) : raws & ~(1u << at.i);
+            if (unseen) phases ^= 1u << at.i;
+            mbar_arrive_expect_tx(bar, C::kTile);
 #pragma unroll
             for (int b = 0; b < C::kSubs; ++b)
               tma_load_3d(base + C::kOffRing + at.i * C::kTile + b * kTcSub, i & 1 ? &map_v : &map_k, b * 64,
-                          it.start + (i >> 1) * kPaTcKeys, kvh, full + at.i);
+                          it.start + (i >> 1) * kPaTcKeys, kvh, bar);
             at.next();
             if (issued < NB) ++issued;
             if (i == 0) {  // Q: when the item before has made its last S
@@ -575,7 +617,10 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
         else
           at.phase ^= 1u;
         for (int i = 0; i < issued; ++i) {
-          mbar_wait_lean(full + at.i, at.phase, &never);
+          if (raws >> at.i & 1u)
+            mbar_wait_lean(raw + at.i, (phases >> at.i & 1u) ^ 1u, &never);
+          else
+            mbar_wait_lean(full + at.i, at.phase, &never);
           at.next();
         }
         if (queries > 0) mbar_wait_lean(&q_full, uint32_t(queries - 1) & 1u, &never);
@@ -623,37 +668,37 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
             left -= entries;
           };
           if (MT == 1 && x == 1) pass(2);
-          ok = wait(&q_full, n) && (mine == 0 || landed(ks));
-          // S is free: the softmax has read the item before's
-          if (!C::kAlias && mine > 0 && kk > 0) ok = ok && wait(s_free + x, kk - 1);
-          if (ok && mine > 0) qk();
-          if (ok && mine <= 1) {
-            if (mine == 1)
-              tc_commit(&q_empty);
-            else
-              mbar_arrive(&q_empty);
-          }
-          for (int k = 0; ok && k < mine; ++k, ++kk) {
-            const bool more = k + 1 < mine;
-            if (more) skip(ks, kStep);
-            if (!C::kAlias && more) {  // the next S under this one's softmax, which has read its own
-              ok = landed(ks) && wait(s_free + x, kk);
-              if (ok) {
-                qk();
-                if (k + 2 == mine) tc_commit(&q_empty);
-              }
-            }
-            ok = ok && landed(vs) && (k > 0 || n == 0 || wait(o_free + x, n - 1)) && wait(&p_full[x][0], kk);
-            if (ok) pv(k == 0, 0);
-            if (C::kAlias && more) ok = ok && landed(ks);
-            ok = ok && wait(&p_full[x][1], kk);
-            if (ok) pv(k == 0, 1);
-            if (C::kAlias && more && ok) {
-              // S takes the place of the P that the MMAs before it read: one thread's MMAs run in order
+          ok = wait(&q_full, n);
+          if (ok && mine == 0) mbar_arrive(&q_empty);
+#pragma unroll 1
+          for (int k = 0; ok && k <= mine; ++k) {  // S of tile k, P V of tile k - 1
+            // S of tile k is free: read by the softmax, or (aliased) in the place of the P that the MMAs before
+            // it read: one thread's MMAs run in order
+            auto ready = [&]() {
+              if (k > 0 && k < mine) skip(ks, kStep);
+              return k == mine || (landed(ks) && (C::kAlias || kk == 0 || wait(s_free + x, kk - 1)));
+            };
+            auto scores = [&]() {
+              if (!ok || k == mine) return;
               qk();
-              if (k + 2 == mine) tc_commit(&q_empty);
+              if (k + 1 == mine) tc_commit(&q_empty);
+            };
+            if (!C::kAlias) {  // under the softmax of the tile before
+              ok = ready();
+              scores();
             }
-            if (more) skip(vs, kStep);
+            if (k > 0) {
+              ok = ok && landed(vs) && (k > 1 || n == 0 || wait(o_free + x, n - 1)) && wait(&p_full[x][0], kk - 1);
+              if (ok) pv(k == 1, 0);
+            }
+            if (C::kAlias) ok = ok && ready();
+            if (k > 0) {
+              ok = ok && wait(&p_full[x][1], kk - 1);
+              if (ok) pv(k == 1, 1);
+              if (k < mine) skip(vs, kStep);
+            }
+            if (C::kAlias) scores();
+            if (k < mine) ++kk;
           }
           // on to the next item's entries, past those that this stream does not read
           if (mine > 0) left -= (mine - 1) * kStep;
@@ -685,7 +730,7 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
     }
     leave();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
     // ---- softmax of stream x
     const int x = (int(threadIdx.x) - 128) >> 7;
     const int quarter = warp & 3, r = quarter * 32 + lane;
@@ -693,7 +738,6 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
     const uint32_t ts = trow + x * C::kS, to = trow + C::kO + x * HD, tp = trow + C::kP + x * C::kPStep;
     const int row = MT == 2 ? x * 128 + r : r;
     const float sl2 = p.scale * kLog2e;
-    uint32_t entry = 0;  // of the ring, counted on: the item's first K tile
     uint32_t kk = 0;  // tiles so far
     bool ok = true;
     for (int n = 0;; ++n) {
@@ -705,14 +749,13 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
         if (MT == 1) named_sync_and(1, 256, false);
         break;
       }
-      int lim, low, keys, mine;  // keys [0, lim) are seen by the row, [0, low) by all, [0, keys) by one
+      int lim, mine;  // keys [0, lim) are seen
       {
         const PaItem it = items[n & 1];
-        keys = keys_of(it);
         mine = tiles_of(it, x);
-        lim = row < it.ntok * p.gs ? it.tok0 + row / p.gs + 1 - it.start : keys;
-        low = it.tok0 + 1 - it.start;
+        lim = it.tok0 + min(pa_div_gs(p, row), it.ntok - 1) + 1 - it.start;
       }
+      const int wlo = __reduce_min_sync(0xffffffffu, lim), whi = __reduce_max_sync(0xffffffffu, lim);
       float m = -INFINITY, l = 0.f;  // reference max (scaled, base 2), sum
       for (int k = 0; k < mine; ++k, ++kk) {
         const int t = MT == 2 ? k : 2 * k + x, j = t * kPaTcKeys;
@@ -728,10 +771,14 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(s_free + x);
         }
-        const bool masked = __any_sync(0xffffffffu, j + kPaTcKeys > lim);
+        const bool masked = j + kPaTcKeys > wlo;
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < kPaTcKeys; ++c) sc[c] = j + c < lim ? sc[c] : -INFINITY;
+          for (int c = 0; c < kPaTcKeys; c += 32)
+            if (j + c + 32 > wlo) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sc[c + i] = c + i < lim - j ? sc[c + i] : -INFINITY;
+            }
         }
         float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
@@ -764,21 +811,22 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        if (j + kPaTcKeys > low) {  // V rows behind the keys, or not seen by all (MT 2: both streams write the same zeros)
-          const uint32_t e = entry + 2 * t + 1, s = e % NB;
-          ok = wait(full + s, e / NB);
-          if (!__all_sync(0xffffffffu, ok)) break;
-          tc_clean_row<HD>(smem + C::kOffRing + s * C::kTile, r, j + r >= keys, j + r >= low, odd_sh + (n & 1), n + 1);
-          fence_async_smem();
-        }
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         // kCubic of 16 pairs on the fp32 pipe, which the special-function unit
         // (8 cycles a warp and value) leaves idle; masked tiles need exact zeros
-        auto exps = [&](auto cubic) {
-          constexpr int kCubic = decltype(cubic)::value;
+        // masked: 32 keys that no row of the warp sees need none at all
+        auto exps = [&](auto mask) {
+          constexpr bool kMask = decltype(mask)::value;
+          constexpr int kCubic = kMask ? 0 : kPaCubic<HD>;
 #pragma unroll
           for (int c = 0; c < kPaTcKeys; c += 32) {
             uint32_t pk[16];
+            const bool none = kMask && j + c >= whi;
+            if (none) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = 0u;
+            }
+            if (!none) {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float2 e = fma2(make_float2(sc[c + i], sc[c + i + 1]), make_float2(sl2, sl2), make_float2(-ref, -ref));
@@ -790,6 +838,7 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
               }
               sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
               pk[i / 2] = pack_bf16(e.x, e.y);
+            }
             }
             if (c == 64) {  // the first half of the keys: its stores have landed meanwhile
               tc_wait_st();
@@ -805,9 +854,9 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
           if (lane == 0) mbar_arrive(&p_full[x][1]);
         };
         if (masked)
-          exps(std::integral_constant<int, 0>{});
+          exps(std::true_type{});
         else
-          exps(std::integral_constant<int, kPaCubic>{});
+          exps(std::false_type{});
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }
@@ -817,68 +866,80 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
         *abort = 1;
       }
       tc_fence_after();
-      float wb = 0.f, wa = 1.f;
+      float w0 = 1.f, w1 = 0.f;  // weights of this stream's O and the other's
       if (MT == 1) {
-        if (x == 1) ml_sh[n & 1][r] = make_float2(m, l);
+        ml_sh[n & 1][x][r] = make_float2(m, l);
         tc_fence_before();
         ok = named_sync_and(1, 256, ok);
         tc_fence_after();
-        const float2 b = ml_sh[n & 1][r];
+        const float2 b = ml_sh[n & 1][1 - x][r];
         // (a NaN sum of either stream makes the whole sum NaN)
         const float top = fmaxf(m, b.x), ref = top == -INFINITY ? 0.f : top;
-        wa = exp2_approx(m - ref);
-        wb = exp2_approx(b.x - ref);
-        l = l * wa + b.y * wb;
+        w0 = exp2_approx(m - ref);
+        w1 = exp2_approx(b.x - ref);
+        l = l * w0 + b.y * w1;
       }
       if (!ok) break;
-      if (MT == 2 || x == 0) {
+      {
         const PaItem it = items[n & 1];
-        const bool write = row < it.ntok * p.gs, two = MT == 1 && keys > kPaTcKeys;
-        const int tok = it.tok0 + row / p.gs;
+        const bool write = row < it.ntok * p.gs, two = MT == 1 && keys_of(it) > kPaTcKeys;
+        const int of = pa_div_gs(p, row), tok = it.tok0 + of;
         const bool odd = *static_cast<volatile int*>(odd_sh + (n & 1)) == n + 1;
+        const bool none = __any_sync(0xffffffffu, l == 0.f);
         const float inv = 1.f / l;
-        bf16* out = static_cast<bf16*>(p.out) + (size_t(tok - p.first) * p.hq + it.plane * p.gs + row % p.gs) * HD;
+        // MT 1: of the sum of both streams' each warpgroup writes half the dims
+        constexpr int kCols = MT == 1 ? HD / 2 : HD;
+        const int c0 = MT == 1 ? x * kCols : 0;
+        const uint32_t oo = trow + C::kO + (1 - x) * HD + c0;
+        bf16* out = static_cast<bf16*>(p.out) + (size_t(tok - p.first) * p.hq + it.plane * p.gs + row - of * p.gs) * HD + c0;
+        // (MT 1, one key tile: stream 1 has no O)
+        const bool own = MT == 2 || two || x == 0;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
+        for (int c = 0; c < kCols; c += 32) {
           float f[32];
-          if (mine > 0) {
-            uint32_t o1[32];
-            tc_ld32(to + c, reinterpret_cast<uint32_t*>(f));
-            if (two) tc_ld32(to + HD + c, o1);
+          if (MT == 2 ? mine > 0 : true) {
+            tc_ld32((own ? to + c0 : oo) + c, reinterpret_cast<uint32_t*>(f));
             tc_wait_ld();
-            if (MT == 1) {
+            const float wi = (own ? w0 : w1) * inv;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                f[e] *= wa;
-                if (two) f[e] = fmaf(__uint_as_float(o1[e]), wb, f[e]);
-              }
+            for (int e = 0; e < 32; ++e) f[e] *= wi;
+            if (two) {
+              uint32_t o1[32];
+              tc_ld32(oo + c, o1);
+              tc_wait_ld();
+              const float wj = w1 * inv;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[e] = fmaf(__uint_as_float(o1[e]), wj, f[e]);
             }
           }
-          if (c == HD - 32) {  // O may be written again
+          if (c == kCols - 32) {  // O may be written again
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
               mbar_arrive(o_free + x);
-              if (MT == 1) mbar_arrive(o_free + 1);
+              if (MT == 1) mbar_arrive(o_free + 1 - x);
             }
           }
           if (write) {
             if (odd) {  // what was taken out of V
-              const bf16* v = static_cast<const bf16*>(p.v) + (it.plane / p.subs) * p.v_hs + it.start * p.v_ts + c;
+              const bf16* v = static_cast<const bf16*>(p.v) + (it.plane / p.subs) * p.v_hs + it.start * p.v_ts + c0 + c;
 #pragma unroll 1
-              for (int i = low * 32; i < lim * 32; ++i) {
+              for (int i = (it.tok0 + 1 - it.start) * 32; i < lim * 32; ++i) {  // (earlier keys are seen by all)
                 const float y = to_f(v[(i >> 5) * p.v_ts + (i & 31)]);
                 if (!(fabsf(y) < INFINITY))
 #pragma unroll
                   for (int e = 0; e < 32; ++e) f[e] = e == (i & 31) ? f[e] + y : f[e];
               }
             }
+            if (none) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : f[e];
+            }
 #pragma unroll
             for (int h = 0; h < 32; h += 16) {
               uint32_t w[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                w[e] = l == 0.f ? 0u : pack_bf16(f[h + 2 * e] * inv, f[h + 2 * e + 1] * inv);
+              for (int e = 0; e < 8; ++e) w[e] = pack_bf16(f[h + 2 * e], f[h + 2 * e + 1]);
               st_v8(out + c + h, w);
             }
           }
@@ -886,7 +947,6 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(item_empty + (n & 1));
-      entry += 2 * ((keys + kPaTcKeys - 1) / kPaTcKeys);
     }
     leave();
   }
