@@ -341,10 +341,10 @@ int mtpb_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const 
  * (k 0: both may be NULL). A NaN logit counts as -inf; +inf logits share the
  * probability. Places without a token above -inf hold -inf and id 0; a row
  * without any has entropy 0 and log-probability -inf. k in [0, 64], V below
- * 2^30, at most 2^24 rows. Sums are fp32 within a chunk of a row and fp64
- * over chunks. `block`: workspace of mtpb_logprobs_block_bytes(rows, V, k)
- * bytes, 16-byte aligned, private to the call until it has run. */
-long long mtpb_logprobs_block_bytes(int rows, int V_plan, int k);
+ * 2^30, at most 2^24 rows. Sums are fp32 within a part of a row and fp64
+ * over parts. `block`: workspace of mtpb_logprobs_block_bytes(rows, V, k,
+ * dtype) bytes, 16-byte aligned, private to the call until it has run. */
+long long mtpb_logprobs_block_bytes(int rows, int V_plan, int k, int dtype);
 int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const int64_t* targets,
                         int k, float* logprobs, float* entropy, float* top_logprobs,
                         int64_t* top_ids, void* block, int dtype, void* stream);
@@ -352,17 +352,17 @@ int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const i
 /* The two halves of mtpb_token_logprobs for a vocabulary in shards.
  * mtpb_logprobs_block reduces one shard (columns [vstart, vstart + V_local) of
  * the vocabulary) of every row to a block of mtpb_logprobs_block_bytes(rows,
- * V_plan, k) bytes; V_plan, the same on every shard, is at least the largest
- * V_local. mtpb_logprobs_join joins `parts` such blocks, one after another in
- * memory in any shard order, all made with the same rows, V_plan and k_block,
+ * V_plan, k, dtype) bytes; V_plan, the same on every shard, is at least the largest
+ * V_local. mtpb_logprobs_join joins `shards` such blocks, one after another in
+ * memory in any shard order, all made with the same rows, V_plan, k_block and dtype,
  * into the outputs of mtpb_token_logprobs; k at most k_block. A target that no
  * shard holds gets NaN. */
 int mtpb_logprobs_block(const void* logits, int64_t ld, int rows, int V_local, int64_t vstart,
                         int V_plan, const int64_t* targets, int k, void* block, int dtype,
                         void* stream);
-int mtpb_logprobs_join(const void* blocks, int parts, int rows, int V_plan, int k_block,
+int mtpb_logprobs_join(const void* blocks, int shards, int rows, int V_plan, int k_block,
                        const int64_t* targets, int k, float* logprobs, float* entropy,
-                       float* top_logprobs, int64_t* top_ids, void* stream);
+                       float* top_logprobs, int64_t* top_ids, int dtype, void* stream);
 
 /* As mtpb_beam_status, of the prompt attentions and log-probabilities. */
 int mtpb_scoring_status(uint32_t* status_out /* host */);

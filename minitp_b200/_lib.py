@@ -118,13 +118,13 @@ SIGNATURES: dict[str, tuple] = {
     "mtpb_prompt_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                       c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                       c_void_p]),
-    "mtpb_logprobs_block_bytes": (c_longlong, [c_int, c_int, c_int]),
+    "mtpb_logprobs_block_bytes": (c_longlong, [c_int, c_int, c_int, c_int]),
     "mtpb_token_logprobs": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_void_p, c_int, c_void_p]),
     "mtpb_logprobs_block": (c_int, [c_void_p, c_int64, c_int, c_int, c_int64, c_int, c_void_p, c_int, c_void_p, c_int,
                                     c_void_p]),
     "mtpb_logprobs_join": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
-                                   c_void_p, c_void_p]),
+                                   c_void_p, c_int, c_void_p]),
     "mtpb_scoring_status": (c_int, [POINTER(c_uint32)]),
     "mtpb_model_create": (c_int, [POINTER(ModelDesc), c_void_p, POINTER(c_void_p)]),
     "mtpb_model_set_layer": (c_int, [c_void_p, c_int, POINTER(LayerDesc)]),

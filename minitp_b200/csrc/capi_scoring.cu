@@ -21,55 +21,63 @@ bool dtype_ok(int dtype) { return dtype == MTPB_BF16 || dtype == MTPB_F32; }
 // ------------------------------------------------------------------ log-probabilities
 constexpr long long kLpMaxRows = 1ll << 24;
 
-// Chunks of a row: a function of the sizes alone, so that every rank cuts its
-// shard alike.
-struct LpPlan {
-  int nchunk, chunk;
-};
-
-LpPlan lp_plan(long long rows, int V) {
+// Runs of tiles: a function of the sizes alone, so that every rank cuts its
+// shard alike. Three CTAs for each of B200's 148 SMs, which is what the ring
+// leaves room for.
+LpPlan lp_plan(long long rows, int V, int dtype) {
   LpPlan b;
-  const long long want = std::max<long long>(1, std::min<long long>(32, 2 * 148 / rows));
-  b.nchunk = int(std::min<long long>(want, (V + 8191) / 8192));
-  b.chunk = (V + b.nchunk - 1) / b.nchunk;
-  b.chunk = (b.chunk + 7) / 8 * 8;
-  b.nchunk = (V + b.chunk - 1) / b.chunk;
+  const int cols = kLpTile * (dtype == MTPB_BF16 ? 8 : 4);
+  b.tiles = (V + cols - 1) / cols;
+  const long long total = rows * b.tiles, ctas = std::min<long long>(total, 3 * 148);
+  b.run = int((total + ctas - 1) / ctas);
+  b.parts = (b.tiles - 2) / b.run + 2;  // a row that begins at a run's last tile; never more than its tiles
+  b.parts = std::max(1, std::min(b.parts, b.tiles));
   return b;
 }
 
-size_t lp_stat_bytes(long long rows, const LpPlan& b) { return size_t(rows) * b.nchunk * sizeof(LpStat); }
+size_t lp_stat_bytes(long long rows, const LpPlan& b) { return size_t(rows) * b.parts * sizeof(LpStat); }
 size_t lp_block(long long rows, const LpPlan& b, int k) {
-  return (lp_stat_bytes(rows, b) + size_t(rows) * b.nchunk * k * 8 + 15) / 16 * 16;
+  return (lp_stat_bytes(rows, b) + size_t(rows) * b.parts * k * 8 + 15) / 16 * 16;
 }
 
 int lp_check(long long rows, long long V, int k) {
   if (rows < 1 || rows > kLpMaxRows) return bad("token_logprobs: need 1 .. 2^24 rows");
   if (V < 1 || V >= 1ll << 30) return bad("token_logprobs: empty vocabulary, or one of 2^30 or more");
+  if (rows * V > 1ll << 40) return bad("token_logprobs: more than 2^40 logits");
   if (k < 0 || k > kLpMaxK) return bad("token_logprobs: the alternatives must be in [0, 64]");
   return MTPB_OK;
 }
 
-int lp_join(const void* blocks, int parts, int rows, int V_plan, int kc, const int64_t* targets, int k,
+template <typename T, bool TOP>
+int lp_rows(const LpRowsParams& p, cudaStream_t st) {
+  const auto kern = lp_rows_kernel<T, TOP>;
+  // (with the static part it passes the 48 KB that a kernel gets unasked)
+  const cudaError_t e = host_allow_smem(reinterpret_cast<const void*>(kern), kLpRing<TOP>);
+  if (e != cudaSuccess) return host_fail_cuda(e, "cudaFuncSetAttribute");
+  const long long total = (long long)p.rows * p.plan.tiles;
+  return host_launch(kern, dim3(unsigned((total + p.plan.run - 1) / p.plan.run)), dim3(kLpThreads + 32), kLpRing<TOP>, st, p);
+}
+
+int lp_join(const void* blocks, int shards, int rows, const LpPlan& b, int kc, const int64_t* targets, int k,
             float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, cudaStream_t st) {
-  const LpPlan b = lp_plan(rows, V_plan);
   const size_t block = lp_block(rows, b, kc);
   LpJoinParams p;
+  std::memset(&p, 0, sizeof(p));
   p.stat = static_cast<const LpStat*>(blocks);
   p.cand = reinterpret_cast<const uint64_t*>(static_cast<const char*>(blocks) + lp_stat_bytes(rows, b));
-  p.stat_part = block / sizeof(LpStat);
-  p.cand_part = block / 8;
-  p.parts = parts;
+  p.stat_shard = block / sizeof(LpStat);
+  p.cand_shard = block / 8;
+  p.plan = b;
+  p.shards = shards;
   p.rows = rows;
-  p.nchunk = b.nchunk;
   p.k = k;
   p.kc = kc;
-  p.targets = reinterpret_cast<const long long*>(targets);
-  p.logprobs = logprobs;
+  p.logprobs = targets ? logprobs : nullptr;
   p.entropy = entropy;
   p.top_logprobs = top_logprobs;
   p.top_ids = reinterpret_cast<long long*>(top_ids);
   return host_launch(lp_join_kernel, dim3((rows + kLpJoinWarps - 1) / kLpJoinWarps), dim3(32 * kLpJoinWarps),
-                     size_t(k ? kLpJoinWarps : 0) * parts * b.nchunk, st, p);
+                     size_t(k ? kLpJoinWarps : 0) * shards * b.parts, st, p);
 }
 
 int join_check(const int64_t* targets, int k, const float* logprobs, const float* entropy, const float* top_logprobs,
@@ -83,10 +91,11 @@ int join_check(const int64_t* targets, int k, const float* logprobs, const float
 
 extern "C" {
 
-long long mtpb_logprobs_block_bytes(int rows, int V_plan, int k) {
+long long mtpb_logprobs_block_bytes(int rows, int V_plan, int k, int dtype) {
   const int r = lp_check(rows, V_plan, k);
   if (r != MTPB_OK) return r;
-  return (long long)lp_block(rows, lp_plan(rows, V_plan), k);
+  if (!dtype_ok(dtype)) return bad("unsupported dtype");
+  return (long long)lp_block(rows, lp_plan(rows, V_plan, dtype), k);
 }
 
 int mtpb_logprobs_block(const void* logits, int64_t ld, int rows, int V_local, int64_t vstart, int V_plan,
@@ -99,34 +108,34 @@ int mtpb_logprobs_block(const void* logits, int64_t ld, int rows, int V_local, i
     return bad("token_logprobs: need 0 <= V_local <= V_plan, ld");
   if (vstart < 0 || vstart > 0xFFFFFFFFll - V_local) return bad("token_logprobs: vocabulary ids out of range");
   if (!al16(block)) return bad("token_logprobs: block must be 16-byte aligned");
-  const LpPlan b = lp_plan(rows, V_plan);
   LpRowsParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.plan = lp_plan(rows, V_plan, dtype);
   p.logits = logits;
   p.ld = ld;
+  p.rows = rows;
   p.V = V_local;
   p.k = k;
   p.vstart = vstart;
-  p.nchunk = b.nchunk;
-  p.chunk = b.chunk;
   p.targets = reinterpret_cast<const long long*>(targets);
   p.stat = static_cast<LpStat*>(block);
-  p.cand = reinterpret_cast<uint64_t*>(static_cast<char*>(block) + lp_stat_bytes(rows, b));
-  const dim3 grid(unsigned(rows) * b.nchunk), threads(kLpThreads);
+  p.cand = reinterpret_cast<uint64_t*>(static_cast<char*>(block) + lp_stat_bytes(rows, p.plan));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == MTPB_BF16 ? host_launch(lp_rows_kernel<bf16>, grid, threads, 0, st, p)
-                            : host_launch(lp_rows_kernel<float>, grid, threads, 0, st, p);
+  return dtype == MTPB_BF16 ? (k ? lp_rows<bf16, true>(p, st) : lp_rows<bf16, false>(p, st))
+                            : (k ? lp_rows<float, true>(p, st) : lp_rows<float, false>(p, st));
 }
 
-int mtpb_logprobs_join(const void* blocks, int parts, int rows, int V_plan, int k_block, const int64_t* targets, int k,
-                       float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, void* stream) {
+int mtpb_logprobs_join(const void* blocks, int shards, int rows, int V_plan, int k_block, const int64_t* targets, int k,
+                       float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, int dtype, void* stream) {
   int r = lp_check(rows, V_plan, k_block);
   if (r == MTPB_OK) r = join_check(targets, k, logprobs, entropy, top_logprobs, top_ids);
   if (r != MTPB_OK) return r;
+  if (!dtype_ok(dtype)) return bad("unsupported dtype");
   if (!blocks || !al16(blocks)) return bad("token_logprobs: blocks must be 16-byte aligned");
-  if (parts < 1 || parts > 64) return bad("token_logprobs: need 1 .. 64 shards");
+  if (shards < 1 || shards > 64) return bad("token_logprobs: need 1 .. 64 shards");
   if (k < 0 || k > k_block) return bad("token_logprobs: more alternatives than the blocks hold");
-  return lp_join(blocks, parts, rows, V_plan, k_block, targets, k, logprobs, entropy, top_logprobs, top_ids,
-                 static_cast<cudaStream_t>(stream));
+  return lp_join(blocks, shards, rows, lp_plan(rows, V_plan, dtype), k_block, targets, k, logprobs, entropy, top_logprobs,
+                 top_ids, static_cast<cudaStream_t>(stream));
 }
 
 int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const int64_t* targets, int k, float* logprobs,
@@ -135,7 +144,7 @@ int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const i
   if (r == MTPB_OK) r = join_check(targets, k, logprobs, entropy, top_logprobs, top_ids);
   if (r == MTPB_OK) r = mtpb_logprobs_block(logits, ld, rows, V, 0, V, targets, k, block, dtype, stream);
   if (r != MTPB_OK) return r;
-  return lp_join(block, 1, rows, V, k, targets, k, logprobs, entropy, top_logprobs, top_ids,
+  return lp_join(block, 1, rows, lp_plan(rows, V, dtype), k, targets, k, logprobs, entropy, top_logprobs, top_ids,
                  static_cast<cudaStream_t>(stream));
 }
 
@@ -295,12 +304,14 @@ extern "C" int mtpb_prompt_attention(const void* q, int64_t q_token, int64_t q_h
 
 extern "C" int mtpb_scoring_status(uint32_t* status_out) {
   if (!status_out) return bad("scoring_status: null argument");
-  uint32_t a = 0;
+  uint32_t a = 0, b = 0;
   const uint32_t zero = 0;
   cudaError_t e = cudaDeviceSynchronize();
   if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&a, g_pa_status, sizeof(a));
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&b, g_lp_status, sizeof(b));
   if (e == cudaSuccess && a) e = cudaMemcpyToSymbol(g_pa_status, &zero, sizeof(zero));
+  if (e == cudaSuccess && b) e = cudaMemcpyToSymbol(g_lp_status, &zero, sizeof(zero));
   if (e != cudaSuccess) return host_fail_cuda(e, "scoring_status");
-  *status_out = a;
+  *status_out = a | b;
   return MTPB_OK;
 }

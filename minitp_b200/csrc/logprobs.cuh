@@ -9,142 +9,431 @@
 // without any token above -inf has no alternatives, entropy 0, and every
 // token's log-probability is -inf.
 //
-// A row is cut into chunks; each is reduced to its statistics and its k best
-// logits (packed keys: value, then lower id), and a second kernel joins the
-// chunks, of every shard of the vocabulary.
+// The rows' columns are cut into tiles of 16 KB, and all tiles of all rows, in
+// order, into equal runs, one a CTA: so every CTA streams the same bytes, and a
+// row may be reduced by several, each to its statistics and its k best logits
+// (packed keys: value, then lower id). A second kernel joins them, of every
+// shard of the vocabulary.
 #pragma once
 
-#include "common.cuh"
+#include "topk.cuh"
 
 namespace mtpb {
 
-constexpr int kLpMaxK = 64;
+constexpr int kLpMaxK = kBeamMaxK;
 
-// Of a chunk: m = max x, s = sum exp(x - m), w = sum exp(x - m) (x - m), and
-// the target's logit (NaN: the target lies elsewhere). m -inf: no token.
+// Of a part of a row: m = max x, s = sum exp(x - m), w = sum exp(x - m) (x - m),
+// and the target's logit (NaN: the target lies elsewhere). s 0: no token.
 struct LpStat {
   float m, s, w, xt;
+};
+
+constexpr int kLpWarps = 8;   // that compute; one more copies
+constexpr int kLpVecs = 4;    // 16-byte vectors a lane and tile
+constexpr int kLpTile = kLpWarps * 32 * kLpVecs;  // vectors
+// Ring of tiles: what three CTAs an SM leave beside the candidates.
+template <bool TOP>
+constexpr int kLpStages = TOP ? 3 : 4;
+template <bool TOP>
+constexpr size_t kLpRing = size_t(kLpStages<TOP>) * kLpTile * 16;
+constexpr int kLpThreads = kLpWarps * 32;
+
+// How the tiles of `rows` rows of `tiles` tiles fall to CTAs of `run` tiles each.
+struct LpPlan {
+  int tiles, run, parts;  // parts: the most CTAs that share a row
+  __host__ __device__ long long first(long long row) const { return row * tiles / run; }  // CTA of a row's first tile
+  __host__ __device__ int count(long long row) const { return int(((row + 1) * tiles - 1) / run - first(row)) + 1; }
 };
 
 struct LpRowsParams {
   const void* logits;
   int64_t ld;      // elements between rows
-  int V, k;        // columns of this shard, candidates a chunk
+  int rows, V, k;  // columns of this shard, candidates a part
   int64_t vstart;  // id of column 0
-  int nchunk, chunk;
+  LpPlan plan;
   const long long* targets;  // [rows] or NULL
-  LpStat* stat;    // [rows][nchunk]
-  uint64_t* cand;  // [rows][nchunk][k], best first, 0-padded
+  LpStat* stat;    // [rows][parts]
+  uint64_t* cand;  // [rows][parts][k], best first, 0-padded
 };
 
-__device__ __forceinline__ uint64_t lp_key(float v, uint32_t id) {
-  if (!(v > -INFINITY)) return 0;
-  const uint32_t b = __float_as_uint(v + 0.f);  // (-0 as +0)
-  return (uint64_t(b & 0x80000000u ? ~b : b | 0x80000000u) << 32) | (0xFFFFFFFFu - id);
-}
-__device__ __forceinline__ float lp_key_val(uint64_t o) {
-  const uint32_t k = uint32_t(o >> 32);
-  return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
-}
-__device__ __forceinline__ uint64_t lp_warp_max(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = u > v ? u : v;
-  }
-  return v;
-}
+// Set when a bounded wait of a log-probability kernel ran out (its results are then void).
+__device__ uint32_t g_lp_status;
 
-constexpr int kLpThreads = 256;
-
-// A CTA a row and chunk: the maximum, the sums, and k times the best below the last.
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) lp_rows_kernel(const LpRowsParams p) {
-  __shared__ float red[32];
-  __shared__ uint64_t best[kLpThreads / 32];
+// One pass over the logits, bound by their bytes for many rows. A lane keeps
+// a reference m, s = sum 2^d and w = sum 2^d d with d = x L - c (c = m L
+// rounded, beam_ref), in fp32; the reference follows the lane's maximum when
+// that has passed it by 8 (natural units), so that d stays small and the
+// entropy's logarithm and mean, which are taken from each other, lose little.
+// Values are raised to at least -2^126 first, which takes NaN and -inf along:
+// they then add 2^d d = 0 x finite. Where the reference is far (2^30 or more:
+// neighbours then lie 64 apart, and the raised ones may hide below) the values
+// equal to the maximum are counted from the bits as they are.
+// Without candidates (TOP false) two thirds of the instructions are left.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRowsParams p) {
+  constexpr int VE = VecTraits<T>::kElems, kLow = sizeof(T) == 2 ? 16 : 0, NS = kLpStages<TOP>;
+  extern __shared__ __align__(128) uint4 ring[];
+  __shared__ uint64_t buf[TOP ? kLpWarps : 1][TOP ? kBeamCap : 1];
+  __shared__ uint64_t all[TOP ? kLpWarps * kLpMaxK : 1];
+  __shared__ uint64_t full[NS], empty[NS];
+  __shared__ LpStat stat[kLpWarps];
+  __shared__ uint32_t floors[2];  // by the part's parity: at least k of its values have this key or a higher one
+  __shared__ int totals[2], abort_sh;
+  volatile int* abort = &abort_sh;
   pdl_launch();
   pdl_wait();
-  const size_t row = blockIdx.x / p.nchunk;
-  const int ch = blockIdx.x % p.nchunk, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int c0 = min(p.V, ch * p.chunk), c1 = min(p.V, c0 + p.chunk);
-  const T* x = static_cast<const T*>(p.logits) + int64_t(row) * p.ld;
-  auto at = [&](int c) {
-    const float v = to_f(x[c]);
-    return v == v ? v : -INFINITY;
-  };
-  float m = -INFINITY;
-  for (int c = c0 + tid; c < c1; c += kLpThreads) m = fmaxf(m, at(c));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[warp] = m;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t0 = (long long)blockIdx.x * p.plan.run;
+  const long long t1 = min(t0 + p.plan.run, (long long)p.rows * p.plan.tiles);
+  if (threadIdx.x == kLpThreads) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, kLpWarps);
+    }
+    mbar_init_fence();
+  }
+  if (threadIdx.x == 0) {
+    floors[0] = floors[1] = 0;
+    totals[0] = totals[1] = 0;
+    *abort = 0;
+  }
   __syncthreads();
-  m = red[0];
-  for (int i = 1; i < kLpThreads / 32; ++i) m = fmaxf(m, red[i]);
-  float s = 0.f, w = 0.f;
-  if (m > -INFINITY)
-    for (int c = c0 + tid; c < c1; c += kLpThreads) {
-      const float v = at(c), d = v == m ? 0.f : v - m, e = expf(d);
-      s += e;
-      if (e > 0.f) w = fmaf(e, d, w);
-    }
-  s = block_sum(s, red);
-  w = block_sum(w, red);
-  if (tid == 0) {
-    LpStat st{m, s, w, __int_as_float(0x7fffffff)};
-    if (p.targets) {
-      const long long c = p.targets[row] - p.vstart;
-      if (c >= c0 && c < c1) st.xt = at(int(c));
-    }
-    p.stat[row * p.nchunk + ch] = st;
-  }
-  uint64_t last = ~0ull;
-  for (int i = 0; i < p.k; ++i) {
-    uint64_t b = 0;
-    if (last)
-      for (int c = c0 + tid; c < c1; c += kLpThreads) {
-        const uint64_t o = lp_key(at(c), uint32_t(p.vstart + c));
-        if (o < last && o > b) b = o;
+  // Row r: its vectors begin `head` columns in, and `tail` columns stand behind the last whole one.
+  struct Row {
+    const T* x;
+    int head, nvec, tail;
+  };
+  auto row_at = [&](int r) {
+    Row w;
+    w.x = static_cast<const T*>(p.logits) + int64_t(r) * p.ld;
+    const int off = int((reinterpret_cast<uintptr_t>(w.x) & 15u) / sizeof(T));
+    w.head = min(p.V, off ? VE - off : 0);
+    w.nvec = (p.V - w.head) / VE;
+    w.tail = p.V - w.head - w.nvec * VE;
+    return w;
+  };
+  int row = int(t0 / p.plan.tiles), tile = int(t0 - (long long)row * p.plan.tiles);
+  int sg = 0;
+  uint32_t phase = 0;
+  if (warp == kLpWarps) {  // ---- copies
+    if (lane == 0) {
+      int issued = 0;
+      bool ok = true;
+      for (long long t = t0; ok && t < t1; ++row, tile = 0) {
+        const Row w = row_at(row);
+        for (; ok && tile < p.plan.tiles && t < t1; ++tile, ++t) {
+          const int n = min(kLpTile, w.nvec - tile * kLpTile);
+          if (n <= 0) continue;  // (a shard of fewer columns than planned for)
+          ok = issued < NS || mbar_wait_lean(empty + sg, phase ^ 1u, abort);
+          if (!ok) break;
+          mbar_arrive_expect_tx(full + sg, uint32_t(n) * 16);
+          bulk_g2s(ring + sg * kLpTile, w.x + w.head + int64_t(tile) * kLpTile * VE, uint32_t(n) * 16, full + sg);
+          if (issued < NS) ++issued;
+          if (++sg == NS) {
+            sg = 0;
+            phase ^= 1u;
+          }
+        }
       }
-    b = lp_warp_max(b);
-    __syncthreads();
-    if (lane == 0) best[warp] = b;
-    __syncthreads();
-    for (int j = 0; j < kLpThreads / 32; ++j) b = best[j] > b ? best[j] : b;
-    last = b;
-    if (tid == 0) p.cand[(row * p.nchunk + ch) * p.k + i] = b;
+      if (!ok) *abort = 1;
+      // copies in flight land before the memory goes away
+      int never = 0;
+      if (issued < NS) {
+        sg = 0;
+        phase = 0;
+      } else {
+        phase ^= 1u;
+      }
+      for (int i = 0; i < issued; ++i) {
+        mbar_wait_lean(full + sg, phase, &never);
+        if (++sg == NS) {
+          sg = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else {
+    bool ok = true;
+    int odd = 0;  // parity of the part
+    for (long long t = t0; t < t1; ++row, tile = 0, odd ^= 1) {
+      uint32_t* floor_key = floors + odd;
+      // ---- this CTA's part of a row
+      const Row w = row_at(row);
+      const int end = int(min((long long)p.plan.tiles, tile + (t1 - t)));
+      const int c0 = tile == 0 ? 0 : min(p.V, w.head + tile * kLpTile * VE);
+      const int c1 = end == p.plan.tiles ? p.V : min(p.V, w.head + end * kLpTile * VE);
+      t += end - tile;
+      float xt = __int_as_float(0x7fffffff);
+      if (threadIdx.x == 0 && p.targets) {
+        const long long c = p.targets[row] - p.vstart;
+        if (c >= c0 && c < c1) {
+          xt = to_f(w.x[c]);
+          if (xt != xt) xt = -INFINITY;
+        }
+      }
+      BeamList l{TOP ? buf[warp] : nullptr, 0, 0x00800000u, 0u};  // least: the key of the lowest finite value
+      float m = -INFINITY, c = 0.f, s = 0.f, ws = 0.f;
+      // a tile: vector u of this lane holds columns col + u * 32 * VE ..
+      auto step = [&](const uint4 (&v)[kLpVecs], int col, bool first) {
+        float q[kLpVecs];  // max of each vector, at least -2^126
+        uint32_t y[kLpVecs][4];
+#pragma unroll
+        for (int u = 0; u < kLpVecs; ++u) {
+          const uint32_t raw[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+          if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %1, %2;" : "=r"(y[u][i]) : "r"(raw[i]), "r"(0xFE80FE80u));
+            uint32_t a, b;
+            asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(y[u][0]), "r"(y[u][1]));
+            asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(y[u][2]), "r"(y[u][3]));
+            asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+            q[u] = fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[u][i] = __float_as_uint(fmaxf(__uint_as_float(raw[i]), -0x1p126f));
+            q[u] = fmaxf(max3(__uint_as_float(y[u][0]), __uint_as_float(y[u][1]), __uint_as_float(y[u][2])),
+                         __uint_as_float(y[u][3]));
+          }
+        }
+        float top = fmaxf(max3(q[0], q[1], q[2]), q[3]);
+        // ---- sums
+        if (!beam_far(fmaxf(m, top))) {
+          if (top - m > 8.f) {
+            if (beam_far(m)) {  // nothing yet, or values that count for nothing beside these
+              s = ws = 0.f;
+            } else {
+              const float d = beam_ref(m) - beam_ref(top), a = exp2_approx(d);
+              ws = fmaf(s, d, ws) * a;
+              s *= a;
+            }
+            m = top;
+            c = beam_ref(m);
+          }
+          float2 sum = make_float2(0.f, 0.f), mean = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int u = 0; u < kLpVecs; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; i += sizeof(T) == 2 ? 1 : 2) {
+              float2 x;
+              if constexpr (sizeof(T) == 2)
+                x = make_float2(__uint_as_float(y[u][i] << 16), __uint_as_float(y[u][i] & 0xFFFF0000u));
+              else
+                x = make_float2(__uint_as_float(y[u][i]), __uint_as_float(y[u][i + 1]));
+              const float2 d = fma2(x, make_float2(kBeamLog2e, kBeamLog2e), make_float2(-c, -c));
+              const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+              sum = add2(sum, e);
+              mean = fma2(e, d, mean);
+            }
+          s += sum.x + sum.y;
+          ws += mean.x + mean.y;
+        } else {
+          float raw_top = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < kLpVecs; ++u) {
+            float g[VE];
+            unpack(v[u], g);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) raw_top = fmaxf(raw_top, g[e]);
+          }
+          if (raw_top > m) {
+            m = raw_top;
+            s = ws = 0.f;
+          }
+          if (m > -INFINITY)
+#pragma unroll
+            for (int u = 0; u < kLpVecs; ++u) {
+              float g[VE];
+              unpack(v[u], g);
+#pragma unroll
+              for (int e = 0; e < VE; ++e) s += g[e] == m ? 1.f : 0.f;
+            }
+        }
+        // ---- candidates
+        if constexpr (TOP) {
+          if (first) {
+            // the k-th of the warp's 32 * kLpVecs vector maxima: k values lie at or above it
+            uint32_t kq[kLpVecs];
+#pragma unroll
+            for (int u = 0; u < kLpVecs; ++u) kq[u] = q[u] > -0x1p126f ? beam_logit_key(q[u]) : 0u;
+            const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(kq[0], kq[1]), max(kq[2], kq[3])));
+            // 32 lanes reach the least of their maxima; for more than 32 the least of all bounds the k-th
+            const uint32_t least = __reduce_min_sync(0xffffffffu, p.k <= 32 ? max(max(kq[0], kq[1]), max(kq[2], kq[3]))
+                                                                            : min(min(kq[0], kq[1]), min(kq[2], kq[3])));
+            const uint32_t cut = beam_search(p.k, least, most, kLow, [&](uint32_t x) {
+              uint32_t n = 0;
+#pragma unroll
+              for (int u = 0; u < kLpVecs; ++u) n += kq[u] >= x ? 1u : 0u;
+              return int(__reduce_add_sync(0xffffffffu, n));
+            });
+            if (lane == 0) atomicMax(floor_key, cut);
+            l.least = max(l.least, cut);
+          }
+          l.least = max(l.least, *static_cast<volatile uint32_t*>(floor_key));
+          const float ge = beam_key_val(l.least);
+          // (q is -2^126 where a vector holds nothing above it: its values are then looked at one by one)
+          if (__any_sync(0xffffffffu, top >= ge || !(ge > -0x1p126f))) {
+            uint32_t mine = 0;  // this lane's values that enter
+#pragma unroll
+            for (int u = 0; u < kLpVecs; ++u) {
+              if (!__any_sync(0xffffffffu, q[u] >= ge || !(ge > -0x1p126f))) continue;
+              float g[VE];
+              unpack(v[u], g);
+#pragma unroll
+              for (int e = 0; e < VE; ++e) mine |= g[e] >= ge ? 1u << (u * VE + e) : 0u;
+            }
+            while (true) {  // one value of each lane at a time
+              const uint32_t b = __ballot_sync(0xffffffffu, mine != 0);
+              if (!b) break;
+              if (mine) {
+                const int i = __ffs(mine) - 1, u = i / VE, e = i - u * VE;
+                mine &= mine - 1;
+                const uint4 x = u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : v[3];
+                const int word = e * int(sizeof(T)) / 4;
+                const uint32_t bits = word == 0 ? x.x : word == 1 ? x.y : word == 2 ? x.z : x.w;
+                const float val = sizeof(T) == 4 ? __uint_as_float(bits) : __uint_as_float(e & 1 ? bits & 0xFFFF0000u : bits << 16);
+                const uint32_t id = uint32_t(p.vstart + col + u * 32 * VE + e);
+                l.buf[l.n + __popc(b & ((1u << lane) - 1u))] = beam_key(beam_logit_key(val), id);
+              }
+              l.n += __popc(b);
+              __syncwarp();
+              if (l.n > kBeamCap - 32) beam_cut<kLow>(l, p.k, floor_key);
+            }
+            // later columns have higher ids: they have to beat the k-th, not to equal it
+            if (l.kth) l.least = max(l.least, l.kth + 1);
+          }
+        }
+      };
+      constexpr uint32_t kNone = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;  // -inf
+      auto edge = [&](int n, int col) {  // columns col .. col + n - 1, n < VE
+        uint4 v[kLpVecs];
+#pragma unroll
+        for (int u = 0; u < kLpVecs; ++u) {
+          float g[VE];
+#pragma unroll
+          for (int e = 0; e < VE; ++e) g[e] = u == 0 && e == 0 && lane < n ? to_f(w.x[col + lane]) : -INFINITY;
+          v[u] = pack_vec(g);
+        }
+        step(v, col + lane, false);
+      };
+      if (warp == 0 && tile == 0 && w.head) edge(w.head, 0);
+      bool first = true;
+      for (; tile < end; ++tile) {
+        const int n = min(kLpTile, w.nvec - tile * kLpTile), at = warp * 32 * kLpVecs + lane;
+        if (n <= 0) continue;
+        ok = ok && mbar_wait_lean(full + sg, phase, abort);
+        if (!__all_sync(0xffffffffu, ok)) {
+          *abort = 1;
+          ok = false;
+        }
+        uint4 v[kLpVecs];
+#pragma unroll
+        for (int u = 0; u < kLpVecs; ++u)
+          v[u] = ok && at + 32 * u < n ? ring[sg * kLpTile + at + 32 * u] : make_uint4(kNone, kNone, kNone, kNone);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + sg);
+        if (++sg == NS) {
+          sg = 0;
+          phase ^= 1u;
+        }
+        if (at - lane < n) step(v, w.head + (tile * kLpTile + at) * VE, first);
+        first = false;
+      }
+      if (warp == kLpWarps - 1 && end == p.plan.tiles && w.tail) edge(w.tail, p.V - w.tail);
+      // ---- the part's statistics
+      float cm = m;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
+      if (!beam_far(m)) {  // against m itself, in natural units
+        const float d = fmaf(m, kBeamLog2e, -c), a = exp2_approx(-d);
+        ws = fmaf(-d, s, ws) * a * 0.69314718055994530942f;
+        s *= a;
+      }
+      // sums against m as sums against the larger top
+      auto raise = [](float mm, float top, float& ss, float& ww) {
+        if (mm == top) return;
+        const float d = mm - top, a = exp2_approx(d * kBeamLog2e);
+        ww = a > 0.f ? fmaf(d, ss, ww) * a : 0.f;
+        ss *= a;
+      };
+      raise(m, cm, s, ws);
+      s = warp_sum(s);
+      ws = warp_sum(ws);
+      if (lane == 0) stat[warp] = LpStat{cm, s, ws, 0.f};
+      const size_t at = size_t(row) * p.plan.parts + size_t(blockIdx.x - p.plan.first(row));
+      if constexpr (TOP) {
+        // ---- its k best: the warps' candidates (at most 64 each) from the common floor on, ranked
+        if (l.n > kLpMaxK) beam_cut<kLow>(l, p.k, floor_key);
+        named_sync(1, kLpThreads);
+        const uint32_t fk = *floor_key;
+        for (int i = lane; i < l.n; i += 32) {
+          const uint64_t o = l.buf[i];
+          if (uint32_t(o >> 32) >= fk) all[atomicAdd(totals + odd, 1)] = o;
+        }
+        named_sync(1, kLpThreads);
+        const int n = totals[odd];
+        uint64_t* out = p.cand + at * p.k;
+        for (int i = threadIdx.x; i < n; i += kLpThreads) {
+          const uint64_t o = all[i];
+          int rank = 0;
+          for (int j = 0; j < n; ++j) rank += all[j] > o ? 1 : 0;
+          if (rank < p.k) out[rank] = o;
+        }
+        for (int i = n + threadIdx.x; i < p.k; i += kLpThreads) out[i] = 0;
+      } else {
+        named_sync(1, kLpThreads);
+      }
+      if (threadIdx.x == 0) {
+        LpStat r{-INFINITY, 0.f, 0.f, xt};
+#pragma unroll
+        for (int u = 0; u < kLpWarps; ++u) r.m = fmaxf(r.m, stat[u].m);
+#pragma unroll
+        for (int u = 0; u < kLpWarps; ++u) {
+          float ss = stat[u].s, ww = stat[u].w;
+          raise(stat[u].m, r.m, ss, ww);
+          r.s += ss;
+          r.w += ww;
+        }
+        p.stat[at] = r;
+        floors[odd ^ 1] = 0;  // (the part before's, which nobody reads any more)
+        totals[odd ^ 1] = 0;
+      }
+      named_sync(1, kLpThreads);  // the next part's lists and statistics
+    }
   }
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort) atomicOr(&g_lp_status, kStatusTimeout);
 }
 
 struct LpJoinParams {
-  const LpStat* stat;    // [parts][rows][nchunk]
-  const uint64_t* cand;  // [parts][rows][nchunk][kc]
-  size_t stat_part, cand_part;  // elements between the shards' blocks
-  int parts, rows, nchunk, k, kc;
-  const long long* targets;  // [rows] or NULL
+  const LpStat* stat;    // [shards][rows][parts]
+  const uint64_t* cand;  // [shards][rows][parts][kc]
+  size_t stat_shard, cand_shard;  // elements between the shards' blocks
+  LpPlan plan;
+  int shards, rows, k, kc;
   float *logprobs, *entropy;  // [rows]; logprobs NULL without targets
   float* top_logprobs;        // [rows][k]
   long long* top_ids;
 };
 
 constexpr int kLpJoinWarps = 4;
-constexpr int kLpMaxLists = 64 * 32;  // shards x chunks
 
-// A warp a row, in fp64. The lists of the chunks are sorted: the best of their
-// heads is the next, k times.
+// A warp a row, in fp64. The parts' lists are sorted: the best of their heads
+// is the next, k times.
 __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoinParams p) {
   extern __shared__ uint8_t lp_heads[];  // [warps][lists]: entries of each list that were taken
   pdl_launch();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lists = p.parts * p.nchunk;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t row = size_t(blockIdx.x) * kLpJoinWarps + warp;
-  if (row >= p.rows) return;
-  auto stat = [&](int i) { return p.stat + (i / p.nchunk) * p.stat_part + row * p.nchunk + i % p.nchunk; };
-  auto cand = [&](int i) { return p.cand + (i / p.nchunk) * p.cand_part + (row * p.nchunk + i % p.nchunk) * p.kc; };
+  if (row >= size_t(p.rows)) return;
+  const int per = p.plan.count((long long)row), lists = p.shards * per;
+  auto stat = [&](int i) { return p.stat + (i / per) * p.stat_shard + row * p.plan.parts + i % per; };
+  auto cand = [&](int i) { return p.cand + (i / per) * p.cand_shard + (row * p.plan.parts + i % per) * p.kc; };
   float m = -INFINITY, xt = -INFINITY;
   bool found = false;
   for (int i = lane; i < lists; i += 32) {
     const LpStat s = *stat(i);
-    m = fmaxf(m, s.m);
+    if (s.s > 0.f) m = fmaxf(m, s.m);
     if (s.xt == s.xt) {
       xt = s.xt;
       found = true;
@@ -159,7 +448,7 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
   double sum = 0.0, w = 0.0;
   for (int i = lane; i < lists; i += 32) {
     const LpStat s = *stat(i);
-    if (s.m == -INFINITY) continue;
+    if (!(s.s > 0.f)) continue;
     const double d = s.m == m ? 0.0 : double(s.m) - double(m), e = exp(d);
     sum += e * s.s;
     if (e > 0.0) w += e * (double(s.w) + d * s.s);
@@ -179,7 +468,7 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
     if (p.logprobs) p.logprobs[row] = found ? logp(xt) : __int_as_float(0x7fffffff);
   }
   if (!p.k) return;
-  uint8_t* head = lp_heads + warp * lists;
+  uint8_t* head = lp_heads + warp * (p.shards * p.plan.parts);
   for (int i = lane; i < lists; i += 32) head[i] = 0;
   for (int j = 0; j < p.k; ++j) {
     uint64_t b = 0;
@@ -191,10 +480,10 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
         at = i;
       }
     }
-    const uint64_t top = lp_warp_max(b);
+    const uint64_t top = warp_max_u64(b);
     if (top && b == top) ++head[at];
     if (lane == 0) {
-      p.top_logprobs[row * p.k + j] = top ? logp(lp_key_val(top)) : -INFINITY;
+      p.top_logprobs[row * p.k + j] = top ? logp(beam_key_val(uint32_t(top >> 32))) : -INFINITY;
       p.top_ids[row * p.k + j] = top ? (long long)(0xFFFFFFFFu - uint32_t(top)) : 0;
     }
   }

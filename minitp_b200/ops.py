@@ -503,15 +503,15 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     out = _logprob_outputs(dev, logits.shape[:-1], targets, top)
     if rows == 0:
         return out
-    block = torch.empty_strided((logprobs_block_bytes(rows, v, top),), (1,), dtype=torch.uint8, device=dev)
+    block = torch.empty_strided((logprobs_block_bytes(rows, v, top, x.dtype),), (1,), dtype=torch.uint8, device=dev)
     _call_on(dev, "mtpb_token_logprobs", x.data_ptr(), ld, rows, v, _lib.ptr(targets), top, _lib.ptr(out[0]),
              out[1].data_ptr(), _lib.ptr(out[2]), _lib.ptr(out[3]), block.data_ptr(), _lib.dtype_code(x.dtype))
     return out
 
 
-def logprobs_block_bytes(rows: int, v_plan: int, top: int) -> int:
+def logprobs_block_bytes(rows: int, v_plan: int, top: int, dtype: torch.dtype) -> int:
     """Bytes of one shard's block (``logprobs_block``)."""
-    n = _lib.load().mtpb_logprobs_block_bytes(rows, v_plan, top)
+    n = _lib.load().mtpb_logprobs_block_bytes(rows, v_plan, top, _lib.dtype_code(dtype))
     if n < 0:
         _lib.check(n)
     return n
@@ -528,14 +528,16 @@ def logprobs_block(local_logits: torch.Tensor, targets: torch.Tensor | None, top
     rows, v = x.shape
     if rows == 0:
         return torch.empty(0, dtype=torch.uint8, device=dev)
-    block = torch.empty(logprobs_block_bytes(rows, v_plan, top), dtype=torch.uint8, device=dev)
+    block = torch.empty(logprobs_block_bytes(rows, v_plan, top, x.dtype), dtype=torch.uint8, device=dev)
     _call_on(dev, "mtpb_logprobs_block", x.data_ptr(), ld, rows, v, vstart, v_plan, _lib.ptr(targets), top,
              block.data_ptr(), _lib.dtype_code(x.dtype))
     return block
 
 
-def logprobs_join(blocks: torch.Tensor, targets: torch.Tensor | None, shape, top: int, v_plan: int):
-    """``token_logprobs``'s result for rows of ``shape`` from the blocks ``[shards, n]`` of every vocabulary shard."""
+def logprobs_join(blocks: torch.Tensor, targets: torch.Tensor | None, shape, top: int, v_plan: int,
+                  dtype: torch.dtype):
+    """``token_logprobs``'s result for rows of ``shape`` from the blocks ``[shards, n]`` of every vocabulary shard
+    (of logits of ``dtype``)."""
     dev = _same_device("logprobs_join", blocks, targets)
     shape = torch.Size(shape)
     rows = shape.numel()
@@ -543,14 +545,14 @@ def logprobs_join(blocks: torch.Tensor, targets: torch.Tensor | None, shape, top
         raise _lib.MinitpB200Error(f"logprobs_join: targets must be int64 {tuple(shape)}")
     if not (0 <= top <= 64 and 1 <= v_plan < 2**30):
         raise _lib.MinitpB200Error(f"logprobs_join: need 0..64 alternatives, got {top}")
-    need = logprobs_block_bytes(rows, v_plan, top) if rows else 0
+    need = logprobs_block_bytes(rows, v_plan, top, dtype) if rows else 0
     if blocks.dim() != 2 or blocks.dtype != torch.uint8 or not blocks.is_contiguous() or blocks.shape[1] != need:
         raise _lib.MinitpB200Error(
-            "logprobs_join: blocks must be contiguous uint8 [shards, logprobs_block_bytes(rows, v_plan, top)]")
+            "logprobs_join: blocks must be contiguous uint8 [shards, logprobs_block_bytes(rows, v_plan, top, dtype)]")
     out = _logprob_outputs(dev, shape, targets, top)
     if rows == 0:
         return out
     targets = None if targets is None else _c(targets)
     _call_on(dev, "mtpb_logprobs_join", blocks.data_ptr(), blocks.shape[0], rows, v_plan, top, _lib.ptr(targets), top,
-             _lib.ptr(out[0]), out[1].data_ptr(), _lib.ptr(out[2]), _lib.ptr(out[3]))
+             _lib.ptr(out[0]), out[1].data_ptr(), _lib.ptr(out[2]), _lib.ptr(out[3]), _lib.dtype_code(dtype))
     return out

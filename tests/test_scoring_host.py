@@ -35,10 +35,11 @@ def test_logprob_refusals(lib):
                           (dict(rows=(1 << 24) + 1), "rows"), (dict(V=0), "vocabulary"), (dict(V=1 << 30), "vocabulary"),
                           (dict(ld=99), "ld"), (dict(dtype=7), "dtype"), (dict(block=P + 8), "aligned")]:
         _refused(lib, "mtpb_token_logprobs", list((ok | change).values()), match)
-    assert lib.mtpb_logprobs_block_bytes(8, 151936, 65) < 0
-    assert lib.mtpb_logprobs_block_bytes(0, 151936, 4) < 0
-    assert lib.mtpb_logprobs_block_bytes(8, 1 << 30, 4) < 0
-    assert 0 < lib.mtpb_logprobs_block_bytes(8, 151936, 0) < lib.mtpb_logprobs_block_bytes(8, 151936, 64)
+    assert lib.mtpb_logprobs_block_bytes(8, 151936, 65, 1) < 0
+    assert lib.mtpb_logprobs_block_bytes(0, 151936, 4, 1) < 0
+    assert lib.mtpb_logprobs_block_bytes(8, 1 << 30, 4, 0) < 0
+    assert 0 < lib.mtpb_logprobs_block_bytes(8, 151936, 0, 1) < lib.mtpb_logprobs_block_bytes(8, 151936, 64, 1)
+    assert lib.mtpb_logprobs_block_bytes(8, 151936, 4, 3) < 0
 
 
 def test_block_and_join_refusals(lib):
@@ -46,10 +47,10 @@ def test_block_and_join_refusals(lib):
     for change, match in [(dict(v=61), "V_plan"), (dict(v=-1), "V_plan"), (dict(vstart=-1), "range"),
                           (dict(vstart=2 ** 32), "range"), (dict(block=None), "null"), (dict(rows=0), "rows")]:
         _refused(lib, "mtpb_logprobs_block", list((ok | change).values()), match)
-    ok = dict(blocks=P, parts=2, rows=8, plan=60, kb=4, targets=P, k=4, lp=P, ent=P, tops=P, ids=P, st=None)
+    ok = dict(blocks=P, parts=2, rows=8, plan=60, kb=4, targets=P, k=4, lp=P, ent=P, tops=P, ids=P, dtype=0, st=None)
     for change, match in [(dict(parts=0), "shards"), (dict(parts=65), "shards"), (dict(k=5), "alternatives"),
                           (dict(blocks=None), "aligned"), (dict(lp=None), "null"), (dict(kb=65), "alternatives"),
-                          (dict(ent=None), "null")]:
+                          (dict(ent=None), "null"), (dict(dtype=2), "dtype")]:
         _refused(lib, "mtpb_logprobs_join", list((ok | change).values()), match)
 
 
@@ -62,4 +63,4 @@ def test_cpu_tensors_are_refused(lib):
     with pytest.raises(_lib.MinitpB200Error, match="CUDA"):
         ops.logprobs_block(torch.zeros(2, 10), None, 2, 0, 10)
     with pytest.raises(_lib.MinitpB200Error, match="CUDA"):
-        ops.logprobs_join(torch.zeros(2, 10, dtype=torch.uint8), None, (2,), 2, 10)
+        ops.logprobs_join(torch.zeros(2, 10, dtype=torch.uint8), None, (2,), 2, 10, torch.float32)
