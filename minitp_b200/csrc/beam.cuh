@@ -37,47 +37,7 @@ struct BeamRowsParams {
   uint64_t* cand;  // [rows][nchunk][k], best first, 0-padded
 };
 
-constexpr int kBeamThreads = 256;
-constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamVecs = 4;   // 16-byte vectors a lane and tile
-
-// Takes the candidates below `least` out of the warp's buffer.
-__device__ __forceinline__ void beam_drop(BeamList& l, uint32_t least) {
-  const int lane = threadIdx.x & 31;
-  int n = 0;
-  for (int i0 = 0; i0 < l.n; i0 += 32) {
-    const uint64_t o = i0 + lane < l.n ? l.buf[i0 + lane] : 0;
-    const bool in = uint32_t(o >> 32) >= least && o;
-    const uint32_t b = __ballot_sync(0xffffffffu, in);  // (reads of this step before its writes, which go no further)
-    if (in) l.buf[n + __popc(b & ((1u << lane) - 1u))] = o;
-    n += __popc(b);
-    __syncwarp();
-  }
-  l.n = n;
-}
-
-// The k-th key among the warps' candidates (at most 32 of each, a lane's keys
-// here), as the chunk's floor.
-template <int LOW>
-__device__ __forceinline__ void beam_floor(const uint32_t (&key)[kBeamWarps], int k, uint32_t* floor_key) {
-  uint32_t most = 0, least = 0xFFFFFFFFu;
-#pragma unroll
-  for (int w = 0; w < kBeamWarps; ++w) {
-    most = max(most, key[w]);
-    least = min(least, key[w] ? key[w] : 0xFFFFFFFFu);
-  }
-  most = __reduce_max_sync(0xffffffffu, most);
-  least = __reduce_min_sync(0xffffffffu, least);
-  auto above = [&](uint32_t x) {
-    uint32_t n = 0;
-#pragma unroll
-    for (int w = 0; w < kBeamWarps; ++w) n += key[w] >= x ? 1u : 0u;
-    return int(__reduce_add_sync(0xffffffffu, n));
-  };
-  if (least > most || above(least) < k) return;
-  const uint32_t cut = beam_search(k, least, most, LOW, above);
-  if ((threadIdx.x & 31) == 0) atomicMax(floor_key, cut);
-}
 
 // The chunk's 16-byte vectors come through a ring in shared memory, 16 KB
 // rounds filled by bulk copies (warp 8, which also finds the floors), so that what is in flight does not

@@ -77,7 +77,7 @@ int lp_join(const void* blocks, int shards, int rows, const LpPlan& b, int kc, c
   p.top_logprobs = top_logprobs;
   p.top_ids = reinterpret_cast<long long*>(top_ids);
   return host_launch(lp_join_kernel, dim3((rows + kLpJoinWarps - 1) / kLpJoinWarps), dim3(32 * kLpJoinWarps),
-                     size_t(k ? kLpJoinWarps : 0) * shards * b.parts, st, p);
+                     size_t(k ? kLpJoinWarps : 0) * (kLpRanked * 8 + size_t(shards) * b.parts), st, p);
 }
 
 int join_check(const int64_t* targets, int k, const float* logprobs, const float* entropy, const float* top_logprobs,

@@ -28,7 +28,7 @@ struct LpStat {
   float m, s, w, xt;
 };
 
-constexpr int kLpWarps = 8;   // that compute; one more copies
+constexpr int kLpWarps = kBeamWarps;  // that compute; one more copies and finds the floors
 constexpr int kLpVecs = 4;    // 16-byte vectors a lane and tile
 constexpr int kLpTile = kLpWarps * 32 * kLpVecs;  // vectors
 // Ring of tiles: what three CTAs an SM leave beside the candidates.
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
   __shared__ uint64_t full[NS], empty[NS];
   __shared__ LpStat stat[kLpWarps];
   __shared__ uint32_t floors[2];  // by the part's parity: at least k of its values have this key or a higher one
-  __shared__ int totals[2], abort_sh;
+  __shared__ int totals[2], count[kLpWarps], abort_sh;
   volatile int* abort = &abort_sh;
   pdl_launch();
   pdl_wait();
@@ -115,46 +115,79 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
   int row = int(t0 / p.plan.tiles), tile = int(t0 - (long long)row * p.plan.tiles);
   int sg = 0;
   uint32_t phase = 0;
-  if (warp == kLpWarps) {  // ---- copies
-    if (lane == 0) {
-      int issued = 0;
-      bool ok = true;
-      for (long long t = t0; ok && t < t1; ++row, tile = 0) {
-        const Row w = row_at(row);
-        for (; ok && tile < p.plan.tiles && t < t1; ++tile, ++t) {
-          const int n = min(kLpTile, w.nvec - tile * kLpTile);
-          if (n <= 0) continue;  // (a shard of fewer columns than planned for)
-          ok = issued < NS || mbar_wait_lean(empty + sg, phase ^ 1u, abort);
-          if (!ok) break;
-          mbar_arrive_expect_tx(full + sg, uint32_t(n) * 16);
-          bulk_g2s(ring + sg * kLpTile, w.x + w.head + int64_t(tile) * kLpTile * VE, uint32_t(n) * 16, full + sg);
-          if (issued < NS) ++issued;
-          if (++sg == NS) {
-            sg = 0;
-            phase ^= 1u;
-          }
+  // After the tiles 0 and 3 of a part the k-th of all warps' candidates becomes
+  // the floor: a later value enters with odds k / (values seen by the CTA), not
+  // k / (values of one warp's first tile). (After 0, 1, 3, 7 .. as well: 1 to 3 %
+  // slower; never: 512 rows with 20 alternatives 90 us and not 76.)
+  auto refloor = [](int i, int last) { return TOP && i < last && (i == 0 || i == 3); };
+  if (warp == kLpWarps) {  // ---- copies, a ring ahead of the tiles that the others are at, and floors
+    int row2 = row, tile2 = tile, issued = 0, s2 = 0;  // of the next copy
+    uint32_t ph2 = 0;
+    long long t2 = t0;
+    Row w2 = row_at(row2);
+    bool ok = true;
+    auto copy = [&]() {  // (skips tiles that the shard, of fewer columns than planned for, does not have)
+      while (t2 < t1) {
+        const int n = min(kLpTile, w2.nvec - tile2 * kLpTile);
+        const T* from = w2.x + w2.head + int64_t(tile2) * kLpTile * VE;
+        ++t2;
+        if (++tile2 == p.plan.tiles) {
+          tile2 = 0;
+          w2 = row_at(min(++row2, p.rows - 1));
         }
-      }
-      if (!ok) *abort = 1;
-      // copies in flight land before the memory goes away
-      int never = 0;
-      if (issued < NS) {
-        sg = 0;
-        phase = 0;
-      } else {
-        phase ^= 1u;
-      }
-      for (int i = 0; i < issued; ++i) {
-        mbar_wait_lean(full + sg, phase, &never);
-        if (++sg == NS) {
-          sg = 0;
-          phase ^= 1u;
+        if (n <= 0) continue;
+        ok = ok && (issued < NS || __all_sync(0xffffffffu, mbar_wait_lean(empty + s2, ph2 ^ 1u, abort)));
+        if (!ok) {
+          *abort = 1;
+          return;
         }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(full + s2, uint32_t(n) * 16);
+          bulk_g2s(ring + s2 * kLpTile, from, uint32_t(n) * 16, full + s2);
+        }
+        __syncwarp();
+        if (issued < NS) ++issued;
+        if (++s2 == NS) {
+          s2 = 0;
+          ph2 ^= 1u;
+        }
+        return;
+      }
+    };
+    for (int i = 0; i < NS; ++i) copy();
+    int odd = 0;
+    for (long long t = t0; t < t1; ++row, tile = 0, odd ^= 1) {
+      const int n = int(min((long long)p.plan.tiles - tile, t1 - t));
+      t += n;
+      for (int i = 0; i < n; ++i) {
+        if (refloor(i, n - 1)) {
+          named_sync(2, kLpThreads + 32);
+          uint32_t key[kLpWarps];
+#pragma unroll
+          for (int u = 0; u < kLpWarps; ++u) key[u] = lane < count[u] ? uint32_t(buf[TOP ? u : 0][TOP ? lane : 0] >> 32) : 0;
+          named_sync(2, kLpThreads + 32);  // the lists may change again
+          beam_floor<kLow>(key, p.k, floors + odd);
+        }
+        copy();
+      }
+    }
+    // copies in flight land before the memory goes away
+    int never = 0;
+    if (issued < NS)
+      s2 = 0, ph2 = 0;
+    else
+      ph2 ^= 1u;
+    for (int i = 0; i < issued; ++i) {
+      mbar_wait_lean(full + s2, ph2, &never);
+      if (++s2 == NS) {
+        s2 = 0;
+        ph2 ^= 1u;
       }
     }
   } else {
     bool ok = true;
     int odd = 0;  // parity of the part
+    long long next_goal = threadIdx.x == 0 && p.targets ? p.targets[row] : 0;
     for (long long t = t0; t < t1; ++row, tile = 0, odd ^= 1) {
       uint32_t* floor_key = floors + odd;
       // ---- this CTA's part of a row
@@ -163,14 +196,12 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
       const int c0 = tile == 0 ? 0 : min(p.V, w.head + tile * kLpTile * VE);
       const int c1 = end == p.plan.tiles ? p.V : min(p.V, w.head + end * kLpTile * VE);
       t += end - tile;
-      float xt = __int_as_float(0x7fffffff);
-      if (threadIdx.x == 0 && p.targets) {
-        const long long c = p.targets[row] - p.vstart;
-        if (c >= c0 && c < c1) {
-          xt = to_f(w.x[c]);
-          if (xt != xt) xt = -INFINITY;
-        }
-      }
+      // (the target's logit is not looked at before the part's end, and the next row's target read ahead)
+      float xt = 0.f;
+      const long long goal = next_goal - p.vstart;
+      const bool here = threadIdx.x == 0 && p.targets && goal >= c0 && goal < c1;
+      if (here) xt = to_f(w.x[goal]);
+      if (threadIdx.x == 0 && p.targets && t < t1) next_goal = p.targets[row + 1];
       BeamList l{TOP ? buf[warp] : nullptr, 0, 0x00800000u, 0u};  // least: the key of the lowest finite value
       float m = -INFINITY, c = 0.f, s = 0.f, ws = 0.f;
       // a tile: vector u of this lane holds columns col + u * 32 * VE ..
@@ -196,6 +227,8 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
           }
         }
         float top = fmaxf(max3(q[0], q[1], q[2]), q[3]);
+        // (read early: an older floor is a floor too)
+        const uint32_t common = TOP ? *static_cast<volatile uint32_t*>(floor_key) : 0u;
         // ---- sums
         if (!beam_far(fmaxf(m, top))) {
           if (top - m > 8.f) {
@@ -268,7 +301,7 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
             if (lane == 0) atomicMax(floor_key, cut);
             l.least = max(l.least, cut);
           }
-          l.least = max(l.least, *static_cast<volatile uint32_t*>(floor_key));
+          l.least = max(l.least, common);
           const float ge = beam_key_val(l.least);
           // (q is -2^126 where a vector holds nothing above it: its values are then looked at one by one)
           if (__any_sync(0xffffffffu, top >= ge || !(ge > -0x1p126f))) {
@@ -317,9 +350,19 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
       };
       if (warp == 0 && tile == 0 && w.head) edge(w.head, 0);
       bool first = true;
-      for (; tile < end; ++tile) {
+      for (int i = 0, last = end - 1 - tile; tile < end; ++tile, ++i) {
         const int n = min(kLpTile, w.nvec - tile * kLpTile), at = warp * 32 * kLpVecs + lane;
-        if (n <= 0) continue;
+        auto join_floor = [&]() {
+          if (!refloor(i, last)) return;
+          beam_drop(l, *static_cast<volatile uint32_t*>(floor_key));
+          if (lane == 0) count[warp] = l.n;
+          named_sync(2, kLpThreads + 32);
+          named_sync(2, kLpThreads + 32);
+        };
+        if (n <= 0) {
+          join_floor();
+          continue;
+        }
         ok = ok && mbar_wait_lean(full + sg, phase, abort);
         if (!__all_sync(0xffffffffu, ok)) {
           *abort = 1;
@@ -337,6 +380,7 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
         }
         if (at - lane < n) step(v, w.head + (tile * kLpTile + at) * VE, first);
         first = false;
+        join_floor();
       }
       if (warp == kLpWarps - 1 && end == p.plan.tiles && w.tail) edge(w.tail, p.V - w.tail);
       // ---- the part's statistics
@@ -382,20 +426,24 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
       } else {
         named_sync(1, kLpThreads);
       }
-      if (threadIdx.x == 0) {
-        LpStat r{-INFINITY, 0.f, 0.f, xt};
+      if (warp == 0) {
+        LpStat r = stat[lane & (kLpWarps - 1)];
+        float top = r.m;
 #pragma unroll
-        for (int u = 0; u < kLpWarps; ++u) r.m = fmaxf(r.m, stat[u].m);
+        for (int o = kLpWarps / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        raise(r.m, top, r.s, r.w);
 #pragma unroll
-        for (int u = 0; u < kLpWarps; ++u) {
-          float ss = stat[u].s, ww = stat[u].w;
-          raise(stat[u].m, r.m, ss, ww);
-          r.s += ss;
-          r.w += ww;
+        for (int o = kLpWarps / 2; o > 0; o >>= 1) {
+          r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+          r.w += __shfl_xor_sync(0xffffffffu, r.w, o);
         }
-        p.stat[at] = r;
-        floors[odd ^ 1] = 0;  // (the part before's, which nobody reads any more)
-        totals[odd ^ 1] = 0;
+        if (lane == 0) {
+          r.m = top;
+          r.xt = !here ? __int_as_float(0x7fffffff) : xt == xt ? xt : -INFINITY;
+          p.stat[at] = r;
+          floors[odd ^ 1] = 0;  // (the part before's, which nobody reads any more)
+          totals[odd ^ 1] = 0;
+        }
       }
       named_sync(1, kLpThreads);  // the next part's lists and statistics
     }
@@ -416,11 +464,11 @@ struct LpJoinParams {
 };
 
 constexpr int kLpJoinWarps = 4;
+constexpr int kLpRanked = 512;  // candidates of a row that are ranked against each other
 
-// A warp a row, in fp64. The parts' lists are sorted: the best of their heads
-// is the next, k times.
+// A warp a row, in fp64.
 __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoinParams p) {
-  extern __shared__ uint8_t lp_heads[];  // [warps][lists]: entries of each list that were taken
+  extern __shared__ uint64_t lp_cands[];  // [warps][kLpRanked]; then [warps][lists] bytes: entries of each list that were taken
   pdl_launch();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -468,7 +516,66 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
     if (p.logprobs) p.logprobs[row] = found ? logp(xt) : __int_as_float(0x7fffffff);
   }
   if (!p.k) return;
-  uint8_t* head = lp_heads + warp * (p.shards * p.plan.parts);
+  const int n = lists * p.kc;
+  uint64_t* mine = lp_cands + warp * kLpRanked;
+  if (n <= kLpRanked) {
+    auto load = [&](int i) -> uint64_t {
+      return i < n ? __ldcg(reinterpret_cast<const unsigned long long*>(cand(i / p.kc)) + i % p.kc) : 0;
+    };
+    int m2 = n;  // candidates left in `mine`
+    if (n <= 64) {
+      for (int i = lane; i < n; i += 32) mine[i] = load(i);
+    } else {  // those below the k-th go first
+      constexpr int H = kLpRanked / 32;
+      uint64_t held[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) held[h] = load(lane + 32 * h);
+      uint32_t most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const uint32_t v = uint32_t(held[h] >> 32);
+        most = max(most, v);
+        least = min(least, v);
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      least = __reduce_min_sync(0xffffffffu, least);
+      const uint32_t cut = beam_search(p.k, least, most, 0, [&](uint32_t v) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int h = 0; h < H; ++h) c += uint32_t(held[h] >> 32) >= v ? 1u : 0u;
+        return int(__reduce_add_sync(0xffffffffu, c));
+      });
+      m2 = 0;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const bool in = held[h] && uint32_t(held[h] >> 32) >= cut;
+        const uint32_t b = __ballot_sync(0xffffffffu, in);
+        if (in) mine[m2 + __popc(b & ((1u << lane) - 1u))] = held[h];
+        m2 += __popc(b);
+      }
+    }
+    __syncwarp();
+    int live = 0;
+    for (int i = lane; i < m2; i += 32) {
+      const uint64_t o = mine[i];
+      if (!o) continue;
+      ++live;
+      int place = 0;  // how many are better
+      for (int j = 0; j < m2; ++j) place += mine[j] > o ? 1 : 0;
+      if (place < p.k) {
+        p.top_logprobs[row * p.k + place] = logp(beam_key_val(uint32_t(o >> 32)));
+        p.top_ids[row * p.k + place] = (long long)(0xFFFFFFFFu - uint32_t(o));
+      }
+    }
+    live = __reduce_add_sync(0xffffffffu, live);
+    for (int j = live + lane; j < p.k; j += 32) {
+      p.top_logprobs[row * p.k + j] = -INFINITY;
+      p.top_ids[row * p.k + j] = 0;
+    }
+    return;
+  }
+  // many lists (few rows, or many shards): they are sorted, the best of their heads is the next
+  uint8_t* head = reinterpret_cast<uint8_t*>(lp_cands + kLpJoinWarps * kLpRanked) + warp * (p.shards * p.plan.parts);
   for (int i = lane; i < lists; i += 32) head[i] = 0;
   for (int j = 0; j < p.k; ++j) {
     uint64_t b = 0;
