@@ -434,6 +434,18 @@ int mtpb_model_forward_shared(void* model, const int64_t* ids, int N, int T,
                               const int* prefix_lens, int prefix_len, int G, int cap_p,
                               void* logits, int last_only, void* stream);
 
+/* Forward of prompts of different lengths packed into one row of T tokens
+ * (seq_starts, S: as mtpb_prompt_attention), for scoring: no logits, no cache
+ * kept. ids device int64 [T]; rope_pos device int64 [T], a token's place in its
+ * prompt; k_scratch, v_scratch: host arrays of n_layers device pointers, each to
+ * [hkv, T, hd]: a layer's K and V while it runs. They may all be the same as long
+ * as T * H * sizeof(dtype) is at most mtpb_comm_slot_bytes; more tokens go in
+ * chunks, whose later ones read what the earlier left. hidden [T, H]: the final norm's output, which the LM head takes. Tokens of no
+ * prompt attend to nothing. No counterpart in the reference. */
+int mtpb_model_forward_packed(void* model, const int64_t* ids, int T, const int64_t* rope_pos,
+                              const int* seq_starts, int S, void* const* k_scratch,
+                              void* const* v_scratch, void* hidden, void* stream);
+
 /* One greedy decode step for B rows, all state on the device: reads the
  * tokens from `tok` (device int64 [B]) and the position from
  * mtpb_comm_pos_ptr(), runs the model, selects the next tokens (distributed

@@ -776,6 +776,13 @@ struct SharedPrefix {
   const void* const* v;
 };
 
+// Prompts of different lengths packed into one row (mtpb_model_forward_packed).
+struct PackedPrompts {
+  const int* starts;  // device [S + 1]
+  int S;
+  void* hidden;  // [T][H]: the final norm's output, in the place of logits
+};
+
 struct FwdArgs {
   const long long* ids;  // embedding input [M]
   int B, T;
@@ -792,6 +799,7 @@ struct FwdArgs {
   long long* out_ids;
   int ld_out;
   const SharedPrefix* shared;  // rows attend to a shared prefix as well (NULL: to their own cache only)
+  const PackedPrompts* packed;  // B = 1: the row holds several prompts (NULL: one)
 };
 
 // The attention of layer l over tokens [pos, pos + tc) of every row (pos:
@@ -822,6 +830,31 @@ SharedAttnArgs shared_args(const ModelHost& mh, const FwdArgs& a, int l, int tc,
   s.dtype = d.dtype;
   s.status = mh.comm->dev.status();
   return s;
+}
+
+// The attention of layer l over the packed tokens [t0, t0 + tc).
+PromptAttnArgs packed_args(const ModelHost& mh, const FwdArgs& a, int l, int t0, int tc) {
+  const mtpb_model_desc& d = mh.d;
+  PromptAttnArgs p;
+  p.q = mh.q;
+  p.q_token = (long long)d.hq_local * d.head_dim;
+  p.q_head = d.head_dim;
+  p.k = a.kc[l];
+  p.v = a.vc[l];
+  p.k_token = p.v_token = d.head_dim;
+  p.k_head = p.v_head = (long long)a.cap * d.head_dim;
+  p.out = mh.attn;
+  p.seq_starts = a.packed->starts;
+  p.S = a.packed->S;
+  p.first = t0;
+  p.n = tc;
+  p.total = a.T;
+  p.hq = d.hq_local;
+  p.hkv = d.hkv_local;
+  p.hd = d.head_dim;
+  p.dtype = d.dtype;
+  p.status = mh.comm->dev.status();
+  return p;
 }
 
 // Workspace of the shared-prefix attention for chunks of tc tokens a row (and a last one of the rest).
@@ -961,6 +994,8 @@ int model_chunk_t(ModelHost& mh, const FwdArgs& a, int t0, int tc, bool last_chu
     if (a.shared) {
       const SharedAttnArgs sa = shared_args(mh, a, l, tc, pos_base);
       MTPB_TRY(shared_attn_run(sa, mh.sa_ws, mh.sa_bytes, st));
+    } else if (a.packed) {
+      MTPB_TRY(prompt_attn_run(packed_args(mh, a, l, t0, tc), st));
     } else {
       MTPB_TRY(attn_run(d.dtype, mh.q, a.kc[l], a.vc[l], mh.attn, a.B, tc, hq, hkv, hd, a.cap, a.pos_ptr,
                         pos_base, mh.ascr, comm.status(), st));
@@ -1002,6 +1037,16 @@ int model_chunk_t(ModelHost& mh, const FwdArgs& a, int t0, int tc, bool last_chu
     }
   }
 
+  if (a.packed) {  // the final norm alone, consuming site 2L
+    ConsumeRowsParams cp;
+    cp.g = gemv_base(d.lm_head, nullptr, M, vloc, H, vloc);
+    consume_into(cp.g, uint32_t(2 * L), d.final_norm);
+    cp.g.M = M;
+    cp.g.K = H;
+    cp.xn = static_cast<char*>(a.packed->hidden) + size_t(t0) * H * sizeof(T);
+    cp.ts_cols = ts;
+    return consume_rows_run(d.dtype, cp, st);
+  }
   // final norm + LM head, consuming site 2L. With last_only, only the last
   // chunk computes logits, and only for the last token of each batch row.
   if (a.last_only && !last_chunk) return MTPB_OK;
@@ -1845,6 +1890,39 @@ int mtpb_model_forward_shared(void* model, const int64_t* ids, int N, int T, con
   a.logits = logits;
   a.last_only = last_only;
   a.shared = &sp;
+  return model_forward(*mh, a, static_cast<cudaStream_t>(stream));
+}
+
+int mtpb_model_forward_packed(void* model, const int64_t* ids, int T, const int64_t* rope_pos, const int* seq_starts,
+                              int S, void* const* k_scratch, void* const* v_scratch, void* hidden, void* stream) {
+  if (!model || !ids || !rope_pos || !seq_starts || !k_scratch || !v_scratch || !hidden)
+    return fail(MTPB_ERR_INVALID, "model_forward_packed: null argument");
+  if (T <= 0 || S < 0) return fail(MTPB_ERR_INVALID, "model_forward_packed: empty batch");
+  auto* mh = static_cast<ModelHost*>(model);
+  const size_t row = mh->d.hidden * dsize(mh->d.dtype);
+  if (row % 16 || !aligned16(hidden))
+    return fail(MTPB_ERR_INVALID, "model_forward_packed: hidden and its rows must be 16-byte aligned");
+  for (int l = 0; l < mh->d.n_layers; ++l) {
+    if (!k_scratch[l] || !v_scratch[l] || !aligned16(k_scratch[l]) || !aligned16(v_scratch[l]))
+      return fail(MTPB_ERR_INVALID, "model_forward_packed: scratch must be 16-byte aligned");
+    // in several chunks, a later one attends to what the earlier ones left of every layer
+    if (l > 0 && size_t(T) * row > mh->comm->dev.slot_bytes && (k_scratch[l] == k_scratch[0] || v_scratch[l] == v_scratch[0]))
+      return fail(MTPB_ERR_INVALID, "model_forward_packed: more tokens than one chunk need scratch of their own in every layer");
+  }
+  PackedPrompts pk;
+  pk.starts = seq_starts;
+  pk.S = S;
+  pk.hidden = hidden;
+  FwdArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.ids = reinterpret_cast<const long long*>(ids);
+  a.B = 1;
+  a.T = T;
+  a.rope_pos = reinterpret_cast<const long long*>(rope_pos);
+  a.kc = k_scratch;
+  a.vc = v_scratch;
+  a.cap = T;
+  a.packed = &pk;
   return model_forward(*mh, a, static_cast<cudaStream_t>(stream));
 }
 

@@ -224,6 +224,45 @@ class TPQwen2ForCausalLM(nn.Module):
             return self.lm_head.gather(out)
         return out
 
+    def forward_packed(self, input_ids: torch.Tensor, seq_starts: torch.Tensor,
+                       positions: torch.Tensor | None = None) -> torch.Tensor:
+        """The final norm's output ``[n, H]`` of prompts packed one behind the other (not in the reference).
+
+        ``input_ids [n]``; prompt s holds the tokens ``[seq_starts[s],
+        seq_starts[s + 1])`` (int32 ``[S + 1]`` on the device, non-decreasing) and
+        attends to itself alone. ``positions [n]`` default to the places in the
+        prompts. The result is what ``lm_head`` takes. No cache is kept.
+        """
+        _lib.require_cuda(input_ids, seq_starts)
+        if input_ids.dim() != 1 or input_ids.numel() < 1:
+            raise ValueError(f"input_ids must be [n] with at least one token, got {tuple(input_ids.shape)}")
+        if seq_starts.dtype != torch.int32 or seq_starts.dim() != 1 or seq_starts.numel() < 1 or \
+                not seq_starts.is_contiguous() or seq_starts.device != input_ids.device:
+            raise ValueError(f"seq_starts must be contiguous int32 [S + 1] on {input_ids.device}")
+        n, dev = input_ids.numel(), input_ids.device
+        h = self.native()
+        if dev != self.model.embed_tokens.weight.device:
+            raise ValueError(f"input_ids on {dev}, the model on {self.model.embed_tokens.weight.device}")
+        if positions is None:
+            tok = torch.arange(n, dtype=torch.int32, device=dev)
+            first = seq_starts[(torch.searchsorted(seq_starts, tok, right=True) - 1).clamp_(min=0)]
+            # (tokens of no prompt are read nowhere; their places need only be in the table)
+            positions = (tok - first).clamp_(0, self.cfg.max_position_embeddings - 1)
+        elif positions.shape != (n,) or positions.device != dev:
+            raise ValueError(f"positions must be [{n}] on {dev}, got {tuple(positions.shape)} on {positions.device}")
+        attn0, w = self.model.layers[0].self_attn, self.model.embed_tokens.weight
+        layers = self.cfg.num_hidden_layers
+        # every layer uses the same scratch, unless the tokens go in several chunks
+        one = n * self.cfg.hidden_size * w.element_size() <= self.ctx.comm().slot_bytes()
+        kv = torch.empty(1 if one else layers, 2, attn0.kv_heads_local, n, self.cfg.head_dim, dtype=w.dtype, device=dev)
+        k, v = ((ctypes.c_void_p * layers)(*[kv[0 if one else i, j].data_ptr() for i in range(layers)]) for j in (0, 1))
+        out = torch.empty(n, self.cfg.hidden_size, dtype=w.dtype, device=dev)
+        ids, pos = input_ids.to(torch.int64).contiguous(), positions.to(torch.int64).contiguous()
+        with torch.cuda.device(dev):
+            _lib.call("mtpb_model_forward_packed", h, ids.data_ptr(), n, pos.data_ptr(), seq_starts.data_ptr(),
+                      seq_starts.numel() - 1, k, v, out.data_ptr(), _lib.stream_ptr(dev))
+        return out
+
     def _forward_shared(self, ids: torch.Tensor, rope_pos: torch.Tensor, kv: KVCache, slot, prefix: KVCache,
                        logits: torch.Tensor, last_only: bool = True) -> None:
         """One forward of ``ids [N, T]`` behind ``prefix`` into ``logits`` (``mtpb_model_forward_shared``).

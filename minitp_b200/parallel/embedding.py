@@ -124,3 +124,19 @@ class VocabParallelLMHead(nn.Module):
         blocks = torch.empty(self.ctx.tp_size, mine.numel(), dtype=mine.dtype, device=mine.device)
         all_gather_dim0(blocks, mine, self.ctx.process_group)
         return ops.beam_pick(blocks, scores, k, plan, finished, eos_token_id)
+
+    @torch.no_grad()
+    def token_logprobs(self, local_logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0):
+        """Log-probabilities of ``targets``, entropy and top alternatives over the sharded vocab
+        (``ops.token_logprobs``), same on all ranks.
+
+        ``local_logits [..., V_local]``. With tp > 1 every rank reduces its shard to statistics and candidates,
+        and the ranks exchange those (not the logits).
+        """
+        if self.ctx.tp_size == 1:
+            return ops.token_logprobs(local_logits, targets, top)
+        plan = self._max_local_vocab()
+        mine = ops.logprobs_block(local_logits, targets, top, self.vocab_start, plan)
+        blocks = torch.empty(self.ctx.tp_size, mine.numel(), dtype=mine.dtype, device=mine.device)
+        all_gather_dim0(blocks, mine, self.ctx.process_group)
+        return ops.logprobs_join(blocks, targets, local_logits.shape[:-1], top, plan, local_logits.dtype)

@@ -1,0 +1,108 @@
+"""Scoring of given prompts: log-probabilities, entropies and top alternatives of their tokens (not in the reference).
+
+``score_prompts`` takes prompts of any lengths in one call. They are packed one
+behind the other, without padding, and run through the model in one forward
+(``TPQwen2ForCausalLM.forward_packed``, whose attention is ``ops.prompt_attention``);
+the LM head and ``VocabParallelLMHead.token_logprobs`` then take the tokens in
+pieces, so that no more than a few hundred megabytes of logits exist at once.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Sequence
+
+import torch
+
+from minitp_b200 import ops
+from minitp_b200.layer import TPQwen2ForCausalLM
+
+_LOGITS_BYTES = 256 << 20  # of one piece
+
+
+@dataclass
+class PromptScores:
+    """Of one prompt of n tokens: row i belongs to token i + 1, given the tokens before it.
+
+    ``logprobs`` and ``entropy`` fp32 ``[n - 1]`` (natural units), ``top_logprobs``
+    fp32 and ``top_ids`` int64 ``[n - 1, top]``, best first (None with ``top`` 0).
+    """
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+@torch.inference_mode()
+def score_prompts(
+    model: TPQwen2ForCausalLM,
+    prompts: Sequence[torch.Tensor | Sequence[int]],
+    top: int = 0,
+    max_tokens: int = 32768,
+) -> list[PromptScores]:
+    """Scores of every prompt's tokens, given the tokens before them.
+
+    ``prompts``: token ids, each a sequence of ints or an integer tensor ``[n]``
+    on any device; a prompt of one token or none has empty scores. ``top``: likeliest
+    alternatives per token (0 to 64). Prompts are packed into forwards of at most
+    ``max_tokens`` tokens (a longer prompt goes alone). The results are on the
+    model's device.
+    """
+    dev = model.model.embed_tokens.weight.device
+    if not 0 <= top <= 64:
+        raise ValueError(f"top must be 0 .. 64, got {top}")
+    if max_tokens < 1:
+        raise ValueError(f"max_tokens must be positive, got {max_tokens}")
+    ids = [p if isinstance(p, torch.Tensor) else torch.tensor(list(p), dtype=torch.int64) for p in prompts]
+    for p in ids:
+        if p.dim() != 1 or p.dtype.is_floating_point or p.dtype.is_complex or p.dtype == torch.bool:
+            raise ValueError(f"prompts must be integer sequences [n], got {p.dtype} {tuple(p.shape)}")
+        if p.numel() > model.cfg.max_position_embeddings:
+            raise ValueError(f"{p.numel()} positions needed, the model has {model.cfg.max_position_embeddings}")
+        if p.numel() and not p.is_cuda and not (0 <= int(p.min()) and int(p.max()) < model.cfg.vocab_size):
+            raise ValueError(f"token ids outside the vocabulary of {model.cfg.vocab_size}")
+    out: list[PromptScores] = []
+    at = 0
+    while at < len(ids):
+        end, tokens = at, 0
+        while end < len(ids) and (end == at or tokens + ids[end].numel() <= max_tokens):
+            tokens += ids[end].numel()
+            end += 1
+        out += _score_packed(model, [p.to(dev, torch.int64) for p in ids[at:end]], top)
+        at = end
+    return out
+
+
+def _score_packed(model: TPQwen2ForCausalLM, prompts: list[torch.Tensor], top: int) -> list[PromptScores]:
+    dev = model.model.embed_tokens.weight.device
+    lengths = [p.numel() for p in prompts]
+    n = sum(lengths)
+    starts = [0]
+    for k in lengths:
+        starts.append(starts[-1] + k)
+    scored = [max(0, k - 1) for k in lengths]
+    if n == 0 or sum(scored) == 0:
+        parts = [torch.empty(0, dtype=torch.float32, device=dev)] * 2
+        if top:
+            parts += [torch.empty(0, top, dtype=torch.float32, device=dev), torch.empty(0, top, dtype=torch.int64, device=dev)]
+    else:
+        packed = torch.cat(prompts)
+        hidden = model.forward_packed(packed, torch.tensor(starts, dtype=torch.int32).to(dev))
+        # every token but a prompt's last predicts the one behind it
+        rows = torch.cat([torch.arange(a, a + k) for a, k in zip(starts, scored)]).to(dev)
+        hidden, targets = hidden[rows], packed[rows + 1]
+        vloc = model.lm_head.vocab_end - model.lm_head.vocab_start
+        piece = max(1, _LOGITS_BYTES // (max(1, vloc) * hidden.element_size()))
+        got = []
+        for i in range(0, rows.numel(), piece):
+            logits = ops.linear(hidden[i:i + piece], model.lm_head.weight)
+            got.append(model.lm_head.token_logprobs(logits, targets[i:i + piece], top))
+        parts = [torch.cat(p) for p in zip(*(g[:4 if top else 2] for g in got))]
+    split = [p.split(scored) for p in parts]
+    if not top:
+        split += [[None] * len(prompts)] * 2
+    return [PromptScores(*row) for row in zip(*split)]
+
+
+__all__ = ["PromptScores", "score_prompts"]

@@ -64,3 +64,71 @@ def test_cpu_tensors_are_refused(lib):
         ops.logprobs_block(torch.zeros(2, 10), None, 2, 0, 10)
     with pytest.raises(_lib.MinitpB200Error, match="CUDA"):
         ops.logprobs_join(torch.zeros(2, 10, dtype=torch.uint8), None, (2,), 2, 10, torch.float32)
+
+
+def _cpu_block(local_logits, targets, top, vstart, v_plan):
+    """A stand-in for a shard's block: its sum of exponentials, its entropy's sum, the targets' logits and its best."""
+    n, v = local_logits.shape
+    x = torch.full((n, v_plan + top), -torch.inf, dtype=torch.float64)
+    x[:, :v] = local_logits.double()
+    e = x.exp()
+    mine = (targets >= vstart) & (targets < vstart + v)
+    xt = torch.where(mine, x.gather(1, (targets - vstart).clamp(0, v_plan - 1)[:, None])[:, 0], torch.nan)
+    val, at = x.sort(dim=-1, descending=True, stable=True)
+    cols = [e.sum(-1, keepdim=True), torch.where(e > 0, e * x, 0.0).sum(-1, keepdim=True), xt[:, None], val[:, :top],
+            (at[:, :top] + vstart).double()]
+    return torch.cat(cols, -1).reshape(-1).view(torch.uint8)
+
+
+def _cpu_join(blocks, targets, shape, top, v_plan, dtype):
+    rows = blocks.contiguous().view(torch.float64).view(blocks.shape[0], *shape, 3 + 2 * top)
+    total = rows[..., 0].sum(0)
+    xt = torch.nan_to_num(rows[..., 2], nan=0.0).sum(0)
+    best = []
+    for i in range(shape[0]):
+        cand = [(-float(rows[r, i, 3 + j]), int(rows[r, i, 3 + top + j])) for r in range(blocks.shape[0]) for j in range(top)
+                if float(rows[r, i, 3 + j]) > -torch.inf]
+        best.append([c[1] for c in sorted(cand)[:top]])
+    return (xt - total.log()).tolist(), (total.log() - rows[..., 1].sum(0) / total).tolist(), best
+
+
+def _w_logprobs(rank, world, v):
+    import torch.distributed as dist
+
+    from minitp_b200.distributed.context import ParallelContext
+    from minitp_b200.parallel import embedding
+
+    embedding.ops.logprobs_block, embedding.ops.logprobs_join = _cpu_block, _cpu_join
+    head = embedding.VocabParallelLMHead(8, v, ParallelContext(rank, rank, world, rank, world, torch.device("cpu"), dist.group.WORLD))
+    x, t = _logprob_case(v)
+    return head.token_logprobs(x[:, head.vocab_start:head.vocab_end], t, 4)
+
+
+def _logprob_case(v):
+    r = torch.Generator().manual_seed(v)
+    return torch.randn(5, v, generator=r), torch.randint(0, v, (5,), generator=r)
+
+
+@pytest.mark.distributed
+@pytest.mark.parametrize("world,v", [(2, 101), (3, 10), (3, 5)])
+def test_logprobs_exchange_the_shards_of_all_ranks(world, v):
+    """`VocabParallelLMHead.token_logprobs` over Gloo ranks (the kernels played by the stand-ins above): every rank
+    gets the whole vocabulary's values, of uneven shards too."""
+    from tests.tp_harness import run_tp
+
+    x, t = _logprob_case(v)
+    lp = torch.log_softmax(x.double(), -1)
+    res = run_tp(world, _w_logprobs, v)
+    for r in range(world):
+        got, ent, best = res[r]
+        assert got == pytest.approx(lp.gather(1, t[:, None])[:, 0].tolist(), abs=1e-9)
+        assert ent == pytest.approx((-(lp.exp() * lp).sum(-1)).tolist(), abs=1e-9)
+        assert best == lp.topk(min(4, v), dim=-1).indices.tolist()
+
+
+def test_packed_forward_refusals(lib):
+    ok = dict(model=P, ids=P, T=4, pos=P, starts=P, S=1, k=P, v=P, hidden=P, st=None)
+    # (a model's own sizes are looked at only after these)
+    for change, match in [(dict(model=None), "null"), (dict(ids=None), "null"), (dict(pos=None), "null"), (dict(starts=None), "null"),
+                          (dict(hidden=None), "null"), (dict(k=None), "null"), (dict(T=0), "empty"), (dict(S=-1), "empty")]:
+        _refused(lib, "mtpb_model_forward_packed", list((ok | change).values()), match)
