@@ -50,6 +50,11 @@ int lp_check(long long rows, long long V, int k) {
 
 template <typename T, bool TOP>
 int lp_rows(const LpRowsParams& p, cudaStream_t st) {
+  // a warp a row where every row is one tile and a CTA would have several of them
+  if (p.plan.tiles == 1 && p.plan.run > 1) {
+    const int grid = std::min((p.rows + kLpWarps - 1) / kLpWarps, 3 * host_sms());
+    return host_launch(lp_short_kernel<T, TOP>, dim3(unsigned(grid)), dim3(kLpThreads), 0, st, p);
+  }
   const auto kern = lp_rows_kernel<T, TOP>;
   // (with the static part it passes the 48 KB that a kernel gets unasked)
   const cudaError_t e = host_allow_smem(reinterpret_cast<const void*>(kern), kLpRing<TOP>);
@@ -203,16 +208,27 @@ int pa_launch_tc(PaParams p, cudaStream_t st) {
   return host_launch(pa_tc_kernel<HD, MT>, dim3(grid), dim3(kPaTcThreads), PaTcCfg<HD, MT>::kSmem, st, p, mq, mk, mv);
 }
 
+template <typename T, int HD, int RPT>
+int pa_launch_simt(PaParams p, cudaStream_t st) {
+  const long long items = pa_items(&p, 16 * RPT) + 1;
+  if (items > 0x7FFFFFFFll) return bad("prompt_attention: too many rows");
+  return host_launch(pa_simt_kernel<T, HD, RPT>, dim3(unsigned(items)), dim3(kPaThreads), pa_simt_smem<HD, RPT>(), st, p);
+}
+
 template <typename T, int HD>
 int pa_launch(PaParams p, cudaStream_t st) {
+  const long long rows = (long long)p.n * p.hq;
   if constexpr (sizeof(T) == 2 && HD >= 64) {
-    const long long rows = (long long)p.n * p.hq;
+    // Two row tiles an item as soon as there is one of those for every SM (us of one / two: one prompt of 512
+    // tokens, 14 heads of 64: 12 / 15; of 1024, 7 heads of 128: 17 / 25; of 2048, 28 heads of 128: 45 / 42; 64 of
+    // <= 509, 14 heads of 64: 59 / 44)
     return rows > 256ll * 148 ? pa_launch_tc<HD, 2>(p, st) : pa_launch_tc<HD, 1>(p, st);
   } else {
-    constexpr int RPT = 4;
-    const long long items = pa_items(&p, 16 * RPT) + 1;
-    if (items > 0x7FFFFFFFll) return bad("prompt_attention: too many rows");
-    return host_launch(pa_simt_kernel<T, HD, RPT>, dim3(unsigned(items)), dim3(kPaThreads), pa_simt_smem<HD, RPT>(), st, p);
+    // Rows a tile: 64; 16 while those leave SMs idle; 128 for prompts that are long on the mean (fp32 us of
+    // 16 / 64 / 128: 3 prompts of <= 300 tokens, 4 heads of 16: 11 / 17 / 25; 8 of <= 1024, 14 heads of 64: 452 /
+    // 167 / 172; 4 of <= 2048, 7 heads of 128: 888 / 412 / 508; one of 7000, 7 heads of 128: 6917 / 2910 / 2505)
+    if (rows <= 16ll * 148 * 4) return pa_launch_simt<T, HD, 1>(p, st);
+    return p.n / 4096 >= std::max(1, p.S) ? pa_launch_simt<T, HD, 8>(p, st) : pa_launch_simt<T, HD, 4>(p, st);
   }
 }
 

@@ -59,6 +59,203 @@ struct LpRowsParams {
 // Set when a bounded wait of a log-probability kernel ran out (its results are then void).
 __device__ uint32_t g_lp_status;
 
+// A lane's sums over its values so far, and its reference.
+struct LpLane {
+  float m = -INFINITY, c = 0.f, s = 0.f, w = 0.f;
+};
+
+// Takes a tile's values in: vector u of this lane holds columns col + u * 32 * VE
+// ... `first`: the warp's first tile (which sets a floor for its candidates).
+template <typename T, bool TOP>
+__device__ __forceinline__ void lp_step(LpLane& a0, BeamList& l, const uint4 (&v)[kLpVecs], int col, bool first, int k,
+                                        int64_t vstart, uint32_t* floor_key) {
+  constexpr int VE = VecTraits<T>::kElems, kLow = sizeof(T) == 2 ? 16 : 0;
+  const int lane = threadIdx.x & 31;
+  float m = a0.m, c = a0.c, s = a0.s, ws = a0.w;
+          float q[kLpVecs];  // max of each vector, at least -2^126
+          uint32_t y[kLpVecs][4];
+#pragma unroll
+          for (int u = 0; u < kLpVecs; ++u) {
+            const uint32_t raw[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %1, %2;" : "=r"(y[u][i]) : "r"(raw[i]), "r"(0xFE80FE80u));
+              uint32_t a, b;
+              asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(y[u][0]), "r"(y[u][1]));
+              asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(y[u][2]), "r"(y[u][3]));
+              asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+              q[u] = fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) y[u][i] = __float_as_uint(fmaxf(__uint_as_float(raw[i]), -0x1p126f));
+              q[u] = fmaxf(max3(__uint_as_float(y[u][0]), __uint_as_float(y[u][1]), __uint_as_float(y[u][2])),
+                           __uint_as_float(y[u][3]));
+            }
+          }
+          float top = fmaxf(max3(q[0], q[1], q[2]), q[3]);
+          // (read early: an older floor is a floor too)
+          const uint32_t common = TOP ? *static_cast<volatile uint32_t*>(floor_key) : 0u;
+          // ---- sums
+          if (!beam_far(fmaxf(m, top))) {
+            if (top - m > 8.f) {
+              if (beam_far(m)) {  // nothing yet, or values that count for nothing beside these
+                s = ws = 0.f;
+              } else {
+                const float d = beam_ref(m) - beam_ref(top), a = exp2_approx(d);
+                ws = fmaf(s, d, ws) * a;
+                s *= a;
+              }
+              m = top;
+              c = beam_ref(m);
+            }
+            float2 sum = make_float2(0.f, 0.f), mean = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < kLpVecs; ++u)
+#pragma unroll
+              for (int i = 0; i < 4; i += sizeof(T) == 2 ? 1 : 2) {
+                float2 x;
+                if constexpr (sizeof(T) == 2)
+                  x = make_float2(__uint_as_float(y[u][i] << 16), __uint_as_float(y[u][i] & 0xFFFF0000u));
+                else
+                  x = make_float2(__uint_as_float(y[u][i]), __uint_as_float(y[u][i + 1]));
+                const float2 d = fma2(x, make_float2(kBeamLog2e, kBeamLog2e), make_float2(-c, -c));
+                const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+                sum = add2(sum, e);
+                mean = fma2(e, d, mean);
+              }
+            s += sum.x + sum.y;
+            ws += mean.x + mean.y;
+          } else {
+            float raw_top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kLpVecs; ++u) {
+              float g[VE];
+              unpack(v[u], g);
+#pragma unroll
+              for (int e = 0; e < VE; ++e) raw_top = fmaxf(raw_top, g[e]);
+            }
+            if (raw_top > m) {
+              m = raw_top;
+              s = ws = 0.f;
+            }
+            if (m > -INFINITY)
+#pragma unroll
+              for (int u = 0; u < kLpVecs; ++u) {
+                float g[VE];
+                unpack(v[u], g);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) s += g[e] == m ? 1.f : 0.f;
+              }
+          }
+          // ---- candidates
+          if constexpr (TOP) {
+            if (first) {
+              // the k-th of the warp's 32 * kLpVecs vector maxima: k values lie at or above it
+              uint32_t kq[kLpVecs];
+#pragma unroll
+              for (int u = 0; u < kLpVecs; ++u) kq[u] = q[u] > -0x1p126f ? beam_logit_key(q[u]) : 0u;
+              const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(kq[0], kq[1]), max(kq[2], kq[3])));
+              // 32 lanes reach the least of their maxima; for more than 32 the least of all bounds the k-th
+              const uint32_t least = __reduce_min_sync(0xffffffffu, k <= 32 ? max(max(kq[0], kq[1]), max(kq[2], kq[3]))
+                                                                              : min(min(kq[0], kq[1]), min(kq[2], kq[3])));
+              const uint32_t cut = beam_search(k, least, most, kLow, [&](uint32_t x) {
+                uint32_t n = 0;
+#pragma unroll
+                for (int u = 0; u < kLpVecs; ++u) n += kq[u] >= x ? 1u : 0u;
+                return int(__reduce_add_sync(0xffffffffu, n));
+              });
+              if (lane == 0) atomicMax(floor_key, cut);
+              l.least = max(l.least, cut);
+            }
+            l.least = max(l.least, common);
+            const float ge = beam_key_val(l.least);
+            // (q is -2^126 where a vector holds nothing above it: its values are then looked at one by one)
+            if (__any_sync(0xffffffffu, top >= ge || !(ge > -0x1p126f))) {
+              uint32_t mine = 0;  // this lane's values that enter
+#pragma unroll
+              for (int u = 0; u < kLpVecs; ++u) {
+                if (!__any_sync(0xffffffffu, q[u] >= ge || !(ge > -0x1p126f))) continue;
+                float g[VE];
+                unpack(v[u], g);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) mine |= g[e] >= ge ? 1u << (u * VE + e) : 0u;
+              }
+              while (true) {  // one value of each lane at a time
+                const uint32_t b = __ballot_sync(0xffffffffu, mine != 0);
+                if (!b) break;
+                if (mine) {
+                  const int i = __ffs(mine) - 1, u = i / VE, e = i - u * VE;
+                  mine &= mine - 1;
+                  const uint4 x = u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : v[3];
+                  const int word = e * int(sizeof(T)) / 4;
+                  const uint32_t bits = word == 0 ? x.x : word == 1 ? x.y : word == 2 ? x.z : x.w;
+                  const float val = sizeof(T) == 4 ? __uint_as_float(bits) : __uint_as_float(e & 1 ? bits & 0xFFFF0000u : bits << 16);
+                  const uint32_t id = uint32_t(vstart + col + u * 32 * VE + e);
+                  l.buf[l.n + __popc(b & ((1u << lane) - 1u))] = beam_key(beam_logit_key(val), id);
+                }
+                l.n += __popc(b);
+                __syncwarp();
+                if (l.n > kBeamCap - 32) beam_cut<kLow>(l, k, floor_key);
+              }
+              // later columns have higher ids: they have to beat the k-th, not to equal it
+              if (l.kth) l.least = max(l.least, l.kth + 1);
+            }
+          }
+  a0 = LpLane{m, c, s, ws};
+}
+
+// Sums against mm as sums against the larger top (natural units).
+__device__ __forceinline__ void lp_raise(float mm, float top, float& ss, float& ww) {
+  if (mm == top) return;
+  const float d = mm - top, a = exp2_approx(d * kBeamLog2e);
+  ww = a > 0.f ? fmaf(d, ss, ww) * a : 0.f;
+  ss *= a;
+}
+
+// The warp's statistics from its lanes'.
+__device__ __forceinline__ LpStat lp_warp_stat(LpLane a) {
+  float cm = a.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
+  if (!beam_far(a.m)) {  // against m itself, in natural units
+    const float d = fmaf(a.m, kBeamLog2e, -a.c), f = exp2_approx(-d);
+    a.w = fmaf(-d, a.s, a.w) * f * 0.69314718055994530942f;
+    a.s *= f;
+  }
+  lp_raise(a.m, cm, a.s, a.w);
+  return LpStat{cm, warp_sum(a.s), warp_sum(a.w), 0.f};
+}
+
+// The vector of a row's first or last columns, those outside its whole vectors:
+// columns col .. col + n - 1, n < VE, one a lane.
+template <typename T>
+__device__ __forceinline__ void lp_edge(const T* x, int n, int col, uint4 (&v)[kLpVecs]) {
+  constexpr int VE = VecTraits<T>::kElems;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int u = 0; u < kLpVecs; ++u) {
+    float g[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) g[e] = u == 0 && e == 0 && lane < n ? to_f(x[col + lane]) : -INFINITY;
+    v[u] = pack_vec(g);
+  }
+}
+
+// Row r of the logits: its vectors begin `head` columns in, and `tail` columns stand behind the last whole one.
+template <typename T>
+struct LpRow {
+  const T* x;
+  int head, nvec, tail;
+  __device__ __forceinline__ LpRow(const LpRowsParams& p, int r) {
+    constexpr int VE = VecTraits<T>::kElems;
+    x = static_cast<const T*>(p.logits) + int64_t(r) * p.ld;
+    const int off = int((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+    head = min(p.V, off ? VE - off : 0);
+    nvec = (p.V - head) / VE;
+    tail = p.V - head - nvec * VE;
+  }
+};
+
 // One pass over the logits, bound by their bytes for many rows. A lane keeps
 // a reference m, s = sum 2^d and w = sum 2^d d with d = x L - c (c = m L
 // rounded, beam_ref), in fp32; the reference follows the lane's maximum when
@@ -98,33 +295,23 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
     *abort = 0;
   }
   __syncthreads();
-  // Row r: its vectors begin `head` columns in, and `tail` columns stand behind the last whole one.
-  struct Row {
-    const T* x;
-    int head, nvec, tail;
-  };
-  auto row_at = [&](int r) {
-    Row w;
-    w.x = static_cast<const T*>(p.logits) + int64_t(r) * p.ld;
-    const int off = int((reinterpret_cast<uintptr_t>(w.x) & 15u) / sizeof(T));
-    w.head = min(p.V, off ? VE - off : 0);
-    w.nvec = (p.V - w.head) / VE;
-    w.tail = p.V - w.head - w.nvec * VE;
-    return w;
-  };
+  auto row_at = [&](int r) { return LpRow<T>(p, r); };
   int row = int(t0 / p.plan.tiles), tile = int(t0 - (long long)row * p.plan.tiles);
   int sg = 0;
   uint32_t phase = 0;
-  // After the tiles 0 and 3 of a part the k-th of all warps' candidates becomes
-  // the floor: a later value enters with odds k / (values seen by the CTA), not
-  // k / (values of one warp's first tile). (After 0, 1, 3, 7 .. as well: 1 to 3 %
-  // slower; never: 512 rows with 20 alternatives 90 us and not 76.)
-  auto refloor = [](int i, int last) { return TOP && i < last && (i == 0 || i == 3); };
+  // After the tiles 0 and 3 of a part (of many candidates 0, 1, 3, 7 ..) the k-th
+  // of all warps' candidates becomes the floor: a later value enters with odds
+  // k / (values seen by the CTA), not k / (values of one warp's first tile).
+  // (2048 bf16 rows of 151936, never / 0, 3 / 0, 1, 3, 7 ..: 1 alternative 172 /
+  // 174 / 183 us, 64 alternatives 546 / 444 / 326; 512 rows, 20: 90 / 74 / 76.)
+  auto refloor = [&](int i, int last) {
+    return TOP && i < last && (p.k > 32 ? (i & (i + 1)) == 0 : i == 0 || i == 3);
+  };
   if (warp == kLpWarps) {  // ---- copies, a ring ahead of the tiles that the others are at, and floors
     int row2 = row, tile2 = tile, issued = 0, s2 = 0;  // of the next copy
     uint32_t ph2 = 0;
     long long t2 = t0;
-    Row w2 = row_at(row2);
+    LpRow<T> w2 = row_at(row2);
     bool ok = true;
     auto copy = [&]() {  // (skips tiles that the shard, of fewer columns than planned for, does not have)
       while (t2 < t1) {
@@ -191,7 +378,7 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
     for (long long t = t0; t < t1; ++row, tile = 0, odd ^= 1) {
       uint32_t* floor_key = floors + odd;
       // ---- this CTA's part of a row
-      const Row w = row_at(row);
+      const LpRow<T> w = row_at(row);
       const int end = int(min((long long)p.plan.tiles, tile + (t1 - t)));
       const int c0 = tile == 0 ? 0 : min(p.V, w.head + tile * kLpTile * VE);
       const int c1 = end == p.plan.tiles ? p.V : min(p.V, w.head + end * kLpTile * VE);
@@ -203,149 +390,14 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
       if (here) xt = to_f(w.x[goal]);
       if (threadIdx.x == 0 && p.targets && t < t1) next_goal = p.targets[row + 1];
       BeamList l{TOP ? buf[warp] : nullptr, 0, 0x00800000u, 0u};  // least: the key of the lowest finite value
-      float m = -INFINITY, c = 0.f, s = 0.f, ws = 0.f;
-      // a tile: vector u of this lane holds columns col + u * 32 * VE ..
+      LpLane sums;
       auto step = [&](const uint4 (&v)[kLpVecs], int col, bool first) {
-        float q[kLpVecs];  // max of each vector, at least -2^126
-        uint32_t y[kLpVecs][4];
-#pragma unroll
-        for (int u = 0; u < kLpVecs; ++u) {
-          const uint32_t raw[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-          if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %1, %2;" : "=r"(y[u][i]) : "r"(raw[i]), "r"(0xFE80FE80u));
-            uint32_t a, b;
-            asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(y[u][0]), "r"(y[u][1]));
-            asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(y[u][2]), "r"(y[u][3]));
-            asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
-            q[u] = fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[u][i] = __float_as_uint(fmaxf(__uint_as_float(raw[i]), -0x1p126f));
-            q[u] = fmaxf(max3(__uint_as_float(y[u][0]), __uint_as_float(y[u][1]), __uint_as_float(y[u][2])),
-                         __uint_as_float(y[u][3]));
-          }
-        }
-        float top = fmaxf(max3(q[0], q[1], q[2]), q[3]);
-        // (read early: an older floor is a floor too)
-        const uint32_t common = TOP ? *static_cast<volatile uint32_t*>(floor_key) : 0u;
-        // ---- sums
-        if (!beam_far(fmaxf(m, top))) {
-          if (top - m > 8.f) {
-            if (beam_far(m)) {  // nothing yet, or values that count for nothing beside these
-              s = ws = 0.f;
-            } else {
-              const float d = beam_ref(m) - beam_ref(top), a = exp2_approx(d);
-              ws = fmaf(s, d, ws) * a;
-              s *= a;
-            }
-            m = top;
-            c = beam_ref(m);
-          }
-          float2 sum = make_float2(0.f, 0.f), mean = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int u = 0; u < kLpVecs; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; i += sizeof(T) == 2 ? 1 : 2) {
-              float2 x;
-              if constexpr (sizeof(T) == 2)
-                x = make_float2(__uint_as_float(y[u][i] << 16), __uint_as_float(y[u][i] & 0xFFFF0000u));
-              else
-                x = make_float2(__uint_as_float(y[u][i]), __uint_as_float(y[u][i + 1]));
-              const float2 d = fma2(x, make_float2(kBeamLog2e, kBeamLog2e), make_float2(-c, -c));
-              const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
-              sum = add2(sum, e);
-              mean = fma2(e, d, mean);
-            }
-          s += sum.x + sum.y;
-          ws += mean.x + mean.y;
-        } else {
-          float raw_top = -INFINITY;
-#pragma unroll
-          for (int u = 0; u < kLpVecs; ++u) {
-            float g[VE];
-            unpack(v[u], g);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) raw_top = fmaxf(raw_top, g[e]);
-          }
-          if (raw_top > m) {
-            m = raw_top;
-            s = ws = 0.f;
-          }
-          if (m > -INFINITY)
-#pragma unroll
-            for (int u = 0; u < kLpVecs; ++u) {
-              float g[VE];
-              unpack(v[u], g);
-#pragma unroll
-              for (int e = 0; e < VE; ++e) s += g[e] == m ? 1.f : 0.f;
-            }
-        }
-        // ---- candidates
-        if constexpr (TOP) {
-          if (first) {
-            // the k-th of the warp's 32 * kLpVecs vector maxima: k values lie at or above it
-            uint32_t kq[kLpVecs];
-#pragma unroll
-            for (int u = 0; u < kLpVecs; ++u) kq[u] = q[u] > -0x1p126f ? beam_logit_key(q[u]) : 0u;
-            const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(kq[0], kq[1]), max(kq[2], kq[3])));
-            // 32 lanes reach the least of their maxima; for more than 32 the least of all bounds the k-th
-            const uint32_t least = __reduce_min_sync(0xffffffffu, p.k <= 32 ? max(max(kq[0], kq[1]), max(kq[2], kq[3]))
-                                                                            : min(min(kq[0], kq[1]), min(kq[2], kq[3])));
-            const uint32_t cut = beam_search(p.k, least, most, kLow, [&](uint32_t x) {
-              uint32_t n = 0;
-#pragma unroll
-              for (int u = 0; u < kLpVecs; ++u) n += kq[u] >= x ? 1u : 0u;
-              return int(__reduce_add_sync(0xffffffffu, n));
-            });
-            if (lane == 0) atomicMax(floor_key, cut);
-            l.least = max(l.least, cut);
-          }
-          l.least = max(l.least, common);
-          const float ge = beam_key_val(l.least);
-          // (q is -2^126 where a vector holds nothing above it: its values are then looked at one by one)
-          if (__any_sync(0xffffffffu, top >= ge || !(ge > -0x1p126f))) {
-            uint32_t mine = 0;  // this lane's values that enter
-#pragma unroll
-            for (int u = 0; u < kLpVecs; ++u) {
-              if (!__any_sync(0xffffffffu, q[u] >= ge || !(ge > -0x1p126f))) continue;
-              float g[VE];
-              unpack(v[u], g);
-#pragma unroll
-              for (int e = 0; e < VE; ++e) mine |= g[e] >= ge ? 1u << (u * VE + e) : 0u;
-            }
-            while (true) {  // one value of each lane at a time
-              const uint32_t b = __ballot_sync(0xffffffffu, mine != 0);
-              if (!b) break;
-              if (mine) {
-                const int i = __ffs(mine) - 1, u = i / VE, e = i - u * VE;
-                mine &= mine - 1;
-                const uint4 x = u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : v[3];
-                const int word = e * int(sizeof(T)) / 4;
-                const uint32_t bits = word == 0 ? x.x : word == 1 ? x.y : word == 2 ? x.z : x.w;
-                const float val = sizeof(T) == 4 ? __uint_as_float(bits) : __uint_as_float(e & 1 ? bits & 0xFFFF0000u : bits << 16);
-                const uint32_t id = uint32_t(p.vstart + col + u * 32 * VE + e);
-                l.buf[l.n + __popc(b & ((1u << lane) - 1u))] = beam_key(beam_logit_key(val), id);
-              }
-              l.n += __popc(b);
-              __syncwarp();
-              if (l.n > kBeamCap - 32) beam_cut<kLow>(l, p.k, floor_key);
-            }
-            // later columns have higher ids: they have to beat the k-th, not to equal it
-            if (l.kth) l.least = max(l.least, l.kth + 1);
-          }
-        }
+        lp_step<T, TOP>(sums, l, v, col, first, p.k, p.vstart, floor_key);
       };
       constexpr uint32_t kNone = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;  // -inf
-      auto edge = [&](int n, int col) {  // columns col .. col + n - 1, n < VE
+      auto edge = [&](int n, int col) {
         uint4 v[kLpVecs];
-#pragma unroll
-        for (int u = 0; u < kLpVecs; ++u) {
-          float g[VE];
-#pragma unroll
-          for (int e = 0; e < VE; ++e) g[e] = u == 0 && e == 0 && lane < n ? to_f(w.x[col + lane]) : -INFINITY;
-          v[u] = pack_vec(g);
-        }
+        lp_edge(w.x, n, col, v);
         step(v, col + lane, false);
       };
       if (warp == 0 && tile == 0 && w.head) edge(w.head, 0);
@@ -384,25 +436,8 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
       }
       if (warp == kLpWarps - 1 && end == p.plan.tiles && w.tail) edge(w.tail, p.V - w.tail);
       // ---- the part's statistics
-      float cm = m;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
-      if (!beam_far(m)) {  // against m itself, in natural units
-        const float d = fmaf(m, kBeamLog2e, -c), a = exp2_approx(-d);
-        ws = fmaf(-d, s, ws) * a * 0.69314718055994530942f;
-        s *= a;
-      }
-      // sums against m as sums against the larger top
-      auto raise = [](float mm, float top, float& ss, float& ww) {
-        if (mm == top) return;
-        const float d = mm - top, a = exp2_approx(d * kBeamLog2e);
-        ww = a > 0.f ? fmaf(d, ss, ww) * a : 0.f;
-        ss *= a;
-      };
-      raise(m, cm, s, ws);
-      s = warp_sum(s);
-      ws = warp_sum(ws);
-      if (lane == 0) stat[warp] = LpStat{cm, s, ws, 0.f};
+      const LpStat mine = lp_warp_stat(sums);
+      if (lane == 0) stat[warp] = mine;
       const size_t at = size_t(row) * p.plan.parts + size_t(blockIdx.x - p.plan.first(row));
       if constexpr (TOP) {
         // ---- its k best: the warps' candidates (at most 64 each) from the common floor on, ranked
@@ -431,7 +466,7 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
         float top = r.m;
 #pragma unroll
         for (int o = kLpWarps / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        raise(r.m, top, r.s, r.w);
+        lp_raise(r.m, top, r.s, r.w);
 #pragma unroll
         for (int o = kLpWarps / 2; o > 0; o >>= 1) {
           r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
@@ -450,6 +485,65 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
   }
   __syncthreads();
   if (threadIdx.x == 0 && *abort) atomicOr(&g_lp_status, kStatusTimeout);
+}
+
+// Many rows of one tile or less: a warp a row, straight from global memory,
+// without the barriers and the ring's start that a part of a CTA's run costs
+// (8192 bf16 rows of 1000 columns with 5 alternatives: 25 us instead of 94).
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kLpThreads, 3) lp_short_kernel(const LpRowsParams p) {
+  constexpr int VE = VecTraits<T>::kElems, kLow = sizeof(T) == 2 ? 16 : 0;
+  __shared__ uint64_t buf[TOP ? kLpWarps : 1][TOP ? kBeamCap : 1];
+  __shared__ uint32_t floors[kLpWarps];
+  pdl_launch();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int row = blockIdx.x * kLpWarps + warp; row < p.rows; row += gridDim.x * kLpWarps) {
+    const LpRow<T> w(p, row);
+    float xt = __int_as_float(0x7fffffff);
+    if (lane == 0 && p.targets) {
+      const long long c = p.targets[row] - p.vstart;
+      if (c >= 0 && c < p.V) xt = to_f(w.x[c]);
+      if (c >= 0 && c < p.V && xt != xt) xt = -INFINITY;
+    }
+    if (lane == 0) floors[warp] = 0;
+    __syncwarp();
+    BeamList l{TOP ? buf[warp] : nullptr, 0, 0x00800000u, 0u};
+    LpLane sums;
+    uint4 v[kLpVecs];
+    const uint4* x = reinterpret_cast<const uint4*>(w.x + w.head);
+    constexpr uint32_t kNone = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;  // -inf
+    if (w.head) {
+      lp_edge(w.x, w.head, 0, v);
+      lp_step<T, TOP>(sums, l, v, lane, false, p.k, p.vstart, floors + warp);
+    }
+    for (int i = lane; i - lane < w.nvec; i += 32 * kLpVecs) {
+#pragma unroll
+      for (int u = 0; u < kLpVecs; ++u)
+        v[u] = i + 32 * u < w.nvec ? ld_stream(x + i + 32 * u) : make_uint4(kNone, kNone, kNone, kNone);
+      lp_step<T, TOP>(sums, l, v, w.head + i * VE, i == lane, p.k, p.vstart, floors + warp);
+    }
+    if (w.tail) {
+      lp_edge(w.x, w.tail, p.V - w.tail, v);
+      lp_step<T, TOP>(sums, l, v, p.V - w.tail + lane, false, p.k, p.vstart, floors + warp);
+    }
+    LpStat r = lp_warp_stat(sums);
+    r.xt = xt;
+    if (lane == 0) p.stat[row] = r;
+    if constexpr (TOP) {
+      if (l.n > kLpMaxK) beam_cut<kLow>(l, p.k, floors + warp);
+      __syncwarp();
+      uint64_t* out = p.cand + size_t(row) * p.k;
+      for (int i = lane; i < l.n; i += 32) {
+        const uint64_t o = l.buf[i];
+        int place = 0;
+        for (int j = 0; j < l.n; ++j) place += l.buf[j] > o ? 1 : 0;
+        if (place < p.k) out[place] = o;
+      }
+      for (int i = l.n + lane; i < p.k; i += 32) out[i] = 0;
+      __syncwarp();
+    }
+  }
 }
 
 struct LpJoinParams {
@@ -518,50 +612,67 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
   if (!p.k) return;
   const int n = lists * p.kc;
   uint64_t* mine = lp_cands + warp * kLpRanked;
-  if (n <= kLpRanked) {
-    auto load = [&](int i) -> uint64_t {
-      return i < n ? __ldcg(reinterpret_cast<const unsigned long long*>(cand(i / p.kc)) + i % p.kc) : 0;
-    };
-    int m2 = n;  // candidates left in `mine`
-    if (n <= 64) {
-      for (int i = lane; i < n; i += 32) mine[i] = load(i);
-    } else {  // those below the k-th go first
-      constexpr int H = kLpRanked / 32;
-      uint64_t held[H];
+  auto load = [&](int i) -> uint64_t {
+    return i < n ? __ldcg(reinterpret_cast<const unsigned long long*>(cand(i / p.kc)) + i % p.kc) : 0;
+  };
+  int left = n;  // candidates in `mine`; more than kLpRanked: they did not fit
+  if (n <= 64) {
+    for (int i = lane; i < n; i += 32) mine[i] = load(i);
+  } else if (n <= kLpRanked) {  // those below the k-th go first
+    constexpr int H = kLpRanked / 32;
+    uint64_t held[H];
 #pragma unroll
-      for (int h = 0; h < H; ++h) held[h] = load(lane + 32 * h);
-      uint32_t most = 0, least = 0xFFFFFFFFu;
+    for (int h = 0; h < H; ++h) held[h] = load(lane + 32 * h);
+    uint32_t most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const uint32_t v = uint32_t(held[h] >> 32);
-        most = max(most, v);
-        least = min(least, v);
-      }
-      most = __reduce_max_sync(0xffffffffu, most);
-      least = __reduce_min_sync(0xffffffffu, least);
-      const uint32_t cut = beam_search(p.k, least, most, 0, [&](uint32_t v) {
-        uint32_t c = 0;
+    for (int h = 0; h < H; ++h) {
+      const uint32_t v = uint32_t(held[h] >> 32);
+      most = max(most, v);
+      least = min(least, v);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    const uint32_t cut = beam_search(p.k, least, most, 0, [&](uint32_t v) {
+      uint32_t c = 0;
 #pragma unroll
-        for (int h = 0; h < H; ++h) c += uint32_t(held[h] >> 32) >= v ? 1u : 0u;
-        return int(__reduce_add_sync(0xffffffffu, c));
-      });
-      m2 = 0;
+      for (int h = 0; h < H; ++h) c += uint32_t(held[h] >> 32) >= v ? 1u : 0u;
+      return int(__reduce_add_sync(0xffffffffu, c));
+    });
+    left = 0;
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const bool in = held[h] && uint32_t(held[h] >> 32) >= cut;
+    for (int h = 0; h < H; ++h) {
+      const bool in = held[h] && uint32_t(held[h] >> 32) >= cut;
+      const uint32_t b = __ballot_sync(0xffffffffu, in);
+      if (in) mine[left + __popc(b & ((1u << lane) - 1u))] = held[h];
+      left += __popc(b);
+    }
+  } else {  // many lists (few rows, or many shards): each has its c best, c * lists >= k, at or above the least of those
+    const int c = (p.k + lists - 1) / lists;
+    uint32_t least = 0xFFFFFFFFu;
+    for (int i = lane; i < lists; i += 32) least = min(least, uint32_t(load(i * p.kc + min(c, p.kc) - 1) >> 32));
+    least = __reduce_min_sync(0xffffffffu, least);
+    left = 0;
+    for (int i0 = 0; i0 < lists && left <= kLpRanked; i0 += 32) {
+      for (int j = 0; j < p.kc && left <= kLpRanked; ++j) {
+        const uint64_t o = i0 + lane < lists ? load((i0 + lane) * p.kc + j) : 0;
+        const bool in = o && uint32_t(o >> 32) >= least;
         const uint32_t b = __ballot_sync(0xffffffffu, in);
-        if (in) mine[m2 + __popc(b & ((1u << lane) - 1u))] = held[h];
-        m2 += __popc(b);
+        if (!b) break;
+        const int at = left + __popc(b & ((1u << lane) - 1u));
+        if (in && at < kLpRanked) mine[at] = o;
+        left += __popc(b);
       }
     }
+  }
+  if (left <= kLpRanked) {
     __syncwarp();
     int live = 0;
-    for (int i = lane; i < m2; i += 32) {
+    for (int i = lane; i < left; i += 32) {
       const uint64_t o = mine[i];
       if (!o) continue;
       ++live;
       int place = 0;  // how many are better
-      for (int j = 0; j < m2; ++j) place += mine[j] > o ? 1 : 0;
+      for (int j = 0; j < left; ++j) place += mine[j] > o ? 1 : 0;
       if (place < p.k) {
         p.top_logprobs[row * p.k + place] = logp(beam_key_val(uint32_t(o >> 32)));
         p.top_ids[row * p.k + place] = (long long)(0xFFFFFFFFu - uint32_t(o));
@@ -574,7 +685,7 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
     }
     return;
   }
-  // many lists (few rows, or many shards): they are sorted, the best of their heads is the next
+  // the lists are sorted: the best of their heads is the next
   uint8_t* head = reinterpret_cast<uint8_t*>(lp_cands + kLpJoinWarps * kLpRanked) + warp * (p.shards * p.plan.parts);
   for (int i = lane; i < lists; i += 32) head[i] = 0;
   for (int j = 0; j < p.k; ++j) {

@@ -202,21 +202,25 @@ __device__ __forceinline__ void pa_zero(const PaParams& p, const PaTiles& t, int
 // served have 64 and 128; those are on the tensor cores). 256 threads as 16 x
 // 16; RPT rows and 4 keys a thread of a tile of 16 RPT rows and 64 keys, in
 // fp32; a row's 16 threads are half a warp, so its probabilities go through
-// shared memory without a barrier of the CTA.
+// shared memory without a barrier of the CTA. The next tile's K and V are on
+// their way into registers under the arithmetic of this one. Bound by shared
+// memory reads beside the fused multiply-adds (a float4 of K serves RPT rows, one
+// of V as well).
 // ---------------------------------------------------------------------------
 constexpr int kPaKeys = 64;
 constexpr int kPaThreads = 256;
 
 template <int HD, int RPT>
 constexpr size_t pa_simt_smem() {
-  return sizeof(float) * (size_t(16 * RPT) * (HD + 4) + size_t(kPaKeys) * (HD + 4) + size_t(kPaKeys) * (HD + 4) +
-                          size_t(16 * RPT) * (kPaKeys + 4));
+  return sizeof(float) * (size_t(16 * RPT) * (HD + 4) + 2 * size_t(kPaKeys) * (HD + 4) + size_t(16 * RPT) * (kPaKeys + 4));
 }
 
 template <typename T, int HD, int RPT>
 __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
   constexpr int ROWS = 16 * RPT, LD = HD + 4, LP = kPaKeys + 4, VE = VecTraits<T>::kElems;
-  constexpr int DP = HD / 16;  // dims a thread of the result: tx, tx + 16, ..
+  constexpr int DP = HD / 16;  // dims a thread of the result, in runs of DV: tx * DV + 16 * DV * g ..
+  constexpr int DV = DP < 4 ? DP : 4, DG = DP / DV;
+  constexpr int NV = (kPaKeys * HD / VE + kPaThreads - 1) / kPaThreads;  // vectors of K (and of V) a thread loads
   extern __shared__ __align__(16) float pa_sm[];
   float* sq = pa_sm;
   float* sk = sq + ROWS * LD;
@@ -239,9 +243,23 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
   if (it.ntok == 0) return;
   const int rows = it.ntok * p.gs, kvh = it.plane / p.subs, head0 = it.plane * p.gs;
   const T* q = static_cast<const T*>(p.q);
-  const T* k = static_cast<const T*>(p.k) + kvh * p.k_hs;
-  const T* v = static_cast<const T*>(p.v) + kvh * p.v_hs;
+  const T* k = static_cast<const T*>(p.k) + kvh * p.k_hs + it.start * p.k_ts;
+  const T* v = static_cast<const T*>(p.v) + kvh * p.v_hs + it.start * p.v_ts;
   auto token = [&](int r) { return it.tok0 + pa_div_gs(p, r); };
+  const int keys = it.tok0 + it.ntok - it.start, low = it.tok0 + 1 - it.start;
+  uint4 hk[NV], hv[NV];  // the next tile
+  auto fetch = [&](int j) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int i = tid + n * kPaThreads, r = i / (HD / VE), c = (i - r * (HD / VE)) * VE;
+      hk[n] = hv[n] = make_uint4(0, 0, 0, 0);
+      if (r < kPaKeys && j + r < keys) {
+        hk[n] = ld_vec(k + (long long)(j + r) * p.k_ts + c);
+        hv[n] = ld_vec(v + (long long)(j + r) * p.v_ts + c);
+      }
+    }
+  };
+  fetch(0);
   for (int i = tid; i < ROWS * (HD / VE); i += kPaThreads) {
     const int r = i / (HD / VE), c = (i - r * (HD / VE)) * VE;
     float f[VE];
@@ -254,7 +272,6 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
   int lim[RPT];  // keys [0, lim) of the prompt are seen
 #pragma unroll
   for (int a = 0; a < RPT; ++a) lim[a] = token(min(ty * RPT + a, rows - 1)) + 1 - it.start;
-  const int keys = token(rows - 1) + 1 - it.start, low = token(0) + 1 - it.start;
   float o[RPT][DP], m[RPT], l[RPT];
 #pragma unroll
   for (int a = 0; a < RPT; ++a) {
@@ -266,22 +283,21 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
   const float sl2 = p.scale * kLog2e;
   for (int j = 0; j < keys; j += kPaKeys) {
     __syncthreads();
-    for (int i = tid; i < kPaKeys * (HD / VE); i += kPaThreads) {
-      const int r = i / (HD / VE), c = (i - r * (HD / VE)) * VE;
-      float f[VE], g[VE];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = g[e] = 0.f;
-      if (j + r < keys) {
-        unpack(ld_vec(k + (long long)(it.start + j + r) * p.k_ts + c), f);
-        unpack(ld_vec(v + (long long)(it.start + j + r) * p.v_ts + c), g);
-      }
+    for (int n = 0; n < NV; ++n) {
+      const int i = tid + n * kPaThreads, r = i / (HD / VE), c = (i - r * (HD / VE)) * VE;
+      if (r < kPaKeys) {
+        float f[VE];
+        unpack(hk[n], f);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        sk[r * LD + c + e] = f[e];
-        sv[r * LD + c + e] = g[e];
+        for (int e = 0; e < VE; e += 4) *reinterpret_cast<float4*>(sk + r * LD + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        unpack(hv[n], f);
+#pragma unroll
+        for (int e = 0; e < VE; e += 4) *reinterpret_cast<float4*>(sv + r * LD + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
       }
     }
     __syncthreads();
+    if (j + kPaKeys < keys) fetch(j + kPaKeys);
     float s[RPT][4];
 #pragma unroll
     for (int a = 0; a < RPT; ++a)
@@ -313,23 +329,36 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 #pragma unroll
       for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
       top = fmaxf(m[a], top);
-      const float ref = top == -INFINITY ? 0.f : top, w = exp2f(m[a] - ref);
+      const float ref = top == -INFINITY ? 0.f : top, w = exp2_approx(m[a] - ref);
       m[a] = top;
       float sum = 0.f;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const float e = exp2f(s[a][b] - ref);
+        const float e = exp2_approx(s[a][b] - ref);
         sum += e;
         sp[(ty * RPT + a) * LP + tx + 16 * b] = e;
       }
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      l[a] = fmaf(l[a], w, sum);
+      l[a] = fmaf(l[a], w, sum);  // (of this thread's keys)
 #pragma unroll
       for (int d = 0; d < DP; ++d) o[a][d] *= w;
     }
     __syncwarp();
     const int nk = min(kPaKeys, keys - j);
+    auto v_at = [&](int key, float (&x)[DP]) {
+#pragma unroll
+      for (int g = 0; g < DG; ++g) {
+        const float* at = sv + key * LD + tx * DV + g * 16 * DV;
+        if constexpr (DV == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(at);
+          x[4 * g] = y.x, x[4 * g + 1] = y.y, x[4 * g + 2] = y.z, x[4 * g + 3] = y.w;
+        } else if constexpr (DV == 2) {
+          const float2 y = *reinterpret_cast<const float2*>(at);
+          x[2 * g] = y.x, x[2 * g + 1] = y.y;
+        } else {
+          x[g] = *at;
+        }
+      }
+    };
     if (!masked) {
 #pragma unroll 2
       for (int key = 0; key < kPaKeys; key += 4) {
@@ -337,35 +366,43 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 #pragma unroll
         for (int a = 0; a < RPT; ++a) pp[a] = *reinterpret_cast<const float4*>(sp + (ty * RPT + a) * LP + key);
 #pragma unroll
-        for (int d = 0; d < DP; ++d) {
-          const float v0 = sv[key * LD + tx + 16 * d], v1 = sv[(key + 1) * LD + tx + 16 * d];
-          const float v2 = sv[(key + 2) * LD + tx + 16 * d], v3 = sv[(key + 3) * LD + tx + 16 * d];
+        for (int i = 0; i < 4; ++i) {
+          float x[DP];
+          v_at(key + i, x);
 #pragma unroll
-          for (int a = 0; a < RPT; ++a)
-            o[a][d] = fmaf(pp[a].w, v3, fmaf(pp[a].z, v2, fmaf(pp[a].y, v1, fmaf(pp[a].x, v0, o[a][d]))));
+          for (int a = 0; a < RPT; ++a) {
+            const float pr = i == 0 ? pp[a].x : i == 1 ? pp[a].y : i == 2 ? pp[a].z : pp[a].w;
+#pragma unroll
+            for (int d = 0; d < DP; ++d) o[a][d] = fmaf(pr, x[d], o[a][d]);
+          }
         }
       }
     } else {  // a key that a row does not see adds nothing to it, whatever its V
-      for (int key = 0; key < nk; ++key)
+#pragma unroll 2
+      for (int key = 0; key < nk; ++key) {
+        float x[DP];
+        v_at(key, x);
 #pragma unroll
-        for (int a = 0; a < RPT; ++a) {
-          const float pr = sp[(ty * RPT + a) * LP + key];
+        for (int a = 0; a < RPT; ++a)
+          if (j + key < lim[a]) {
+            const float pr = sp[(ty * RPT + a) * LP + key];
 #pragma unroll
-          for (int d = 0; d < DP; ++d) {
-            const float x = fmaf(pr, sv[key * LD + tx + 16 * d], o[a][d]);
-            o[a][d] = j + key < lim[a] ? x : o[a][d];
+            for (int d = 0; d < DP; ++d) o[a][d] = fmaf(pr, x[d], o[a][d]);
           }
-        }
+      }
     }
     __syncwarp();
   }
 #pragma unroll
   for (int a = 0; a < RPT; ++a) {
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) l[a] += __shfl_xor_sync(0xffffffffu, l[a], x);
     const int r = ty * RPT + a;
     if (r < rows) {
       T* out = static_cast<T*>(p.out) + (size_t(token(r) - p.first) * p.hq + head0 + r - pa_div_gs(p, r) * p.gs) * HD;
 #pragma unroll
-      for (int d = 0; d < DP; ++d) out[tx + 16 * d] = from_f<T>(l[a] == 0.f ? 0.f : o[a][d] / l[a]);
+      for (int d = 0; d < DP; ++d)
+        out[tx * DV + (d / DV) * 16 * DV + d % DV] = from_f<T>(l[a] == 0.f ? 0.f : o[a][d] / l[a]);
     }
   }
 }

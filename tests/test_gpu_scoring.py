@@ -413,6 +413,44 @@ def test_token_logprobs_of_shards(lib):
                 scoring_ref.check_logprobs(got, x, t, top)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_token_logprobs_joined_from_many_lists(lib, dtype):
+    """Few long rows with many alternatives, and shards of every kind: more candidates than are ranked at once, among
+    them runs of equal values and rows with fewer tokens than alternatives."""
+    from minitp_b200 import ops
+
+    r = _gen(77)
+    v, top = 200003, 64
+    x = (torch.randn(6, v, generator=r) * 3).to(DT[dtype])
+    x[1] = torch.randint(-3, 3, (v,), generator=r).to(DT[dtype])
+    x[2] = 0.0
+    x[3] = -math.inf
+    x[3, torch.randint(0, v, (40,), generator=r)] = 1.0
+    x[4, 100000:] = -math.inf
+    x[5, :4000] = 7.5
+    t = torch.randint(0, v, (6,), generator=r)
+    scoring_ref.check_logprobs(ops.token_logprobs(x.cuda(), t.cuda(), top), x, t, top)
+    cuts = list(range(0, v, 6251)) + [v]
+    blocks = [ops.logprobs_block(x[:, a:b].cuda(), t.cuda(), top, a, 6251) for a, b in zip(cuts, cuts[1:])]
+    scoring_ref.check_logprobs(ops.logprobs_join(torch.stack(blocks), t.cuda(), (6,), top, 6251, DT[dtype]), x, t, top)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("v", [1, 9, 500, 4096, 8192])
+def test_token_logprobs_many_short_rows(lib, dtype, v):
+    """More rows than CTAs, of one tile each; every start in memory."""
+    from minitp_b200 import ops
+
+    r = _gen(v)
+    wide = (torch.randn(3001, v + 3, generator=r) * 3).to(DT[dtype])
+    wide[::5, ::3] = -math.inf
+    for off in (0, 1, 3):
+        x = wide[:, off:off + v]
+        t = torch.randint(0, v, (3001,), generator=r)
+        for top in (0, 3, 64):
+            scoring_ref.check_logprobs(ops.token_logprobs(wide.cuda()[:, off:off + v], t.cuda(), top), x, t, top)
+
+
 def test_token_logprobs_captured_and_on_another_stream(lib):
     from minitp_b200 import ops
 
