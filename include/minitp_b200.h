@@ -323,7 +323,7 @@ int mtpb_beam_status(uint32_t* status_out /* host */);
  * [n, hq, hd]. Strides are in elements, at least hd and multiples of 16 bytes
  * (that of an axis of one place too); q, k and v are 16-byte aligned, out 32-byte. A
  * token of no prompt, and one whose scores are all -inf, gets 0. scale =
- * 1/sqrt(hd); hd 16, 32, 64 or 128; total * hq at most 2^30, S at most 2^20.
+ * 1/sqrt(hd); hd 16, 32, 64 or 128; total * hq at most 2^28, hq 2^16, S 2^20.
  * Softmax statistics and sums are fp32; bf16 probabilities are rounded to bf16
  * for their product with V. What a token does not see does not reach it, NaN
  * and infinities included. out may not overlap an input. */

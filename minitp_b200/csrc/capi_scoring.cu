@@ -191,7 +191,7 @@ long long pa_items(PaParams* p, int rows) {
   p->gs = G / p->subs;
   p->planes = p->hkv * p->subs;
   p->tt = rows / p->gs;
-  p->tt_mul = ((1ull << 40) + p->tt - 1) / p->tt;
+  p->tt_mul = ((1ull << 37) + p->tt - 1) / p->tt;
   p->gs_mul = (65536u + p->gs - 1) / p->gs;
   return ((long long)p->n / p->tt + p->S) * p->planes;
 }
@@ -254,7 +254,8 @@ int prompt_attn_run(const PromptAttnArgs& a, cudaStream_t st) {
   if (!dtype_ok(a.dtype)) return bad("unsupported dtype");
   if (a.first < 0 || (long long)a.first + a.n > a.total)
     return bad("prompt_attention: the queries' tokens lie outside the packed tokens");
-  if ((long long)a.total * a.hq > 1 << 30) return bad("prompt_attention: more than 2^30 (token, head) rows");
+  if ((long long)a.total * a.hq > 1 << 28) return bad("prompt_attention: more than 2^28 (token, head) rows");
+  if (a.hq > 1 << 16) return bad("prompt_attention: more than 2^16 heads");
   if (a.S > 1 << 20) return bad("prompt_attention: more than 2^20 prompts");
   if (a.n == 0) return MTPB_OK;
   if (!a.q || !a.k || !a.v || !a.out || !a.seq_starts) return bad("prompt_attention: null tensor");

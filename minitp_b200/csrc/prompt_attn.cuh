@@ -32,14 +32,14 @@ struct PaParams {
   int S, first, n, total, hq, hkv;
   int gs, subs;  // heads of a row group, groups of a KV head: gs * subs = G
   int tt;        // tokens a tile: as many as its rows hold, gs rows each
-  unsigned long long tt_mul;  // ceil(2^40 / tt): n / tt = n * tt_mul >> 40 for n < 2^30
+  unsigned long long tt_mul;  // ceil(2^37 / tt): n / tt = n * tt_mul >> 37, exact for the n there can be (n * hq <= 2^28)
   uint32_t gs_mul;            // ceil(2^16 / gs), the same for rows of a tile
   int planes;    // hkv * subs
   float scale;
   uint32_t* status;  // error bits
 };
 
-__device__ __forceinline__ int pa_div_tt(const PaParams& p, int n) { return int((unsigned long long)n * p.tt_mul >> 40); }
+__device__ __forceinline__ int pa_div_tt(const PaParams& p, int n) { return int((unsigned long long)n * p.tt_mul >> 37); }
 __device__ __forceinline__ int pa_div_gs(const PaParams& p, int row) { return int(uint32_t(row) * p.gs_mul >> 16); }
 
 // Set when a bounded wait of a prompt attention ran out (its results are then void).
@@ -68,7 +68,7 @@ struct PaTiles {
   int at_least;  // the largest start so far
   int gap0, gap1;  // tokens [first, gap0) and [gap1, first + n) are of no prompt (gap1: once all were read)
   int all;  // tiles: of all prompts, or (not ordered) of those before block b
-  int b, most;
+  int b, most, ahead;  // ahead: ends of block b + 1, loaded
   Seq q[kPaOrdered / 32];
 
   static __device__ __forceinline__ int cut(const PaParams& p, int t) { return min(max(t, 0), p.total); }
@@ -106,6 +106,7 @@ struct PaTiles {
     all = b = most = 0;
     if (p.S > kPaOrdered) {
       q[0] = load(p, ends[0]);
+      ahead = ends[1];
       return;
     }
 #pragma unroll
@@ -148,7 +149,8 @@ struct PaTiles {
         }
         if (32 * (b + 1) >= p.S) break;
         all += sum;
-        q[0] = load(p, end_of(p, b + 1));
+        q[0] = load(p, ahead);
+        ahead = end_of(p, b + 2);
       }
       gap1 = min(max(at_least, p.first), p.first + p.n);
       return it;

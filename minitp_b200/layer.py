@@ -247,7 +247,8 @@ class TPQwen2ForCausalLM(nn.Module):
             tok = torch.arange(n, dtype=torch.int32, device=dev)
             first = seq_starts[(torch.searchsorted(seq_starts, tok, right=True) - 1).clamp_(min=0)]
             # (tokens of no prompt are read nowhere; their places need only be in the table)
-            positions = (tok - first).clamp_(0, self.cfg.max_position_embeddings - 1)
+            none = (tok < seq_starts[0]) | (tok >= seq_starts[-1])
+            positions = (tok - first).masked_fill_(none, 0)
         elif positions.shape != (n,) or positions.device != dev:
             raise ValueError(f"positions must be [{n}] on {dev}, got {tuple(positions.shape)} on {positions.device}")
         attn0, w = self.model.layers[0].self_attn, self.model.embed_tokens.weight

@@ -406,12 +406,16 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 # ---------------------------------------------------------------------- #
 # scoring of prompts (no counterpart in the reference)
 # ---------------------------------------------------------------------- #
-def _packed_strides(name: str, t: torch.Tensor):
+def _packed_strides(t: torch.Tensor):
     """``t [tokens, heads, hd]`` with its token and head strides, copied only where the kernels cannot read it in place."""
     n, h, hd = t.shape
-    ts, hs = t.stride(0) if n > 1 else h * hd, t.stride(1) if h > 1 else hd
+    ts, hs, ds = t.stride()
+    if n <= 1:  # (an axis of one place may have any stride)
+        ts = h * hd
+    if h <= 1:
+        hs = hd
     ve = 16 // t.element_size()
-    if t.stride(2) != 1 or ts < hd or hs < hd or ts % ve or hs % ve or t.data_ptr() % 16:
+    if ds != 1 or ts < hd or hs < hd or ts % ve or hs % ve or t.data_ptr() % 16:
         t = t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 == 0 else t.clone()
         ts, hs = h * hd, hd
     return t, ts, hs
@@ -445,8 +449,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     if not 0 <= first <= total - n:
         raise _lib.MinitpB200Error(f"{name}: tokens {first} .. {first + n} of {total} packed ones")
     code = _lib.dtype_code(q.dtype)
-    out = torch.empty(n, hq, hd, dtype=q.dtype, device=dev)
-    (q, qt, qh), (k, kt, kh), (v, vt, vh) = (_packed_strides(name, t) for t in (q, k, v))
+    out = torch.empty_strided((n, hq, hd), (hq * hd, hd, 1), dtype=q.dtype, device=dev)
+    q, qt, qh = _packed_strides(q)
+    k, kt, kh = _packed_strides(k)
+    v, vt, vh = _packed_strides(v)
     _call_on(dev, "mtpb_prompt_attention", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
              out.data_ptr(), seq_starts.data_ptr(), seq_starts.numel() - 1, first, n, total, hq, hkv, hd, code)
     return out
@@ -477,13 +483,21 @@ def _logprob_rows(name: str, logits: torch.Tensor, targets: torch.Tensor | None,
     return dev, x, ld, targets
 
 
+def _packed_empty(shape, dtype, dev) -> torch.Tensor:
+    # (empty_strided takes half of empty's time, which counts in a call of 20 us)
+    strides, n = [], 1
+    for size in reversed(shape):
+        strides.append(n)
+        n *= max(size, 1)
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=dev)
+
+
 def _logprob_outputs(dev, shape, targets, top: int):
-    lp = None if targets is None else torch.empty(shape, dtype=torch.float32, device=dev)
-    ent = torch.empty(shape, dtype=torch.float32, device=dev)
+    lp = None if targets is None else _packed_empty(shape, torch.float32, dev)
+    ent = _packed_empty(shape, torch.float32, dev)
     if not top:
         return lp, ent, None, None
-    tops = torch.empty(*shape, top, dtype=torch.float32, device=dev)
-    return lp, ent, tops, torch.empty(*shape, top, dtype=torch.int64, device=dev)
+    return lp, ent, _packed_empty((*shape, top), torch.float32, dev), _packed_empty((*shape, top), torch.int64, dev)
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0):

@@ -71,6 +71,53 @@ def test_prompt_attention_many_prompts(lib, dtype, hq, hkv, hd):
         _close(ops.prompt_attention(q, k, v, _cuda_starts(starts)), *scoring_ref.attend(q, k, v, starts))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,hd", [(40, 1, 64), (130, 1, 64), (300, 1, 128), (131, 1, 64), (257, 1, 16)])
+def test_prompt_attention_many_heads_a_kv_head(lib, dtype, hq, hkv, hd):
+    """More query heads of a KV head than a tile has rows, prime numbers of them too."""
+    from minitp_b200 import ops
+
+    starts = _starts([19, 1, 40])
+    q, k, v = _parts(_gen(hq), starts[-1], hq, hkv, hd, dtype)
+    _close(ops.prompt_attention(q, k, v, _cuda_starts(starts)), *scoring_ref.attend(q, k, v, starts))
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,hd", [("fp32", 4, 2, 16), ("bf16", 14, 2, 64), ("bf16", 4, 4, 128)])
+def test_prompt_attention_thousands_of_prompts(lib, dtype, hq, hkv, hd):
+    from minitp_b200 import ops
+
+    lengths = torch.randint(0, 13, (5000,), generator=_gen(1)).tolist()
+    starts = _starts(lengths, at=3)
+    q, k, v = _parts(_gen(2), starts[-1] + 5, hq, hkv, hd, dtype)
+    got = ops.prompt_attention(q, k, v, _cuda_starts(starts))
+    want, tol = scoring_ref.attend(q, k, v, starts)
+    _close(got, want, tol)
+    part = ops.prompt_attention(q[1000:9001], k, v, _cuda_starts(starts), first=1000)
+    _close(part, want[1000:9001], tol[1000:9001])
+
+
+def test_two_calls_at_once(lib):
+    """Calls of every kind on two streams at the same time: each call's results are its own."""
+    from minitp_b200 import ops
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    q, k, v = _parts(_gen(50), 3000, 14, 2, 64, "bf16")
+    starts = [_cuda_starts([0, 1700, 3000]), _cuda_starts([0, 40, 2000, 3000])]
+    x = torch.randn(600, 30000, generator=_gen(51)).cuda()
+    t = torch.randint(0, 30000, (600,), generator=_gen(52)).cuda()
+    alone = [(ops.prompt_attention(q, k, v, s), *ops.token_logprobs(x[i * 50:], t[i * 50:], 7 - i)) for i, s in enumerate(starts)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for i, (st, s) in enumerate(zip(streams, starts)):
+            with torch.cuda.stream(st):
+                got.append((ops.prompt_attention(q, k, v, s), *ops.token_logprobs(x[i * 50:], t[i * 50:], 7 - i)))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            for y, z in zip(a, b):
+                assert torch.equal(y, z)
+
+
 @pytest.mark.parametrize("dtype,hq,hkv,hd", [("fp32", 4, 2, 16), ("bf16", 14, 2, 64), ("bf16", 8, 2, 128), ("bf16", 6, 3, 32)])
 def test_prompt_attention_pieces(lib, dtype, hq, hkv, hd):
     """Queries of a piece of the packed tokens give the whole call's rows, wherever the pieces are cut."""

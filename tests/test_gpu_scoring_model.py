@@ -119,6 +119,35 @@ def test_packed_forward_in_chunks(lib):
     assert model.ctx.comm().status() == 0
 
 
+@pytest.mark.parametrize("name,dtype", [("tiny", torch.float32), ("q05b", torch.bfloat16)])
+def test_packed_forward_of_one_token(lib, name, dtype):
+    """A single token, and a last chunk of one token."""
+    model, cfg = _model(name, dtype)
+    ids = _prompts(cfg, [1], 10)[0].cuda()
+    one = torch.tensor([0, 1], dtype=torch.int32).cuda()
+    want = model(ids[None])[0]
+    got = model.lm_head(model.forward_packed(ids, one))
+    off = 1e-4 * float(want.abs().max()) if dtype == torch.float32 else 0.5
+    assert float((got - want).abs().max()) <= off
+    n = model.ctx.comm().slot_bytes() // (cfg.hidden_size * ids.new_empty(0, dtype=dtype).element_size()) + 1
+    ids = _prompts(cfg, [n], 11)[0].cuda()
+    starts = torch.tensor([*range(0, n - 40, 1000), n - 40, n], dtype=torch.int32).cuda()
+    got = model.lm_head(model.forward_packed(ids, starts)[n - 40:])
+    want = model(ids[None, n - 40:])[0]
+    assert float((got - want).abs().max()) <= (1e-4 * float(want.abs().max()) if dtype == torch.float32 else 0.5)
+    assert model.ctx.comm().status() == 0
+
+
+def test_prompts_longer_than_the_position_table_are_flagged(lib):
+    model, cfg = _model("tiny")
+    ids = _prompts(cfg, [cfg.max_position_embeddings + 9], 12)[0].cuda()
+    model.forward_packed(ids, torch.tensor([0, 8, ids.numel() - 1], dtype=torch.int32).cuda())
+    assert model.ctx.comm().status() == 0
+    model.forward_packed(ids, torch.tensor([0, ids.numel()], dtype=torch.int32).cuda())
+    assert model.ctx.comm().status() == 2
+    model.ctx.comm().clear_status()
+
+
 def test_tokens_of_no_prompt_change_nothing(lib):
     model, cfg = _model("tiny")
     ids = _prompts(cfg, [100], 5)[0].cuda()

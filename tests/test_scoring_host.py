@@ -21,7 +21,8 @@ def test_attention_refusals(lib):
                           (dict(first=1), "outside"), (dict(first=-1), "outside"), (dict(n=11), "outside"),
                           (dict(n=-1), "size"), (dict(S=-1), "size"), (dict(S=1 << 21), "prompts"), (dict(q=P + 2), "aligned"),
                           (dict(qt=14 * 64 + 4), "strides"), (dict(kh=32), "strides"), (dict(vt=0), "strides"),
-                          (dict(vh=-64), "strides"), (dict(n=1, total=1 << 27), "rows")]:
+                          (dict(vh=-64), "strides"), (dict(n=1, total=1 << 25), "rows"),
+                          (dict(n=1, total=1, hq=1 << 17, hkv=1), "heads")]:
         _refused(lib, "mtpb_prompt_attention", list((ok | change).values()), match)
     assert lib.mtpb_prompt_attention(*(ok | dict(n=0)).values()) == 0  # nothing to do
 
