@@ -8,6 +8,7 @@ stream. None of them has a CPU path: CPU tensors raise.
 from __future__ import annotations
 
 import array
+import functools
 import operator
 
 import torch
@@ -483,21 +484,20 @@ def _logprob_rows(name: str, logits: torch.Tensor, targets: torch.Tensor | None,
     return dev, x, ld, targets
 
 
-def _packed_empty(shape, dtype, dev) -> torch.Tensor:
+def _logprob_outputs(dev, shape, targets, top: int):
     # (empty_strided takes half of empty's time, which counts in a call of 20 us)
     strides, n = [], 1
     for size in reversed(shape):
-        strides.append(n)
+        strides.insert(0, n)
         n *= max(size, 1)
-    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=dev)
-
-
-def _logprob_outputs(dev, shape, targets, top: int):
-    lp = None if targets is None else _packed_empty(shape, torch.float32, dev)
-    ent = _packed_empty(shape, torch.float32, dev)
+    new = torch.empty_strided
+    lp = None if targets is None else new(shape, strides, dtype=torch.float32, device=dev)
+    ent = new(shape, strides, dtype=torch.float32, device=dev)
     if not top:
         return lp, ent, None, None
-    return lp, ent, _packed_empty((*shape, top), torch.float32, dev), _packed_empty((*shape, top), torch.int64, dev)
+    shape, strides = (*shape, top), (*(s * top for s in strides), 1)
+    return (lp, ent, new(shape, strides, dtype=torch.float32, device=dev),
+            new(shape, strides, dtype=torch.int64, device=dev))
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0):
@@ -523,8 +523,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def logprobs_block_bytes(rows: int, v_plan: int, top: int, dtype: torch.dtype) -> int:
-    """Bytes of one shard's block (``logprobs_block``)."""
+    """Bytes of one shard's block (``logprobs_block``): a function of the sizes alone."""
     n = _lib.load().mtpb_logprobs_block_bytes(rows, v_plan, top, _lib.dtype_code(dtype))
     if n < 0:
         _lib.check(n)
