@@ -224,11 +224,10 @@ int pa_launch(PaParams p, cudaStream_t st) {
     // <= 509, 14 heads of 64: 59 / 44)
     return rows > 256ll * 148 ? pa_launch_tc<HD, 2>(p, st) : pa_launch_tc<HD, 1>(p, st);
   } else {
-    // Rows a tile: 64; 16 while those leave SMs idle; 128 for prompts that are long on the mean (fp32 us of
-    // 16 / 64 / 128: 3 prompts of <= 300 tokens, 4 heads of 16: 11 / 17 / 25; 8 of <= 1024, 14 heads of 64: 452 /
-    // 167 / 172; 4 of <= 2048, 7 heads of 128: 888 / 412 / 508; one of 7000, 7 heads of 128: 6917 / 2910 / 2505)
-    if (rows <= 16ll * 148 * 4) return pa_launch_simt<T, HD, 1>(p, st);
-    return p.n / 4096 >= std::max(1, p.S) ? pa_launch_simt<T, HD, 8>(p, st) : pa_launch_simt<T, HD, 4>(p, st);
+    // Rows a tile: 64; 16 while those leave SMs idle (fp32 us of 16 / 64: 3 prompts of <= 300 tokens, 4 heads of 16:
+    // 11 / 17; 8 of <= 1024, 14 heads of 64: 452 / 156). 128 rows spill registers at 128 dims (one prompt of 7000, 7
+    // heads of 128: 2384 with 64, 2559 with 128).
+    return rows <= 16ll * 148 * 4 ? pa_launch_simt<T, HD, 1>(p, st) : pa_launch_simt<T, HD, 4>(p, st);
   }
 }
 

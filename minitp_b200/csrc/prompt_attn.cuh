@@ -205,9 +205,13 @@ __device__ __forceinline__ void pa_zero(const PaParams& p, const PaTiles& t, int
 // 16; RPT rows and 4 keys a thread of a tile of 16 RPT rows and 64 keys, in
 // fp32; a row's 16 threads are half a warp, so its probabilities go through
 // shared memory without a barrier of the CTA. The next tile's K and V are on
-// their way into registers under the arithmetic of this one. Bound by shared
-// memory reads beside the fused multiply-adds (a float4 of K serves RPT rows, one
-// of V as well).
+// their way into registers under the arithmetic of this one. Two products an
+// instruction, over even and odd dims (fp32 us without / with, 64-row tiles: 4
+// prompts of <= 2048 tokens, 7 heads of 128: 410 / 332; 5 of <= 701, 8 heads of 32:
+// 45 / 43). Two CTAs an SM up to 64 dims, at 128 registers (one / two: 8 of <= 1024,
+// 14 heads of 64: 182 / 156; one of 1000: 78 / 103). Bound by shared memory reads
+// beside the fused multiply-adds (a float4 of K serves RPT rows, one of V as well):
+// 31 to 37 TFLOP/s.
 // ---------------------------------------------------------------------------
 constexpr int kPaKeys = 64;
 constexpr int kPaThreads = 256;
@@ -218,7 +222,7 @@ constexpr size_t pa_simt_smem() {
 }
 
 template <typename T, int HD, int RPT>
-__global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
+__global__ void __launch_bounds__(kPaThreads, HD <= 64 ? 2 : 1) pa_simt_kernel(const PaParams p) {
   constexpr int ROWS = 16 * RPT, LD = HD + 4, LP = kPaKeys + 4, VE = VecTraits<T>::kElems;
   constexpr int DP = HD / 16;  // dims a thread of the result, in runs of DV: tx * DV + 16 * DV * g ..
   constexpr int DV = DP < 4 ? DP : 4, DG = DP / DV;
@@ -300,11 +304,11 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
     }
     __syncthreads();
     if (j + kPaKeys < keys) fetch(j + kPaKeys);
-    float s[RPT][4];
+    float2 s2[RPT][4];  // sums over even and odd dims: two products an instruction
 #pragma unroll
     for (int a = 0; a < RPT; ++a)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) s[a][b] = 0.f;
+      for (int b = 0; b < 4; ++b) s2[a][b] = make_float2(0.f, 0.f);
 #pragma unroll 4
     for (int d = 0; d < HD; d += 4) {
       float4 kk[4];
@@ -314,10 +318,17 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
       for (int a = 0; a < RPT; ++a) {
         const float4 qq = *reinterpret_cast<const float4*>(sq + (ty * RPT + a) * LD + d);
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          s[a][b] = fmaf(qq.w, kk[b].w, fmaf(qq.z, kk[b].z, fmaf(qq.y, kk[b].y, fmaf(qq.x, kk[b].x, s[a][b]))));
+        for (int b = 0; b < 4; ++b) {
+          s2[a][b] = fma2(make_float2(qq.x, qq.y), make_float2(kk[b].x, kk[b].y), s2[a][b]);
+          s2[a][b] = fma2(make_float2(qq.z, qq.w), make_float2(kk[b].z, kk[b].w), s2[a][b]);
+        }
       }
     }
+    float s[RPT][4];
+#pragma unroll
+    for (int a = 0; a < RPT; ++a)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) s[a][b] = s2[a][b].x + s2[a][b].y;
     const bool masked = j + kPaKeys > low;
 #pragma unroll
     for (int a = 0; a < RPT; ++a) {
@@ -374,8 +385,16 @@ __global__ void __launch_bounds__(kPaThreads) pa_simt_kernel(const PaParams p) {
 #pragma unroll
           for (int a = 0; a < RPT; ++a) {
             const float pr = i == 0 ? pp[a].x : i == 1 ? pp[a].y : i == 2 ? pp[a].z : pp[a].w;
+            if constexpr (DP == 1) {
+              o[a][0] = fmaf(pr, x[0], o[a][0]);
+            } else {
 #pragma unroll
-            for (int d = 0; d < DP; ++d) o[a][d] = fmaf(pr, x[d], o[a][d]);
+              for (int d = 0; d < DP; d += 2) {
+                const float2 y = fma2(make_float2(pr, pr), make_float2(x[d], x[d + 1]), make_float2(o[a][d], o[a][d + 1]));
+                o[a][d] = y.x;
+                o[a][d + 1] = y.y;
+              }
+            }
           }
         }
       }
