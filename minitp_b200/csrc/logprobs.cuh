@@ -14,6 +14,14 @@
 // row may be reduced by several, each to its statistics and its k best logits
 // (packed keys: value, then lower id). A second kernel joins them, of every
 // shard of the vocabulary.
+//
+// Sums are fp32 per lane against a reference that follows the maximum only when
+// it has to; parts of a row are joined in fp64.
+//
+// Without alternatives bound by HBM: 4096 bf16 rows of 151936 235 us, 5.3 TB/s;
+// DRAM reads are the logits once. With alternatives each part of a row costs its
+// start, floors and ranking, about 10 000 cycles beside 2400 a tile: 2048 rows of
+// 151936 124 us without, 175 / 230 / 324 with 1 / 20 / 64; 512 rows with 20 76.
 #pragma once
 
 #include "topk.cuh"
