@@ -92,8 +92,8 @@ def _score_packed(model: TPQwen2ForCausalLM, prompts: list[torch.Tensor], top: i
         # every token but a prompt's last predicts the one behind it
         rows = torch.cat([torch.arange(a, a + k) for a, k in zip(starts, scored)]).to(dev)
         hidden, targets = hidden[rows], packed[rows + 1]
-        vloc = model.lm_head.vocab_end - model.lm_head.vocab_start
-        piece = max(1, _LOGITS_BYTES // (max(1, vloc) * hidden.element_size()))
+        # (pieces of the largest shard's logits: every rank takes the same ones, as each is an exchange)
+        piece = max(1, _LOGITS_BYTES // (model.lm_head._max_local_vocab() * hidden.element_size()))
         got = []
         for i in range(0, rows.numel(), piece):
             logits = ops.linear(hidden[i:i + piece], model.lm_head.weight)

@@ -127,6 +127,50 @@ def test_logprobs_exchange_the_shards_of_all_ranks(world, v):
         assert best == lp.topk(min(4, v), dim=-1).indices.tolist()
 
 
+
+def _w_score(rank, world, v):
+    from types import SimpleNamespace
+
+    import torch.distributed as dist
+
+    from minitp_b200 import scoring
+    from minitp_b200.distributed.context import ParallelContext
+    from minitp_b200.parallel import embedding
+
+    embedding.ops.logprobs_block = _cpu_block
+    embedding.ops.logprobs_join = lambda *a: tuple(torch.tensor(x) for x in _cpu_join(*a)) + (None,)
+    embedding.ops.linear = torch.nn.functional.linear
+    scoring._LOGITS_BYTES = 1000  # 4 rows of the larger shard, 5 of the smaller one
+    table, weight = _score_case(v)
+    head = embedding.VocabParallelLMHead(8, v, ParallelContext(rank, rank, world, rank, world, torch.device("cpu"), dist.group.WORLD))
+    head.weight.data = weight[head.vocab_start:head.vocab_end]
+    model = SimpleNamespace(model=SimpleNamespace(embed_tokens=SimpleNamespace(weight=table)), lm_head=head,
+                            cfg=SimpleNamespace(max_position_embeddings=64, vocab_size=v),
+                            forward_packed=lambda ids, starts: table[ids])
+    return [s.logprobs.tolist() for s in scoring.score_prompts(model, [[3, 1, 4, 1, 5, 9, 2], [6], [5, 3, 5, 8, 9]])]
+
+
+def _score_case(v):
+    r = torch.Generator().manual_seed(v)
+    return torch.randn(v, 8, generator=r), torch.randn(v, 8, generator=r)
+
+
+@pytest.mark.distributed
+def test_ranks_with_uneven_shards_score_in_the_same_pieces(lib):
+    """Every rank cuts the tokens into the same pieces, whatever its share of the vocabulary (the kernels played by
+    stand-ins, the hidden states by a table)."""
+    from tests.tp_harness import run_tp
+
+    table, weight = _score_case(101)
+    want = []
+    for ids in ([3, 1, 4, 1, 5, 9, 2], [6], [5, 3, 5, 8, 9]):
+        lp = torch.log_softmax((table[ids[:-1]] @ weight.T).double(), -1)
+        want.append([float(lp[i, t]) for i, t in enumerate(ids[1:])])
+    for got in run_tp(2, _w_score, 101).values():
+        for g, w in zip(got, want):
+            assert g == pytest.approx(w, abs=1e-4)  # (fp32 logits of magnitude 10 to 20, their log-sum in 64 bits)
+
+
 def test_packed_forward_refusals(lib):
     ok = dict(model=P, ids=P, T=4, pos=P, starts=P, S=1, k=P, v=P, hidden=P, st=None)
     # (a model's own sizes are looked at only after these)
