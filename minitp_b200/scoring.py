@@ -18,6 +18,7 @@ from minitp_b200 import ops
 from minitp_b200.layer import TPQwen2ForCausalLM
 
 _LOGITS_BYTES = 256 << 20  # of one piece
+_PROMPTS = 1 << 16  # of one forward (empty ones add no tokens; the attention takes 2^20)
 
 
 @dataclass
@@ -66,7 +67,7 @@ def score_prompts(
     at = 0
     while at < len(ids):
         end, tokens = at, 0
-        while end < len(ids) and (end == at or tokens + ids[end].numel() <= max_tokens):
+        while end < len(ids) and end - at < _PROMPTS and (end == at or tokens + ids[end].numel() <= max_tokens):
             tokens += ids[end].numel()
             end += 1
         out += _score_packed(model, [p.to(dev, torch.int64) for p in ids[at:end]], top)

@@ -253,6 +253,27 @@ def test_prompt_attention_strides(lib, dtype, hd):
     assert torch.equal(ops.prompt_attention(q, k1, v1, st), ops.prompt_attention(q, k1.contiguous(), v1.contiguous(), st))
 
 
+@pytest.mark.parametrize("dtype,heads_apart", [("bf16", False), ("fp32", False), ("bf16", True), ("fp32", True)])
+def test_prompt_attention_offsets_past_32_bits(lib, dtype, heads_apart):
+    """Tokens, or heads, that lie more than 2^31 elements apart."""
+    from minitp_b200 import ops
+
+    starts = [0, 3, 5]
+    far = 2 ** 29 + 64 if not heads_apart else 2 ** 28 + 64  # 5 tokens, or 8 heads
+    r = _gen(15)
+    packed = torch.randn(5, 8, 64, generator=r).to(DT[dtype]).cuda()
+    buf = torch.empty(4 * far + 8 * 64 if not heads_apart else 7 * far + 5 * 64, dtype=DT[dtype], device="cuda")
+    wide = buf.as_strided((5, 8, 64), (64, far, 1) if heads_apart else (far, 64, 1))
+    wide.copy_(packed)
+    (q, k, v), (fq, fk, fv) = ((t[:, :4], t[:, 4:6], t[:, 6:]) for t in (packed, wide))
+    if heads_apart:  # (two heads are not far apart: the second KV head is the last but one)
+        fk, fv, k, v = wide[:, 0:8:7], wide[:, 1:8:6], packed[:, 0:8:7], packed[:, 1:8:6]
+    st = _cuda_starts(starts)
+    got = ops.prompt_attention(fq, fk, fv, st)
+    _close(got, *scoring_ref.attend(q, k, v, starts))
+    assert torch.equal(got, ops.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), st))
+
+
 def test_prompt_attention_empty(lib):
     from minitp_b200 import ops
 
@@ -430,6 +451,21 @@ def test_token_logprobs_shapes_and_strides(lib):
         scoring_ref.check_logprobs([a[None] for a in single], x[1, 2:], t[1, 2:], 3)
         none = ops.token_logprobs(x[:0], t[:0], 3)
         assert none[0].shape == (0, 3) and none[3].shape == (0, 3, 3)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("v,top", [(1000, 0), (9001, 5)])
+def test_token_logprobs_offsets_past_32_bits(lib, dtype, v, top):
+    """Rows that lie more than 2^31 elements apart."""
+    from minitp_b200 import ops
+
+    r = _gen(16)
+    ld = 2 ** 30 + 8
+    x = (torch.randn(4, v, generator=r) * 2).to(DT[dtype]).cuda()
+    t = torch.randint(0, v, (4,), generator=r).cuda()
+    wide = torch.empty(3 * ld + v, dtype=DT[dtype], device="cuda").as_strided((4, v), (ld, 1))
+    wide.copy_(x)
+    scoring_ref.check_logprobs(ops.token_logprobs(wide, t, top), x, t, top)
 
 
 def test_token_logprobs_refusals(lib):

@@ -203,6 +203,20 @@ def test_greedy_generation_around_scoring(lib):
     assert torch.equal(generate_greedy(model, ids, 9, early_stop=False), first)
 
 
+def test_many_empty_prompts(lib):
+    """Prompts of no token add none to a forward, however many there are."""
+    from minitp_b200.scoring import score_prompts
+
+    model, cfg = _model("tiny")
+    ids = _prompts(cfg, [7, 5], 10)
+    want = score_prompts(model, ids, 2)
+    none = ids[0][:0]
+    got = score_prompts(model, [ids[0], *[none] * 70000, ids[1]], 2)
+    assert len(got) == 70002 and all(g.logprobs.numel() == 0 for g in got[1:-1])
+    for g, w in zip((got[0], got[-1]), want):
+        assert torch.allclose(g.logprobs, w.logprobs, rtol=0, atol=1e-4) and g.top_ids.shape == w.top_ids.shape
+
+
 def test_scoring_refusals(lib):
     from minitp_b200.scoring import score_prompts
 
