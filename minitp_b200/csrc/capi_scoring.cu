@@ -224,10 +224,13 @@ int pa_launch(PaParams p, cudaStream_t st) {
     // <= 509, 14 heads of 64: 59 / 44)
     return rows > 256ll * 148 ? pa_launch_tc<HD, 2>(p, st) : pa_launch_tc<HD, 1>(p, st);
   } else {
-    // Rows a tile: 64; 16 while those leave SMs idle (fp32 us of 16 / 64: 3 prompts of <= 300 tokens, 4 heads of 16:
-    // 11 / 17; 8 of <= 1024, 14 heads of 64: 452 / 156). 128 rows spill registers at 128 dims (one prompt of 7000, 7
-    // heads of 128: 2384 with 64, 2559 with 128).
-    return rows <= 16ll * 148 * 4 ? pa_launch_simt<T, HD, 1>(p, st) : pa_launch_simt<T, HD, 4>(p, st);
+    // Rows a tile: 64; 32 while those leave SMs idle (head dims 16 and 32, whose CTAs do less: one of two places an
+    // SM); 16 while 16 do. fp32 us of 16 / 32 / 64: 3 prompts of <= 300 tokens, 4 heads of 16: 11 / 12 / 15; one of 300,
+    // 14 of 64: 27 / 25 / 31; 10 of <= 200, 7 of 128: 54 / 37 / 43; 5 of <= 701, 8 of 32: 79 / 38 / 43; one of 2300:
+    // - / 149 / 136; one of 1300, 14 of 64: 261 / 164 / 140; 4 of <= 2048, 7 of 128: 888 / 556 / 332. 128 rows spill
+    // registers at 128 dims (one of 7000, 7 heads: 2384 with 64, 2559 with 128).
+    if (rows <= 16ll * 148) return pa_launch_simt<T, HD, 1>(p, st);
+    return rows <= (HD <= 32 ? 128ll : 64ll) * 148 ? pa_launch_simt<T, HD, 2>(p, st) : pa_launch_simt<T, HD, 4>(p, st);
   }
 }
 

@@ -882,8 +882,8 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
         const float ref = m == -INFINITY ? 0.f : m;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         // kCubic of 16 pairs on the fp32 pipe, which the special-function unit
-        // (8 cycles a warp and value) leaves idle; masked tiles need exact zeros
-        // masked: 32 keys that no row of the warp sees need none at all
+        // (8 cycles a warp and value) leaves idle; masked tiles need exact zeros,
+        // and of 32 keys that no row of the warp sees none at all
         auto exps = [&](auto mask) {
           constexpr bool kMask = decltype(mask)::value;
           constexpr int kCubic = kMask ? 0 : kPaCubic<HD>;

@@ -332,6 +332,24 @@ def test_prompt_attention_long_prompt(lib, dtype, hq, hkv, hd):
         _close(got[a:b], want, tol)
 
 
+@pytest.mark.parametrize("dtype,hd", [("fp32", 16), ("fp32", 32), ("fp32", 64), ("fp32", 128), ("bf16", 16), ("bf16", 32)])
+@pytest.mark.parametrize("lengths", [[40, 1, 61], [150, 0, 1, 201], [700, 1, 0, 450, 31]])
+def test_prompt_attention_row_tiles_of_every_size(lib, dtype, hd, lengths):
+    """Few, more and many rows, which take tiles of 16, 32 and 64 rows on the CUDA cores; values that are not finite."""
+    from minitp_b200 import ops
+
+    starts = _starts(lengths, at=2)
+    q, k, v = (t.clone() for t in _parts(_gen(17 + hd), starts[-1] + 3, 20, 4, hd, dtype))
+    v[starts[1] - 1, 0, 3] = math.nan  # the first prompt's last token alone
+    v[starts[-2] + 20, 1, 5] = math.inf
+    v[starts[-1] - 1, 3, 7] = -math.inf
+    got = ops.prompt_attention(q, k, v, _cuda_starts(starts))
+    _close(got, *scoring_ref.attend(q, k, v, starts))
+    a, b = starts[1] - 5, starts[-1] + 1  # a piece that begins and ends inside a tile
+    want, tol = scoring_ref.attend(q[a:b], k, v, starts, first=a)
+    _close(ops.prompt_attention(q[a:b], k, v, _cuda_starts(starts), first=a), want, tol)
+
+
 # ------------------------------------------------------------------ log-probabilities
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("rows,v,top", [(1, 1, 1), (1, 1000, 4), (3, 7, 7), (2, 7, 20), (5, 4097, 0), (4, 151936, 5),
