@@ -21,19 +21,7 @@ bool dtype_ok(int dtype) { return dtype == MTPB_BF16 || dtype == MTPB_F32; }
 // ------------------------------------------------------------------ log-probabilities
 constexpr long long kLpMaxRows = 1ll << 24;
 
-// Runs of tiles: a function of the sizes alone, so that every rank cuts its
-// shard alike. Three CTAs for each of B200's 148 SMs, which is what the ring
-// leaves room for.
-LpPlan lp_plan(long long rows, int V, int dtype) {
-  LpPlan b;
-  const int cols = kLpTile * (dtype == MTPB_BF16 ? 8 : 4);
-  b.tiles = (V + cols - 1) / cols;
-  const long long total = rows * b.tiles, ctas = std::min<long long>(total, 3 * 148);
-  b.run = int((total + ctas - 1) / ctas);
-  b.parts = (b.tiles - 2) / b.run + 2;  // a row that begins at a run's last tile; never more than its tiles
-  b.parts = std::max(1, std::min(b.parts, b.tiles));
-  return b;
-}
+LpPlan lp_plan_of(long long rows, int V, int dtype) { return lp_plan(rows, V, dtype == MTPB_BF16 ? 2 : 4); }
 
 size_t lp_stat_bytes(long long rows, const LpPlan& b) { return size_t(rows) * b.parts * sizeof(LpStat); }
 size_t lp_block(long long rows, const LpPlan& b, int k) {
@@ -100,7 +88,7 @@ long long mtpb_logprobs_block_bytes(int rows, int V_plan, int k, int dtype) {
   const int r = lp_check(rows, V_plan, k);
   if (r != MTPB_OK) return r;
   if (!dtype_ok(dtype)) return bad("unsupported dtype");
-  return (long long)lp_block(rows, lp_plan(rows, V_plan, dtype), k);
+  return (long long)lp_block(rows, lp_plan_of(rows, V_plan, dtype), k);
 }
 
 int mtpb_logprobs_block(const void* logits, int64_t ld, int rows, int V_local, int64_t vstart, int V_plan,
@@ -115,7 +103,7 @@ int mtpb_logprobs_block(const void* logits, int64_t ld, int rows, int V_local, i
   if (!al16(block)) return bad("token_logprobs: block must be 16-byte aligned");
   LpRowsParams p;
   std::memset(&p, 0, sizeof(p));
-  p.plan = lp_plan(rows, V_plan, dtype);
+  p.plan = lp_plan_of(rows, V_plan, dtype);
   p.logits = logits;
   p.ld = ld;
   p.rows = rows;
@@ -139,7 +127,7 @@ int mtpb_logprobs_join(const void* blocks, int shards, int rows, int V_plan, int
   if (!blocks || !al16(blocks)) return bad("token_logprobs: blocks must be 16-byte aligned");
   if (shards < 1 || shards > 64) return bad("token_logprobs: need 1 .. 64 shards");
   if (k < 0 || k > k_block) return bad("token_logprobs: more alternatives than the blocks hold");
-  return lp_join(blocks, shards, rows, lp_plan(rows, V_plan, dtype), k_block, targets, k, logprobs, entropy, top_logprobs,
+  return lp_join(blocks, shards, rows, lp_plan_of(rows, V_plan, dtype), k_block, targets, k, logprobs, entropy, top_logprobs,
                  top_ids, static_cast<cudaStream_t>(stream));
 }
 
@@ -149,7 +137,7 @@ int mtpb_token_logprobs(const void* logits, int64_t ld, int rows, int V, const i
   if (r == MTPB_OK) r = join_check(targets, k, logprobs, entropy, top_logprobs, top_ids);
   if (r == MTPB_OK) r = mtpb_logprobs_block(logits, ld, rows, V, 0, V, targets, k, block, dtype, stream);
   if (r != MTPB_OK) return r;
-  return lp_join(block, 1, rows, lp_plan(rows, V, dtype), k, targets, k, logprobs, entropy, top_logprobs, top_ids,
+  return lp_join(block, 1, rows, lp_plan_of(rows, V, dtype), k, targets, k, logprobs, entropy, top_logprobs, top_ids,
                  static_cast<cudaStream_t>(stream));
 }
 

@@ -24,6 +24,7 @@
 // 151936 124 us without, 175 / 230 / 324 with 1 / 20 / 64; 512 rows with 20 76.
 #pragma once
 
+#include "logprobs_plan.cuh"
 #include "topk.cuh"
 
 namespace mtpb {
@@ -36,22 +37,10 @@ struct LpStat {
   float m, s, w, xt;
 };
 
-constexpr int kLpWarps = kBeamWarps;  // that compute; one more copies and finds the floors
-constexpr int kLpVecs = 4;    // 16-byte vectors a lane and tile
-constexpr int kLpTile = kLpWarps * 32 * kLpVecs;  // vectors
-// Ring of tiles: what three CTAs an SM leave beside the candidates.
-template <bool TOP>
-constexpr int kLpStages = TOP ? 3 : 4;
+static_assert(kLpWarps == kBeamWarps, "beam_floor takes the candidates of as many warps");
 template <bool TOP>
 constexpr size_t kLpRing = size_t(kLpStages<TOP>) * kLpTile * 16;
 constexpr int kLpThreads = kLpWarps * 32;
-
-// How the tiles of `rows` rows of `tiles` tiles fall to CTAs of `run` tiles each.
-struct LpPlan {
-  int tiles, run, parts;  // parts: the most CTAs that share a row
-  __host__ __device__ long long first(long long row) const { return row * tiles / run; }  // CTA of a row's first tile
-  __host__ __device__ int count(long long row) const { return int(((row + 1) * tiles - 1) / run - first(row)) + 1; }
-};
 
 struct LpRowsParams {
   const void* logits;
@@ -249,18 +238,13 @@ __device__ __forceinline__ void lp_edge(const T* x, int n, int col, uint4 (&v)[k
   }
 }
 
-// Row r of the logits: its vectors begin `head` columns in, and `tail` columns stand behind the last whole one.
+// Row r of the logits.
 template <typename T>
-struct LpRow {
+struct LpRow : LpCols {
   const T* x;
-  int head, nvec, tail;
   __device__ __forceinline__ LpRow(const LpRowsParams& p, int r) {
-    constexpr int VE = VecTraits<T>::kElems;
     x = static_cast<const T*>(p.logits) + int64_t(r) * p.ld;
-    const int off = int((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
-    head = min(p.V, off ? VE - off : 0);
-    nvec = (p.V - head) / VE;
-    tail = p.V - head - nvec * VE;
+    static_cast<LpCols&>(*this) = lp_cols(reinterpret_cast<uintptr_t>(x), p.V, int(sizeof(T)));
   }
 };
 
@@ -307,46 +291,41 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
   int row = int(t0 / p.plan.tiles), tile = int(t0 - (long long)row * p.plan.tiles);
   int sg = 0;
   uint32_t phase = 0;
-  // After the tiles 0 and 3 of a part (of many candidates 0, 1, 3, 7 ..) the k-th
-  // of all warps' candidates becomes the floor: a later value enters with odds
-  // k / (values seen by the CTA), not k / (values of one warp's first tile).
-  // (2048 bf16 rows of 151936, never / 0, 3 / 0, 1, 3, 7 ..: 1 alternative 172 /
-  // 174 / 183 us, 64 alternatives 546 / 444 / 326; 512 rows, 20: 90 / 74 / 76.)
-  auto refloor = [&](int i, int last) {
-    return TOP && i < last && (p.k > 32 ? (i & (i + 1)) == 0 : i == 0 || i == 3);
-  };
+  auto refloor = [&](int i, int last) { return TOP && lp_refloor(p.k, i, last); };
   if (warp == kLpWarps) {  // ---- copies, a ring ahead of the tiles that the others are at, and floors
     int row2 = row, tile2 = tile, issued = 0, s2 = 0;  // of the next copy
     uint32_t ph2 = 0;
     long long t2 = t0;
     LpRow<T> w2 = row_at(row2);
     bool ok = true;
-    auto copy = [&]() {  // (skips tiles that the shard, of fewer columns than planned for, does not have)
-      while (t2 < t1) {
-        const int n = min(kLpTile, w2.nvec - tile2 * kLpTile);
-        const T* from = w2.x + w2.head + int64_t(tile2) * kLpTile * VE;
-        ++t2;
-        if (++tile2 == p.plan.tiles) {
-          tile2 = 0;
-          w2 = row_at(min(++row2, p.rows - 1));
-        }
-        if (n <= 0) continue;
-        ok = ok && (issued < NS || __all_sync(0xffffffffu, mbar_wait_lean(empty + s2, ph2 ^ 1u, abort)));
-        if (!ok) {
-          *abort = 1;
-          return;
-        }
-        if (lane == 0) {
-          mbar_arrive_expect_tx(full + s2, uint32_t(n) * 16);
-          bulk_g2s(ring + s2 * kLpTile, from, uint32_t(n) * 16, full + s2);
-        }
-        __syncwarp();
-        if (issued < NS) ++issued;
-        if (++s2 == NS) {
-          s2 = 0;
-          ph2 ^= 1u;
-        }
+    // One call a tile, whether it holds vectors or not: the slot that a call waits
+    // for then held a tile at or before the one that the others are at. (A call
+    // that passed over empty tiles would be ahead of them by a tile for each of
+    // those, and both would wait, here and at the floor's barrier, for one another.)
+    auto copy = [&]() {
+      if (t2 >= t1) return;
+      const int n = lp_tile_vecs(w2.nvec, tile2);
+      const T* from = w2.x + w2.head + int64_t(tile2) * kLpTile * VE;
+      ++t2;
+      if (++tile2 == p.plan.tiles) {
+        tile2 = 0;
+        w2 = row_at(min(++row2, p.rows - 1));
+      }
+      if (n <= 0) return;
+      ok = ok && (issued < NS || __all_sync(0xffffffffu, mbar_wait_lean(empty + s2, ph2 ^ 1u, abort)));
+      if (!ok) {
+        *abort = 1;
         return;
+      }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(full + s2, uint32_t(n) * 16);
+        bulk_g2s(ring + s2 * kLpTile, from, uint32_t(n) * 16, full + s2);
+      }
+      __syncwarp();
+      if (issued < NS) ++issued;
+      if (++s2 == NS) {
+        s2 = 0;
+        ph2 ^= 1u;
       }
     };
     for (int i = 0; i < NS; ++i) copy();
@@ -411,7 +390,7 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
       if (warp == 0 && tile == 0 && w.head) edge(w.head, 0);
       bool first = true;
       for (int i = 0, last = end - 1 - tile; tile < end; ++tile, ++i) {
-        const int n = min(kLpTile, w.nvec - tile * kLpTile), at = warp * 32 * kLpVecs + lane;
+        const int n = lp_tile_vecs(w.nvec, tile), at = warp * 32 * kLpVecs + lane;
         auto join_floor = [&]() {
           if (!refloor(i, last)) return;
           beam_drop(l, *static_cast<volatile uint32_t*>(floor_key));
