@@ -56,3 +56,36 @@ def test_shards_of_fewer_tiles_than_planned(lib, dtype, top):
     blocks = [ops.logprobs_block(x[:, a:b], t, top, a, plan) for a, b in zip(cuts, cuts[1:])]
     _check_some(ops.logprobs_join(torch.stack(blocks), t, (rows,), top, plan, DT[dtype]), x, t, top, 41)
     _status_is_clean(lib)
+
+
+# ------------------------------------------------------------------ attention
+# (query heads, KV heads, head dim, prompts) on the tensor cores; more than 256 x 148 (token, head) rows take
+# items of 256 rows, fewer items of 128
+LARGE = [(14, 2, 64, [600, 1, 0, 700, 300, 129, 850, 400]), (16, 2, 128, [513, 900, 1, 256, 128, 0, 640]),
+         (28, 4, 128, [301, 700, 420])]
+SMALL = [(4, 2, 64, [300, 600]), (4, 2, 128, [600, 300])]
+
+
+def _case(hq, hkv, hd, lengths, seed, large, at=0, behind=0):
+    starts = _starts(lengths, at=at)
+    total = starts[-1] + behind
+    assert (total * hq > 256 * 148) == large
+    return starts, *(t.clone() for t in _parts(_gen(seed), total, hq, hkv, hd, "bf16"))
+
+
+@pytest.mark.parametrize("large,hq,hkv,hd,lengths", [(True, *c) for c in LARGE] + [(False, *c) for c in SMALL])
+def test_rows_without_a_score_above_minus_infinity(lib, large, hq, hkv, hd, lengths):
+    """Tokens whose scores are all -inf get 0, however many keys they see; those with one finite score that key's V."""
+    from minitp_b200 import ops
+
+    starts, q, k, v = _case(hq, hkv, hd, lengths, 60 + hd, large)
+    per = hq // hkv
+    q[..., 0] = 1.0
+    whole = lengths.index(max(lengths))  # a prompt whose keys are all -inf for the first KV head
+    a, b = starts[whole], starts[whole + 1]
+    k[a:b, 0, 0] = -math.inf
+    k[a:b - 40, 1, 0] = -math.inf  # for the second one up to the last 40
+    k[starts[0]:starts[0] + 250, 0, 0] = -math.inf  # another prompt's first 250
+    got = ops.prompt_attention(q, k, v, _cuda_starts(starts))
+    assert not got[a:b, :per].any() and not got[a:b - 40, per:2 * per].any()
+    _close(got, *scoring_ref.attend(q, k, v, starts))
