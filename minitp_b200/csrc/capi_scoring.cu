@@ -169,21 +169,6 @@ int pa_map(CUtensorMap* map, const void* ptr, int tokens, int heads, long long t
   return r == CUDA_SUCCESS ? MTPB_OK : host_fail(MTPB_ERR_CUDA, "cuTensorMapEncodeTiled failed");
 }
 
-// Row groups and tokens of tiles of `rows` rows, and the items that there can
-// be at most: all heads of a KV head side by side, or as many of them as divide
-// them and fit.
-long long pa_items(PaParams* p, int rows) {
-  const int G = p->hq / p->hkv;
-  p->subs = 1;
-  while (G % p->subs || G / p->subs > rows) ++p->subs;
-  p->gs = G / p->subs;
-  p->planes = p->hkv * p->subs;
-  p->tt = rows / p->gs;
-  p->tt_mul = ((1ull << 37) + p->tt - 1) / p->tt;
-  p->gs_mul = (65536u + p->gs - 1) / p->gs;
-  return ((long long)p->n / p->tt + p->S) * p->planes;
-}
-
 template <int HD, int MT>
 int pa_launch_tc(PaParams p, cudaStream_t st) {
   const long long items = pa_items(&p, 128 * MT);
