@@ -48,4 +48,26 @@ int pt_find(const int* starts, int S, int first, int n, int total, int hq, int h
   });
   return apart;
 }
+
+// The same with a finder of its own for every number, as a CTA with one tile has it.
+int pt_only(const int* starts, int S, int first, int n, int total, int hq, int hkv, int rows, const int* numbers, int count,
+            int* out, int* tt, long long* items, int* gaps) {
+  const PaParams p = params(starts, S, first, n, total, hq, hkv, rows, items);
+  *tt = p.tt;
+  int apart = 0;
+  for (int i = 0; i < count; ++i)
+    warp_host::run([&](int lane) {
+      alignas(PaTiles) unsigned char memory[sizeof(PaTiles)];
+      std::memset(memory, 0xA5, sizeof(memory));
+      PaTiles& t = *reinterpret_cast<PaTiles*>(memory);
+      const PaItem it = t.only(p, numbers[i]);
+      const int got[3] = {it.start, it.tok0, it.ntok};
+      if (lane == 0) {
+        std::memcpy(out + 3 * i, got, sizeof(got));
+        gaps[0] = t.gap0, gaps[1] = t.gap1;
+      }
+      apart |= std::memcmp(out + 3 * i, got, sizeof(got)) != 0 || gaps[0] != t.gap0 || gaps[1] != t.gap1;
+    });
+  return apart;
+}
 }

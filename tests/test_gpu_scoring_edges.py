@@ -89,3 +89,55 @@ def test_rows_without_a_score_above_minus_infinity(lib, large, hq, hkv, hd, leng
     got = ops.prompt_attention(q, k, v, _cuda_starts(starts))
     assert not got[a:b, :per].any() and not got[a:b - 40, per:2 * per].any()
     _close(got, *scoring_ref.attend(q, k, v, starts))
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,hd", [("fp32", 4, 2, 16), ("bf16", 6, 3, 32), ("fp32", 7, 1, 128), ("bf16", 14, 2, 64),
+                                             ("bf16", 4, 1, 128)])
+def test_prompts_around_the_number_that_is_put_in_order(lib, dtype, hq, hkv, hd):
+    """31 to 33 and 63 to 65 prompts, and more; empty ones among them, a long one last, whole calls and pieces."""
+    from minitp_b200 import ops
+
+    for count in (31, 32, 33, 63, 64, 65, 129, 300):
+        r = _gen(count)
+        lengths = torch.randint(0, 9, (count,), generator=r).tolist()
+        lengths[count // 3] = 0
+        lengths[count - 1] = 150
+        starts = _starts(lengths, at=2)
+        q, k, v = _parts(r, starts[-1] + 3, hq, hkv, hd, dtype)
+        want, tol = scoring_ref.attend(q, k, v, starts)
+        _close(ops.prompt_attention(q, k, v, _cuda_starts(starts)), want, tol)
+        a, b = starts[count // 4] + 1, starts[-1] - 20
+        _close(ops.prompt_attention(q[a:b], k, v, _cuda_starts(starts), first=a), want[a:b], tol[a:b])
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,hd", [("fp32", 4, 2, 16), ("bf16", 4, 2, 64)])
+def test_as_many_prompts_as_a_scoring_forward_takes(lib, dtype, hq, hkv, hd):
+    """2^16 prompts of a few tokens: a token sees its own prompt, by the plain sums over up to four keys."""
+    from minitp_b200 import ops
+
+    count = 1 << 16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    lengths = torch.randint(0, 5, (count,), generator=g, device="cuda")
+    starts = torch.cat([lengths.new_zeros(1), lengths.cumsum(0)]).int()
+    n = int(starts[-1])
+    q, k, v = (torch.randn(n, h, hd, generator=g, device="cuda").to(DT[dtype]) for h in (hq, hkv, hkv))
+    got = ops.prompt_attention(q, k, v, starts)
+    tok = torch.arange(n, device="cuda")
+    first = starts.long().repeat_interleave(torch.cat([lengths, lengths.new_zeros(1)]))
+    per = hq // hkv
+    kd, vd = (x.double().repeat_interleave(per, 1) for x in (k, v))
+    back = tok[:, None] - torch.arange(4, device="cuda")  # a token and the three before it
+    seen = (back >= first[:, None])[:, None]
+    back = back.clamp(min=0)
+    s = (q.double()[:, :, None] * kd[back].transpose(1, 2)).sum(-1) / math.sqrt(hd)
+    p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+    want = (p[..., None] * vd[back].transpose(1, 2)).sum(2)
+    # (scoring_ref.attend's tolerance with |q k| <= 6 sqrt(hd) |q|, |v| <= 6 for these values: 4 keys)
+    half = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -24
+    mag = (q.double().abs()[:, :, None] * kd.abs()[back].transpose(1, 2)).sum(-1).amax(-1, keepdim=True) / math.sqrt(hd)
+    rel = 2 * (hd + 4) * 2.0 ** -24 * mag + 68 * 2.0 ** -24 + (2.0 ** -14 if dtype == "bf16" else 0.0)
+    tol = rel * vd[back].abs().amax(dim=(1, 3))[..., None] + 1.01 * half * want.abs()
+    if dtype == "bf16":
+        tol = tol + 1.01 * half * (p[..., None] * vd[back].abs().transpose(1, 2)).sum(2)
+    assert bool(((got.double() - want).abs() <= tol).all())
+    _status_is_clean(lib)

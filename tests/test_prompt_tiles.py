@@ -1,5 +1,6 @@
 """The finder of prompt attention's tiles on the host: every token in one tile, and nothing outside the queries."""
 
+import bisect
 import ctypes
 import os
 import random
@@ -101,3 +102,52 @@ def test_a_finder_left_early_leaves_gaps_within_the_tokens(host, count):
         _, _, _, gaps = _find(host, starts, 2, total - 2, total, 4, 2, 16, numbers)
         assert gaps[0] == 4 and 2 <= gaps[1] <= total
         assert gaps[1] in (starts[-1], total)  # the last prompt's end, or (not read yet) nothing to zero
+
+
+@pytest.mark.parametrize("count", COUNTS)
+def test_a_tile_found_by_itself(host, count):
+    """Each number on its own, as a CTA with one tile asks for it: every token in one tile, planned numbers only."""
+    r = random.Random(count + 7)
+    for hq, hkv, rows, longest in [(4, 2, 16, 9), (8, 4, 32, 20), (300, 1, 16, 4)]:
+        starts = _starts(r, count, longest, at=r.randint(0, 5))
+        total = starts[-1] + r.randint(0, 7)
+        for first, n in [(0, total), (total // 3, total - total // 3), (total // 4, total // 2)]:
+            if n == 0:
+                continue
+            tt = _find(host, starts, first, n, total, hq, hkv, rows, [])[1]
+            numbers = list(range(n // tt + count + 1))
+            tiles, _, _, gaps = _find(host, starts, first, n, total, hq, hkv, rows, numbers, "pt_only")
+            assert tiles[-1][2] == 0
+            _check(tiles, tt, starts, first, n)
+            assert gaps == (min(max(starts[0], first), first + n), min(max(starts[-1], first), first + n))
+
+
+def test_a_tile_among_a_million_prompts(host):
+    r = random.Random(3)
+    starts = _starts(r, 1 << 20, 3)
+    total = starts[-1]
+    for first, n in [(0, total), (1000, total - 2000)]:
+        tt = _find(host, starts, first, n, total, 4, 2, 16, [0], "pt_only")[1]
+        numbers = sorted(r.randrange(n // tt + (1 << 20)) for _ in range(1500))
+        tiles, _, _, _ = _find(host, starts, first, n, total, 4, 2, 16, numbers, "pt_only")
+        at = {}
+        for start, tok0, ntok in tiles:
+            if ntok:
+                at[tok0] = start
+        for tok0, start in at.items():
+            s = bisect.bisect_right(starts, tok0) - 1
+            assert starts[s] == start and first <= tok0 < first + n
+        assert len(at) > 500
+
+
+def test_a_tile_by_itself_of_starts_in_disorder(host):
+    r = random.Random(9)
+    for count in (65, 200, 1000):
+        for _ in range(10):
+            total = r.randint(1, 400)
+            starts = [r.choice([r.randint(-50, total + 50), -2 ** 31, 2 ** 31 - 1]) for _ in range(count + 1)]
+            first = r.randint(0, total - 1)
+            n = r.randint(1, total - first)
+            tiles, _, _, gaps = _find(host, starts, first, n, total, 4, 2, 16, list(range(n + count + 1)), "pt_only")
+            assert all(first <= tok0 and tok0 + ntok <= first + n and 0 <= start <= tok0 for start, tok0, ntok in tiles if ntok)
+            assert all(first <= g <= first + n for g in gaps)

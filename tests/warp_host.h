@@ -40,7 +40,7 @@ inline void entry() {
 // Runs body(lane) as one warp.
 inline void run(const std::function<void(int)>& body) {
   auto w = std::make_unique<State>();
-  std::vector<std::vector<char>> stacks(kLanes, std::vector<char>(256 << 10));
+  static std::vector<std::vector<char>> stacks(kLanes, std::vector<char>(64 << 10));
   g_warp = w.get();
   w->body = &body;
   for (int l = 0; l < kLanes; ++l) {
