@@ -183,7 +183,7 @@ int pa_launch_tc(PaParams p, cudaStream_t st) {
 
 template <typename T, int HD, int RPT>
 int pa_launch_simt(PaParams p, cudaStream_t st) {
-  const long long items = pa_items(&p, 16 * RPT) + 1;
+  const long long items = std::max<long long>(1, pa_items(&p, 16 * RPT));
   if (items > 0x7FFFFFFFll) return bad("prompt_attention: too many rows");
   return host_launch(pa_simt_kernel<T, HD, RPT>, dim3(unsigned(items)), dim3(kPaThreads), pa_simt_smem<HD, RPT>(), st, p);
 }

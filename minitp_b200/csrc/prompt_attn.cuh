@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kPaThreads, HD <= 64 ? 2 : 1) pa_simt_kernel(c
     PaItem it = tiles.only(p, blockIdx.x / p.planes);
     it.plane = blockIdx.x % p.planes;
     if (tid == 0) it_sh = it;
-    if (blockIdx.x == gridDim.x - 1) pa_zero<T>(p, tiles, HD, 0, 1);  // (the grid has a CTA more than tiles)
+    pa_zero<T>(p, tiles, HD, blockIdx.x, gridDim.x);
   }
   __syncthreads();
   const PaItem it = it_sh;

@@ -141,3 +141,18 @@ def test_as_many_prompts_as_a_scoring_forward_takes(lib, dtype, hq, hkv, hd):
         tol = tol + 1.01 * half * (p[..., None] * vd[back].abs().transpose(1, 2)).sum(2)
     assert bool(((got.double() - want).abs() <= tol).all())
     _status_is_clean(lib)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,hd", [("fp32", 4, 2, 16), ("fp32", 28, 4, 128), ("bf16", 14, 2, 64)])
+def test_few_tokens_of_many_are_in_a_prompt(lib, dtype, hq, hkv, hd):
+    """Tokens of no prompt in the thousands, before and behind few or many prompts, and no prompt at all, become 0."""
+    from minitp_b200 import ops
+
+    for total, starts in [(1, [0]), (3, [3]), (5000, [2500, 2520]), (5000, [4999]), (3000, list(range(1000, 1100)))]:
+        q, k, v = _parts(_gen(total), total, hq, hkv, hd, dtype)
+        for t in (q, k, v):
+            t[:starts[0]] = math.nan
+            t[starts[-1]:] = math.nan
+        want, tol = scoring_ref.attend(q, k, v, starts)
+        torch.empty(total, hq, hd, dtype=DT[dtype], device="cuda").fill_(math.nan)  # (what the output's memory may hold)
+        _close(ops.prompt_attention(q, k, v, _cuda_starts(starts)), want, tol)
