@@ -364,7 +364,9 @@ int mtpb_logprobs_join(const void* blocks, int shards, int rows, int V_plan, int
                        const int64_t* targets, int k, float* logprobs, float* entropy,
                        float* top_logprobs, int64_t* top_ids, int dtype, void* stream);
 
-/* As mtpb_beam_status, of the prompt attentions and log-probabilities. */
+/* As mtpb_beam_status, of the prompt attentions and log-probabilities. A row of
+ * log-probabilities that a wait ran out for is NaN; what an attention did not
+ * write holds anything. */
 int mtpb_scoring_status(uint32_t* status_out /* host */);
 
 /* ---------------------------------------------------------------- model

@@ -32,7 +32,8 @@ namespace mtpb {
 constexpr int kLpMaxK = kBeamMaxK;
 
 // Of a part of a row: m = max x, s = sum exp(x - m), w = sum exp(x - m) (x - m),
-// and the target's logit (NaN: the target lies elsewhere). s 0: no token.
+// and the target's logit (NaN: the target lies elsewhere). s 0: no token; NaN: a
+// wait for the part's logits ran out, and its row comes out as NaN.
 struct LpStat {
   float m, s, w, xt;
 };
@@ -462,6 +463,7 @@ __global__ void __launch_bounds__(kLpThreads + 32, 3) lp_rows_kernel(const LpRow
         if (lane == 0) {
           r.m = top;
           r.xt = !here ? __int_as_float(0x7fffffff) : xt == xt ? xt : -INFINITY;
+          if (*abort) r.s = __int_as_float(0x7fffffff);
           p.stat[at] = r;
           floors[odd ^ 1] = 0;  // (the part before's, which nobody reads any more)
           totals[odd ^ 1] = 0;
@@ -559,9 +561,10 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
   auto stat = [&](int i) { return p.stat + (i / per) * p.stat_shard + row * p.plan.parts + i % per; };
   auto cand = [&](int i) { return p.cand + (i / per) * p.cand_shard + (row * p.plan.parts + i % per) * p.kc; };
   float m = -INFINITY, xt = -INFINITY;
-  bool found = false;
+  bool found = false, lost = false;
   for (int i = lane; i < lists; i += 32) {
     const LpStat s = *stat(i);
+    lost = lost || s.s != s.s;
     if (s.s > 0.f) m = fmaxf(m, s.m);
     if (s.xt == s.xt) {
       xt = s.xt;
@@ -569,6 +572,8 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
     }
   }
   found = __any_sync(0xffffffffu, found);
+  lost = __any_sync(0xffffffffu, lost);
+  const float nan = __int_as_float(0x7fffffff);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -589,12 +594,13 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
   }
   const double logs = sum > 0.0 ? log(sum) : 0.0;
   auto logp = [&](float x) {
+    if (lost) return nan;
     if (x == -INFINITY) return -INFINITY;
     return float((x == m ? 0.0 : double(x) - double(m)) - logs);
   };
   if (lane == 0) {
-    p.entropy[row] = sum > 0.0 ? float(logs - w / sum) : 0.f;
-    if (p.logprobs) p.logprobs[row] = found ? logp(xt) : __int_as_float(0x7fffffff);
+    p.entropy[row] = lost ? nan : sum > 0.0 ? float(logs - w / sum) : 0.f;
+    if (p.logprobs) p.logprobs[row] = found ? logp(xt) : nan;
   }
   if (!p.k) return;
   const int n = lists * p.kc;
@@ -667,7 +673,7 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
     }
     live = __reduce_add_sync(0xffffffffu, live);
     for (int j = live + lane; j < p.k; j += 32) {
-      p.top_logprobs[row * p.k + j] = -INFINITY;
+      p.top_logprobs[row * p.k + j] = logp(-INFINITY);
       p.top_ids[row * p.k + j] = 0;
     }
     return;
@@ -688,7 +694,7 @@ __global__ void __launch_bounds__(32 * kLpJoinWarps) lp_join_kernel(const LpJoin
     const uint64_t top = warp_max_u64(b);
     if (top && b == top) ++head[at];
     if (lane == 0) {
-      p.top_logprobs[row * p.k + j] = top ? logp(beam_key_val(uint32_t(top >> 32))) : -INFINITY;
+      p.top_logprobs[row * p.k + j] = logp(top ? beam_key_val(uint32_t(top >> 32)) : -INFINITY);
       p.top_ids[row * p.k + j] = top ? (long long)(0xFFFFFFFFu - uint32_t(top)) : 0;
     }
   }

@@ -8,6 +8,7 @@ stream. None of them has a CPU path: CPU tensors raise.
 from __future__ import annotations
 
 import array
+import ctypes
 import functools
 import operator
 
@@ -457,6 +458,18 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     _call_on(dev, "mtpb_prompt_attention", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
              out.data_ptr(), seq_starts.data_ptr(), seq_starts.numel() - 1, first, n, total, hq, hkv, hd, code)
     return out
+
+
+def raise_on_scoring_error(device: torch.device | str | int) -> None:
+    """Wait for the device's work, and raise when a bounded wait of a prompt attention or log-probability kernel ran
+    out there since the last look: what those calls returned is then void (log-probabilities show NaN, outputs of an
+    attention hold anything). ``score_prompts`` looks itself; a forward's attentions report to its communicator."""
+    status = ctypes.c_uint32()
+    with torch.cuda.device(device):
+        _lib.call("mtpb_scoring_status", ctypes.byref(status))
+    if status.value:
+        raise _lib.MinitpB200Error("a bounded wait of a prompt attention or log-probability kernel ran out: the results "
+                                   f"since the last look are void (status {status.value:#x})")
 
 
 def _logprob_rows(name: str, logits: torch.Tensor, targets: torch.Tensor | None, top: int, least: int = 1):

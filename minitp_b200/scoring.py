@@ -14,7 +14,7 @@ from typing import Sequence
 
 import torch
 
-from minitp_b200 import ops
+from minitp_b200 import _lib, ops
 from minitp_b200.layer import TPQwen2ForCausalLM
 
 _LOGITS_BYTES = 256 << 20  # of one piece
@@ -48,7 +48,8 @@ def score_prompts(
     on any device; a prompt of one token or none has empty scores. ``top``: likeliest
     alternatives per token (0 to 64). Prompts are packed into forwards of at most
     ``max_tokens`` tokens (a longer prompt goes alone). The results are on the
-    model's device.
+    model's device, and complete: errors that a kernel can only report to the
+    device's status words (a wait that ran out) raise here.
     """
     dev = model.model.embed_tokens.weight.device
     if not 0 <= top <= 64:
@@ -63,6 +64,8 @@ def score_prompts(
             raise ValueError(f"{p.numel()} positions needed, the model has {model.cfg.max_position_embeddings}")
         if p.numel() and not p.is_cuda and not (0 <= int(p.min()) and int(p.max()) < model.cfg.vocab_size):
             raise ValueError(f"token ids outside the vocabulary of {model.cfg.vocab_size}")
+    comm = model.ctx.comm() if dev.type == "cuda" else None
+    before = comm.status() if comm else 0  # (what earlier calls left there is theirs, but for a peer that is gone)
     out: list[PromptScores] = []
     at = 0
     while at < len(ids):
@@ -72,6 +75,10 @@ def score_prompts(
             end += 1
         out += _score_packed(model, [p.to(dev, torch.int64) for p in ids[at:end]], top)
         at = end
+    if comm:
+        ops.raise_on_scoring_error(dev)
+        if comm.status() & (~before | _lib.STATUS_TIMEOUT):
+            comm.raise_on_error()
     return out
 
 

@@ -156,3 +156,93 @@ def test_few_tokens_of_many_are_in_a_prompt(lib, dtype, hq, hkv, hd):
         want, tol = scoring_ref.attend(q, k, v, starts)
         torch.empty(total, hq, hd, dtype=DT[dtype], device="cuda").fill_(math.nan)  # (what the output's memory may hold)
         _close(ops.prompt_attention(q, k, v, _cuda_starts(starts)), want, tol)
+
+
+# ------------------------------------------------------------------ errors that only the device knows of
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("top", [0, 3, 64])
+def test_rows_of_lost_parts_are_nan(lib, dtype, top):
+    """Statistics that say that a part's logits never came make their row NaN, alternatives too, and no other row."""
+    from minitp_b200 import ops
+
+    rows, v = 40, 60000
+    x = torch.randn(rows, v, generator=_gen(top)).to(DT[dtype]).cuda()
+    t = torch.arange(rows, device="cuda") * 7
+    blocks = torch.stack([ops.logprobs_block(x[:, :30000], t, top, 0, 30000), ops.logprobs_block(x[:, 30000:], t, top, 30000, 30000)])
+    want = ops.logprobs_join(blocks, t, (rows,), top, 30000, DT[dtype])
+    # a row has a part at least; its statistics are {max, sum, mean, target}, at the block's start
+    parts = (blocks.shape[1] // rows) // (16 + 8 * top)
+    for row in (0, 17, rows - 1):
+        at = row * parts * 16 + 4
+        blocks[row % 2, at:at + 4] = torch.tensor([255, 255, 255, 127], dtype=torch.uint8)  # the sum: NaN
+    got = ops.logprobs_join(blocks, t, (rows,), top, 30000, DT[dtype])
+    lost = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    lost[[0, 17, rows - 1]] = True
+    for g, w in zip(got[:3], want[:3]):
+        if g is not None:
+            assert bool(g[lost].isnan().all()) and torch.equal(g[~lost], w[~lost])
+    if top:
+        assert torch.equal(got[3][~lost], want[3][~lost])
+
+
+def test_a_wait_that_ran_out_raises(lib, monkeypatch):
+    """`raise_on_scoring_error` by a status that a stand-in of the library call hands back, and by the real one."""
+    from minitp_b200 import _lib, ops
+
+    ops.raise_on_scoring_error("cuda")
+    call = _lib.call
+
+    def fake(name, *args):
+        if name == "mtpb_scoring_status":
+            args[0]._obj.value = _lib.STATUS_TIMEOUT
+            return
+        call(name, *args)
+
+    monkeypatch.setattr(_lib, "call", fake)
+    with pytest.raises(_lib.MinitpB200Error, match="ran out"):
+        ops.raise_on_scoring_error("cuda")
+
+
+def _tiny_model():
+    from minitp_b200 import config as mcfg
+    from minitp_b200.distributed.context import context_for
+    from minitp_b200.weight_loader import load_synthetic_tp
+
+    cfg = mcfg.baseline_tiny()
+    return load_synthetic_tp(cfg, context_for(1, "cuda"), dtype=torch.float32, device=torch.device("cuda")), cfg
+
+
+def test_scores_whose_forward_reported_an_error_are_not_returned(lib, monkeypatch):
+    """A forward that flags its communicator makes `score_prompts` raise; a word set before does not."""
+    from minitp_b200 import _lib, ops
+    from minitp_b200.scoring import score_prompts
+
+    model, cfg = _tiny_model()
+    comm = model.ctx.comm()
+    prompts = [[1, 2, 3], [4, 5]]
+    want = score_prompts(model, prompts)
+    real = model.forward_packed
+
+    def behind_the_table(ids, starts):
+        return real(ids, starts, torch.full_like(ids, cfg.max_position_embeddings + 5))
+
+    try:
+        monkeypatch.setattr(model, "forward_packed", behind_the_table)
+        with pytest.raises(_lib.MinitpB200Error, match="position"):
+            score_prompts(model, prompts)
+        monkeypatch.undo()
+        again = score_prompts(model, prompts)  # (the word still holds what the call before reported)
+        assert all(torch.equal(a.logprobs, w.logprobs) for a, w in zip(again, want))
+    finally:
+        comm.clear_status()
+    status = _lib.call
+
+    def ran_out(name, *args):
+        if name == "mtpb_scoring_status":
+            args[0]._obj.value = _lib.STATUS_TIMEOUT
+            return
+        status(name, *args)
+
+    monkeypatch.setattr(_lib, "call", ran_out)
+    with pytest.raises(_lib.MinitpB200Error, match="ran out"):
+        score_prompts(model, prompts)
