@@ -62,7 +62,9 @@ def score_prompts(
             raise ValueError(f"prompts must be integer sequences [n], got {p.dtype} {tuple(p.shape)}")
         if p.numel() > model.cfg.max_position_embeddings:
             raise ValueError(f"{p.numel()} positions needed, the model has {model.cfg.max_position_embeddings}")
-        if p.numel() and not p.is_cuda and not (0 <= int(p.min()) and int(p.max()) < model.cfg.vocab_size):
+    for where in {p.device for p in ids}:  # (one look at each device's ids)
+        some = torch.cat([p.to(torch.int64) for p in ids if p.device == where])
+        if some.numel() and not bool(((some >= 0) & (some < model.cfg.vocab_size)).all()):
             raise ValueError(f"token ids outside the vocabulary of {model.cfg.vocab_size}")
     comm = model.ctx.comm() if dev.type == "cuda" else None
     before = comm.status() if comm else 0  # (what earlier calls left there is theirs, but for a peer that is gone)

@@ -246,3 +246,17 @@ def test_scores_whose_forward_reported_an_error_are_not_returned(lib, monkeypatc
     monkeypatch.setattr(_lib, "call", ran_out)
     with pytest.raises(_lib.MinitpB200Error, match="ran out"):
         score_prompts(model, prompts)
+
+
+def test_ids_outside_the_vocabulary_are_refused_on_either_device(lib):
+    from minitp_b200.scoring import score_prompts
+
+    model, cfg = _tiny_model()
+    for wrong in (-1, cfg.vocab_size, 2 ** 40, -2 ** 40):
+        for device in ("cpu", "cuda"):
+            with pytest.raises(ValueError, match="vocabulary"):
+                score_prompts(model, [[1, 2], torch.tensor([3, wrong], device=device), torch.tensor([5], device="cuda")])
+    assert model.ctx.comm().status() == 0
+    last = torch.tensor([0, cfg.vocab_size - 1])
+    for ids in (last, last.cuda(), last.to(torch.int16 if cfg.vocab_size < 2 ** 15 else torch.int32).cuda(), last.tolist()):
+        assert bool(torch.isfinite(score_prompts(model, [ids])[0].logprobs).all())
