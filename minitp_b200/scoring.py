@@ -9,6 +9,7 @@ pieces, so that no more than a few hundred megabytes of logits exist at once.
 
 from __future__ import annotations
 
+import operator
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -56,7 +57,7 @@ def score_prompts(
         raise ValueError(f"top must be 0 .. 64, got {top}")
     if max_tokens < 1:
         raise ValueError(f"max_tokens must be positive, got {max_tokens}")
-    ids = [p if isinstance(p, torch.Tensor) else torch.tensor(list(p), dtype=torch.int64) for p in prompts]
+    ids = [p if isinstance(p, torch.Tensor) else _id_tensor(p) for p in prompts]
     for p in ids:
         if p.dim() != 1 or p.dtype.is_floating_point or p.dtype.is_complex or p.dtype == torch.bool:
             raise ValueError(f"prompts must be integer sequences [n], got {p.dtype} {tuple(p.shape)}")
@@ -82,6 +83,13 @@ def score_prompts(
         if comm.status() & (~before | _lib.STATUS_TIMEOUT):
             comm.raise_on_error()
     return out
+
+
+def _id_tensor(prompt: Sequence[int]) -> torch.Tensor:
+    try:  # (torch would cut 1.5 to 1)
+        return torch.tensor([operator.index(i) for i in prompt], dtype=torch.int64)
+    except (TypeError, ValueError, OverflowError, RuntimeError) as e:
+        raise ValueError(f"prompts must be integer sequences [n]: {e}") from None
 
 
 def _score_packed(model: TPQwen2ForCausalLM, prompts: list[torch.Tensor], top: int) -> list[PromptScores]:

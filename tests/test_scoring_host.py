@@ -177,3 +177,21 @@ def test_packed_forward_refusals(lib):
     for change, match in [(dict(model=None), "null"), (dict(ids=None), "null"), (dict(pos=None), "null"), (dict(starts=None), "null"),
                           (dict(hidden=None), "null"), (dict(k=None), "null"), (dict(T=0), "empty"), (dict(S=-1), "empty")]:
         _refused(lib, "mtpb_model_forward_packed", list((ok | change).values()), match)
+
+
+def test_prompts_that_are_no_integers_are_refused():
+    """Lists are held to what tensors are: nothing is cut to an integer on the way (before any use of the model)."""
+    from types import SimpleNamespace
+
+    import numpy as np
+
+    from minitp_b200 import scoring
+
+    model = SimpleNamespace(model=SimpleNamespace(embed_tokens=SimpleNamespace(weight=torch.zeros(1))),
+                            cfg=SimpleNamespace(max_position_embeddings=64, vocab_size=10))
+    for wrong in ([1.5, 2], [1.0, 2.0], np.array([1.0, 2.0]), "12", [[1, 2], [3, 4]], [1, None], [2 ** 70], torch.zeros(2)):
+        with pytest.raises(ValueError, match="sequences"):
+            scoring.score_prompts(model, [[1, 2], wrong])
+    for fine in ([1, 2], (1, 2), np.array([1, 2]), np.array([1, 2], dtype=np.uint16), range(1, 3), [torch.tensor(1), np.int32(2)]):
+        assert scoring._id_tensor(fine).tolist() == [1, 2]
+    assert scoring._id_tensor([]).dtype == torch.int64
