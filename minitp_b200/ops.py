@@ -432,7 +432,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     own prompt up to itself. ``k`` and ``v [tokens, hkv, hd]`` hold all tokens,
     ``q [n, hq, hd]`` those from ``first`` on (all by default). Tokens and heads
     may be strided (the parts of one projection's output are read in place). A
-    token of no prompt gets 0.
+    token of no prompt gets 0. At most 2^28 (token, head) rows, 2^16 heads and
+    2^20 prompts.
     """
     name = "prompt_attention"
     dev = _same_device(name, q, k, v, seq_starts)
@@ -450,6 +451,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
         raise _lib.MinitpB200Error(f"{name}: {hq} heads over {hkv}")
     if not 0 <= first <= total - n:
         raise _lib.MinitpB200Error(f"{name}: tokens {first} .. {first + n} of {total} packed ones")
+    if hd not in (16, 32, 64, 128):
+        raise _lib.MinitpB200Error(f"{name}: head_dim must be 16, 32, 64 or 128, got {hd}")
+    if total * hq > 1 << 28 or hq > 1 << 16 or seq_starts.numel() > (1 << 20) + 1:  # (here, before they become C ints)
+        raise _lib.MinitpB200Error(f"{name}: more than 2^28 (token, head) rows, 2^16 heads or 2^20 prompts")
     code = _lib.dtype_code(q.dtype)
     out = torch.empty_strided((n, hq, hd), (hq * hd, hd, 1), dtype=q.dtype, device=dev)
     q, qt, qh = _packed_strides(q)
@@ -472,6 +477,12 @@ def raise_on_scoring_error(device: torch.device | str | int) -> None:
                                    f"since the last look are void (status {status.value:#x})")
 
 
+def _logprob_limits(name: str, rows: int, v: int) -> None:
+    """The C calls' limits, before sizes become C ints."""
+    if rows > 1 << 24 or rows * v > 1 << 40:
+        raise _lib.MinitpB200Error(f"{name}: more than 2^24 rows or 2^40 logits: {rows} of {v}")
+
+
 def _logprob_rows(name: str, logits: torch.Tensor, targets: torch.Tensor | None, top: int, least: int = 1):
     """Checks shared by the log-probability calls -> (device, logits as rows, row stride, targets as rows)."""
     if logits.dim() < 1:
@@ -480,13 +491,14 @@ def _logprob_rows(name: str, logits: torch.Tensor, targets: torch.Tensor | None,
     v = logits.shape[-1]
     if not (0 <= top <= 64 and least <= v < 2**30):
         raise _lib.MinitpB200Error(f"{name}: need 0..64 alternatives and a vocabulary of 1 .. 2^30 - 1")
+    rows = 1
+    for s in logits.shape[:-1]:
+        rows *= s
+    _logprob_limits(name, rows, v)
     if targets is not None:
         if targets.dtype != torch.int64 or targets.shape != logits.shape[:-1]:
             raise _lib.MinitpB200Error(f"{name}: targets must be int64 {tuple(logits.shape[:-1])}")
         targets = _c(targets)
-    rows = 1
-    for s in logits.shape[:-1]:
-        rows *= s
     # rows of one stride are read in place; anything else is packed first
     x = logits if logits.dim() == 2 else logits.reshape(rows, v)
     if x.stride(1) != 1 and v > 1:
@@ -523,7 +535,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     ``[..., top]``, best first, equal ones by the lower id (None with ``top``
     0; at most 64). A NaN logit counts as -inf (a banned token); +inf logits
     share the probability. Places without a token above -inf hold -inf and id
-    0; a row without any has entropy 0.
+    0; a row without any has entropy 0. At most 2^24 rows and 2^40 logits.
     """
     dev, x, ld, targets = _logprob_rows("token_logprobs", logits, targets, top)
     rows, v = x.shape
@@ -548,7 +560,7 @@ def logprobs_block_bytes(rows: int, v_plan: int, top: int, dtype: torch.dtype) -
 def logprobs_block(local_logits: torch.Tensor, targets: torch.Tensor | None, top: int, vstart: int,
                    v_plan: int) -> torch.Tensor:
     """One vocabulary shard ``[..., V_local]`` (columns from ``vstart``; it may be empty) reduced to a block (uint8
-    [n]). ``v_plan``: the largest shard's columns, the same on every rank."""
+    [n]). ``v_plan``: the largest shard's columns, the same on every rank; at most 2^24 rows and 2^40 logits."""
     if not (0 <= vstart < 2**32 and 1 <= v_plan < 2**30):
         raise _lib.MinitpB200Error(f"logprobs_block: need a start below 2^32 and a plan of at least one column, got "
                                    f"{vstart} and {v_plan}")
@@ -573,6 +585,9 @@ def logprobs_join(blocks: torch.Tensor, targets: torch.Tensor | None, shape, top
         raise _lib.MinitpB200Error(f"logprobs_join: targets must be int64 {tuple(shape)}")
     if not (0 <= top <= 64 and 1 <= v_plan < 2**30):
         raise _lib.MinitpB200Error(f"logprobs_join: need 0..64 alternatives, got {top}")
+    _logprob_limits("logprobs_join", rows, v_plan)
+    if blocks.dim() == 2 and not 1 <= blocks.shape[0] <= 64:
+        raise _lib.MinitpB200Error(f"logprobs_join: need 1 .. 64 shards, got {blocks.shape[0]}")
     need = logprobs_block_bytes(rows, v_plan, top, dtype) if rows else 0
     if blocks.dim() != 2 or blocks.dtype != torch.uint8 or not blocks.is_contiguous() or blocks.shape[1] != need:
         raise _lib.MinitpB200Error(

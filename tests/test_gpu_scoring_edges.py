@@ -260,3 +260,28 @@ def test_ids_outside_the_vocabulary_are_refused_on_either_device(lib):
     last = torch.tensor([0, cfg.vocab_size - 1])
     for ids in (last, last.cuda(), last.to(torch.int16 if cfg.vocab_size < 2 ** 15 else torch.int32).cuda(), last.tolist()):
         assert bool(torch.isfinite(score_prompts(model, [ids])[0].logprobs).all())
+
+
+def test_sizes_past_the_c_types_are_refused(lib):
+    """Sizes whose lower 32 bits look fine are refused, not cut to those (expanded tensors: no memory behind them)."""
+    from minitp_b200 import _lib, ops
+
+    far = 2 ** 32
+    q, k = torch.zeros(5, 2, 64, device="cuda"), torch.zeros(5, 1, 64, device="cuda")
+    st = _cuda_starts([0, 5])
+    wide = torch.zeros(1, device="cuda").expand(5, 1, far + 64)
+    for args, match in [((q, k[:1].expand(far + 5, 1, 64), k[:1].expand(far + 5, 1, 64), st), "rows"),
+                        ((q[:, :1].expand(5, far + 2, 64), k, k, st), "heads"), ((wide, wide, wide, st), "head_dim"),
+                        ((q, k, k, torch.zeros(2 ** 20 + 2, dtype=torch.int32, device="cuda")), "prompts")]:
+        with pytest.raises(_lib.MinitpB200Error, match=match):
+            ops.prompt_attention(*args)
+    x, t = torch.zeros(1, 10, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    for rows in (far + 8, 2 ** 24 + 1):
+        for call in (lambda: ops.token_logprobs(x.expand(rows, 10), t.expand(rows), 2),
+                     lambda: ops.logprobs_block(x.expand(rows, 10), None, 2, 0, 10),
+                     lambda: ops.logprobs_join(torch.zeros(1, 16, dtype=torch.uint8, device="cuda"), None, (rows,), 2, 10,
+                                               torch.float32)):
+            with pytest.raises(_lib.MinitpB200Error, match="rows"):
+                call()
+    with pytest.raises(_lib.MinitpB200Error, match="shards"):
+        ops.logprobs_join(torch.zeros(65, 16, dtype=torch.uint8, device="cuda"), None, (1,), 0, 10, torch.float32)
