@@ -1105,6 +1105,8 @@ int model_forward_t(ModelHost& mh, const FwdArgs& a, cudaStream_t st) {
     return fail(MTPB_ERR_INVALID, "forward: batch x hidden exceeds the communicator slot");
   if (a.decode && (a.T != 1 || a.B > 64)) return fail(MTPB_ERR_INVALID, "decode step: T == 1 and B <= 64");
   const int tc = int(std::min<size_t>(size_t(a.T), comm.slot_bytes / row_bytes));
+  // (a refusal in the middle of the chain would leave its AllReduce sites half used)
+  if (a.packed) MTPB_TRY(prompt_attn_check(packed_args(mh, a, 0, 0, tc)));
   MTPB_TRY(model_reserve(mh, a.B * tc, st));
   if (a.shared) MTPB_TRY(shared_reserve(mh, a, tc, st));
   for (int t0 = 0; t0 < a.T; t0 += tc) {

@@ -221,7 +221,7 @@ int pa_launch_hd(const PaParams& p, int hd, cudaStream_t st) {
 
 namespace mtpb {
 
-int prompt_attn_run(const PromptAttnArgs& a, cudaStream_t st) {
+int prompt_attn_check(const PromptAttnArgs& a) {
   if (a.n < 0 || a.total < 0 || a.S < 0 || a.hq < 1 || a.hkv < 1) return bad("prompt_attention: negative size");
   if (a.hq % a.hkv) return bad("prompt_attention: hq must be a multiple of hkv");
   if (a.hd != 16 && a.hd != 32 && a.hd != 64 && a.hd != 128)
@@ -232,6 +232,12 @@ int prompt_attn_run(const PromptAttnArgs& a, cudaStream_t st) {
   if ((long long)a.total * a.hq > 1 << 28) return bad("prompt_attention: more than 2^28 (token, head) rows");
   if (a.hq > 1 << 16) return bad("prompt_attention: more than 2^16 heads");
   if (a.S > 1 << 20) return bad("prompt_attention: more than 2^20 prompts");
+  return MTPB_OK;
+}
+
+int prompt_attn_run(const PromptAttnArgs& a, cudaStream_t st) {
+  const int fits = prompt_attn_check(a);
+  if (fits != MTPB_OK) return fits;
   if (a.n == 0) return MTPB_OK;
   if (!a.q || !a.k || !a.v || !a.out || !a.seq_starts) return bad("prompt_attention: null tensor");
   const int es = a.dtype == MTPB_BF16 ? 2 : 4, ve = 16 / es;

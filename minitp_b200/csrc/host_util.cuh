@@ -86,6 +86,8 @@ struct PromptAttnArgs {
   int S, first, n, total, hq, hkv, hd, dtype;
   uint32_t* status = nullptr;  // word for error bits, or NULL: the library's own
 };
+// Whether a call of these sizes is taken (no pointer and no device is looked at).
+int prompt_attn_check(const PromptAttnArgs& a);
 int prompt_attn_run(const PromptAttnArgs& a, cudaStream_t st);
 
 }  // namespace mtpb

@@ -285,3 +285,32 @@ def test_sizes_past_the_c_types_are_refused(lib):
                 call()
     with pytest.raises(_lib.MinitpB200Error, match="shards"):
         ops.logprobs_join(torch.zeros(65, 16, dtype=torch.uint8, device="cuda"), None, (1,), 0, 10, torch.float32)
+
+
+def test_a_packed_forward_that_is_refused_launches_nothing(lib):
+    """Limits of the attention are looked at before the first kernel: a capture of the refused call holds no node."""
+    from cuda.bindings import runtime
+
+    from minitp_b200 import _lib
+
+    model, cfg = _tiny_model()
+    ids = torch.arange(8, device="cuda")
+    few, many = _cuda_starts([0, 8]), torch.zeros(2 ** 20 + 2, dtype=torch.int32, device="cuda")
+    want = model.forward_packed(ids, few, ids)
+
+    def nodes(starts, refused):
+        g = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(g):
+            if refused:
+                with pytest.raises(_lib.MinitpB200Error, match="prompts"):
+                    model.forward_packed(ids, starts, ids)
+            else:
+                model.forward_packed(ids, starts, ids)
+        err, _, count = runtime.cudaGraphGetNodes(g.raw_cuda_graph(), 0)
+        assert int(err) == 0
+        return count
+
+    assert nodes(few, False) > 0
+    assert nodes(many, True) == 0
+    assert torch.equal(model.forward_packed(ids, few, ids), want)
+    assert model.ctx.comm().status() == 0
