@@ -777,8 +777,9 @@ __global__ void __launch_bounds__(kPaTcThreads, 1)
       }
       tc_fence_after();
       // no score above -inf: the sum is what the cubic, which ends at 2^-125, made of those (the growth from -inf
-      // to a first score takes it out, and so does MT 1's weight of a stream)
-      if (m == -INFINITY) l = 0.f;
+      // to a first score takes it out, and so does MT 1's weight of a stream). A NaN sum stays: behind a NaN score
+      // a tile that the row does not see sets m to -inf.
+      if (m == -INFINITY && l == l) l = 0.f;
       float w0 = 1.f, w1 = 0.f;  // weights of this stream's O and the other's
       if (MT == 1) {
         ml_sh[n & 1][x][r] = make_float2(m, l);

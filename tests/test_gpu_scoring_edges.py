@@ -91,6 +91,121 @@ def test_rows_without_a_score_above_minus_infinity(lib, large, hq, hkv, hd, leng
     _close(got, *scoring_ref.attend(q, k, v, starts))
 
 
+@pytest.mark.parametrize("hq,hkv,hd,lengths", LARGE)
+def test_large_items_nan_and_infinities(lib, hq, hkv, hd, lengths):
+    """Of K and V, in the middle of prompts, at tiles' edges and at their last tokens, for one KV head each."""
+    from minitp_b200 import ops
+
+    starts, q, k, v = _case(hq, hkv, hd, lengths, 70 + hd, True)
+    per, last = hq // hkv, hkv - 1
+    ends = [b for a, b in zip(starts, starts[1:]) if b > a]
+    v[100, 0, 3] = math.nan
+    v[127, 0, 5] = math.inf
+    v[128, last, 7] = -math.inf
+    for i, b in enumerate(ends):  # seen by the last token alone
+        v[b - 1, i % hkv, 8 + i] = (math.nan, math.inf, -math.inf)[i % 3]
+    a = starts[-2]
+    k[a + 290, 0, 2] = math.nan  # later tokens' scores
+    got = ops.prompt_attention(q, k, v, _cuda_starts(starts))
+    want, tol = scoring_ref.attend(q, k, v, starts)
+    want[a + 290:starts[-1], :per] = math.nan
+    _close(got, want, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,hd,lengths", LARGE)
+def test_large_items_large_scores(lib, hq, hkv, hd, lengths):
+    """Scores of some thousands that grow along the tokens (the running maximum moves at every tile) or fall."""
+    from minitp_b200 import ops
+
+    starts, q, k, v = _case(hq, hkv, hd, lengths, 80 + hd, True)
+    q[..., 0] = 40.0
+    for sign in (1, -1):
+        k[..., 0] = (sign * torch.arange(starts[-1]) * 0.5).to(k.dtype).cuda()[:, None]
+        _close(ops.prompt_attention(q, k, v, _cuda_starts(starts)), *scoring_ref.attend(q, k, v, starts))
+
+
+@pytest.mark.parametrize("hq,hkv,hd,lengths", LARGE)
+def test_large_items_strides(lib, hq, hkv, hd, lengths):
+    """Heads before tokens, padded rows beside NaN, an unaligned view and strided dims: one result."""
+    from minitp_b200 import ops
+
+    starts, q, k, v = _case(hq, hkv, hd, lengths, 90 + hd, True)
+    st, n = _cuda_starts(starts), starts[-1]
+    want = ops.prompt_attention(q, k, v, st)
+    _close(want, *scoring_ref.attend(q, k, v, starts))
+
+    def padded(t):
+        w = torch.full((n + 3, t.shape[1] + 2, hd + 16), math.nan, dtype=t.dtype, device="cuda")
+        w[1:n + 1, 1:-1, 16:] = t
+        return w[1:n + 1, 1:-1, 16:]
+
+    def unaligned(t):
+        w = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        w[1:] = t.reshape(-1)
+        return w[1:].view(t.shape)
+
+    for f in (lambda t: t.transpose(0, 1).contiguous().transpose(0, 1), padded, unaligned,
+              lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)):
+        assert torch.equal(ops.prompt_attention(f(q), f(k), f(v), st), want)
+
+
+@pytest.mark.parametrize("hq,hkv,hd,lengths", LARGE)
+def test_large_items_tokens_of_no_prompt_and_pieces(lib, hq, hkv, hd, lengths):
+    """NaN before, behind and (by the pieces) around what is asked for; tokens of no prompt become 0."""
+    from minitp_b200 import ops
+
+    starts, q, k, v = _case(hq, hkv, hd, lengths, 100 + hd, True, at=130, behind=77)
+    for t in (q, k, v):
+        t[:130] = math.nan
+        t[starts[-1]:] = math.nan
+    want, tol = scoring_ref.attend(q, k, v, starts)
+    got = ops.prompt_attention(q, k, v, _cuda_starts(starts))
+    assert not got[:130].any() and not got[starts[-1]:].any()
+    _close(got, want, tol)
+    total = q.shape[0]
+    a, b = 3, total - 5
+    assert (b - a) * hq > 256 * 148
+    _close(ops.prompt_attention(q[a:b], k, v, _cuda_starts(starts), first=a), want[a:b], tol[a:b])
+
+
+@pytest.mark.parametrize("hq,hkv,hd,lengths", LARGE)
+def test_large_items_starts_out_of_range(lib, hq, hkv, hd, lengths):
+    from minitp_b200 import ops
+
+    starts, q, k, v = _case(hq, hkv, hd, lengths, 110 + hd, True)
+    total = starts[-1]
+    for given, meant in [([-5, 700, total + 900], [0, 700, total]), ([500, 30, 1200, total], [500, 500, 1200, total]),
+                         ([total + 3, total + 9], [total, total])]:
+        got = ops.prompt_attention(q, k, v, _cuda_starts(given))
+        want, tol = scoring_ref.attend(q[:1500], k, v, meant)
+        _close(got[:1500], want, tol)
+        assert bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("hq,hkv,hd,lengths", LARGE)
+def test_large_items_captured_and_on_another_stream(lib, hq, hkv, hd, lengths):
+    """A captured call replays on new contents and new starts; another stream's call gives the same."""
+    from minitp_b200 import ops
+
+    starts, q, k, v = _case(hq, hkv, hd, lengths, 120 + hd, True)
+    n, st = starts[-1], _cuda_starts(starts)
+    ops.prompt_attention(q, k, v, st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.prompt_attention(q, k, v, st)
+    side = torch.cuda.Stream()
+    other_starts = [starts[0] + 1, *sorted(s // 2 for s in starts[1:-1]), n - 1]
+    for seed, new in [(121, starts), (122, sorted(other_starts))]:
+        nq, nk, nv = _parts(_gen(seed), n, hq, hkv, hd, "bf16")
+        q.copy_(nq), k.copy_(nk), v.copy_(nv), st.copy_(_cuda_starts(new))
+        g.replay()
+        _close(out, *scoring_ref.attend(nq, nk, nv, new))
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = ops.prompt_attention(q, k, v, st)
+        side.synchronize()
+        assert torch.equal(other, out)
+
 @pytest.mark.parametrize("dtype,hq,hkv,hd", [("fp32", 4, 2, 16), ("bf16", 6, 3, 32), ("fp32", 7, 1, 128), ("bf16", 14, 2, 64),
                                              ("bf16", 4, 1, 128)])
 def test_prompts_around_the_number_that_is_put_in_order(lib, dtype, hq, hkv, hd):
