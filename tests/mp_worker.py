@@ -243,6 +243,27 @@ def w_beam(rank, world):
     return res
 
 
+def score_prompts_of():
+    r = torch.Generator().manual_seed(32)
+    return [torch.randint(0, 997, (n,), generator=r) for n in (19, 1, 0, 40, 2, 130)]
+
+
+def w_score(rank, world):
+    """Scores of prompts of different lengths on the ranks of a TP group, whole and in pieces of a few tokens."""
+    from minitp_b200 import scoring
+    from minitp_b200.weight_loader import load_synthetic_tp
+
+    ctx = ctx_for(rank, world)
+    model = load_synthetic_tp(beam_cfg(), ctx, dtype=torch.float32, device=ctx.device)
+    res = {}
+    for name, logits_bytes in (("whole", 256 << 20), ("pieces", 8 * 4 * 499)):
+        scoring._LOGITS_BYTES = logits_bytes
+        got = scoring.score_prompts(model, score_prompts_of(), 5)
+        for k in ("logprobs", "entropy", "top_logprobs", "top_ids"):
+            res[f"{name}_{k}"] = torch.cat([getattr(g, k) for g in got]).cpu().numpy()
+    return res
+
+
 def w_peer_timeout(rank, world):
     """Rank 1 skips one collective: rank 0's bounded wait must expire and report it.
 

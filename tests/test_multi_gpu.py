@@ -127,6 +127,40 @@ def test_tp2_beam_search_and_shared_prefixes():
     assert np.array_equal(res[0]["shared"], oracle.generate(whole, 5)[:, 17:].numpy())
 
 
+def test_tp2_scores():
+    """Scores at TP=2 (blocks of an uneven vocabulary exchanged, pieces of a few tokens): equal on both ranks, and the
+    oracle's log-probabilities."""
+    res = mp_worker.run(2, mp_worker.w_score)
+    for k in res[0]:
+        assert np.array_equal(res[0][k], res[1][k]), k
+    check_scores(res[0])
+
+
+def check_scores(res):
+    """Against the oracle: fp32 logits right to 1e-4 of the largest, log-probabilities to twice that."""
+    from oracle.model import OracleConfig, OracleModel, checkpoint_tensors
+
+    cfg = mp_worker.beam_cfg()
+    oracle = OracleModel(OracleConfig.of(cfg), checkpoint_tensors(cfg), tp=1)
+    at = 0
+    for ids in mp_worker.score_prompts_of():
+        n = max(0, ids.numel() - 1)
+        if n:
+            oracle.reset(1, ids.numel())
+            logits = oracle.forward(ids[None], torch.arange(ids.numel()))[0].double()
+            off = 2e-4 * float(logits.abs().max())
+            lp = torch.log_softmax(logits, -1)[:-1]
+            for name in ("whole", "pieces"):
+                got = {k: torch.from_numpy(res[f"{name}_{k}"][at:at + n]) for k in ("logprobs", "entropy", "top_logprobs", "top_ids")}
+                assert float((got["logprobs"] - lp.gather(1, ids[1:, None])[:, 0]).abs().max()) <= off
+                ent = -(lp.exp() * lp).sum(-1)
+                assert float(((got["entropy"] - ent).abs() / (1 + ent)).max()) <= off
+                assert float((got["top_logprobs"] - lp.topk(5).values).abs().max()) <= off
+                assert float((lp.gather(1, got["top_ids"]) - lp.topk(5).values).abs().max()) <= 2 * off
+        at += n
+    assert at == res["whole_logprobs"].shape[0]
+
+
 def test_peer_timeout_is_reported():
     res = mp_worker.run(2, mp_worker.w_peer_timeout)
     assert bool(res[0]["ok_before"]) and bool(res[1]["ok_before"])
