@@ -326,7 +326,8 @@ int mtpb_beam_status(uint32_t* status_out /* host */);
  * 1/sqrt(hd); hd 16, 32, 64 or 128; total * hq at most 2^28, hq 2^16, S 2^20.
  * Softmax statistics and sums are fp32; bf16 probabilities are rounded to bf16
  * for their product with V. What a token does not see does not reach it, NaN
- * and infinities included. out may not overlap an input. */
+ * and infinities included; of an infinity of V that it sees under a probability
+ * of 0 its sum is NaN or that infinity. out may not overlap an input. */
 int mtpb_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                           int64_t k_head, const void* v, int64_t v_token, int64_t v_head, void* out,
                           const int* seq_starts, int S, int first, int n, int total, int hq, int hkv,

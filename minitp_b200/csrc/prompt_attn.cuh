@@ -15,7 +15,9 @@
 //
 // NaN and infinities go where the formula takes them and nowhere else: a score
 // that is NaN makes its row NaN, a NaN among V the dim of the rows that see
-// it, and what a token does not see does not reach it.
+// it, and what a token does not see does not reach it. (Of an infinity of V under
+// a probability that is 0, or that fp32 or bf16 take for 0, the sum is NaN or that
+// infinity.)
 #pragma once
 
 #include <type_traits>
@@ -51,9 +53,10 @@ __device__ __forceinline__ void pa_zero(const PaParams& p, const PaTiles& t, int
 // instruction, over even and odd dims (fp32 us without / with, 64-row tiles: 4
 // prompts of <= 2048 tokens, 7 heads of 128: 410 / 332; 5 of <= 701, 8 heads of 32:
 // 45 / 43). Two CTAs an SM up to 64 dims, at 128 registers (one / two: 8 of <= 1024,
-// 14 heads of 64: 182 / 156; one of 1000: 78 / 103). Bound by shared memory reads
-// beside the fused multiply-adds (a float4 of K serves RPT rows, one of V as well):
-// 31 to 37 TFLOP/s.
+// 14 heads of 64: 182 / 156; one of 1000: 78 / 103). What binds these thread tiles
+// is shared memory reads beside the fused multiply-adds (a float4 of K serves RPT
+// rows, one of V as well): 31 to 37 TFLOP/s of 72. Tiles of 4 rows x 8 keys a thread,
+// which would read less for a product, have not been tried.
 // ---------------------------------------------------------------------------
 constexpr int kPaKeys = 64;
 constexpr int kPaThreads = 256;
@@ -299,9 +302,10 @@ __global__ void __launch_bounds__(kPaThreads, HD <= 64 ? 2 : 1) pa_simt_kernel(c
 // Bound by the softmax: a key tile of both streams costs 3500 to 3900 cycles
 // (head dim 128), of which the products take 2048 of the tensor cores, the 7/8
 // of the exponentials that the special-function unit makes 1800 of that unit,
-// and the softmax warps alone, with no products to wait for, 2700. Measured, GPU time: one
-// prompt of 32768 tokens, 28 heads of 128: 6.25 to 6.45 ms, 1.23 PFLOP/s; 12 of <= 4096,
-// 28 heads of 128: 475 us, 1.04; of short prompts the turn from item to item (3000 to
+// and the softmax warps alone, with no products to wait for, 2700. Measured, GPU time of
+// single calls (1965 MHz) and of a second of calls (1580 to 1800 MHz, under the power
+// cap): one prompt of 32768 tokens, 28 heads of 128: 6.3 to 6.9 / 7.1 ms, 1.08 PFLOP/s of
+// the latter; 12 of <= 4096, 28 heads of 128: 480 / 564 us, 0.88; of short prompts the turn from item to item (3000 to
 // 4000 cycles: the last P V, the output) weighs as much as their one or two key
 // tiles. Four softmax warpgroups (half a row a thread), S in two halves of 64
 // keys, and rolled loops that read S twice were 10 to 40 % slower.

@@ -53,7 +53,8 @@ constexpr int kPaOrdered = 2 * 32;
 // The tiles of all prompts, by one warp, in the order of growing numbers. They
 // are numbered in descending order of their place in their prompt, which is how
 // many keys they see, over all prompts, so that the longest do not start last;
-// with more than kPaOrdered prompts prompt after prompt (the last tile first).
+// with more than kPaOrdered prompts prompt after prompt (the last tile first; a
+// long prompt that comes last then starts last).
 // The starts are made non-decreasing and cut to [0, total] first, so that no
 // values of theirs lead out of the tensors or make two tiles of a token.
 struct PaTiles {

@@ -5,6 +5,9 @@ behind the other, without padding, and run through the model in one forward
 (``TPQwen2ForCausalLM.forward_packed``, whose attention is ``ops.prompt_attention``);
 the LM head and ``VocabParallelLMHead.token_logprobs`` then take the tokens in
 pieces, so that no more than a few hundred megabytes of logits exist at once.
+(The forward itself goes in chunks of what one AllReduce message of the
+communicator holds, 8 MB of hidden states by default: 4681 tokens of the 0.5B
+shape in bf16, 1170 of the 7B one.)
 """
 
 from __future__ import annotations
@@ -46,11 +49,12 @@ def score_prompts(
     """Scores of every prompt's tokens, given the tokens before them.
 
     ``prompts``: token ids, each a sequence of ints or an integer tensor ``[n]``
-    on any device; a prompt of one token or none has empty scores. ``top``: likeliest
-    alternatives per token (0 to 64). Prompts are packed into forwards of at most
-    ``max_tokens`` tokens (a longer prompt goes alone). The results are on the
-    model's device, and complete: errors that a kernel can only report to the
-    device's status words (a wait that ran out) raise here.
+    on any device; ids outside the vocabulary are refused, and a prompt of one
+    token or none has empty scores. ``top``: likeliest alternatives per token (0 to
+    64). Prompts are packed into forwards of at most ``max_tokens`` tokens (a longer
+    prompt goes alone). The results are on the model's device, and complete: errors
+    that a kernel can only report to the device's status words (a wait that ran
+    out) raise here.
     """
     dev = model.model.embed_tokens.weight.device
     if not 0 <= top <= 64:

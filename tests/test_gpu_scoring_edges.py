@@ -402,6 +402,7 @@ def test_sizes_past_the_c_types_are_refused(lib):
         ops.logprobs_join(torch.zeros(65, 16, dtype=torch.uint8, device="cuda"), None, (1,), 0, 10, torch.float32)
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 def test_a_packed_forward_that_is_refused_launches_nothing(lib):
     """Limits of the attention are looked at before the first kernel: a capture of the refused call holds no node."""
     from cuda.bindings import runtime
