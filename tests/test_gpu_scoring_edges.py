@@ -430,3 +430,60 @@ def test_a_packed_forward_that_is_refused_launches_nothing(lib):
     assert nodes(many, True) == 0
     assert torch.equal(model.forward_packed(ids, few, ids), want)
     assert model.ctx.comm().status() == 0
+
+
+# ------------------------------------------------------------------ the largest sizes that are taken
+@pytest.mark.parametrize("dtype,hd", [("fp32", 16), ("bf16", 64)])
+def test_as_many_prompts_as_are_taken(lib, dtype, hd):
+    """2^20 prompts of up to three tokens: first tokens return their V, last ones the sums over their prompt."""
+    from minitp_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    lengths = torch.randint(0, 4, (1 << 20,), generator=g, device="cuda")
+    starts = torch.cat([lengths.new_zeros(1), lengths.cumsum(0)]).int()
+    q, k, v = (torch.randn(int(starts[-1]), h, hd, generator=g, device="cuda").to(DT[dtype]) for h in (4, 2, 2))
+    got = ops.prompt_attention(q, k, v, starts)
+    first = starts[:-1][lengths > 0].long()
+    assert torch.equal(got[first], v[first].repeat_interleave(2, 1))
+    pick = first[lengths[lengths > 0] == 3][::97]
+    rows = torch.stack([pick, pick + 1, pick + 2], 1).reshape(-1)
+    small = list(range(0, rows.numel() + 1, 3))
+    _close(got[rows], *scoring_ref.attend(q[rows], k[rows], v[rows], small))
+    _status_is_clean(lib)
+
+
+def test_as_many_rows_as_are_taken(lib):
+    from minitp_b200 import ops
+
+    rows, v = 1 << 24, 17
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, v, generator=g, device="cuda").bfloat16()
+    t = torch.randint(0, v, (rows,), generator=g, device="cuda")
+    got = ops.token_logprobs(x, t, 2)
+    _check_some(got, x, t, 2, 9973)
+    # all rows in fp32: off by a few of its half steps of values below 16, on either side
+    assert float((got[0] - torch.log_softmax(x.float(), -1).gather(1, t[:, None])[:, 0]).abs().max()) <= 40 * 2.0 ** -24 * 16
+
+
+def test_a_vocabulary_as_large_as_is_taken(lib):
+    from minitp_b200 import ops
+
+    v = (1 << 30) - 1
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.empty(1, v, dtype=torch.bfloat16, device="cuda").normal_(0.0, 2.0, generator=g)
+    x[0, v - 2:] = 30.0
+    x[0, 0] = 29.0
+    lp, entropy, best, ids = ops.token_logprobs(x, torch.tensor([v - 1], device="cuda"), 3)
+    total = mean = 0.0
+    for i in range(0, v, 1 << 26):
+        d = x[0, i:i + (1 << 26)].double() - 30.0
+        e = d.exp()
+        total += float(e.sum())
+        mean += float((e * d).sum())
+    logs = math.log(total)
+    # a lane adds 2^30 / (444 x 256) values: scoring_ref.check_logprobs' tolerance at that depth
+    off = (v / (444 * 256) + 40) * 2.0 ** -24
+    assert ids.tolist() == [[v - 2, v - 1, 0]]
+    assert abs(float(lp) + logs) <= off * (1 + logs) and abs(float(best[0, 2]) + 1 + logs) <= off * (2 + logs)
+    assert abs(float(entropy) - (logs - mean / total)) <= off * (2 + logs)
+    _status_is_clean(lib)
